@@ -9,7 +9,8 @@ The same Python surface as the reference package (delta_matching/__init__.py:44-
 Constraints: self-attention; head_dim 128 (seqlen % 256 == 0) or 256 (seqlen % 128 == 0); bf16; softmax_scale =
 head_dim ** -0.5; mode "matched" needs causal=True.  Violations raise ValueError / TypeError / NotImplementedError.
 `dm_attn_func_bhnd` takes (B, H, N, D) and returns (B, N, H, D).  `flash_attn_func` has flash-attention 2's signature
-and refuses the arguments the kernels do not implement.  All work runs in hand-written CUDA for sm_100a behind the C
+and refuses the arguments the kernels do not implement.  For answering with what was trained there is an 8-bit key/value cache:
+`KVCache8`, `dm_cache_append`, `dm_cache_attn`, `dm_cache_evict` (cache.py).  All work runs in hand-written CUDA for sm_100a behind the C
 ABI of include/dm_b200.h; there is no fallback path.
 """
 from __future__ import annotations
@@ -20,6 +21,7 @@ import torch
 
 from . import _lib
 from .attn import blocks, dm_attn_func_bhnd, dm_attn_debug
+from .cache import KVCache8, dm_cache_append, dm_cache_attn, dm_cache_evict
 
 __version__ = "0.1.0"
 # the quantisation contract the kernels implement, by head dim: the reference's Blackwell presets
@@ -30,7 +32,7 @@ NUMERICS_ARMS = ("sm100-mx", "sm100-mx-d256", "sm100-mx-ds32", "sm100-mx-d256-ds
 FA_SRC_COMMIT = "none (from-scratch sm_100a build)"
 CUTLASS_COMMIT = "none (from-scratch sm_100a build)"
 __all__ = ["dm_attn_func", "dm_attn_func_bhnd", "dm_attn_func_plain", "flash_attn_func", "blocks", "kernel_version",
-           "__version__", "KERNEL_NUMERICS", "NUMERICS_ARMS"]
+           "__version__", "KERNEL_NUMERICS", "NUMERICS_ARMS", "KVCache8", "dm_cache_append", "dm_cache_attn", "dm_cache_evict"]
 
 # The reference keeps a second "plain" route as a cross-check of its Triton producers (delta_matching/core.py:178-271);
 # there is one producer implementation here, so the name is an alias.

@@ -10,6 +10,7 @@
 #include <initializer_list>
 
 #include "../../include/dm_b200.h"
+#include "dm_abi_util.h"
 #include "dm_kernels.h"
 #include "dm_probe.h"
 
@@ -27,9 +28,10 @@ int sm_count() {
 long long launch_count() { return g_launches.load(std::memory_order_relaxed); }
 }  // namespace dm
 
-namespace {
+namespace dm {
+namespace abi {
 
-thread_local char g_err[512] = "";
+static thread_local char g_err[512] = "";
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -43,11 +45,7 @@ int cuda_fail(cudaError_t e, const char* what) {
   return fail(DM_ERR_CUDA, "delta_matching: %s failed: %s", what, cudaGetErrorString(e));
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
+static EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
   if (fn == nullptr) {
     void* p = nullptr;
@@ -60,16 +58,12 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// 2-D map over dense e4m3 codes viewed as [rows][D]: boxes of 128 rows x 128 bytes, 128-byte swizzle.
-int make_code_map(CUtensorMap* m, const void* base, uint64_t rows, int D) {
+int encode_byte_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(DM_ERR_CUDA, "delta_matching: cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), rows};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(D)};
-  const cuuint32_t box[2] = {128, 128};
-  const cuuint32_t estr[2] = {1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
   auto encode = [&]() {
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = encode();
@@ -80,7 +74,15 @@ int make_code_map(CUtensorMap* m, const void* base, uint64_t rows, int D) {
   return 0;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// 2-D map over dense e4m3 codes viewed as [rows][D]: boxes of 128 rows x 128 bytes, 128-byte swizzle.
+static int make_code_map(CUtensorMap* m, const void* base, uint64_t rows, int D) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), rows};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(D)};
+  const cuuint32_t box[2] = {128, 128};
+  return encode_byte_map(m, base, 2, dims, strides, box);
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int check_address(const void* p, const char* name) {
   if (p == nullptr) return fail(DM_ERR_ARG, "delta_matching: %s is NULL (every tensor must be a CUDA buffer)", name);
@@ -88,17 +90,13 @@ int check_address(const void* p, const char* name) {
   return 0;
 }
 
-struct NamedPtr {
-  const void* p;
-  const char* name;
-};
 int check_addresses(std::initializer_list<NamedPtr> ptrs) {
   for (const NamedPtr& x : ptrs)
     if (int r = check_address(x.p, x.name)) return r;
   return 0;
 }
 
-int check_device_ptr(const void* p, const char* name) {
+static int check_device_ptr(const void* p, const char* name) {
   if (p == nullptr) return check_address(p, name);
   cudaPointerAttributes a;
   cudaError_t e = cudaPointerGetAttributes(&a, p);
@@ -116,7 +114,7 @@ int check_device_ptr(const void* p, const char* name) {
   return check_address(p, name);
 }
 
-int check_shape(int B, int N, int H, int Hk, int D) {
+static int check_shape(int B, int N, int H, int Hk, int D) {
   if (D != 128 && D != 256) return fail(DM_ERR_ARG, "delta_matching: head_dim must be 128 or 256 (got %d)", D);
   if (B <= 0 || N <= 0 || H <= 0 || Hk <= 0) return fail(DM_ERR_ARG, "delta_matching: empty tensor (B=%d N=%d H=%d Hk=%d)", B, N, H, Hk);
   if (N % 128) return fail(DM_ERR_ARG, "delta_matching: seqlen must be a multiple of 128 (got %d)", N);
@@ -125,7 +123,7 @@ int check_shape(int B, int N, int H, int Hk, int D) {
   return 0;
 }
 
-int check_strides(const char* name, int64_t a, int64_t b, int64_t c) {
+static int check_strides(const char* name, int64_t a, int64_t b, int64_t c) {
   if ((a % 8) || (b % 8) || (c % 8))
     return fail(DM_ERR_ARG, "delta_matching: %s strides must be multiples of 8 elements (16-byte aligned rows)", name);
   return 0;
@@ -145,13 +143,10 @@ int check_sm100() {
   return 0;
 }
 
-#define DM_TRY(expr)            \
-  do {                          \
-    int _r = (expr);            \
-    if (_r != 0) return _r;     \
-  } while (0)
+}  // namespace abi
+}  // namespace dm
 
-}  // namespace
+using namespace dm::abi;
 
 extern "C" {
 

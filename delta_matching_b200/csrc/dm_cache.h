@@ -1,0 +1,85 @@
+// Internal launch interface of the 8-bit key / value cache (append, attention, eviction) between its C-ABI layer (dm_cache_abi.cu) and the
+// kernel translation units.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace dm {
+
+// Pools of pages and one block table over them.  Token j of sequence b is slot j % page of page table[b, j / page]; a slot's row of D codes
+// is contiguous; 32 slots of a page and head share a scale.
+struct CacheView {
+  uint8_t* k8;
+  uint8_t* v8;
+  float* ks;
+  float* vs;
+  int64_t c_page, c_head, c_slot;   // byte strides of k8 and v8
+  int64_t s_page, s_head;           // element strides of ks and vs (the page / 32 scales of a head are adjacent)
+  int pages, Hk, page;
+  const int* table;                 // (B, T), rows t_row entries apart
+  int64_t t_row;
+  int T;
+  const int* lengths;               // (B)
+  int B;
+  int* status;
+};
+
+struct CacheAppendParams {
+  CacheView c;
+  const __nv_bfloat16* k;           // (B, N, Hk, D) by element strides, rows 16-byte aligned
+  const __nv_bfloat16* v;
+  int64_t k_sb, k_sn, k_sh, v_sb, v_sn, v_sh;
+  const int* counts;                // (B) or null: N each
+  int* new_lengths;                 // (B)
+  int N;
+};
+
+struct CacheAttnParams {
+  CacheView c;
+  const __nv_bfloat16* q;           // (B, Nq, H, D) by element strides, rows 16-byte aligned
+  int64_t q_sb, q_sn, q_sh;
+  const int* counts;                // (B) or null: Nq each
+  int Nq, H, rep;
+  int causal;
+  float scale;                      // softmax scale
+  __nv_bfloat16* o;                 // (B, Nq, H, D) contiguous
+  float* lse;                       // (B, H, Nq)
+  float* part_o;                    // partial results: 2 x grid slots of (row tile, D) fp32, and their (maximum, sum) pairs
+  float2* part_ml;
+  float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null
+  float* weights;                   // (B, Hk, W) or null
+  int64_t w_sb, w_sh;
+  int W;
+  int accumulate;
+  int grid;                         // CTAs of the main kernel
+};
+
+struct CacheEvictParams {
+  CacheView c;                      // the pages read
+  const int* new_table;             // (B, T2): the pages written
+  int64_t nt_row;
+  int T2;
+  const float* weights;             // (B, Hk, >= T * page)
+  int64_t w_sb, w_sh;
+  int budget, recent;
+  int* new_lengths;                 // (B)
+  int* kept;                        // (B, Hk, budget), -1 beyond what is kept
+  float* new_weights;               // (B, Hk, T2 * page), 0 beyond
+};
+
+// Slots of partial results and their sizes for a call of dm_cache_attn.
+struct CacheAttnPlan {
+  int row_tile;                     // query rows (new tokens x heads of a group) a CTA keeps
+  int row_tiles;
+  int grid;
+  int64_t part_o_bytes, part_ml_bytes, row_ml_bytes;
+};
+CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights);
+
+cudaError_t launch_cache_append(int D, const CacheAppendParams& p, cudaStream_t stream);
+cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, cudaStream_t stream);
+cudaError_t launch_cache_evict(int D, const CacheEvictParams& p, cudaStream_t stream);
+
+}  // namespace dm

@@ -6,13 +6,15 @@
 namespace dm {
 
 // Status word values a kernel may leave in its int* status argument (0 = no problem seen).  A non-zero value means a
-// bounded wait ran out; the output of that launch is not valid.
+// bounded wait ran out, or that the cache kernels met a page or length that cannot be; the output of that launch is not valid.
 enum : int {
   kStatusOk = 0,
   kStatusTimeoutProducer = 1,   // TMA producer gave up waiting for a free stage
   kStatusTimeoutMma = 2,        // MMA issuer gave up waiting for operands or for the compute warps
   kStatusTimeoutCompute = 3,    // compute warps gave up waiting for an accumulator
   kStatusTimeoutProbe = 4,
+  kStatusBadPage = 5,           // a block table entry that names no page
+  kStatusBadLength = 6,         // a length or count outside what the block table has room for
   // which kernel it was, added to the code
   kInForward = 1 << 4,
   kInDelta = 2 << 4,
@@ -20,6 +22,7 @@ enum : int {
   kInDq = 4 << 4,
   kInDqPass2 = 5 << 4,
   kInTiles = 6 << 4,
+  kInCache = 7 << 4,
 };
 
 constexpr float kLog2e = 1.4426950408889634f;

@@ -35,6 +35,8 @@ extern "C" {
 #define DM_STATUS_TIMEOUT_MMA 2
 #define DM_STATUS_TIMEOUT_COMPUTE 3
 #define DM_STATUS_TIMEOUT_PROBE 4
+#define DM_STATUS_BAD_PAGE 5      /* cache: an entry of the block table that names no page (no access was made) */
+#define DM_STATUS_BAD_LENGTH 6    /* cache: a length or count beyond what the block table has room for (it was cut) */
 /* the low four bits; the bits above name the kernel: 1 forward, 2 matched delta, 3 dK/dV, 4 dQ, 5 streaming pass, 6 tile pass */
 
 /* Library identity.  Replaces the build-sanity ops build_gt() / build_hd128() / build_bf16dp() of
@@ -230,6 +232,56 @@ int dm_kmean_static(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, int
  * the reference has no host-memory path).  Returns 0 or a negative code. */
 int dm_copy_2d_async(void* dst, int64_t dpitch, const void* src, int64_t spitch, int64_t width, int64_t height,
                      int to_device, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ 8-bit key / value cache
+ * Serving beside the training attention above; the reference has no counterpart.
+ *
+ * Pools of pages in device memory: k8 / v8 (pages, heads, page_size, head_dim) e4m3 codes, ks / vs (pages, heads, page_size / 32) fp32 powers
+ * of two, one for each block of 32 slots and head (value = code * scale).  Pages, heads and slots lie the given strides apart (codes: bytes,
+ * multiples of 16; scales: elements, the blocks of a head adjacent); a slot's head_dim codes are contiguous.  K and V have equal strides.
+ * A block table (B, T) int32, rows table_row entries apart, names each sequence's pages: token j is slot j % page_size of page
+ * table[b, j / page_size].  lengths (B) int32 = tokens held; entries of the table beyond them are not read.
+ * Table entries, lengths and counts are device data that the host does not see: a kernel that meets one out of range reports it through
+ * `status` (DM_STATUS_BAD_PAGE, DM_STATUS_BAD_LENGTH), stays inside the buffers, and its outputs are invalid.
+ * All pointers are the caller's word to be memory of the current device, as in dm_attn_fwd. */
+typedef struct dm_kv_cache {
+  void* k8;
+  void* v8;
+  float* ks;
+  float* vs;
+  int64_t code_page, code_head, code_slot;    /* byte strides of k8 and v8 */
+  int64_t scale_page, scale_head;             /* element strides of ks and vs */
+  int pages, heads, page_size, head_dim;
+} dm_kv_cache;
+
+/* N new tokens a sequence (k, v: bf16 by element strides for (batch, token, head); of sequence b the first counts[b], all when counts is
+ * NULL) to positions lengths[b], lengths[b] + 1, ...  new_lengths (B) = lengths + counts; lengths itself is not changed.  The scale of a
+ * block that already holds tokens only grows, and its codes are rounded anew when it does.  The same call again leaves the same cache. */
+int dm_cache_append(const dm_kv_cache* cache, const void* k, int64_t k_sb, int64_t k_sn, int64_t k_sh,
+                    const void* v, int64_t v_sb, int64_t v_sn, int64_t v_sh, int B, int N,
+                    const int* table, int64_t table_row, int T, const int* lengths, const int* counts, int* new_lengths,
+                    int* status, void* stream);
+
+/* Attention of Nq new tokens a sequence (q: bf16 by element strides for (batch, token, head); of sequence b the first q_counts[b], all when
+ * NULL) over the lengths[b] tokens that the cache holds, the new ones among them: causal, token i sees the first lengths[b] - q_counts[b] + i
+ * + 1, else all.  o (B, Nq, H, head_dim) bf16 contiguous, lse (B, H, Nq) fp32 natural log; rows that see nothing, and those beyond q_counts: 0 and
+ * -inf.  weights (may be NULL; strides w_sb, w_sh, W >= T * page_size): weights[b, hk, j] = sum over the new tokens and the heads of the
+ * group of their softmax weight on token j, added to what is there when accumulate is set, otherwise 0 beyond the length.
+ * workspace: dm_cache_attn_workspace_bytes, 16-byte aligned, contents ignored (0: a shape that is refused). */
+int64_t dm_cache_attn_workspace_bytes(int B, int Nq, int H, int Hk, int D, int T, int page_size, int with_weights);
+int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, int B, int Nq, int H,
+                  const int* table, int64_t table_row, int T, const int* lengths, const int* q_counts, int causal, float softmax_scale,
+                  void* o, float* lse, float* weights, int64_t w_sb, int64_t w_sh, int W, int accumulate,
+                  void* workspace, int64_t workspace_bytes, int* status, void* stream);
+
+/* At most `budget` tokens a (sequence, head) into the pages of new_table, which must not be pages that hold the tokens: all where lengths[b]
+ * <= budget, else the last `recent` and the budget - recent others of greatest weight (weights (B, heads, >= T * page_size) by strides; equal ones:
+ * the lowest positions; NaN is least), in their order, requantised to the scales of their new blocks (slots of the last block beyond the kept
+ * tokens: zeros).  new_lengths (B); kept (B, heads, budget) int32: old positions, -1 beyond; new_weights (B, heads, new_T * page_size): the
+ * kept tokens' weights, 0 beyond. */
+int dm_cache_evict(const dm_kv_cache* cache, int B, const int* table, int64_t table_row, int T, const int* lengths,
+                   const float* weights, int64_t w_sb, int64_t w_sh, const int* new_table, int64_t new_table_row, int new_T,
+                   int budget, int recent, int* new_lengths, int* kept, float* new_weights, int* status, void* stream);
 
 #ifdef __cplusplus
 }
