@@ -139,8 +139,29 @@ def native_attn():
                                 addr("dm_quant_qkv_workspace_bytes"),
                                 lambda idx: ops.status_word(torch.device("cuda", idx)).data_ptr(), ops._raise_if_set,
                                 lambda *a: ops.bwd_fp8(*a[:11], ds32=a[11]), ops._SMALL_WS, ops._MAX_WS_TILES)
+                _dm_native.bind_cache(*(addr("dm_cache_" + n) for n in ("append", "attn", "attn_workspace_bytes", "evict")))
                 _NATIVE = _dm_native.attn
     return _NATIVE
+
+
+class _NoCacheRoute:
+    """In the place of the native module where the Python route has to take every call."""
+    cache_append = cache_attn = cache_evict = staticmethod(lambda *_: None)
+
+
+_CACHE_ROUTE = None
+
+
+def native_cache():
+    """The native eager route of the cache functions (csrc/dm_torch_cache.cpp): cache_append, cache_attn and cache_evict of the bound
+    module, each of which returns None when the Python route has to take the call."""
+    global _CACHE_ROUTE
+    if _CACHE_ROUTE is None:
+        if native_attn() is _decline:
+            return _NoCacheRoute
+        from . import _dm_native
+        _CACHE_ROUTE = _dm_native
+    return _CACHE_ROUTE
 
 
 def _decline(*_):

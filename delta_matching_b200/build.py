@@ -1,5 +1,6 @@
 """Build the CUDA library in-tree: nvcc for sm_100a only, one shared object `libdm_b200.so` next to this file, and the
-Python extension `_dm_native.so` (csrc/dm_torch.cpp: the eager route of the attention functions against torch's C++ API).
+Python extension `_dm_native.so` (csrc/dm_torch.cpp, dm_torch_cache.cpp: the eager route of the attention and cache functions against torch's
+C++ API).
 
     python -m delta_matching_b200.build [--force] [--verbose]
 
@@ -21,7 +22,7 @@ LIB = os.path.join(HERE, "libdm_b200.so")
 SOURCES = ("dm_abi.cu", "dm_quant.cu", "dm_fwd.cu", "dm_fwd_teams.cu", "dm_delta.cu", "dm_bwd_kv.cu", "dm_bwd_pipe.cu", "dm_bwd_tiles.cu", "dm_bwd.cu", "dm_bwd_p2.cu", "dm_probe.cu", "dm_static_scratch.cu",
            "dm_cache_abi.cu", "dm_cache_append.cu", "dm_cache_attn.cu", "dm_cache_evict.cu")
 NATIVE = os.path.join(HERE, "_dm_native.so")
-NATIVE_SOURCE = "dm_torch.cpp"
+NATIVE_SOURCES = ("dm_torch.cpp", "dm_torch_cache.cpp")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 
@@ -62,13 +63,20 @@ def _build_native(verbose: bool) -> None:
     from torch.utils import cpp_extension
     inc = [f for d in (*cpp_extension.include_paths(), sysconfig.get_path("include"), "/usr/local/cuda/include") for f in ("-isystem", d)]
     lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, os.path.join(CSRC, NATIVE_SOURCE), "-o", NATIVE,
-           f"-L{lib_dir}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
-           "-nostdlib++", "-l:libstdc++.so.6", "-lm"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {NATIVE_SOURCE}:\n{r.stdout}\n{r.stderr[-6000:]}")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc]
+    gxx = os.environ.get("CXX", "g++")
+    objs = [os.path.join(OBJ, src[:-4] + ".native.o") for src in NATIVE_SOURCES]
+
+    def run(what, cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed for {what}:\n{r.stdout}\n{r.stderr[-6000:]}")
+        return r
+
+    with ThreadPoolExecutor(max_workers=len(objs)) as ex:
+        list(ex.map(lambda x: run(x[0], [gxx, *flags, "-c", os.path.join(CSRC, x[0]), "-o", x[1]]), zip(NATIVE_SOURCES, objs)))
+    r = run(os.path.basename(NATIVE), [gxx, "-shared", *objs, "-o", NATIVE, f"-L{lib_dir}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+                                       "-ltorch_cuda", "-lc10", "-lc10_cuda", "-nostdlib++", "-l:libstdc++.so.6", "-lm"])
     if verbose:
         sys.stderr.write(r.stderr)
 

@@ -149,6 +149,9 @@ def dm_cache_append(cache, k, v, block_table, lengths, counts=None):
 
     Each block of 32 slots and head gets the smallest power-of-two scale that holds its new values; a block that already holds tokens keeps
     the larger of the two scales, and its codes are rounded anew when that grows."""
+    new = _lib.native_cache().cache_append(cache, k, v, block_table, lengths, counts)
+    if new is not None:
+        return new
     pages, Hk, P, D = _check_cache(cache)
     dev = cache.k8.device
     k, v = _check_rows("k", k, Hk, D, dev), _check_rows("v", v, Hk, D, dev)
@@ -180,6 +183,9 @@ def dm_cache_attn(q, cache, block_table, lengths, q_counts=None, causal=True, so
     tokens and over the query heads of its kv head; accumulate=True adds it to what is there.  return_lse=True also returns the LSE (B, H, N)
     fp32, natural log.  The logits and the softmax are those of the codes' exact values: q and the probabilities keep 8 and 11 bits or
     more, sums and statistics are fp32."""
+    out = _lib.native_cache().cache_attn(q, cache, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, return_lse)
+    if out is not None:
+        return out
     pages, Hk, P, D = _check_cache(cache)
     dev = cache.k8.device
     q = _check_rows("q", q, None, D, dev)
@@ -223,6 +229,9 @@ def dm_cache_evict(cache, block_table, lengths, weights, new_block_table, budget
 
     Returns (new lengths (B) int32, kept (B, Hk, budget) int32: the old positions in order, -1 beyond, new weights (B, Hk, T2 * page_size) fp32: those of the
     kept tokens, 0 beyond).  The heads of a sequence keep different tokens but equally many."""
+    out = _lib.native_cache().cache_evict(cache, block_table, lengths, weights, new_block_table, budget, recent)
+    if out is not None:
+        return out
     pages, Hk, P, D = _check_cache(cache)
     dev = cache.k8.device
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1 or lengths.numel() == 0:

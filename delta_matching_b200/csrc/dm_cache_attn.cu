@@ -585,15 +585,22 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
   }
 }
 
-template <typename K>
-cudaError_t allow_smem(K kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// Once per kernel and device: the driver call takes longer than a launch.
+template <auto kKernel>
+cudaError_t allow_smem(int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
 }
 
 template <int D, int NT>
 cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, int row_tiles, cudaStream_t stream) {
   using C = AttnCfg<D, NT>;
-  cudaError_t e = allow_smem(cache_attn_kernel<D, NT>, C::kSmem);
+  cudaError_t e = allow_smem<cache_attn_kernel<D, NT>>(C::kSmem);
   if (e != cudaSuccess) return e;
   count_launch();
   e = launch_chained(cache_attn_kernel<D, NT>, dim3(p.grid), 128, C::kSmem, stream, tk, tv, p, row_tiles);
@@ -602,7 +609,7 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttn
   e = launch_chained(cache_join_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(p.c.B) * p.H * p.Nq)), 128, 0, stream, p, row_tiles, C::kRows);
   if (e != cudaSuccess || p.weights == nullptr) return e;
   constexpr int smem = 1024 + 4 * 4 * 32 * D + 4 * 4 * 8 + 136 * 4 + 64;
-  e = allow_smem(cache_weights_kernel<D, NT>, smem);
+  e = allow_smem<cache_weights_kernel<D, NT>>(smem);
   if (e != cudaSuccess) return e;
   count_launch();
   return launch_chained(cache_weights_kernel<D, NT>, dim3(p.grid), 128, smem, stream, tk, p, row_tiles);

@@ -32,6 +32,7 @@
 #include <mutex>
 
 #include "../../include/dm_b200.h"
+#include "dm_torch.h"
 
 namespace {
 
@@ -47,7 +48,7 @@ struct Lib {
   decltype(&dm_quant_qkv_workspace_bytes) quant_workspace_bytes = nullptr;
 } g_lib;
 
-constexpr int kMaxDevices = 64;
+using dm_native::kMaxDevices;
 std::atomic<int*> g_status[kMaxDevices] = {};  // pinned status words (ops.status_word), one per device that has been used
 PyObject* g_status_word = nullptr;        // ops: device index -> address of its status word
 PyObject* g_raise_if_set = nullptr;       // ops._raise_if_set
@@ -344,12 +345,7 @@ int64_t numerics_flags(PyObject* name, int64_t D) {
 }
 
 bool plain_cuda_bf16(PyObject* o, const Tensor*& t) {
-  if (!THPVariable_CheckExact(o)) return false;
-  t = &THPVariable_Unpack(o);
-  constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Functionalize,
-                                          c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative});
-  return t->dim() == 4 && t->is_cuda() && t->scalar_type() == at::kBFloat16 && t->layout() == at::kStrided &&
-         !t->unsafeGetTensorImpl()->key_set().has_any(kWrapped) && !t->_fw_grad(0).defined();
+  return dm_native::plain_cuda(o, t) && t->dim() == 4 && t->scalar_type() == at::kBFloat16;
 }
 
 // attn(q, k, v, softmax_scale, causal, mode, numerics, head_major) -> o, or None for the Python route
@@ -421,10 +417,20 @@ PyObject* bind(PyObject*, PyObject* args) {
 
 PyMethodDef kMethods[] = {
     {"attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&attn)), METH_FASTCALL, "attention on CUDA tensors, or None"},
+    {"cache_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::cache_append)), METH_FASTCALL, "cache append on CUDA tensors, or None"},
+    {"cache_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::cache_attn)), METH_FASTCALL, "cache attention on CUDA tensors, or None"},
+    {"cache_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::cache_evict)), METH_FASTCALL, "cache eviction on CUDA tensors, or None"},
+    {"bind_cache", dm_native::bind_cache, METH_VARARGS, "addresses of the kernel library's cache entry points"},
     {"bind", bind, METH_VARARGS, "addresses of the kernel library's entry points and the op layer's callbacks"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_dm_native", "native eager route", -1, kMethods};
 
 }  // namespace
+
+namespace dm_native {
+void check(int rc) { ::check(rc); }
+int* status_of(int dev) { return ::status_of(dev); }
+Tensor rows(const Tensor& t) { return ::rows(t); }
+}  // namespace dm_native
 
 PyMODINIT_FUNC PyInit__dm_native(void) { return PyModule_Create(&kModule); }
