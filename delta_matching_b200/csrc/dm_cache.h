@@ -46,7 +46,7 @@ struct CacheAttnParams {
   float scale;                      // softmax scale
   __nv_bfloat16* o;                 // (B, Nq, H, D) contiguous
   float* lse;                       // (B, H, Nq)
-  float* part_o;                    // partial results: 2 x grid slots of (row tile, D) fp32, and their (maximum, sum) pairs
+  float* part_o;                    // partial results: 2 slots a warp of (row tile, D) fp32, and their (maximum, sum) pairs
   float2* part_ml;
   float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null
   float* weights;                   // (B, Hk, W) or null

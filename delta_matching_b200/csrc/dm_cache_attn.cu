@@ -9,9 +9,10 @@
 // power-of-two scale of V's block goes into the exponent of p, relative to the largest the warp has met, and the scale of K's block into
 // the factor of the logits, so no code is ever multiplied by a scale.
 //
-// A CTA is four warps without a common loop: each takes every fourth block of 32 tokens of its CTA's range (dm_cache_sched.cuh), keeps its own
-// maximum, sum and accumulator, and fills its own ring of TMA boxes (32 rows x 128 bytes, 128-byte swizzle, straight from the pages).
-// Warps meet at the end of a segment only.
+// Every warp works for itself: it takes an even share of the blocks of 32 tokens of the whole call (dm_cache_sched.cuh), one after the other, with
+// its own maximum, sum and accumulator, and fills its own ring of TMA boxes (32 rows x 128 bytes, 128-byte swizzle, straight from the pages),
+// K and V of a block in turn, each refilled as soon as it has been read.  Units that one warp holds whole are written at once; the pieces
+// of the others are joined by a second kernel.
 #include "dm_cache_sched.cuh"
 #include "dm_kernels.h"
 
@@ -23,16 +24,11 @@ template <int D, int NT>
 struct AttnCfg {
   static constexpr int kWarps = 4;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kStageBytes = 64 * D;                  // K box(es), V box(es)
-  static constexpr int kStages = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 3 : 3);
-  static constexpr int kLd = D + 4;                           // row pitch of the slabs: float2 stores without bank conflicts
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kSlab = 2 * kRows * kLd * 4;
-  static constexpr int kStats = kWarps * kRows * 8;           // (maximum, sum) per warp and row
-  static constexpr int kBars = kWarps * kStages * 8;
-  static constexpr int kInts = 16 + 136 * 4;                  // exponents, abort flag; flat range
-  static constexpr int kSmem = 1024 + kRing + kSlab + kStats + kBars + kInts + 64;
-  static constexpr int kCtasPerSm = D == 128 ? 2 : 1;
+  static constexpr int kSlotBytes = 32 * D;                   // K or V of a block
+  static constexpr int kCtasPerSm = D == 128 && NT == 1 ? 3 : NT == 4 ? 2 : 2;
+  static constexpr int kSlots = D == 128 ? (NT == 1 ? 4 : 6) : 3;
+  static constexpr int kRing = kWarps * kSlots * kSlotBytes;
+  static constexpr int kSmem = 1024 + kRing + kWarps * kSlots * 8 + 136 * 4 + 64;
 };
 
 // Row r of a unit's tile rt: new token i, head, and how many keys it sees.
@@ -117,17 +113,14 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
-  float* slab = reinterpret_cast<float*>(smem + C::kRing);
-  float2* stats = reinterpret_cast<float2*>(smem + C::kRing + C::kSlab);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kSlab + C::kStats);
-  int* exps = reinterpret_cast<int*>(bars + C::kWarps * C::kStages);
-  int* cum = exps + 4;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing);
+  int* cum = reinterpret_cast<int*>(bars + C::kWarps * C::kSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(cum + 134);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   if (tid == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < C::kWarps * C::kStages; ++i) mbar_init(bars + i, 1);
+    for (int i = 0; i < C::kWarps * C::kSlots; ++i) mbar_init(bars + i, 1);
     mbar_fence_init();
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
@@ -135,44 +128,62 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   grid_dep_wait();
   const int units = p.c.Hk * row_tiles;
   const FlatRange range = flat_range(p.c, units, cum);        // its barriers publish the mbarriers too
-  const int f0 = range_start(blockIdx.x, p.grid, range.total), f_end = range_start(blockIdx.x + 1, p.grid, range.total);
+  const int worker = blockIdx.x * C::kWarps + warp, workers = p.grid * C::kWarps;
+  const int f0 = range_start(worker, workers, range.total), f_end = range_start(worker + 1, workers, range.total);
   if (f0 >= f_end) return;
-  Segment seg = first_segment(p.c, units, range, f0, f_end);
-  Cursor ahead = cursor_start(p.c, units, seg, warp, f_end);
+  Piece seg = first_piece(p.c, units, range, f0, f_end);
+  Cursor ahead = cursor_start(p.c, units, seg, f_end);
 
-  const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStageBytes;
-  const uint32_t my_bars = smem_u32(bars + warp * C::kStages);
-  const int bpp = p.c.page / 32;
-  float ks_reg = 0.f, vs_reg = 0.f;                           // lane s: the scales of the block in stage s
-  // The cursor's block into a stage of this warp's ring.
-  auto issue = [&](int st) {
-    const int page = max(0, checked_page(p.c, ahead.page)), sub = ahead.kb % bpp, hk = ahead.s.unit / row_tiles;
+  const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
+  const uint32_t my_bars = smem_u32(bars + warp * C::kSlots);
+  float ks_reg = 0.f, vs_reg = 0.f;                           // lane i % 8: the scales of the i-th block of this warp
+  int issued = 0, used = 0;                                   // boxes: K and V of a block in turn
+  int put = 0, get = 0;                                       // their places in the ring
+  uint32_t parity = 0;
+  // The next box of this warp into its ring, if there is one.
+  auto issue = [&]() {
+    if (!ahead.live) return;
+    const int page = max(0, checked_page(p.c, ahead.page)), hk = row_tiles == 1 ? ahead.s.unit : ahead.s.unit / row_tiles;
+    const bool is_v = issued & 1;
     if (lane == 0) {
-      const uint32_t bar = my_bars + 8 * st, dst = ring + st * C::kStageBytes;
-      asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(C::kStageBytes) : "memory");
+      const uint32_t bar = my_bars + 8 * put, dst = ring + put * C::kSlotBytes;
+      asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(C::kSlotBytes) : "memory");
 #pragma unroll
-      for (int x = 0; x < D; x += 128) {
-        tma_load_4d(dst + x * 32, &tk, bar, x, sub * 32, hk, page);
-        tma_load_4d(dst + 32 * D + x * 32, &tv, bar, x, sub * 32, hk, page);
-      }
+      for (int x = 0; x < D; x += 128) tma_load_4d(dst + x * 32, is_v ? &tv : &tk, bar, x, ahead.sub * 32, hk, page);
     }
-    if (lane == st) {
-      const int64_t at = page * p.c.s_page + hk * p.c.s_head + sub;
+    if (is_v) {
+      cursor_next(p.c, units, ahead, f_end);
+    } else if (lane == ((issued >> 1) & 7)) {
+      const int64_t at = page * p.c.s_page + hk * p.c.s_head + ahead.sub;
       ks_reg = __ldg(p.c.ks + at);
       vs_reg = __ldg(p.c.vs + at);
     }
-  };
-  int issued = 0, used = 0;
-  for (int st = 0; st < C::kStages && ahead.live; ++st) {
-    issue(st);
     ++issued;
-    cursor_next(p.c, units, ahead, warp, f_end);
-  }
+    if (++put == C::kSlots) put = 0;
+  };
+  for (int i = 0; i < C::kSlots; ++i) issue();
 
-  bool ok = true, first = true;
-  int st = 0;
-  uint32_t parity = 0;
-  for (;;) {
+  bool ok = true;
+  auto arrived = [&]() {
+    if (ok && !wait_warp(my_bars + 8 * get, parity, abort_flag)) {
+      ok = false;
+      raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
+    }
+  };
+  auto release = [&]() {
+    __syncwarp();
+    ++used;
+    if (++get == C::kSlots) {
+      get = 0;
+      parity ^= 1;
+    }
+    if (ok) issue();
+  };
+  for (int slot = 2 * worker;; ) {
+    if (seg.blk0 >= seg.blk1) {                               // nothing but the unit's own cost
+      if (!next_piece(p.c, units, seg, f_end)) break;
+      continue;
+    }
     const int hk = seg.unit / row_tiles, rt = seg.unit - hk * row_tiles;
     const int count = checked_count(p.c.status, p.counts, seg.b, p.Nq);
     uint32_t qf[NT][D / 16][2];
@@ -194,199 +205,150 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       for (int c = 0; c < D / 16; ++c) acc[j][c][0] = acc[j][c][1] = acc[j][c][2] = acc[j][c][3] = 0.f;
     }
 
-    for (int kb = seg.blk0 + warp; kb < seg.blk1; kb += C::kWarps) {
-      if (ok && !wait_warp(my_bars + 8 * st, parity, abort_flag)) {
-        ok = false;
-        raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
+    for (int kb = seg.blk0; kb < seg.blk1; ++kb) {
+      const int at = (used >> 1) & 7;
+      arrived();
+      if (!ok) break;
+      const float ks = __shfl_sync(0xffffffffu, ks_reg, at), vs = __shfl_sync(0xffffffffu, vs_reg, at);
+      float s[NT][2][4];
+      keys_times_queries<D, NT>(ring + get * C::kSlotBytes, qf, s);
+      release();
+      const int key0 = kb * 32;
+      const bool cut = key0 + 32 > lim_min;                   // some row does not see all keys of the block
+      const int e_blk = static_cast<int>((__float_as_uint(vs) >> 23) & 0xFF) - 127, e_new = max(vexp, e_blk);
+      // p comes out as 2^off exp(s - m); where V's scale is 2^-60 of another's the product vanishes anyway, but the sum must not
+      const int off = max(15 + e_blk - e_new, -45);
+      const float back = __uint_as_float((127 - off) << 23), shrink = exp2f(static_cast<float>(vexp - e_new));
+      bool moved = e_new != vexp;
+      vexp = e_new;
+      uint32_t pb[NT][2][2];
+      float2 alpha[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const float2 fs = make_float2(f[j].x * ks, f[j].y * ks);
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[j][mt][i] *= (i & 1) ? fs.y : fs.x;
+            if (cut && key0 + 16 * mt + g + 8 * (i >> 1) >= lim[j][i & 1]) s[j][mt][i] = -CUDART_INF_F;
+          }
+        float2 mx = make_float2(fmaxf(fmaxf(s[j][0][0], s[j][0][2]), fmaxf(s[j][1][0], s[j][1][2])),
+                                fmaxf(fmaxf(s[j][0][1], s[j][0][3]), fmaxf(s[j][1][1], s[j][1][3])));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o));
+          mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o));
+        }
+        mx.x = fmaxf(mx.x, m[j][0]);
+        mx.y = fmaxf(mx.y, m[j][1]);
+        moved |= mx.x != m[j][0] || mx.y != m[j][1];
+        const float2 mu = make_float2(mx.x == -CUDART_INF_F ? 0.f : mx.x, mx.y == -CUDART_INF_F ? 0.f : mx.y);
+        alpha[j] = make_float2(ex2_approx(m[j][0] - mu.x), ex2_approx(m[j][1] - mu.y));
+        m[j][0] = mx.x;
+        m[j][1] = mx.y;
+        const float2 sub = make_float2(off - mu.x, off - mu.y);
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          float e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[i] = ex2_approx(s[j][mt][i] + ((i & 1) ? sub.y : sub.x));
+            if (i & 1) sum.y += e[i]; else sum.x += e[i];
+          }
+          pb[j][mt][0] = movmatrix_trans(pack_f16x2(e[0], e[1]));
+          pb[j][mt][1] = movmatrix_trans(pack_f16x2(e[2], e[3]));
+        }
+        l[j][0] = fmaf(l[j][0], alpha[j].x, sum.x * back);
+        l[j][1] = fmaf(l[j][1], alpha[j].y, sum.y * back);
       }
-      if (ok) {
-        const uint32_t kbase = ring + st * C::kStageBytes, vbase = kbase + 32 * D;
-        const float ks = __shfl_sync(0xffffffffu, ks_reg, st), vs = __shfl_sync(0xffffffffu, vs_reg, st);
-        float s[NT][2][4];
-        keys_times_queries<D, NT>(kbase, qf, s);
-        const int key0 = kb * 32;
-        const bool cut = key0 + 32 > lim_min;                 // some row does not see all keys of the block
-        const int e_blk = static_cast<int>((__float_as_uint(vs) >> 23) & 0xFF) - 127, e_new = max(vexp, e_blk);
-        // p comes out as 2^off exp(s - m); where V's scale is 2^-60 of another's the product vanishes anyway, but the sum must not
-        const int off = max(15 + e_blk - e_new, -45);
-        const float back = __uint_as_float((127 - off) << 23), shrink = exp2f(static_cast<float>(vexp - e_new));
-        bool moved = e_new != vexp;
-        vexp = e_new;
-        uint32_t pb[NT][2][2];
-        float2 alpha[NT];
+      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const float2 fs = make_float2(f[j].x * ks, f[j].y * ks);
+          const float ax = alpha[j].x * shrink, ay = alpha[j].y * shrink;
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              s[j][mt][i] *= (i & 1) ? fs.y : fs.x;
-              if (cut && key0 + 16 * mt + g + 8 * (i >> 1) >= lim[j][i & 1]) s[j][mt][i] = -CUDART_INF_F;
-            }
-          float2 mx = make_float2(fmaxf(fmaxf(s[j][0][0], s[j][0][2]), fmaxf(s[j][1][0], s[j][1][2])),
-                                  fmaxf(fmaxf(s[j][0][1], s[j][0][3]), fmaxf(s[j][1][1], s[j][1][3])));
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o));
-            mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o));
-          }
-          mx.x = fmaxf(mx.x, m[j][0]);
-          mx.y = fmaxf(mx.y, m[j][1]);
-          moved |= mx.x != m[j][0] || mx.y != m[j][1];
-          const float2 mu = make_float2(mx.x == -CUDART_INF_F ? 0.f : mx.x, mx.y == -CUDART_INF_F ? 0.f : mx.y);
-          alpha[j] = make_float2(ex2_approx(m[j][0] - mu.x), ex2_approx(m[j][1] - mu.y));
-          m[j][0] = mx.x;
-          m[j][1] = mx.y;
-          const float2 sub = make_float2(off - mu.x, off - mu.y);
-          float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-            float e[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              e[i] = ex2_approx(s[j][mt][i] + ((i & 1) ? sub.y : sub.x));
-              if (i & 1) sum.y += e[i]; else sum.x += e[i];
-            }
-            pb[j][mt][0] = movmatrix_trans(pack_f16x2(e[0], e[1]));
-            pb[j][mt][1] = movmatrix_trans(pack_f16x2(e[2], e[3]));
-          }
-          l[j][0] = fmaf(l[j][0], alpha[j].x, sum.x * back);
-          l[j][1] = fmaf(l[j][1], alpha[j].y, sum.y * back);
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const float ax = alpha[j].x * shrink, ay = alpha[j].y * shrink;
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              acc[j][c][0] *= ax;
-              acc[j][c][1] *= ay;
-              acc[j][c][2] *= ax;
-              acc[j][c][3] *= ay;
-            }
-          }
-        }
-        // slots beyond the length hold anything, NaN codes too: zero times NaN must not reach the sums
-        uint32_t sel[4] = {0x3120u, 0x3120u, 0x3120u, 0x3120u};
-        if (key0 + 32 > seg.n) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = key0 + 8 * i + 2 * t;
-            sel[i] = k + 1 < seg.n ? 0x3120u : k < seg.n ? 0x4140u : 0x4444u;
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t r[4], lo[4], hi[4];
-          ldmatrix4_trans(vbase + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4), r);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            r[i] = prmt(r[i], 0u, sel[i]);
-            lo[i] = e4m3_lo_f16x2(r[i]);
-            hi[i] = e4m3_hi_f16x2(r[i]);
-          }
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            mma_f16(acc[j][c], lo[0], hi[0], lo[1], hi[1], pb[j][0][0], pb[j][0][1]);
-            mma_f16(acc[j][c], lo[2], hi[2], lo[3], hi[3], pb[j][1][0], pb[j][1][1]);
+          for (int c = 0; c < D / 16; ++c) {
+            acc[j][c][0] *= ax;
+            acc[j][c][1] *= ay;
+            acc[j][c][2] *= ax;
+            acc[j][c][3] *= ay;
           }
         }
       }
-      __syncwarp();
-      ++used;
-      if (ok && ahead.live) {
-        issue(st);
-        ++issued;
-        cursor_next(p.c, units, ahead, warp, f_end);
+      arrived();
+      if (!ok) break;
+      const uint32_t vbase = ring + get * C::kSlotBytes;
+      // slots beyond the length hold anything, NaN codes too: zero times NaN must not reach the sums
+      uint32_t sel[4] = {0x3120u, 0x3120u, 0x3120u, 0x3120u};
+      if (key0 + 32 > seg.n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = key0 + 8 * i + 2 * t;
+          sel[i] = k + 1 < seg.n ? 0x3120u : k < seg.n ? 0x4140u : 0x4444u;
+        }
       }
-      if (++st == C::kStages) {
-        st = 0;
-        parity ^= 1;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t r[4], lo[4], hi[4];
+        ldmatrix4_trans(vbase + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4), r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          r[i] = prmt(r[i], 0u, sel[i]);
+          lo[i] = e4m3_lo_f16x2(r[i]);
+          hi[i] = e4m3_hi_f16x2(r[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma_f16(acc[j][c], lo[0], hi[0], lo[1], hi[1], pb[j][0][0], pb[j][0][1]);
+          mma_f16(acc[j][c], lo[2], hi[2], lo[3], hi[3], pb[j][1][0], pb[j][1][1]);
+        }
       }
+      release();
     }
+    if (!ok) break;
 
-    // the four warps' results: maxima and sums, then the accumulators on the common maximum, added in a fixed order
+    const float unit_exp = exp2f(static_cast<float>(vexp - 15));
+    const bool whole = seg.blk0 == 0 && seg.blk1 == seg.blocks;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        float sum = l[j][e];
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], o);
-        if (g == 0) stats[warp * C::kRows + 8 * j + 2 * t + e] = make_float2(m[j][e], l[j][e]);
-      }
-    __syncthreads();
-    const float unit_exp = exp2f(static_cast<float>(max(vexp, -200) - 15));
+        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int in_tile = 8 * j + 2 * t + e, r = rt * C::kRows + in_tile;
+        if (r >= p.Nq * p.rep) continue;
+        if (whole) {
+          const RowInfo ri = row_info(p, r, hk, seg.n, count);
+          const bool any = ri.limit > 0;
+          const float inv = any ? 1.f / sum : 0.f;
+          __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(seg.b) * p.Nq + ri.i) * p.H + ri.head) * D + 2 * g);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (warp / 2 == half) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          float a[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = 8 * j + 2 * t + e;
-            const float top = fmaxf(fmaxf(stats[r].x, stats[C::kRows + r].x), fmaxf(stats[2 * C::kRows + r].x, stats[3 * C::kRows + r].x));
-            a[e] = m[j][e] == -CUDART_INF_F ? 0.f : exp2f(m[j][e] - top) * unit_exp;
+          for (int c = 0; c < D / 16; ++c)
+            o[8 * c] = any ? __floats2bfloat162_rn(acc[j][c][e] * unit_exp * inv, acc[j][c][2 + e] * unit_exp * inv) : __floats2bfloat162_rn(0.f, 0.f);
+          if (g == 0) {
+            p.lse[(static_cast<int64_t>(seg.b) * p.H + ri.head) * p.Nq + ri.i] = any ? (m[j][e] + log2f(sum)) * kLn2 : -CUDART_INF_F;
+            if (p.row_ml != nullptr)
+              p.row_ml[(static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.Nq * p.rep + r] = make_float2(any ? m[j][e] : 0.f, inv);
           }
+        } else {
+          const int64_t row = static_cast<int64_t>(slot) * C::kRows + in_tile;
+          float2* o = reinterpret_cast<float2*>(p.part_o + row * D + 2 * g);
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            float2* r0 = reinterpret_cast<float2*>(slab + ((warp & 1) * C::kRows + 8 * j + 2 * t) * C::kLd + 16 * c + 2 * g);
-            float2* r1 = reinterpret_cast<float2*>(slab + ((warp & 1) * C::kRows + 8 * j + 2 * t + 1) * C::kLd + 16 * c + 2 * g);
-            float2 x = make_float2(acc[j][c][0] * a[0], acc[j][c][2] * a[0]), y = make_float2(acc[j][c][1] * a[1], acc[j][c][3] * a[1]);
-            if (half == 1) {
-              x = add2(x, *r0);
-              y = add2(y, *r1);
-            }
-            *r0 = x;
-            *r1 = y;
-          }
+          for (int c = 0; c < D / 16; ++c) o[8 * c] = make_float2(acc[j][c][e] * unit_exp, acc[j][c][2 + e] * unit_exp);
+          if (g == 0) p.part_ml[row] = make_float2(m[j][e], sum);
         }
       }
-      __syncthreads();
-    }
-    const bool whole = seg.blk0 == 0 && seg.blk1 == seg.blocks;
-    const int rows = p.Nq * p.rep - rt * C::kRows;            // of this tile that exist
-    const int slot = 2 * blockIdx.x + (first ? 0 : 1);
-    for (int x = tid; x < min(rows, C::kRows) * (D / 4); x += 128) {
-      const int r = x / (D / 4), d = (x % (D / 4)) * 4;
-      float2 ml[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) ml[w] = stats[w * C::kRows + r];
-      const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) sum += ml[w].x == -CUDART_INF_F ? 0.f : ml[w].y * exp2f(ml[w].x - top);
-      const float4 u = *reinterpret_cast<const float4*>(slab + r * C::kLd + d), v = *reinterpret_cast<const float4*>(slab + (C::kRows + r) * C::kLd + d);
-      float4 o = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
-      if (whole) {
-        const RowInfo ri = row_info(p, rt * C::kRows + r, hk, seg.n, count);
-        const bool any = ri.limit > 0;
-        const float inv = any ? 1.f / sum : 0.f;
-        uint2 packed;
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(any ? o.x * inv : 0.f, any ? o.y * inv : 0.f);
-        const __nv_bfloat162 hi = __floats2bfloat162_rn(any ? o.z * inv : 0.f, any ? o.w * inv : 0.f);
-        packed.x = *reinterpret_cast<const uint32_t*>(&lo);
-        packed.y = *reinterpret_cast<const uint32_t*>(&hi);
-        *reinterpret_cast<uint2*>(p.o + ((static_cast<int64_t>(seg.b) * p.Nq + ri.i) * p.H + ri.head) * D + d) = packed;
-        if (d == 0) {
-          p.lse[(static_cast<int64_t>(seg.b) * p.H + ri.head) * p.Nq + ri.i] = any ? (top + log2f(sum)) * kLn2 : -CUDART_INF_F;
-          if (p.row_ml != nullptr)
-            p.row_ml[(static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.Nq * p.rep + rt * C::kRows + r] = make_float2(any ? top : 0.f, inv);
-        }
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * C::kRows + r) * D + d) = o;
-        if (d == 0) p.part_ml[static_cast<int64_t>(slot) * C::kRows + r] = make_float2(top, sum);
-      }
-    }
-    first = false;
-    if (!next_segment(p.c, units, seg, f_end)) break;
-    __syncthreads();
+    slot = 2 * worker + 1;
+    if (!next_piece(p.c, units, seg, f_end)) break;
   }
   // given up: the copies in flight must land before the shared memory goes
-  if (!ok) {
-    for (; used < issued; ++used) {
-      wait_or_abort(my_bars + 8 * (used % C::kStages), (used / C::kStages) & 1, abort_flag);
+  for (; used < issued; ++used) {
+    wait_or_abort(my_bars + 8 * get, parity, abort_flag);
+    if (++get == C::kSlots) {
+      get = 0;
+      parity ^= 1;
     }
   }
 }
@@ -398,13 +360,15 @@ template <int D>
 __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p, const int row_tiles, const int row_tile) {
   __shared__ int cum[136];
   __shared__ float part[4][D];
+  __shared__ int slots[128];
+  __shared__ float factors[128], red[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dep_wait();
   const int units = p.c.Hk * row_tiles, R = p.Nq * p.rep;
   const FlatRange range = flat_range(p.c, units, cum);
   const int64_t item = blockIdx.x;                            // (b, hk, r)
   const int r = static_cast<int>(item % R), hk = static_cast<int>(item / R % p.c.Hk), b = static_cast<int>(item / R / p.c.Hk);
-  const int n = cache_length(p.c, b), blocks = (n + 31) / 32, rt = r / row_tile;
+  const int n = cache_length(p.c, b), rt = r / row_tile;
   const int count = checked_count(p.c.status, p.counts, b, p.Nq);
   const RowInfo ri = row_info(p, r, hk, n, count);
   __nv_bfloat16* o = p.o + ((static_cast<int64_t>(b) * p.Nq + ri.i) * p.H + ri.head) * D;
@@ -417,43 +381,66 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
     }
     return;
   }
-  const int f0 = blocks_before(p.c, units, range, b) + (hk * row_tiles + rt) * blocks, f1 = f0 + blocks;
-  const int c0 = range_owner(f0, p.grid, range.total), c1 = range_owner(f1 - 1, p.grid, range.total);
-  if (c0 == c1) return;                                       // whole: written by its CTA
+  const int workers = 4 * p.grid;
+  const int f0 = steps_before(p.c, units, range, b) + sequence_steps(n, hk * row_tiles + rt), f1 = f0 + sequence_steps(n, 1);
+  // the warps that hold blocks of the unit, whose first kUnitCost steps are none
+  const int c0 = range_owner(f0 + kUnitCost, workers, range.total), c1 = range_owner(f1 - 1, workers, range.total);
+  if (c0 == c1) return;                                       // whole: written by its warp
   const int in_tile = r - rt * row_tile;
-  // CTAs between c0 and c1 may own nothing where there are more CTAs than blocks; those that do begin before f1
-  auto slot_of = [&](int c) { return 2 * c + (range_start(c, p.grid, range.total) >= f0 ? 0 : 1); };
-  auto owns = [&](int c) { return range_start(c, p.grid, range.total) < range_start(c + 1, p.grid, range.total); };
+  // Slot of the w-th warp: only c0 can have begun with another unit; warps between c0 and c1 own nothing where there are more of them than steps.
+  auto slot_of = [&](int w) {
+    const int start = range_start(w, workers, range.total);
+    return start == range_start(w + 1, workers, range.total) ? -1 : 2 * w + (start >= f0 ? 0 : 1);
+  };
   float top = -CUDART_INF_F;
-  for (int c = c0 + lane; c <= c1; c += 32)
-    if (owns(c)) top = fmaxf(top, p.part_ml[static_cast<int64_t>(slot_of(c)) * row_tile + in_tile].x);
+  for (int w = c0 + tid; w <= c1; w += 128) {
+    const int at = slot_of(w);
+    if (at >= 0) top = fmaxf(top, p.part_ml[static_cast<int64_t>(at) * row_tile + in_tile].x);
+  }
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   float sum = 0.f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    if (!owns(c)) continue;
-    const int64_t at = static_cast<int64_t>(slot_of(c)) * row_tile + in_tile;
-    const float2 ml = p.part_ml[at];
-    const float w = ml.x == -CUDART_INF_F ? 0.f : exp2f(ml.x - top);
-    sum += ml.y * w;
-    if ((c - c0) % 4 == warp) {
-      const float4* src = reinterpret_cast<const float4*>(p.part_o + at * D) + lane;
+  for (int w0 = c0; w0 <= c1; w0 += 128) {                    // 128 slots at a time: their factors, then their rows
+    const int w = w0 + tid, at = w <= c1 ? slot_of(w) : -1;
+    float f = 0.f;
+    if (at >= 0) {
+      const float2 ml = p.part_ml[static_cast<int64_t>(at) * row_tile + in_tile];
+      f = ml.x == -CUDART_INF_F ? 0.f : exp2f(ml.x - top);
+      sum = fmaf(ml.y, f, sum);
+    }
+    __syncthreads();
+    slots[tid] = max(at, 0);
+    factors[tid] = f;
+    __syncthreads();
+    const int here = min(128, c1 - w0 + 1);
+#pragma unroll 8
+    for (int i = warp; i < here; i += 4) {
+      const float f_i = factors[i];
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slots[i]) * row_tile + in_tile) * D) + lane;
 #pragma unroll
-      for (int i = 0; i < D / 128; ++i) {
-        const float4 v = src[32 * i];
-        acc[4 * i] = fmaf(v.x, w, acc[4 * i]);
-        acc[4 * i + 1] = fmaf(v.y, w, acc[4 * i + 1]);
-        acc[4 * i + 2] = fmaf(v.z, w, acc[4 * i + 2]);
-        acc[4 * i + 3] = fmaf(v.w, w, acc[4 * i + 3]);
+      for (int x = 0; x < D / 128; ++x) {
+        const float4 v = f_i != 0.f ? src[32 * x] : make_float4(0.f, 0.f, 0.f, 0.f);      // a slot without keys, or none, holds anything
+        acc[4 * x] = fmaf(v.x, f_i, acc[4 * x]);
+        acc[4 * x + 1] = fmaf(v.y, f_i, acc[4 * x + 1]);
+        acc[4 * x + 2] = fmaf(v.z, f_i, acc[4 * x + 2]);
+        acc[4 * x + 3] = fmaf(v.w, f_i, acc[4 * x + 3]);
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < D / 128; ++i)
     *reinterpret_cast<float4*>(&part[warp][128 * i + 4 * lane]) = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   __syncthreads();
+  if (lane == 0) red[warp] = sum;
+  __syncthreads();
+  sum = (red[0] + red[1]) + (red[2] + red[3]);
   const float inv = 1.f / sum;
   for (int d = tid; d < D; d += 128) o[d] = __float2bfloat16(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
   if (tid == 0) {
@@ -493,15 +480,15 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
   }
   const int units = p.c.Hk;
   const FlatRange range = flat_range(p.c, units, cum);
-  const int f0 = range_start(blockIdx.x, gridDim.x, range.total), f_end = range_start(blockIdx.x + 1, gridDim.x, range.total);
+  const int worker = blockIdx.x * 4 + warp, workers = gridDim.x * 4;
+  const int f0 = range_start(worker, workers, range.total), f_end = range_start(worker + 1, workers, range.total);
   if (f0 >= f_end) return;
-  Segment seg = first_segment(p.c, units, range, f0, f_end);
-  Cursor ahead = cursor_start(p.c, units, seg, warp, f_end);
+  Piece seg = first_piece(p.c, units, range, f0, f_end);
+  Cursor ahead = cursor_start(p.c, units, seg, f_end);
   const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes, my_bars = smem_u32(bars + warp * kStages);
-  const int bpp = p.c.page / 32;
   float ks_reg = 0.f;
   auto issue = [&](int st) {
-    const int page = max(0, checked_page(p.c, ahead.page)), sub = ahead.kb % bpp, hk = ahead.s.unit;
+    const int page = max(0, checked_page(p.c, ahead.page)), sub = ahead.sub, hk = ahead.s.unit;
     if (lane == 0) {
       const uint32_t bar = my_bars + 8 * st, dst = ring + st * kStageBytes;
       asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kStageBytes) : "memory");
@@ -514,7 +501,7 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
   for (int st = 0; st < kStages && ahead.live; ++st) {
     issue(st);
     ++issued;
-    cursor_next(p.c, units, ahead, warp, f_end);
+    cursor_next(p.c, units, ahead, f_end);
   }
   bool ok = true;
   int st = 0;
@@ -526,7 +513,7 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
     uint32_t qf[NT][D / 16][2];
     float2 f[NT];
     if (row_tiles == 1) load_queries<D, NT>(p, seg.b, hk, 0, count, qf, f);
-    for (int kb = seg.blk0 + warp; kb < seg.blk1; kb += 4) {
+    for (int kb = seg.blk0; kb < seg.blk1; ++kb) {
       if (ok && !wait_warp(my_bars + 8 * st, parity, abort_flag)) {
         ok = false;
         raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
@@ -571,14 +558,14 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
       if (ok && ahead.live) {
         issue(st);
         ++issued;
-        cursor_next(p.c, units, ahead, warp, f_end);
+        cursor_next(p.c, units, ahead, f_end);
       }
       if (++st == kStages) {
         st = 0;
         parity ^= 1;
       }
     }
-    if (!next_segment(p.c, units, seg, f_end)) break;
+    if (!next_piece(p.c, units, seg, f_end)) break;
   }
   if (!ok) {
     for (; used < issued; ++used) wait_or_abort(my_bars + 8 * (used % kStages), (used / kStages) & 1, abort_flag);
@@ -622,12 +609,12 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   const int R = Nq * (H / Hk);
   x.row_tile = R <= 8 ? 8 : R <= 16 || D == 256 ? 16 : 32;
   x.row_tiles = (R + x.row_tile - 1) / x.row_tile;
-  // two CTAs an SM at head_dim 128, one at 256; no more than there can be groups of four blocks
+  // one wave, and no more warps than there can be blocks
   const int64_t most = (static_cast<int64_t>(B) * Hk * x.row_tiles * (static_cast<int64_t>(T) * page / 32) + 3) / 4;
-  const int64_t wave = static_cast<int64_t>(sm_count()) * (D == 128 ? 2 : 1);
-  x.grid = static_cast<int>(most < wave ? (most < 1 ? 1 : most) : wave);
-  x.part_o_bytes = 2ll * x.grid * x.row_tile * D * 4;
-  x.part_ml_bytes = 2ll * x.grid * x.row_tile * 8;
+  const int64_t wave = static_cast<int64_t>(sm_count()) * (D == 128 && x.row_tile == 8 ? AttnCfg<128, 1>::kCtasPerSm : AttnCfg<128, 2>::kCtasPerSm);
+  x.grid = static_cast<int>(most < wave ? most : wave);
+  x.part_o_bytes = 8ll * x.grid * x.row_tile * D * 4;
+  x.part_ml_bytes = 8ll * x.grid * x.row_tile * 8;
   x.row_ml_bytes = weights ? static_cast<int64_t>(B) * Hk * R * 8 : 0;
   return x;
 }
