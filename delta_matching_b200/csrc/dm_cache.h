@@ -71,6 +71,7 @@ struct CacheEvictParams {
 
 // Slots of partial results and their sizes for a call of dm_cache_attn.
 struct CacheAttnPlan {
+  bool chunk;                       // dm_cache_chunk.cu: head_dim 128 and many rows
   int row_tile;                     // query rows (new tokens x heads of a group) a CTA keeps
   int row_tiles;
   int grid;
@@ -80,6 +81,9 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
 
 cudaError_t launch_cache_append(int D, const CacheAppendParams& p, cudaStream_t stream);
 cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, cudaStream_t stream);
+// The form for many rows (its partial results: 2 slots a CTA), and what a row tile of it holds.
+cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, cudaStream_t stream);
+int cache_chunk_rows();
 cudaError_t launch_cache_evict(int D, const CacheEvictParams& p, cudaStream_t stream);
 
 }  // namespace dm

@@ -585,7 +585,7 @@ cudaError_t allow_smem(int bytes) {
 }
 
 template <int D, int NT>
-cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, int row_tiles, cudaStream_t stream) {
+cudaError_t launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, int row_tiles, cudaStream_t stream) {
   using C = AttnCfg<D, NT>;
   cudaError_t e = allow_smem<cache_attn_kernel<D, NT>>(C::kSmem);
   if (e != cudaSuccess) return e;
@@ -593,40 +593,58 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttn
   e = launch_chained(cache_attn_kernel<D, NT>, dim3(p.grid), 128, C::kSmem, stream, tk, tv, p, row_tiles);
   if (e != cudaSuccess) return e;
   count_launch();
-  e = launch_chained(cache_join_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(p.c.B) * p.H * p.Nq)), 128, 0, stream, p, row_tiles, C::kRows);
-  if (e != cudaSuccess || p.weights == nullptr) return e;
-  constexpr int smem = 1024 + 4 * 4 * 32 * D + 4 * 4 * 8 + 136 * 4 + 64;
-  e = allow_smem<cache_weights_kernel<D, NT>>(smem);
-  if (e != cudaSuccess) return e;
-  count_launch();
-  return launch_chained(cache_weights_kernel<D, NT>, dim3(p.grid), 128, smem, stream, tk, p, row_tiles);
+  return launch_chained(cache_join_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(p.c.B) * p.H * p.Nq)), 128, 0, stream, p, row_tiles, C::kRows);
 }
+
+template <int D, int NT>
+cudaError_t launch_weights(const CUtensorMap& tk, const CacheAttnParams& p, cudaStream_t stream) {
+  constexpr int smem = 1024 + 4 * 4 * 32 * D + 4 * 4 * 8 + 136 * 4 + 64;
+  const cudaError_t e = allow_smem<cache_weights_kernel<D, NT>>(smem);
+  if (e != cudaSuccess) return e;
+  // a wave, and no more warps than there can be blocks
+  const int64_t most = (static_cast<int64_t>(p.c.B) * p.c.Hk * p.c.T * (p.c.page / 32) + 3) / 4, wave = sm_count() * 2ll;
+  count_launch();
+  return launch_chained(cache_weights_kernel<D, NT>, dim3(static_cast<unsigned>(most < wave ? most : wave)), 128, smem, stream, tk, p,
+                        (p.Nq * p.rep + 8 * NT - 1) / (8 * NT));
+}
+
+// Rows (new tokens x heads of a group) from which the tcgen05 form is taken, at head_dim 128.
+constexpr int kChunkFrom = 33;
+int small_row_tile(int D, int R) { return R <= 8 ? 8 : R <= 16 || D == 256 ? 16 : 32; }
 
 }  // namespace
 
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights) {
   CacheAttnPlan x;
   const int R = Nq * (H / Hk);
-  x.row_tile = R <= 8 ? 8 : R <= 16 || D == 256 ? 16 : 32;
+  x.chunk = D == 128 && R >= kChunkFrom;
+  x.row_tile = x.chunk ? cache_chunk_rows() : small_row_tile(D, R);
   x.row_tiles = (R + x.row_tile - 1) / x.row_tile;
-  // one wave, and no more warps than there can be blocks
+  // one wave, and no more workers than there can be blocks (tiles of four blocks for a CTA of the tcgen05 form)
   const int64_t most = (static_cast<int64_t>(B) * Hk * x.row_tiles * (static_cast<int64_t>(T) * page / 32) + 3) / 4;
-  const int64_t wave = static_cast<int64_t>(sm_count()) * (D == 128 && x.row_tile == 8 ? AttnCfg<128, 1>::kCtasPerSm : AttnCfg<128, 2>::kCtasPerSm);
+  const int ctas = x.chunk ? 1 : D == 128 && x.row_tile == 8 ? AttnCfg<128, 1>::kCtasPerSm : AttnCfg<128, 2>::kCtasPerSm;
+  const int64_t wave = static_cast<int64_t>(sm_count()) * ctas;
   x.grid = static_cast<int>(most < wave ? most : wave);
-  x.part_o_bytes = 8ll * x.grid * x.row_tile * D * 4;
-  x.part_ml_bytes = 8ll * x.grid * x.row_tile * 8;
+  const int64_t slots = 2ll * x.grid * (x.chunk ? 1 : 4);
+  x.part_o_bytes = slots * x.row_tile * D * 4;
+  x.part_ml_bytes = slots * x.row_tile * 8;
   x.row_ml_bytes = weights ? static_cast<int64_t>(B) * Hk * R * 8 : 0;
   return x;
 }
 
 cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, cudaStream_t stream) {
-  const int R = p.Nq * p.rep;
-  const int tile = R <= 8 ? 8 : R <= 16 || D == 256 ? 16 : 32, row_tiles = (R + tile - 1) / tile;
+  const int R = p.Nq * p.rep, tile = small_row_tile(D, R), row_tiles = (R + tile - 1) / tile;
+  cudaError_t e;
   if (D == 128) {
-    return tile == 8 ? launch<128, 1>(tk, tv, p, row_tiles, stream)
-         : tile == 16 ? launch<128, 2>(tk, tv, p, row_tiles, stream) : launch<128, 4>(tk, tv, p, row_tiles, stream);
+    e = R >= kChunkFrom ? launch_cache_chunk(tk, tv, p, stream)
+      : tile == 8 ? launch_main<128, 1>(tk, tv, p, row_tiles, stream)
+      : tile == 16 ? launch_main<128, 2>(tk, tv, p, row_tiles, stream) : launch_main<128, 4>(tk, tv, p, row_tiles, stream);
+  } else {
+    e = tile == 8 ? launch_main<256, 1>(tk, tv, p, row_tiles, stream) : launch_main<256, 2>(tk, tv, p, row_tiles, stream);
   }
-  return tile == 8 ? launch<256, 1>(tk, tv, p, row_tiles, stream) : launch<256, 2>(tk, tv, p, row_tiles, stream);
+  if (e != cudaSuccess || p.weights == nullptr) return e;
+  if (D == 128) return tile == 8 ? launch_weights<128, 1>(tk, p, stream) : tile == 16 ? launch_weights<128, 2>(tk, p, stream) : launch_weights<128, 4>(tk, p, stream);
+  return tile == 8 ? launch_weights<256, 1>(tk, p, stream) : launch_weights<256, 2>(tk, p, stream);
 }
 
 }  // namespace dm

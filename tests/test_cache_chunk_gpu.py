@@ -1,0 +1,103 @@
+"""Attention over the cache for many new tokens at once (the tcgen05 form at head_dim 128) against its definition in 64 bits: units of 256 rows, whole
+and cut, with one and two row tiles; ranges; special values.  The bounds are those of tests/cache_ref.py."""
+import pytest
+import torch
+
+import delta_matching_b200 as dm
+from delta_matching_b200 import ops
+
+from . import cache_ref as ref
+from .test_cache_gpu import _check, _filled, _ints, _rand
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("N, rep, P", [(48, 8, 64), (150, 1, 32), (40, 5, 160), (9, 4, 96), (259, 2, 128)])
+def test_units(N, rep, P, causal):
+    """33 and more rows: in one row tile, in both, in several units, ending anywhere; lengths below, at and above the counts."""
+    lengths = [700, N, 1000, N + 129, 5]
+    counts = [N, N, N // 2, N - 1, N]
+    cache, pools, table = _filled(lengths, P, 2, 128, seed=N)
+    q = _rand(torch.Generator().manual_seed(N), len(lengths), N, 2 * rep, 128)
+    _check(q, cache, pools, table, lengths, counts, causal, weights=N in (9, 40))
+
+
+@pytest.mark.parametrize("n", [2048, 3000])
+def test_one_sequence_is_cut(n):
+    """One head's keys divided over many CTAs: every row joined from pieces, some of which a row does not see."""
+    N = 64
+    cache, pools, table = _filled([n], 64, 1, 128, seed=n)
+    q = _rand(torch.Generator().manual_seed(n), 1, N, 1, 128)
+    _check(q, cache, pools, table, [n])
+
+
+@pytest.mark.parametrize("kscale, vscale, qscale, scale", [(1e-20, 1.0, 1e20, None), (1.0, 1e-30, 1.0, None), (1.0, 1e30, 1.0, None), (30.0, 1.0, 30.0, None),
+                                                           (1.0, 1.0, 1.0, 3.0), (1.0, 1.0, 1e-30, None)])
+def test_ranges(kscale, vscale, qscale, scale):
+    lengths = [450, 97]
+    cache, pools, table = _filled(lengths, 32, 1, 128, kscale=kscale, vscale=vscale)
+    q = _rand(torch.Generator().manual_seed(1), 2, 14, 3, 128, scale=qscale)
+    q[0, 0, 1] = 0                                               # a query of zeros sees all keys alike
+    _check(q, cache, pools, table, lengths, scale=scale, weights=True)
+
+
+def test_blocks_of_very_different_size():
+    """V blocks 2^-100 ... 2^100 of one another and blocks of zeros, in an order that makes the running scale jump; a key that takes all; maxima that
+    rise from tile to tile."""
+    B, Hk, D, P, n = 3, 1, 128, 32, 32 * 21 + 5
+    cache = ref.make_cache(B * 22, P, Hk, D)
+    table = ref.make_table(B, 22, B * 22)
+    g = torch.Generator().manual_seed(8)
+    k, v, q = _rand(g, B, n, Hk, D), _rand(g, B, n, Hk, D), _rand(g, B, 10, 4, D)
+    for j, e in enumerate((0, -100, 3, 100, -3, -40, 40, 0, 20, -20, 99, 1, -99, 0, 7, -7, 30, -30, 2, 60, -60, 101)):
+        v[0, 32 * j:32 * j + 32] *= 2.0 ** e
+    v[1, 64:300] = 0
+    k[1, 96:160] = 0
+    k[1, 400] *= 40
+    k[2] *= torch.linspace(0.1, 6.0, n)[:, None, None].to(k.dtype)
+    dm.dm_cache_append(cache, k.cuda(), v.cuda(), table.cuda(), _ints([0] * B).cuda())
+    _check(q, cache, ref.Pools(cache), table, [n] * B)
+    _check(q, cache, ref.Pools(cache), table, [32 * 3, 32 * 6 + 1, 400])
+
+
+def test_nan_inputs():
+    """A NaN among the held values or in a query reaches the rows that see it and no others."""
+    lengths, N, rep = [300, 300], 24, 2
+    cache, pools, table = _filled(lengths, 32, 1, 128)
+    q = _rand(torch.Generator().manual_seed(2), 2, N, rep, 128).cuda()
+    clean = dm.dm_cache_attn(q, cache, table.cuda(), _ints(lengths).cuda())
+    bad = q.clone()
+    bad[0, 3, 1, 7] = float("nan")
+    o = dm.dm_cache_attn(bad, cache, table.cuda(), _ints(lengths).cuda())
+    want = torch.zeros_like(o, dtype=torch.bool)
+    want[0, 3, 1] = True
+    assert torch.equal(o.isnan(), want) and torch.equal(o[~want], clean[~want])
+    cache.k8.view(torch.uint8)[int(table[1, 280 // 32]), 0, 280 % 32, 3] = 0x7F
+    o = dm.dm_cache_attn(q, cache, table.cuda(), _ints(lengths).cuda())
+    assert torch.equal(o[0], clean[0])
+    seen = torch.arange(N) + 300 - N >= 280                      # the tokens whose causal view reaches it
+    assert torch.equal(o[1].isnan().all(-1).all(-1).cpu(), seen) and torch.equal(o[1].isnan().any(-1).any(-1).cpu(), seen)
+
+
+def test_repeats_bit_for_bit():
+    lengths = [1900, 117, 833]
+    cache, pools, table = _filled(lengths, 64, 2, 128)
+    q = _rand(torch.Generator().manual_seed(4), 3, 70, 8, 128).cuda()
+    t, n = table.cuda(), _ints(lengths).cuda()
+    first = dm.dm_cache_attn(q, cache, t, n, return_lse=True)
+    for _ in range(10):
+        again = dm.dm_cache_attn(q, cache, t, n, return_lse=True)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+    ops.check_status("cuda")
+
+
+def test_bad_device_values_are_reported():
+    cache, pools, table = _filled([40, 40], 32, 1, 128)
+    q = torch.randn(2, 20, 2, 128, device="cuda", dtype=torch.bfloat16)
+    n = _ints([40, 40]).cuda()
+    for bad_table, bad_n, counts, says in ((_ints([[0, 99], [1, 2]]), n, None, "page"), (_ints([[0, -1], [1, 2]]), n, None, "page"),
+                                           (table, _ints([40, 1000]).cuda(), None, "length"), (table, n, _ints([1, 70]).cuda(), "length")):
+        dm.dm_cache_attn(q, cache, bad_table.cuda(), bad_n, q_counts=counts)
+        with pytest.raises(RuntimeError, match=says):
+            ops.check_status("cuda")
