@@ -48,6 +48,7 @@ struct CacheAttnParams {
   float* lse;                       // (B, H, Nq)
   float* part_o;                    // partial results: 2 slots a warp of (row tile, D) fp32, and their (maximum, sum) pairs
   float2* part_ml;
+  int2* unit_slots;                 // per unit (B, Hk, row tiles): slot of its first piece (-1: whole), the last worker that has one
   float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null
   float* weights;                   // (B, Hk, W) or null
   int64_t w_sb, w_sh;
@@ -75,7 +76,7 @@ struct CacheAttnPlan {
   int row_tile;                     // query rows (new tokens x heads of a group) a CTA keeps
   int row_tiles;
   int grid;
-  int64_t part_o_bytes, part_ml_bytes, row_ml_bytes;
+  int64_t part_o_bytes, part_ml_bytes, unit_bytes, row_ml_bytes;
 };
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights);
 

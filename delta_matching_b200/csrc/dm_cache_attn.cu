@@ -128,9 +128,9 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   grid_dep_wait();
   const int units = p.c.Hk * row_tiles;
   const FlatRange range = flat_range(p.c, units, cum);        // its barriers publish the mbarriers too
-  const int worker = blockIdx.x * C::kWarps + warp, workers = p.grid * C::kWarps;
+  const int worker = blockIdx.x * C::kWarps + warp, workers = min(p.grid * C::kWarps, range.total);      // each has a step at least
+  if (worker >= workers) return;
   const int f0 = range_start(worker, workers, range.total), f_end = range_start(worker + 1, workers, range.total);
-  if (f0 >= f_end) return;
   Piece seg = first_piece(p.c, units, range, f0, f_end);
   Cursor ahead = cursor_start(p.c, units, seg, f_end);
 
@@ -310,6 +310,12 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
     const float unit_exp = exp2f(static_cast<float>(vexp - 15));
     const bool whole = seg.blk0 == 0 && seg.blk1 == seg.blocks;
+    // where the join finds the unit: the slot of its first piece, and the last warp that has one (the pieces between are their warps' first)
+    if (lane == 0) {
+      int2* u = p.unit_slots + (static_cast<int64_t>(seg.b) * units + seg.unit);
+      if (seg.blk0 == 0) u->x = whole ? -1 : slot;
+      if (seg.blk1 == seg.blocks) u->y = worker;
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -358,17 +364,15 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 // Also rows of sequences that hold nothing.
 template <int D>
 __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p, const int row_tiles, const int row_tile) {
-  __shared__ int cum[136];
   __shared__ float part[4][D];
-  __shared__ int slots[128];
   __shared__ float factors[128], red[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dep_wait();
-  const int units = p.c.Hk * row_tiles, R = p.Nq * p.rep;
-  const FlatRange range = flat_range(p.c, units, cum);
+  const int R = p.Nq * p.rep;
   const int64_t item = blockIdx.x;                            // (b, hk, r)
-  const int r = static_cast<int>(item % R), hk = static_cast<int>(item / R % p.c.Hk), b = static_cast<int>(item / R / p.c.Hk);
-  const int n = cache_length(p.c, b), rt = r / row_tile;
+  const int bh = static_cast<int>(item / R), r = static_cast<int>(item - static_cast<int64_t>(bh) * R), hk = bh % p.c.Hk, b = bh / p.c.Hk, rt = r / row_tile;
+  const int2 unit = p.unit_slots[static_cast<int64_t>(bh) * row_tiles + rt];
+  const int n = cache_length(p.c, b);
   const int count = checked_count(p.c.status, p.counts, b, p.Nq);
   const RowInfo ri = row_info(p, r, hk, n, count);
   __nv_bfloat16* o = p.o + ((static_cast<int64_t>(b) * p.Nq + ri.i) * p.H + ri.head) * D;
@@ -381,22 +385,13 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
     }
     return;
   }
-  const int workers = 4 * p.grid;
-  const int f0 = steps_before(p.c, units, range, b) + sequence_steps(n, hk * row_tiles + rt), f1 = f0 + sequence_steps(n, 1);
-  // the warps that hold blocks of the unit, whose first kUnitCost steps are none
-  const int c0 = range_owner(f0 + kUnitCost, workers, range.total), c1 = range_owner(f1 - 1, workers, range.total);
-  if (c0 == c1) return;                                       // whole: written by its warp
+  if (unit.x < 0) return;                                     // whole: written by its warp
+  // pieces: the first one's slot, then the first slots of the warps behind it
+  const int w0 = unit.x / 2, pieces = unit.y - w0 + 1;
   const int in_tile = r - rt * row_tile;
-  // Slot of the w-th warp: only c0 can have begun with another unit; warps between c0 and c1 own nothing where there are more of them than steps.
-  auto slot_of = [&](int w) {
-    const int start = range_start(w, workers, range.total);
-    return start == range_start(w + 1, workers, range.total) ? -1 : 2 * w + (start >= f0 ? 0 : 1);
-  };
+  auto row_of = [&](int i) { return static_cast<int64_t>(i == 0 ? unit.x : 2 * (w0 + i)) * row_tile + in_tile; };
   float top = -CUDART_INF_F;
-  for (int w = c0 + tid; w <= c1; w += 128) {
-    const int at = slot_of(w);
-    if (at >= 0) top = fmaxf(top, p.part_ml[static_cast<int64_t>(at) * row_tile + in_tile].x);
-  }
+  for (int i = tid; i < pieces; i += 128) top = fmaxf(top, p.part_ml[row_of(i)].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) red[warp] = top;
@@ -405,26 +400,23 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
   float sum = 0.f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  for (int w0 = c0; w0 <= c1; w0 += 128) {                    // 128 slots at a time: their factors, then their rows
-    const int w = w0 + tid, at = w <= c1 ? slot_of(w) : -1;
+  for (int i0 = 0; i0 < pieces; i0 += 128) {                  // 128 pieces at a time: their factors, then their rows
     float f = 0.f;
-    if (at >= 0) {
-      const float2 ml = p.part_ml[static_cast<int64_t>(at) * row_tile + in_tile];
+    if (i0 + tid < pieces) {
+      const float2 ml = p.part_ml[row_of(i0 + tid)];
       f = ml.x == -CUDART_INF_F ? 0.f : exp2f(ml.x - top);
       sum = fmaf(ml.y, f, sum);
     }
-    __syncthreads();
-    slots[tid] = max(at, 0);
+    if (i0 > 0) __syncthreads();
     factors[tid] = f;
     __syncthreads();
-    const int here = min(128, c1 - w0 + 1);
 #pragma unroll 8
-    for (int i = warp; i < here; i += 4) {
+    for (int i = warp; i < min(128, pieces - i0); i += 4) {
       const float f_i = factors[i];
-      const float4* src = reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slots[i]) * row_tile + in_tile) * D) + lane;
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + row_of(i0 + i) * D) + lane;
 #pragma unroll
       for (int x = 0; x < D / 128; ++x) {
-        const float4 v = f_i != 0.f ? src[32 * x] : make_float4(0.f, 0.f, 0.f, 0.f);      // a slot without keys, or none, holds anything
+        const float4 v = src[32 * x];
         acc[4 * x] = fmaf(v.x, f_i, acc[4 * x]);
         acc[4 * x + 1] = fmaf(v.y, f_i, acc[4 * x + 1]);
         acc[4 * x + 2] = fmaf(v.z, f_i, acc[4 * x + 2]);
@@ -628,6 +620,7 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   const int64_t slots = 2ll * x.grid * (x.chunk ? 1 : 4);
   x.part_o_bytes = slots * x.row_tile * D * 4;
   x.part_ml_bytes = slots * x.row_tile * 8;
+  x.unit_bytes = static_cast<int64_t>(B) * Hk * x.row_tiles * 8;
   x.row_ml_bytes = weights ? static_cast<int64_t>(B) * Hk * R * 8 : 0;
   return x;
 }

@@ -1,8 +1,8 @@
 // Attention of many new queries over the 8-bit cache (chunks of a prompt): the same result as dm_cache_attn.cu, on tcgen05.
 //
 //   S = Q K^T and O += P V as f16 tcgen05 chains with fp32 accumulators in TMEM.  The codes are exact in f16, q is brought to f16 with a power
-//   of two per row, P is f16 with the row's reference maximum at 2^15 (11 bits, never closer than 2^-40 of the row's largest); K's
-//   block scales go into the factors of the logits, V's into the exponent of P relative to the largest the row tile has met.
+//   of two per row, P is f16 with the row's reference maximum at 2^12 (11 bits, never closer than 2^-37 of it); K's block scales go into
+//   the factors of the logits, V's into the exponent of P relative to the largest the row tile has met.
 //
 // A unit is (sequence, kv head, 256 rows); rows are (new token, head of the group).  The key tiles of 128 tokens of all units are one flat
 // range, divided evenly over one CTA per SM (as the warps' blocks are in dm_cache_sched.cuh); pieces of cut units are joined by a second kernel.
@@ -11,7 +11,9 @@
 // one is in its softmax the tensor cores work for the other.
 //
 // TMEM: S0 0-127, S1 128-255 (P of a tile over the first 64 columns of its S), O0 256-383, O1 384-511.
-// The maximum moves only when a row exceeds its reference by a factor of two (P then still fits f16's range), so O is seldom rescaled.
+// The reference moves only when a row exceeds it by more than 2^3.9 (P then still fits f16's range), so O is seldom rescaled: a move costs its
+// row tile about 3000 cycles, and with a reference that follows within a factor of two some warp moved it in most tiles (6800 cycles a tile).
+#include <type_traits>
 #include "dm_cache.cuh"
 #include "dm_kernels.h"
 
@@ -20,6 +22,8 @@ namespace dm {
 namespace {
 
 constexpr int kChunkCost = 2;               // key tiles that a unit's queries and output are worth
+constexpr int kPBase = 12;                  // log2 of P at the reference maximum,
+constexpr float kHeadroom = 3.9f;           // and what a row may exceed it by: P stays below 2^16
 
 struct ChunkCfg {
   static constexpr int D = 128;
@@ -71,7 +75,7 @@ __device__ __forceinline__ int head_steps(const CacheAttnParams& p, int b) {
 }
 
 // Steps before each group of sequences, 128 groups; executed by the first 128 threads (barrier 1).
-__device__ __forceinline__ int chunk_range(const CacheAttnParams& p, int* cum, int tid) {
+__device__ __forceinline__ void chunk_range(const CacheAttnParams& p, int* cum, int tid) {
   const int lane = tid & 31, chunk = (p.c.B + 127) / 128;
   int incl = 0;
   for (int i = tid * chunk; i < min(p.c.B, (tid + 1) * chunk); ++i) incl += head_steps(p, i) * p.c.Hk;
@@ -85,13 +89,8 @@ __device__ __forceinline__ int chunk_range(const CacheAttnParams& p, int* cum, i
   for (int w = 0; w < (tid >> 5); ++w) incl += cum[129 + w];
   cum[tid + 1] = incl;
   if (tid == 0) cum[0] = 0;
-  return chunk;
 }
 __device__ __forceinline__ int share_start(int cta, int grid, int total) { return static_cast<int>(static_cast<int64_t>(cta) * total / grid); }
-__device__ __forceinline__ int share_owner(int f, int grid, int total) {
-  return static_cast<int>(((static_cast<int64_t>(f) + 1) * grid - 1) / total);
-}
-
 // A CTA's piece of a unit: key tiles t0 ... t1 - 1.
 struct ChunkPiece {
   int b, hk, rt;
@@ -228,7 +227,9 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int total = cum[128];
-  const int f0 = share_start(blockIdx.x, p.grid, total), f_end = share_start(blockIdx.x + 1, p.grid, total);
+  const int sharers = min(p.grid, total);                     // each has a step at least
+  const int cta = blockIdx.x;
+  const int f0 = cta < sharers ? share_start(cta, sharers, total) : 0, f_end = cta < sharers ? share_start(cta + 1, sharers, total) : 0;
   bool ok = true;
   auto bar = [&](int i) { return smem_u32(bars + i); };
 
@@ -239,37 +240,65 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     }
     if (warp == 12) {
       // ---------------------------------------------------------------------------------------- TMA: code tiles and their scales
-      int g = 0;                                              // running tile
+      // Lane i < 4 looks after block i of a tile.  A tile's pages are asked for two tiles ahead of its loads and its scales one tile ahead, so
+      // that the loads wait for free buffers alone.
+      struct Ahead {
+        bool live, held;
+        int hk, page, sub;
+        float ks, vs;
+      };
       const int bpp = p.c.page / 32;
-      do {
-        for (int t = x.t0; t < x.t1 && ok; ++t, ++g) {
-          // lane i < 4: block 4 t + i of the sequence, its page and scales
-          const int blk = 4 * t + lane;
-          const bool held = lane < 4 && blk * 32 < x.s.n;
-          int page = 0, sub = 0;
-          if (held) {
-            const int entry = blk / bpp;
-            sub = blk - entry * bpp;
-            page = max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + entry)));
-          }
-          const int boxes = __popc(__ballot_sync(0xffffffffu, held));
-          for (int kv = 0; kv < 2; ++kv) {
-            if (g > 0) ok = ok && wait_warp(bar(kCodeEmpty + kv), (g - 1) & 1, abort_flag);
-            if (!ok) break;
-            if (lane == 0) mbar_expect_tx(bars + kCodeFull + kv, boxes * 4096);
-            __syncwarp();
-            if (held) tma_load_4d(sbase + C::kSmemCode + kv * C::kTile + lane * 4096, kv ? &tv : &tk, bar(kCodeFull + kv), 0, sub * 32, x.hk, page);
-          }
-          if (!ok) break;
-          if (lane < 4) {
-            const int64_t at = page * p.c.s_page + x.hk * p.c.s_head + sub;
-            scales[(g & 7) * 8 + lane] = held ? __ldg(p.c.ks + at) : 0.f;
-            scales[(g & 7) * 8 + 4 + lane] = held ? __ldg(p.c.vs + at) : 0.f;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
+      int t = x.t0;
+      bool more = true;                                       // (x, t) is the next tile to be looked up
+      auto look_up = [&]() {
+        Ahead a{};
+        while (more && t >= x.t1) {
+          more = next_chunk(p, x, f_end);
+          t = x.t0;
         }
-      } while (ok && next_chunk(p, x, f_end));
+        a.live = more;
+        if (!more) return a;
+        const int blk = 4 * t++ + lane;
+        a.held = lane < 4 && blk * 32 < x.s.n;
+        a.hk = x.hk;
+        if (a.held) {
+          const int entry = blk / bpp;
+          a.sub = blk - entry * bpp;
+          a.page = __ldg(p.c.table + x.b * p.c.t_row + entry);
+        }
+        return a;
+      };
+      auto ask_scales = [&](Ahead& a) {
+        if (!a.held) return;
+        a.page = max(0, checked_page(p.c, a.page));
+        const int64_t at = a.page * p.c.s_page + a.hk * p.c.s_head + a.sub;
+        a.ks = __ldg(p.c.ks + at);
+        a.vs = __ldg(p.c.vs + at);
+      };
+      int g = 0;                                              // running tile
+      Ahead now = look_up(), next = look_up();
+      ask_scales(now);
+      for (; now.live; ++g) {
+        const Ahead after = look_up();
+        ask_scales(next);
+        const int boxes = __popc(__ballot_sync(0xffffffffu, now.held));
+        for (int kv = 0; kv < 2; ++kv) {
+          if (g > 0) ok = ok && wait_warp(bar(kCodeEmpty + kv), (g - 1) & 1, abort_flag);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(bars + kCodeFull + kv, boxes * 4096);
+          __syncwarp();
+          if (now.held) tma_load_4d(sbase + C::kSmemCode + kv * C::kTile + lane * 4096, kv ? &tv : &tk, bar(kCodeFull + kv), 0, now.sub * 32, now.hk, now.page);
+        }
+        if (!ok) break;
+        if (lane < 4) {
+          scales[(g & 7) * 8 + lane] = now.ks;                // zero where there is no block
+          scales[(g & 7) * 8 + 4 + lane] = now.vs;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
+        now = next;
+        next = after;
+      }
       if (!ok) {
         if (lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutProducer + kInCache);
         // what is in flight lands before the shared memory goes
@@ -380,41 +409,53 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const int r = warp >> 2, in_tile = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t t_s = tmem + lanes + 128 * r, t_o = tmem + lanes + 256 + 128 * r;
-      const uint32_t q_row = sbase + C::kSmemQ + r * 2 * C::kTile + in_tile * 128;
+      // the warp's own 32 rows of the query tile's two panels: 8 KB for its output on the way out
+      const uint32_t stage = sbase + C::kSmemQ + r * 2 * C::kTile + (warp & 3) * 4096;
       int g = 0, mine = 0;                                    // running tile, those of this row tile
-      int slot = 2 * blockIdx.x;
+      int slot = 2 * cta;
       do {
         if (x.t0 >= x.t1) continue;
         if (r >= x.row_tiles(p)) {
           g += x.t1 - x.t0;
-          slot = 2 * blockIdx.x + 1;
+          slot = 2 * cta + 1;
           continue;
         }
         const int row = x.rt * C::kRows + r * 128 + in_tile, limit = row_limit(p, x.s, row);
         const int i_tok = row / p.rep, head = x.hk * p.rep + row - i_tok * p.rep;
+        // The warp's 32 query rows, sixteen lanes a row: to f16 with a power of two per row, into the operand tile.
         float f;                                              // factor of the row's logits, K's scale aside
         {
-          const __nv_bfloat16* src = p.q + x.b * p.q_sb + i_tok * p.q_sn + head * p.q_sh;
-          uint4 w[16];
-          float amax = 0.f;
+          const int c16 = lane & 15;
+          uint32_t my_eb = 0;
+#pragma unroll 1
+          for (int i0 = 0; i0 < 16; i0 += 8) {
+            uint4 w[8];
+            int tr = (warp & 3) * 32 + 2 * i0 + (lane >> 4);  // row of the tile
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            w[i] = row < x.s.count * p.rep ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-            const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            for (int i = 0; i < 8; ++i) {
+              const int q_r = x.rt * C::kRows + r * 128 + tr + 2 * i, tok = q_r / p.rep;
+              w[i] = make_uint4(0, 0, 0, 0);
+              if (tok < x.s.count) w[i] = __ldg(reinterpret_cast<const uint4*>(p.q + x.b * p.q_sb + tok * p.q_sn + (x.hk * p.rep + q_r - tok * p.rep) * p.q_sh) + c16);
+            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(v[j] << 16)), fabsf(__uint_as_float(v[j] & 0xFFFF0000u))));
+            for (int i = 0; i < 8; ++i, tr += 2) {
+              const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+              float amax = 0.f;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) amax = max3(amax, fabsf(__uint_as_float(v[j] << 16)), fabsf(__uint_as_float(v[j] & 0xFFFF0000u)));
+#pragma unroll
+              for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+              const uint32_t eb = min(254u, max(14u, __float_as_uint(amax) >> 23));
+              const float up = sb_to_scale(267u - eb);        // largest element to [2^13, 2^14)
+              uint32_t h[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) h[j] = pack_f16x2(__uint_as_float(v[j] << 16) * up, __uint_as_float(v[j] & 0xFFFF0000u) * up);
+              sts_u4(sbase + C::kSmemQ + r * 2 * C::kTile + (c16 >> 3) * C::kTile + tr * 128 + (((c16 & 7) ^ (tr & 7)) << 4), h[0], h[1], h[2], h[3]);
+              const uint32_t of_mine = __shfl_sync(0xffffffffu, eb, (lane & 1) * 16);
+              if ((lane >> 1) == i0 + i) my_eb = of_mine;
+            }
           }
-          const uint32_t eb = min(254u, max(14u, __float_as_uint(amax) >> 23));
-          const float up = sb_to_scale(267u - eb);            // largest element to [2^13, 2^14)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-            uint32_t h[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = pack_f16x2(__uint_as_float(v[j] << 16) * up, __uint_as_float(v[j] & 0xFFFF0000u) * up);
-            sts_u4(q_row + (i >> 3) * C::kTile + (((i & 7) ^ (in_tile & 7)) << 4), h[0], h[1], h[2], h[3]);
-          }
-          f = sb_to_scale(eb - 13u) * p.scale * kLog2e;
+          f = sb_to_scale(my_eb - 13u) * p.scale * kLog2e;
         }
         fence_async_smem();
         __syncwarp();
@@ -422,45 +463,48 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 
         float m = -CUDART_INF_F, l = 0.f;
         int vexp = -1000;
-        for (int t = x.t0; t < x.t1; ++t, ++g, ++mine) {
-          ok = wait_warp(bar(kScales + (g & 7)), (g >> 3) & 1, abort_flag) && wait_warp(bar(kSFull + r), mine & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
+        // One key tile.  kCut: some row of the warp does not see all its keys (a compile-time variant: no select per element elsewhere).
+        auto tile = [&](int t, auto cut_tag) -> bool {
+          constexpr bool kCut = decltype(cut_tag)::value;
           const float4 ks = lds_f4(sbase + C::kSmemScales + (g & 7) * 32), vs = lds_f4(sbase + C::kSmemScales + (g & 7) * 32 + 16);
           const float fc[4] = {f * ks.x, f * ks.y, f * ks.z, f * ks.w};
           const int ev[4] = {static_cast<int>(scale_to_sb(vs.x)) - 127, static_cast<int>(scale_to_sb(vs.y)) - 127, static_cast<int>(scale_to_sb(vs.z)) - 127,
                              static_cast<int>(scale_to_sb(vs.w)) - 127};
           const int seen = limit - 128 * t;                   // keys of the tile that the row sees
-          const bool cut = __any_sync(0xffffffffu, seen < 128);
-          float top = -CUDART_INF_F;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tmem_ld32(t_s + 32 * c, s);
+          const int v_new = max(max(vexp, max(ev[0], ev[1])), max(ev[2], ev[3]));
+          // 32 columns at a time, the next ones in flight; what a row does not see is -inf
+          uint32_t s_buf[2][32];
+          auto columns = [&](int c) {
             tmem_wait_ld();
-            if (cut) {
+            if (c < 3) tmem_ld32(t_s + 32 * (c + 1), s_buf[(c + 1) & 1]);
+            if (kCut) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (32 * c + e >= seen) s[e] = 0xff800000u;
+                if (32 * c + e >= seen) s_buf[c & 1][e] = 0xff800000u;
             }
+          };
+          auto pair = [&](int c, int e) { return make_float2(__uint_as_float(s_buf[c & 1][2 * e]), __uint_as_float(s_buf[c & 1][2 * e + 1])); };
+          float top = -CUDART_INF_F;
+          tmem_ld32(t_s, s_buf[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            columns(c);
             float2 s2[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s2[e] = make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+            for (int e = 0; e < 16; ++e) s2[e] = pair(c, e);
             const float top_c = max32(s2);
-            top = fmaxf(top, top_c == -CUDART_INF_F ? top_c : top_c * fc[c]);
+            top = fmaxf(top, kCut && top_c == -CUDART_INF_F ? top_c : top_c * fc[c]);     // the factor may be zero
           }
-          // the reference moves where the row exceeds it by a factor of two: P stays below 2^16
-          const float m_new = top > m + 0.999f ? top : m;
-          const int v_new = max(max(vexp, max(ev[0], ev[1])), max(ev[2], ev[3]));
+          const float m_new = top > m + kHeadroom ? top : m;
           const float mu = m_new == -CUDART_INF_F ? 0.f : m_new;
-          const float keep = ex2_approx(m - mu);
+          tmem_ld32(t_s, s_buf[0]);
           if (__any_sync(0xffffffffu, m_new != m || v_new != vexp)) {
+            const float keep = ex2_approx(m - mu);
             if (t > x.t0) {
-              ok = wait_warp(bar(kPvDone + r), (mine - 1) & 1, abort_flag);
-              if (!ok) break;
+              if (!wait_warp(bar(kPvDone + r), (mine - 1) & 1, abort_flag)) return false;
               tc_fence_after();
               const float a = keep * exp2f(static_cast<float>(vexp - v_new));
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
                 tmem_ld32(t_o + 32 * c, o);
@@ -469,7 +513,6 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
                 tmem_st32(t_o + 32 * c, o);
               }
-              tmem_wait_st();
             }
             l *= keep;
             m = m_new;
@@ -477,18 +520,16 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tmem_ld32(t_s + 32 * c, s);
-            // P comes out as 2^off exp(s - m); where V's scale is 2^-60 of another's the product vanishes anyway, but the sum must not
-            const int off = max(15 + ev[c] - vexp, -45);
+            // P comes out as 2^off exp(s - m); where V's scale is 2^-57 of another's the product vanishes anyway, but the sum must not
+            const int off = max(kPBase + ev[c] - vexp, -45);
             const float2 f2 = splat2(fc[c]), sub = splat2(static_cast<float>(off) - mu);
+            columns(c);
             float2 sum = make_float2(0.f, 0.f);
             uint32_t h[16];
-            tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              float2 y = fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), f2, sub);
-              if (cut) {
+              float2 y = fma2(pair(c, e), f2, sub);
+              if (kCut) {                                     // zero times infinity is none
                 if (32 * c + 2 * e >= seen) y.x = -CUDART_INF_F;
                 if (32 * c + 2 * e + 1 >= seen) y.y = -CUDART_INF_F;
               }
@@ -497,33 +538,43 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
               h[e] = pack_f16x2(y.x, y.y);
             }
             l = fmaf(sum.x + sum.y, __uint_as_float(static_cast<uint32_t>(127 - off) << 23), l);
-            tmem_st16(t_s + 16 * c, h);
+            tmem_st16(t_s + 16 * c, h);                       // over columns that have been read: 16 c + 15 < 32 c + 32
           }
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bars + kPFull + r);
+          return true;
+        };
+        for (int t = x.t0; t < x.t1; ++t, ++g, ++mine) {
+          ok = wait_warp(bar(kScales + (g & 7)), (g >> 3) & 1, abort_flag) && wait_warp(bar(kSFull + r), mine & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const bool cut = __any_sync(0xffffffffu, limit < 128 * (t + 1));
+          if (!(ok = cut ? tile(t, std::true_type{}) : tile(t, std::false_type{}))) break;
         }
         if (!ok) break;
         ok = wait_warp(bar(kPvDone + r), (mine - 1) & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
         const bool whole = x.t0 == 0 && x.t1 == x.tiles;
-        const float unit_exp = exp2f(static_cast<float>(vexp - 15));
+        const float unit_exp = exp2f(static_cast<float>(vexp - kPBase));
         const float scale = whole ? unit_exp / l : unit_exp;
-        __nv_bfloat16* o16 = p.o + ((static_cast<int64_t>(x.b) * p.Nq + i_tok) * p.H + head) * D;
-        const int64_t part = static_cast<int64_t>(slot) * C::kRows + r * 128 + in_tile;
-        float* o32 = p.part_o + part * D;
+        // Through shared memory (the queries are done with), so that the lanes of a store write whole rows: a row a thread, 16 bytes at a
+        // time, took 11000 cycles a piece.  Staged: 32 rows x 256 bytes, 16-byte pieces XORed with the row.
+        const int64_t part0 = static_cast<int64_t>(slot) * C::kRows + r * 128 + (warp & 3) * 32;
+        auto staged = [&](int row32, int piece) { return stage + (piece >> 3) * C::kTile + row32 * 128 + (((piece & 7) ^ (row32 & 7)) << 4); };
+#pragma unroll 1
+        for (int half = 0; half < (whole ? 1 : 2); ++half) {
+#pragma unroll 1
+          for (int c = whole ? 0 : 2 * half; c < (whole ? 4 : 2 * half + 2); ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o + 32 * c, o);
+            tmem_wait_ld();
+            float v[32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + 32 * c, o);
-          tmem_wait_ld();
-          float v[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * scale;
-          if (whole) {
-            if (limit > 0) {
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * scale;
+            if (whole) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 uint32_t w[4];
@@ -532,24 +583,46 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                   const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[8 * e + 2 * j], v[8 * e + 2 * j + 1]);
                   w[j] = *reinterpret_cast<const uint32_t*>(&b2);
                 }
-                *reinterpret_cast<uint4*>(o16 + 32 * c + 8 * e) = make_uint4(w[0], w[1], w[2], w[3]);
+                sts_u4(staged(lane, 4 * c + e), w[0], w[1], w[2], w[3]);
               }
-            }
-          } else if (limit > 0) {
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) *reinterpret_cast<float4*>(o32 + 32 * c + 4 * e) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+              for (int e = 0; e < 8; ++e)
+                sts_u4(staged(lane, 8 * (c & 1) + e), __float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
+            }
           }
+          __syncwarp();
+#pragma unroll 2
+          for (int i = 0; i < 16; ++i) {
+            const int row32 = 2 * i + (lane >> 4), piece = lane & 15;
+            const float4 v = lds_f4(staged(row32, piece));
+            const int row_limit32 = __shfl_sync(0xffffffffu, limit, row32);
+            if (row_limit32 == 0) continue;
+            if (whole) {
+              const int q_r = x.rt * C::kRows + r * 128 + (warp & 3) * 32 + row32, tok = q_r / p.rep;
+              reinterpret_cast<float4*>(p.o + ((static_cast<int64_t>(x.b) * p.Nq + tok) * p.H + x.hk * p.rep + q_r - tok * p.rep) * D)[piece] = v;
+            } else {
+              reinterpret_cast<float4*>(p.part_o + (part0 + row32) * D + 64 * half)[piece] = v;
+            }
+          }
+          __syncwarp();
+        }
+        // where the join finds the unit: the slot of its first piece, and the last CTA that has one (the pieces between are first ones)
+        if (r == 0 && in_tile == 0) {
+          int2* u = p.unit_slots + (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + C::kRows - 1) / C::kRows) + x.rt;
+          if (x.t0 == 0) u->x = whole ? -1 : slot;
+          if (x.t1 == x.tiles) u->y = cta;
         }
         if (limit > 0) {
           if (whole) {
             p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.Nq + i_tok] = (m + log2f(l)) * kLn2;
             if (p.row_ml != nullptr) p.row_ml[(static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * p.Nq * p.rep + row] = make_float2(m, 1.f / l);
           } else {
-            p.part_ml[part] = make_float2(m, l);
+            p.part_ml[part0 + lane] = make_float2(m, l);
           }
         }
         tc_fence_before();
-        slot = 2 * blockIdx.x + 1;
+        slot = 2 * cta + 1;
       } while (next_chunk(p, x, f_end));
       if (!ok && lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
     }
@@ -564,36 +637,23 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// Rows of units that were cut, and rows that see nothing: one CTA per 32 rows of a (sequence, head), a warp a row at a time.
+// Rows of units that were cut, and rows that see nothing: one CTA per 8 rows of a (sequence, head), a warp a row at a time.
 __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnParams p) {
   constexpr int D = ChunkCfg::D;
-  __shared__ int cum[136];
   grid_dep_wait();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int R = p.Nq * p.rep, groups = (R + 31) / 32;
-  const int r0 = static_cast<int>(blockIdx.x % groups) * 32, hk = static_cast<int>(blockIdx.x / groups % p.c.Hk), b = static_cast<int>(blockIdx.x / groups / p.c.Hk);
-  const int chunk = chunk_range(p, cum, tid);
-  __syncthreads();
-  const int total = cum[128], grid = p.grid;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int R = p.Nq * p.rep, groups = (R + 7) / 8, unit_tiles_max = (R + ChunkCfg::kRows - 1) / ChunkCfg::kRows;
+  const int r0 = static_cast<int>(blockIdx.x % groups) * 8, bh = static_cast<int>(blockIdx.x / groups), hk = bh % p.c.Hk, b = bh / p.c.Hk;
+  const int2 unit = p.unit_slots[static_cast<int64_t>(bh) * unit_tiles_max + r0 / ChunkCfg::kRows];
   const ChunkSeq s = chunk_seq(p, b);
-  int c0 = 0, c1 = 0, f0 = 0;
-  if (r0 < s.count * p.rep) {
-    f0 = cum[b / chunk];
-    for (int k = b / chunk * chunk; k < b; ++k) f0 += head_steps(p, k) * p.c.Hk;
-    f0 += hk * head_steps(p, b);
-    const int rt = r0 / ChunkCfg::kRows;
-    for (int k = 0; k < rt; ++k) f0 += unit_steps(p, s, k);
-    const int steps = unit_steps(p, s, rt);
-    if (steps > 0) {
-      c0 = share_owner(f0 + kChunkCost, grid, total);
-      c1 = share_owner(f0 + steps - 1, grid, total);
-    }
-  }
-  for (int r = r0 + warp; r < min(R, r0 + 32); r += 4) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = r0 + warp + 4 * k;
+    if (r >= R) break;
     const int i_tok = r / p.rep, head = hk * p.rep + r - i_tok * p.rep;
     __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(b) * p.Nq + i_tok) * p.H + head) * D) + 2 * lane;
     float* lse = p.lse + (static_cast<int64_t>(b) * p.H + head) * p.Nq + i_tok;
-    float2* row_ml = p.row_ml == nullptr ? nullptr : p.row_ml + (static_cast<int64_t>(b) * p.c.Hk + hk) * R + r;
+    float2* row_ml = p.row_ml == nullptr ? nullptr : p.row_ml + static_cast<int64_t>(bh) * R + r;
     if (row_limit(p, s, r) == 0) {
       o[0] = o[1] = __floats2bfloat162_rn(0.f, 0.f);
       if (lane == 0) {
@@ -602,16 +662,14 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
       }
       continue;
     }
-    if (c0 == c1) continue;                                   // whole: written by its CTA
+    if (unit.x < 0) continue;                                 // whole: written by its CTA
     float top = -CUDART_INF_F, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = c0; c <= c1; ++c) {
-      const int start = share_start(c, grid, total);
-      if (start == share_start(c + 1, grid, total)) continue;
-      const int64_t at = static_cast<int64_t>(2 * c + (start >= f0 ? 0 : 1)) * ChunkCfg::kRows + (r & (ChunkCfg::kRows - 1));
+    for (int c = unit.x / 2; c <= unit.y; ++c) {
+      const int64_t at = static_cast<int64_t>(c == unit.x / 2 ? unit.x : 2 * c) * ChunkCfg::kRows + (r & (ChunkCfg::kRows - 1));
       const float2 ml = p.part_ml[at];
-      if (ml.x == -CUDART_INF_F) continue;
       const float4 v = reinterpret_cast<const float4*>(p.part_o + at * D)[lane];
+      if (ml.x == -CUDART_INF_F) continue;                    // a piece of which the row sees nothing
       const float top_new = fmaxf(top, ml.x), a = exp2f(top - top_new), w = exp2f(ml.x - top_new);
       sum = sum * a + ml.y * w;
       acc = make_float4(acc.x * a + v.x * w, acc.y * a + v.y * w, acc.z * a + v.z * w, acc.w * a + v.w * w);
@@ -649,7 +707,7 @@ cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, con
   const cudaError_t e = launch_chained(cache_chunk_kernel, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, p);
   if (e != cudaSuccess) return e;
   count_launch();
-  const int groups = (p.Nq * p.rep + 31) / 32;
+  const int groups = (p.Nq * p.rep + 7) / 8;
   return launch_chained(cache_chunk_join_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * groups), 128, 0, stream, p);
 }
 

@@ -2,8 +2,8 @@
 //
 // A unit is (sequence, kv head, tile of query rows); it costs as many steps as its sequence holds blocks of 32 tokens, and kUnitCost more for
 // its queries and its output.  The steps of all units, in order, are one flat range; warp w of G takes steps [w total / G, (w + 1) total / G),
-// whatever the lengths are.  So a unit may be cut between warps: a cut leaves a partial result in a slot of its warp (2 w for the warp's
-// first piece, else 2 w + 1), which cache_join_kernel joins.  The division depends on the lengths and the grid alone: the same call gives
+// whatever the lengths are (G: the grid's warps, or as many as there are steps).  So a unit may be cut between warps: a cut leaves a partial
+// result in a slot of its warp (2 w for the warp's first piece, else 2 w + 1), which cache_join_kernel joins.  The division depends on the lengths and the grid alone: the same call gives
 // the same bits.
 #pragma once
 #include "dm_cache.cuh"
@@ -42,18 +42,6 @@ __device__ __forceinline__ FlatRange flat_range(const CacheView& c, int units, i
 __device__ __forceinline__ int range_start(int w, int workers, int total) {
   return static_cast<int>(static_cast<int64_t>(w) * total / workers);
 }
-// The warp that takes step f: the largest w with w total / G <= f.
-__device__ __forceinline__ int range_owner(int f, int workers, int total) {
-  return static_cast<int>(((static_cast<int64_t>(f) + 1) * workers - 1) / total);
-}
-// Steps before sequence b.
-__device__ __forceinline__ int steps_before(const CacheView& c, int units, const FlatRange& r, int b) {
-  const int i = b / r.chunk;
-  int f = r.cum[i];
-  for (int k = i * r.chunk; k < b; ++k) f += sequence_steps(cache_length(c, k), units);
-  return f;
-}
-
 // A warp's piece of a unit.
 struct Piece {
   int b, unit, n, blocks;         // sequence, unit within it, its length and blocks
