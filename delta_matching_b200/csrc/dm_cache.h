@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -48,6 +49,9 @@ struct CacheAttnParams {
   float* lse;                       // (B, H, Nq)
   float* part_o;                    // partial results: 2 slots a warp of (row tile, D) fp32, and their (maximum, sum) pairs
   float2* part_ml;
+  __half* q16;                      // many rows: the queries in f16 and the order of the row tiles, and the factors of their logits
+  float* factors;
+  void* starts;                     // and what each CTA begins with
   int2* unit_slots;                 // per unit (B, Hk, row tiles): slot of its first piece (-1: whole), the last worker that has one
   float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null
   float* weights;                   // (B, Hk, W) or null
@@ -76,15 +80,19 @@ struct CacheAttnPlan {
   int row_tile;                     // query rows (new tokens x heads of a group) a CTA keeps
   int row_tiles;
   int grid;
-  int64_t part_o_bytes, part_ml_bytes, unit_bytes, row_ml_bytes;
+  int64_t part_o_bytes, part_ml_bytes, q16_bytes, factor_bytes, start_bytes, unit_bytes, row_ml_bytes;
+  int64_t bytes() const { return part_o_bytes + part_ml_bytes + q16_bytes + factor_bytes + start_bytes + unit_bytes + row_ml_bytes; }
 };
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights);
 
 cudaError_t launch_cache_append(int D, const CacheAppendParams& p, cudaStream_t stream);
-cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, cudaStream_t stream);
+// tq: p.q16 as 64 x 128 boxes, for the form for many rows.
+cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream);
 // The form for many rows (its partial results: 2 slots a CTA), and what a row tile of it holds.
-cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, cudaStream_t stream);
+cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream);
 int cache_chunk_rows();
+int64_t cache_chunk_start_bytes();                           // of a CTA's start
+int64_t cache_chunk_query_rows(int B, int Hk, int R);         // rows of 128 f16 values
 cudaError_t launch_cache_evict(int D, const CacheEvictParams& p, cudaStream_t stream);
 
 }  // namespace dm

@@ -108,7 +108,7 @@ static int check_attn_shape(int B, int Nq, int H, int Hk, int D, int T, int page
 int64_t dm_cache_attn_workspace_bytes(int B, int Nq, int H, int Hk, int D, int T, int page_size, int with_weights) {
   if (check_attn_shape(B, Nq, H, Hk, D, T, page_size) != 0) return 0;
   const dm::CacheAttnPlan x = dm::plan_cache_attn(B, Nq, H, Hk, D, T, page_size, with_weights != 0);
-  return x.part_o_bytes + x.part_ml_bytes + x.unit_bytes + x.row_ml_bytes;
+  return x.bytes();
 }
 
 int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, int B, int Nq, int H,
@@ -124,7 +124,7 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   if (weights != nullptr && W < T * cache->page_size)
     return fail(DM_ERR_ARG, "delta_matching: weights must have room for the %d tokens of a row of the block table (got %d)", T * cache->page_size, W);
   const dm::CacheAttnPlan x = dm::plan_cache_attn(B, Nq, H, cache->heads, cache->head_dim, T, cache->page_size, weights != nullptr);
-  const int64_t need = x.part_o_bytes + x.part_ml_bytes + x.unit_bytes + x.row_ml_bytes;
+  const int64_t need = x.bytes();
   if (workspace_bytes < need)
     return fail(DM_ERR_ARG, "delta_matching: workspace of %lld bytes given, %lld needed", static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   DM_TRY(check_sm100());
@@ -139,17 +139,30 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   p.o = static_cast<__nv_bfloat16*>(o);
   p.lse = lse;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(ws + x.part_o_bytes);
-  p.unit_slots = reinterpret_cast<int2*>(ws + x.part_o_bytes + x.part_ml_bytes);
-  p.row_ml = weights != nullptr ? reinterpret_cast<float2*>(ws + x.part_o_bytes + x.part_ml_bytes + x.unit_bytes) : nullptr;
+  auto take = [&ws](int64_t bytes) {                          // every part is a multiple of 8 bytes, the first ones of 16
+    uint8_t* at = ws;
+    ws += bytes;
+    return at;
+  };
+  p.part_o = reinterpret_cast<float*>(take(x.part_o_bytes));
+  p.q16 = reinterpret_cast<__half*>(take(x.q16_bytes));
+  p.part_ml = reinterpret_cast<float2*>(take(x.part_ml_bytes));
+  p.factors = reinterpret_cast<float*>(take(x.factor_bytes));
+  p.starts = take(x.start_bytes);
+  p.unit_slots = reinterpret_cast<int2*>(take(x.unit_bytes));
+  p.row_ml = weights != nullptr ? reinterpret_cast<float2*>(take(x.row_ml_bytes)) : nullptr;
   p.weights = weights;
   p.w_sb = w_sb; p.w_sh = w_sh; p.W = W; p.accumulate = accumulate ? 1 : 0;
   p.grid = x.grid;
-  CUtensorMap tk, tv;
+  CUtensorMap tk, tv, tq{};
   DM_TRY(pool_map(&tk, cache, cache->k8));
   DM_TRY(pool_map(&tv, cache, cache->v8));
-  const cudaError_t e = dm::launch_cache_attn(cache->head_dim, tk, tv, p, static_cast<cudaStream_t>(stream));
+  if (x.chunk) {                                              // f16 rows as bytes: boxes of 64 values x 128 rows
+    const cuuint64_t dims[2] = {256, static_cast<cuuint64_t>(x.q16_bytes / 256)}, strides[1] = {256};
+    const cuuint32_t box[2] = {128, 128};
+    DM_TRY(encode_byte_map(&tq, p.q16, 2, dims, strides, box));
+  }
+  const cudaError_t e = dm::launch_cache_attn(cache->head_dim, tk, tv, tq, p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : cuda_fail(e, "cache attention launch");
 }
 

@@ -620,16 +620,20 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   const int64_t slots = 2ll * x.grid * (x.chunk ? 1 : 4);
   x.part_o_bytes = slots * x.row_tile * D * 4;
   x.part_ml_bytes = slots * x.row_tile * 8;
+  const int64_t q_rows = x.chunk ? cache_chunk_query_rows(B, Hk, R) : 0;
+  x.q16_bytes = q_rows * D * 2;
+  x.factor_bytes = q_rows * 4;
+  x.start_bytes = x.chunk ? x.grid * cache_chunk_start_bytes() : 0;
   x.unit_bytes = static_cast<int64_t>(B) * Hk * x.row_tiles * 8;
   x.row_ml_bytes = weights ? static_cast<int64_t>(B) * Hk * R * 8 : 0;
   return x;
 }
 
-cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, cudaStream_t stream) {
+cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
   const int R = p.Nq * p.rep, tile = small_row_tile(D, R), row_tiles = (R + tile - 1) / tile;
   cudaError_t e;
   if (D == 128) {
-    e = R >= kChunkFrom ? launch_cache_chunk(tk, tv, p, stream)
+    e = R >= kChunkFrom ? launch_cache_chunk(tk, tv, tq, p, stream)
       : tile == 8 ? launch_main<128, 1>(tk, tv, p, row_tiles, stream)
       : tile == 16 ? launch_main<128, 2>(tk, tv, p, row_tiles, stream) : launch_main<128, 4>(tk, tv, p, row_tiles, stream);
   } else {

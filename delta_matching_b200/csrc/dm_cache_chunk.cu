@@ -7,8 +7,8 @@
 // A unit is (sequence, kv head, 256 rows); rows are (new token, head of the group).  The key tiles of 128 tokens of all units are one flat
 // range, divided evenly over one CTA per SM (as the warps' blocks are in dm_cache_sched.cuh); pieces of cut units are joined by a second kernel.
 // Warps 0-3 and 4-7: softmax of the unit's two row tiles (thread = row = TMEM lane).  Warps 8-11: codes -> f16 operand tiles in shared
-// memory, shared by both row tiles.  Warp 12: TMA of the code tiles from the pages.  Warp 13: MMA.  The two row tiles take turns: while
-// one is in its softmax the tensor cores work for the other.
+// memory, shared by both row tiles.  Warp 12: TMA of the code tiles from the pages.  Warp 13: MMA.  Warp 14: TMA of the
+// queries, which a small kernel has brought to f16 in the order of the row tiles.  The two row tiles take turns: while one is in its softmax the tensor cores work for the other.
 //
 // TMEM: S0 0-127, S1 128-255 (P of a tile over the first 64 columns of its S), O0 256-383, O1 384-511.
 // The reference moves only when a row exceeds it by more than 2^3.9 (P then still fits f16's range), so O is seldom rescaled: a move costs its
@@ -21,25 +21,26 @@ namespace dm {
 
 namespace {
 
-constexpr int kChunkCost = 2;               // key tiles that a unit's queries and output are worth
+constexpr int kChunkCost = 3;               // key tiles that a unit's queries and output are worth
 constexpr int kPBase = 12;                  // log2 of P at the reference maximum,
 constexpr float kHeadroom = 3.9f;           // and what a row may exceed it by: P stays below 2^16
 
 struct ChunkCfg {
   static constexpr int D = 128;
-  static constexpr int kThreads = 512;                        // four warpgroups, the last two of its warps idle
+  static constexpr int kThreads = 512;                        // four warpgroups
   static constexpr int kRegsSoftmax = 168, kRegsOther = 88;
   static_assert(256 * kRegsSoftmax + 256 * kRegsOther <= kThreads * 128, "a split above the launch's own registers would wait for ever");
   static constexpr int kRows = 256;
   static constexpr int kTile = 128 * 128;                     // a code tile; also a 64-column f16 panel of 128 rows
   static constexpr int kSmemQ = 0;                            // two row tiles x two panels
-  static constexpr int kSmemK = 4 * kTile;                    // two buffers x two panels
-  static constexpr int kSmemV = kSmemK + 4 * kTile;
+  static constexpr int kSmemK = 4 * kTile;                    // two panels: between the uses of two tiles lies a softmax, longer than a conversion
+  static constexpr int kSmemV = kSmemK + 2 * kTile;           // two buffers x two panels
   static constexpr int kSmemCode = kSmemV + 4 * kTile;        // K codes, V codes
-  static constexpr int kSmemBars = kSmemCode + 2 * kTile;
+  static constexpr int kSmemOut = kSmemCode + 2 * kTile;      // output staging: 4 KB a softmax warp
+  static constexpr int kSmemBars = kSmemOut + 2 * kTile;
   static constexpr int kSmemScales = kSmemBars + 256;         // 8 tiles x (4 K scales, 4 V scales)
-  static constexpr int kSmemCum = kSmemScales + 8 * 32;
-  static constexpr int kSmem = kSmemCum + 136 * 4 + 64 + 1024;
+  static constexpr int kSmem = kSmemScales + 8 * 32 + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 // ------------------------------------------------------------------------------------------------ schedule
@@ -147,6 +148,27 @@ __device__ __forceinline__ bool next_chunk(const CacheAttnParams& p, ChunkPiece&
   return true;
 }
 
+// What a CTA begins with: made once per call by the queries' kernel (8000 cycles in each CTA of the main kernel otherwise).
+struct ChunkStart {
+  ChunkPiece x;
+  int f0, f_end;
+};
+__device__ __forceinline__ void chunk_starts(const CacheAttnParams& p, int* cum) {
+  const int tid = threadIdx.x, chunk = (p.c.B + 127) / 128;
+  if (tid < 128) chunk_range(p, cum, tid);
+  __syncthreads();
+  const int total = cum[128], sharers = min(p.grid, total);   // each has a step at least
+  for (int c = tid; c < p.grid; c += blockDim.x) {
+    ChunkStart s{};
+    if (c < sharers) {
+      s.f0 = share_start(c, sharers, total);
+      s.f_end = share_start(c + 1, sharers, total);
+      s.x = first_chunk(p, cum, chunk, s.f0, s.f_end);
+    }
+    reinterpret_cast<ChunkStart*>(p.starts)[c] = s;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ instructions
 // kind::f16, f16 operands, fp32 accumulator: the descriptor's fields are those of kind::f8f6f4 with type code 0.
 __device__ __forceinline__ void mma_h_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool acc) {
@@ -174,15 +196,49 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 
 enum ChunkBar : int {
   kCodeFull = 0, kCodeEmpty = 2,            // K codes, V codes
-  kKFull = 4, kKEmpty = 6, kVFull = 8, kVEmpty = 10,          // by parity of the running tile
-  kQFull = 12, kSFull = 14, kPFull = 16, kPvDone = 18,        // by row tile
-  kScales = 20,                             // of running tile g: entry g % 8 (the loads are at most four tiles ahead of the softmax)
-  kBars = 28,
+  kKFull = 4, kKEmpty = 5,
+  kVFull = 6, kVEmpty = 8,                  // by parity of the running tile
+  kQFull = 10, kQFree = 12, kSFull = 14, kPHalf = 16, kPFull = 18, kPvDone = 20,      // by row tile
+  kScales = 22,                             // of running tile g: entry g % 8 (the loads are at most four tiles ahead of the softmax)
+  kBars = 30,
 };
+
+// ------------------------------------------------------------------------------------------------ queries
+// q (bf16, any strides) -> f16 rows with a power of two per row, in the order of the row tiles (b, kv head, new token, head of the group; rows
+// of a head filled up to whole tiles with zeros), and the factor of each row's logits.  Sixteen lanes a row.  In the main kernel this took
+// its softmax warps 7000 cycles a unit, and a warp of its own 40000 and more.  The first CTA makes the division of the tiles instead.
+__global__ void __launch_bounds__(256) cache_chunk_queries_kernel(const CacheAttnParams p) {
+  __shared__ int cum[136];
+  grid_dep_wait();
+  if (blockIdx.x == 0) {
+    chunk_starts(p, cum);
+    return;
+  }
+  const int lane = threadIdx.x & 15, R = p.Nq * p.rep, padded = (R + 127) / 128 * 128;
+  const int64_t row = static_cast<int64_t>(blockIdx.x - 1) * 16 + (threadIdx.x >> 4);       // the grid is whole tiles
+  const int bh = static_cast<int>(row / padded), r = static_cast<int>(row - static_cast<int64_t>(bh) * padded), b = bh / p.c.Hk, hk = bh - b * p.c.Hk;
+  const int tok = r / p.rep, head = hk * p.rep + r - tok * p.rep;
+  uint4 w = make_uint4(0, 0, 0, 0);
+  if (r < R) w = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + tok * p.q_sn + head * p.q_sh) + lane);
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) amax = max3(amax, fabsf(__uint_as_float(v[j] << 16)), fabsf(__uint_as_float(v[j] & 0xFFFF0000u)));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const uint32_t eb = min(254u, max(14u, __float_as_uint(amax) >> 23));
+  const float up = sb_to_scale(267u - eb);                    // largest element to [2^13, 2^14)
+  uint32_t h[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = pack_f16x2(__uint_as_float(v[j] << 16) * up, __uint_as_float(v[j] & 0xFFFF0000u) * up);
+  reinterpret_cast<uint4*>(p.q16 + row * ChunkCfg::D)[lane] = make_uint4(h[0], h[1], h[2], h[3]);
+  if (lane == 0) p.factors[row] = sb_to_scale(eb - 13u) * p.scale * kLog2e;
+}
 
 // ------------------------------------------------------------------------------------------------ main kernel
 __global__ void __launch_bounds__(ChunkCfg::kThreads, 1)
-cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const CacheAttnParams p) {
+cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tq,
+                   const CacheAttnParams p) {
   using C = ChunkCfg;
   constexpr int D = C::D;
   extern __shared__ uint8_t smem_raw[];
@@ -193,27 +249,29 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kBars + 1);
   float* scales = reinterpret_cast<float*>(smem + C::kSmemScales);
-  int* cum = reinterpret_cast<int*>(smem + C::kSmemCum);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bars + kCodeFull + i, 1);
       mbar_init(bars + kCodeEmpty + i, 4);
-      mbar_init(bars + kKFull + i, 4);
-      mbar_init(bars + kKEmpty + i, 1);
       mbar_init(bars + kVFull + i, 4);
       mbar_init(bars + kVEmpty + i, 1);
-      mbar_init(bars + kQFull + i, 4);
+      mbar_init(bars + kQFull + i, 1);
+      mbar_init(bars + kQFree + i, 1);
       mbar_init(bars + kSFull + i, 1);
+      mbar_init(bars + kPHalf + i, 4);
       mbar_init(bars + kPFull + i, 4);
       mbar_init(bars + kPvDone + i, 1);
     }
+    mbar_init(bars + kKFull, 4);
+    mbar_init(bars + kKEmpty, 1);
     for (int i = 0; i < 8; ++i) mbar_init(bars + kScales + i, 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
+    tma_prefetch_desc(&tq);
   }
   if (warp == 13) {
     tmem_alloc(tmem_slot, 512);
@@ -221,20 +279,17 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     tc_fence_before();
   }
   grid_dep_wait();
-  const int chunk = (p.c.B + 127) / 128;
-  if (tid < 128) chunk_range(p, cum, tid);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int total = cum[128];
-  const int sharers = min(p.grid, total);                     // each has a step at least
   const int cta = blockIdx.x;
-  const int f0 = cta < sharers ? share_start(cta, sharers, total) : 0, f_end = cta < sharers ? share_start(cta + 1, sharers, total) : 0;
+  const ChunkStart start = reinterpret_cast<const ChunkStart*>(p.starts)[cta];
+  const int f_end = start.f_end;
   bool ok = true;
   auto bar = [&](int i) { return smem_u32(bars + i); };
 
-  if (f0 < f_end) {
-    ChunkPiece x = first_chunk(p, cum, chunk, f0, f_end);
+  if (start.f0 < f_end) {
+    ChunkPiece x = start.x;
     if (warp >= 12) {
       reg_dec<C::kRegsOther>();
     }
@@ -313,45 +368,75 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         // V's panels of 64 columns lie kTile apart: the leading offset of an operand wider than 128 bytes
         const uint32_t v_lo = (((sbase + C::kSmemV) & 0x3FFFFu) >> 4) | (static_cast<uint32_t>(C::kTile >> 4) << 16);
         int g = 0, tiles[2] = {0, 0}, units[2] = {0, 0};      // running tile; tiles and units of each row tile
-        auto issue_s = [&](int r, int gi, bool last) {
-          const uint32_t a = q_lo + r * (2 * C::kTile >> 4), b = k_lo + (gi & 1) * (2 * C::kTile >> 4);
+        auto issue_s = [&](int r, bool last) {
+          const uint32_t a = q_lo + r * (2 * C::kTile >> 4), b = k_lo;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t off = (k >> 2) * (C::kTile >> 4) + (k & 3) * 2;
             mma_h_ss(tmem + 128 * r, a + off, b + off, kIdescS, k > 0);
           }
-          if (last) tc_commit(bars + kKEmpty + (gi & 1));
+          if (last) tc_commit(bars + kKEmpty);
           tc_commit(bars + kSFull + r);
         };
         do {
           if (x.t0 >= x.t1) continue;
           const int nr = x.row_tiles(p);
-          ok = wait_or_abort(bar(kKFull + (g & 1)), (g >> 1) & 1, abort_flag);
+          ok = wait_or_abort(bar(kKFull), g & 1, abort_flag);
           for (int r = 0; r < nr && ok; ++r) {
             if (!(ok = wait_or_abort(bar(kQFull + r), units[r]++ & 1, abort_flag))) break;
             tc_fence_after();
-            issue_s(r, g, r == nr - 1);
+            issue_s(r, r == nr - 1);
+            if (x.t0 + 1 == x.t1) tc_commit(bars + kQFree + r);
           }
           for (int t = x.t0; t < x.t1 && ok; ++t, ++g) {
-            const uint32_t v = v_lo + (g & 1) * (2 * C::kTile >> 4);
             for (int r = 0; r < nr; ++r) {
-              if (!(ok = wait_or_abort(bar(kPFull + r), tiles[r]++ & 1, abort_flag))) break;
-              if (r == 0 && !(ok = wait_or_abort(bar(kVFull + (g & 1)), (g >> 1) & 1, abort_flag))) break;
-              tc_fence_after();
+              // 16 keys a step: 8 columns of P, 16 rows of V; the first half of the keys while the softmax is at the second
 #pragma unroll
-              for (int k = 0; k < 8; ++k)                     // 16 keys: 8 columns of P, 16 rows of V
-                mma_h_ts(tmem + 256 + 128 * r, tmem + 128 * r + 8 * k, v + k * (2048 >> 4), kIdescO, t > x.t0 || k > 0);
+              for (int half = 0; half < 2; ++half) {
+                if (!(ok = wait_or_abort(bar((half == 0 ? kPHalf : kPFull) + r), tiles[r] & 1, abort_flag))) break;
+                if (r == 0 && half == 0 && !(ok = wait_or_abort(bar(kVFull + (g & 1)), (g >> 1) & 1, abort_flag))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 4 * half; k < 4 * half + 4; ++k)
+                  mma_h_ts(tmem + 256 + 128 * r, tmem + 128 * r + 8 * k, v_lo + (g & 1) * (2 * C::kTile >> 4) + k * (2048 >> 4), kIdescO, t > x.t0 || k > 0);
+              }
+              if (!ok) break;
+              ++tiles[r];
               if (r == nr - 1) tc_commit(bars + kVEmpty + (g & 1));
               tc_commit(bars + kPvDone + r);
               if (t + 1 < x.t1) {
-                if (r == 0 && !(ok = wait_or_abort(bar(kKFull + ((g + 1) & 1)), ((g + 1) >> 1) & 1, abort_flag))) break;
+                if (r == 0 && !(ok = wait_or_abort(bar(kKFull), (g + 1) & 1, abort_flag))) break;
                 tc_fence_after();
-                issue_s(r, g + 1, r == nr - 1);
+                issue_s(r, r == nr - 1);
+                if (t + 2 == x.t1) tc_commit(bars + kQFree + r);      // the unit's last S
               }
             }
           }
         } while (ok && next_chunk(p, x, f_end));
         if (!ok) raise_abort(abort_flag, p.c.status, kStatusTimeoutMma + kInCache);
+      }
+    } else if (warp == 14) {
+      // ---------------------------------------------------------------------------------------- queries of the next unit
+      if (elect_one()) {
+        int units[2] = {0, 0};
+        const int tiles_of_head = (p.Nq * p.rep + 127) / 128;
+        do {
+          if (x.t0 >= x.t1) continue;
+          for (int r = 0; r < x.row_tiles(p) && ok; ++r) {
+            if (units[r] > 0) ok = wait_or_abort(bar(kQFree + r), (units[r] - 1) & 1, abort_flag);
+            if (!ok) break;
+            ++units[r];
+            mbar_expect_tx(bars + kQFull + r, 2 * C::kTile);
+            const int row = ((x.b * p.c.Hk + x.hk) * tiles_of_head + 2 * x.rt + r) * 128;
+            for (int panel = 0; panel < 2; ++panel)
+              tma_load_2d(smem + C::kSmemQ + (2 * r + panel) * C::kTile, &tq, bars + kQFull + r, 128 * panel, row);        // x in bytes
+          }
+        } while (ok && next_chunk(p, x, f_end));
+        if (!ok) {
+          raise_abort(abort_flag, p.c.status, kStatusTimeoutProducer + kInCache);
+          for (int r = 0; r < 2; ++r)                         // what is in flight lands before the shared memory goes
+            if (units[r] > 0) wait_or_abort(bar(kQFull + r), (units[r] - 1) & 1, abort_flag);
+        }
       }
     } else if (warp >= 8 && warp < 12) {
       reg_dec<C::kRegsOther>();
@@ -365,10 +450,11 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 #pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
             ok = wait_warp(bar(kCodeFull + kv), g & 1, abort_flag);
-            if (ok && g >= 2) ok = wait_warp(bar((kv ? kVEmpty : kKEmpty) + (g & 1)), ((g >> 1) - 1) & 1, abort_flag);
+            if (ok && kv == 0 && g >= 1) ok = wait_warp(bar(kKEmpty), (g - 1) & 1, abort_flag);
+            if (ok && kv == 1 && g >= 2) ok = wait_warp(bar(kVEmpty + (g & 1)), ((g >> 1) - 1) & 1, abort_flag);
             if (!ok) break;
             const uint32_t src = sbase + C::kSmemCode + kv * C::kTile;
-            const uint32_t dst = sbase + (kv ? C::kSmemV : C::kSmemK) + (g & 1) * 2 * C::kTile + panel * C::kTile;
+            const uint32_t dst = sbase + (kv ? C::kSmemV + (g & 1) * 2 * C::kTile : C::kSmemK) + panel * C::kTile;
             const int held = kv ? x.s.n - 128 * t : 128;      // V's slots beyond the length hold anything, NaN codes too: zeros
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -396,7 +482,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              mbar_arrive(bars + (kv ? kVFull : kKFull) + (g & 1));
+              mbar_arrive(bars + (kv ? kVFull + (g & 1) : kKFull));
               mbar_arrive(bars + kCodeEmpty + kv);
             }
           }
@@ -409,9 +495,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const int r = warp >> 2, in_tile = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t t_s = tmem + lanes + 128 * r, t_o = tmem + lanes + 256 + 128 * r;
-      // the warp's own 32 rows of the query tile's two panels: 8 KB for its output on the way out
-      const uint32_t stage = sbase + C::kSmemQ + r * 2 * C::kTile + (warp & 3) * 4096;
-      int g = 0, mine = 0;                                    // running tile, those of this row tile
+      const uint32_t stage = sbase + C::kSmemOut + warp * 4096;
+      int g = 0, mine = 0;                                    // running tile; tiles of this row tile
       int slot = 2 * cta;
       do {
         if (x.t0 >= x.t1) continue;
@@ -422,45 +507,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         const int row = x.rt * C::kRows + r * 128 + in_tile, limit = row_limit(p, x.s, row);
         const int i_tok = row / p.rep, head = x.hk * p.rep + row - i_tok * p.rep;
-        // The warp's 32 query rows, sixteen lanes a row: to f16 with a power of two per row, into the operand tile.
-        float f;                                              // factor of the row's logits, K's scale aside
-        {
-          const int c16 = lane & 15;
-          uint32_t my_eb = 0;
-#pragma unroll 1
-          for (int i0 = 0; i0 < 16; i0 += 8) {
-            uint4 w[8];
-            int tr = (warp & 3) * 32 + 2 * i0 + (lane >> 4);  // row of the tile
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int q_r = x.rt * C::kRows + r * 128 + tr + 2 * i, tok = q_r / p.rep;
-              w[i] = make_uint4(0, 0, 0, 0);
-              if (tok < x.s.count) w[i] = __ldg(reinterpret_cast<const uint4*>(p.q + x.b * p.q_sb + tok * p.q_sn + (x.hk * p.rep + q_r - tok * p.rep) * p.q_sh) + c16);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i, tr += 2) {
-              const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-              float amax = 0.f;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) amax = max3(amax, fabsf(__uint_as_float(v[j] << 16)), fabsf(__uint_as_float(v[j] & 0xFFFF0000u)));
-#pragma unroll
-              for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-              const uint32_t eb = min(254u, max(14u, __float_as_uint(amax) >> 23));
-              const float up = sb_to_scale(267u - eb);        // largest element to [2^13, 2^14)
-              uint32_t h[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) h[j] = pack_f16x2(__uint_as_float(v[j] << 16) * up, __uint_as_float(v[j] & 0xFFFF0000u) * up);
-              sts_u4(sbase + C::kSmemQ + r * 2 * C::kTile + (c16 >> 3) * C::kTile + tr * 128 + (((c16 & 7) ^ (tr & 7)) << 4), h[0], h[1], h[2], h[3]);
-              const uint32_t of_mine = __shfl_sync(0xffffffffu, eb, (lane & 1) * 16);
-              if ((lane >> 1) == i0 + i) my_eb = of_mine;
-            }
-          }
-          f = sb_to_scale(my_eb - 13u) * p.scale * kLog2e;
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kQFull + r);
-
+        // of the row's logits, K's scale aside
+        const float f = __ldg(p.factors + (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + 127) / 128 * 128) + row);
         float m = -CUDART_INF_F, l = 0.f;
         int vexp = -1000;
         // One key tile.  kCut: some row of the warp does not see all its keys (a compile-time variant: no select per element elsewhere).
@@ -539,6 +587,12 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             }
             l = fmaf(sum.x + sum.y, __uint_as_float(static_cast<uint32_t>(127 - off) << 23), l);
             tmem_st16(t_s + 16 * c, h);                       // over columns that have been read: 16 c + 15 < 32 c + 32
+            if (c == 1) {                                     // the first half of the keys: the tensor cores may begin
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bars + kPHalf + r);
+            }
           }
           tmem_wait_st();
           tc_fence_before();
@@ -560,50 +614,52 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const bool whole = x.t0 == 0 && x.t1 == x.tiles;
         const float unit_exp = exp2f(static_cast<float>(vexp - kPBase));
         const float scale = whole ? unit_exp / l : unit_exp;
-        // Through shared memory (the queries are done with), so that the lanes of a store write whole rows: a row a thread, 16 bytes at a
-        // time, took 11000 cycles a piece.  Staged: 32 rows x 256 bytes, 16-byte pieces XORed with the row.
+        // where a row that sees something goes
+        const int64_t out_row = limit == 0 ? -1 : ((static_cast<int64_t>(x.b) * p.Nq + i_tok) * p.H + head) * D;
+        // Through shared memory, so that the lanes of a store write whole rows (a row a thread, 16 bytes at a time, took 11000 cycles a piece):
+        // 32 rows x 128 bytes at a time, 16-byte pieces XORed with the row.
         const int64_t part0 = static_cast<int64_t>(slot) * C::kRows + r * 128 + (warp & 3) * 32;
-        auto staged = [&](int row32, int piece) { return stage + (piece >> 3) * C::kTile + row32 * 128 + (((piece & 7) ^ (row32 & 7)) << 4); };
 #pragma unroll 1
-        for (int half = 0; half < (whole ? 1 : 2); ++half) {
-#pragma unroll 1
-          for (int c = whole ? 0 : 2 * half; c < (whole ? 4 : 2 * half + 2); ++c) {
-            uint32_t o[32];
-            tmem_ld32(t_o + 32 * c, o);
-            tmem_wait_ld();
-            float v[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + 32 * c, o);
+          tmem_wait_ld();
+          if (whole) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * scale;
-            if (whole) {
+            for (int e = 0; e < 4; ++e) {
+              uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[8 * e + 2 * j], v[8 * e + 2 * j + 1]);
-                  w[j] = *reinterpret_cast<const uint32_t*>(&b2);
-                }
-                sts_u4(staged(lane, 4 * c + e), w[0], w[1], w[2], w[3]);
+              for (int j = 0; j < 4; ++j) {
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(__uint_as_float(o[8 * e + 2 * j]) * scale, __uint_as_float(o[8 * e + 2 * j + 1]) * scale);
+                w[j] = *reinterpret_cast<const uint32_t*>(&b2);
               }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                sts_u4(staged(lane, 8 * (c & 1) + e), __float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3]));
+              sts_u4(stage + lane * 128 + ((((4 * c + e) & 7) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
+            if ((c & 1) == 0) continue;                       // 64 columns make 128 bytes
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              sts_u4(stage + lane * 128 + ((e ^ (lane & 7)) << 4), __float_as_uint(__uint_as_float(o[4 * e]) * scale), __float_as_uint(__uint_as_float(o[4 * e + 1]) * scale),
+                     __float_as_uint(__uint_as_float(o[4 * e + 2]) * scale), __float_as_uint(__uint_as_float(o[4 * e + 3]) * scale));
           }
           __syncwarp();
-#pragma unroll 2
-          for (int i = 0; i < 16; ++i) {
-            const int row32 = 2 * i + (lane >> 4), piece = lane & 15;
-            const float4 v = lds_f4(staged(row32, piece));
-            const int row_limit32 = __shfl_sync(0xffffffffu, limit, row32);
-            if (row_limit32 == 0) continue;
-            if (whole) {
-              const int q_r = x.rt * C::kRows + r * 128 + (warp & 3) * 32 + row32, tok = q_r / p.rep;
-              reinterpret_cast<float4*>(p.o + ((static_cast<int64_t>(x.b) * p.Nq + tok) * p.H + x.hk * p.rep + q_r - tok * p.rep) * D)[piece] = v;
-            } else {
-              reinterpret_cast<float4*>(p.part_o + (part0 + row32) * D + 64 * half)[piece] = v;
+          const int piece = lane & 7;
+          float4 v[8];                                        // of rows lane / 8, + 4, ...: four rows a store, eight lanes each
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row32 = 4 * i + (lane >> 3);
+            v[i] = lds_f4(stage + row32 * 128 + ((piece ^ (row32 & 7)) << 4));
+          }
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int64_t at = __shfl_sync(0xffffffffu, out_row, 4 * i + (lane >> 3));
+              if (at >= 0) reinterpret_cast<float4*>(p.o + at + 64 * (c >> 1))[piece] = v[i];
             }
+          } else {                                            // rows that see nothing too: their slots are not read
+            float4* to = reinterpret_cast<float4*>(p.part_o + (part0 + (lane >> 3)) * D + 32 * c) + piece;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[4 * i * (D / 4)] = v[i];
           }
           __syncwarp();
         }
@@ -688,8 +744,10 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
 }  // namespace
 
 int cache_chunk_rows() { return ChunkCfg::kRows; }
+int64_t cache_chunk_start_bytes() { return (sizeof(ChunkStart) + 7) / 8 * 8; }
+int64_t cache_chunk_query_rows(int B, int Hk, int R) { return static_cast<int64_t>(B) * Hk * ((R + 127) / 128 * 128); }
 
-cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, cudaStream_t stream) {
+cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
   using C = ChunkCfg;
   static bool attr_set[64] = {};
   int dev = 0;
@@ -703,8 +761,12 @@ cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, con
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
+  const unsigned row_tiles = static_cast<unsigned>(p.c.B) * p.c.Hk * ((p.Nq * p.rep + 127) / 128);
   count_launch();
-  const cudaError_t e = launch_chained(cache_chunk_kernel, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, p);
+  cudaError_t e = launch_chained(cache_chunk_queries_kernel, dim3(row_tiles * 8 + 1), 256, 0, stream, p);
+  if (e != cudaSuccess) return e;
+  count_launch();
+  e = launch_chained(cache_chunk_kernel, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, tq, p);
   if (e != cudaSuccess) return e;
   count_launch();
   const int groups = (p.Nq * p.rep + 7) / 8;
