@@ -15,7 +15,10 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kSelThreads = 512;
-constexpr int kBins = 2048;
+constexpr int kBins = 4096;
+constexpr int kSelKeys = 40960;             // keys of a CTA's slice that shared memory holds; longer slices are read again in each pass
+constexpr int kSelSmem = kSelKeys * 4;
+constexpr int kMaxCluster = 8;
 
 // Unsigned integers that order like the weights.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -36,167 +39,277 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
   __syncthreads();                                            // the sums of the scan before have been read
   if (lane == 31) warp_sums[tid >> 5] = incl;
   __syncthreads();
-  uint32_t before = 0;
-  total = 0;
+  uint32_t sums = lane < kSelThreads / 32 ? warp_sums[lane] : 0;        // every warp scans the warps' sums
 #pragma unroll
-  for (int w = 0; w < kSelThreads / 32; ++w) {
-    if (w < (tid >> 5)) before += warp_sums[w];
-    total += warp_sums[w];
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, sums, off);
+    if (lane >= off) sums += o;
   }
-  return before + incl - v;
+  total = __shfl_sync(0xffffffffu, sums, 31);
+  const uint32_t before = __shfl_sync(0xffffffffu, sums, (tid >> 5) > 0 ? (tid >> 5) - 1 : 0);
+  return ((tid >> 5) > 0 ? before : 0) + incl - v;
 }
 
-// One cluster per (sequence, kv head), each CTA a contiguous slice of the candidates.  The k-th greatest key by three digits of 11, 11 and 10
-// bits, histograms added over the cluster; then the kept positions in order, by scans.
+// One cluster per (sequence, kv head), each CTA a contiguous slice of the candidates, whose keys it keeps in shared memory.  The k-th greatest
+// key by three digits of 12, 10 and 10 bits (the first is sign, exponent and three bits: weights of one size spread over many bins),
+// histograms added over the cluster; then the kept positions in order, by scans.  Bound by the latency of its barriers: a barrier of eight CTAs
+// takes 1200 - 3500 cycles, so of each other's histograms the CTAs read eight sums and then the eighth of the bins that matters.
 __global__ void __launch_bounds__(kSelThreads) cache_select_kernel(const CacheEvictParams p) {
+  extern __shared__ uint4 keys4[];
   __shared__ uint4 hist4[kBins / 4];
   __shared__ uint32_t warp_sums[kSelThreads / 32];
   __shared__ uint32_t found[2];
-  __shared__ uint32_t counts[2];
+  __shared__ uint32_t counts[2], eighths[8];
+  uint32_t* keys = reinterpret_cast<uint32_t*>(keys4);
   uint32_t* hist = reinterpret_cast<uint32_t*>(hist4);
-  grid_dep_wait();
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x;
-  const int row = blockIdx.x / C, b = row / p.c.Hk, hk = row % p.c.Hk;
+  const int C = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x, lane = tid & 31;
+  for (int i = tid; i < kBins / 4; i += kSelThreads) hist4[i] = make_uint4(0, 0, 0, 0);
+  if (tid < 8) eighths[tid] = 0;
+  grid_dep_wait();
+  const auto sync_all = [&]() {
+    if (C > 1) cluster.sync(); else __syncthreads();
+  };
+  const int row = blockIdx.x / C, b = row / p.c.Hk, hk = row - b * p.c.Hk;
   const int n = cache_length(p.c, b), left = min(n, p.budget);
-  const float* w = p.weights + b * p.w_sb + hk * p.w_sh;
+  const float* w_row = p.weights + b * p.w_sb + hk * p.w_sh;
   int* kept = p.kept + static_cast<int64_t>(row) * p.budget;
   const int W2 = p.T2 * p.c.page;
   float* nw = p.new_weights + static_cast<int64_t>(row) * W2;
   const int me = rank * kSelThreads + tid, all = C * kSelThreads;
-  if (hk == 0 && me == 0) p.new_lengths[b] = left;
-  for (int i = left + me; i < p.budget; i += all) kept[i] = -1;
-  for (int i = left + me; i < W2; i += all) nw[i] = 0.f;
-  if (n <= p.budget) {
-    for (int i = me; i < n; i += all) {
-      kept[i] = i;
-      nw[i] = w[i];
+  const int late = n > p.budget ? min(p.recent, p.budget) : n, k = left - late, cand = n - late;      // k of the first cand, and the late ones
+  if (k > 0) {
+    const int per = ((cand + C - 1) / C + 3) & ~3, s0 = min(cand, rank * per), len = min(cand, s0 + per) - s0;
+    const bool held = per <= kSelKeys;
+    const float* w = w_row + s0;
+    auto key_at = [&](int i) { return held ? keys[i] : weight_key(__ldg(w + i)); };
+    __syncthreads();
+
+    uint32_t prefix = 0, mask = 0, want = k;                  // the want-th greatest among the keys that agree with prefix in mask
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 20 : pass == 1 ? 10 : 0, quads = (pass == 0 ? kBins : 1024) / 4;
+      if (pass == 0) {
+        const int loads = (reinterpret_cast<uintptr_t>(w) & 15) == 0 ? len / 4 : 0;
+#pragma unroll 4
+        for (int i = tid; i < loads; i += kSelThreads) {
+          const float4 x = __ldg(reinterpret_cast<const float4*>(w) + i);
+          const uint4 key = make_uint4(weight_key(x.x), weight_key(x.y), weight_key(x.z), weight_key(x.w));
+          if (held) keys4[i] = key;
+          atomicAdd(hist + (key.x >> 20), 1u);
+          atomicAdd(hist + (key.y >> 20), 1u);
+          atomicAdd(hist + (key.z >> 20), 1u);
+          atomicAdd(hist + (key.w >> 20), 1u);
+        }
+        for (int i = 4 * loads + tid; i < len; i += kSelThreads) {
+          const uint32_t key = weight_key(__ldg(w + i));
+          if (held) keys[i] = key;
+          atomicAdd(hist + (key >> 20), 1u);
+        }
+      } else {
+        const auto take = [&](uint32_t key) {
+          if ((key & mask) == prefix) atomicAdd(hist + ((key >> shift) & 1023u), 1u);
+        };
+        const int loads = held ? len / 4 : 0;
+#pragma unroll 2
+        for (int i = tid; i < loads; i += kSelThreads) {
+          const uint4 key = keys4[i];
+          take(key.x);
+          take(key.y);
+          take(key.z);
+          take(key.w);
+        }
+        for (int i = 4 * loads + tid; i < len; i += kSelThreads) take(key_at(i));
+      }
+      __syncthreads();
+      // which eighth of the bins holds the want-th key: from the CTAs' sums
+      for (int i = tid; i < quads; i += kSelThreads) {        // a warp's quads lie in one eighth
+        const uint4 v = hist4[i];
+        const uint32_t sum = __reduce_add_sync(0xffffffffu, v.x + v.y + v.z + v.w);
+        if (lane == 0) atomicAdd(eighths + i / (quads / 8), sum);
+      }
+      sync_all();
+      if (tid < 32) {
+        const int q = lane & 7, r = lane >> 3;                // lane (r, q) adds the sums of eighth q of CTAs r and r + 4
+        uint32_t sum = 0;
+        if (C == 1) {
+          if (r == 0) sum = eighths[q];
+        } else {
+          if (r < C) sum += *cluster.map_shared_rank(eighths + q, r);
+          if (r + 4 < C) sum += *cluster.map_shared_rank(eighths + q, r + 4);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        uint32_t from = sum;                                  // keys in this eighth and the greater ones
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          const uint32_t x = __shfl_down_sync(0xffffffffu, from, o, 8);
+          if (q + o < 8) from += x;
+        }
+        const int eighth = __ffs(__ballot_sync(0xffffffffu, from - sum < want && want <= from) & 0xFFu) - 1;
+        uint32_t above = __shfl_sync(0xffffffffu, from, eighth);        // keys in this bin and the greater ones, from here on
+        // its bins over the cluster, 32 quads at a time
+        for (int i0 = 0; i0 < quads / 8; i0 += 32) {
+          const uint4* mine = hist4 + eighth * (quads / 8) + i0 + lane;
+          uint4 v[kMaxCluster];                               // all on their way together
+          v[0] = C > 1 ? *cluster.map_shared_rank(mine, 0) : *mine;
+#pragma unroll
+          for (int r2 = 1; r2 < kMaxCluster; ++r2) v[r2] = r2 < C ? *cluster.map_shared_rank(mine, r2) : make_uint4(0, 0, 0, 0);
+          uint32_t h[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int r2 = 0; r2 < kMaxCluster; ++r2) {
+            h[0] += v[r2].x; h[1] += v[r2].y; h[2] += v[r2].z; h[3] += v[r2].w;
+          }
+          const uint32_t four = h[0] + h[1] + h[2] + h[3];
+          uint32_t incl = four;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+          }
+          uint32_t at = above - (incl - four);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t greater = at - h[i];
+            if (greater < want && want <= at) {
+              found[0] = 4 * (eighth * (quads / 8) + i0 + lane) + i;
+              found[1] = greater;
+            }
+            at = greater;
+          }
+          above -= __shfl_sync(0xffffffffu, incl, 31);
+        }
+      }
+      sync_all();                                             // found is there, and nobody reads the histograms any more
+      prefix |= found[0] << shift;
+      mask |= (pass == 0 ? 4095u : 1023u) << shift;
+      want -= found[1];
+      if (pass < 2) {
+        for (int i = tid; i < 1024 / 4; i += kSelThreads) hist4[i] = make_uint4(0, 0, 0, 0);
+        if (tid < 8) eighths[tid] = 0;
+        __syncthreads();
+      }
     }
-    return;
+
+    // how many of the slices before mine are above the threshold, and equal to it
+    uint32_t gt = 0, eq = 0;
+    if (C > 1) {
+      uint32_t mine = 0, equal = 0;
+      const int loads = held ? len / 4 : 0;
+      for (int i = tid; i < loads; i += kSelThreads) {
+        const uint4 key = keys4[i];
+        mine += (key.x > prefix) + (key.y > prefix) + (key.z > prefix) + (key.w > prefix);
+        equal += (key.x == prefix) + (key.y == prefix) + (key.z == prefix) + (key.w == prefix);
+      }
+      for (int i = 4 * loads + tid; i < len; i += kSelThreads) {
+        const uint32_t key = key_at(i);
+        mine += key > prefix;
+        equal += key == prefix;
+      }
+      mine = __reduce_add_sync(0xffffffffu, mine);
+      equal = __reduce_add_sync(0xffffffffu, equal);
+      if (tid < 2) counts[tid] = 0;
+      __syncthreads();
+      if (lane == 0) {
+        atomicAdd(counts, mine);
+        atomicAdd(counts + 1, equal);
+      }
+      cluster.sync();
+      gt = __reduce_add_sync(0xffffffffu, lane < rank ? *cluster.map_shared_rank(counts, lane) : 0u);       // a lane per CTA before this one
+      eq = __reduce_add_sync(0xffffffffu, lane < rank ? *cluster.map_shared_rank(counts + 1, lane) : 0u);
+    }
+    constexpr int kTake = 8;                                  // adjacent tokens of a thread per scan
+    for (int at = 0; at < len; at += kSelThreads * kTake) {
+      const int j0 = at + tid * kTake;
+      uint32_t key[kTake], flags = 0;
+      if (held) {
+#pragma unroll
+        for (int i = 0; i < kTake; i += 4) {
+          const uint4 v = j0 + i < len ? keys4[(j0 + i) / 4] : make_uint4(0, 0, 0, 0);      // a slice's keys are whole quads
+          key[i] = v.x; key[i + 1] = v.y; key[i + 2] = v.z; key[i + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTake; ++i) key[i] = j0 + i < len ? weight_key(__ldg(w + j0 + i)) : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < kTake; ++i) {
+        const bool is_gt = j0 + i < len && key[i] > prefix, is_eq = j0 + i < len && key[i] == prefix;
+        flags |= (is_gt ? 1u : 0u) << i | (is_eq ? 1u : 0u) << (16 + i);
+      }
+      uint32_t total;
+      const uint32_t before = block_scan(__popc(flags & 0xFFFFu) | __popc(flags >> 16) << 16, warp_sums, total);
+      const uint32_t g = gt + (before & 0xFFFFu), e = eq + (before >> 16);
+      // of mine that are equal to the threshold, the first ones until there are `want`
+      uint32_t picks = flags & 0xFFFFu, equals = flags >> 16;
+      for (uint32_t room = e < want ? want - e : 0; equals != 0 && room > 0; --room) {
+        picks |= equals & -equals;
+        equals &= equals - 1;
+      }
+      // a list of the picked ones over the keys that have been read (behind the scan's barriers), written out by adjacent threads
+      uint32_t* list = held ? keys + at : keys;
+      const uint32_t first = gt + min(eq, want);
+      for (uint32_t to = g + min(e, want) - first; picks != 0; ++to) {
+        list[to] = j0 + __ffs(picks) - 1;
+        picks &= picks - 1;
+      }
+      gt += total & 0xFFFFu;
+      eq += total >> 16;
+      __syncthreads();
+      const int picked = gt + min(eq, want) - first;
+#pragma unroll 4
+      for (int i = tid; i < picked; i += kSelThreads) {
+        const int j = list[i];
+        kept[first + i] = s0 + j;
+        nw[first + i] = __ldg(w + j);
+      }
+    }
   }
-  const int late = min(p.recent, p.budget), k = p.budget - late, cand = n - late;
+  // the late ones (all, within the budget), and what lies behind
   for (int i = me; i < late; i += all) {
     kept[k + i] = cand + i;
-    nw[k + i] = w[cand + i];
+    nw[k + i] = __ldg(w_row + cand + i);
   }
-  if (k == 0) return;
-  const int per = (cand + C - 1) / C, s0 = min(cand, rank * per), s1 = min(cand, s0 + per);
-
-  uint32_t prefix = 0, mask = 0, want = k;                    // the want-th greatest among the keys that agree with prefix in mask
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const uint32_t digit = pass == 2 ? 1023u : 2047u;
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = s0 + tid; i < s1; i += kSelThreads) {
-      const uint32_t key = weight_key(w[i]);
-      if ((key & mask) == prefix) atomicAdd(hist + ((key >> shift) & digit), 1u);
-    }
-    cluster.sync();
-    uint32_t h[4] = {0, 0, 0, 0};                             // bins 4 tid ... + 3 over the cluster
-    for (int r = 0; r < C; ++r) {
-      const uint4 v = *cluster.map_shared_rank(hist4 + tid, r);
-      h[0] += v.x; h[1] += v.y; h[2] += v.z; h[3] += v.w;
-    }
-    uint32_t total;
-    const uint32_t below = block_scan(h[0] + h[1] + h[2] + h[3], warp_sums, total);
-    uint32_t above = total - below;                           // keys in this bin and the greater ones
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t greater = above - h[i];
-      if (greater < want && want <= above) {
-        found[0] = 4 * tid + i;
-        found[1] = greater;
-      }
-      above = greater;
-    }
-    cluster.sync();                                           // found is there, and nobody reads the histograms any more
-    prefix |= found[0] << shift;
-    mask |= digit << shift;
-    want -= found[1];
-    __syncthreads();
-  }
-
-  // how many of the slices before mine are above the threshold, and equal to it
-  uint32_t mine = 0, equal = 0;
-  for (int i = s0 + tid; i < s1; i += kSelThreads) {
-    const uint32_t key = weight_key(w[i]);
-    mine += key > prefix;
-    equal += key == prefix;
-  }
-  uint32_t total_mine, total_equal;
-  block_scan(mine, warp_sums, total_mine);
-  block_scan(equal, warp_sums, total_equal);
-  if (tid == 0) {
-    counts[0] = total_mine;
-    counts[1] = total_equal;
-  }
-  cluster.sync();
-  uint32_t gt = 0, eq = 0;
-  for (int r = 0; r < rank; ++r) {
-    gt += *cluster.map_shared_rank(counts, r);
-    eq += *cluster.map_shared_rank(counts + 1, r);
-  }
-  cluster.sync();                                             // a CTA's shared memory stays until all have read it
-  for (int at = s0; at < s1; at += kSelThreads * 4) {
-    uint32_t flags = 0, ngt = 0, neq = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = at + tid * 4 + i;
-      const uint32_t key = j < s1 ? weight_key(w[j]) : 0u;    // no weight has key 0
-      if (key > prefix) {
-        flags |= 1u << i;
-        ++ngt;
-      } else if (key == prefix && j < s1) {
-        flags |= 16u << i;
-        ++neq;
-      }
-    }
-    uint32_t total;
-    const uint32_t before = block_scan(ngt | neq << 16, warp_sums, total);
-    uint32_t g = gt + (before & 0xFFFFu), e = eq + (before >> 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = at + tid * 4 + i;
-      const bool is_gt = (flags >> i) & 1, is_eq = (flags >> (4 + i)) & 1;
-      if (is_gt || (is_eq && e < want)) {
-        const uint32_t to = g + min(e, want);
-        kept[to] = j;
-        nw[to] = w[j];
-      }
-      g += is_gt;
-      e += is_eq;
-    }
-    gt += total & 0xFFFFu;
-    eq += total >> 16;
-  }
+  for (int i = left + me; i < p.budget; i += all) kept[i] = -1;
+  for (int i = left + me; i < W2; i += all) nw[i] = 0.f;
+  if (hk == 0 && me == 0) p.new_lengths[b] = left;
+  if (C > 1) cluster.sync();                                  // a CTA's counts stay until all have read them
 }
 
-// Largest magnitude of four codes, NaN aside, as a code.
-__device__ __forceinline__ uint32_t max_code4(uint32_t w) {
-  w &= 0x7F7F7F7Fu;
-  return w & ~__vcmpeq4(w, 0x7F7F7F7Fu);
+// Two f16 values, as words: largest magnitudes (NaN aside), product, e4m3 codes (round to nearest even).
+__device__ __forceinline__ uint32_t h2_max_abs(uint32_t a, uint32_t b) {
+  const __half2 m = __hmax2(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t h2_scaled_codes(uint32_t a, uint32_t b, __half2 by) {
+  const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), by), y = __hmul2(*reinterpret_cast<const __half2*>(&b), by);
+  uint32_t w;
+  asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f16x2 lo, %1;\n\tcvt.rn.satfinite.e4m3x2.f16x2 hi, %2;\n\tmov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(w) : "r"(*reinterpret_cast<const uint32_t*>(&x)), "r"(*reinterpret_cast<const uint32_t*>(&y)));
+  return w;
 }
 
 // The kept tokens of a new block: one warp per (sequence, kv head, new block, K or V), rows in registers as in the append kernel.
+// Registers are held down (the f16 values of the maximum are made again for the codes): what hides the loads is many warps.
 template <int D>
-__global__ void __launch_bounds__(128) cache_move_kernel(const CacheEvictParams p, int blocks, int64_t items) {
+__global__ void __launch_bounds__(128, D == 128 ? 7 : 4) cache_move_kernel(const CacheEvictParams p, int blocks, int64_t items) {
   constexpr int kTpr = D / 16, kRpp = 32 / kTpr, kPass = 32 / kRpp;
-  grid_dep_wait();
   const CacheView& c = p.c;
   const int lane = threadIdx.x & 31;
   int64_t rest = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (rest >= items) return;
+  if (rest >= items) {
+    grid_dep_wait();
+    return;
+  }
   const bool is_v = (rest & 1) != 0;
   rest >>= 1;
   const int j = static_cast<int>(rest % blocks);
   rest /= blocks;
   const int hk = static_cast<int>(rest % c.Hk), b = static_cast<int>(rest / c.Hk);
-  const int left = min(cache_length(c, b), p.budget);
-  if (j * 32 >= left) return;
-  const int bpp = c.page / 32;
-  const int to_page = checked_page(c, __ldg(p.new_table + b * p.nt_row + j / bpp));
+  // what the caller gave, before the wait for the selection (which has itself waited for all kernels before it)
+  const int left = min(cache_length(c, b), p.budget), bpp = c.page / 32;
+  const int to_page = j * 32 < left ? checked_page(c, __ldg(p.new_table + b * p.nt_row + j / bpp)) : -1;
+  grid_dep_wait();
   if (to_page < 0) return;
   // lane r looks row r up
   const uint8_t* pool = is_v ? c.v8 : c.k8;
@@ -221,28 +334,46 @@ __global__ void __launch_bounds__(128) cache_move_kernel(const CacheEvictParams 
   float amax = 0.f;
 #pragma unroll
   for (int ps = 0; ps < kPass; ++ps) {
-    uint32_t m = __vmaxu4(__vmaxu4(max_code4(y[ps].x), max_code4(y[ps].y)), __vmaxu4(max_code4(y[ps].z), max_code4(y[ps].w)));
-    m = __vmaxu4(m, m >> 16);
-    m = max(m & 0xFFu, (m >> 8) & 0xFFu);
-    amax = fmaxf(amax, f16x2_to_float2(e4m3_lo_f16x2(m)).x * __shfl_sync(0xffffffffu, scale, r0 + ps * kRpp));
+    uint32_t m = 0;
+    const uint32_t v[4] = {y[ps].x, y[ps].y, y[ps].z, y[ps].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = h2_max_abs(m, h2_max_abs(e4m3_lo_f16x2(v[i]), e4m3_hi_f16x2(v[i])));
+    const float2 top = f16x2_to_float2(m);
+    amax = fmaxf(amax, fmaxf(top.x, top.y) * __shfl_sync(0xffffffffu, scale, r0 + ps * kRpp));
   }
   amax = warp_max(amax);
   const uint32_t sb = pow2_sb(amax, 1u);
-  const float inv = sb_to_inv(sb);
+  const float ratio = scale * sb_to_inv(sb);                  // of this lane's row
   uint8_t* to = (is_v ? c.v8 : c.k8) + to_page * c.c_page + hk * c.c_head + static_cast<int64_t>(j % bpp) * 32 * c.c_slot + c16;
+  if (__all_sync(0xffffffffu, ratio == 1.f || src < 0)) {     // all from blocks of the new scale: as they are
 #pragma unroll
-  for (int ps = 0; ps < kPass; ++ps) {
-    const int r = r0 + ps * kRpp;
-    // codes other than zero need at most 2^18; more would make zero times infinity of a zero row on a coarse scale
-    const float ratio = fminf(__shfl_sync(0xffffffffu, scale, r) * inv, 1.099511627776e12f);
-    uint4 v = y[ps];
-    if (ratio != 1.f) {
-      v.x = requant4(v.x, ratio);
-      v.y = requant4(v.y, ratio);
-      v.z = requant4(v.z, ratio);
-      v.w = requant4(v.w, ratio);
+    for (int ps = 0; ps < kPass; ++ps) *reinterpret_cast<uint4*>(to + (r0 + ps * kRpp) * c.c_slot) = y[ps];
+  } else if (__all_sync(0xffffffffu, ratio <= 32768.f)) {
+    // in f16: what its subnormals round away is far below half of e4m3's smallest step
+#pragma unroll
+    for (int ps = 0; ps < kPass; ++ps) {
+      const __half2 by = __float2half2_rn(__shfl_sync(0xffffffffu, ratio, r0 + ps * kRpp));
+      uint4 v = y[ps];
+      asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w));      // not the f16 values from above, kept in registers
+      v.x = h2_scaled_codes(e4m3_lo_f16x2(v.x), e4m3_hi_f16x2(v.x), by);
+      v.y = h2_scaled_codes(e4m3_lo_f16x2(v.y), e4m3_hi_f16x2(v.y), by);
+      v.z = h2_scaled_codes(e4m3_lo_f16x2(v.z), e4m3_hi_f16x2(v.z), by);
+      v.w = h2_scaled_codes(e4m3_lo_f16x2(v.w), e4m3_hi_f16x2(v.w), by);
+      *reinterpret_cast<uint4*>(to + (r0 + ps * kRpp) * c.c_slot) = v;
     }
-    *reinterpret_cast<uint4*>(to + r * c.c_slot) = v;
+  } else {
+#pragma unroll 1
+    for (int r = r0; r < 32; r += kRpp) {
+      // codes other than zero need at most 2^18; more would make zero times infinity of a zero row on a coarse scale
+      const float by = fminf(__shfl_sync(0xffffffffu, ratio, r), 1.099511627776e12f);
+      const int64_t at = __shfl_sync(0xffffffffu, src, r);
+      uint4 v = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(pool + at + c16)) : make_uint4(0, 0, 0, 0);
+      v.x = requant4(v.x, by);
+      v.y = requant4(v.y, by);
+      v.z = requant4(v.z, by);
+      v.w = requant4(v.w, by);
+      *reinterpret_cast<uint4*>(to + r * c.c_slot) = v;
+    }
   }
   if (lane == 0) scales[to_page * c.s_page + hk * c.s_head + j % bpp] = sb_to_scale(sb);
 }
@@ -250,10 +381,19 @@ __global__ void __launch_bounds__(128) cache_move_kernel(const CacheEvictParams 
 }  // namespace
 
 cudaError_t launch_cache_evict(int D, const CacheEvictParams& p, cudaStream_t stream) {
-  // a CTA of the cluster takes 4096 tokens or more
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(cache_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  // a CTA of the cluster takes 4096 tokens or more (clusters of 16: few are resident at a time; eight rows of 131072 tokens took 75 us against 33)
   const int64_t most = static_cast<int64_t>(p.c.T) * p.c.page;
   int C = 1;
-  while (C < 8 && most > 4096ll * C) C *= 2;
+  while (C < kMaxCluster && most > 4096ll * C) C *= 2;
+  const int64_t slice = ((most + C - 1) / C + 3) / 4 * 4;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -264,6 +404,7 @@ cudaError_t launch_cache_evict(int D, const CacheEvictParams& p, cudaStream_t st
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * C);
   cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = (slice <= kSelKeys ? slice : kSelKeys) * 4;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
