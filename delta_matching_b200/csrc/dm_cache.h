@@ -52,13 +52,15 @@ struct CacheAttnParams {
   __half* q16;                      // many rows: the queries in f16 and the order of the row tiles, and the factors of their logits
   float* factors;
   void* starts;                     // and what each CTA begins with
-  int2* unit_slots;                 // per unit (B, Hk, row tiles): slot of its first piece (-1: whole), the last worker that has one
+  int2* unit_slots;                 // per unit (B, Hk, row tiles), where its pieces are: slot of the first (-1: whole); the last worker (for the
+                                    // small form twice that, plus one where its piece lies in a slot of its own)
   float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null
   float* weights;                   // (B, Hk, W) or null
   int64_t w_sb, w_sh;
   int W;
   int accumulate;
   int grid;                         // CTAs of the main kernel
+  int cluster;                      // of a unit, or 0: the even division
 };
 
 struct CacheEvictParams {
@@ -80,6 +82,7 @@ struct CacheAttnPlan {
   int row_tile;                     // query rows (new tokens x heads of a group) a CTA keeps
   int row_tiles;
   int grid;
+  int cluster;                      // CTAs a unit, or 0: the even division
   int64_t part_o_bytes, part_ml_bytes, q16_bytes, factor_bytes, start_bytes, unit_bytes, row_ml_bytes;
   int64_t bytes() const { return part_o_bytes + part_ml_bytes + q16_bytes + factor_bytes + start_bytes + unit_bytes + row_ml_bytes; }
 };

@@ -13,12 +13,15 @@
 // its own maximum, sum and accumulator, and fills its own ring of TMA boxes (32 rows x 128 bytes, 128-byte swizzle, straight from the pages),
 // K and V of a block in turn, each refilled as soon as it has been read.  Units that one warp holds whole are written at once; the pieces
 // of the others are joined by a second kernel.
+#include <cooperative_groups.h>
 #include "dm_cache_sched.cuh"
 #include "dm_kernels.h"
 
 namespace dm {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 template <int D, int NT>
 struct AttnCfg {
@@ -28,7 +31,9 @@ struct AttnCfg {
   static constexpr int kCtasPerSm = D == 128 && NT == 1 ? 3 : NT == 4 ? 2 : 2;
   static constexpr int kSlots = D == 128 ? (NT == 1 ? 4 : 6) : 3;
   static constexpr int kRing = kWarps * kSlots * kSlotBytes;
-  static constexpr int kSmem = 1024 + kRing + kWarps * kSlots * 8 + 136 * 4 + 64;
+  static constexpr int kStats = kWarps * kRows * 8;           // maximum and sum of a warp's rows, for the CTA's own join
+  static constexpr int kSmem = 1024 + kRing + kStats + kWarps * kSlots * 8 + 136 * 4 + 64;
+  static_assert(NT * D * 32 <= kSlots * kSlotBytes, "a warp leaves its accumulator in its ring");
 };
 
 // Row r of a unit's tile rt: new token i, head, and how many keys it sees.
@@ -106,16 +111,20 @@ __device__ __forceinline__ void keys_times_queries(uint32_t kbase, const uint32_
 }
 
 // ------------------------------------------------------------------------------------------------ main kernel
-template <int D, int NT>
+// kCluster: a cluster of CTAs per unit instead of the even division, its results joined through distributed shared memory: nothing is left
+// to a second kernel.
+template <int D, int NT, bool kCluster>
 __global__ void __launch_bounds__(128, AttnCfg<D, NT>::kCtasPerSm)
 cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const CacheAttnParams p, const int row_tiles) {
   using C = AttnCfg<D, NT>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing);
+  float2* stats = reinterpret_cast<float2*>(smem + C::kRing);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kStats);
   int* cum = reinterpret_cast<int*>(bars + C::kWarps * C::kSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(cum + 134);
+  __shared__ int left_unit[C::kWarps], left_end[C::kWarps];   // what a warp leaves to the CTA's join: its unit (-1: nothing), its last block
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   if (tid == 0) {
@@ -127,12 +136,33 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   }
   grid_dep_wait();
   const int units = p.c.Hk * row_tiles;
-  const FlatRange range = flat_range(p.c, units, cum);        // its barriers publish the mbarriers too
-  const int worker = blockIdx.x * C::kWarps + warp, workers = min(p.grid * C::kWarps, range.total);      // each has a step at least
-  if (worker >= workers) return;
-  const int f0 = range_start(worker, workers, range.total), f_end = range_start(worker + 1, workers, range.total);
-  Piece seg = first_piece(p.c, units, range, f0, f_end);
-  Cursor ahead = cursor_start(p.c, units, seg, f_end);
+  Piece seg{};
+  int worker = warp, f_end = 0;
+  bool have;                                                  // this warp has a piece
+  if constexpr (kCluster) {
+    const int cl = p.cluster, unit = blockIdx.x / cl;
+    seg.b = unit / units;
+    seg.unit = unit - seg.b * units;
+    seg.n = cache_length(p.c, seg.b);
+    seg.blocks = (seg.n + 31) / 32;
+    const int w = (blockIdx.x - unit * cl) * C::kWarps + warp, all = cl * C::kWarps;
+    seg.blk0 = static_cast<int>(static_cast<int64_t>(w) * seg.blocks / all);
+    seg.blk1 = static_cast<int>(static_cast<int64_t>(w + 1) * seg.blocks / all);
+    have = seg.blk0 < seg.blk1;
+    __syncthreads();                                          // publishes the mbarriers
+  } else {
+    const FlatRange range = flat_range(p.c, units, cum);      // its barriers publish the mbarriers too
+    worker = blockIdx.x * C::kWarps + warp;
+    const int workers = min(p.grid * C::kWarps, range.total); // each has a step at least
+    have = worker < workers;
+    if (have) {
+      const int f0 = range_start(worker, workers, range.total);
+      f_end = range_start(worker + 1, workers, range.total);
+      seg = first_piece(p.c, units, range, f0, f_end);
+    }
+  }
+  Cursor ahead{};
+  if (have) ahead = cursor_start(p.c, units, seg, f_end);
 
   const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
   const uint32_t my_bars = smem_u32(bars + warp * C::kSlots);
@@ -179,7 +209,56 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
     if (ok) issue();
   };
-  for (int slot = 2 * worker;; ) {
+  float m[NT][2], l[NT][2], acc[NT][D / 16][4];
+  int vexp = -1000, slot = 2 * worker;
+  // Of a finished piece: the accumulator in its true scale and the rows' sums, complete in every lane.
+  auto settle = [&]() {
+    const float unit_exp = exp2f(static_cast<float>(max(vexp, -200) - 15));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], o);
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][c][i] *= unit_exp;
+    }
+  };
+  // The settled results of a warp: to where they belong, or to a slot for the join.  (c0, c1: the sixteenths of head_dim that it writes.)
+  auto write_out = [&](bool whole, int to_slot, int c0, int c1) {
+    const int hk = seg.unit / row_tiles, rt = seg.unit - hk * row_tiles, count = checked_count(p.c.status, p.counts, seg.b, p.Nq);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int in_tile = 8 * j + 2 * t + e, r = rt * C::kRows + in_tile;
+        if (r >= p.Nq * p.rep) continue;
+        if (whole) {
+          const RowInfo ri = row_info(p, r, hk, seg.n, count);
+          const bool any = ri.limit > 0;
+          const float inv = any ? 1.f / l[j][e] : 0.f;
+          __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(seg.b) * p.Nq + ri.i) * p.H + ri.head) * D + 2 * g);
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c)
+            if (c >= c0 && c < c1) o[8 * c] = any ? __floats2bfloat162_rn(acc[j][c][e] * inv, acc[j][c][2 + e] * inv) : __floats2bfloat162_rn(0.f, 0.f);
+          if (g == 0 && c0 == 0) {
+            p.lse[(static_cast<int64_t>(seg.b) * p.H + ri.head) * p.Nq + ri.i] = any ? (m[j][e] + log2f(l[j][e])) * kLn2 : -CUDART_INF_F;
+            if (p.row_ml != nullptr)
+              p.row_ml[(static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.Nq * p.rep + r] = make_float2(any ? m[j][e] : 0.f, inv);
+          }
+        } else {
+          const int64_t row = static_cast<int64_t>(to_slot) * C::kRows + in_tile;
+          float2* o = reinterpret_cast<float2*>(p.part_o + row * D + 2 * g);
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) o[8 * c] = make_float2(acc[j][c][e], acc[j][c][2 + e]);
+          if (g == 0) p.part_ml[row] = make_float2(m[j][e], l[j][e]);
+        }
+      }
+  };
+  bool pending = false;                                       // the last piece waits for the CTA's join
+  while (have) {
     if (seg.blk0 >= seg.blk1) {                               // nothing but the unit's own cost
       if (!next_piece(p.c, units, seg, f_end)) break;
       continue;
@@ -195,8 +274,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
       for (int e = 0; e < 2; ++e) lim[j][e] = row_info(p, rt * C::kRows + 8 * j + 2 * t + e, hk, seg.n, count).limit;
     if (p.causal) lim_min = seg.n - count + 1;                // of the rows that are any
-    float m[NT][2], l[NT][2], acc[NT][D / 16][4];
-    int vexp = -1000;                                         // largest exponent of a V scale so far: the accumulator counts in 2^(vexp - 15)
+    vexp = -1000;                                             // largest exponent of a V scale so far: the accumulator counts in 2^(vexp - 15)
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       m[j][0] = m[j][1] = -CUDART_INF_F;
@@ -308,44 +386,18 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
     if (!ok) break;
 
-    const float unit_exp = exp2f(static_cast<float>(vexp - 15));
-    const bool whole = seg.blk0 == 0 && seg.blk1 == seg.blocks;
-    // where the join finds the unit: the slot of its first piece, and the last warp that has one (the pieces between are their warps' first)
-    if (lane == 0) {
-      int2* u = p.unit_slots + (static_cast<int64_t>(seg.b) * units + seg.unit);
-      if (seg.blk0 == 0) u->x = whole ? -1 : slot;
-      if (seg.blk1 == seg.blocks) u->y = worker;
+    settle();
+    const bool whole = seg.blk0 == 0 && seg.blk1 == seg.blocks, last = seg.f1 >= f_end;
+    if (kCluster || (last && !whole)) {
+      pending = true;
+      break;
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float sum = l[j][e];
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const int in_tile = 8 * j + 2 * t + e, r = rt * C::kRows + in_tile;
-        if (r >= p.Nq * p.rep) continue;
-        if (whole) {
-          const RowInfo ri = row_info(p, r, hk, seg.n, count);
-          const bool any = ri.limit > 0;
-          const float inv = any ? 1.f / sum : 0.f;
-          __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(seg.b) * p.Nq + ri.i) * p.H + ri.head) * D + 2 * g);
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c)
-            o[8 * c] = any ? __floats2bfloat162_rn(acc[j][c][e] * unit_exp * inv, acc[j][c][2 + e] * unit_exp * inv) : __floats2bfloat162_rn(0.f, 0.f);
-          if (g == 0) {
-            p.lse[(static_cast<int64_t>(seg.b) * p.H + ri.head) * p.Nq + ri.i] = any ? (m[j][e] + log2f(sum)) * kLn2 : -CUDART_INF_F;
-            if (p.row_ml != nullptr)
-              p.row_ml[(static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.Nq * p.rep + r] = make_float2(any ? m[j][e] : 0.f, inv);
-          }
-        } else {
-          const int64_t row = static_cast<int64_t>(slot) * C::kRows + in_tile;
-          float2* o = reinterpret_cast<float2*>(p.part_o + row * D + 2 * g);
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) o[8 * c] = make_float2(acc[j][c][e] * unit_exp, acc[j][c][2 + e] * unit_exp);
-          if (g == 0) p.part_ml[row] = make_float2(m[j][e], sum);
-        }
-      }
+    if (lane == 0) {                                          // for the join (see unit_slots): a whole unit, or the end of one
+      int2* u = p.unit_slots + (static_cast<int64_t>(seg.b) * units + seg.unit);
+      if (whole) u->x = -1;
+      u->y = 2 * worker + 1;
+    }
+    write_out(whole, slot, 0, D / 16);
     slot = 2 * worker + 1;
     if (!next_piece(p.c, units, seg, f_end)) break;
   }
@@ -355,6 +407,102 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (++get == C::kSlots) {
       get = 0;
       parity ^= 1;
+    }
+  }
+
+  // The CTA's join.  Neighbouring warps that end in one unit: the first of them takes over the others' results, in their order, from their
+  // rings (which are done with).  In a cluster all warps are of one unit, those without blocks too.
+  float4* parked = reinterpret_cast<float4*>(smem + warp * C::kSlots * C::kSlotBytes);
+  if (kCluster && !pending) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      m[j][0] = m[j][1] = -CUDART_INF_F;
+      l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) acc[j][c][0] = acc[j][c][1] = acc[j][c][2] = acc[j][c][3] = 0.f;
+    }
+  }
+  if (lane == 0) {
+    left_unit[warp] = kCluster ? 0 : pending ? seg.b * units + seg.unit : -1;
+    left_end[warp] = seg.blk1;
+  }
+  __syncthreads();
+  const bool follows = warp > 0 && left_unit[warp] >= 0 && left_unit[warp - 1] == left_unit[warp];
+  auto park = [&]() {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if (g == 0) {
+        stats[warp * C::kRows + 8 * j + 2 * t] = make_float2(m[j][0], l[j][0]);
+        stats[warp * C::kRows + 8 * j + 2 * t + 1] = make_float2(m[j][1], l[j][1]);
+      }
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) parked[(j * (D / 16) + c) * 32 + lane] = make_float4(acc[j][c][0], acc[j][c][1], acc[j][c][2], acc[j][c][3]);
+    }
+  };
+  // Parked results, by their base and statistics, into this warp's.
+  auto take_over = [&](const float4* from, const float2* st, int c0, int c1) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float2 mine, theirs;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 x = st[8 * j + 2 * t + e];
+        const float top = fmaxf(m[j][e], x.x), mu = top == -CUDART_INF_F ? 0.f : top;
+        const float a = ex2_approx(m[j][e] - mu), b = ex2_approx(x.x - mu);
+        l[j][e] = l[j][e] * a + x.y * b;
+        m[j][e] = top;
+        (e ? mine.y : mine.x) = a;
+        (e ? theirs.y : theirs.x) = b;
+      }
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        if (c < c0 || c >= c1) continue;
+        const float4 x = from[(j * (D / 16) + c) * 32 + lane];
+        acc[j][c][0] = acc[j][c][0] * mine.x + x.x * theirs.x;
+        acc[j][c][1] = acc[j][c][1] * mine.y + x.y * theirs.y;
+        acc[j][c][2] = acc[j][c][2] * mine.x + x.z * theirs.x;
+        acc[j][c][3] = acc[j][c][3] * mine.y + x.w * theirs.y;
+      }
+    }
+  };
+  if (follows) park();
+  __syncthreads();
+  if constexpr (kCluster) {
+    if (warp == 0) {
+      for (int w = 1; w < C::kWarps; ++w) take_over(reinterpret_cast<const float4*>(smem + w * C::kSlots * C::kSlotBytes), stats + w * C::kRows, 0, D / 16);
+      park();
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // CTA r of the cluster joins and writes its share of the sixteenths of head_dim, over the CTAs in order
+    const int cl = p.cluster, rank = blockIdx.x % cl, c0 = rank * (D / 16) / cl, c1 = (rank + 1) * (D / 16) / cl;
+    if (warp == 0) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        m[j][0] = m[j][1] = -CUDART_INF_F;
+        l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) acc[j][c][0] = acc[j][c][1] = acc[j][c][2] = acc[j][c][3] = 0.f;
+      }
+      for (int r = 0; r < cl; ++r) take_over(cluster.map_shared_rank(parked, r), cluster.map_shared_rank(stats, r), c0, c1);
+      write_out(true, 0, c0, c1);
+    }
+    cluster.sync();                                           // shared memory stays until all have read it
+  } else {
+    if (pending && !follows) {
+      int end = seg.blk1, last = worker;
+      for (int w = warp + 1; w < C::kWarps && left_unit[w] == left_unit[warp]; ++w) {
+        take_over(reinterpret_cast<const float4*>(smem + w * C::kSlots * C::kSlotBytes), stats + w * C::kRows, 0, D / 16);
+        end = left_end[w];
+        ++last;
+      }
+      const bool whole = seg.blk0 == 0 && end == seg.blocks;
+      if (lane == 0) {
+        int2* u = p.unit_slots + (static_cast<int64_t>(seg.b) * units + seg.unit);
+        if (seg.blk0 == 0) u->x = whole ? -1 : slot;
+        if (end == seg.blocks) u->y = 2 * last;
+      }
+      write_out(whole, slot, 0, D / 16);
     }
   }
 }
@@ -386,10 +534,14 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
     return;
   }
   if (unit.x < 0) return;                                     // whole: written by its warp
-  // pieces: the first one's slot, then the first slots of the warps behind it
-  const int w0 = unit.x / 2, pieces = unit.y - w0 + 1;
+  // Pieces: the first slot, then the joined ones of the CTAs behind it, then the last warp's own where that went on with another unit.
+  const int cta0 = unit.x / 8, last = unit.y >> 1, cta1 = last / 4, own = unit.y & 1;
+  const int pieces = 1 + cta1 - cta0 - (own && cta1 > cta0 && last == 4 * cta1 ? 1 : 0) + own;
   const int in_tile = r - rt * row_tile;
-  auto row_of = [&](int i) { return static_cast<int64_t>(i == 0 ? unit.x : 2 * (w0 + i)) * row_tile + in_tile; };
+  auto row_of = [&](int i) {
+    const int at = i == 0 ? unit.x : own && i == pieces - 1 ? 2 * last : 8 * (cta0 + i);
+    return static_cast<int64_t>(at) * row_tile + in_tile;
+  };
   float top = -CUDART_INF_F;
   for (int i = tid; i < pieces; i += 128) top = fmaxf(top, p.part_ml[row_of(i)].x);
 #pragma unroll
@@ -579,10 +731,29 @@ cudaError_t allow_smem(int bytes) {
 template <int D, int NT>
 cudaError_t launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnParams& p, int row_tiles, cudaStream_t stream) {
   using C = AttnCfg<D, NT>;
-  cudaError_t e = allow_smem<cache_attn_kernel<D, NT>>(C::kSmem);
+  if (p.cluster > 0) {
+    const cudaError_t e = allow_smem<cache_attn_kernel<D, NT, true>>(C::kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.grid);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, NT, true>, tk, tv, p, row_tiles);
+  }
+  cudaError_t e = allow_smem<cache_attn_kernel<D, NT, false>>(C::kSmem);
   if (e != cudaSuccess) return e;
   count_launch();
-  e = launch_chained(cache_attn_kernel<D, NT>, dim3(p.grid), 128, C::kSmem, stream, tk, tv, p, row_tiles);
+  e = launch_chained(cache_attn_kernel<D, NT, false>, dim3(p.grid), 128, C::kSmem, stream, tk, tv, p, row_tiles);
   if (e != cudaSuccess) return e;
   count_launch();
   return launch_chained(cache_join_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(p.c.B) * p.H * p.Nq)), 128, 0, stream, p, row_tiles, C::kRows);
@@ -602,6 +773,7 @@ cudaError_t launch_weights(const CUtensorMap& tk, const CacheAttnParams& p, cuda
 
 // Rows (new tokens x heads of a group) from which the tcgen05 form is taken, at head_dim 128.
 constexpr int kChunkFrom = 33;
+constexpr int kClusterBlocks = 8;
 int small_row_tile(int D, int R) { return R <= 8 ? 8 : R <= 16 || D == 256 ? 16 : 32; }
 
 }  // namespace
@@ -612,12 +784,20 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   x.chunk = D == 128 && R >= kChunkFrom;
   x.row_tile = x.chunk ? cache_chunk_rows() : small_row_tile(D, R);
   x.row_tiles = (R + x.row_tile - 1) / x.row_tile;
-  // one wave, and no more workers than there can be blocks (tiles of four blocks for a CTA of the tcgen05 form)
-  const int64_t most = (static_cast<int64_t>(B) * Hk * x.row_tiles * (static_cast<int64_t>(T) * page / 32) + 3) / 4;
+  const int64_t blocks = static_cast<int64_t>(T) * (page / 32), units = static_cast<int64_t>(B) * Hk * x.row_tiles;       // of a sequence; in all
   const int ctas = x.chunk ? 1 : D == 128 && x.row_tile == 8 ? AttnCfg<128, 1>::kCtasPerSm : AttnCfg<128, 2>::kCtasPerSm;
   const int64_t wave = static_cast<int64_t>(sm_count()) * ctas;
-  x.grid = static_cast<int>(most < wave ? most : wave);
-  const int64_t slots = 2ll * x.grid * (x.chunk ? 1 : 4);
+  // A cluster per unit where a warp of it has at most kClusterBlocks blocks and all clusters are resident at a time.
+  x.cluster = 0;
+  if (!x.chunk) {
+    int cl = 1;
+    while (cl < 8 && units * cl * 2 <= wave && cl * 4 < blocks) cl *= 2;
+    if (units * cl <= wave && blocks <= static_cast<int64_t>(kClusterBlocks) * 4 * cl) x.cluster = cl;
+  }
+  // otherwise one wave, and no more workers than there can be blocks (tiles of four blocks for a CTA of the tcgen05 form)
+  const int64_t most = (units * blocks + 3) / 4;
+  x.grid = x.cluster > 0 ? static_cast<int>(units) * x.cluster : static_cast<int>(most < wave ? most : wave);
+  const int64_t slots = x.cluster > 0 ? 0 : 2ll * x.grid * (x.chunk ? 1 : 4);
   x.part_o_bytes = slots * x.row_tile * D * 4;
   x.part_ml_bytes = slots * x.row_tile * 8;
   const int64_t q_rows = x.chunk ? cache_chunk_query_rows(B, Hk, R) : 0;
