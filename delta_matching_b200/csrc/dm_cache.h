@@ -55,6 +55,7 @@ struct CacheAttnParams {
   int2* unit_slots;                 // per unit (B, Hk, row tiles), where its pieces are: slot of the first (-1: whole); the last worker (for the
                                     // small form twice that, plus one where its piece lies in a slot of its own)
   float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null
+  float* logits;                    // (B, Hk, T * page, row tile), log2 domain, masked: for the weights of up to 16 rows; or null
   float* weights;                   // (B, Hk, W) or null
   int64_t w_sb, w_sh;
   int W;
@@ -83,8 +84,8 @@ struct CacheAttnPlan {
   int row_tiles;
   int grid;
   int cluster;                      // CTAs a unit, or 0: the even division
-  int64_t part_o_bytes, part_ml_bytes, q16_bytes, factor_bytes, start_bytes, unit_bytes, row_ml_bytes;
-  int64_t bytes() const { return part_o_bytes + part_ml_bytes + q16_bytes + factor_bytes + start_bytes + unit_bytes + row_ml_bytes; }
+  int64_t part_o_bytes, part_ml_bytes, q16_bytes, factor_bytes, start_bytes, unit_bytes, row_ml_bytes, logit_bytes;
+  int64_t bytes() const { return part_o_bytes + part_ml_bytes + q16_bytes + factor_bytes + start_bytes + unit_bytes + row_ml_bytes + logit_bytes; }
 };
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights);
 

@@ -23,6 +23,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+constexpr int kMaxCluster = 8;
+
 template <int D, int NT>
 struct AttnCfg {
   static constexpr int kWarps = 4;
@@ -49,10 +51,11 @@ __device__ __forceinline__ RowInfo row_info(const CacheAttnParams& p, int r, int
   return x;
 }
 
-// Query fragments of a row tile: row 8 j + g, elements 16 c + 4 t ... + 3, as f16 scaled by a power of two per row.  Returns the factors of
-// this thread's accumulator rows 8 j + 2 t and + 1 (softmax scale and log2 e included) in f.
+// Query fragments of a row tile: row 8 j + g, elements 16 c + 4 t ... + 3.  In two steps, so that other loads can be sent off between them:
+// the bf16 values; then the same as f16, scaled by a power of two per row, with the factors of this thread's accumulator rows 8 j + 2 t and
+// + 1 (softmax scale and log2 e included) in f.
 template <int D, int NT>
-__device__ __forceinline__ void load_queries(const CacheAttnParams& p, int b, int hk, int rt, int count, uint32_t (&qf)[NT][D / 16][2], float2 (&f)[NT]) {
+__device__ __forceinline__ void ask_queries(const CacheAttnParams& p, int b, int hk, int rt, int count, uint32_t (&qf)[NT][D / 16][2]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -60,26 +63,42 @@ __device__ __forceinline__ void load_queries(const CacheAttnParams& p, int b, in
     const int i = r / p.rep, head = hk * p.rep + r - i * p.rep;
     const bool valid = i < count;                             // rows beyond the call's: zeros
     const __nv_bfloat16* src = p.q + b * p.q_sb + i * p.q_sn + head * p.q_sh + 4 * t;
-    uint2 raw[D / 16];
-    float amax = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
-      raw[c] = valid ? __ldg(reinterpret_cast<const uint2*>(src + 16 * c)) : make_uint2(0, 0);
-      amax = fmaxf(amax, fmaxf(fmaxf(fabsf(__uint_as_float(raw[c].x << 16)), fabsf(__uint_as_float(raw[c].x & 0xFFFF0000u))),
-                               fmaxf(fabsf(__uint_as_float(raw[c].y << 16)), fabsf(__uint_as_float(raw[c].y & 0xFFFF0000u)))));
+      const uint2 raw = valid ? __ldg(reinterpret_cast<const uint2*>(src + 16 * c)) : make_uint2(0, 0);
+      qf[j][c][0] = raw.x;
+      qf[j][c][1] = raw.y;
     }
+  }
+}
+template <int D, int NT>
+__device__ __forceinline__ void scale_queries(const CacheAttnParams& p, uint32_t (&qf)[NT][D / 16][2], float2 (&f)[NT]) {
+  const int t = threadIdx.x & 3;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    float amax = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        amax = max3(amax, fabsf(__uint_as_float(qf[j][c][i] << 16)), fabsf(__uint_as_float(qf[j][c][i] & 0xFFFF0000u)));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const uint32_t eb = min(254u, max(14u, __float_as_uint(amax) >> 23));
     const float up = sb_to_scale(267u - eb);                  // largest element to [2^13, 2^14)
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      qf[j][c][0] = pack_f16x2(__uint_as_float(raw[c].x << 16) * up, __uint_as_float(raw[c].x & 0xFFFF0000u) * up);
-      qf[j][c][1] = pack_f16x2(__uint_as_float(raw[c].y << 16) * up, __uint_as_float(raw[c].y & 0xFFFF0000u) * up);
-    }
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        qf[j][c][i] = pack_f16x2(__uint_as_float(qf[j][c][i] << 16) * up, __uint_as_float(qf[j][c][i] & 0xFFFF0000u) * up);
     const float back = sb_to_scale(eb - 13u) * p.scale * kLog2e;
     f[j] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t), __shfl_sync(0xffffffffu, back, 8 * t + 4));
   }
+}
+template <int D, int NT>
+__device__ __forceinline__ void load_queries(const CacheAttnParams& p, int b, int hk, int rt, int count, uint32_t (&qf)[NT][D / 16][2], float2 (&f)[NT]) {
+  ask_queries<D, NT>(p, b, hk, rt, count, qf);
+  scale_queries<D, NT>(p, qf, f);
 }
 
 // S^T of a block: acc[j][mt] rows: keys 16 mt + g (elements 0, 1) and + 8 (2, 3); columns: query rows 8 j + 2 t, + 1.
@@ -92,6 +111,9 @@ __device__ __forceinline__ void keys_times_queries(uint32_t kbase, const uint32_
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[j][mt][i] = 0.f;
+  // even and odd chunks in accumulators of their own where registers allow: a chain of dependent MMAs is what a block waits for
+  constexpr bool kTwo = NT == 1;
+  float s2[kTwo ? NT : 1][2][4] = {};
 #pragma unroll
   for (int c = 0; c < D / 16; ++c) {
     uint32_t r[4];
@@ -104,9 +126,15 @@ __device__ __forceinline__ void keys_times_queries(uint32_t kbase, const uint32_
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      mma_f16(s[j][0], lo[0], lo[1], hi[0], hi[1], qf[j][c][0], qf[j][c][1]);
-      mma_f16(s[j][1], lo[2], lo[3], hi[2], hi[3], qf[j][c][0], qf[j][c][1]);
+      mma_f16(kTwo && (c & 1) ? s2[kTwo ? j : 0][0] : s[j][0], lo[0], lo[1], hi[0], hi[1], qf[j][c][0], qf[j][c][1]);
+      mma_f16(kTwo && (c & 1) ? s2[kTwo ? j : 0][1] : s[j][1], lo[2], lo[3], hi[2], hi[3], qf[j][c][0], qf[j][c][1]);
     }
+  }
+  if (kTwo) {
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[0][mt][i] += s2[0][mt][i];
   }
 }
 
@@ -161,8 +189,15 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       seg = first_piece(p.c, units, range, f0, f_end);
     }
   }
+  // the first piece's queries, then its pages: the loads are under way together
+  while (have && seg.blk0 >= seg.blk1) have = next_piece(p.c, units, seg, f_end);       // no blocks: nothing but a unit's own cost
+  uint32_t qf[NT][D / 16][2];
   Cursor ahead{};
-  if (have) ahead = cursor_start(p.c, units, seg, f_end);
+  if (have) {
+    const int hk = seg.unit / row_tiles;
+    ask_queries<D, NT>(p, seg.b, hk, seg.unit - hk * row_tiles, checked_count(p.c.status, p.counts, seg.b, p.Nq), qf);
+    ahead = cursor_start(p.c, units, seg, f_end);
+  }
 
   const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
   const uint32_t my_bars = smem_u32(bars + warp * C::kSlots);
@@ -173,20 +208,21 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   // The next box of this warp into its ring, if there is one.
   auto issue = [&]() {
     if (!ahead.live) return;
-    const int page = max(0, checked_page(p.c, ahead.page)), hk = row_tiles == 1 ? ahead.s.unit : ahead.s.unit / row_tiles;
+    const int2 at = cursor_at(p.c, ahead);                    // page, place
+    const int hk = row_tiles == 1 ? ahead.s.unit : ahead.s.unit / row_tiles;
     const bool is_v = issued & 1;
     if (lane == 0) {
       const uint32_t bar = my_bars + 8 * put, dst = ring + put * C::kSlotBytes;
       asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(C::kSlotBytes) : "memory");
 #pragma unroll
-      for (int x = 0; x < D; x += 128) tma_load_4d(dst + x * 32, is_v ? &tv : &tk, bar, x, ahead.sub * 32, hk, page);
+      for (int x = 0; x < D; x += 128) tma_load_4d(dst + x * 32, is_v ? &tv : &tk, bar, x, at.y * 32, hk, at.x);
     }
     if (is_v) {
       cursor_next(p.c, units, ahead, f_end);
     } else if (lane == ((issued >> 1) & 7)) {
-      const int64_t at = page * p.c.s_page + hk * p.c.s_head + ahead.sub;
-      ks_reg = __ldg(p.c.ks + at);
-      vs_reg = __ldg(p.c.vs + at);
+      const int64_t scale = at.x * p.c.s_page + hk * p.c.s_head + at.y;
+      ks_reg = __ldg(p.c.ks + scale);
+      vs_reg = __ldg(p.c.vs + scale);
     }
     ++issued;
     if (++put == C::kSlots) put = 0;
@@ -226,8 +262,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         for (int i = 0; i < 4; ++i) acc[j][c][i] *= unit_exp;
     }
   };
-  // The settled results of a warp: to where they belong, or to a slot for the join.  (c0, c1: the sixteenths of head_dim that it writes.)
-  auto write_out = [&](bool whole, int to_slot, int c0, int c1) {
+  // The settled results of a warp: to where they belong, or to a slot for the join.  `one`: only this sixteenth of head_dim, held in the first.
+  auto write_out = [&](bool whole, int to_slot, int one) {
     const int hk = seg.unit / row_tiles, rt = seg.unit - hk * row_tiles, count = checked_count(p.c.status, p.counts, seg.b, p.Nq);
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -240,10 +276,14 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           const bool any = ri.limit > 0;
           const float inv = any ? 1.f / l[j][e] : 0.f;
           __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(seg.b) * p.Nq + ri.i) * p.H + ri.head) * D + 2 * g);
+          if (kCluster) {
+            o[8 * one] = any ? __floats2bfloat162_rn(acc[j][0][e] * inv, acc[j][0][2 + e] * inv) : __floats2bfloat162_rn(0.f, 0.f);
+          } else {
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c)
-            if (c >= c0 && c < c1) o[8 * c] = any ? __floats2bfloat162_rn(acc[j][c][e] * inv, acc[j][c][2 + e] * inv) : __floats2bfloat162_rn(0.f, 0.f);
-          if (g == 0 && c0 == 0) {
+            for (int c = 0; c < D / 16; ++c)
+              o[8 * c] = any ? __floats2bfloat162_rn(acc[j][c][e] * inv, acc[j][c][2 + e] * inv) : __floats2bfloat162_rn(0.f, 0.f);
+          }
+          if (g == 0 && one == 0) {
             p.lse[(static_cast<int64_t>(seg.b) * p.H + ri.head) * p.Nq + ri.i] = any ? (m[j][e] + log2f(l[j][e])) * kLn2 : -CUDART_INF_F;
             if (p.row_ml != nullptr)
               p.row_ml[(static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.Nq * p.rep + r] = make_float2(any ? m[j][e] : 0.f, inv);
@@ -258,6 +298,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       }
   };
   bool pending = false;                                       // the last piece waits for the CTA's join
+  bool asked = true;                                          // the piece's queries are on their way
   while (have) {
     if (seg.blk0 >= seg.blk1) {                               // nothing but the unit's own cost
       if (!next_piece(p.c, units, seg, f_end)) break;
@@ -265,9 +306,10 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
     const int hk = seg.unit / row_tiles, rt = seg.unit - hk * row_tiles;
     const int count = checked_count(p.c.status, p.counts, seg.b, p.Nq);
-    uint32_t qf[NT][D / 16][2];
     float2 f[NT];
-    load_queries<D, NT>(p, seg.b, hk, rt, count, qf, f);
+    if (!asked) ask_queries<D, NT>(p, seg.b, hk, rt, count, qf);
+    asked = false;
+    scale_queries<D, NT>(p, qf, f);
     int lim[NT][2], lim_min = seg.n;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -290,14 +332,14 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       const float ks = __shfl_sync(0xffffffffu, ks_reg, at), vs = __shfl_sync(0xffffffffu, vs_reg, at);
       float s[NT][2][4];
       keys_times_queries<D, NT>(ring + get * C::kSlotBytes, qf, s);
-      release();
       const int key0 = kb * 32;
       const bool cut = key0 + 32 > lim_min;                   // some row does not see all keys of the block
       const int e_blk = static_cast<int>((__float_as_uint(vs) >> 23) & 0xFF) - 127, e_new = max(vexp, e_blk);
       // p comes out as 2^off exp(s - m); where V's scale is 2^-60 of another's the product vanishes anyway, but the sum must not
       const int off = max(15 + e_blk - e_new, -45);
-      const float back = __uint_as_float((127 - off) << 23), shrink = exp2f(static_cast<float>(vexp - e_new));
-      bool moved = e_new != vexp;
+      const float back = __uint_as_float((127 - off) << 23);
+      const int shrink = vexp - e_new;
+      bool moved = shrink != 0;
       vexp = e_new;
       uint32_t pb[NT][2][2];
       float2 alpha[NT];
@@ -311,6 +353,14 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             s[j][mt][i] *= (i & 1) ? fs.y : fs.x;
             if (cut && key0 + 16 * mt + g + 8 * (i >> 1) >= lim[j][i & 1]) s[j][mt][i] = -CUDART_INF_F;
           }
+        if (NT <= 2 && p.logits != nullptr) {                 // for the weights: (b, kv head, token, row of the tile)
+          float* to = p.logits + ((static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.c.T * p.c.page + key0 + g) * C::kRows + 8 * j + 2 * t;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              *reinterpret_cast<float2*>(to + (16 * mt + 8 * i) * C::kRows) = make_float2(s[j][mt][2 * i], s[j][mt][2 * i + 1]);
+        }
         float2 mx = make_float2(fmaxf(fmaxf(s[j][0][0], s[j][0][2]), fmaxf(s[j][1][0], s[j][1][2])),
                                 fmaxf(fmaxf(s[j][0][1], s[j][0][3]), fmaxf(s[j][1][1], s[j][1][3])));
 #pragma unroll
@@ -341,10 +391,12 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         l[j][0] = fmaf(l[j][0], alpha[j].x, sum.x * back);
         l[j][1] = fmaf(l[j][1], alpha[j].y, sum.y * back);
       }
+      release();
       if (__any_sync(0xffffffffu, moved)) {
+        const float by = shrink == 0 ? 1.f : exp2f(static_cast<float>(shrink));
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const float ax = alpha[j].x * shrink, ay = alpha[j].y * shrink;
+          const float ax = alpha[j].x * by, ay = alpha[j].y * by;
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
             acc[j][c][0] *= ax;
@@ -397,7 +449,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       if (whole) u->x = -1;
       u->y = 2 * worker + 1;
     }
-    write_out(whole, slot, 0, D / 16);
+    write_out(whole, slot, 0);
     slot = 2 * worker + 1;
     if (!next_piece(p.c, units, seg, f_end)) break;
   }
@@ -440,7 +492,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
   };
   // Parked results, by their base and statistics, into this warp's.
-  auto take_over = [&](const float4* from, const float2* st, int c0, int c1) {
+  auto take_over = [&](const float4* from, const float2* st) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float2 mine, theirs;
@@ -456,7 +508,6 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       }
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
-        if (c < c0 || c >= c1) continue;
         const float4 x = from[(j * (D / 16) + c) * 32 + lane];
         acc[j][c][0] = acc[j][c][0] * mine.x + x.x * theirs.x;
         acc[j][c][1] = acc[j][c][1] * mine.y + x.y * theirs.y;
@@ -469,30 +520,56 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   __syncthreads();
   if constexpr (kCluster) {
     if (warp == 0) {
-      for (int w = 1; w < C::kWarps; ++w) take_over(reinterpret_cast<const float4*>(smem + w * C::kSlots * C::kSlotBytes), stats + w * C::kRows, 0, D / 16);
+      for (int w = 1; w < C::kWarps; ++w) take_over(reinterpret_cast<const float4*>(smem + w * C::kSlots * C::kSlotBytes), stats + w * C::kRows);
       park();
     }
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    // CTA r of the cluster joins and writes its share of the sixteenths of head_dim, over the CTAs in order
-    const int cl = p.cluster, rank = blockIdx.x % cl, c0 = rank * (D / 16) / cl, c1 = (rank + 1) * (D / 16) / cl;
-    if (warp == 0) {
+    // CTA r of the cluster joins and writes its share of the sixteenths of head_dim, a warp a sixteenth, over the CTAs in order
+    const int cl = p.cluster, rank = blockIdx.x % cl, c1 = (rank + 1) * (D / 16) / cl;
+    for (int c = rank * (D / 16) / cl + warp; c < c1; c += C::kWarps) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        m[j][0] = m[j][1] = -CUDART_INF_F;
-        l[j][0] = l[j][1] = 0.f;
+        float2 st[kMaxCluster][2];
+        float4 x[kMaxCluster];                                // all on their way together
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) acc[j][c][0] = acc[j][c][1] = acc[j][c][2] = acc[j][c][3] = 0.f;
+        for (int r = 0; r < kMaxCluster; ++r) {
+          if (r >= cl) continue;
+          const float2* from = cluster.map_shared_rank(stats, r) + 8 * j + 2 * t;
+          st[r][0] = from[0];
+          st[r][1] = from[1];
+          x[r] = cluster.map_shared_rank(reinterpret_cast<float4*>(smem), r)[(j * (D / 16) + c) * 32 + lane];
+        }
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < kMaxCluster; ++r)
+            if (r < cl) top = fmaxf(top, st[r][e].x);
+          const float mu = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll
+          for (int r = 0; r < kMaxCluster; ++r) {
+            if (r >= cl) continue;
+            const float w = ex2_approx(st[r][e].x - mu);
+            sum = fmaf(st[r][e].y, w, sum);
+            o[e] = fmaf(e ? x[r].y : x[r].x, w, o[e]);
+            o[2 + e] = fmaf(e ? x[r].w : x[r].z, w, o[2 + e]);
+          }
+          m[j][e] = top;
+          l[j][e] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][0][i] = o[i];
       }
-      for (int r = 0; r < cl; ++r) take_over(cluster.map_shared_rank(parked, r), cluster.map_shared_rank(stats, r), c0, c1);
-      write_out(true, 0, c0, c1);
+      write_out(true, 0, c);
     }
     cluster.sync();                                           // shared memory stays until all have read it
   } else {
     if (pending && !follows) {
       int end = seg.blk1, last = worker;
       for (int w = warp + 1; w < C::kWarps && left_unit[w] == left_unit[warp]; ++w) {
-        take_over(reinterpret_cast<const float4*>(smem + w * C::kSlots * C::kSlotBytes), stats + w * C::kRows, 0, D / 16);
+        take_over(reinterpret_cast<const float4*>(smem + w * C::kSlots * C::kSlotBytes), stats + w * C::kRows);
         end = left_end[w];
         ++last;
       }
@@ -502,7 +579,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (seg.blk0 == 0) u->x = whole ? -1 : slot;
         if (end == seg.blocks) u->y = 2 * last;
       }
-      write_out(whole, slot, 0, D / 16);
+      write_out(whole, slot, 0);
     }
   }
 }
@@ -596,6 +673,35 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
 // ------------------------------------------------------------------------------------------------ weights
 // weights[b, hk, j] (+)= sum over the group's rows of exp(s_rj - m_r) / l_r, with the rows' m and l from the kernels before: K is read once
 // more, a block of 32 tokens a warp, all row tiles on it; no result is shared between warps, and the sum's order is that of the rows.
+// This is the form for many rows; up to 16 rows the main kernel leaves its logits (32 or 64 bytes a token instead of K's 128 or 256, and no
+// products), and cache_weights_of_logits_kernel adds their exponentials: one thread a token.
+__global__ void __launch_bounds__(256) cache_weights_of_logits_kernel(const CacheAttnParams p, const int row_tile, const int pieces) {
+  __shared__ float2 ml[16];
+  grid_dep_wait();
+  const int bh = blockIdx.x / pieces, j = (blockIdx.x - bh * pieces) * 256 + threadIdx.x, b = bh / p.c.Hk, hk = bh - b * p.c.Hk, R = p.Nq * p.rep;
+  const int n = cache_length(p.c, b);
+  if (threadIdx.x < R) ml[threadIdx.x] = p.row_ml[static_cast<int64_t>(bh) * R + threadIdx.x];
+  __syncthreads();
+  if (j >= p.W) return;
+  float* at = p.weights + b * p.w_sb + hk * p.w_sh + j;
+  if (j >= n) {                                               // beyond the length: zero, unless the sums go on
+    if (!p.accumulate) *at = 0.f;
+    return;
+  }
+  const float* x = p.logits + (static_cast<int64_t>(bh) * p.c.T * p.c.page + j) * row_tile;
+  float w = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    if (r >= R) break;
+    const float4 v = *reinterpret_cast<const float4*>(x + r);
+    w += ex2_approx(v.x - ml[r].x) * ml[r].y;
+    if (r + 1 < R) w += ex2_approx(v.y - ml[r + 1].x) * ml[r + 1].y;
+    if (r + 2 < R) w += ex2_approx(v.z - ml[r + 2].x) * ml[r + 2].y;
+    if (r + 3 < R) w += ex2_approx(v.w - ml[r + 3].x) * ml[r + 3].y;
+  }
+  *at = p.accumulate ? *at + w : w;
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constant__ CUtensorMap tk, const CacheAttnParams p, const int row_tiles) {
   constexpr int kStages = 4, kStageBytes = 32 * D, kRows = 8 * NT;
@@ -632,7 +738,8 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
   const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes, my_bars = smem_u32(bars + warp * kStages);
   float ks_reg = 0.f;
   auto issue = [&](int st) {
-    const int page = max(0, checked_page(p.c, ahead.page)), sub = ahead.sub, hk = ahead.s.unit;
+    const int2 where = cursor_at(p.c, ahead);
+    const int page = where.x, sub = where.y, hk = ahead.s.unit;
     if (lane == 0) {
       const uint32_t bar = my_bars + 8 * st, dst = ring + st * kStageBytes;
       asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kStageBytes) : "memory");
@@ -805,6 +912,8 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   x.factor_bytes = q_rows * 4;
   x.start_bytes = x.chunk ? x.grid * cache_chunk_start_bytes() : 0;
   x.unit_bytes = static_cast<int64_t>(B) * Hk * x.row_tiles * 8;
+  // logits for the weights, where they are fewer bytes than K
+  x.logit_bytes = weights && R <= 16 ? static_cast<int64_t>(B) * Hk * T * page * x.row_tile * 4 : 0;
   x.row_ml_bytes = weights ? static_cast<int64_t>(B) * Hk * R * 8 : 0;
   return x;
 }
@@ -820,8 +929,12 @@ cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& t
     e = tile == 8 ? launch_main<256, 1>(tk, tv, p, row_tiles, stream) : launch_main<256, 2>(tk, tv, p, row_tiles, stream);
   }
   if (e != cudaSuccess || p.weights == nullptr) return e;
-  if (D == 128) return tile == 8 ? launch_weights<128, 1>(tk, p, stream) : tile == 16 ? launch_weights<128, 2>(tk, p, stream) : launch_weights<128, 4>(tk, p, stream);
-  return tile == 8 ? launch_weights<256, 1>(tk, p, stream) : launch_weights<256, 2>(tk, p, stream);
+  if (p.logits != nullptr) {
+    const int pieces = (p.W + 255) / 256;
+    count_launch();
+    return launch_chained(cache_weights_of_logits_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * pieces), 256, 0, stream, p, tile, pieces);
+  }
+  return D == 128 ? launch_weights<128, 4>(tk, p, stream) : launch_weights<256, 2>(tk, p, stream);
 }
 
 }  // namespace dm

@@ -39,9 +39,12 @@ __device__ __forceinline__ FlatRange flat_range(const CacheView& c, int units, i
   __syncthreads();
   return FlatRange{cum[128], chunk, cum};
 }
+// w total / workers, without 64-bit division (workers^2 < 2^32).
 __device__ __forceinline__ int range_start(int w, int workers, int total) {
-  return static_cast<int>(static_cast<int64_t>(w) * total / workers);
+  const unsigned q = static_cast<unsigned>(total) / workers, r = static_cast<unsigned>(total) - q * workers;
+  return static_cast<int>(w * q + w * r / workers);
 }
+
 // A warp's piece of a unit.
 struct Piece {
   int b, unit, n, blocks;         // sequence, unit within it, its length and blocks
@@ -94,13 +97,20 @@ __device__ __forceinline__ bool next_piece(const CacheView& c, int units, Piece&
   return true;
 }
 
-// The blocks of a warp's pieces in order, with their pages: what its loads run ahead on.
+// The blocks of a warp's pieces in order, with their pages: what its loads run ahead on.  Pages are looked up for 32 blocks at a time, one a
+// lane, so that a block costs no load and no division of its own.
 struct Cursor {
   Piece s;
-  int kb, sub, entry;             // block, its place in its page, the page's place in the table
-  int page;                       // looked up when the cursor comes to it
+  int kb, window;                 // block; first block of the window
+  int page, sub;                  // of block window + lane: its page, and its place in it
   bool live;
 };
+__device__ __forceinline__ void cursor_window(const CacheView& c, Cursor& k) {
+  const int bpp = c.page / 32, blk = k.kb + (threadIdx.x & 31), entry = blk / bpp;
+  k.window = k.kb;
+  k.sub = blk - entry * bpp;
+  k.page = blk < k.s.blk1 ? __ldg(c.table + k.s.b * c.t_row + entry) : 0;
+}
 __device__ __forceinline__ void cursor_enter(const CacheView& c, int units, Cursor& k, int f_end) {
   while (k.s.blk0 >= k.s.blk1) {
     if (!next_piece(c, units, k.s, f_end)) {
@@ -108,11 +118,8 @@ __device__ __forceinline__ void cursor_enter(const CacheView& c, int units, Curs
       return;
     }
   }
-  const int bpp = c.page / 32;
   k.kb = k.s.blk0;
-  k.entry = k.kb / bpp;
-  k.sub = k.kb - k.entry * bpp;
-  k.page = __ldg(c.table + k.s.b * c.t_row + k.entry);
+  cursor_window(c, k);
 }
 __device__ __forceinline__ Cursor cursor_start(const CacheView& c, int units, const Piece& s, int f_end) {
   Cursor k{s, 0, 0, 0, 0, true};
@@ -121,14 +128,16 @@ __device__ __forceinline__ Cursor cursor_start(const CacheView& c, int units, co
 }
 __device__ __forceinline__ void cursor_next(const CacheView& c, int units, Cursor& k, int f_end) {
   if (++k.kb < k.s.blk1) {
-    if (++k.sub == c.page / 32) {
-      k.sub = 0;
-      k.page = __ldg(c.table + k.s.b * c.t_row + ++k.entry);
-    }
+    if (k.kb - k.window == 32) cursor_window(c, k);
     return;
   }
   k.s.blk0 = k.s.blk1;            // done with this piece
   cursor_enter(c, units, k, f_end);
+}
+// Page and place of the cursor's block, for the whole warp; a page that is none is reported and replaced by page 0.
+__device__ __forceinline__ int2 cursor_at(const CacheView& c, const Cursor& k) {
+  const int page = __shfl_sync(0xffffffffu, k.page, k.kb - k.window), sub = __shfl_sync(0xffffffffu, k.sub, k.kb - k.window);
+  return make_int2(max(0, checked_page(c, page)), sub);
 }
 
 }  // namespace dm
