@@ -30,11 +30,15 @@ struct AttnCfg {
   static constexpr int kWarps = 4;
   static constexpr int kRows = 8 * NT;
   static constexpr int kSlotBytes = 32 * D;                   // K or V of a block
-  static constexpr int kCtasPerSm = D == 128 && NT == 1 ? 3 : NT == 4 ? 2 : 2;
-  static constexpr int kSlots = D == 128 ? (NT == 1 ? 4 : 6) : 3;
+  static constexpr int kCtasPerSm = D == 128 && NT == 1 ? 3 : 2;
+  // 32 rows: the query fragments wait in shared memory (64 registers beside an accumulator of 128 spilled: B=8 with 4096 - 8192 tokens, H=32 Hk=8,
+  // 8 new tokens 79 us against 57)
+  static constexpr bool kSharedQ = NT == 4;
+  static constexpr int kSlots = D == 128 ? (NT == 2 ? 6 : 4) : 3;
   static constexpr int kRing = kWarps * kSlots * kSlotBytes;
+  static constexpr int kQBytes = kSharedQ ? NT * D * 16 : 0;  // of a warp
   static constexpr int kStats = kWarps * kRows * 8;           // maximum and sum of a warp's rows, for the CTA's own join
-  static constexpr int kSmem = 1024 + kRing + kStats + kWarps * kSlots * 8 + 136 * 4 + 64;
+  static constexpr int kSmem = 1024 + kRing + kWarps * kQBytes + kStats + kWarps * kSlots * 8 + 136 * 4 + 64;
   static_assert(NT * D * 32 <= kSlots * kSlotBytes, "a warp leaves its accumulator in its ring");
 };
 
@@ -101,9 +105,10 @@ __device__ __forceinline__ void load_queries(const CacheAttnParams& p, int b, in
   scale_queries<D, NT>(p, qf, f);
 }
 
-// S^T of a block: acc[j][mt] rows: keys 16 mt + g (elements 0, 1) and + 8 (2, 3); columns: query rows 8 j + 2 t, + 1.
-template <int D, int NT>
-__device__ __forceinline__ void keys_times_queries(uint32_t kbase, const uint32_t (&qf)[NT][D / 16][2], float (&s)[NT][2][4]) {
+// S^T of a block: acc[j][mt] rows: keys 16 mt + g (elements 0, 1) and + 8 (2, 3); columns: query rows 8 j + 2 t, + 1.  The query fragments
+// come from registers, or (kShared) from q_sm: fragment (j, c) of this lane 8 bytes at (j D / 16 + c) 256.
+template <int D, int NT, bool kShared>
+__device__ __forceinline__ void keys_times_queries(uint32_t kbase, uint32_t q_sm, const uint32_t (&qf)[NT][D / 16][2], float (&s)[NT][2][4]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -126,8 +131,17 @@ __device__ __forceinline__ void keys_times_queries(uint32_t kbase, const uint32_
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      mma_f16(kTwo && (c & 1) ? s2[kTwo ? j : 0][0] : s[j][0], lo[0], lo[1], hi[0], hi[1], qf[j][c][0], qf[j][c][1]);
-      mma_f16(kTwo && (c & 1) ? s2[kTwo ? j : 0][1] : s[j][1], lo[2], lo[3], hi[2], hi[3], qf[j][c][0], qf[j][c][1]);
+      uint32_t q0, q1;
+      if (kShared) {
+        const float2 q = lds_f2(q_sm + (j * (D / 16) + c) * 256);
+        q0 = __float_as_uint(q.x);
+        q1 = __float_as_uint(q.y);
+      } else {
+        q0 = qf[j][c][0];
+        q1 = qf[j][c][1];
+      }
+      mma_f16(kTwo && (c & 1) ? s2[kTwo ? j : 0][0] : s[j][0], lo[0], lo[1], hi[0], hi[1], q0, q1);
+      mma_f16(kTwo && (c & 1) ? s2[kTwo ? j : 0][1] : s[j][1], lo[2], lo[3], hi[2], hi[3], q0, q1);
     }
   }
   if (kTwo) {
@@ -148,8 +162,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
-  float2* stats = reinterpret_cast<float2*>(smem + C::kRing);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kStats);
+  float2* stats = reinterpret_cast<float2*>(smem + C::kRing + C::kWarps * C::kQBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kWarps * C::kQBytes + C::kStats);
   int* cum = reinterpret_cast<int*>(bars + C::kWarps * C::kSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(cum + 134);
   __shared__ int left_unit[C::kWarps], left_end[C::kWarps];   // what a warp leaves to the CTA's join: its unit (-1: nothing), its last block
@@ -201,6 +215,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
   const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
   const uint32_t my_bars = smem_u32(bars + warp * C::kSlots);
+  const uint32_t q_sm = smem_u32(smem) + C::kRing + warp * C::kQBytes + lane * 8;         // a lane reads what it has written
   float ks_reg = 0.f, vs_reg = 0.f;                           // lane i % 8: the scales of the i-th block of this warp
   int issued = 0, used = 0;                                   // boxes: K and V of a block in turn
   int put = 0, get = 0;                                       // their places in the ring
@@ -310,6 +325,12 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (!asked) ask_queries<D, NT>(p, seg.b, hk, rt, count, qf);
     asked = false;
     scale_queries<D, NT>(p, qf, f);
+    if (C::kSharedQ) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) sts_f2(q_sm + (j * (D / 16) + c) * 256, __uint_as_float(qf[j][c][0]), __uint_as_float(qf[j][c][1]));
+    }
     int lim[NT][2], lim_min = seg.n;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -331,7 +352,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       if (!ok) break;
       const float ks = __shfl_sync(0xffffffffu, ks_reg, at), vs = __shfl_sync(0xffffffffu, vs_reg, at);
       float s[NT][2][4];
-      keys_times_queries<D, NT>(ring + get * C::kSlotBytes, qf, s);
+      keys_times_queries<D, NT, C::kSharedQ>(ring + get * C::kSlotBytes, q_sm, qf, s);
       const int key0 = kb * 32;
       const bool cut = key0 + 32 > lim_min;                   // some row does not see all keys of the block
       const int e_blk = static_cast<int>((__float_as_uint(vs) >> 23) & 0xFF) - 127, e_new = max(vexp, e_blk);
@@ -776,7 +797,7 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
         for (int rt = 0; rt < row_tiles; ++rt) {
           if (row_tiles > 1) load_queries<D, NT>(p, seg.b, hk, rt, count, qf, f);
           float s[NT][2][4];
-          keys_times_queries<D, NT>(ring + st * kStageBytes, qf, s);
+          keys_times_queries<D, NT, false>(ring + st * kStageBytes, 0, qf, s);
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll

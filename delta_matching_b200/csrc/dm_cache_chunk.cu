@@ -22,6 +22,9 @@ namespace dm {
 namespace {
 
 constexpr int kChunkCost = 3;               // key tiles that a unit's queries and output are worth
+// Key tiles of a piece from which one row tile is worth two results: us with and without at H=32 Hk=8, B=8 with 4096 - 8192 tokens and 9 new ones
+// (about 21 tiles a piece) 101 and 113, B=2 with 16 new ones (5 tiles) 62 and 53.
+constexpr int kSplitFrom = 10;
 constexpr int kPBase = 12;                  // log2 of P at the reference maximum,
 constexpr float kHeadroom = 3.9f;           // and what a row may exceed it by: P stays below 2^16
 
@@ -97,7 +100,11 @@ struct ChunkPiece {
   int b, hk, rt;
   ChunkSeq s;
   int tiles, t0, t1, f1;
-  __device__ __forceinline__ int row_tiles(const CacheAttnParams& p) const { return s.count * p.rep - rt * ChunkCfg::kRows > 128 ? 2 : 1; }
+  // Softmax groups at work: both, except that a short piece of a unit of one row tile has one.
+  // A long piece of such a unit is split: its key tiles go to the two groups in turn, each with a result of its own for the join.
+  __device__ __forceinline__ bool one_tile(const CacheAttnParams& p) const { return s.count * p.rep - rt * ChunkCfg::kRows <= 128; }
+  __device__ __forceinline__ bool split(const CacheAttnParams& p) const { return one_tile(p) && t1 - t0 >= kSplitFrom; }
+  __device__ __forceinline__ int groups(const CacheAttnParams& p) const { return one_tile(p) && t1 - t0 < kSplitFrom ? 1 : 2; }
 };
 __device__ __forceinline__ void chunk_cut(const CacheAttnParams& p, ChunkPiece& x, int at, int f, int f_end) {
   x.tiles = unit_tiles(p, x.s, x.rt);
@@ -380,35 +387,37 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         };
         do {
           if (x.t0 >= x.t1) continue;
-          const int nr = x.row_tiles(p);
-          ok = wait_or_abort(bar(kKFull), g & 1, abort_flag);
-          for (int r = 0; r < nr && ok; ++r) {
+          // both groups work on every key tile, or (split) each on every second one
+          const bool split = x.split(p);
+          const int step = split ? 2 : 1, n = x.t1 - x.t0, groups = x.groups(p);
+          for (int r = 0; r < groups; ++r) {
+            if ((r == 0 || split) && !(ok = wait_or_abort(bar(kKFull), (g + (split ? r : 0)) & 1, abort_flag))) break;
             if (!(ok = wait_or_abort(bar(kQFull + r), units[r]++ & 1, abort_flag))) break;
             tc_fence_after();
-            issue_s(r, r == nr - 1);
-            if (x.t0 + 1 == x.t1) tc_commit(bars + kQFree + r);
+            issue_s(r, split || r == groups - 1);
+            if ((split ? r : 0) + step >= n) tc_commit(bars + kQFree + r);      // the group's last S of the unit
           }
-          for (int t = x.t0; t < x.t1 && ok; ++t, ++g) {
-            for (int r = 0; r < nr; ++r) {
+          for (int i = 0; i < n && ok; ++i, ++g) {
+            for (int r = split ? i & 1 : 0; r < groups; r += step) {
               // 16 keys a step: 8 columns of P, 16 rows of V; the first half of the keys while the softmax is at the second
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
                 if (!(ok = wait_or_abort(bar((half == 0 ? kPHalf : kPFull) + r), tiles[r] & 1, abort_flag))) break;
-                if (r == 0 && half == 0 && !(ok = wait_or_abort(bar(kVFull + (g & 1)), (g >> 1) & 1, abort_flag))) break;
+                if ((r == 0 || split) && half == 0 && !(ok = wait_or_abort(bar(kVFull + (g & 1)), (g >> 1) & 1, abort_flag))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  mma_h_ts(tmem + 256 + 128 * r, tmem + 128 * r + 8 * k, v_lo + (g & 1) * (2 * C::kTile >> 4) + k * (2048 >> 4), kIdescO, t > x.t0 || k > 0);
+                  mma_h_ts(tmem + 256 + 128 * r, tmem + 128 * r + 8 * k, v_lo + (g & 1) * (2 * C::kTile >> 4) + k * (2048 >> 4), kIdescO, i >= step || k > 0);
               }
               if (!ok) break;
               ++tiles[r];
-              if (r == nr - 1) tc_commit(bars + kVEmpty + (g & 1));
+              if (split || r == groups - 1) tc_commit(bars + kVEmpty + (g & 1));
               tc_commit(bars + kPvDone + r);
-              if (t + 1 < x.t1) {
-                if (r == 0 && !(ok = wait_or_abort(bar(kKFull), (g + 1) & 1, abort_flag))) break;
+              if (i + step < n) {
+                if ((r == 0 || split) && !(ok = wait_or_abort(bar(kKFull), (g + step) & 1, abort_flag))) break;
                 tc_fence_after();
-                issue_s(r, r == nr - 1);
-                if (t + 2 == x.t1) tc_commit(bars + kQFree + r);      // the unit's last S
+                issue_s(r, split || r == groups - 1);
+                if (i + 2 * step >= n) tc_commit(bars + kQFree + r);
               }
             }
           }
@@ -422,12 +431,13 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int tiles_of_head = (p.Nq * p.rep + 127) / 128;
         do {
           if (x.t0 >= x.t1) continue;
-          for (int r = 0; r < x.row_tiles(p) && ok; ++r) {
+          const bool split = x.split(p);
+          for (int r = 0; r < x.groups(p) && ok; ++r) {
             if (units[r] > 0) ok = wait_or_abort(bar(kQFree + r), (units[r] - 1) & 1, abort_flag);
             if (!ok) break;
             ++units[r];
             mbar_expect_tx(bars + kQFull + r, 2 * C::kTile);
-            const int row = ((x.b * p.c.Hk + x.hk) * tiles_of_head + 2 * x.rt + r) * 128;
+            const int row = ((x.b * p.c.Hk + x.hk) * tiles_of_head + 2 * x.rt + (split ? 0 : r)) * 128;
             for (int panel = 0; panel < 2; ++panel)
               tma_load_2d(smem + C::kSmemQ + (2 * r + panel) * C::kTile, &tq, bars + kQFull + r, 128 * panel, row);        // x in bytes
           }
@@ -500,12 +510,15 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       int slot = 2 * cta;
       do {
         if (x.t0 >= x.t1) continue;
-        if (r >= x.row_tiles(p)) {
+        const bool split = x.split(p);
+        const int step = split ? 2 : 1, first = x.t0 + (split ? r : 0);       // this group's key tiles
+        if (r >= x.groups(p)) {                               // none: a result of nothing
+          p.part_ml[static_cast<int64_t>(slot) * C::kRows + r * 128 + in_tile] = make_float2(-CUDART_INF_F, 0.f);
           g += x.t1 - x.t0;
           slot = 2 * cta + 1;
           continue;
         }
-        const int row = x.rt * C::kRows + r * 128 + in_tile, limit = row_limit(p, x.s, row);
+        const int row = x.rt * C::kRows + (split ? 0 : r * 128) + in_tile, limit = row_limit(p, x.s, row);
         const int i_tok = row / p.rep, head = x.hk * p.rep + row - i_tok * p.rep;
         // of the row's logits, K's scale aside
         const float f = __ldg(p.factors + (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + 127) / 128 * 128) + row);
@@ -514,7 +527,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         // One key tile.  kCut: some row of the warp does not see all its keys (a compile-time variant: no select per element elsewhere).
         auto tile = [&](int t, auto cut_tag) -> bool {
           constexpr bool kCut = decltype(cut_tag)::value;
-          const float4 ks = lds_f4(sbase + C::kSmemScales + (g & 7) * 32), vs = lds_f4(sbase + C::kSmemScales + (g & 7) * 32 + 16);
+          const int entry = (g + t - x.t0) & 7;
+          const float4 ks = lds_f4(sbase + C::kSmemScales + entry * 32), vs = lds_f4(sbase + C::kSmemScales + entry * 32 + 16);
           const float fc[4] = {f * ks.x, f * ks.y, f * ks.z, f * ks.w};
           const int ev[4] = {static_cast<int>(scale_to_sb(vs.x)) - 127, static_cast<int>(scale_to_sb(vs.y)) - 127, static_cast<int>(scale_to_sb(vs.z)) - 127,
                              static_cast<int>(scale_to_sb(vs.w)) - 127};
@@ -548,7 +562,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           tmem_ld32(t_s, s_buf[0]);
           if (__any_sync(0xffffffffu, m_new != m || v_new != vexp)) {
             const float keep = ex2_approx(m - mu);
-            if (t > x.t0) {
+            if (t > first) {
               if (!wait_warp(bar(kPvDone + r), (mine - 1) & 1, abort_flag)) return false;
               tc_fence_after();
               const float a = keep * exp2f(static_cast<float>(vexp - v_new));
@@ -600,18 +614,20 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           if (lane == 0) mbar_arrive(bars + kPFull + r);
           return true;
         };
-        for (int t = x.t0; t < x.t1; ++t, ++g, ++mine) {
-          ok = wait_warp(bar(kScales + (g & 7)), (g >> 3) & 1, abort_flag) && wait_warp(bar(kSFull + r), mine & 1, abort_flag);
+        for (int t = first; t < x.t1; t += step, ++mine) {
+          const int gt = g + t - x.t0;
+          ok = wait_warp(bar(kScales + (gt & 7)), (gt >> 3) & 1, abort_flag) && wait_warp(bar(kSFull + r), mine & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
           const bool cut = __any_sync(0xffffffffu, limit < 128 * (t + 1));
           if (!(ok = cut ? tile(t, std::true_type{}) : tile(t, std::false_type{}))) break;
         }
+        g += x.t1 - x.t0;
         if (!ok) break;
         ok = wait_warp(bar(kPvDone + r), (mine - 1) & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const bool whole = x.t0 == 0 && x.t1 == x.tiles;
+        const bool whole = x.t0 == 0 && x.t1 == x.tiles && !split;
         const float unit_exp = exp2f(static_cast<float>(vexp - kPBase));
         const float scale = whole ? unit_exp / l : unit_exp;
         // where a row that sees something goes
@@ -721,11 +737,14 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
     if (unit.x < 0) continue;                                 // whole: written by its CTA
     float top = -CUDART_INF_F, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = unit.x / 2; c <= unit.y; ++c) {
-      const int64_t at = static_cast<int64_t>(c == unit.x / 2 ? unit.x : 2 * c) * ChunkCfg::kRows + (r & (ChunkCfg::kRows - 1));
+    const int halves = s.count * p.rep - r / ChunkCfg::kRows * ChunkCfg::kRows <= 128 ? 2 : 1;      // a split unit's pieces have two results
+    const int first = unit.x / 2 * halves, n = unit.y * halves + halves;
+    for (int i = first; i < n; ++i) {
+      const int c = i / halves;
+      const int64_t at = static_cast<int64_t>(c == unit.x / 2 ? unit.x : 2 * c) * ChunkCfg::kRows + (r & (ChunkCfg::kRows - 1)) + (i - c * halves) * 128;
       const float2 ml = p.part_ml[at];
-      const float4 v = reinterpret_cast<const float4*>(p.part_o + at * D)[lane];
       if (ml.x == -CUDART_INF_F) continue;                    // a piece of which the row sees nothing
+      const float4 v = reinterpret_cast<const float4*>(p.part_o + at * D)[lane];
       const float top_new = fmaxf(top, ml.x), a = exp2f(top - top_new), w = exp2f(ml.x - top_new);
       sum = sum * a + ml.y * w;
       acc = make_float4(acc.x * a + v.x * w, acc.y * a + v.y * w, acc.z * a + v.z * w, acc.w * a + v.w * w);

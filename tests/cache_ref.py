@@ -166,3 +166,35 @@ def same_values(cache, pools):
         if not bool(((a == b) | (((a | b) & 0x7F) == 0) | (((a & 0x7F) == 0x7F) & ((b & 0x7F) == 0x7F))).all()):
             return False
     return all(torch.equal(a.cpu().view(torch.int32), b.view(torch.int32)) for a, b in zip((cache.ks, cache.vs), pools.scales))
+
+
+def attention_on_device(q, cache, table, lengths, counts, causal, scale):
+    """attention() for sizes that take the CPU too long: the same formulas and bounds, in fp64 on the GPU, one (sequence, kv head) at a time.  -> o, lse and
+    bounds; rows that see nothing are 0 and -inf."""
+    B, N, H, D = q.shape
+    Hk, P = cache.k8.shape[1:3]
+    rep = H // Hk
+    o, do = torch.zeros(B, N, H, D, dtype=torch.float64, device="cuda"), torch.zeros(B, N, H, D, dtype=torch.float64, device="cuda")
+    lse, dlse = torch.full((B, H, N), -math.inf, dtype=torch.float64, device="cuda"), torch.zeros(B, H, N, dtype=torch.float64, device="cuda")
+    for b in range(B):
+        n, count = int(lengths[b]), int(counts[b])
+        if n == 0 or count == 0:
+            continue
+        at = torch.arange(n, device="cuda")
+        page = table[b].to("cuda").long()[at // P]
+        see = at[None] < ((n - count + 1 + torch.arange(count, device="cuda")).clamp(min=0)[:, None] if causal else n)
+        for h in range(Hk):
+            k, v = (c[page, h, at % P].double() * s[page, h, at % P // BLK].double()[:, None] for c, s in ((cache.k8.float(), cache.ks), (cache.v8.float(), cache.vs)))
+            coarsest = float(cache.vs[page, h, at % P // BLK].max())
+            for hh in range(h * rep, (h + 1) * rep):
+                qi = q[b, :count, hh].cuda().double()
+                s = (qi @ k.T * scale).masked_fill(~see, -math.inf)
+                eps = (qi.abs() @ k.abs().T * scale).masked_fill(~see, 0.0).amax(1) * 2.0 ** -19
+                some = see.any(1)
+                lse[b, hh, :count] = torch.logsumexp(s, 1)
+                p = torch.nan_to_num(torch.softmax(s, 1))
+                o[b, :count, hh] = p @ v
+                do[b, :count, hh] = (2.0 ** -8 * o[b, :count, hh].abs() + (2.0 ** -11 + 2 * eps + 2.0 ** -19)[:, None] * (p @ v.abs())
+                                     + (2.0 ** -40 * see.sum(1) * 448 * coarsest + 1e-37)[:, None])
+                dlse[b, hh, :count] = torch.where(some, eps + 2.0 ** -19 + 2.0 ** -22 * lse[b, hh, :count].abs(), 0.0)
+    return (o, lse), (do, dlse)

@@ -101,3 +101,18 @@ def test_bad_device_values_are_reported():
         dm.dm_cache_attn(q, cache, bad_table.cuda(), bad_n, q_counts=counts)
         with pytest.raises(RuntimeError, match=says):
             ops.check_status("cuda")
+
+
+@pytest.mark.parametrize("B, Hk, rep, N, lo, hi", [(6, 8, 4, 9, 3000, 4100), (5, 8, 3, 43, 2900, 4097), (3, 8, 8, 40, 3000, 5000)])
+def test_long_pieces(B, Hk, rep, N, lo, hi):
+    """Pieces of ten key tiles and more: of one row tile (their tiles go to two groups in turn), of one and a bit, of several."""
+    lengths = [lo + (hi - lo) * b // (B - 1) for b in range(B)]
+    counts = [N - b % 3 for b in range(B)]
+    cache, pools, table = _filled(lengths, 64, Hk, 128, seed=N)
+    q = _rand(torch.Generator().manual_seed(N), B, N, Hk * rep, 128).cuda()
+    o, lse = dm.dm_cache_attn(q, cache, table.cuda(), _ints(lengths).cuda(), q_counts=_ints(counts).cuda(), return_lse=True)
+    ops.check_status("cuda")
+    want, off = ref.attention_on_device(q, cache, table, lengths, counts, True, 128 ** -0.5)
+    assert bool(((o.double() - want[0]).abs() <= off[0]).all())
+    seen = want[1] > -torch.inf
+    assert torch.equal(lse > -torch.inf, seen) and bool(((lse.double() - want[1])[seen].abs() <= off[1][seen]).all())
