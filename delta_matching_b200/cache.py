@@ -15,8 +15,8 @@ int32 is what each sequence holds.  Both are device tensors and are never copied
 replayed with other lengths.  An entry or length out of range is therefore reported like a kernel that gave up (RuntimeError from the next
 call, or from ops.check_status), and nothing outside the buffers is touched.
 
-Input errors raise ValueError / TypeError / NotImplementedError.  These are serving operators: no autograd graph is recorded.  The reference
-package has no counterpart.
+Input errors raise ValueError / TypeError.  These are serving operators: no autograd graph is recorded.  Under torch.compile they are
+registered ops without a graph break.  examples/decode_with_cache.py runs the three together.  The reference package has no counterpart.
 """
 from __future__ import annotations
 
@@ -26,8 +26,10 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, ops
+from . import torch_ops as _torch_ops  # noqa: F401  (registers torch.ops.delta_matching_b200.*)
 
 E4M3 = torch.float8_e4m3fn
+_OPS = torch.ops.delta_matching_b200
 
 
 class _CCache(ctypes.Structure):
@@ -149,6 +151,8 @@ def dm_cache_append(cache, k, v, block_table, lengths, counts=None):
 
     Each block of 32 slots and head gets the smallest power-of-two scale that holds its new values; a block that already holds tokens keeps
     the larger of the two scales, and its codes are rounded anew when that grows."""
+    if torch.compiler.is_compiling():
+        return _OPS.cache_append(*cache, k, v, block_table, lengths, counts)
     new = _lib.native_cache().cache_append(cache, k, v, block_table, lengths, counts)
     if new is not None:
         return new
@@ -183,6 +187,10 @@ def dm_cache_attn(q, cache, block_table, lengths, q_counts=None, causal=True, so
     tokens and over the query heads of its kv head; accumulate=True adds it to what is there.  return_lse=True also returns the LSE (B, H, N)
     fp32, natural log.  The logits and the softmax are those of the codes' exact values: q and the probabilities keep 8 and 11 bits or
     more, sums and statistics are fp32."""
+    if torch.compiler.is_compiling():
+        args = (q, *cache, block_table, lengths, q_counts, bool(causal), softmax_scale)
+        o, lse = _OPS.cache_attn(*args) if weights is None else _OPS.cache_attn_weights(*args, weights, bool(accumulate))
+        return (o, lse) if return_lse else o
     out = _lib.native_cache().cache_attn(q, cache, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, return_lse)
     if out is not None:
         return out
@@ -229,6 +237,8 @@ def dm_cache_evict(cache, block_table, lengths, weights, new_block_table, budget
 
     Returns (new lengths (B) int32, kept (B, Hk, budget) int32: the old positions in order, -1 beyond, new weights (B, Hk, T2 * page_size) fp32: those of the
     kept tokens, 0 beyond).  The heads of a sequence keep different tokens but equally many."""
+    if torch.compiler.is_compiling():
+        return _OPS.cache_evict(*cache, block_table, lengths, weights, new_block_table, budget, recent)
     out = _lib.native_cache().cache_evict(cache, block_table, lengths, weights, new_block_table, budget, recent)
     if out is not None:
         return out

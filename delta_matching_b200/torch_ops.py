@@ -1,4 +1,4 @@
-"""The op layer registered with torch.library, so that a tracing compiler sees five opaque ops with known output shapes
+"""The op layer registered with torch.library, so that a tracing compiler sees opaque ops with known output shapes
 instead of ctypes calls it cannot look into.
 
     torch.ops.delta_matching_b200.quant_qkv(q, k, v)                     -> q8, qs, k8, ks, v8, vs, kmean
@@ -6,17 +6,23 @@ instead of ctypes calls it cannot look into.
     torch.ops.delta_matching_b200.quant_do(do, o, with_o)                -> do8, dos, delta
     torch.ops.delta_matching_b200.delta_fp8(q8, k8, v8, do8, qs, ks, vs, dos, lse, causal, norm) -> delta
     torch.ops.delta_matching_b200.bwd_fp8(q8, k8, v8, do8, qs, ks, vs, dos, lse, delta, causal, ds32) -> dq, dk, dv
+    torch.ops.delta_matching_b200.cache_append(k8!, v8!, ks!, vs!, k, v, block_table, lengths, counts) -> new lengths
+    torch.ops.delta_matching_b200.cache_attn(q, k8, v8, ks, vs, block_table, lengths, q_counts, causal, softmax_scale) -> O, LSE
+    torch.ops.delta_matching_b200.cache_attn_weights(..., weights!, accumulate) -> O, LSE
+    torch.ops.delta_matching_b200.cache_evict(k8!, v8!, ks!, vs!, block_table, lengths, weights, new_block_table, budget, recent)
+        -> new lengths, kept, new weights
 
 The reference registers the same roles as real ops (csrc/delta_matching_api.cpp:683-715: fwd_fp8, delta_fp8, bwd_fp8_t)
 and its autograd function calls them through torch.ops (delta_matching/attn.py:37-118), which is what lets its API run
 under torch.compile without a graph break (tests/test_api.py:304-317).  The implementations are the functions of
 delta_matching_b200.ops (CUDA only; there is no CPU implementation to fall back to); the fake implementations only
 state shapes, dtypes and devices.  Tensors are in the op layer's layout: inputs (B, H, N, D) views, codes (B, H, N, D)
-e4m3, scales (B, H, N // 32) fp32, O / dQ (B, N, H, D), dK / dV (B, N, Hk, D) bf16.
+e4m3, scales (B, H, N // 32) fp32, O / dQ (B, N, H, D), dK / dV (B, N, Hk, D) bf16.  The cache's ops take its four pools one by one (those
+marked ! are written in place) and are what the functions of cache.py call while a compiler is tracing.
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -105,8 +111,67 @@ def _(q8, k8, v8, do8, qs, ks, vs, dos, lse, delta, causal, ds32):
             q8.new_empty((B, N, Hk, D), dtype=BF16))
 
 
+def _cache_append(k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, k: Tensor, v: Tensor, block_table: Tensor, lengths: Tensor,
+                  counts: Optional[Tensor]) -> Tensor:
+    from . import cache
+    return cache.dm_cache_append(cache.KVCache8(k8, v8, ks, vs), k, v, block_table, lengths, counts)
+
+
+cache_append = torch.library.custom_op(f"{NS}::cache_append", _cache_append, mutates_args=("k8", "v8", "ks", "vs"), device_types="cuda")
+
+
+@cache_append.register_fake
+def _(k8, v8, ks, vs, k, v, block_table, lengths, counts):
+    return lengths.new_empty(lengths.shape)
+
+
+def _cache_attn(q: Tensor, k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, q_counts: Optional[Tensor],
+                causal: bool, softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor]:
+    from . import cache
+    return cache.dm_cache_attn(q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, return_lse=True)
+
+
+cache_attn = torch.library.custom_op(f"{NS}::cache_attn", _cache_attn, mutates_args=(), device_types="cuda")
+
+
+@cache_attn.register_fake
+def _(q, k8, v8, ks, vs, block_table, lengths, q_counts, causal, softmax_scale):
+    B, N, H, D = q.shape
+    return q.new_empty((B, N, H, D)), q.new_empty((B, H, N), dtype=F32)
+
+
+def _cache_attn_weights(q: Tensor, k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, q_counts: Optional[Tensor],
+                        causal: bool, softmax_scale: Optional[float], weights: Tensor, accumulate: bool) -> Tuple[Tensor, Tensor]:
+    from . import cache
+    return cache.dm_cache_attn(q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, True)
+
+
+cache_attn_weights = torch.library.custom_op(f"{NS}::cache_attn_weights", _cache_attn_weights, mutates_args=("weights",), device_types="cuda")
+
+
+@cache_attn_weights.register_fake
+def _(q, k8, v8, ks, vs, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate):
+    B, N, H, D = q.shape
+    return q.new_empty((B, N, H, D)), q.new_empty((B, H, N), dtype=F32)
+
+
+def _cache_evict(k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, weights: Tensor, new_block_table: Tensor,
+                 budget: int, recent: int) -> Tuple[Tensor, Tensor, Tensor]:
+    from . import cache
+    return cache.dm_cache_evict(cache.KVCache8(k8, v8, ks, vs), block_table, lengths, weights, new_block_table, budget, recent)
+
+
+cache_evict = torch.library.custom_op(f"{NS}::cache_evict", _cache_evict, mutates_args=("k8", "v8", "ks", "vs"), device_types="cuda")
+
+
+@cache_evict.register_fake
+def _(k8, v8, ks, vs, block_table, lengths, weights, new_block_table, budget, recent):
+    B, Hk = weights.shape[:2]
+    return (lengths.new_empty((B,)), lengths.new_empty((B, Hk, budget)), weights.new_empty((B, Hk, new_block_table.shape[1] * k8.shape[2])))
+
+
 class _Direct:
-    """The same five calls without the dispatcher in between: what the eager path uses (a registered op costs tens of
+    """The attention's five calls without the dispatcher in between: what the eager path uses (a registered op costs tens of
     microseconds of host time per call, which shows once the kernels of a step take about two milliseconds)."""
     quant_qkv = staticmethod(_quant_qkv)
     fwd_fp8 = staticmethod(_fwd_fp8)

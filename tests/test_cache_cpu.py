@@ -102,3 +102,20 @@ def test_python_refusals_before_the_device():
         dm.dm_cache_attn(x, dm.KVCache8(code[0], code, scale, scale), t, i)
     with pytest.raises(ValueError, match="page_size"):
         dm.KVCache8.empty(4, 40, 2, 128, device="cpu")
+
+
+def test_registered_ops_state_their_layout():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ns = torch.ops.delta_matching_b200
+    B, N, H, Hk, D, P, T = 3, 5, 8, 2, 128, 64, 7
+    with FakeTensorMode():
+        new = lambda *s, d=torch.float32: torch.empty(*s, device="cuda", dtype=d)
+        pools = (new(9, Hk, P, D, d=torch.float8_e4m3fn), new(9, Hk, P, D, d=torch.float8_e4m3fn), new(9, Hk, P // 32), new(9, Hk, P // 32))
+        k, q = new(B, N, Hk, D, d=torch.bfloat16), new(B, N, H, D, d=torch.bfloat16)
+        table, lengths, w = new(B, T, d=torch.int32), new(B, d=torch.int32), new(B, Hk, T * P)
+        got = ns.cache_append(*pools, k, k, table, lengths, None)
+        assert got.shape == (B,) and got.dtype == torch.int32
+        for o, lse in (ns.cache_attn(q, *pools, table, lengths, lengths, True, None), ns.cache_attn_weights(q, *pools, table, lengths, None, True, 0.1, w, False)):
+            assert o.shape == q.shape and o.dtype == torch.bfloat16 and lse.shape == (B, H, N) and lse.dtype == torch.float32
+        n, kept, nw = ns.cache_evict(*pools, table, lengths, w, new(B, 2, d=torch.int32), 100, 10)
+        assert n.shape == (B,) and kept.shape == (B, Hk, 100) and kept.dtype == torch.int32 and nw.shape == (B, Hk, 2 * P) and nw.dtype == torch.float32
