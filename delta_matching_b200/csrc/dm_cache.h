@@ -54,7 +54,8 @@ struct CacheAttnParams {
   void* starts;                     // and what each CTA begins with
   int2* unit_slots;                 // per unit (B, Hk, row tiles), where its pieces are: slot of the first (-1: whole); the last worker (for the
                                     // small form twice that, plus one where its piece lies in a slot of its own)
-  float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null
+  float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null.  Of the form
+                                    // for many rows: factor of the logits and log2 of the sum, rows of a head filled up to whole tiles
   float* logits;                    // (B, Hk, T * page, row tile), log2 domain, masked: for the weights of up to 16 rows; or null
   float* weights;                   // (B, Hk, W) or null
   int64_t w_sb, w_sh;

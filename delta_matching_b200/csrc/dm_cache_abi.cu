@@ -139,7 +139,7 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   p.o = static_cast<__nv_bfloat16*>(o);
   p.lse = lse;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  auto take = [&ws](int64_t bytes) {                          // every part is a multiple of 8 bytes, the first ones of 16
+  auto take = [&ws](int64_t bytes) {                          // every part is a multiple of 8 bytes, those up to the factors of 16
     uint8_t* at = ws;
     ws += bytes;
     return at;
@@ -149,9 +149,9 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   p.q16 = reinterpret_cast<__half*>(take(x.q16_bytes));
   p.part_ml = reinterpret_cast<float2*>(take(x.part_ml_bytes));
   p.factors = reinterpret_cast<float*>(take(x.factor_bytes));
+  p.row_ml = weights != nullptr ? reinterpret_cast<float2*>(take(x.row_ml_bytes)) : nullptr;
   p.starts = take(x.start_bytes);
   p.unit_slots = reinterpret_cast<int2*>(take(x.unit_bytes));
-  p.row_ml = weights != nullptr ? reinterpret_cast<float2*>(take(x.row_ml_bytes)) : nullptr;
   p.weights = weights;
   p.w_sb = w_sb; p.w_sh = w_sh; p.W = W; p.accumulate = accumulate ? 1 : 0;
   p.grid = x.grid;

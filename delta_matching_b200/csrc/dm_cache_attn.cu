@@ -935,7 +935,7 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   x.unit_bytes = static_cast<int64_t>(B) * Hk * x.row_tiles * 8;
   // logits for the weights, where they are fewer bytes than K
   x.logit_bytes = weights && R <= 16 ? static_cast<int64_t>(B) * Hk * T * page * x.row_tile * 4 : 0;
-  x.row_ml_bytes = weights ? static_cast<int64_t>(B) * Hk * R * 8 : 0;
+  x.row_ml_bytes = !weights ? 0 : x.chunk ? q_rows * 8 : static_cast<int64_t>(B) * Hk * R * 8;
   return x;
 }
 
@@ -949,7 +949,7 @@ cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& t
   } else {
     e = tile == 8 ? launch_main<256, 1>(tk, tv, p, row_tiles, stream) : launch_main<256, 2>(tk, tv, p, row_tiles, stream);
   }
-  if (e != cudaSuccess || p.weights == nullptr) return e;
+  if (e != cudaSuccess || p.weights == nullptr || (D == 128 && R >= kChunkFrom)) return e;
   if (p.logits != nullptr) {
     const int pieces = (p.W + 255) / 256;
     count_launch();

@@ -239,7 +239,11 @@ __global__ void __launch_bounds__(256) cache_chunk_queries_kernel(const CacheAtt
 #pragma unroll
   for (int j = 0; j < 4; ++j) h[j] = pack_f16x2(__uint_as_float(v[j] << 16) * up, __uint_as_float(v[j] & 0xFFFF0000u) * up);
   reinterpret_cast<uint4*>(p.q16 + row * ChunkCfg::D)[lane] = make_uint4(h[0], h[1], h[2], h[3]);
-  if (lane == 0) p.factors[row] = sb_to_scale(eb - 13u) * p.scale * kLog2e;
+  if (lane == 0) {
+    const float f = sb_to_scale(eb - 13u) * p.scale * kLog2e;
+    p.factors[row] = f;
+    if (p.row_ml != nullptr) p.row_ml[row] = make_float2(f, CUDART_INF_F);      // sees nothing, until its sum is known
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ main kernel
@@ -521,7 +525,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int row = x.rt * C::kRows + (split ? 0 : r * 128) + in_tile, limit = row_limit(p, x.s, row);
         const int i_tok = row / p.rep, head = x.hk * p.rep + row - i_tok * p.rep;
         // of the row's logits, K's scale aside
-        const float f = __ldg(p.factors + (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + 127) / 128 * 128) + row);
+        const int64_t padded_row = (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + 127) / 128 * 128) + row;
+        const float f = __ldg(p.factors + padded_row);
         float m = -CUDART_INF_F, l = 0.f;
         int vexp = -1000;
         // One key tile.  kCut: some row of the warp does not see all its keys (a compile-time variant: no select per element elsewhere).
@@ -688,7 +693,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         if (limit > 0) {
           if (whole) {
             p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.Nq + i_tok] = (m + log2f(l)) * kLn2;
-            if (p.row_ml != nullptr) p.row_ml[(static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * p.Nq * p.rep + row] = make_float2(m, 1.f / l);
+            if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(f, m + log2f(l));
           } else {
             p.part_ml[part0 + lane] = make_float2(m, l);
           }
@@ -725,13 +730,10 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
     const int i_tok = r / p.rep, head = hk * p.rep + r - i_tok * p.rep;
     __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(b) * p.Nq + i_tok) * p.H + head) * D) + 2 * lane;
     float* lse = p.lse + (static_cast<int64_t>(b) * p.H + head) * p.Nq + i_tok;
-    float2* row_ml = p.row_ml == nullptr ? nullptr : p.row_ml + static_cast<int64_t>(bh) * R + r;
+    const int64_t padded_row = static_cast<int64_t>(bh) * ((R + 127) / 128 * 128) + r;
     if (row_limit(p, s, r) == 0) {
       o[0] = o[1] = __floats2bfloat162_rn(0.f, 0.f);
-      if (lane == 0) {
-        *lse = -CUDART_INF_F;
-        if (row_ml != nullptr) *row_ml = make_float2(0.f, 0.f);
-      }
+      if (lane == 0) *lse = -CUDART_INF_F;
       continue;
     }
     if (unit.x < 0) continue;                                 // whole: written by its CTA
@@ -755,8 +757,264 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
     o[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
     if (lane == 0) {
       *lse = (top + log2f(sum)) * kLn2;
-      if (row_ml != nullptr) *row_ml = make_float2(top, inv);
+      if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(p.factors[padded_row], top + log2f(sum));
     }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ weights
+// weights[b, hk, j] (+)= sum over the rows r that see token j of exp(s_rj) / sum_r = 2^(f_r ks s_rj - c_r), c_r = log2 of the row's sum.
+// S^T = K Q^T on tcgen05 with 128 tokens as M and 256 rows as N: a token's sum stays in its thread (TMEM lane) over all row tiles, in the order of the
+// rows.  An item is a key tile of a (sequence, head): its codes become an f16 tile once, the row tiles pass by.  Warps 0-3 take rows 0-127 of each row
+// tile, warps 4-7 the others; warp 8: TMA, warp 9: MMA.  Two S^T buffers of 256 columns.  Bound by its exponentials (2048 cycles of 32768).
+// The first row that sees token j.
+__device__ __forceinline__ int first_row(const CacheAttnParams& p, const ChunkSeq& s, int j) { return p.causal ? max(0, j - s.n + s.count) * p.rep : 0; }
+
+struct ChunkWeightsCfg {
+  static constexpr int kThreads = 320;
+  static constexpr int kTile = 128 * 128;
+  static constexpr int kQBytes = 4 * kTile;                   // 256 rows: two panels of 256 x 128 bytes
+  static constexpr int kSmemK = 2 * kQBytes;                  // two panels
+  static constexpr int kSmemCode = kSmemK + 2 * kTile;        // two buffers
+  static constexpr int kSmemRows = kSmemCode + 2 * kTile;     // (factor, log2 sum) of the rows, by row tile buffer
+  static constexpr int kSmemSums = kSmemRows + 2 * 256 * 8;
+  static constexpr int kSmemBars = kSmemSums + 128 * 4;
+  static constexpr int kSmem = kSmemBars + 256 + 1024;
+};
+enum ChunkWeightsBar : int { kwCode = 0, kwCodeFree = 2, kwQ = 4, kwQFree = 6, kwS = 8, kwSFree = 10, kwK = 12, kwSums = 13, kwSumsFree = 14, kwBars = 15 };
+
+__global__ void __launch_bounds__(ChunkWeightsCfg::kThreads, 1)
+cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tq, const CacheAttnParams p, const int tiles_of_row) {
+  using C = ChunkWeightsCfg;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kSmemBars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kwBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kwBars + 1);
+  float* sums = reinterpret_cast<float*>(smem + C::kSmemSums);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bars + kwCode + i, 1);
+      mbar_init(bars + kwCodeFree + i, 8);
+      mbar_init(bars + kwQ + i, 1);
+      mbar_init(bars + kwQFree + i, 9);                       // the MMA, and the warps that read the rows' constants
+      mbar_init(bars + kwS + i, 1);
+      mbar_init(bars + kwSFree + i, 8);
+    }
+    mbar_init(bars + kwK, 8);
+    mbar_init(bars + kwSums, 4);
+    mbar_init(bars + kwSumsFree, 4);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tq);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  grid_dep_wait();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  const int R = p.Nq * p.rep, row_tiles_max = (R + 127) / 128;
+  const int64_t items = static_cast<int64_t>(p.c.B) * p.c.Hk * tiles_of_row;
+  bool ok = true;
+  // Item i: a key tile that exists, and its row tiles that see any of it: rt0 ... rt1 - 1, of 256 rows.
+  struct Item {
+    int b, hk, t, n, rt0, rt1;
+    ChunkSeq s;
+  };
+  auto item_at = [&](int64_t i, Item& x) {
+    const int bh = static_cast<int>(i / tiles_of_row);
+    x.t = static_cast<int>(i - static_cast<int64_t>(bh) * tiles_of_row);
+    x.b = bh / p.c.Hk;
+    x.hk = bh - x.b * p.c.Hk;
+    x.s = chunk_seq(p, x.b);
+    x.n = x.s.n;
+    x.rt1 = x.s.units;
+    x.rt0 = min(x.rt1, first_row(p, x.s, 128 * x.t) / 256);
+    return 128 * x.t < x.n;
+  };
+  int g = 0, q = 0;                                           // running item, running row tile
+  Item x;
+  if (warp == 8) {
+    // ------------------------------------------------------------------------------------------ TMA
+    const int bpp = p.c.page / 32;
+    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      if (!item_at(i, x) || x.rt0 >= x.rt1) continue;
+      const int blk = 4 * x.t + lane, entry = blk / bpp;
+      const bool held = lane < 4 && blk * 32 < x.n;
+      const int page = held ? max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + entry))) : 0;
+      if (g >= 2) ok = wait_warp(bar(kwCodeFree + (g & 1)), ((g >> 1) - 1) & 1, abort_flag);
+      if (!ok) break;
+      const int boxes = __popc(__ballot_sync(0xffffffffu, held));
+      if (lane == 0) mbar_expect_tx(bars + kwCode + (g & 1), boxes * 4096);
+      __syncwarp();
+      if (held) tma_load_4d(sbase + C::kSmemCode + (g & 1) * C::kTile + lane * 4096, &tk, bar(kwCode + (g & 1)), 0, (blk - entry * bpp) * 32, x.hk, page);
+      ++g;
+      for (int rt = x.rt0; rt < x.rt1; ++rt, ++q) {
+        if (q >= 2 && !(ok = wait_warp(bar(kwQFree + (q & 1)), ((q >> 1) - 1) & 1, abort_flag))) break;
+        if (lane == 0) {
+          // the last row tile of a head may lack its second half: those columns hold what was there, and its rows see nothing
+          const int tile0 = (x.b * p.c.Hk + x.hk) * row_tiles_max + 2 * rt, halves = min(2, row_tiles_max - 2 * rt);
+          const uint32_t to = (q & 1) * C::kQBytes;
+          mbar_expect_tx(bars + kwQ + (q & 1), halves * (2 * C::kTile + 1024));
+          for (int r = 0; r < halves; ++r) {
+            for (int panel = 0; panel < 2; ++panel)
+              tma_load_2d(smem + to + panel * 2 * C::kTile + r * C::kTile, &tq, bars + kwQ + (q & 1), 128 * panel, (tile0 + r) * 128);
+            bulk_load_1d(smem + C::kSmemRows + (q & 1) * 2048 + r * 1024, p.row_ml + static_cast<int64_t>(tile0 + r) * 128, 1024, bars + kwQ + (q & 1));
+          }
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {
+      if (lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutProducer + kInCache);
+      for (int k = 1; k <= 2; ++k) {                          // what is in flight lands before the shared memory goes
+        if (g >= k) wait_or_abort(bar(kwCode + ((g - k) & 1)), ((g - k) >> 1) & 1, abort_flag);
+        if (q >= k) wait_or_abort(bar(kwQ + ((q - k) & 1)), ((q - k) >> 1) & 1, abort_flag);
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------------------------------ MMA
+    if (elect_one()) {
+      constexpr uint32_t kIdesc = idesc_f8(128, 256, false, false);
+      const uint32_t k_lo = desc_lo(sbase + C::kSmemK), q_lo = desc_lo(sbase);
+      for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+        if (!item_at(i, x) || x.rt0 >= x.rt1) continue;
+        if (!(ok = wait_or_abort(bar(kwK), g & 1, abort_flag))) break;
+        ++g;
+        for (int rt = x.rt0; rt < x.rt1; ++rt, ++q) {
+          if (!(ok = wait_or_abort(bar(kwQ + (q & 1)), (q >> 1) & 1, abort_flag))) break;
+          if (q >= 2 && !(ok = wait_or_abort(bar(kwSFree + (q & 1)), ((q >> 1) - 1) & 1, abort_flag))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_h_ss(tmem + 256 * (q & 1), k_lo + (k >> 2) * (C::kTile >> 4) + (k & 3) * 2,
+                     q_lo + (q & 1) * (C::kQBytes >> 4) + (k >> 2) * (2 * C::kTile >> 4) + (k & 3) * 2, kIdesc, k > 0);
+          tc_commit(bars + kwQFree + (q & 1));
+          tc_commit(bars + kwS + (q & 1));
+        }
+      }
+      if (!ok) raise_abort(abort_flag, p.c.status, kStatusTimeoutMma + kInCache);
+    }
+  } else {
+    // ------------------------------------------------------------------------------------------ codes, exponentials, sums
+    const int half = warp >> 2, key = (warp & 3) * 32 + lane;           // rows of a tile; token of a tile = TMEM lane
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    int it = 0;
+    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x, ++it) {
+      const bool exists = item_at(i, x);
+      float total = 0.f;
+      const int j = 128 * x.t + key;
+      if (exists && x.rt0 < x.rt1) {
+        float ks = 0.f;                                       // of this token's block
+        if (j < x.n) {
+          const int page = max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + j / p.c.page)));
+          ks = __ldg(p.c.ks + page * p.c.s_page + x.hk * p.c.s_head + j % p.c.page / 32);
+        }
+        if (!(ok = wait_warp(bar(kwCode + (g & 1)), (g >> 1) & 1, abort_flag))) break;
+        {
+          // as in the main kernel: 16-byte pieces c of keys tid / 8, + 32, ...; the f16 tile is free, all its products having been seen
+          const int c = tid & 7, panel = c >> 2, cc = (c & 3) * 2;
+          const uint32_t src = sbase + C::kSmemCode + (g & 1) * C::kTile, dst = sbase + C::kSmemK + panel * C::kTile;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = (tid >> 3) + 32 * k;
+            const float4 w4 = lds_f4(src + row * 128 + ((c ^ (row & 7)) << 4));
+            const uint32_t w[4] = {__float_as_uint(w4.x), __float_as_uint(w4.y), __float_as_uint(w4.z), __float_as_uint(w4.w)};
+            uint32_t h[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              h[2 * e] = e4m3_lo_f16x2(w[e]);
+              h[2 * e + 1] = e4m3_hi_f16x2(w[e]);
+            }
+            const int flip = panel;                           // which half first: eight lanes' stores on different banks
+            sts_u4(dst + row * 128 + (((cc + flip) ^ (row & 7)) << 4), flip ? h[4] : h[0], flip ? h[5] : h[1], flip ? h[6] : h[2], flip ? h[7] : h[3]);
+            sts_u4(dst + row * 128 + (((cc + 1 - flip) ^ (row & 7)) << 4), flip ? h[0] : h[4], flip ? h[1] : h[5], flip ? h[2] : h[6], flip ? h[3] : h[7]);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bars + kwCodeFree + (g & 1));
+            mbar_arrive(bars + kwK);
+          }
+        }
+        ++g;
+        for (int rt = x.rt0; rt < x.rt1; ++rt, ++q) {
+          // the products; and the rows' constants, seen by this warp itself
+          if (!(ok = wait_warp(bar(kwS + (q & 1)), (q >> 1) & 1, abort_flag) && wait_warp(bar(kwQ + (q & 1)), (q >> 1) & 1, abort_flag))) break;
+          tc_fence_after();
+          const int row0 = rt * 256 + half * 128;
+          if (row0 < x.s.count * p.rep) {
+            const int from_row = first_row(p, x.s, j) - row0;                 // of mine, the first that sees this token
+            const bool cut = __any_sync(0xffffffffu, from_row > 0);
+            const uint32_t from = tmem + lanes + 256 * (q & 1) + 128 * half, rows = sbase + C::kSmemRows + (q & 1) * 2048 + half * 1024;
+            uint32_t s_buf[2][32];
+            tmem_ld32(from, s_buf[0]);
+#pragma unroll 1
+            for (int c2 = 0; c2 < 2; ++c2) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                tmem_wait_ld();
+                if (!(c2 == 1 && k == 1)) tmem_ld32(from + 64 * c2 + 32 * (k + 1), s_buf[k ^ 1]);
+                float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const float4 fc = lds_f4(rows + (64 * c2 + 32 * k + 2 * e) * 8);        // factor and log2 sum of two rows
+                  float2 y = fma2(mul2(make_float2(__uint_as_float(s_buf[k][2 * e]), __uint_as_float(s_buf[k][2 * e + 1])), make_float2(fc.x, fc.z)), splat2(ks),
+                                  make_float2(-fc.y, -fc.w));
+                  if (cut) {
+                    if (64 * c2 + 32 * k + 2 * e < from_row) y.x = -CUDART_INF_F;
+                    if (64 * c2 + 32 * k + 2 * e + 1 < from_row) y.y = -CUDART_INF_F;
+                  }
+                  sum = add2(sum, ex2_2(y));
+                }
+                total += sum.x + sum.y;
+              }
+            }
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bars + kwSFree + (q & 1));
+            mbar_arrive(bars + kwQFree + (q & 1));
+          }
+        }
+        if (!ok) break;
+      }
+      // the two halves' sums, and zeros beyond the length
+      if (half == 1) {
+        if (it > 0 && !(ok = wait_warp(bar(kwSumsFree), (it - 1) & 1, abort_flag))) break;
+        sums[key] = total;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kwSums);
+      } else {
+        if (!(ok = wait_warp(bar(kwSums), it & 1, abort_flag))) break;
+        total += sums[key];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kwSumsFree);
+        if (j < p.W) {
+          float* at = p.weights + x.b * p.w_sb + x.hk * p.w_sh + j;
+          if (j < x.n) *at = p.accumulate ? *at + total : total;
+          else if (!p.accumulate) *at = 0.f;
+        }
+      }
+    }
+    if (!ok && lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -777,6 +1035,7 @@ cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, con
     if (e != cudaSuccess) return e;
     if (attr.numRegs * C::kThreads < 256 * (C::kRegsSoftmax + C::kRegsOther)) return cudaErrorLaunchOutOfResources;
     e = cudaFuncSetAttribute(cache_chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(cache_chunk_weights_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkWeightsCfg::kSmem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
@@ -789,7 +1048,13 @@ cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, con
   if (e != cudaSuccess) return e;
   count_launch();
   const int groups = (p.Nq * p.rep + 7) / 8;
-  return launch_chained(cache_chunk_join_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * groups), 128, 0, stream, p);
+  e = launch_chained(cache_chunk_join_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * groups), 128, 0, stream, p);
+  if (e != cudaSuccess || p.weights == nullptr) return e;
+  const int tiles_of_row = (p.W + 127) / 128;                 // what lies beyond the length too: its weights are zeros
+  const int64_t items = static_cast<int64_t>(p.c.B) * p.c.Hk * tiles_of_row;
+  count_launch();
+  return launch_chained(cache_chunk_weights_kernel, dim3(static_cast<unsigned>(items < sm_count() ? items : sm_count())), ChunkWeightsCfg::kThreads,
+                        ChunkWeightsCfg::kSmem, stream, tk, tq, p, tiles_of_row);
 }
 
 }  // namespace dm
