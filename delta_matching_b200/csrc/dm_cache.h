@@ -63,6 +63,7 @@ struct CacheAttnParams {
   int accumulate;
   int grid;                         // CTAs of the main kernel
   int cluster;                      // of a unit, or 0: the even division
+  int unit_shift;                   // log2 of the rows of a unit of the form for many rows
 };
 
 struct CacheEvictParams {
@@ -80,7 +81,7 @@ struct CacheEvictParams {
 
 // Slots of partial results and their sizes for a call of dm_cache_attn.
 struct CacheAttnPlan {
-  bool chunk;                       // dm_cache_chunk.cu: head_dim 128 and many rows
+  bool chunk;                       // dm_cache_chunk.cu: many rows
   int row_tile;                     // query rows (new tokens x heads of a group) a CTA keeps
   int row_tiles;
   int grid;
@@ -94,10 +95,10 @@ cudaError_t launch_cache_append(int D, const CacheAppendParams& p, cudaStream_t 
 // tq: p.q16 as 64 x 128 boxes, for the form for many rows.
 cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream);
 // The form for many rows (its partial results: 2 slots a CTA), and what a row tile of it holds.
-cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream);
-int cache_chunk_rows();
+cudaError_t launch_cache_chunk(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream);
+int cache_chunk_rows(int D);
 int64_t cache_chunk_start_bytes();                           // of a CTA's start
-int64_t cache_chunk_query_rows(int B, int Hk, int R);         // rows of 128 f16 values
+int64_t cache_chunk_query_rows(int B, int Hk, int R);         // rows of D f16 values
 cudaError_t launch_cache_evict(int D, const CacheEvictParams& p, cudaStream_t stream);
 
 }  // namespace dm

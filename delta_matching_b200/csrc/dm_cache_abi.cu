@@ -156,11 +156,12 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   p.w_sb = w_sb; p.w_sh = w_sh; p.W = W; p.accumulate = accumulate ? 1 : 0;
   p.grid = x.grid;
   p.cluster = x.cluster;
+  for (p.unit_shift = 0; 1 << p.unit_shift < x.row_tile;) ++p.unit_shift;
   CUtensorMap tk, tv, tq{};
   DM_TRY(pool_map(&tk, cache, cache->k8));
   DM_TRY(pool_map(&tv, cache, cache->v8));
   if (x.chunk) {                                              // f16 rows as bytes: boxes of 64 values x 128 rows
-    const cuuint64_t dims[2] = {256, static_cast<cuuint64_t>(x.q16_bytes / 256)}, strides[1] = {256};
+    const cuuint64_t row = 2ull * cache->head_dim, dims[2] = {row, static_cast<cuuint64_t>(x.q16_bytes) / row}, strides[1] = {row};
     const cuuint32_t box[2] = {128, 128};
     DM_TRY(encode_byte_map(&tq, p.q16, 2, dims, strides, box));
   }

@@ -899,7 +899,7 @@ cudaError_t launch_weights(const CUtensorMap& tk, const CacheAttnParams& p, cuda
                         (p.Nq * p.rep + 8 * NT - 1) / (8 * NT));
 }
 
-// Rows (new tokens x heads of a group) from which the tcgen05 form is taken, at head_dim 128.
+// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.
 constexpr int kChunkFrom = 33;
 constexpr int kClusterBlocks = 8;
 int small_row_tile(int D, int R) { return R <= 8 ? 8 : R <= 16 || D == 256 ? 16 : 32; }
@@ -909,8 +909,8 @@ int small_row_tile(int D, int R) { return R <= 8 ? 8 : R <= 16 || D == 256 ? 16 
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights) {
   CacheAttnPlan x;
   const int R = Nq * (H / Hk);
-  x.chunk = D == 128 && R >= kChunkFrom;
-  x.row_tile = x.chunk ? cache_chunk_rows() : small_row_tile(D, R);
+  x.chunk = R >= kChunkFrom;
+  x.row_tile = x.chunk ? cache_chunk_rows(D) : small_row_tile(D, R);
   x.row_tiles = (R + x.row_tile - 1) / x.row_tile;
   const int64_t blocks = static_cast<int64_t>(T) * (page / 32), units = static_cast<int64_t>(B) * Hk * x.row_tiles;       // of a sequence; in all
   const int ctas = x.chunk ? 1 : D == 128 && x.row_tile == 8 ? AttnCfg<128, 1>::kCtasPerSm : AttnCfg<128, 2>::kCtasPerSm;
@@ -941,15 +941,15 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
 
 cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
   const int R = p.Nq * p.rep, tile = small_row_tile(D, R), row_tiles = (R + tile - 1) / tile;
+  if (R >= kChunkFrom) return launch_cache_chunk(D, tk, tv, tq, p, stream);
   cudaError_t e;
   if (D == 128) {
-    e = R >= kChunkFrom ? launch_cache_chunk(tk, tv, tq, p, stream)
-      : tile == 8 ? launch_main<128, 1>(tk, tv, p, row_tiles, stream)
+    e = tile == 8 ? launch_main<128, 1>(tk, tv, p, row_tiles, stream)
       : tile == 16 ? launch_main<128, 2>(tk, tv, p, row_tiles, stream) : launch_main<128, 4>(tk, tv, p, row_tiles, stream);
   } else {
     e = tile == 8 ? launch_main<256, 1>(tk, tv, p, row_tiles, stream) : launch_main<256, 2>(tk, tv, p, row_tiles, stream);
   }
-  if (e != cudaSuccess || p.weights == nullptr || (D == 128 && R >= kChunkFrom)) return e;
+  if (e != cudaSuccess || p.weights == nullptr) return e;
   if (p.logits != nullptr) {
     const int pieces = (p.W + 255) / 256;
     count_launch();

@@ -28,21 +28,30 @@ constexpr int kSplitFrom = 10;
 constexpr int kPBase = 12;                  // log2 of P at the reference maximum,
 constexpr float kHeadroom = 3.9f;           // and what a row may exceed it by: P stays below 2^16
 
+// D = 256: as D = 128, but one row tile, whose two softmax groups take half of the keys each, and O of 256 columns.
+template <int kD>
 struct ChunkCfg {
-  static constexpr int D = 128;
+  static constexpr int D = kD;
+  static constexpr bool kWide = D == 256;
   static constexpr int kThreads = 512;                        // four warpgroups
   static constexpr int kRegsSoftmax = 168, kRegsOther = 88;
   static_assert(256 * kRegsSoftmax + 256 * kRegsOther <= kThreads * 128, "a split above the launch's own registers would wait for ever");
-  static constexpr int kRows = 256;
-  static constexpr int kTile = 128 * 128;                     // a code tile; also a 64-column f16 panel of 128 rows
-  static constexpr int kSmemQ = 0;                            // two row tiles x two panels
-  static constexpr int kSmemK = 4 * kTile;                    // two panels: between the uses of two tiles lies a softmax, longer than a conversion
-  static constexpr int kSmemV = kSmemK + 2 * kTile;           // two buffers x two panels
-  static constexpr int kSmemCode = kSmemV + 4 * kTile;        // K codes, V codes
-  static constexpr int kSmemOut = kSmemCode + 2 * kTile;      // output staging: 4 KB a softmax warp
-  static constexpr int kSmemBars = kSmemOut + 2 * kTile;
-  static constexpr int kSmemScales = kSmemBars + 256;         // 8 tiles x (4 K scales, 4 V scales)
-  static constexpr int kSmem = kSmemScales + 8 * 32 + 1024;
+  static constexpr int kRows = kWide ? 128 : 256;
+  static constexpr int kPanels = D / 64;                      // of 64 columns, of an f16 operand tile
+  static constexpr int kCols = kWide ? 64 : 128;              // keys of a tile that a softmax group looks after
+  static constexpr int kTile = 128 * 128;                     // 128 keys x 128 codes; also an f16 panel of 128 rows
+  static constexpr int kChunks = 2 * D / 128;                 // pieces of kTile in which the codes of a key tile come: K, then V
+  static constexpr int kVBufs = kWide ? 1 : 2;
+  static constexpr int kSmemQ = 0;                            // row tiles x panels
+  static constexpr int kSmemK = 4 * kTile;                    // between the uses of two tiles lies a softmax, longer than a conversion
+  static constexpr int kSmemV = kSmemK + kPanels * kTile;
+  static constexpr int kSmemCode = kSmemV + 4 * kTile;        // two pieces
+  // output staging, 4 KB a softmax warp: with 256 columns over the queries, which then wait for it
+  static constexpr int kSmemOut = kWide ? kSmemQ : kSmemCode + 2 * kTile;
+  static constexpr int kSmemBars = kSmemCode + (kWide ? 2 : 4) * kTile;
+  static constexpr int kSmemScales = kSmemBars + 320;         // 8 tiles x (4 K scales, 4 V scales)
+  static constexpr int kSmemRows = kSmemScales + 8 * 32;      // what the two groups tell each other of their rows
+  static constexpr int kSmem = kSmemRows + (kWide ? 1024 : 0) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -55,7 +64,7 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const CacheAttnParams& p, int b) {
   ChunkSeq s;
   s.n = cache_length(p.c, b);
   s.count = checked_count(p.c.status, p.counts, b, p.Nq);
-  s.units = (s.count * p.rep + ChunkCfg::kRows - 1) / ChunkCfg::kRows;
+  s.units = (s.count * p.rep + (1 << p.unit_shift) - 1) >> p.unit_shift;
   return s;
 }
 // Keys that row r of the sequence sees.
@@ -64,7 +73,7 @@ __device__ __forceinline__ int row_limit(const CacheAttnParams& p, const ChunkSe
   return i >= s.count ? 0 : p.causal ? max(0, s.n - s.count + i + 1) : s.n;
 }
 __device__ __forceinline__ int unit_tiles(const CacheAttnParams& p, const ChunkSeq& s, int rt) {
-  return (row_limit(p, s, min(s.count * p.rep, (rt + 1) * ChunkCfg::kRows) - 1) + 127) / 128;
+  return (row_limit(p, s, min(s.count * p.rep, (rt + 1) << p.unit_shift) - 1) + 127) / 128;
 }
 __device__ __forceinline__ int unit_steps(const CacheAttnParams& p, const ChunkSeq& s, int rt) {
   const int tiles = unit_tiles(p, s, rt);
@@ -100,9 +109,9 @@ struct ChunkPiece {
   int b, hk, rt;
   ChunkSeq s;
   int tiles, t0, t1, f1;
-  // Softmax groups at work: both, except that a short piece of a unit of one row tile has one.
+  // Softmax groups at work (head_dim 128): both, except that a short piece of a unit of one row tile has one.
   // A long piece of such a unit is split: its key tiles go to the two groups in turn, each with a result of its own for the join.
-  __device__ __forceinline__ bool one_tile(const CacheAttnParams& p) const { return s.count * p.rep - rt * ChunkCfg::kRows <= 128; }
+  __device__ __forceinline__ bool one_tile(const CacheAttnParams& p) const { return p.unit_shift == 8 && s.count * p.rep - (rt << 8) <= 128; }
   __device__ __forceinline__ bool split(const CacheAttnParams& p) const { return one_tile(p) && t1 - t0 >= kSplitFrom; }
   __device__ __forceinline__ int groups(const CacheAttnParams& p) const { return one_tile(p) && t1 - t0 < kSplitFrom ? 1 : 2; }
 };
@@ -205,24 +214,27 @@ enum ChunkBar : int {
   kCodeFull = 0, kCodeEmpty = 2,            // K codes, V codes
   kKFull = 4, kKEmpty = 5,
   kVFull = 6, kVEmpty = 8,                  // by parity of the running tile
-  kQFull = 10, kQFree = 12, kSFull = 14, kPHalf = 16, kPFull = 18, kPvDone = 20,      // by row tile
+  kQFull = 10, kQFree = 12, kSFull = 14, kPHalf = 16, kPFull = 18, kPvDone = 20,      // by row tile; kSFull and kPFull of 256 columns by tile
   kScales = 22,                             // of running tile g: entry g % 8 (the loads are at most four tiles ahead of the softmax)
-  kBars = 30,
+  kVote = 30, kTell = 32,                   // 256 columns: a row's maximum has moved; maxima and sums lie ready
+  kBars = 33,                               // behind them the TMEM slot, the abort flag and two words of votes
 };
 
 // ------------------------------------------------------------------------------------------------ queries
 // q (bf16, any strides) -> f16 rows with a power of two per row, in the order of the row tiles (b, kv head, new token, head of the group; rows
-// of a head filled up to whole tiles with zeros), and the factor of each row's logits.  Sixteen lanes a row.  In the main kernel this took
+// of a head filled up to whole tiles with zeros), and the factor of each row's logits.  Eight elements a lane.  In the main kernel this took
 // its softmax warps 7000 cycles a unit, and a warp of its own 40000 and more.  The first CTA makes the division of the tiles instead.
+template <int D>
 __global__ void __launch_bounds__(256) cache_chunk_queries_kernel(const CacheAttnParams p) {
+  constexpr int kLanes = D / 8;
   __shared__ int cum[136];
   grid_dep_wait();
   if (blockIdx.x == 0) {
     chunk_starts(p, cum);
     return;
   }
-  const int lane = threadIdx.x & 15, R = p.Nq * p.rep, padded = (R + 127) / 128 * 128;
-  const int64_t row = static_cast<int64_t>(blockIdx.x - 1) * 16 + (threadIdx.x >> 4);       // the grid is whole tiles
+  const int lane = threadIdx.x & (kLanes - 1), R = p.Nq * p.rep, padded = (R + 127) / 128 * 128;
+  const int64_t row = static_cast<int64_t>(blockIdx.x - 1) * (256 / kLanes) + threadIdx.x / kLanes;       // the grid is whole tiles
   const int bh = static_cast<int>(row / padded), r = static_cast<int>(row - static_cast<int64_t>(bh) * padded), b = bh / p.c.Hk, hk = bh - b * p.c.Hk;
   const int tok = r / p.rep, head = hk * p.rep + r - tok * p.rep;
   uint4 w = make_uint4(0, 0, 0, 0);
@@ -232,13 +244,13 @@ __global__ void __launch_bounds__(256) cache_chunk_queries_kernel(const CacheAtt
 #pragma unroll
   for (int j = 0; j < 4; ++j) amax = max3(amax, fabsf(__uint_as_float(v[j] << 16)), fabsf(__uint_as_float(v[j] & 0xFFFF0000u)));
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   const uint32_t eb = min(254u, max(14u, __float_as_uint(amax) >> 23));
   const float up = sb_to_scale(267u - eb);                    // largest element to [2^13, 2^14)
   uint32_t h[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) h[j] = pack_f16x2(__uint_as_float(v[j] << 16) * up, __uint_as_float(v[j] & 0xFFFF0000u) * up);
-  reinterpret_cast<uint4*>(p.q16 + row * ChunkCfg::D)[lane] = make_uint4(h[0], h[1], h[2], h[3]);
+  reinterpret_cast<uint4*>(p.q16 + row * D)[lane] = make_uint4(h[0], h[1], h[2], h[3]);
   if (lane == 0) {
     const float f = sb_to_scale(eb - 13u) * p.scale * kLog2e;
     p.factors[row] = f;
@@ -247,10 +259,11 @@ __global__ void __launch_bounds__(256) cache_chunk_queries_kernel(const CacheAtt
 }
 
 // ------------------------------------------------------------------------------------------------ main kernel
-__global__ void __launch_bounds__(ChunkCfg::kThreads, 1)
+template <int kD>
+__global__ void __launch_bounds__(ChunkCfg<kD>::kThreads, 1)
 cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tq,
                    const CacheAttnParams p) {
-  using C = ChunkCfg;
+  using C = ChunkCfg<kD>;
   constexpr int D = C::D;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -269,14 +282,16 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       mbar_init(bars + kVFull + i, 4);
       mbar_init(bars + kVEmpty + i, 1);
       mbar_init(bars + kQFull + i, 1);
-      mbar_init(bars + kQFree + i, 1);
+      mbar_init(bars + kQFree + i, C::kWide ? 8 : 1);
       mbar_init(bars + kSFull + i, 1);
       mbar_init(bars + kPHalf + i, 4);
-      mbar_init(bars + kPFull + i, 4);
+      mbar_init(bars + kPFull + i, C::kWide ? 8 : 4);
       mbar_init(bars + kPvDone + i, 1);
+      mbar_init(bars + kVote + i, 8);
     }
     mbar_init(bars + kKFull, 4);
     mbar_init(bars + kKEmpty, 1);
+    mbar_init(bars + kTell, 8);
     for (int i = 0; i < 8; ++i) mbar_init(bars + kScales + i, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -341,19 +356,21 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         a.ks = __ldg(p.c.ks + at);
         a.vs = __ldg(p.c.vs + at);
       };
-      int g = 0;                                              // running tile
+      int g = 0, j = 0;                                       // running tile, running piece of codes
       Ahead now = look_up(), next = look_up();
       ask_scales(now);
       for (; now.live; ++g) {
         const Ahead after = look_up();
         ask_scales(next);
         const int boxes = __popc(__ballot_sync(0xffffffffu, now.held));
-        for (int kv = 0; kv < 2; ++kv) {
-          if (g > 0) ok = ok && wait_warp(bar(kCodeEmpty + kv), (g - 1) & 1, abort_flag);
+        for (int c = 0; c < C::kChunks; ++c, ++j) {
+          const int buf = j & 1, x0 = C::kWide ? (c & 1) * 128 : 0;
+          if (j >= 2) ok = ok && wait_warp(bar(kCodeEmpty + buf), ((j >> 1) - 1) & 1, abort_flag);
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(bars + kCodeFull + kv, boxes * 4096);
+          if (lane == 0) mbar_expect_tx(bars + kCodeFull + buf, boxes * 4096);
           __syncwarp();
-          if (now.held) tma_load_4d(sbase + C::kSmemCode + kv * C::kTile + lane * 4096, kv ? &tv : &tk, bar(kCodeFull + kv), 0, now.sub * 32, now.hk, now.page);
+          if (now.held)
+            tma_load_4d(sbase + C::kSmemCode + buf * C::kTile + lane * 4096, 2 * c >= C::kChunks ? &tv : &tk, bar(kCodeFull + buf), x0, now.sub * 32, now.hk, now.page);
         }
         if (!ok) break;
         if (lane < 4) {
@@ -368,64 +385,92 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       if (!ok) {
         if (lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutProducer + kInCache);
         // what is in flight lands before the shared memory goes
-        for (int kv = 0; kv < 2; ++kv)
-          if (g > 0) wait_or_abort(bar(kCodeFull + kv), (g - 1) & 1, abort_flag);
+        for (int k = 1; k <= 2; ++k)
+          if (j >= k) wait_or_abort(bar(kCodeFull + ((j - k) & 1)), ((j - k) >> 1) & 1, abort_flag);
       }
     } else if (warp == 13) {
       // ---------------------------------------------------------------------------------------- MMA
       if (elect_one()) {
-        constexpr uint32_t kIdescS = idesc_f8(128, 128, false, false), kIdescO = idesc_f8(128, 128, false, true);
+        constexpr uint32_t kIdescS = idesc_f8(128, 128, false, false), kIdescO = idesc_f8(128, D, false, true);
         const uint32_t q_lo = desc_lo(sbase + C::kSmemQ), k_lo = desc_lo(sbase + C::kSmemK);
         // V's panels of 64 columns lie kTile apart: the leading offset of an operand wider than 128 bytes
         const uint32_t v_lo = (((sbase + C::kSmemV) & 0x3FFFFu) >> 4) | (static_cast<uint32_t>(C::kTile >> 4) << 16);
-        int g = 0, tiles[2] = {0, 0}, units[2] = {0, 0};      // running tile; tiles and units of each row tile
+        int g = 0;                                            // running tile
+        // S of a row tile, or (256 columns) into S buffer r
         auto issue_s = [&](int r, bool last) {
-          const uint32_t a = q_lo + r * (2 * C::kTile >> 4), b = k_lo;
+          const uint32_t a = q_lo + (C::kWide ? 0 : r * (2 * C::kTile >> 4)), b = k_lo;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = (k >> 2) * (C::kTile >> 4) + (k & 3) * 2;
             mma_h_ss(tmem + 128 * r, a + off, b + off, kIdescS, k > 0);
           }
           if (last) tc_commit(bars + kKEmpty);
           tc_commit(bars + kSFull + r);
         };
-        do {
-          if (x.t0 >= x.t1) continue;
-          // both groups work on every key tile, or (split) each on every second one
-          const bool split = x.split(p);
-          const int step = split ? 2 : 1, n = x.t1 - x.t0, groups = x.groups(p);
-          for (int r = 0; r < groups; ++r) {
-            if ((r == 0 || split) && !(ok = wait_or_abort(bar(kKFull), (g + (split ? r : 0)) & 1, abort_flag))) break;
-            if (!(ok = wait_or_abort(bar(kQFull + r), units[r]++ & 1, abort_flag))) break;
+        if constexpr (C::kWide) {
+          int units = 0;
+          do {
+            if (x.t0 >= x.t1) continue;
+            const int n = x.t1 - x.t0;
+            if (!(ok = wait_or_abort(bar(kQFull), units++ & 1, abort_flag) && wait_or_abort(bar(kKFull), g & 1, abort_flag))) break;
             tc_fence_after();
-            issue_s(r, split || r == groups - 1);
-            if ((split ? r : 0) + step >= n) tc_commit(bars + kQFree + r);      // the group's last S of the unit
-          }
-          for (int i = 0; i < n && ok; ++i, ++g) {
-            for (int r = split ? i & 1 : 0; r < groups; r += step) {
-              // 16 keys a step: 8 columns of P, 16 rows of V; the first half of the keys while the softmax is at the second
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                if (!(ok = wait_or_abort(bar((half == 0 ? kPHalf : kPFull) + r), tiles[r] & 1, abort_flag))) break;
-                if ((r == 0 || split) && half == 0 && !(ok = wait_or_abort(bar(kVFull + (g & 1)), (g >> 1) & 1, abort_flag))) break;
+            issue_s(g & 1, true);
+            for (int i = 0; i < n && ok; ++i, ++g) {
+              if (i + 1 < n) {                                // the next S, while the softmax is at this one
+                if (!(ok = wait_or_abort(bar(kKFull), (g + 1) & 1, abort_flag))) break;
                 tc_fence_after();
-#pragma unroll
-                for (int k = 4 * half; k < 4 * half + 4; ++k)
-                  mma_h_ts(tmem + 256 + 128 * r, tmem + 128 * r + 8 * k, v_lo + (g & 1) * (2 * C::kTile >> 4) + k * (2048 >> 4), kIdescO, i >= step || k > 0);
+                issue_s((g + 1) & 1, true);
               }
-              if (!ok) break;
-              ++tiles[r];
-              if (split || r == groups - 1) tc_commit(bars + kVEmpty + (g & 1));
-              tc_commit(bars + kPvDone + r);
-              if (i + step < n) {
-                if ((r == 0 || split) && !(ok = wait_or_abort(bar(kKFull), (g + step) & 1, abort_flag))) break;
-                tc_fence_after();
-                issue_s(r, split || r == groups - 1);
-                if (i + 2 * step >= n) tc_commit(bars + kQFree + r);
+              // both groups' P before any product: both may have rescaled O
+              if (!(ok = wait_or_abort(bar(kPFull + (g & 1)), (g >> 1) & 1, abort_flag) && wait_or_abort(bar(kVFull), g & 1, abort_flag))) break;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                mma_h_ts(tmem + 256, tmem + 128 * (g & 1) + 64 * (k >> 2) + 8 * (k & 3), v_lo + k * (2048 >> 4), kIdescO, i > 0 || k > 0);
+              tc_commit(bars + kVEmpty);
+              tc_commit(bars + kPvDone);
+            }
+          } while (ok && next_chunk(p, x, f_end));
+        } else {
+          int tiles[2] = {0, 0}, units[2] = {0, 0};           // tiles and units of each row tile
+          do {
+            if (x.t0 >= x.t1) continue;
+            // both groups work on every key tile, or (split) each on every second one
+            const bool split = x.split(p);
+            const int step = split ? 2 : 1, n = x.t1 - x.t0, groups = x.groups(p);
+            for (int r = 0; r < groups; ++r) {
+              if ((r == 0 || split) && !(ok = wait_or_abort(bar(kKFull), (g + (split ? r : 0)) & 1, abort_flag))) break;
+              if (!(ok = wait_or_abort(bar(kQFull + r), units[r]++ & 1, abort_flag))) break;
+              tc_fence_after();
+              issue_s(r, split || r == groups - 1);
+              if ((split ? r : 0) + step >= n) tc_commit(bars + kQFree + r);      // the group's last S of the unit
+            }
+            for (int i = 0; i < n && ok; ++i, ++g) {
+              for (int r = split ? i & 1 : 0; r < groups; r += step) {
+                // 16 keys a step: 8 columns of P, 16 rows of V; the first half of the keys while the softmax is at the second
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  if (!(ok = wait_or_abort(bar((half == 0 ? kPHalf : kPFull) + r), tiles[r] & 1, abort_flag))) break;
+                  if ((r == 0 || split) && half == 0 && !(ok = wait_or_abort(bar(kVFull + (g & 1)), (g >> 1) & 1, abort_flag))) break;
+                  tc_fence_after();
+#pragma unroll
+                  for (int k = 4 * half; k < 4 * half + 4; ++k)
+                    mma_h_ts(tmem + 256 + 128 * r, tmem + 128 * r + 8 * k, v_lo + (g & 1) * (2 * C::kTile >> 4) + k * (2048 >> 4), kIdescO, i >= step || k > 0);
+                }
+                if (!ok) break;
+                ++tiles[r];
+                if (split || r == groups - 1) tc_commit(bars + kVEmpty + (g & 1));
+                tc_commit(bars + kPvDone + r);
+                if (i + step < n) {
+                  if ((r == 0 || split) && !(ok = wait_or_abort(bar(kKFull), (g + step) & 1, abort_flag))) break;
+                  tc_fence_after();
+                  issue_s(r, split || r == groups - 1);
+                  if (i + 2 * step >= n) tc_commit(bars + kQFree + r);
+                }
               }
             }
-          }
-        } while (ok && next_chunk(p, x, f_end));
+          } while (ok && next_chunk(p, x, f_end));
+        }
         if (!ok) raise_abort(abort_flag, p.c.status, kStatusTimeoutMma + kInCache);
       }
     } else if (warp == 14) {
@@ -436,13 +481,13 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         do {
           if (x.t0 >= x.t1) continue;
           const bool split = x.split(p);
-          for (int r = 0; r < x.groups(p) && ok; ++r) {
+          for (int r = 0; r < (C::kWide ? 1 : x.groups(p)) && ok; ++r) {
             if (units[r] > 0) ok = wait_or_abort(bar(kQFree + r), (units[r] - 1) & 1, abort_flag);
             if (!ok) break;
             ++units[r];
-            mbar_expect_tx(bars + kQFull + r, 2 * C::kTile);
-            const int row = ((x.b * p.c.Hk + x.hk) * tiles_of_head + 2 * x.rt + (split ? 0 : r)) * 128;
-            for (int panel = 0; panel < 2; ++panel)
+            mbar_expect_tx(bars + kQFull + r, C::kPanels * C::kTile);
+            const int row = ((x.b * p.c.Hk + x.hk) * tiles_of_head + (C::kWide ? x.rt : 2 * x.rt + (split ? 0 : r))) * 128;
+            for (int panel = 0; panel < C::kPanels; ++panel)
               tma_load_2d(smem + C::kSmemQ + (2 * r + panel) * C::kTile, &tq, bars + kQFull + r, 128 * panel, row);        // x in bytes
           }
         } while (ok && next_chunk(p, x, f_end));
@@ -458,17 +503,19 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const int ct = tid - 256, c = ct & 7;                   // a thread takes 16-byte pieces c of keys ct / 8, + 16, ...
       // a piece's two halves of eight elements: which goes first is chosen so that the stores of eight lanes fall on different banks
       const int panel = c >> 2, flip = panel;
-      int g = 0;
+      int g = 0, j = 0;                                       // running tile, running piece of codes
       do {
         for (int t = x.t0; t < x.t1 && ok; ++t, ++g) {
 #pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv) {
-            ok = wait_warp(bar(kCodeFull + kv), g & 1, abort_flag);
-            if (ok && kv == 0 && g >= 1) ok = wait_warp(bar(kKEmpty), (g - 1) & 1, abort_flag);
-            if (ok && kv == 1 && g >= 2) ok = wait_warp(bar(kVEmpty + (g & 1)), ((g >> 1) - 1) & 1, abort_flag);
+          for (int part = 0; part < C::kChunks; ++part, ++j) {
+            const bool kv = 2 * part >= C::kChunks, first = 2 * part % C::kChunks == 0;      // V; the first piece of K or V
+            const int side = C::kWide ? part & 1 : 0, vbuf = C::kVBufs == 2 ? g & 1 : 0;
+            ok = wait_warp(bar(kCodeFull + (j & 1)), (j >> 1) & 1, abort_flag);
+            if (ok && first && !kv && g >= 1) ok = wait_warp(bar(kKEmpty), (g - 1) & 1, abort_flag);
+            if (ok && first && kv && g >= C::kVBufs) ok = wait_warp(bar(kVEmpty + vbuf), (g / C::kVBufs - 1) & 1, abort_flag);
             if (!ok) break;
-            const uint32_t src = sbase + C::kSmemCode + kv * C::kTile;
-            const uint32_t dst = sbase + (kv ? C::kSmemV + (g & 1) * 2 * C::kTile : C::kSmemK) + panel * C::kTile;
+            const uint32_t src = sbase + C::kSmemCode + (j & 1) * C::kTile;
+            const uint32_t dst = sbase + (kv ? C::kSmemV + vbuf * C::kPanels * C::kTile : C::kSmemK) + (2 * side + panel) * C::kTile;
             const int held = kv ? x.s.n - 128 * t : 128;      // V's slots beyond the length hold anything, NaN codes too: zeros
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -496,8 +543,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              mbar_arrive(bars + (kv ? kVFull + (g & 1) : kKFull));
-              mbar_arrive(bars + kCodeEmpty + kv);
+              if (2 * (part + 1) % C::kChunks == 0) mbar_arrive(bars + (kv ? kVFull + vbuf : kKFull));
+              mbar_arrive(bars + kCodeEmpty + (j & 1));
             }
           }
         }
@@ -508,42 +555,53 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       // ---------------------------------------------------------------------------------------- softmax and output
       const int r = warp >> 2, in_tile = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t t_s = tmem + lanes + 128 * r, t_o = tmem + lanes + 256 + 128 * r;
+      const uint32_t t_o = tmem + lanes + 256 + 128 * r;      // of 256 columns, the half that this group rescales and writes
+      volatile float* told = reinterpret_cast<volatile float*>(smem + C::kSmemRows) + in_tile;        // by group 0 of this row; by group 1 128 values on
       const uint32_t stage = sbase + C::kSmemOut + warp * 4096;
-      int g = 0, mine = 0;                                    // running tile; tiles of this row tile
+      int g = 0, mine = 0, tells = 0;                         // running tile; tiles of this row tile; times the groups have told each other
       int slot = 2 * cta;
       do {
         if (x.t0 >= x.t1) continue;
         const bool split = x.split(p);
         const int step = split ? 2 : 1, first = x.t0 + (split ? r : 0);       // this group's key tiles
-        if (r >= x.groups(p)) {                               // none: a result of nothing
+        if (!C::kWide && r >= x.groups(p)) {                  // none: a result of nothing
           p.part_ml[static_cast<int64_t>(slot) * C::kRows + r * 128 + in_tile] = make_float2(-CUDART_INF_F, 0.f);
           g += x.t1 - x.t0;
           slot = 2 * cta + 1;
           continue;
         }
-        const int row = x.rt * C::kRows + (split ? 0 : r * 128) + in_tile, limit = row_limit(p, x.s, row);
+        const int row = x.rt * C::kRows + (C::kWide || split ? 0 : r * 128) + in_tile, limit = row_limit(p, x.s, row);
         const int i_tok = row / p.rep, head = x.hk * p.rep + row - i_tok * p.rep;
         // of the row's logits, K's scale aside
         const int64_t padded_row = (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + 127) / 128 * 128) + row;
         const float f = __ldg(p.factors + padded_row);
         float m = -CUDART_INF_F, l = 0.f;
         int vexp = -1000;
+        // What the two groups know of a row (256 columns): the other's value.
+        auto tell = [&](float mine_v, float& other) -> bool {
+          told[128 * r] = mine_v;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + kTell);
+          if (!wait_warp(bar(kTell), tells++ & 1, abort_flag)) return false;
+          other = told[128 * (r ^ 1)];
+          return true;
+        };
         // One key tile.  kCut: some row of the warp does not see all its keys (a compile-time variant: no select per element elsewhere).
         auto tile = [&](int t, auto cut_tag) -> bool {
           constexpr bool kCut = decltype(cut_tag)::value;
           const int entry = (g + t - x.t0) & 7;
           const float4 ks = lds_f4(sbase + C::kSmemScales + entry * 32), vs = lds_f4(sbase + C::kSmemScales + entry * 32 + 16);
-          const float fc[4] = {f * ks.x, f * ks.y, f * ks.z, f * ks.w};
+          const uint32_t t_s = tmem + lanes + (C::kWide ? 128 * (mine & 1) + 64 * r : 128 * r);
+          const float fc[4] = {f * (C::kWide && r ? ks.z : ks.x), f * (C::kWide && r ? ks.w : ks.y), f * ks.z, f * ks.w};
           const int ev[4] = {static_cast<int>(scale_to_sb(vs.x)) - 127, static_cast<int>(scale_to_sb(vs.y)) - 127, static_cast<int>(scale_to_sb(vs.z)) - 127,
                              static_cast<int>(scale_to_sb(vs.w)) - 127};
-          const int seen = limit - 128 * t;                   // keys of the tile that the row sees
+          const int seen = limit - 128 * t - (C::kWide ? 64 * r : 0);         // keys of the tile, from this group's first on, that the row sees
           const int v_new = max(max(vexp, max(ev[0], ev[1])), max(ev[2], ev[3]));
           // 32 columns at a time, the next ones in flight; what a row does not see is -inf
           uint32_t s_buf[2][32];
           auto columns = [&](int c) {
             tmem_wait_ld();
-            if (c < 3) tmem_ld32(t_s + 32 * (c + 1), s_buf[(c + 1) & 1]);
+            if (c < C::kCols / 32 - 1) tmem_ld32(t_s + 32 * (c + 1), s_buf[(c + 1) & 1]);
             if (kCut) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
@@ -554,7 +612,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           float top = -CUDART_INF_F;
           tmem_ld32(t_s, s_buf[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < C::kCols / 32; ++c) {
             columns(c);
             float2 s2[16];
 #pragma unroll
@@ -562,13 +620,28 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             const float top_c = max32(s2);
             top = fmaxf(top, kCut && top_c == -CUDART_INF_F ? top_c : top_c * fc[c]);     // the factor may be zero
           }
+          if (C::kWide) {
+            // a common reference: seldom does a row move, so that one flag a warp says whether any does
+            const bool moves = __any_sync(0xffffffffu, top > m + kHeadroom);
+            volatile uint8_t* votes = smem + C::kSmemBars + 8 * (kBars + 2 + (mine & 1));       // behind the TMEM slot and the abort flag
+            if (lane == 0) {
+              votes[warp] = moves;
+              mbar_arrive(bars + kVote + (mine & 1));
+            }
+            if (!wait_warp(bar(kVote + (mine & 1)), (mine >> 1) & 1, abort_flag)) return false;
+            if (*reinterpret_cast<volatile uint64_t*>(votes) != 0) {
+              float other;
+              if (!tell(top, other)) return false;
+              top = fmaxf(top, other);
+            }
+          }
           const float m_new = top > m + kHeadroom ? top : m;
           const float mu = m_new == -CUDART_INF_F ? 0.f : m_new;
           tmem_ld32(t_s, s_buf[0]);
           if (__any_sync(0xffffffffu, m_new != m || v_new != vexp)) {
             const float keep = ex2_approx(m - mu);
             if (t > first) {
-              if (!wait_warp(bar(kPvDone + r), (mine - 1) & 1, abort_flag)) return false;
+              if (!wait_warp(bar(kPvDone + (C::kWide ? 0 : r)), (mine - 1) & 1, abort_flag)) return false;
               tc_fence_after();
               const float a = keep * exp2f(static_cast<float>(vexp - v_new));
 #pragma unroll 1
@@ -586,9 +659,9 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             vexp = v_new;
           }
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < C::kCols / 32; ++c) {
             // P comes out as 2^off exp(s - m); where V's scale is 2^-57 of another's the product vanishes anyway, but the sum must not
-            const int off = max(kPBase + ev[c] - vexp, -45);
+            const int off = max(kPBase + (C::kWide && r ? ev[(c + 2) & 3] : ev[c]) - vexp, -45);
             const float2 f2 = splat2(fc[c]), sub = splat2(static_cast<float>(off) - mu);
             columns(c);
             float2 sum = make_float2(0.f, 0.f);
@@ -606,7 +679,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             }
             l = fmaf(sum.x + sum.y, __uint_as_float(static_cast<uint32_t>(127 - off) << 23), l);
             tmem_st16(t_s + 16 * c, h);                       // over columns that have been read: 16 c + 15 < 32 c + 32
-            if (c == 1) {                                     // the first half of the keys: the tensor cores may begin
+            if (!C::kWide && c == 1) {                        // the first half of the keys: the tensor cores may begin
               tmem_wait_st();
               tc_fence_before();
               __syncwarp();
@@ -616,12 +689,13 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bars + kPFull + r);
+          if (lane == 0) mbar_arrive(bars + kPFull + (C::kWide ? mine & 1 : r));
           return true;
         };
         for (int t = first; t < x.t1; t += step, ++mine) {
           const int gt = g + t - x.t0;
-          ok = wait_warp(bar(kScales + (gt & 7)), (gt >> 3) & 1, abort_flag) && wait_warp(bar(kSFull + r), mine & 1, abort_flag);
+          ok = wait_warp(bar(kScales + (gt & 7)), (gt >> 3) & 1, abort_flag) &&
+               (C::kWide ? wait_warp(bar(kSFull + (mine & 1)), (mine >> 1) & 1, abort_flag) : wait_warp(bar(kSFull + r), mine & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
           const bool cut = __any_sync(0xffffffffu, limit < 128 * (t + 1));
@@ -629,7 +703,12 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         g += x.t1 - x.t0;
         if (!ok) break;
-        ok = wait_warp(bar(kPvDone + r), (mine - 1) & 1, abort_flag);
+        ok = wait_warp(bar(kPvDone + (C::kWide ? 0 : r)), (mine - 1) & 1, abort_flag);
+        if (ok && C::kWide) {                                 // the sum over both halves of the keys
+          float other = 0.f;
+          ok = tell(l, other);
+          l += other;
+        }
         if (!ok) break;
         tc_fence_after();
         const bool whole = x.t0 == 0 && x.t1 == x.tiles && !split;
@@ -639,7 +718,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int64_t out_row = limit == 0 ? -1 : ((static_cast<int64_t>(x.b) * p.Nq + i_tok) * p.H + head) * D;
         // Through shared memory, so that the lanes of a store write whole rows (a row a thread, 16 bytes at a time, took 11000 cycles a piece):
         // 32 rows x 128 bytes at a time, 16-byte pieces XORed with the row.
-        const int64_t part0 = static_cast<int64_t>(slot) * C::kRows + r * 128 + (warp & 3) * 32;
+        const int64_t part0 = static_cast<int64_t>(slot) * C::kRows + (C::kWide ? 0 : r * 128) + (warp & 3) * 32;
+        const int col0 = C::kWide ? 128 * r : 0;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
@@ -675,10 +755,10 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int64_t at = __shfl_sync(0xffffffffu, out_row, 4 * i + (lane >> 3));
-              if (at >= 0) reinterpret_cast<float4*>(p.o + at + 64 * (c >> 1))[piece] = v[i];
+              if (at >= 0) reinterpret_cast<float4*>(p.o + at + col0 + 64 * (c >> 1))[piece] = v[i];
             }
           } else {                                            // rows that see nothing too: their slots are not read
-            float4* to = reinterpret_cast<float4*>(p.part_o + (part0 + (lane >> 3)) * D + 32 * c) + piece;
+            float4* to = reinterpret_cast<float4*>(p.part_o + (part0 + (lane >> 3)) * D + col0 + 32 * c) + piece;
 #pragma unroll
             for (int i = 0; i < 8; ++i) to[4 * i * (D / 4)] = v[i];
           }
@@ -690,7 +770,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           if (x.t0 == 0) u->x = whole ? -1 : slot;
           if (x.t1 == x.tiles) u->y = cta;
         }
-        if (limit > 0) {
+        if (limit > 0 && (!C::kWide || r == 0)) {
           if (whole) {
             p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.Nq + i_tok] = (m + log2f(l)) * kLn2;
             if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(f, m + log2f(l));
@@ -699,6 +779,11 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           }
         }
         tc_fence_before();
+        if (C::kWide) {                                       // the staging has been read: the next queries may come
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + kQFree);
+        }
         slot = 2 * cta + 1;
       } while (next_chunk(p, x, f_end));
       if (!ok && lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
@@ -715,13 +800,14 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 
 // ------------------------------------------------------------------------------------------------ join
 // Rows of units that were cut, and rows that see nothing: one CTA per 8 rows of a (sequence, head), a warp a row at a time.
+template <int D>
 __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnParams p) {
-  constexpr int D = ChunkCfg::D;
+  constexpr int kRows = ChunkCfg<D>::kRows, kVecs = D / 128;
   grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int R = p.Nq * p.rep, groups = (R + 7) / 8, unit_tiles_max = (R + ChunkCfg::kRows - 1) / ChunkCfg::kRows;
+  const int R = p.Nq * p.rep, groups = (R + 7) / 8, unit_tiles_max = (R + kRows - 1) / kRows;
   const int r0 = static_cast<int>(blockIdx.x % groups) * 8, bh = static_cast<int>(blockIdx.x / groups), hk = bh % p.c.Hk, b = bh / p.c.Hk;
-  const int2 unit = p.unit_slots[static_cast<int64_t>(bh) * unit_tiles_max + r0 / ChunkCfg::kRows];
+  const int2 unit = p.unit_slots[static_cast<int64_t>(bh) * unit_tiles_max + r0 / kRows];
   const ChunkSeq s = chunk_seq(p, b);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -732,29 +818,37 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
     float* lse = p.lse + (static_cast<int64_t>(b) * p.H + head) * p.Nq + i_tok;
     const int64_t padded_row = static_cast<int64_t>(bh) * ((R + 127) / 128 * 128) + r;
     if (row_limit(p, s, r) == 0) {
-      o[0] = o[1] = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x) o[64 * x] = o[64 * x + 1] = __floats2bfloat162_rn(0.f, 0.f);
       if (lane == 0) *lse = -CUDART_INF_F;
       continue;
     }
     if (unit.x < 0) continue;                                 // whole: written by its CTA
     float top = -CUDART_INF_F, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int halves = s.count * p.rep - r / ChunkCfg::kRows * ChunkCfg::kRows <= 128 ? 2 : 1;      // a split unit's pieces have two results
+    float4 acc[kVecs] = {};
+    const int halves = kRows == 256 && s.count * p.rep - r / kRows * kRows <= 128 ? 2 : 1;      // a split unit's pieces have two results
     const int first = unit.x / 2 * halves, n = unit.y * halves + halves;
     for (int i = first; i < n; ++i) {
       const int c = i / halves;
-      const int64_t at = static_cast<int64_t>(c == unit.x / 2 ? unit.x : 2 * c) * ChunkCfg::kRows + (r & (ChunkCfg::kRows - 1)) + (i - c * halves) * 128;
+      const int64_t at = static_cast<int64_t>(c == unit.x / 2 ? unit.x : 2 * c) * kRows + (r & (kRows - 1)) + (i - c * halves) * 128;
       const float2 ml = p.part_ml[at];
       if (ml.x == -CUDART_INF_F) continue;                    // a piece of which the row sees nothing
-      const float4 v = reinterpret_cast<const float4*>(p.part_o + at * D)[lane];
+      float4 v[kVecs];
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x) v[x] = reinterpret_cast<const float4*>(p.part_o + at * D)[32 * x + lane];
       const float top_new = fmaxf(top, ml.x), a = exp2f(top - top_new), w = exp2f(ml.x - top_new);
       sum = sum * a + ml.y * w;
-      acc = make_float4(acc.x * a + v.x * w, acc.y * a + v.y * w, acc.z * a + v.z * w, acc.w * a + v.w * w);
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x)
+        acc[x] = make_float4(acc[x].x * a + v[x].x * w, acc[x].y * a + v[x].y * w, acc[x].z * a + v[x].z * w, acc[x].w * a + v[x].w * w);
       top = top_new;
     }
     const float inv = 1.f / sum;
-    o[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-    o[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+#pragma unroll
+    for (int x = 0; x < kVecs; ++x) {
+      o[64 * x] = __floats2bfloat162_rn(acc[x].x * inv, acc[x].y * inv);
+      o[64 * x + 1] = __floats2bfloat162_rn(acc[x].z * inv, acc[x].w * inv);
+    }
     if (lane == 0) {
       *lse = (top + log2f(sum)) * kLn2;
       if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(p.factors[padded_row], top + log2f(sum));
@@ -770,22 +864,29 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
 // The first row that sees token j.
 __device__ __forceinline__ int first_row(const CacheAttnParams& p, const ChunkSeq& s, int j) { return p.causal ? max(0, j - s.n + s.count) * p.rep : 0; }
 
+template <int D>
 struct ChunkWeightsCfg {
   static constexpr int kThreads = 320;
+  static constexpr int kRows = ChunkCfg<D>::kRows, kHalf = kRows / 2;          // of a row tile; of a softmax group
+  static constexpr int kPanels = D / 64;
   static constexpr int kTile = 128 * 128;
-  static constexpr int kQBytes = 4 * kTile;                   // 256 rows: two panels of 256 x 128 bytes
-  static constexpr int kSmemK = 2 * kQBytes;                  // two panels
-  static constexpr int kSmemCode = kSmemK + 2 * kTile;        // two buffers
-  static constexpr int kSmemRows = kSmemCode + 2 * kTile;     // (factor, log2 sum) of the rows, by row tile buffer
-  static constexpr int kSmemSums = kSmemRows + 2 * 256 * 8;
+  static constexpr int kQBytes = 4 * kTile;                   // panels of kRows x 128 bytes
+  static constexpr int kSmemK = 2 * kQBytes;                  // panels
+  static constexpr int kCodeBufs = D == 128 ? 2 : 1;          // what fits of the pieces of kTile in which codes come
+  static constexpr int kChunks = D / 128;
+  static constexpr int kSmemCode = kSmemK + kPanels * kTile;
+  static constexpr int kSmemRows = kSmemCode + kCodeBufs * kTile;     // (factor, log2 sum) of the rows, by row tile buffer
+  static constexpr int kSmemSums = kSmemRows + 2 * kRows * 8;
   static constexpr int kSmemBars = kSmemSums + 128 * 4;
   static constexpr int kSmem = kSmemBars + 256 + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 enum ChunkWeightsBar : int { kwCode = 0, kwCodeFree = 2, kwQ = 4, kwQFree = 6, kwS = 8, kwSFree = 10, kwK = 12, kwSums = 13, kwSumsFree = 14, kwBars = 15 };
 
-__global__ void __launch_bounds__(ChunkWeightsCfg::kThreads, 1)
+template <int D>
+__global__ void __launch_bounds__(ChunkWeightsCfg<D>::kThreads, 1)
 cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tq, const CacheAttnParams p, const int tiles_of_row) {
-  using C = ChunkWeightsCfg;
+  using C = ChunkWeightsCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
@@ -825,7 +926,7 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
   const int R = p.Nq * p.rep, row_tiles_max = (R + 127) / 128;
   const int64_t items = static_cast<int64_t>(p.c.B) * p.c.Hk * tiles_of_row;
   bool ok = true;
-  // Item i: a key tile that exists, and its row tiles that see any of it: rt0 ... rt1 - 1, of 256 rows.
+  // Item i: a key tile that exists, and its row tiles that see any of it: rt0 ... rt1 - 1.
   struct Item {
     int b, hk, t, n, rt0, rt1;
     ChunkSeq s;
@@ -838,10 +939,10 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
     x.s = chunk_seq(p, x.b);
     x.n = x.s.n;
     x.rt1 = x.s.units;
-    x.rt0 = min(x.rt1, first_row(p, x.s, 128 * x.t) / 256);
+    x.rt0 = min(x.rt1, first_row(p, x.s, 128 * x.t) / C::kRows);
     return 128 * x.t < x.n;
   };
-  int g = 0, q = 0;                                           // running item, running row tile
+  int g = 0, j = 0, q = 0;                                    // running item, running piece of codes, running row tile
   Item x;
   if (warp == 8) {
     // ------------------------------------------------------------------------------------------ TMA
@@ -851,24 +952,27 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
       const int blk = 4 * x.t + lane, entry = blk / bpp;
       const bool held = lane < 4 && blk * 32 < x.n;
       const int page = held ? max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + entry))) : 0;
-      if (g >= 2) ok = wait_warp(bar(kwCodeFree + (g & 1)), ((g >> 1) - 1) & 1, abort_flag);
-      if (!ok) break;
       const int boxes = __popc(__ballot_sync(0xffffffffu, held));
-      if (lane == 0) mbar_expect_tx(bars + kwCode + (g & 1), boxes * 4096);
-      __syncwarp();
-      if (held) tma_load_4d(sbase + C::kSmemCode + (g & 1) * C::kTile + lane * 4096, &tk, bar(kwCode + (g & 1)), 0, (blk - entry * bpp) * 32, x.hk, page);
-      ++g;
+      for (int c = 0; c < C::kChunks && ok; ++c, ++j) {
+        const int buf = j % C::kCodeBufs;
+        if (j >= C::kCodeBufs && !(ok = wait_warp(bar(kwCodeFree + buf), (j / C::kCodeBufs - 1) & 1, abort_flag))) break;
+        if (lane == 0) mbar_expect_tx(bars + kwCode + buf, boxes * 4096);
+        __syncwarp();
+        if (held) tma_load_4d(sbase + C::kSmemCode + buf * C::kTile + lane * 4096, &tk, bar(kwCode + buf), 128 * c, (blk - entry * bpp) * 32, x.hk, page);
+      }
+      if (!ok) break;
       for (int rt = x.rt0; rt < x.rt1; ++rt, ++q) {
         if (q >= 2 && !(ok = wait_warp(bar(kwQFree + (q & 1)), ((q >> 1) - 1) & 1, abort_flag))) break;
         if (lane == 0) {
           // the last row tile of a head may lack its second half: those columns hold what was there, and its rows see nothing
-          const int tile0 = (x.b * p.c.Hk + x.hk) * row_tiles_max + 2 * rt, halves = min(2, row_tiles_max - 2 * rt);
+          constexpr int kParts = C::kRows / 128;
+          const int tile0 = (x.b * p.c.Hk + x.hk) * row_tiles_max + kParts * rt, parts = min(kParts, row_tiles_max - kParts * rt);
           const uint32_t to = (q & 1) * C::kQBytes;
-          mbar_expect_tx(bars + kwQ + (q & 1), halves * (2 * C::kTile + 1024));
-          for (int r = 0; r < halves; ++r) {
-            for (int panel = 0; panel < 2; ++panel)
-              tma_load_2d(smem + to + panel * 2 * C::kTile + r * C::kTile, &tq, bars + kwQ + (q & 1), 128 * panel, (tile0 + r) * 128);
-            bulk_load_1d(smem + C::kSmemRows + (q & 1) * 2048 + r * 1024, p.row_ml + static_cast<int64_t>(tile0 + r) * 128, 1024, bars + kwQ + (q & 1));
+          mbar_expect_tx(bars + kwQ + (q & 1), parts * (C::kPanels * C::kTile + 1024));
+          for (int r = 0; r < parts; ++r) {
+            for (int panel = 0; panel < C::kPanels; ++panel)
+              tma_load_2d(smem + to + (panel * kParts + r) * C::kTile, &tq, bars + kwQ + (q & 1), 128 * panel, (tile0 + r) * 128);
+            bulk_load_1d(smem + C::kSmemRows + ((q & 1) * kParts + r) * 1024, p.row_ml + static_cast<int64_t>(tile0 + r) * 128, 1024, bars + kwQ + (q & 1));
           }
         }
         __syncwarp();
@@ -877,14 +981,14 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
     if (!ok) {
       if (lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutProducer + kInCache);
       for (int k = 1; k <= 2; ++k) {                          // what is in flight lands before the shared memory goes
-        if (g >= k) wait_or_abort(bar(kwCode + ((g - k) & 1)), ((g - k) >> 1) & 1, abort_flag);
+        if (j >= k && k <= C::kCodeBufs) wait_or_abort(bar(kwCode + (j - k) % C::kCodeBufs), (j - k) / C::kCodeBufs & 1, abort_flag);
         if (q >= k) wait_or_abort(bar(kwQ + ((q - k) & 1)), ((q - k) >> 1) & 1, abort_flag);
       }
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------------------------------ MMA
     if (elect_one()) {
-      constexpr uint32_t kIdesc = idesc_f8(128, 256, false, false);
+      constexpr uint32_t kIdesc = idesc_f8(128, C::kRows, false, false);
       const uint32_t k_lo = desc_lo(sbase + C::kSmemK), q_lo = desc_lo(sbase);
       for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
         if (!item_at(i, x) || x.rt0 >= x.rt1) continue;
@@ -895,9 +999,9 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
           if (q >= 2 && !(ok = wait_or_abort(bar(kwSFree + (q & 1)), ((q >> 1) - 1) & 1, abort_flag))) break;
           tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
+          for (int k = 0; k < D / 16; ++k)
             mma_h_ss(tmem + 256 * (q & 1), k_lo + (k >> 2) * (C::kTile >> 4) + (k & 3) * 2,
-                     q_lo + (q & 1) * (C::kQBytes >> 4) + (k >> 2) * (2 * C::kTile >> 4) + (k & 3) * 2, kIdesc, k > 0);
+                     q_lo + (q & 1) * (C::kQBytes >> 4) + (k >> 2) * (C::kRows * 128 >> 4) + (k & 3) * 2, kIdesc, k > 0);
           tc_commit(bars + kwQFree + (q & 1));
           tc_commit(bars + kwS + (q & 1));
         }
@@ -912,18 +1016,19 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
     for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x, ++it) {
       const bool exists = item_at(i, x);
       float total = 0.f;
-      const int j = 128 * x.t + key;
+      const int tok = 128 * x.t + key;
       if (exists && x.rt0 < x.rt1) {
         float ks = 0.f;                                       // of this token's block
-        if (j < x.n) {
-          const int page = max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + j / p.c.page)));
-          ks = __ldg(p.c.ks + page * p.c.s_page + x.hk * p.c.s_head + j % p.c.page / 32);
+        if (tok < x.n) {
+          const int page = max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + tok / p.c.page)));
+          ks = __ldg(p.c.ks + page * p.c.s_page + x.hk * p.c.s_head + tok % p.c.page / 32);
         }
-        if (!(ok = wait_warp(bar(kwCode + (g & 1)), (g >> 1) & 1, abort_flag))) break;
-        {
-          // as in the main kernel: 16-byte pieces c of keys tid / 8, + 32, ...; the f16 tile is free, all its products having been seen
+        // as in the main kernel: 16-byte pieces c of keys tid / 8, + 32, ...; the f16 tile is free, all its products having been seen
+        for (int part = 0; part < C::kChunks; ++part, ++j) {
+          const int buf = j % C::kCodeBufs;
+          if (!(ok = wait_warp(bar(kwCode + buf), j / C::kCodeBufs & 1, abort_flag))) break;
           const int c = tid & 7, panel = c >> 2, cc = (c & 3) * 2;
-          const uint32_t src = sbase + C::kSmemCode + (g & 1) * C::kTile, dst = sbase + C::kSmemK + panel * C::kTile;
+          const uint32_t src = sbase + C::kSmemCode + buf * C::kTile, dst = sbase + C::kSmemK + (2 * part + panel) * C::kTile;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int row = (tid >> 3) + 32 * k;
@@ -942,28 +1047,29 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
           fence_async_smem();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(bars + kwCodeFree + (g & 1));
-            mbar_arrive(bars + kwK);
+            mbar_arrive(bars + kwCodeFree + buf);
+            if (part == C::kChunks - 1) mbar_arrive(bars + kwK);
           }
         }
+        if (!ok) break;
         ++g;
         for (int rt = x.rt0; rt < x.rt1; ++rt, ++q) {
           // the products; and the rows' constants, seen by this warp itself
           if (!(ok = wait_warp(bar(kwS + (q & 1)), (q >> 1) & 1, abort_flag) && wait_warp(bar(kwQ + (q & 1)), (q >> 1) & 1, abort_flag))) break;
           tc_fence_after();
-          const int row0 = rt * 256 + half * 128;
+          const int row0 = rt * C::kRows + half * C::kHalf;
           if (row0 < x.s.count * p.rep) {
-            const int from_row = first_row(p, x.s, j) - row0;                 // of mine, the first that sees this token
+            const int from_row = first_row(p, x.s, tok) - row0;                 // of mine, the first that sees this token
             const bool cut = __any_sync(0xffffffffu, from_row > 0);
-            const uint32_t from = tmem + lanes + 256 * (q & 1) + 128 * half, rows = sbase + C::kSmemRows + (q & 1) * 2048 + half * 1024;
+            const uint32_t from = tmem + lanes + 256 * (q & 1) + C::kHalf * half, rows = sbase + C::kSmemRows + ((q & 1) * C::kRows + half * C::kHalf) * 8;
             uint32_t s_buf[2][32];
             tmem_ld32(from, s_buf[0]);
 #pragma unroll 1
-            for (int c2 = 0; c2 < 2; ++c2) {
+            for (int c2 = 0; c2 < C::kHalf / 64; ++c2) {
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 tmem_wait_ld();
-                if (!(c2 == 1 && k == 1)) tmem_ld32(from + 64 * c2 + 32 * (k + 1), s_buf[k ^ 1]);
+                if (!(c2 == C::kHalf / 64 - 1 && k == 1)) tmem_ld32(from + 64 * c2 + 32 * (k + 1), s_buf[k ^ 1]);
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -1000,9 +1106,9 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
         total += sums[key];
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kwSumsFree);
-        if (j < p.W) {
-          float* at = p.weights + x.b * p.w_sb + x.hk * p.w_sh + j;
-          if (j < x.n) *at = p.accumulate ? *at + total : total;
+        if (tok < p.W) {
+          float* at = p.weights + x.b * p.w_sb + x.hk * p.w_sh + tok;
+          if (tok < x.n) *at = p.accumulate ? *at + total : total;
           else if (!p.accumulate) *at = 0.f;
         }
       }
@@ -1020,41 +1126,46 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
 
 }  // namespace
 
-int cache_chunk_rows() { return ChunkCfg::kRows; }
+int cache_chunk_rows(int D) { return D == 128 ? ChunkCfg<128>::kRows : ChunkCfg<256>::kRows; }
 int64_t cache_chunk_start_bytes() { return (sizeof(ChunkStart) + 7) / 8 * 8; }
 int64_t cache_chunk_query_rows(int B, int Hk, int R) { return static_cast<int64_t>(B) * Hk * ((R + 127) / 128 * 128); }
 
-cudaError_t launch_cache_chunk(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
-  using C = ChunkCfg;
+template <int D>
+static cudaError_t launch_chunk(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
+  using C = ChunkCfg<D>;
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
     cudaFuncAttributes attr;
-    cudaError_t e = cudaFuncGetAttributes(&attr, cache_chunk_kernel);
+    cudaError_t e = cudaFuncGetAttributes(&attr, cache_chunk_kernel<D>);
     if (e != cudaSuccess) return e;
     if (attr.numRegs * C::kThreads < 256 * (C::kRegsSoftmax + C::kRegsOther)) return cudaErrorLaunchOutOfResources;
-    e = cudaFuncSetAttribute(cache_chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(cache_chunk_weights_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkWeightsCfg::kSmem);
+    e = cudaFuncSetAttribute(cache_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(cache_chunk_weights_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkWeightsCfg<D>::kSmem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   const unsigned row_tiles = static_cast<unsigned>(p.c.B) * p.c.Hk * ((p.Nq * p.rep + 127) / 128);
   count_launch();
-  cudaError_t e = launch_chained(cache_chunk_queries_kernel, dim3(row_tiles * 8 + 1), 256, 0, stream, p);
+  cudaError_t e = launch_chained(cache_chunk_queries_kernel<D>, dim3(row_tiles * (D / 16) + 1), 256, 0, stream, p);      // 2048 / D rows a CTA
   if (e != cudaSuccess) return e;
   count_launch();
-  e = launch_chained(cache_chunk_kernel, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, tq, p);
+  e = launch_chained(cache_chunk_kernel<D>, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, tq, p);
   if (e != cudaSuccess) return e;
   count_launch();
   const int groups = (p.Nq * p.rep + 7) / 8;
-  e = launch_chained(cache_chunk_join_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * groups), 128, 0, stream, p);
+  e = launch_chained(cache_chunk_join_kernel<D>, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * groups), 128, 0, stream, p);
   if (e != cudaSuccess || p.weights == nullptr) return e;
   const int tiles_of_row = (p.W + 127) / 128;                 // what lies beyond the length too: its weights are zeros
   const int64_t items = static_cast<int64_t>(p.c.B) * p.c.Hk * tiles_of_row;
   count_launch();
-  return launch_chained(cache_chunk_weights_kernel, dim3(static_cast<unsigned>(items < sm_count() ? items : sm_count())), ChunkWeightsCfg::kThreads,
-                        ChunkWeightsCfg::kSmem, stream, tk, tq, p, tiles_of_row);
+  return launch_chained(cache_chunk_weights_kernel<D>, dim3(static_cast<unsigned>(items < sm_count() ? items : sm_count())), ChunkWeightsCfg<D>::kThreads,
+                        ChunkWeightsCfg<D>::kSmem, stream, tk, tq, p, tiles_of_row);
+}
+
+cudaError_t launch_cache_chunk(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
+  return D == 128 ? launch_chunk<128>(tk, tv, tq, p, stream) : launch_chunk<256>(tk, tv, tq, p, stream);
 }
 
 }  // namespace dm
