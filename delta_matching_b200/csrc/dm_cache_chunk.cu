@@ -45,11 +45,11 @@ struct ChunkCfg {
   static constexpr int kSmemQ = 0;                            // row tiles x panels
   static constexpr int kSmemK = 4 * kTile;                    // between the uses of two tiles lies a softmax, longer than a conversion
   static constexpr int kSmemV = kSmemK + kPanels * kTile;
-  static constexpr int kSmemCode = kSmemV + 4 * kTile;        // two pieces
+  static constexpr int kSmemCode = kSmemV + 4 * kTile;        // two pieces: a load takes 2000 cycles, a conversion 1200; with four it was not faster
   // output staging, 4 KB a softmax warp: with 256 columns over the queries, which then wait for it
   static constexpr int kSmemOut = kWide ? kSmemQ : kSmemCode + 2 * kTile;
   static constexpr int kSmemBars = kSmemCode + (kWide ? 2 : 4) * kTile;
-  static constexpr int kSmemScales = kSmemBars + 320;         // 8 tiles x (4 K scales, 4 V scales)
+  static constexpr int kSmemScales = kSmemBars + 352;         // 8 tiles x (4 K scales, 4 V scales)
   static constexpr int kSmemRows = kSmemScales + 8 * 32;      // what the two groups tell each other of their rows
   static constexpr int kSmem = kSmemRows + (kWide ? 1024 : 0) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
@@ -211,13 +211,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 
 enum ChunkBar : int {
-  kCodeFull = 0, kCodeEmpty = 2,            // K codes, V codes
-  kKFull = 4, kKEmpty = 5,
-  kVFull = 6, kVEmpty = 8,                  // by parity of the running tile
-  kQFull = 10, kQFree = 12, kSFull = 14, kPHalf = 16, kPFull = 18, kPvDone = 20,      // by row tile; kSFull and kPFull of 256 columns by tile
-  kScales = 22,                             // of running tile g: entry g % 8 (the loads are at most four tiles ahead of the softmax)
-  kVote = 30, kTell = 32,                   // 256 columns: a row's maximum has moved; maxima and sums lie ready
-  kBars = 33,                               // behind them the TMEM slot, the abort flag and two words of votes
+  kCodeFull = 0, kCodeEmpty = 4,            // of the ring of pieces
+  kKFull = 8, kKEmpty = 9,
+  kVFull = 10, kVEmpty = 12,                // by parity of the running tile
+  kQFull = 14, kQFree = 16, kSFull = 18, kPHalf = 20, kPFull = 22, kPvDone = 24,      // by row tile; kSFull, kPFull and kPvDone of 256 columns by tile
+  kVote = 26, kTell = 28,                   // 256 columns: a row's maximum has moved; maxima and sums lie ready
+  kScales = 29,                             // of running tile g: entry g % 8 (the loads are at most five tiles ahead of the softmax)
+  kBars = 37,                               // behind them the TMEM slot, the abort flag and two words of votes
 };
 
 // ------------------------------------------------------------------------------------------------ queries
@@ -277,8 +277,6 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bars + kCodeFull + i, 1);
-      mbar_init(bars + kCodeEmpty + i, 4);
       mbar_init(bars + kVFull + i, 4);
       mbar_init(bars + kVEmpty + i, 1);
       mbar_init(bars + kQFull + i, 1);
@@ -288,6 +286,10 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       mbar_init(bars + kPFull + i, C::kWide ? 8 : 4);
       mbar_init(bars + kPvDone + i, 1);
       mbar_init(bars + kVote + i, 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bars + kCodeFull + i, 1);
+      mbar_init(bars + kCodeEmpty + i, 4);
     }
     mbar_init(bars + kKFull, 4);
     mbar_init(bars + kKEmpty, 1);
@@ -357,28 +359,37 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         a.vs = __ldg(p.c.vs + at);
       };
       int g = 0, j = 0;                                       // running tile, running piece of codes
-      Ahead now = look_up(), next = look_up();
-      ask_scales(now);
-      for (; now.live; ++g) {
-        const Ahead after = look_up();
-        ask_scales(next);
-        const int boxes = __popc(__ballot_sync(0xffffffffu, now.held));
-        for (int c = 0; c < C::kChunks; ++c, ++j) {
-          const int buf = j & 1, x0 = C::kWide ? (c & 1) * 128 : 0;
-          if (j >= 2) ok = ok && wait_warp(bar(kCodeEmpty + buf), ((j >> 1) - 1) & 1, abort_flag);
-          if (!ok) break;
+      auto load = [&](const Ahead& a, bool is_v) {
+        const int boxes = __popc(__ballot_sync(0xffffffffu, a.held));
+        for (int c = 0; c < D / 128 && ok; ++c, ++j) {
+          const int buf = j & 1;
+          if (j >= 2 && !(ok = wait_warp(bar(kCodeEmpty + buf), ((j >> 1) - 1) & 1, abort_flag))) break;
           if (lane == 0) mbar_expect_tx(bars + kCodeFull + buf, boxes * 4096);
           __syncwarp();
-          if (now.held)
-            tma_load_4d(sbase + C::kSmemCode + buf * C::kTile + lane * 4096, 2 * c >= C::kChunks ? &tv : &tk, bar(kCodeFull + buf), x0, now.sub * 32, now.hk, now.page);
+          if (a.held)
+            tma_load_4d(sbase + C::kSmemCode + buf * C::kTile + lane * 4096, is_v ? &tv : &tk, bar(kCodeFull + buf), 128 * c, a.sub * 32, a.hk, a.page);
         }
-        if (!ok) break;
+      };
+      Ahead now = look_up(), next = look_up();
+      ask_scales(now);
+      bool first = C::kWide && now.live;
+      for (; now.live && ok; ++g) {
+        const Ahead after = look_up();
+        ask_scales(next);
         if (lane < 4) {
           scales[(g & 7) * 8 + lane] = now.ks;                // zero where there is no block
           scales[(g & 7) * 8 + 4 + lane] = now.vs;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
+        // K of the next tile before V with 256 columns: its S is computed while the softmax is at this one.  (One place calls load: with more of
+        // them the kernel outgrew its instruction cache.)
+#pragma unroll 1
+        for (int i = first ? 0 : 1; i < 3; ++i) {
+          const bool ahead = C::kWide && i == 1;
+          if ((ahead ? next.live : true) && ok) load(ahead ? next : now, i == 2);
+        }
+        first = false;
         now = next;
         next = after;
       }
@@ -417,7 +428,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             issue_s(g & 1, true);
             for (int i = 0; i < n && ok; ++i, ++g) {
               if (i + 1 < n) {                                // the next S, while the softmax is at this one
-                if (!(ok = wait_or_abort(bar(kKFull), (g + 1) & 1, abort_flag))) break;
+                // its buffer held the P of the tile before this one, and the products of different shapes need not keep their order
+                if (!(ok = wait_or_abort(bar(kKFull), (g + 1) & 1, abort_flag) && (i == 0 || wait_or_abort(bar(kPvDone + ((g - 1) & 1)), ((g - 1) >> 1) & 1, abort_flag)))) break;
                 tc_fence_after();
                 issue_s((g + 1) & 1, true);
               }
@@ -428,7 +440,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
               for (int k = 0; k < 8; ++k)
                 mma_h_ts(tmem + 256, tmem + 128 * (g & 1) + 64 * (k >> 2) + 8 * (k & 3), v_lo + k * (2048 >> 4), kIdescO, i > 0 || k > 0);
               tc_commit(bars + kVEmpty);
-              tc_commit(bars + kPvDone);
+              tc_commit(bars + kPvDone + (g & 1));
             }
           } while (ok && next_chunk(p, x, f_end));
         } else {
@@ -503,52 +515,69 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const int ct = tid - 256, c = ct & 7;                   // a thread takes 16-byte pieces c of keys ct / 8, + 16, ...
       // a piece's two halves of eight elements: which goes first is chosen so that the stores of eight lanes fall on different banks
       const int panel = c >> 2, flip = panel;
-      int g = 0, j = 0;                                       // running tile, running piece of codes
-      do {
-        for (int t = x.t0; t < x.t1 && ok; ++t, ++g) {
+      int j = 0;                                              // running piece of codes
+      // K or V of running tile g; V's slots beyond the length hold anything, NaN codes too: zeros
+      auto convert = [&](bool is_v, int g, int held) {
+        const int vbuf = C::kVBufs == 2 ? g & 1 : 0;
 #pragma unroll 1
-          for (int part = 0; part < C::kChunks; ++part, ++j) {
-            const bool kv = 2 * part >= C::kChunks, first = 2 * part % C::kChunks == 0;      // V; the first piece of K or V
-            const int side = C::kWide ? part & 1 : 0, vbuf = C::kVBufs == 2 ? g & 1 : 0;
-            ok = wait_warp(bar(kCodeFull + (j & 1)), (j >> 1) & 1, abort_flag);
-            if (ok && first && !kv && g >= 1) ok = wait_warp(bar(kKEmpty), (g - 1) & 1, abort_flag);
-            if (ok && first && kv && g >= C::kVBufs) ok = wait_warp(bar(kVEmpty + vbuf), (g / C::kVBufs - 1) & 1, abort_flag);
-            if (!ok) break;
-            const uint32_t src = sbase + C::kSmemCode + (j & 1) * C::kTile;
-            const uint32_t dst = sbase + (kv ? C::kSmemV + vbuf * C::kPanels * C::kTile : C::kSmemK) + (2 * side + panel) * C::kTile;
-            const int held = kv ? x.s.n - 128 * t : 128;      // V's slots beyond the length hold anything, NaN codes too: zeros
+        for (int part = 0; part < D / 128 && ok; ++part, ++j) {
+          const int buf = j & 1;
+          ok = wait_warp(bar(kCodeFull + buf), (j >> 1) & 1, abort_flag);
+          if (ok && part == 0 && !is_v && g >= 1) ok = wait_warp(bar(kKEmpty), (g - 1) & 1, abort_flag);
+          if (ok && part == 0 && is_v && g >= C::kVBufs) ok = wait_warp(bar(kVEmpty + vbuf), (g / C::kVBufs - 1) & 1, abort_flag);
+          if (!ok) break;
+          const uint32_t src = sbase + C::kSmemCode + buf * C::kTile;
+          const uint32_t dst = sbase + (is_v ? C::kSmemV + vbuf * C::kPanels * C::kTile : C::kSmemK) + (2 * part + panel) * C::kTile;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int key = (ct >> 3) + 16 * i;
-              const float4 w4 = lds_f4(src + key * 128 + ((c ^ (key & 7)) << 4));
-              uint32_t w[4] = {__float_as_uint(w4.x), __float_as_uint(w4.y), __float_as_uint(w4.z), __float_as_uint(w4.w)};
-              if (key >= held) w[0] = w[1] = w[2] = w[3] = 0;
-              uint32_t h[8];
+          for (int i = 0; i < 8; ++i) {
+            const int key = (ct >> 3) + 16 * i;
+            const float4 w4 = lds_f4(src + key * 128 + ((c ^ (key & 7)) << 4));
+            uint32_t w[4] = {__float_as_uint(w4.x), __float_as_uint(w4.y), __float_as_uint(w4.z), __float_as_uint(w4.w)};
+            if (key >= held) w[0] = w[1] = w[2] = w[3] = 0;
+            uint32_t h[8];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                h[2 * j] = e4m3_lo_f16x2(w[j]);
-                h[2 * j + 1] = e4m3_hi_f16x2(w[j]);
-              }
-              const int cc = (c & 3) * 2;
-              const uint32_t row = dst + key * 128;
-              const uint32_t first = row + (((cc + flip) ^ (key & 7)) << 4), second = row + (((cc + 1 - flip) ^ (key & 7)) << 4);
-              if (flip) {
-                sts_u4(first, h[4], h[5], h[6], h[7]);
-                sts_u4(second, h[0], h[1], h[2], h[3]);
-              } else {
-                sts_u4(first, h[0], h[1], h[2], h[3]);
-                sts_u4(second, h[4], h[5], h[6], h[7]);
-              }
+            for (int e = 0; e < 4; ++e) {
+              h[2 * e] = e4m3_lo_f16x2(w[e]);
+              h[2 * e + 1] = e4m3_hi_f16x2(w[e]);
             }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (2 * (part + 1) % C::kChunks == 0) mbar_arrive(bars + (kv ? kVFull + vbuf : kKFull));
-              mbar_arrive(bars + kCodeEmpty + (j & 1));
+            const int cc = (c & 3) * 2;
+            const uint32_t row = dst + key * 128;
+            const uint32_t first = row + (((cc + flip) ^ (key & 7)) << 4), second = row + (((cc + 1 - flip) ^ (key & 7)) << 4);
+            if (flip) {
+              sts_u4(first, h[4], h[5], h[6], h[7]);
+              sts_u4(second, h[0], h[1], h[2], h[3]);
+            } else {
+              sts_u4(first, h[0], h[1], h[2], h[3]);
+              sts_u4(second, h[4], h[5], h[6], h[7]);
             }
           }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (part == D / 128 - 1) mbar_arrive(bars + (is_v ? kVFull + vbuf : kKFull));
+            mbar_arrive(bars + kCodeEmpty + buf);
+          }
         }
-      } while (ok && next_chunk(p, x, f_end));
+      };
+      int t = x.t0;
+      auto find = [&]() {                                     // from tile t of the piece on: is there one?
+        while (t >= x.t1) {
+          if (!next_chunk(p, x, f_end)) return false;
+          t = x.t0;
+        }
+        return true;
+      };
+      int held = 0;                                           // of the tile whose V is next
+      bool live = true;
+      for (int g = 0; live && ok; ++g) {                      // in the order of the loads: K of tile g, V of the same or (256 columns) the one before
+        live = find();
+        const int held_g = live ? x.s.n - 128 * t++ : 0;
+        if (!C::kWide) held = held_g;
+#pragma unroll 1
+        for (int kv = 0; kv < 2 && ok; ++kv)
+          if (C::kWide && kv == 1 ? g > 0 : live) convert(kv == 1, C::kWide ? g - kv : g, kv == 1 ? held : 128);
+        held = held_g;
+      }
       if (!ok && lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
     } else if (warp < 8) {
       reg_inc<C::kRegsSoftmax>();
@@ -577,6 +606,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const float f = __ldg(p.factors + padded_row);
         float m = -CUDART_INF_F, l = 0.f;
         int vexp = -1000;
+        // P V of this group's tile i is in O.  With 256 columns the softmax may be two tiles ahead of the products, so that these have two barriers.
+        auto products_of = [&](int i) { return C::kWide ? wait_warp(bar(kPvDone + (i & 1)), (i >> 1) & 1, abort_flag) : wait_warp(bar(kPvDone + r), i & 1, abort_flag); };
         // What the two groups know of a row (256 columns): the other's value.
         auto tell = [&](float mine_v, float& other) -> bool {
           told[128 * r] = mine_v;
@@ -641,7 +672,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           if (__any_sync(0xffffffffu, m_new != m || v_new != vexp)) {
             const float keep = ex2_approx(m - mu);
             if (t > first) {
-              if (!wait_warp(bar(kPvDone + (C::kWide ? 0 : r)), (mine - 1) & 1, abort_flag)) return false;
+              if (!products_of(mine - 1)) return false;
               tc_fence_after();
               const float a = keep * exp2f(static_cast<float>(vexp - v_new));
 #pragma unroll 1
@@ -703,7 +734,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         g += x.t1 - x.t0;
         if (!ok) break;
-        ok = wait_warp(bar(kPvDone + (C::kWide ? 0 : r)), (mine - 1) & 1, abort_flag);
+        ok = products_of(mine - 1);
         if (ok && C::kWide) {                                 // the sum over both halves of the keys
           float other = 0.f;
           ok = tell(l, other);
