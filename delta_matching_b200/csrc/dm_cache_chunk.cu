@@ -49,7 +49,7 @@ struct ChunkCfg {
   // output staging, 4 KB a softmax warp: with 256 columns over the queries, which then wait for it
   static constexpr int kSmemOut = kWide ? kSmemQ : kSmemCode + 2 * kTile;
   static constexpr int kSmemBars = kSmemCode + (kWide ? 2 : 4) * kTile;
-  static constexpr int kSmemScales = kSmemBars + 352;         // 8 tiles x (4 K scales, 4 V scales)
+  static constexpr int kSmemScales = kSmemBars + 416;         // 8 tiles x (4 K scales, 4 V scales)
   static constexpr int kSmemRows = kSmemScales + 8 * 32;      // what the two groups tell each other of their rows
   static constexpr int kSmem = kSmemRows + (kWide ? 1024 : 0) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
@@ -215,9 +215,10 @@ enum ChunkBar : int {
   kKFull = 8, kKEmpty = 9,
   kVFull = 10, kVEmpty = 12,                // by parity of the running tile
   kQFull = 14, kQFree = 16, kSFull = 18, kPHalf = 20, kPFull = 22, kPvDone = 24,      // by row tile; kSFull, kPFull and kPvDone of 256 columns by tile
-  kVote = 26, kTell = 28,                   // 256 columns: a row's maximum has moved; maxima and sums lie ready
-  kScales = 29,                             // of running tile g: entry g % 8 (the loads are at most five tiles ahead of the softmax)
-  kBars = 37,                               // behind them the TMEM slot, the abort flag and two words of votes
+  // 256 columns, by pair of warps (the two of the same rows): a row's maximum has moved, by parity of the tile; maxima and sums lie ready
+  kVote = 26, kTell = 34,
+  kScales = 38,                             // of running tile g: entry g % 8 (the loads are at most five tiles ahead of the softmax)
+  kBars = 46,                               // behind them the TMEM slot, the abort flag and two words of votes
 };
 
 // ------------------------------------------------------------------------------------------------ queries
@@ -285,7 +286,6 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       mbar_init(bars + kPHalf + i, 4);
       mbar_init(bars + kPFull + i, C::kWide ? 8 : 4);
       mbar_init(bars + kPvDone + i, 1);
-      mbar_init(bars + kVote + i, 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bars + kCodeFull + i, 1);
@@ -293,7 +293,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     }
     mbar_init(bars + kKFull, 4);
     mbar_init(bars + kKEmpty, 1);
-    mbar_init(bars + kTell, 8);
+    for (int i = 0; i < 8; ++i) mbar_init(bars + kVote + i, 2);
+    for (int i = 0; i < 4; ++i) mbar_init(bars + kTell + i, 2);
     for (int i = 0; i < 8; ++i) mbar_init(bars + kScales + i, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -587,7 +588,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const uint32_t t_o = tmem + lanes + 256 + 128 * r;      // of 256 columns, the half that this group rescales and writes
       volatile float* told = reinterpret_cast<volatile float*>(smem + C::kSmemRows) + in_tile;        // by group 0 of this row; by group 1 128 values on
       const uint32_t stage = sbase + C::kSmemOut + warp * 4096;
-      int g = 0, mine = 0, tells = 0;                         // running tile; tiles of this row tile; times the groups have told each other
+      int g = 0, mine = 0, asked = 0, tells = 0;              // running tile; tiles of this row tile; votes and values that the pair has exchanged
       int slot = 2 * cta;
       do {
         if (x.t0 >= x.t1) continue;
@@ -601,6 +602,10 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         const int row = x.rt * C::kRows + (C::kWide || split ? 0 : r * 128) + in_tile, limit = row_limit(p, x.s, row);
         const int i_tok = row / p.rep, head = x.hk * p.rep + row - i_tok * p.rep;
+        // A row that sees nothing is not written here: its logits need no mask (one of them had its warp take the masked path in all tiles), and a warp
+        // of such rows makes none, whatever its P holds.
+        const int sees = limit > 0 ? limit : INT_MAX;
+        const bool idle = !__any_sync(0xffffffffu, limit > 0);
         // of the row's logits, K's scale aside
         const int64_t padded_row = (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + 127) / 128 * 128) + row;
         const float f = __ldg(p.factors + padded_row);
@@ -608,12 +613,12 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         int vexp = -1000;
         // P V of this group's tile i is in O.  With 256 columns the softmax may be two tiles ahead of the products, so that these have two barriers.
         auto products_of = [&](int i) { return C::kWide ? wait_warp(bar(kPvDone + (i & 1)), (i >> 1) & 1, abort_flag) : wait_warp(bar(kPvDone + r), i & 1, abort_flag); };
-        // What the two groups know of a row (256 columns): the other's value.
+        // What the two warps of a row's two groups know of it (256 columns): the other's value.
         auto tell = [&](float mine_v, float& other) -> bool {
           told[128 * r] = mine_v;
           __syncwarp();
-          if (lane == 0) mbar_arrive(bars + kTell);
-          if (!wait_warp(bar(kTell), tells++ & 1, abort_flag)) return false;
+          if (lane == 0) mbar_arrive(bars + kTell + (warp & 3));
+          if (!wait_warp(bar(kTell + (warp & 3)), tells++ & 1, abort_flag)) return false;
           other = told[128 * (r ^ 1)];
           return true;
         };
@@ -626,7 +631,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           const float fc[4] = {f * (C::kWide && r ? ks.z : ks.x), f * (C::kWide && r ? ks.w : ks.y), f * ks.z, f * ks.w};
           const int ev[4] = {static_cast<int>(scale_to_sb(vs.x)) - 127, static_cast<int>(scale_to_sb(vs.y)) - 127, static_cast<int>(scale_to_sb(vs.z)) - 127,
                              static_cast<int>(scale_to_sb(vs.w)) - 127};
-          const int seen = limit - 128 * t - (C::kWide ? 64 * r : 0);         // keys of the tile, from this group's first on, that the row sees
+          const int seen = sees - 128 * t - (C::kWide ? 64 * r : 0);         // keys of the tile, from this group's first on, that the row sees
           const int v_new = max(max(vexp, max(ev[0], ev[1])), max(ev[2], ev[3]));
           // 32 columns at a time, the next ones in flight; what a row does not see is -inf
           uint32_t s_buf[2][32];
@@ -652,15 +657,16 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             top = fmaxf(top, kCut && top_c == -CUDART_INF_F ? top_c : top_c * fc[c]);     // the factor may be zero
           }
           if (C::kWide) {
-            // a common reference: seldom does a row move, so that one flag a warp says whether any does
+            // a common reference: seldom does a row move, so that the pair first tell each other whether any does
             const bool moves = __any_sync(0xffffffffu, top > m + kHeadroom);
-            volatile uint8_t* votes = smem + C::kSmemBars + 8 * (kBars + 2 + (mine & 1));       // behind the TMEM slot and the abort flag
+            volatile uint8_t* votes = smem + C::kSmemBars + 8 * (kBars + 2 + (asked & 1));      // behind the TMEM slot and the abort flag
+            const int vote = kVote + 2 * (warp & 3) + (asked & 1);
             if (lane == 0) {
               votes[warp] = moves;
-              mbar_arrive(bars + kVote + (mine & 1));
+              mbar_arrive(bars + vote);
             }
-            if (!wait_warp(bar(kVote + (mine & 1)), (mine >> 1) & 1, abort_flag)) return false;
-            if (*reinterpret_cast<volatile uint64_t*>(votes) != 0) {
+            if (!wait_warp(bar(vote), (asked++ >> 1) & 1, abort_flag)) return false;
+            if (moves || votes[warp ^ 4]) {
               float other;
               if (!tell(top, other)) return false;
               top = fmaxf(top, other);
@@ -725,17 +731,24 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         };
         for (int t = first; t < x.t1; t += step, ++mine) {
           const int gt = g + t - x.t0;
-          ok = wait_warp(bar(kScales + (gt & 7)), (gt >> 3) & 1, abort_flag) &&
+          ok = (idle || wait_warp(bar(kScales + (gt & 7)), (gt >> 3) & 1, abort_flag)) &&
                (C::kWide ? wait_warp(bar(kSFull + (mine & 1)), (mine >> 1) & 1, abort_flag) : wait_warp(bar(kSFull + r), mine & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
-          const bool cut = __any_sync(0xffffffffu, limit < 128 * (t + 1));
+          if (idle) {
+            if (lane == 0) {
+              if (!C::kWide) mbar_arrive(bars + kPHalf + r);
+              mbar_arrive(bars + kPFull + (C::kWide ? mine & 1 : r));
+            }
+            continue;
+          }
+          const bool cut = __any_sync(0xffffffffu, sees < 128 * (t + 1));
           if (!(ok = cut ? tile(t, std::true_type{}) : tile(t, std::false_type{}))) break;
         }
         g += x.t1 - x.t0;
         if (!ok) break;
-        ok = products_of(mine - 1);
-        if (ok && C::kWide) {                                 // the sum over both halves of the keys
+        ok = idle || products_of(mine - 1);
+        if (ok && !idle && C::kWide) {                                 // the sum over both halves of the keys
           float other = 0.f;
           ok = tell(l, other);
           l += other;
@@ -752,7 +765,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int64_t part0 = static_cast<int64_t>(slot) * C::kRows + (C::kWide ? 0 : r * 128) + (warp & 3) * 32;
         const int col0 = C::kWide ? 128 * r : 0;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+        for (int c = idle ? 4 : 0; c < 4; ++c) {
           uint32_t o[32];
           tmem_ld32(t_o + 32 * c, o);
           tmem_wait_ld();
@@ -830,60 +843,72 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// Rows of units that were cut, and rows that see nothing: one CTA per 8 rows of a (sequence, head), a warp a row at a time.
+// Rows of units that were cut, and rows that see nothing: a warp a row, four of a (sequence, head) a CTA.
 template <int D>
 __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnParams p) {
   constexpr int kRows = ChunkCfg<D>::kRows, kVecs = D / 128;
   grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int R = p.Nq * p.rep, groups = (R + 7) / 8, unit_tiles_max = (R + kRows - 1) / kRows;
-  const int r0 = static_cast<int>(blockIdx.x % groups) * 8, bh = static_cast<int>(blockIdx.x / groups), hk = bh % p.c.Hk, b = bh / p.c.Hk;
-  const int2 unit = p.unit_slots[static_cast<int64_t>(bh) * unit_tiles_max + r0 / kRows];
+  const int R = p.Nq * p.rep, groups = (R + 3) / 4, unit_tiles_max = (R + kRows - 1) / kRows;
+  const int r = static_cast<int>(blockIdx.x % groups) * 4 + warp, bh = static_cast<int>(blockIdx.x / groups), hk = bh % p.c.Hk, b = bh / p.c.Hk;
+  if (r >= R) return;
+  const int2 unit = p.unit_slots[static_cast<int64_t>(bh) * unit_tiles_max + r / kRows];
   const ChunkSeq s = chunk_seq(p, b);
+  const int i_tok = r / p.rep, head = hk * p.rep + r - i_tok * p.rep;
+  __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(b) * p.Nq + i_tok) * p.H + head) * D) + 2 * lane;
+  float* lse = p.lse + (static_cast<int64_t>(b) * p.H + head) * p.Nq + i_tok;
+  const int64_t padded_row = static_cast<int64_t>(bh) * ((R + 127) / 128 * 128) + r;
+  if (row_limit(p, s, r) == 0) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int r = r0 + warp + 4 * k;
-    if (r >= R) break;
-    const int i_tok = r / p.rep, head = hk * p.rep + r - i_tok * p.rep;
-    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(b) * p.Nq + i_tok) * p.H + head) * D) + 2 * lane;
-    float* lse = p.lse + (static_cast<int64_t>(b) * p.H + head) * p.Nq + i_tok;
-    const int64_t padded_row = static_cast<int64_t>(bh) * ((R + 127) / 128 * 128) + r;
-    if (row_limit(p, s, r) == 0) {
+    for (int x = 0; x < kVecs; ++x) o[64 * x] = o[64 * x + 1] = __floats2bfloat162_rn(0.f, 0.f);
+    if (lane == 0) *lse = -CUDART_INF_F;
+    return;
+  }
+  if (unit.x < 0) return;                                 // whole: written by its CTA
+  float top = -CUDART_INF_F, sum = 0.f;
+  float4 acc[kVecs] = {};
+  const int halves = kRows == 256 && s.count * p.rep - r / kRows * kRows <= 128 ? 2 : 1;      // a split unit's pieces have two results
+  const int first = unit.x / 2 * halves, n = unit.y * halves + halves;
+  // 32 results at a time, a lane each: their maxima and sums together, then the values of those that count
+  for (int i0 = first; i0 < n; i0 += 32) {
+    const int i = i0 + lane, c = i / halves;
+    const int at = (c == unit.x / 2 ? unit.x : 2 * c) * kRows + (r & (kRows - 1)) + (i - c * halves) * 128;
+    const float2 ml = i < n ? p.part_ml[at] : make_float2(-CUDART_INF_F, 0.f);         // -inf: a piece of which the row sees nothing
+    float top_new = ml.x;
 #pragma unroll
-      for (int x = 0; x < kVecs; ++x) o[64 * x] = o[64 * x + 1] = __floats2bfloat162_rn(0.f, 0.f);
-      if (lane == 0) *lse = -CUDART_INF_F;
-      continue;
+    for (int o = 16; o > 0; o >>= 1) top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, o));
+    top_new = fmaxf(top, top_new);
+    if (top_new == -CUDART_INF_F) continue;
+    const float a = exp2f(top - top_new), w = exp2f(ml.x - top_new);
+    float l = ml.y * w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    sum = sum * a + l;
+    top = top_new;
+#pragma unroll
+    for (int x = 0; x < kVecs; ++x) acc[x] = make_float4(acc[x].x * a, acc[x].y * a, acc[x].z * a, acc[x].w * a);
+    const uint32_t counts = __ballot_sync(0xffffffffu, ml.x > -CUDART_INF_F);
+#pragma unroll 8
+    for (int k = 0; k < min(32, n - i0); ++k) {
+      const float w_k = __shfl_sync(0xffffffffu, w, k);
+      const int64_t at_k = __shfl_sync(0xffffffffu, at, k);
+      if (!((counts >> k) & 1)) continue;
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x) {
+        const float4 v = reinterpret_cast<const float4*>(p.part_o + at_k * D)[32 * x + lane];
+        acc[x] = make_float4(acc[x].x + v.x * w_k, acc[x].y + v.y * w_k, acc[x].z + v.z * w_k, acc[x].w + v.w * w_k);
+      }
     }
-    if (unit.x < 0) continue;                                 // whole: written by its CTA
-    float top = -CUDART_INF_F, sum = 0.f;
-    float4 acc[kVecs] = {};
-    const int halves = kRows == 256 && s.count * p.rep - r / kRows * kRows <= 128 ? 2 : 1;      // a split unit's pieces have two results
-    const int first = unit.x / 2 * halves, n = unit.y * halves + halves;
-    for (int i = first; i < n; ++i) {
-      const int c = i / halves;
-      const int64_t at = static_cast<int64_t>(c == unit.x / 2 ? unit.x : 2 * c) * kRows + (r & (kRows - 1)) + (i - c * halves) * 128;
-      const float2 ml = p.part_ml[at];
-      if (ml.x == -CUDART_INF_F) continue;                    // a piece of which the row sees nothing
-      float4 v[kVecs];
+  }
+  const float inv = 1.f / sum;
 #pragma unroll
-      for (int x = 0; x < kVecs; ++x) v[x] = reinterpret_cast<const float4*>(p.part_o + at * D)[32 * x + lane];
-      const float top_new = fmaxf(top, ml.x), a = exp2f(top - top_new), w = exp2f(ml.x - top_new);
-      sum = sum * a + ml.y * w;
-#pragma unroll
-      for (int x = 0; x < kVecs; ++x)
-        acc[x] = make_float4(acc[x].x * a + v[x].x * w, acc[x].y * a + v[x].y * w, acc[x].z * a + v[x].z * w, acc[x].w * a + v[x].w * w);
-      top = top_new;
-    }
-    const float inv = 1.f / sum;
-#pragma unroll
-    for (int x = 0; x < kVecs; ++x) {
-      o[64 * x] = __floats2bfloat162_rn(acc[x].x * inv, acc[x].y * inv);
-      o[64 * x + 1] = __floats2bfloat162_rn(acc[x].z * inv, acc[x].w * inv);
-    }
-    if (lane == 0) {
-      *lse = (top + log2f(sum)) * kLn2;
-      if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(p.factors[padded_row], top + log2f(sum));
-    }
+  for (int x = 0; x < kVecs; ++x) {
+    o[64 * x] = __floats2bfloat162_rn(acc[x].x * inv, acc[x].y * inv);
+    o[64 * x + 1] = __floats2bfloat162_rn(acc[x].z * inv, acc[x].w * inv);
+  }
+  if (lane == 0) {
+    *lse = (top + log2f(sum)) * kLn2;
+    if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(p.factors[padded_row], top + log2f(sum));
   }
 }
 
@@ -1185,7 +1210,7 @@ static cudaError_t launch_chunk(const CUtensorMap& tk, const CUtensorMap& tv, co
   e = launch_chained(cache_chunk_kernel<D>, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, tq, p);
   if (e != cudaSuccess) return e;
   count_launch();
-  const int groups = (p.Nq * p.rep + 7) / 8;
+  const int groups = (p.Nq * p.rep + 3) / 4;
   e = launch_chained(cache_chunk_join_kernel<D>, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * groups), 128, 0, stream, p);
   if (e != cudaSuccess || p.weights == nullptr) return e;
   const int tiles_of_row = (p.W + 127) / 128;                 // what lies beyond the length too: its weights are zeros
