@@ -40,7 +40,6 @@ struct ChunkCfg {
   static constexpr int kPanels = D / 64;                      // of 64 columns, of an f16 operand tile
   static constexpr int kCols = kWide ? 64 : 128;              // keys of a tile that a softmax group looks after
   static constexpr int kTile = 128 * 128;                     // 128 keys x 128 codes; also an f16 panel of 128 rows
-  static constexpr int kChunks = 2 * D / 128;                 // pieces of kTile in which the codes of a key tile come: K, then V
   static constexpr int kVBufs = kWide ? 1 : 2;
   static constexpr int kSmemQ = 0;                            // row tiles x panels
   static constexpr int kSmemK = 4 * kTile;                    // between the uses of two tiles lies a softmax, longer than a conversion
@@ -914,34 +913,37 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
 
 // ------------------------------------------------------------------------------------------------ weights
 // weights[b, hk, j] (+)= sum over the rows r that see token j of exp(s_rj) / sum_r = 2^(f_r ks s_rj - c_r), c_r = log2 of the row's sum.
-// S^T = K Q^T on tcgen05 with 128 tokens as M and 256 rows as N: a token's sum stays in its thread (TMEM lane) over all row tiles, in the order of the
-// rows.  An item is a key tile of a (sequence, head): its codes become an f16 tile once, the row tiles pass by.  Warps 0-3 take rows 0-127 of each row
-// tile, warps 4-7 the others; warp 8: TMA, warp 9: MMA.  Two S^T buffers of 256 columns.  Bound by its exponentials (2048 cycles of 32768).
+// S^T = K Q^T on tcgen05 with 128 tokens as M and up to 128 rows as N: a token's sum stays in its thread (TMEM lane) over all row tiles, in
+// the order of the rows.  An item is a key tile of a (sequence, head): its codes become an f16 tile once, the row tiles pass by.  Where a
+// head has but one row tile it stays for the next items of the head.  Warps 0-3 and 4-7 take row tiles in turn (32 rows each of an only one);
+// warp 8: TMA, warp 9: MMA.  Four S^T buffers of 128 columns.
 // The first row that sees token j.
 __device__ __forceinline__ int first_row(const CacheAttnParams& p, const ChunkSeq& s, int j) { return p.causal ? max(0, j - s.n + s.count) * p.rep : 0; }
 
 template <int D>
 struct ChunkWeightsCfg {
   static constexpr int kThreads = 320;
-  static constexpr int kRows = ChunkCfg<D>::kRows, kHalf = kRows / 2;          // of a row tile; of a softmax group
+  static constexpr int kRows = 128;                           // of a row tile
   static constexpr int kPanels = D / 64;
   static constexpr int kTile = 128 * 128;
-  static constexpr int kQBytes = 4 * kTile;                   // panels of kRows x 128 bytes
-  static constexpr int kSmemK = 2 * kQBytes;                  // panels
-  static constexpr int kCodeBufs = D == 128 ? 2 : 1;          // what fits of the pieces of kTile in which codes come
-  static constexpr int kChunks = D / 128;
+  static constexpr int kQBytes = kPanels * kTile;             // of a row tile
+  static constexpr int kQBufs = D == 128 ? 4 : 2, kQShift = D == 128 ? 2 : 1;
+  static constexpr int kSmemK = kQBufs * kQBytes;             // panels
+  static constexpr int kChunks = D / 128;                     // pieces of kTile in which an item's codes come
+  static constexpr int kCodeBufs = D == 128 ? 3 : 1;          // what fits of them
   static constexpr int kSmemCode = kSmemK + kPanels * kTile;
   static constexpr int kSmemRows = kSmemCode + kCodeBufs * kTile;     // (factor, log2 sum) of the rows, by row tile buffer
-  static constexpr int kSmemSums = kSmemRows + 2 * kRows * 8;
-  static constexpr int kSmemBars = kSmemSums + 128 * 4;
+  static constexpr int kSmemSums = kSmemRows + kQBufs * kRows * 8;    // by parity of the item
+  static constexpr int kSmemBars = kSmemSums + 2 * 128 * 4;
   static constexpr int kSmem = kSmemBars + 256 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
-enum ChunkWeightsBar : int { kwCode = 0, kwCodeFree = 2, kwQ = 4, kwQFree = 6, kwS = 8, kwSFree = 10, kwK = 12, kwSums = 13, kwSumsFree = 14, kwBars = 15 };
+enum ChunkWeightsBar : int { kwCode = 0, kwCodeFree = 3, kwQ = 6, kwQFree = 10, kwS = 14, kwSFree = 18, kwK = 22, kwSums = 23, kwSumsFree = 25, kwBars = 27 };
 
 template <int D>
 __global__ void __launch_bounds__(ChunkWeightsCfg<D>::kThreads, 1)
-cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tq, const CacheAttnParams p, const int tiles_of_row) {
+cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tq, const CacheAttnParams p, const int tiles_of_row,
+                           const int run) {
   using C = ChunkWeightsCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -953,17 +955,21 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
   float* sums = reinterpret_cast<float*>(smem + C::kSmemSums);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bars + kwCode + i, 1);
-      mbar_init(bars + kwCodeFree + i, 8);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(bars + kwQ + i, 1);
       mbar_init(bars + kwQFree + i, 9);                       // the MMA, and the warps that read the rows' constants
       mbar_init(bars + kwS + i, 1);
       mbar_init(bars + kwSFree + i, 8);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bars + kwSums + i, 4);
+      mbar_init(bars + kwSumsFree + i, 4);
+    }
+    for (int i = 0; i < C::kCodeBufs; ++i) {
+      mbar_init(bars + kwCode + i, 1);
+      mbar_init(bars + kwCodeFree + i, 8);
+    }
     mbar_init(bars + kwK, 8);
-    mbar_init(bars + kwSums, 4);
-    mbar_init(bars + kwSumsFree, 4);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tk);
@@ -980,195 +986,279 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
   const uint32_t tmem = *tmem_slot;
   auto bar = [&](int i) { return smem_u32(bars + i); };
   const int R = p.Nq * p.rep, row_tiles_max = (R + 127) / 128;
-  const int64_t items = static_cast<int64_t>(p.c.B) * p.c.Hk * tiles_of_row;
+  const int items = p.c.B * p.c.Hk * tiles_of_row;            // 128 weights each: they fit
   bool ok = true;
   // Item i: a key tile that exists, and its row tiles that see any of it: rt0 ... rt1 - 1.
   struct Item {
     int b, hk, t, n, rt0, rt1;
     ChunkSeq s;
   };
-  auto item_at = [&](int64_t i, Item& x) {
-    const int bh = static_cast<int>(i / tiles_of_row);
-    x.t = static_cast<int>(i - static_cast<int64_t>(bh) * tiles_of_row);
+  auto item_at = [&](int i, Item& x) {
+    const int bh = i / tiles_of_row;
+    x.t = i - bh * tiles_of_row;
     x.b = bh / p.c.Hk;
     x.hk = bh - x.b * p.c.Hk;
     x.s = chunk_seq(p, x.b);
     x.n = x.s.n;
-    x.rt1 = x.s.units;
+    x.rt1 = (x.s.count * p.rep + C::kRows - 1) / C::kRows;
     x.rt0 = min(x.rt1, first_row(p, x.s, 128 * x.t) / C::kRows);
     return 128 * x.t < x.n;
   };
-  int g = 0, j = 0, q = 0;                                    // running item, running piece of codes, running row tile
-  Item x;
+  // The CTA's items that some row sees, one by one: runs of them, a grid apart (n: where it stands, k: in the run).
+  struct Place {
+    int n, k;
+  };
+  const int runs = (items + run - 1) / run;
+  auto find = [&](Place& at, Item& x, auto&& unseen) {
+    while (at.n < runs) {
+      const int i = at.n * run + at.k;
+      if (++at.k == run) {
+        at.k = 0;
+        at.n += gridDim.x;
+      }
+      if (i >= items) continue;
+      if (item_at(i, x) && x.rt0 < x.rt1) return true;
+      unseen(x);
+    }
+    return false;
+  };
+  // y's row tile is x's, the only one of both: it stays where it is.
+  auto same_rows = [](const Item& x, const Item& y) { return x.b == y.b && x.hk == y.hk && x.rt0 == y.rt0 && x.rt1 - x.rt0 == 1 && y.rt1 - y.rt0 == 1; };
+  auto none = [](const Item&) {};
+  Place n{static_cast<int>(blockIdx.x), 0};
+  int q = 0;                                                  // row tiles loaded
+  bool fresh = true;                                          // this item's are loaded for it
+  Item x, y;                                                  // this item, the next one
+  bool live = find(n, x, none);
   if (warp == 8) {
     // ------------------------------------------------------------------------------------------ TMA
     const int bpp = p.c.page / 32;
-    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
-      if (!item_at(i, x) || x.rt0 >= x.rt1) continue;
+    int j = 0;                                                // running piece of codes
+    auto load_codes = [&](const Item& x) {
       const int blk = 4 * x.t + lane, entry = blk / bpp;
       const bool held = lane < 4 && blk * 32 < x.n;
       const int page = held ? max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + entry))) : 0;
       const int boxes = __popc(__ballot_sync(0xffffffffu, held));
-      for (int c = 0; c < C::kChunks && ok; ++c, ++j) {
+      for (int c = 0; c < C::kChunks; ++c, ++j) {
         const int buf = j % C::kCodeBufs;
-        if (j >= C::kCodeBufs && !(ok = wait_warp(bar(kwCodeFree + buf), (j / C::kCodeBufs - 1) & 1, abort_flag))) break;
+        if (j >= C::kCodeBufs && !(ok = wait_warp(bar(kwCodeFree + buf), (j / C::kCodeBufs - 1) & 1, abort_flag))) return;
         if (lane == 0) mbar_expect_tx(bars + kwCode + buf, boxes * 4096);
         __syncwarp();
         if (held) tma_load_4d(sbase + C::kSmemCode + buf * C::kTile + lane * 4096, &tk, bar(kwCode + buf), 128 * c, (blk - entry * bpp) * 32, x.hk, page);
       }
-      if (!ok) break;
-      for (int rt = x.rt0; rt < x.rt1; ++rt, ++q) {
-        if (q >= 2 && !(ok = wait_warp(bar(kwQFree + (q & 1)), ((q >> 1) - 1) & 1, abort_flag))) break;
+    };
+    if (live) load_codes(x);
+    while (live && ok) {
+      const bool more = find(n, y, none);
+      if (C::kChunks <= C::kCodeBufs && more) load_codes(y);  // (otherwise its second piece would wait for this item's end)
+      for (int rt = x.rt0; rt < x.rt1 && fresh && ok; ++rt, ++q) {
+        const int qb = q & (C::kQBufs - 1);
+        if (q >= C::kQBufs && !(ok = wait_warp(bar(kwQFree + qb), ((q >> C::kQShift) - 1) & 1, abort_flag))) break;
         if (lane == 0) {
-          // the last row tile of a head may lack its second half: those columns hold what was there, and its rows see nothing
-          constexpr int kParts = C::kRows / 128;
-          const int tile0 = (x.b * p.c.Hk + x.hk) * row_tiles_max + kParts * rt, parts = min(kParts, row_tiles_max - kParts * rt);
-          const uint32_t to = (q & 1) * C::kQBytes;
-          mbar_expect_tx(bars + kwQ + (q & 1), parts * (C::kPanels * C::kTile + 1024));
-          for (int r = 0; r < parts; ++r) {
-            for (int panel = 0; panel < C::kPanels; ++panel)
-              tma_load_2d(smem + to + (panel * kParts + r) * C::kTile, &tq, bars + kwQ + (q & 1), 128 * panel, (tile0 + r) * 128);
-            bulk_load_1d(smem + C::kSmemRows + ((q & 1) * kParts + r) * 1024, p.row_ml + static_cast<int64_t>(tile0 + r) * 128, 1024, bars + kwQ + (q & 1));
-          }
+          const int tile = (x.b * p.c.Hk + x.hk) * row_tiles_max + rt;
+          mbar_expect_tx(bars + kwQ + qb, C::kQBytes + 1024);
+          for (int panel = 0; panel < C::kPanels; ++panel)
+            tma_load_2d(smem + qb * C::kQBytes + panel * C::kTile, &tq, bars + kwQ + qb, 128 * panel, tile * 128);
+          bulk_load_1d(smem + C::kSmemRows + qb * 1024, p.row_ml + static_cast<int64_t>(tile) * 128, 1024, bars + kwQ + qb);
         }
         __syncwarp();
       }
+      if (C::kChunks > C::kCodeBufs && more && ok) load_codes(y);
+      fresh = more && !same_rows(x, y);
+      x = y;
+      live = more;
     }
     if (!ok) {
       if (lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutProducer + kInCache);
-      for (int k = 1; k <= 2; ++k) {                          // what is in flight lands before the shared memory goes
-        if (j >= k && k <= C::kCodeBufs) wait_or_abort(bar(kwCode + (j - k) % C::kCodeBufs), (j - k) / C::kCodeBufs & 1, abort_flag);
-        if (q >= k) wait_or_abort(bar(kwQ + ((q - k) & 1)), ((q - k) >> 1) & 1, abort_flag);
-      }
+      for (int k = 1; k <= C::kCodeBufs; ++k)                 // what is in flight lands before the shared memory goes
+        if (j >= k) wait_or_abort(bar(kwCode + (j - k) % C::kCodeBufs), (j - k) / C::kCodeBufs & 1, abort_flag);
+      for (int k = 1; k <= C::kQBufs; ++k)
+        if (q >= k) wait_or_abort(bar(kwQ + ((q - k) & (C::kQBufs - 1))), ((q - k) >> C::kQShift) & 1, abort_flag);
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------------------------------------ MMA
     if (elect_one()) {
-      constexpr uint32_t kIdesc = idesc_f8(128, C::kRows, false, false);
       const uint32_t k_lo = desc_lo(sbase + C::kSmemK), q_lo = desc_lo(sbase);
-      for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
-        if (!item_at(i, x) || x.rt0 >= x.rt1) continue;
+      int s = 0;                                              // running product
+      for (int g = 0; live && ok; ++g) {
+        const bool more = find(n, y, none), stays = more && same_rows(x, y);
         if (!(ok = wait_or_abort(bar(kwK), g & 1, abort_flag))) break;
-        ++g;
-        for (int rt = x.rt0; rt < x.rt1; ++rt, ++q) {
-          if (!(ok = wait_or_abort(bar(kwQ + (q & 1)), (q >> 1) & 1, abort_flag))) break;
-          if (q >= 2 && !(ok = wait_or_abort(bar(kwSFree + (q & 1)), ((q >> 1) - 1) & 1, abort_flag))) break;
+        for (int rt = x.rt0; rt < x.rt1; ++rt, ++s) {
+          if (fresh && !(ok = wait_or_abort(bar(kwQ + (q & (C::kQBufs - 1))), (q >> C::kQShift) & 1, abort_flag))) break;
+          q += fresh;
+          if (s >= 4 && !(ok = wait_or_abort(bar(kwSFree + (s & 3)), ((s >> 2) - 1) & 1, abort_flag))) break;
           tc_fence_after();
+          const int qb = (q - 1) & (C::kQBufs - 1), rows = min(C::kRows, x.s.count * p.rep - rt * C::kRows);
+          const uint32_t idesc = idesc_f8(128, (rows + 31) / 32 * 32, false, false);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_h_ss(tmem + 256 * (q & 1), k_lo + (k >> 2) * (C::kTile >> 4) + (k & 3) * 2,
-                     q_lo + (q & 1) * (C::kQBytes >> 4) + (k >> 2) * (C::kRows * 128 >> 4) + (k & 3) * 2, kIdesc, k > 0);
-          tc_commit(bars + kwQFree + (q & 1));
-          tc_commit(bars + kwS + (q & 1));
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = (k >> 2) * (C::kTile >> 4) + (k & 3) * 2;
+            mma_h_ss(tmem + 128 * (s & 3), k_lo + off, q_lo + qb * (C::kQBytes >> 4) + off, idesc, k > 0);
+          }
+          if (!stays) tc_commit(bars + kwQFree + qb);
+          tc_commit(bars + kwS + (s & 3));
         }
+        fresh = !stays;
+        x = y;
+        live = more;
       }
       if (!ok) raise_abort(abort_flag, p.c.status, kStatusTimeoutMma + kInCache);
     }
   } else {
     // ------------------------------------------------------------------------------------------ codes, exponentials, sums
-    const int half = warp >> 2, key = (warp & 3) * 32 + lane;           // rows of a tile; token of a tile = TMEM lane
+    const int half = warp >> 2, key = (warp & 3) * 32 + lane;           // token of a tile = TMEM lane
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    int it = 0;
-    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x, ++it) {
-      const bool exists = item_at(i, x);
-      float total = 0.f;
-      const int tok = 128 * x.t + key;
-      if (exists && x.rt0 < x.rt1) {
-        float ks = 0.f;                                       // of this token's block
-        if (tok < x.n) {
-          const int page = max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + tok / p.c.page)));
-          ks = __ldg(p.c.ks + page * p.c.s_page + x.hk * p.c.s_head + tok % p.c.page / 32);
-        }
-        // as in the main kernel: 16-byte pieces c of keys tid / 8, + 32, ...; the f16 tile is free, all its products having been seen
-        for (int part = 0; part < C::kChunks; ++part, ++j) {
-          const int buf = j % C::kCodeBufs;
-          if (!(ok = wait_warp(bar(kwCode + buf), j / C::kCodeBufs & 1, abort_flag))) break;
-          const int c = tid & 7, panel = c >> 2, cc = (c & 3) * 2;
-          const uint32_t src = sbase + C::kSmemCode + buf * C::kTile, dst = sbase + C::kSmemK + (2 * part + panel) * C::kTile;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int row = (tid >> 3) + 32 * k;
-            const float4 w4 = lds_f4(src + row * 128 + ((c ^ (row & 7)) << 4));
-            const uint32_t w[4] = {__float_as_uint(w4.x), __float_as_uint(w4.y), __float_as_uint(w4.z), __float_as_uint(w4.w)};
-            uint32_t h[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              h[2 * e] = e4m3_lo_f16x2(w[e]);
-              h[2 * e + 1] = e4m3_hi_f16x2(w[e]);
-            }
-            const int flip = panel;                           // which half first: eight lanes' stores on different banks
-            sts_u4(dst + row * 128 + (((cc + flip) ^ (row & 7)) << 4), flip ? h[4] : h[0], flip ? h[5] : h[1], flip ? h[6] : h[2], flip ? h[7] : h[3]);
-            sts_u4(dst + row * 128 + (((cc + 1 - flip) ^ (row & 7)) << 4), flip ? h[0] : h[4], flip ? h[1] : h[5], flip ? h[2] : h[6], flip ? h[3] : h[7]);
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(bars + kwCodeFree + buf);
-            if (part == C::kChunks - 1) mbar_arrive(bars + kwK);
-          }
-        }
-        if (!ok) break;
-        ++g;
-        for (int rt = x.rt0; rt < x.rt1; ++rt, ++q) {
-          // the products; and the rows' constants, seen by this warp itself
-          if (!(ok = wait_warp(bar(kwS + (q & 1)), (q >> 1) & 1, abort_flag) && wait_warp(bar(kwQ + (q & 1)), (q >> 1) & 1, abort_flag))) break;
-          tc_fence_after();
-          const int row0 = rt * C::kRows + half * C::kHalf;
-          if (row0 < x.s.count * p.rep) {
-            const int from_row = first_row(p, x.s, tok) - row0;                 // of mine, the first that sees this token
-            const bool cut = __any_sync(0xffffffffu, from_row > 0);
-            const uint32_t from = tmem + lanes + 256 * (q & 1) + C::kHalf * half, rows = sbase + C::kSmemRows + ((q & 1) * C::kRows + half * C::kHalf) * 8;
-            uint32_t s_buf[2][32];
-            tmem_ld32(from, s_buf[0]);
+    auto weight_at = [&](const Item& x) { return p.weights + x.b * p.w_sb + x.hk * p.w_sh + 128 * x.t + key; };
+    auto zeros = [&](const Item& x) {
+      if (half == 0 && !p.accumulate && 128 * x.t + key < p.W) *weight_at(x) = 0.f;
+    };
+    int j = 0;                                                // running piece of codes
+    // An item's codes as its f16 tile, as in the main kernel: 16-byte pieces c of keys tid / 8, + 32, ...  All products of the last item have been seen.
+    auto convert = [&]() {
 #pragma unroll 1
-            for (int c2 = 0; c2 < C::kHalf / 64; ++c2) {
+      for (int part = 0; part < C::kChunks && ok; ++part, ++j) {
+        const int buf = j % C::kCodeBufs;
+        if (!(ok = wait_warp(bar(kwCode + buf), j / C::kCodeBufs & 1, abort_flag))) break;
+        const int c = tid & 7, panel = c >> 2, cc = (c & 3) * 2;
+        const uint32_t src = sbase + C::kSmemCode + buf * C::kTile, dst = sbase + C::kSmemK + (2 * part + panel) * C::kTile;
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                tmem_wait_ld();
-                if (!(c2 == C::kHalf / 64 - 1 && k == 1)) tmem_ld32(from + 64 * c2 + 32 * (k + 1), s_buf[k ^ 1]);
-                float2 sum = make_float2(0.f, 0.f);
+        for (int k = 0; k < 4; ++k) {
+          const int row = (tid >> 3) + 32 * k;
+          const float4 w4 = lds_f4(src + row * 128 + ((c ^ (row & 7)) << 4));
+          const uint32_t w[4] = {__float_as_uint(w4.x), __float_as_uint(w4.y), __float_as_uint(w4.z), __float_as_uint(w4.w)};
+          uint32_t h[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const float4 fc = lds_f4(rows + (64 * c2 + 32 * k + 2 * e) * 8);        // factor and log2 sum of two rows
-                  float2 y = fma2(mul2(make_float2(__uint_as_float(s_buf[k][2 * e]), __uint_as_float(s_buf[k][2 * e + 1])), make_float2(fc.x, fc.z)), splat2(ks),
-                                  make_float2(-fc.y, -fc.w));
-                  if (cut) {
-                    if (64 * c2 + 32 * k + 2 * e < from_row) y.x = -CUDART_INF_F;
-                    if (64 * c2 + 32 * k + 2 * e + 1 < from_row) y.y = -CUDART_INF_F;
-                  }
-                  sum = add2(sum, ex2_2(y));
-                }
-                total += sum.x + sum.y;
+          for (int e = 0; e < 4; ++e) {
+            h[2 * e] = e4m3_lo_f16x2(w[e]);
+            h[2 * e + 1] = e4m3_hi_f16x2(w[e]);
+          }
+          const int flip = panel;                             // which half first: eight lanes' stores on different banks
+          sts_u4(dst + row * 128 + (((cc + flip) ^ (row & 7)) << 4), flip ? h[4] : h[0], flip ? h[5] : h[1], flip ? h[6] : h[2], flip ? h[7] : h[3]);
+          sts_u4(dst + row * 128 + (((cc + 1 - flip) ^ (row & 7)) << 4), flip ? h[0] : h[4], flip ? h[1] : h[5], flip ? h[2] : h[6], flip ? h[3] : h[7]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bars + kwCodeFree + buf);
+          if (part == C::kChunks - 1) mbar_arrive(bars + kwK);
+        }
+      }
+    };
+    // of this thread's token: its page, and the scale of its block
+    auto page_of = [&](const Item& x) {
+      const int tok = 128 * x.t + key;
+      return tok < x.n ? max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + tok / p.c.page))) : 0;
+    };
+    auto scale_of = [&](const Item& x, int page) {
+      const int tok = 128 * x.t + key;
+      return tok < x.n ? __ldg(p.c.ks + page * p.c.s_page + x.hk * p.c.s_head + tok % p.c.page / 32) : 0.f;
+    };
+    // of the last item: this half's sum, where it goes, whether the token exists
+    float mine = 0.f;
+    float* at = nullptr;
+    bool held = false;
+    int last = -1;
+    auto finish = [&](int g) -> bool {
+      if (!wait_warp(bar(kwSums + (g & 1)), (g >> 1) & 1, abort_flag)) return false;
+      mine += sums[128 * (g & 1) + key];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + kwSumsFree + (g & 1));
+      if (at != nullptr) *at = !held ? 0.f : p.accumulate ? *at + mine : mine;
+      return true;
+    };
+    n = Place{static_cast<int>(blockIdx.x), 0};
+    live = find(n, x, zeros);
+    float ks = live ? scale_of(x, page_of(x)) : 0.f;
+    int s = 0;                                                // running product
+    for (int g = 0; live && ok; ++g) {
+      convert();
+      if (!ok) break;
+      // while the first product is under way
+      const bool more = find(n, y, zeros), stays = more && same_rows(x, y);
+      const int next_page = more ? page_of(y) : 0;
+      const int tok = 128 * x.t + key;
+      float total = 0.f;
+      for (int rt = x.rt0; rt < x.rt1; ++rt, ++s) {
+        q += fresh;
+        const int qb = (q - 1) & (C::kQBufs - 1);
+        // the products; and the rows' constants, seen by this warp itself
+        if (!(ok = wait_warp(bar(kwS + (s & 3)), (s >> 2) & 1, abort_flag) && wait_warp(bar(kwQ + qb), ((q - 1) >> C::kQShift) & 1, abort_flag))) break;
+        tc_fence_after();
+        const int parts = (min(C::kRows, x.s.count * p.rep - rt * C::kRows) + 31) / 32;    // of 32 rows
+        const int from_row = first_row(p, x.s, tok) - rt * C::kRows;      // of the row tile, the first that sees this token
+        const bool cut = __any_sync(0xffffffffu, from_row > 0);
+        const uint32_t from = tmem + lanes + 128 * (s & 3), rows = sbase + C::kSmemRows + qb * 1024;
+        uint32_t s_buf[2][32];
+        auto part_sum = [&](int c, const uint32_t (&v)[32], auto cut_tag) {
+          constexpr bool kCut = decltype(cut_tag)::value;     // some token of the warp is not seen by all rows
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e8 = 0; e8 < 16; e8 += 8) {
+            float4 fc[8];                                     // factors and log2 sums of two rows each, asked for together
+#pragma unroll
+            for (int e = 0; e < 8; ++e) fc[e] = lds_f4(rows + (32 * c + 2 * (e8 + e)) * 8);
+            float2 z[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              z[e] = fma2(mul2(make_float2(__uint_as_float(v[2 * (e8 + e)]), __uint_as_float(v[2 * (e8 + e) + 1])), make_float2(fc[e].x, fc[e].z)), splat2(ks),
+                          make_float2(-fc[e].y, -fc[e].w));
+              if (kCut) {
+                if (32 * c + 2 * (e8 + e) < from_row) z[e].x = -CUDART_INF_F;
+                if (32 * c + 2 * (e8 + e) + 1 < from_row) z[e].y = -CUDART_INF_F;
               }
             }
-            tc_fence_before();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = ex2_2(z[e]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = add2(sum, z[e]);
           }
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(bars + kwSFree + (q & 1));
-            mbar_arrive(bars + kwQFree + (q & 1));
+          total += sum.x + sum.y;
+        };
+        auto parts_from = [&](int c, int step, auto cut_tag) {
+          if (c < parts) tmem_ld32(from + 32 * c, s_buf[0]);
+#pragma unroll 1
+          for (; c < parts; c += 2 * step) {
+            tmem_wait_ld();
+            if (c + step < parts) tmem_ld32(from + 32 * (c + step), s_buf[1]);
+            part_sum(c, s_buf[0], cut_tag);
+            if (c + step >= parts) break;
+            tmem_wait_ld();
+            if (c + 2 * step < parts) tmem_ld32(from + 32 * (c + 2 * step), s_buf[0]);
+            part_sum(c + step, s_buf[1], cut_tag);
           }
+        };
+        // the two groups of warps: halves of an only row tile, or every second one
+        const bool only = x.rt1 - x.rt0 == 1;
+        const int first = only ? half : (rt - x.rt0 & 1) == half ? 0 : parts, step = only ? 2 : 1;
+        if (cut) parts_from(first, step, std::true_type{});
+        else parts_from(first, step, std::false_type{});
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bars + kwSFree + (s & 3));
+          if (!stays) mbar_arrive(bars + kwQFree + qb);
         }
-        if (!ok) break;
       }
-      // the two halves' sums, and zeros beyond the length
+      if (!ok) break;
+      ks = more ? scale_of(y, next_page) : 0.f;
+      // The two halves' sums: the second leaves its own, the first picks it up an item later.
       if (half == 1) {
-        if (it > 0 && !(ok = wait_warp(bar(kwSumsFree), (it - 1) & 1, abort_flag))) break;
-        sums[key] = total;
+        if (g >= 2 && !(ok = wait_warp(bar(kwSumsFree + (g & 1)), ((g >> 1) - 1) & 1, abort_flag))) break;
+        sums[128 * (g & 1) + key] = total;
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kwSums);
+        if (lane == 0) mbar_arrive(bars + kwSums + (g & 1));
       } else {
-        if (!(ok = wait_warp(bar(kwSums), it & 1, abort_flag))) break;
-        total += sums[key];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kwSumsFree);
-        if (tok < p.W) {
-          float* at = p.weights + x.b * p.w_sb + x.hk * p.w_sh + tok;
-          if (tok < x.n) *at = p.accumulate ? *at + total : total;
-          else if (!p.accumulate) *at = 0.f;
-        }
+        if (g > 0 && !(ok = finish(g - 1))) break;
+        mine = total;
+        at = tok < x.n || (!p.accumulate && tok < p.W) ? weight_at(x) : nullptr;
+        held = tok < x.n;
       }
+      last = g;
+      fresh = !stays;
+      x = y;
+      live = more;
     }
+    if (ok && half == 0 && last >= 0) ok = finish(last);
     if (!ok && lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
   }
   __syncwarp();
@@ -1215,9 +1305,12 @@ static cudaError_t launch_chunk(const CUtensorMap& tk, const CUtensorMap& tv, co
   if (e != cudaSuccess || p.weights == nullptr) return e;
   const int tiles_of_row = (p.W + 127) / 128;                 // what lies beyond the length too: its weights are zeros
   const int64_t items = static_cast<int64_t>(p.c.B) * p.c.Hk * tiles_of_row;
+  // One row tile stays where it is for a run of four items; several pass by in any case, and items one by one divide more evenly.
+  const int run = p.Nq * p.rep <= 128 && items >= 16ll * sm_count() ? 4 : 1;
+  const int64_t n_runs = (items + run - 1) / run;
   count_launch();
-  return launch_chained(cache_chunk_weights_kernel<D>, dim3(static_cast<unsigned>(items < sm_count() ? items : sm_count())), ChunkWeightsCfg<D>::kThreads,
-                        ChunkWeightsCfg<D>::kSmem, stream, tk, tq, p, tiles_of_row);
+  return launch_chained(cache_chunk_weights_kernel<D>, dim3(static_cast<unsigned>(n_runs < sm_count() ? n_runs : sm_count())), ChunkWeightsCfg<D>::kThreads,
+                        ChunkWeightsCfg<D>::kSmem, stream, tk, tq, p, tiles_of_row, run);
 }
 
 cudaError_t launch_cache_chunk(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
