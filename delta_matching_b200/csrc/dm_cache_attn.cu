@@ -31,14 +31,10 @@ struct AttnCfg {
   static constexpr int kRows = 8 * NT;
   static constexpr int kSlotBytes = 32 * D;                   // K or V of a block
   static constexpr int kCtasPerSm = D == 128 && NT == 1 ? 3 : 2;
-  // 32 rows: the query fragments wait in shared memory (64 registers beside an accumulator of 128 spilled: B=8 with 4096 - 8192 tokens, H=32 Hk=8,
-  // 8 new tokens 79 us against 57)
-  static constexpr bool kSharedQ = NT == 4;
   static constexpr int kSlots = D == 128 ? (NT == 2 ? 6 : 4) : 3;
   static constexpr int kRing = kWarps * kSlots * kSlotBytes;
-  static constexpr int kQBytes = kSharedQ ? NT * D * 16 : 0;  // of a warp
   static constexpr int kStats = kWarps * kRows * 8;           // maximum and sum of a warp's rows, for the CTA's own join
-  static constexpr int kSmem = 1024 + kRing + kWarps * kQBytes + kStats + kWarps * kSlots * 8 + 136 * 4 + 64;
+  static constexpr int kSmem = 1024 + kRing + kStats + kWarps * kSlots * 8 + 136 * 4 + 64;
   static_assert(NT * D * 32 <= kSlots * kSlotBytes, "a warp leaves its accumulator in its ring");
 };
 
@@ -105,10 +101,9 @@ __device__ __forceinline__ void load_queries(const CacheAttnParams& p, int b, in
   scale_queries<D, NT>(p, qf, f);
 }
 
-// S^T of a block: acc[j][mt] rows: keys 16 mt + g (elements 0, 1) and + 8 (2, 3); columns: query rows 8 j + 2 t, + 1.  The query fragments
-// come from registers, or (kShared) from q_sm: fragment (j, c) of this lane 8 bytes at (j D / 16 + c) 256.
-template <int D, int NT, bool kShared>
-__device__ __forceinline__ void keys_times_queries(uint32_t kbase, uint32_t q_sm, const uint32_t (&qf)[NT][D / 16][2], float (&s)[NT][2][4]) {
+// S^T of a block: acc[j][mt] rows: keys 16 mt + g (elements 0, 1) and + 8 (2, 3); columns: query rows 8 j + 2 t, + 1.
+template <int D, int NT>
+__device__ __forceinline__ void keys_times_queries(uint32_t kbase, const uint32_t (&qf)[NT][D / 16][2], float (&s)[NT][2][4]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -131,15 +126,7 @@ __device__ __forceinline__ void keys_times_queries(uint32_t kbase, uint32_t q_sm
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      uint32_t q0, q1;
-      if (kShared) {
-        const float2 q = lds_f2(q_sm + (j * (D / 16) + c) * 256);
-        q0 = __float_as_uint(q.x);
-        q1 = __float_as_uint(q.y);
-      } else {
-        q0 = qf[j][c][0];
-        q1 = qf[j][c][1];
-      }
+      const uint32_t q0 = qf[j][c][0], q1 = qf[j][c][1];
       mma_f16(kTwo && (c & 1) ? s2[kTwo ? j : 0][0] : s[j][0], lo[0], lo[1], hi[0], hi[1], q0, q1);
       mma_f16(kTwo && (c & 1) ? s2[kTwo ? j : 0][1] : s[j][1], lo[2], lo[3], hi[2], hi[3], q0, q1);
     }
@@ -162,8 +149,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
-  float2* stats = reinterpret_cast<float2*>(smem + C::kRing + C::kWarps * C::kQBytes);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kWarps * C::kQBytes + C::kStats);
+  float2* stats = reinterpret_cast<float2*>(smem + C::kRing);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kStats);
   int* cum = reinterpret_cast<int*>(bars + C::kWarps * C::kSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(cum + 134);
   __shared__ int left_unit[C::kWarps], left_end[C::kWarps];   // what a warp leaves to the CTA's join: its unit (-1: nothing), its last block
@@ -215,7 +202,6 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
   const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
   const uint32_t my_bars = smem_u32(bars + warp * C::kSlots);
-  const uint32_t q_sm = smem_u32(smem) + C::kRing + warp * C::kQBytes + lane * 8;         // a lane reads what it has written
   float ks_reg = 0.f, vs_reg = 0.f;                           // lane i % 8: the scales of the i-th block of this warp
   int issued = 0, used = 0;                                   // boxes: K and V of a block in turn
   int put = 0, get = 0;                                       // their places in the ring
@@ -325,12 +311,6 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (!asked) ask_queries<D, NT>(p, seg.b, hk, rt, count, qf);
     asked = false;
     scale_queries<D, NT>(p, qf, f);
-    if (C::kSharedQ) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) sts_f2(q_sm + (j * (D / 16) + c) * 256, __uint_as_float(qf[j][c][0]), __uint_as_float(qf[j][c][1]));
-    }
     int lim[NT][2], lim_min = seg.n;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -352,7 +332,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       if (!ok) break;
       const float ks = __shfl_sync(0xffffffffu, ks_reg, at), vs = __shfl_sync(0xffffffffu, vs_reg, at);
       float s[NT][2][4];
-      keys_times_queries<D, NT, C::kSharedQ>(ring + get * C::kSlotBytes, q_sm, qf, s);
+      keys_times_queries<D, NT>(ring + get * C::kSlotBytes, qf, s);
       const int key0 = kb * 32;
       const bool cut = key0 + 32 > lim_min;                   // some row does not see all keys of the block
       const int e_blk = static_cast<int>((__float_as_uint(vs) >> 23) & 0xFF) - 127, e_new = max(vexp, e_blk);
@@ -797,7 +777,7 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
         for (int rt = 0; rt < row_tiles; ++rt) {
           if (row_tiles > 1) load_queries<D, NT>(p, seg.b, hk, rt, count, qf, f);
           float s[NT][2][4];
-          keys_times_queries<D, NT, false>(ring + st * kStageBytes, 0, qf, s);
+          keys_times_queries<D, NT>(ring + st * kStageBytes, qf, s);
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -899,10 +879,18 @@ cudaError_t launch_weights(const CUtensorMap& tk, const CacheAttnParams& p, cuda
                         (p.Nq * p.rep + 8 * NT - 1) / (8 * NT));
 }
 
-// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.
+// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.  us of this form and of that, 4096 - 8192 tokens: at head_dim 128, H=32 Hk=8,
+// 36 rows B=1 35 and 32, B=8 91 and 65; 32 rows B=8 55 and 64; at head_dim 256, H=16 Hk=4, 36 rows B=1 31 and 37, B=8 81 and 63; 32
+// rows B=1 31 and 36, B=8 62 and 62.
 constexpr int kChunkFrom = 33;
+// Blocks of a warp up to which a cluster takes a unit, joining its warps' results itself, instead of the even division with a kernel that joins.  us with and
+// without, H=32 Hk=8, one new token: B=1 with 4096 tokens 11.7 and 15.4, B=4 with 3601 - 4096 14.8 and 17.3, B=8 with 2048 14.5 and 18.0; with
+// 16 instead of 8, B=1 with 16384 tokens 25.0 against 19.4.
 constexpr int kClusterBlocks = 8;
-int small_row_tile(int D, int R) { return R <= 8 ? 8 : R <= 16 || D == 256 ? 16 : 32; }
+// A tile of 32 rows reads the codes once where two of 16 read them twice (the second time from L2), but its accumulators leave fewer warps in flight:
+// us with 32 and 16 at H=32 Hk=8, 8 new tokens: B=64 with 17 - 8191 tokens 232 and 243, B=8 with 4096 - 8192 56.4 and 54.7, B=1 with 1000
+// 15.0 and 10.8.
+int small_row_tile(int R) { return R <= 8 ? 8 : 16; }
 
 }  // namespace
 
@@ -910,7 +898,7 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   CacheAttnPlan x;
   const int R = Nq * (H / Hk);
   x.chunk = R >= kChunkFrom;
-  x.row_tile = x.chunk ? cache_chunk_rows(D) : small_row_tile(D, R);
+  x.row_tile = x.chunk ? cache_chunk_rows(D) : small_row_tile(R);
   x.row_tiles = (R + x.row_tile - 1) / x.row_tile;
   const int64_t blocks = static_cast<int64_t>(T) * (page / 32), units = static_cast<int64_t>(B) * Hk * x.row_tiles;       // of a sequence; in all
   const int ctas = x.chunk ? 1 : D == 128 && x.row_tile == 8 ? AttnCfg<128, 1>::kCtasPerSm : AttnCfg<128, 2>::kCtasPerSm;
@@ -940,12 +928,11 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
 }
 
 cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
-  const int R = p.Nq * p.rep, tile = small_row_tile(D, R), row_tiles = (R + tile - 1) / tile;
+  const int R = p.Nq * p.rep, tile = small_row_tile(R), row_tiles = (R + tile - 1) / tile;
   if (R >= kChunkFrom) return launch_cache_chunk(D, tk, tv, tq, p, stream);
   cudaError_t e;
   if (D == 128) {
-    e = tile == 8 ? launch_main<128, 1>(tk, tv, p, row_tiles, stream)
-      : tile == 16 ? launch_main<128, 2>(tk, tv, p, row_tiles, stream) : launch_main<128, 4>(tk, tv, p, row_tiles, stream);
+    e = tile == 8 ? launch_main<128, 1>(tk, tv, p, row_tiles, stream) : launch_main<128, 2>(tk, tv, p, row_tiles, stream);
   } else {
     e = tile == 8 ? launch_main<256, 1>(tk, tv, p, row_tiles, stream) : launch_main<256, 2>(tk, tv, p, row_tiles, stream);
   }

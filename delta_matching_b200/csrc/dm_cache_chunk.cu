@@ -21,10 +21,9 @@ namespace dm {
 
 namespace {
 
-constexpr int kChunkCost = 3;               // key tiles that a unit's queries and output are worth
-// Key tiles of a piece from which one row tile is worth two results: us with and without at H=32 Hk=8, B=8 with 4096 - 8192 tokens and 9 new ones
-// (about 21 tiles a piece) 101 and 113, B=2 with 16 new ones (5 tiles) 62 and 53.
-constexpr int kSplitFrom = 10;
+// Key tiles that a unit's queries and output are worth.  us with 1, 3 and 6 at H=32 Hk=8: 512 new tokens, B=2 with 4096 - 8192 126, 123.8 and 130.6; 128
+// new ones, B=4 with 512 35.2, 32.6 and 33.0.
+constexpr int kChunkCost = 3;
 constexpr int kPBase = 12;                  // log2 of P at the reference maximum,
 constexpr float kHeadroom = 3.9f;           // and what a row may exceed it by: P stays below 2^16
 
@@ -108,11 +107,8 @@ struct ChunkPiece {
   int b, hk, rt;
   ChunkSeq s;
   int tiles, t0, t1, f1;
-  // Softmax groups at work (head_dim 128): both, except that a short piece of a unit of one row tile has one.
-  // A long piece of such a unit is split: its key tiles go to the two groups in turn, each with a result of its own for the join.
-  __device__ __forceinline__ bool one_tile(const CacheAttnParams& p) const { return p.unit_shift == 8 && s.count * p.rep - (rt << 8) <= 128; }
-  __device__ __forceinline__ bool split(const CacheAttnParams& p) const { return one_tile(p) && t1 - t0 >= kSplitFrom; }
-  __device__ __forceinline__ int groups(const CacheAttnParams& p) const { return one_tile(p) && t1 - t0 < kSplitFrom ? 1 : 2; }
+  // Row tiles (head_dim 128): two, but for the last unit of a head.
+  __device__ __forceinline__ int groups(const CacheAttnParams& p) const { return s.count * p.rep - (rt << 8) <= 128 ? 1 : 2; }
 };
 __device__ __forceinline__ void chunk_cut(const CacheAttnParams& p, ChunkPiece& x, int at, int f, int f_end) {
   x.tiles = unit_tiles(p, x.s, x.rt);
@@ -447,37 +443,35 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           int tiles[2] = {0, 0}, units[2] = {0, 0};           // tiles and units of each row tile
           do {
             if (x.t0 >= x.t1) continue;
-            // both groups work on every key tile, or (split) each on every second one
-            const bool split = x.split(p);
-            const int step = split ? 2 : 1, n = x.t1 - x.t0, groups = x.groups(p);
+            const int n = x.t1 - x.t0, groups = x.groups(p);
             for (int r = 0; r < groups; ++r) {
-              if ((r == 0 || split) && !(ok = wait_or_abort(bar(kKFull), (g + (split ? r : 0)) & 1, abort_flag))) break;
+              if (r == 0 && !(ok = wait_or_abort(bar(kKFull), g & 1, abort_flag))) break;
               if (!(ok = wait_or_abort(bar(kQFull + r), units[r]++ & 1, abort_flag))) break;
               tc_fence_after();
-              issue_s(r, split || r == groups - 1);
-              if ((split ? r : 0) + step >= n) tc_commit(bars + kQFree + r);      // the group's last S of the unit
+              issue_s(r, r == groups - 1);
+              if (n == 1) tc_commit(bars + kQFree + r);       // the row tile's last S of the unit
             }
             for (int i = 0; i < n && ok; ++i, ++g) {
-              for (int r = split ? i & 1 : 0; r < groups; r += step) {
+              for (int r = 0; r < groups; ++r) {
                 // 16 keys a step: 8 columns of P, 16 rows of V; the first half of the keys while the softmax is at the second
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                   if (!(ok = wait_or_abort(bar((half == 0 ? kPHalf : kPFull) + r), tiles[r] & 1, abort_flag))) break;
-                  if ((r == 0 || split) && half == 0 && !(ok = wait_or_abort(bar(kVFull + (g & 1)), (g >> 1) & 1, abort_flag))) break;
+                  if (r == 0 && half == 0 && !(ok = wait_or_abort(bar(kVFull + (g & 1)), (g >> 1) & 1, abort_flag))) break;
                   tc_fence_after();
 #pragma unroll
                   for (int k = 4 * half; k < 4 * half + 4; ++k)
-                    mma_h_ts(tmem + 256 + 128 * r, tmem + 128 * r + 8 * k, v_lo + (g & 1) * (2 * C::kTile >> 4) + k * (2048 >> 4), kIdescO, i >= step || k > 0);
+                    mma_h_ts(tmem + 256 + 128 * r, tmem + 128 * r + 8 * k, v_lo + (g & 1) * (2 * C::kTile >> 4) + k * (2048 >> 4), kIdescO, i > 0 || k > 0);
                 }
                 if (!ok) break;
                 ++tiles[r];
-                if (split || r == groups - 1) tc_commit(bars + kVEmpty + (g & 1));
+                if (r == groups - 1) tc_commit(bars + kVEmpty + (g & 1));
                 tc_commit(bars + kPvDone + r);
-                if (i + step < n) {
-                  if ((r == 0 || split) && !(ok = wait_or_abort(bar(kKFull), (g + step) & 1, abort_flag))) break;
+                if (i + 1 < n) {
+                  if (r == 0 && !(ok = wait_or_abort(bar(kKFull), (g + 1) & 1, abort_flag))) break;
                   tc_fence_after();
-                  issue_s(r, split || r == groups - 1);
-                  if (i + 2 * step >= n) tc_commit(bars + kQFree + r);
+                  issue_s(r, r == groups - 1);
+                  if (i + 2 >= n) tc_commit(bars + kQFree + r);
                 }
               }
             }
@@ -492,13 +486,12 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int tiles_of_head = (p.Nq * p.rep + 127) / 128;
         do {
           if (x.t0 >= x.t1) continue;
-          const bool split = x.split(p);
           for (int r = 0; r < (C::kWide ? 1 : x.groups(p)) && ok; ++r) {
             if (units[r] > 0) ok = wait_or_abort(bar(kQFree + r), (units[r] - 1) & 1, abort_flag);
             if (!ok) break;
             ++units[r];
             mbar_expect_tx(bars + kQFull + r, C::kPanels * C::kTile);
-            const int row = ((x.b * p.c.Hk + x.hk) * tiles_of_head + (C::kWide ? x.rt : 2 * x.rt + (split ? 0 : r))) * 128;
+            const int row = ((x.b * p.c.Hk + x.hk) * tiles_of_head + (C::kWide ? x.rt : 2 * x.rt + r)) * 128;
             for (int panel = 0; panel < C::kPanels; ++panel)
               tma_load_2d(smem + C::kSmemQ + (2 * r + panel) * C::kTile, &tq, bars + kQFull + r, 128 * panel, row);        // x in bytes
           }
@@ -591,15 +584,12 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       int slot = 2 * cta;
       do {
         if (x.t0 >= x.t1) continue;
-        const bool split = x.split(p);
-        const int step = split ? 2 : 1, first = x.t0 + (split ? r : 0);       // this group's key tiles
-        if (!C::kWide && r >= x.groups(p)) {                  // none: a result of nothing
-          p.part_ml[static_cast<int64_t>(slot) * C::kRows + r * 128 + in_tile] = make_float2(-CUDART_INF_F, 0.f);
+        if (!C::kWide && r >= x.groups(p)) {
           g += x.t1 - x.t0;
           slot = 2 * cta + 1;
           continue;
         }
-        const int row = x.rt * C::kRows + (C::kWide || split ? 0 : r * 128) + in_tile, limit = row_limit(p, x.s, row);
+        const int row = x.rt * C::kRows + (C::kWide ? 0 : r * 128) + in_tile, limit = row_limit(p, x.s, row);
         const int i_tok = row / p.rep, head = x.hk * p.rep + row - i_tok * p.rep;
         // A row that sees nothing is not written here: its logits need no mask (one of them had its warp take the masked path in all tiles), and a warp
         // of such rows makes none, whatever its P holds.
@@ -676,7 +666,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           tmem_ld32(t_s, s_buf[0]);
           if (__any_sync(0xffffffffu, m_new != m || v_new != vexp)) {
             const float keep = ex2_approx(m - mu);
-            if (t > first) {
+            if (t > x.t0) {
               if (!products_of(mine - 1)) return false;
               tc_fence_after();
               const float a = keep * exp2f(static_cast<float>(vexp - v_new));
@@ -728,7 +718,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           if (lane == 0) mbar_arrive(bars + kPFull + (C::kWide ? mine & 1 : r));
           return true;
         };
-        for (int t = first; t < x.t1; t += step, ++mine) {
+        for (int t = x.t0; t < x.t1; ++t, ++mine) {
           const int gt = g + t - x.t0;
           ok = (idle || wait_warp(bar(kScales + (gt & 7)), (gt >> 3) & 1, abort_flag)) &&
                (C::kWide ? wait_warp(bar(kSFull + (mine & 1)), (mine >> 1) & 1, abort_flag) : wait_warp(bar(kSFull + r), mine & 1, abort_flag));
@@ -754,7 +744,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         if (!ok) break;
         tc_fence_after();
-        const bool whole = x.t0 == 0 && x.t1 == x.tiles && !split;
+        const bool whole = x.t0 == 0 && x.t1 == x.tiles;
         const float unit_exp = exp2f(static_cast<float>(vexp - kPBase));
         const float scale = whole ? unit_exp / l : unit_exp;
         // where a row that sees something goes
@@ -866,12 +856,10 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
   if (unit.x < 0) return;                                 // whole: written by its CTA
   float top = -CUDART_INF_F, sum = 0.f;
   float4 acc[kVecs] = {};
-  const int halves = kRows == 256 && s.count * p.rep - r / kRows * kRows <= 128 ? 2 : 1;      // a split unit's pieces have two results
-  const int first = unit.x / 2 * halves, n = unit.y * halves + halves;
+  const int first = unit.x / 2, n = unit.y + 1;               // the CTAs that have a piece of it
   // 32 results at a time, a lane each: their maxima and sums together, then the values of those that count
   for (int i0 = first; i0 < n; i0 += 32) {
-    const int i = i0 + lane, c = i / halves;
-    const int at = (c == unit.x / 2 ? unit.x : 2 * c) * kRows + (r & (kRows - 1)) + (i - c * halves) * 128;
+    const int i = i0 + lane, at = (i == first ? unit.x : 2 * i) * kRows + (r & (kRows - 1));
     const float2 ml = i < n ? p.part_ml[at] : make_float2(-CUDART_INF_F, 0.f);         // -inf: a piece of which the row sees nothing
     float top_new = ml.x;
 #pragma unroll
