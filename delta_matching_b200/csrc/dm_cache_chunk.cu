@@ -13,6 +13,14 @@
 // TMEM: S0 0-127, S1 128-255 (P of a tile over the first 64 columns of its S), O0 256-383, O1 384-511.
 // The reference moves only when a row exceeds it by more than 2^3.9 (P then still fits f16's range), so O is seldom rescaled: a move costs its
 // row tile about 3000 cycles, and with a reference that follows within a factor of two some warp moved it in most tiles (6800 cycles a tile).
+//
+// Head_dim 256: a unit is 128 rows, the two softmax groups take half of a tile's keys each and half of O, S has two buffers (0-127, 128-255) and
+// O the columns 256-511.
+//
+// Bound by the chain of a tile at head_dim 128: softmax 2000 - 2500 cycles, P V and the next S 1300 - 1700 until seen, beside which the other row tile
+// works; its exponentials alone are 2048 cycles for both row tiles.  512 new tokens, H=32 Hk=8, B=2 with 4096 - 8192 tokens: 122 - 130 us =
+// 760 - 810 TFLOP/s (cuBLAS in bf16: 1635).  At head_dim 256 by the conversion of the codes, 4400 cycles a tile, and their loads, for which 32 KB are left:
+// H=16 Hk=4 165 us.
 #include <type_traits>
 #include "dm_cache.cuh"
 #include "dm_kernels.h"
