@@ -53,20 +53,19 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
 // One cluster per (sequence, kv head), each CTA a contiguous slice of the candidates, whose keys it keeps in shared memory.  The k-th greatest
 // key by three digits of 12, 10 and 10 bits (the first is sign, exponent and three bits: weights of one size spread over many bins),
 // histograms added over the cluster; then the kept positions in order, by scans.  Bound by the latency of its barriers: a barrier of eight CTAs
-// takes 1200 - 3500 cycles, so of each other's histograms the CTAs read eight sums and then the eighth of the bins that matters.  Eight rows of
+// takes 1200 - 3500 cycles, so of each other's histograms the CTAs read 32 sums and then the 32nd of the bins that matters.  Eight rows of
 // 131071 tokens, 32768 kept: 23 us; 32 rows of 3001 - 4096: 8.
 __global__ void __launch_bounds__(kSelThreads) cache_select_kernel(const CacheEvictParams p) {
   extern __shared__ uint4 keys4[];
   __shared__ uint4 hist4[kBins / 4];
   __shared__ uint32_t warp_sums[kSelThreads / 32];
-  __shared__ uint32_t found[2];
-  __shared__ uint32_t counts[2], eighths[8];
+  __shared__ uint32_t found[3];                               // bin, keys in greater ones, keys in it
+  __shared__ uint32_t counts[2], sums[32];                    // sums: of the 32nds of the histogram
   uint32_t* keys = reinterpret_cast<uint32_t*>(keys4);
   uint32_t* hist = reinterpret_cast<uint32_t*>(hist4);
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < kBins / 4; i += kSelThreads) hist4[i] = make_uint4(0, 0, 0, 0);
-  if (tid < 8) eighths[tid] = 0;
   grid_dep_wait();
   const auto sync_all = [&]() {
     if (C > 1) cluster.sync(); else __syncthreads();
@@ -123,126 +122,136 @@ __global__ void __launch_bounds__(kSelThreads) cache_select_kernel(const CacheEv
         for (int i = 4 * loads + tid; i < len; i += kSelThreads) take(key_at(i));
       }
       __syncthreads();
-      // which eighth of the bins holds the want-th key: from the CTAs' sums
-      for (int i = tid; i < quads; i += kSelThreads) {        // a warp's quads lie in one eighth
+      // which 32nd of the bins holds the want-th key: from the CTAs' sums
+      const int part = quads / 32;                            // quads of a 32nd: a warp's, or those of eight lanes
+      for (int i = tid; i < quads; i += kSelThreads) {
         const uint4 v = hist4[i];
-        const uint32_t sum = __reduce_add_sync(0xffffffffu, v.x + v.y + v.z + v.w);
-        if (lane == 0) atomicAdd(eighths + i / (quads / 8), sum);
+        uint32_t sum = v.x + v.y + v.z + v.w;
+        for (int o = part / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if ((i & (part - 1)) == 0) sums[i / part] = sum;
       }
       sync_all();
       if (tid < 32) {
-        const int q = lane & 7, r = lane >> 3;                // lane (r, q) adds the sums of eighth q of CTAs r and r + 4
-        uint32_t sum = 0;
-        if (C == 1) {
-          if (r == 0) sum = eighths[q];
-        } else {
-          if (r < C) sum += *cluster.map_shared_rank(eighths + q, r);
-          if (r + 4 < C) sum += *cluster.map_shared_rank(eighths + q, r + 4);
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        uint32_t from = sum;                                  // keys in this eighth and the greater ones
+        uint32_t sum = C == 1 ? sums[lane] : 0;
+        if (C > 1) {
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-          const uint32_t x = __shfl_down_sync(0xffffffffu, from, o, 8);
-          if (q + o < 8) from += x;
+          for (int r = 0; r < kMaxCluster; ++r) sum += r < C ? *cluster.map_shared_rank(sums + lane, r) : 0;      // all on their way together
         }
-        const int eighth = __ffs(__ballot_sync(0xffffffffu, from - sum < want && want <= from) & 0xFFu) - 1;
-        uint32_t above = __shfl_sync(0xffffffffu, from, eighth);        // keys in this bin and the greater ones, from here on
-        // its bins over the cluster, 32 quads at a time
-        for (int i0 = 0; i0 < quads / 8; i0 += 32) {
-          const uint4* mine = hist4 + eighth * (quads / 8) + i0 + lane;
-          uint4 v[kMaxCluster];                               // all on their way together
+        uint32_t from = sum;                                  // keys in this 32nd and the greater ones
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x = __shfl_down_sync(0xffffffffu, from, o);
+          if (lane + o < 32) from += x;
+        }
+        const int which = __ffs(__ballot_sync(0xffffffffu, from - sum < want && want <= from)) - 1;
+        const uint32_t above = __shfl_sync(0xffffffffu, from, which);         // keys in its bins and the greater ones
+        // its bins over the cluster
+        uint32_t h[4] = {0, 0, 0, 0};
+        if (lane < part) {
+          const uint4* mine = hist4 + which * part + lane;
+          uint4 v[kMaxCluster];
           v[0] = C > 1 ? *cluster.map_shared_rank(mine, 0) : *mine;
 #pragma unroll
-          for (int r2 = 1; r2 < kMaxCluster; ++r2) v[r2] = r2 < C ? *cluster.map_shared_rank(mine, r2) : make_uint4(0, 0, 0, 0);
-          uint32_t h[4] = {0, 0, 0, 0};
+          for (int r = 1; r < kMaxCluster; ++r) v[r] = r < C ? *cluster.map_shared_rank(mine, r) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int r2 = 0; r2 < kMaxCluster; ++r2) {
-            h[0] += v[r2].x; h[1] += v[r2].y; h[2] += v[r2].z; h[3] += v[r2].w;
+          for (int r = 0; r < kMaxCluster; ++r) {
+            h[0] += v[r].x; h[1] += v[r].y; h[2] += v[r].z; h[3] += v[r].w;
           }
-          const uint32_t four = h[0] + h[1] + h[2] + h[3];
-          uint32_t incl = four;
+        }
+        const uint32_t four = h[0] + h[1] + h[2] + h[3];
+        uint32_t incl = four;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += x;
-          }
-          uint32_t at = above - (incl - four);
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += x;
+        }
+        uint32_t at = above - (incl - four);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t greater = at - h[i];
-            if (greater < want && want <= at) {
-              found[0] = 4 * (eighth * (quads / 8) + i0 + lane) + i;
-              found[1] = greater;
-            }
-            at = greater;
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t greater = at - h[i];
+          if (greater < want && want <= at) {
+            found[0] = 4 * (which * part + lane) + i;
+            found[1] = greater;
+            found[2] = h[i];
           }
-          above -= __shfl_sync(0xffffffffu, incl, 31);
+          at = greater;
         }
       }
       sync_all();                                             // found is there, and nobody reads the histograms any more
       prefix |= found[0] << shift;
       mask |= (pass == 0 ? 4095u : 1023u) << shift;
       want -= found[1];
+      if (found[2] == want && prefix > 0) {                   // all of the bin are taken: what is above its lower end, and none that is equal to that
+        --prefix;
+        want = 0;
+        break;
+      }
       if (pass < 2) {
         for (int i = tid; i < 1024 / 4; i += kSelThreads) hist4[i] = make_uint4(0, 0, 0, 0);
-        if (tid < 8) eighths[tid] = 0;
         __syncthreads();
       }
     }
 
-    // how many of the slices before mine are above the threshold, and equal to it
-    uint32_t gt = 0, eq = 0;
+    // Adjacent tokens a thread takes at a time, and a slice that is taken at once: above the threshold, equal to it, as bits.  (Eight at a time in any
+    // case, and the numbers for the cluster counted on their own, took 14000 cycles of a slice of 16384; a slice of 4096 by 32 at a time leaves
+    // most threads idle.)
+    const int take = per > 8 * kSelThreads ? 32 : 8;
+    const bool once = per <= take * kSelThreads;
+    uint32_t above = 0, equal = 0, before = 0, total = 0;
+    const auto look = [&](int j0) {
+      above = equal = 0;
+      for (int i = 0; i < take / 4; ++i) {
+        const int q = take == 32 ? 4 * ((i + lane) & 7) : 4 * i, j = j0 + q;        // (lanes on different banks)
+        if (j >= len) continue;
+        uint32_t key[4];
+        if (held) {                                           // a slice's keys are whole quads
+          const uint4 v = keys4[j / 4];
+          key[0] = v.x; key[1] = v.y; key[2] = v.z; key[3] = v.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) key[e] = weight_key(__ldg(w + min(j + e, len - 1)));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (j + e >= len) break;
+          above |= (key[e] > prefix ? 1u : 0u) << (q + e);
+          equal |= (key[e] == prefix ? 1u : 0u) << (q + e);
+        }
+      }
+      before = block_scan(__popc(above) | __popc(equal) << 16, warp_sums, total);
+    };
+    if (once) look(tid * take);
+    uint32_t gt = 0, eq = 0;                                  // of the slices before mine
     if (C > 1) {
-      uint32_t mine = 0, equal = 0;
-      const int loads = held ? len / 4 : 0;
-      for (int i = tid; i < loads; i += kSelThreads) {
-        const uint4 key = keys4[i];
-        mine += (key.x > prefix) + (key.y > prefix) + (key.z > prefix) + (key.w > prefix);
-        equal += (key.x == prefix) + (key.y == prefix) + (key.z == prefix) + (key.w == prefix);
-      }
-      for (int i = 4 * loads + tid; i < len; i += kSelThreads) {
-        const uint32_t key = key_at(i);
-        mine += key > prefix;
-        equal += key == prefix;
-      }
-      mine = __reduce_add_sync(0xffffffffu, mine);
-      equal = __reduce_add_sync(0xffffffffu, equal);
-      if (tid < 2) counts[tid] = 0;
-      __syncthreads();
-      if (lane == 0) {
-        atomicAdd(counts, mine);
-        atomicAdd(counts + 1, equal);
+      if (!once) {
+        uint32_t mine = 0, same = 0;
+        for (int i = tid; i < len; i += kSelThreads) {
+          const uint32_t key = key_at(i);
+          mine += key > prefix;
+          same += key == prefix;
+        }
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        same = __reduce_add_sync(0xffffffffu, same);
+        if (tid < 2) counts[tid] = 0;
+        __syncthreads();
+        if (lane == 0) {
+          atomicAdd(counts, mine);
+          atomicAdd(counts + 1, same);
+        }
+      } else if (tid == 0) {
+        counts[0] = total & 0xFFFFu;
+        counts[1] = total >> 16;
       }
       cluster.sync();
       gt = __reduce_add_sync(0xffffffffu, lane < rank ? *cluster.map_shared_rank(counts, lane) : 0u);       // a lane per CTA before this one
       eq = __reduce_add_sync(0xffffffffu, lane < rank ? *cluster.map_shared_rank(counts + 1, lane) : 0u);
     }
-    constexpr int kTake = 8;                                  // adjacent tokens of a thread per scan
-    for (int at = 0; at < len; at += kSelThreads * kTake) {
-      const int j0 = at + tid * kTake;
-      uint32_t key[kTake], flags = 0;
-      if (held) {
-#pragma unroll
-        for (int i = 0; i < kTake; i += 4) {
-          const uint4 v = j0 + i < len ? keys4[(j0 + i) / 4] : make_uint4(0, 0, 0, 0);      // a slice's keys are whole quads
-          key[i] = v.x; key[i + 1] = v.y; key[i + 2] = v.z; key[i + 3] = v.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kTake; ++i) key[i] = j0 + i < len ? weight_key(__ldg(w + j0 + i)) : 0;
-      }
-#pragma unroll
-      for (int i = 0; i < kTake; ++i) {
-        const bool is_gt = j0 + i < len && key[i] > prefix, is_eq = j0 + i < len && key[i] == prefix;
-        flags |= (is_gt ? 1u : 0u) << i | (is_eq ? 1u : 0u) << (16 + i);
-      }
-      uint32_t total;
-      const uint32_t before = block_scan(__popc(flags & 0xFFFFu) | __popc(flags >> 16) << 16, warp_sums, total);
+    for (int at = 0; at < len; at += kSelThreads * take) {
+      const int j0 = at + tid * take;
+      if (!once) look(j0);
       const uint32_t g = gt + (before & 0xFFFFu), e = eq + (before >> 16);
       // of mine that are equal to the threshold, the first ones until there are `want`
-      uint32_t picks = flags & 0xFFFFu, equals = flags >> 16;
+      uint32_t picks = above, equals = equal;
       for (uint32_t room = e < want ? want - e : 0; equals != 0 && room > 0; --room) {
         picks |= equals & -equals;
         equals &= equals - 1;

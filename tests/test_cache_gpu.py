@@ -333,6 +333,13 @@ def test_evict_long_rows(n, budget, recent, kind):
     assert torch.equal(got, moved.view(torch.float8_e4m3fn)[want // P, h, want % P].float())
 
 
+@pytest.mark.parametrize("n, budget, recent, kind", [(150001, 50000, 64, "random"), (150001, 149000, 3, "few values"), (340003, 1001, 1, "random"),
+                                                    (340003, 340001, 0, "few values")])
+def test_evict_longest_rows(n, budget, recent, kind):
+    """Slices of a row that a CTA takes in several turns, and that its shared memory does not hold."""
+    test_evict_long_rows(n, budget, recent, kind)
+
+
 def test_evict_scales_far_apart():
     """Zero rows on a coarse scale beside tiny rows; NaN codes move and do not set the scale."""
     cache = ref.make_cache(4, 32, 1, 128)
