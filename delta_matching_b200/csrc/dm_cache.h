@@ -56,7 +56,8 @@ struct CacheAttnParams {
                                     // small form twice that, plus one where its piece lies in a slot of its own)
   float2* row_ml;                   // (B, Hk, Nq * rep): maximum (log2 domain) and 1 / sum of each row, for the weights; may be null.  Of the form
                                     // for many rows: factor of the logits and log2 of the sum, rows of a head filled up to whole tiles
-  float* logits;                    // (B, Hk, T * page, row tile), log2 domain, masked: for the weights of up to 16 rows; or null
+  float* logits;                    // (B, Hk, T * page, logit_rows), log2 domain, masked: for the weights of up to 16 rows; or null
+  int logit_rows;                   // a token's, a multiple of four
   float* weights;                   // (B, Hk, W) or null
   int64_t w_sb, w_sh;
   int W;
@@ -86,6 +87,7 @@ struct CacheAttnPlan {
   int row_tiles;
   int grid;
   int cluster;                      // CTAs a unit, or 0: the even division
+  int logit_rows;
   int64_t part_o_bytes, part_ml_bytes, q16_bytes, factor_bytes, start_bytes, unit_bytes, row_ml_bytes, logit_bytes;
   int64_t bytes() const { return part_o_bytes + part_ml_bytes + q16_bytes + factor_bytes + start_bytes + unit_bytes + row_ml_bytes + logit_bytes; }
 };

@@ -359,13 +359,14 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             s[j][mt][i] *= (i & 1) ? fs.y : fs.x;
             if (cut && key0 + 16 * mt + g + 8 * (i >> 1) >= lim[j][i & 1]) s[j][mt][i] = -CUDART_INF_F;
           }
-        if (NT <= 2 && p.logits != nullptr) {                 // for the weights: (b, kv head, token, row of the tile)
-          float* to = p.logits + ((static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.c.T * p.c.page + key0 + g) * C::kRows + 8 * j + 2 * t;
+        const int logit_rows = NT == 1 ? p.logit_rows : C::kRows;
+        if (p.logits != nullptr && 8 * j + 2 * t < logit_rows) {        // for the weights: (b, kv head, token, row of the tile)
+          float* to = p.logits + ((static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.c.T * p.c.page + key0 + g) * logit_rows + 8 * j + 2 * t;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              *reinterpret_cast<float2*>(to + (16 * mt + 8 * i) * C::kRows) = make_float2(s[j][mt][2 * i], s[j][mt][2 * i + 1]);
+              *reinterpret_cast<float2*>(to + (16 * mt + 8 * i) * logit_rows) = make_float2(s[j][mt][2 * i], s[j][mt][2 * i + 1]);
         }
         float2 mx = make_float2(fmaxf(fmaxf(s[j][0][0], s[j][0][2]), fmaxf(s[j][1][0], s[j][1][2])),
                                 fmaxf(fmaxf(s[j][0][1], s[j][0][3]), fmaxf(s[j][1][1], s[j][1][3])));
@@ -679,13 +680,16 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
 // ------------------------------------------------------------------------------------------------ weights
 // weights[b, hk, j] (+)= sum over the group's rows of exp(s_rj - m_r) / l_r, with the rows' m and l from the kernels before: K is read once
 // more, a block of 32 tokens a warp, all row tiles on it; no result is shared between warps, and the sum's order is that of the rows.
-// This is the form for 17 to 32 rows.  Up to 16 the main kernel leaves its logits (32 or 64 bytes a token instead of K's 128 or 256, and no
+// This is the form for 17 to 32 rows.  Up to 16 the main kernel leaves its logits (16 - 64 bytes a token instead of K's 128 or 256, and no
 // products), and cache_weights_of_logits_kernel adds their exponentials, one thread a token: a call with weights at H=32 Hk=8, B=16 with 2049 - 4096
 // tokens takes 35 us with one new token (59 with K read again) and 45 with four (66).
-__global__ void __launch_bounds__(256) cache_weights_of_logits_kernel(const CacheAttnParams p, const int row_tile, const int pieces) {
+__global__ void __launch_bounds__(256) cache_weights_of_logits_kernel(const CacheAttnParams p, const int pieces) {
   __shared__ float2 ml[16];
   grid_dep_wait();
   const int bh = blockIdx.x / pieces, j = (blockIdx.x - bh * pieces) * 256 + threadIdx.x, b = bh / p.c.Hk, hk = bh - b * p.c.Hk, R = p.Nq * p.rep;
+  // the first logits before it is known whether the token exists (its place does): the loads are under way together
+  const float4* x = reinterpret_cast<const float4*>(p.logits + (static_cast<int64_t>(bh) * p.c.T * p.c.page + j) * p.logit_rows);
+  const float4 first = j < p.c.T * p.c.page ? *x : make_float4(0.f, 0.f, 0.f, 0.f);
   const int n = cache_length(p.c, b);
   if (threadIdx.x < R) ml[threadIdx.x] = p.row_ml[static_cast<int64_t>(bh) * R + threadIdx.x];
   __syncthreads();
@@ -695,16 +699,15 @@ __global__ void __launch_bounds__(256) cache_weights_of_logits_kernel(const Cach
     if (!p.accumulate) *at = 0.f;
     return;
   }
-  const float* x = p.logits + (static_cast<int64_t>(bh) * p.c.T * p.c.page + j) * row_tile;
   float w = 0.f;
 #pragma unroll
   for (int r = 0; r < 16; r += 4) {
     if (r >= R) break;
-    const float4 v = *reinterpret_cast<const float4*>(x + r);
-    w += ex2_approx(v.x - ml[r].x) * ml[r].y;
-    if (r + 1 < R) w += ex2_approx(v.y - ml[r + 1].x) * ml[r + 1].y;
-    if (r + 2 < R) w += ex2_approx(v.z - ml[r + 2].x) * ml[r + 2].y;
-    if (r + 3 < R) w += ex2_approx(v.w - ml[r + 3].x) * ml[r + 3].y;
+    const float4 y = r == 0 ? first : x[r / 4];
+    w += ex2_approx(y.x - ml[r].x) * ml[r].y;
+    if (r + 1 < R) w += ex2_approx(y.y - ml[r + 1].x) * ml[r + 1].y;
+    if (r + 2 < R) w += ex2_approx(y.z - ml[r + 2].x) * ml[r + 2].y;
+    if (r + 3 < R) w += ex2_approx(y.w - ml[r + 3].x) * ml[r + 3].y;
   }
   *at = p.accumulate ? *at + w : w;
 }
@@ -928,7 +931,8 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   x.start_bytes = x.chunk ? x.grid * cache_chunk_start_bytes() : 0;
   x.unit_bytes = static_cast<int64_t>(B) * Hk * x.row_tiles * 8;
   // logits for the weights, where they are fewer bytes than K
-  x.logit_bytes = weights && R <= 16 ? static_cast<int64_t>(B) * Hk * T * page * x.row_tile * 4 : 0;
+  x.logit_rows = R <= 4 ? 4 : x.row_tile;
+  x.logit_bytes = weights && R <= 16 ? static_cast<int64_t>(B) * Hk * T * page * x.logit_rows * 4 : 0;
   x.row_ml_bytes = !weights ? 0 : x.chunk ? q_rows * 8 : static_cast<int64_t>(B) * Hk * R * 8;
   return x;
 }
@@ -946,7 +950,7 @@ cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& t
   if (p.logits != nullptr) {
     const int pieces = (p.W + 255) / 256;
     count_launch();
-    return launch_chained(cache_weights_of_logits_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * pieces), 256, 0, stream, p, tile, pieces);
+    return launch_chained(cache_weights_of_logits_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * pieces), 256, 0, stream, p, pieces);
   }
   return D == 128 ? launch_weights<128, 4>(tk, p, stream) : launch_weights<256, 2>(tk, p, stream);
 }
