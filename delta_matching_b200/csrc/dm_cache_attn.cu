@@ -173,16 +173,23 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   Piece seg{};
   int worker = warp, f_end = 0;
   bool have;                                                  // this warp has a piece
+  int blk_first = 0, blk_step = 1;                            // block kb of it is block blk_first + kb blk_step of the sequence
+  int page = 0, sub = 0;
   if constexpr (kCluster) {
+    // The warps take the blocks in turn: which ones does not depend on the length, so that their pages are looked up beside it (in a call of a few
+    // blocks a warp every load of this chain counts).  A warp has no more than kClusterBlocks of them.
     const int cl = p.cluster, unit = blockIdx.x / cl;
     seg.b = unit / units;
     seg.unit = unit - seg.b * units;
+    blk_first = (blockIdx.x - unit * cl) * C::kWarps + warp;
+    blk_step = cl * C::kWarps;
+    const int bpp = p.c.page / 32, blk = blk_first + min(lane, 8) * blk_step, entry = blk / bpp;
+    sub = blk - entry * bpp;
+    if (entry < p.c.T) page = __ldg(p.c.table + seg.b * p.c.t_row + entry);
     seg.n = cache_length(p.c, seg.b);
     seg.blocks = (seg.n + 31) / 32;
-    const int w = (blockIdx.x - unit * cl) * C::kWarps + warp, all = cl * C::kWarps;
-    seg.blk0 = static_cast<int>(static_cast<int64_t>(w) * seg.blocks / all);
-    seg.blk1 = static_cast<int>(static_cast<int64_t>(w + 1) * seg.blocks / all);
-    have = seg.blk0 < seg.blk1;
+    seg.blk1 = max(0, (seg.blocks - blk_first + blk_step - 1) / blk_step);
+    have = seg.blk1 > 0;
     __syncthreads();                                          // publishes the mbarriers
   } else {
     const FlatRange range = flat_range(p.c, units, cum);      // its barriers publish the mbarriers too
@@ -202,7 +209,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   if (have) {
     const int hk = seg.unit / row_tiles;
     ask_queries<D, NT>(p, seg.b, hk, seg.unit - hk * row_tiles, checked_count(p.c.status, p.counts, seg.b, p.Nq), qf);
-    ahead = cursor_start(p.c, units, seg, f_end);
+    if constexpr (kCluster) ahead = Cursor{seg, 0, 0, page, sub, true};
+    else ahead = cursor_start(p.c, units, seg, f_end);
   }
 
   const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
@@ -338,7 +346,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       const float ks = __shfl_sync(0xffffffffu, ks_reg, at), vs = __shfl_sync(0xffffffffu, vs_reg, at);
       float s[NT][2][4];
       keys_times_queries<D, NT>(ring + get * C::kSlotBytes, qf, s);
-      const int key0 = kb * 32;
+      const int key0 = (kCluster ? blk_first + kb * blk_step : kb) * 32;
       const bool cut = key0 + 32 > lim_min;                   // some row does not see all keys of the block
       const int e_blk = static_cast<int>((__float_as_uint(vs) >> 23) & 0xFF) - 127, e_new = max(vexp, e_blk);
       // p comes out as 2^off exp(s - m); where V's scale is 2^-60 of another's the product vanishes anyway, but the sum must not
