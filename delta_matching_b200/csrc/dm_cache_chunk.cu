@@ -1132,10 +1132,15 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
         if (!(ok = wait_warp(bar(kwCode + buf), j / C::kCodeBufs & 1, abort_flag))) break;
         const int c = tid & 7, panel = c >> 2, cc = (c & 3) * 2;
         const uint32_t src = sbase + C::kSmemCode + buf * C::kTile, dst = sbase + C::kSmemK + (2 * part + panel) * C::kTile;
+        float4 in[4];                                         // then the buffer is free for the next load
+#pragma unroll
+        for (int k = 0; k < 4; ++k) in[k] = lds_f4(src + ((tid >> 3) + 32 * k) * 128 + ((c ^ ((tid >> 3) & 7)) << 4));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kwCodeFree + buf);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int row = (tid >> 3) + 32 * k;
-          const float4 w4 = lds_f4(src + row * 128 + ((c ^ (row & 7)) << 4));
+          const float4 w4 = in[k];
           const uint32_t w[4] = {__float_as_uint(w4.x), __float_as_uint(w4.y), __float_as_uint(w4.z), __float_as_uint(w4.w)};
           uint32_t h[8];
 #pragma unroll
@@ -1147,12 +1152,10 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
           sts_u4(dst + row * 128 + (((cc + flip) ^ (row & 7)) << 4), flip ? h[4] : h[0], flip ? h[5] : h[1], flip ? h[6] : h[2], flip ? h[7] : h[3]);
           sts_u4(dst + row * 128 + (((cc + 1 - flip) ^ (row & 7)) << 4), flip ? h[0] : h[4], flip ? h[1] : h[5], flip ? h[2] : h[6], flip ? h[3] : h[7]);
         }
+        if (part < C::kChunks - 1) continue;
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bars + kwCodeFree + buf);
-          if (part == C::kChunks - 1) mbar_arrive(bars + kwK);
-        }
+        if (lane == 0) mbar_arrive(bars + kwK);
       }
     };
     // of this thread's token: its page, and the scale of its block
