@@ -1158,14 +1158,11 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
         if (lane == 0) mbar_arrive(bars + kwK);
       }
     };
-    // of this thread's token: its page, and the scale of its block
-    auto page_of = [&](const Item& x) {
-      const int tok = 128 * x.t + key;
-      return tok < x.n ? max(0, checked_page(p.c, __ldg(p.c.table + x.b * p.c.t_row + tok / p.c.page))) : 0;
-    };
+    // Of this thread's token: its page, and the scale of its block.  Each is asked for long before it is looked at, page an item ahead.
+    auto page_of = [&](const Item& x) { return __ldg(p.c.table + x.b * p.c.t_row + min(128 * x.t + key, x.n - 1) / p.c.page); };
     auto scale_of = [&](const Item& x, int page) {
-      const int tok = 128 * x.t + key;
-      return tok < x.n ? __ldg(p.c.ks + page * p.c.s_page + x.hk * p.c.s_head + tok % p.c.page / 32) : 0.f;
+      const int tok = min(128 * x.t + key, x.n - 1);
+      return __ldg(p.c.ks + max(0, checked_page(p.c, page)) * p.c.s_page + x.hk * p.c.s_head + tok % p.c.page / 32);
     };
     // of the last item: this half's sum, where it goes, whether the token exists
     float mine = 0.f;
@@ -1182,14 +1179,15 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
     };
     n = Place{static_cast<int>(blockIdx.x), 0};
     live = find(n, x, zeros);
-    float ks = live ? scale_of(x, page_of(x)) : 0.f;
+    int page = live ? page_of(x) : 0;
     int s = 0;                                                // running product
     for (int g = 0; live && ok; ++g) {
+      const float ks = scale_of(x, page);
       convert();
       if (!ok) break;
       // while the first product is under way
       const bool more = find(n, y, zeros), stays = more && same_rows(x, y);
-      const int next_page = more ? page_of(y) : 0;
+      if (more) page = page_of(y);
       const int tok = 128 * x.t + key;
       float total = 0.f;
       for (int rt = x.rt0; rt < x.rt1; ++rt, ++s) {
@@ -1254,7 +1252,6 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
         }
       }
       if (!ok) break;
-      ks = more ? scale_of(y, next_page) : 0.f;
       // The two halves' sums: the second leaves its own, the first picks it up an item later.
       if (half == 1) {
         if (g >= 2 && !(ok = wait_warp(bar(kwSumsFree + (g & 1)), ((g >> 1) - 1) & 1, abort_flag))) break;
