@@ -64,7 +64,7 @@ struct CacheAttnParams {
   int accumulate;
   int grid;                         // CTAs of the main kernel
   int cluster;                      // of a unit, or 0: the even division
-  int unit_shift;                   // log2 of the rows of a unit of the form for many rows
+  int unit_shift;                   // of the form for many rows: log2 of a unit's; otherwise 0
 };
 
 struct CacheEvictParams {

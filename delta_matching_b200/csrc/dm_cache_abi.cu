@@ -157,7 +157,7 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   p.w_sb = w_sb; p.w_sh = w_sh; p.W = W; p.accumulate = accumulate ? 1 : 0;
   p.grid = x.grid;
   p.cluster = x.cluster;
-  for (p.unit_shift = 0; 1 << p.unit_shift < x.row_tile;) ++p.unit_shift;
+  for (p.unit_shift = 0; x.chunk && 1 << p.unit_shift < x.row_tile;) ++p.unit_shift;
   CUtensorMap tk, tv, tq{};
   DM_TRY(pool_map(&tk, cache, cache->k8));
   DM_TRY(pool_map(&tv, cache, cache->v8));

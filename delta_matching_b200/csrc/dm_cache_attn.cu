@@ -17,7 +17,7 @@
 // Bound by its bytes where there are many blocks a warp: one new token, H=32 Hk=8, B=64 with 17 - 8191 tokens 102 us = 5.3 TB/s of codes and
 // scales (the card copies at 6.5); H=64 Hk=8, one sequence of 131071 tokens 58 us = 4.7 TB/s; head_dim 256, H=16 Hk=16, B=8 with 4001 - 8192 73 us
 // = 5.4 TB/s.  Small calls are bound by the chain from the lengths through the block table to the first codes (about 6700 cycles), 2300 cycles a
-// block and the join (3000 - 6000): B=4 with 3601 - 4096 15 us, one sequence of 255 tokens 7.2 us.
+// block and the join (3000 - 6000): B=4 with 3601 - 4096 15 us, one sequence of 255 tokens 7.0 us.
 #include <cooperative_groups.h>
 #include "dm_cache_sched.cuh"
 #include "dm_kernels.h"
@@ -688,9 +688,9 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
 // ------------------------------------------------------------------------------------------------ weights
 // weights[b, hk, j] (+)= sum over the group's rows of exp(s_rj - m_r) / l_r, with the rows' m and l from the kernels before: K is read once
 // more, a block of 32 tokens a warp, all row tiles on it; no result is shared between warps, and the sum's order is that of the rows.
-// This is the form for 17 to 32 rows.  Up to 16 the main kernel leaves its logits (16 - 64 bytes a token instead of K's 128 or 256, and no
+// This is the form for 17 to 32 rows of head_dim 128.  Up to 16 the main kernel leaves its logits (16 - 64 bytes a token instead of K's 128 or 256, and no
 // products), and cache_weights_of_logits_kernel adds their exponentials, one thread a token: a call with weights at H=32 Hk=8, B=16 with 2049 - 4096
-// tokens takes 35 us with one new token (59 with K read again) and 45 with four (66).
+// tokens takes 33 us with one new token (59 with K read again) and 46 with four (66).
 __global__ void __launch_bounds__(256) cache_weights_of_logits_kernel(const CacheAttnParams p, const int pieces) {
   __shared__ float2 ml[16];
   grid_dep_wait();
@@ -896,10 +896,10 @@ cudaError_t launch_weights(const CUtensorMap& tk, const CacheAttnParams& p, cuda
                         (p.Nq * p.rep + 8 * NT - 1) / (8 * NT));
 }
 
-// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.  us of this form and of that, 4096 - 8192 tokens: at head_dim 128, H=32 Hk=8,
-// 36 rows B=1 35 and 32, B=8 91 and 65; 32 rows B=8 55 and 64; at head_dim 256, H=16 Hk=4, 36 rows B=1 31 and 37, B=8 81 and 63; 32
-// rows B=1 31 and 36, B=8 62 and 62.
-constexpr int kChunkFrom = 33;
+// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.  us of this form and of that: at head_dim 128, H=32 Hk=8, 4096 - 8192
+// tokens, 36 rows B=1 35 and 32, B=8 91 and 65, 32 rows B=8 55 and 64; at head_dim 256, where this form takes two passes over 17 rows, H=16 Hk=4,
+// 24 rows B=1 with 8192 tokens 32 and 35 (with weights 56 and 47), B=8 77 and 65 (148 and 115), B=64 with 17 - 8191 256 and 213 (581 and 466).
+int chunk_from(int D) { return D == 128 ? 33 : 17; }
 // Blocks of a warp up to which a cluster takes a unit, joining its warps' results itself, instead of the even division with a kernel that joins.  us with and
 // without, H=32 Hk=8, one new token: B=1 with 4096 tokens 11.7 and 15.4, B=4 with 3601 - 4096 14.8 and 17.3, B=8 with 2048 14.5 and 18.0; with
 // 16 instead of 8, B=1 with 16384 tokens 25.0 against 19.4.
@@ -914,7 +914,7 @@ int small_row_tile(int R) { return R <= 8 ? 8 : 16; }
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights) {
   CacheAttnPlan x;
   const int R = Nq * (H / Hk);
-  x.chunk = R >= kChunkFrom;
+  x.chunk = R >= chunk_from(D);
   x.row_tile = x.chunk ? cache_chunk_rows(D) : small_row_tile(R);
   x.row_tiles = (R + x.row_tile - 1) / x.row_tile;
   const int64_t blocks = static_cast<int64_t>(T) * (page / 32), units = static_cast<int64_t>(B) * Hk * x.row_tiles;       // of a sequence; in all
@@ -947,7 +947,7 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
 
 cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tq, const CacheAttnParams& p, cudaStream_t stream) {
   const int R = p.Nq * p.rep, tile = small_row_tile(R), row_tiles = (R + tile - 1) / tile;
-  if (R >= kChunkFrom) return launch_cache_chunk(D, tk, tv, tq, p, stream);
+  if (p.unit_shift > 0) return launch_cache_chunk(D, tk, tv, tq, p, stream);
   cudaError_t e;
   if (D == 128) {
     e = tile == 8 ? launch_main<128, 1>(tk, tv, p, row_tiles, stream) : launch_main<128, 2>(tk, tv, p, row_tiles, stream);
@@ -960,7 +960,7 @@ cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& t
     count_launch();
     return launch_chained(cache_weights_of_logits_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * pieces), 256, 0, stream, p, pieces);
   }
-  return D == 128 ? launch_weights<128, 4>(tk, p, stream) : launch_weights<256, 2>(tk, p, stream);
+  return launch_weights<128, 4>(tk, p, stream);              // head_dim 256 has its logits or the form for many rows
 }
 
 }  // namespace dm

@@ -8,7 +8,8 @@
 // range, divided evenly over one CTA per SM (as the warps' blocks are in dm_cache_sched.cuh); pieces of cut units are joined by a second kernel.
 // Warps 0-3 and 4-7: softmax of the unit's two row tiles (thread = row = TMEM lane).  Warps 8-11: codes -> f16 operand tiles in shared
 // memory, shared by both row tiles.  Warp 12: TMA of the code tiles from the pages.  Warp 13: MMA.  Warp 14: TMA of the
-// queries, which a small kernel has brought to f16 in the order of the row tiles.  The two row tiles take turns: while one is in its softmax the tensor cores work for the other.
+// queries, which a small kernel has brought to f16 in the order of the row tiles.  The two row tiles take turns: while one is in its softmax the
+// tensor cores work for the other.
 //
 // TMEM: S0 0-127, S1 128-255 (P of a tile over the first 64 columns of its S), O0 256-383, O1 384-511.
 // The reference moves only when a row exceeds it by more than 2^3.9 (P then still fits f16's range), so O is seldom rescaled: a move costs its
@@ -20,7 +21,7 @@
 // Bound by the chain of a tile at head_dim 128: softmax 2000 - 2500 cycles, P V and the next S 1300 - 1700 until seen, beside which the other row tile
 // works; its exponentials alone are 2048 cycles for both row tiles.  512 new tokens, H=32 Hk=8, B=2 with 4096 - 8192 tokens: 122 - 130 us =
 // 760 - 810 TFLOP/s (cuBLAS in bf16: 1635).  At head_dim 256 by the conversion of the codes, 4400 cycles a tile, and their loads, for which 32 KB are left:
-// H=16 Hk=4 165 us.
+// H=16 Hk=4 145 us = 680 TFLOP/s.
 #include <type_traits>
 #include "dm_cache.cuh"
 #include "dm_kernels.h"

@@ -54,7 +54,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
 // key by three digits of 12, 10 and 10 bits (the first is sign, exponent and three bits: weights of one size spread over many bins),
 // histograms added over the cluster; then the kept positions in order, by scans.  Bound by the latency of its barriers: a barrier of eight CTAs
 // takes 1200 - 3500 cycles, so of each other's histograms the CTAs read 32 sums and then the 32nd of the bins that matters.  Eight rows of
-// 131071 tokens, 32768 kept: 23 us; 32 rows of 3001 - 4096: 8.
+// 131071 tokens, 32768 kept: 19 us; 32 rows of 3001 - 4096: 8.
 __global__ void __launch_bounds__(kSelThreads) cache_select_kernel(const CacheEvictParams p) {
   extern __shared__ uint4 keys4[];
   __shared__ uint4 hist4[kBins / 4];
@@ -400,7 +400,7 @@ cudaError_t launch_cache_evict(int D, const CacheEvictParams& p, cudaStream_t st
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   // A CTA of the cluster takes 4096 tokens or more.  us of a call with 2048, 4096 and 8192: 32 rows of 3001 - 4096 tokens 17.7, 14.5 and 14.5, 128 rows of
-  // 2500 - 4096 51, 38 and 38, 16 rows of 16384 34, 24 and 26, 8 rows of 32768 18.8, 18.8 and 20.8.  (Clusters of 16: few are resident at
+  // 2500 - 4096 51, 38 and 38, 16 rows of 16384 34, 24 and 26, 8 rows of 32768 18.8, 18.8 and 20.8 (before the tokens of a slice were taken at once).  (Clusters of 16: few are resident at
   // a time; eight rows of 131072 tokens took 75 against 33.)
   const int64_t most = static_cast<int64_t>(p.c.T) * p.c.page;
   int C = 1;
