@@ -479,7 +479,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 if (i + 1 < n) {
                   if (r == 0 && !(ok = wait_or_abort(bar(kKFull), (g + 1) & 1, abort_flag))) break;
                   tc_fence_after();
-                  issue_s(r, r == groups - 1);
+                  issue_s(r, r == groups - 1);                // over the P just read: products of one shape run in the order of their issue
                   if (i + 2 >= n) tc_commit(bars + kQFree + r);
                 }
               }
