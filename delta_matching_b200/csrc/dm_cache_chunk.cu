@@ -227,8 +227,10 @@ enum ChunkBar : int {
 
 // ------------------------------------------------------------------------------------------------ queries
 // q (bf16, any strides) -> f16 rows with a power of two per row, in the order of the row tiles (b, kv head, new token, head of the group; rows
-// of a head filled up to whole tiles with zeros), and the factor of each row's logits.  Eight elements a lane.  In the main kernel this took
-// its softmax warps 7000 cycles a unit, and a warp of its own 40000 and more.  The first CTA makes the division of the tiles instead.
+// of a head filled up to whole tiles with zeros), and the factor of each row's logits.  Tokens beyond the sequence's count are zeros too: their q
+// may hold anything, and the weights kernel drops such rows by a sum of infinity, which a logit that is NaN or infinite would outlive.  Eight
+// elements a lane.  In the main kernel this took its softmax warps 7000 cycles a unit, and a warp of its own 40000 and more.  The first CTA makes
+// the division of the tiles instead.
 template <int D>
 __global__ void __launch_bounds__(256) cache_chunk_queries_kernel(const CacheAttnParams p) {
   constexpr int kLanes = D / 8;
@@ -243,7 +245,7 @@ __global__ void __launch_bounds__(256) cache_chunk_queries_kernel(const CacheAtt
   const int bh = static_cast<int>(row / padded), r = static_cast<int>(row - static_cast<int64_t>(bh) * padded), b = bh / p.c.Hk, hk = bh - b * p.c.Hk;
   const int tok = r / p.rep, head = hk * p.rep + r - tok * p.rep;
   uint4 w = make_uint4(0, 0, 0, 0);
-  if (r < R) w = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + tok * p.q_sn + head * p.q_sh) + lane);
+  if (tok < checked_count(p.c.status, p.counts, b, p.Nq)) w = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + tok * p.q_sn + head * p.q_sh) + lane);
   const uint32_t v[4] = {w.x, w.y, w.z, w.w};
   float amax = 0.f;
 #pragma unroll
