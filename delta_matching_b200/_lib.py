@@ -56,6 +56,7 @@ SIGNATURES = {
     "dm_cache_append": (_I, [_P, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _P, _L, _I, _P, _P, _P, _P, _P]),
     "dm_cache_attn_workspace_bytes": (_L, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "dm_cache_attn": (_I, [_P, _P, _L, _L, _L, _I, _I, _I, _P, _L, _I, _P, _P, _I, _F, _P, _P, _P, _L, _L, _I, _I, _P, _L, _P, _P]),
+    "dm_dbg_cache_join_slots": (_I, [_I, _I, _I, _I, _I]),
     "dm_cache_evict": (_I, [_P, _I, _P, _L, _I, _P, _P, _L, _L, _P, _L, _I, _I, _I, _P, _P, _P, _P, _P]),
     "dm_kmean_static": (_I, [_P, _L, _L, _L, _I, _I, _I, _I, _P, _P, ctypes.c_char_p, _I]),
 }

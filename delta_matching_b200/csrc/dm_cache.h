@@ -80,6 +80,36 @@ struct CacheEvictParams {
   float* new_weights;               // (B, Hk, T2 * page), 0 beyond
 };
 
+// Where the join finds the pieces of a cut unit, from its entry of unit_slots.  A main kernel that gave up has left entries as the workspace came, so
+// that any value may be met: none() where the entry does not stand for slots that a grid of this size has.
+struct JoinSlots {
+  int first, count;                 // slot of the first piece; pieces, at most the grid's CTAs and one
+  int next, step;                   // slots of the pieces between: next, next + step, ...
+  int last;                         // slot of the last piece
+  __host__ __device__ bool none() const { return count == 0; }
+  __host__ __device__ int slot(int i) const { return i == 0 ? first : i == count - 1 ? last : next + (i - 1) * step; }
+};
+// dm_cache_attn.cu, four warps a CTA, two slots a warp: after the first piece the joined ones of the CTAs behind it, then the last warp's own where that
+// went on with another unit.
+__host__ __device__ inline JoinSlots join_slots_of_warps(int2 unit, int grid) {
+  const int end = unit.y >> 1;      // the last warp that has a piece
+  if (unit.x < 0 || unit.y < 0 || unit.x / 2 > end || end / 4 >= grid) return JoinSlots{};
+  const int cta0 = unit.x / 8, cta1 = end / 4, own = unit.y & 1;
+  JoinSlots x;
+  x.first = unit.x;
+  x.count = 1 + cta1 - cta0 - (own && cta1 > cta0 && end == 4 * cta1 ? 1 : 0) + own;
+  x.next = 8 * (cta0 + 1);
+  x.step = 8;
+  x.last = own ? 2 * end : 8 * cta1;
+  return x;
+}
+// dm_cache_chunk.cu, two slots a CTA: the pieces behind the first one are the first ones of their CTAs.
+__host__ __device__ inline JoinSlots join_slots_of_ctas(int2 unit, int grid) {
+  if (unit.x < 0 || unit.x / 2 > unit.y || unit.y >= grid) return JoinSlots{};
+  const int cta0 = unit.x / 2;
+  return JoinSlots{unit.x, 1 + unit.y - cta0, 2 * (cta0 + 1), 2, 2 * unit.y};
+}
+
 // Slots of partial results and their sizes for a call of dm_cache_attn.
 struct CacheAttnPlan {
   bool chunk;                       // dm_cache_chunk.cu: many rows

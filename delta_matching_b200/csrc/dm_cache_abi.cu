@@ -170,6 +170,14 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   return e == cudaSuccess ? 0 : cuda_fail(e, "cache attention launch");
 }
 
+int dm_dbg_cache_join_slots(int many_rows, int x, int y, int grid, int i) {
+  if (grid <= 0) return fail(DM_ERR_ARG, "delta_matching: grid must be positive (got %d)", grid);
+  const dm::JoinSlots s = many_rows ? dm::join_slots_of_ctas(make_int2(x, y), grid) : dm::join_slots_of_warps(make_int2(x, y), grid);
+  if (i < 0) return s.count;
+  if (i >= s.count) return fail(DM_ERR_ARG, "delta_matching: piece %d of %d", i, s.count);
+  return s.slot(i);
+}
+
 int dm_cache_evict(const dm_kv_cache* cache, int B, const int* table, int64_t table_row, int T, const int* lengths,
                    const float* weights, int64_t w_sb, int64_t w_sh, const int* new_table, int64_t new_table_row, int new_T,
                    int budget, int recent, int* new_lengths, int* kept, float* new_weights, int* status, void* stream) {

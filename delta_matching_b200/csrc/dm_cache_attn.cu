@@ -625,15 +625,10 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
     }
     return;
   }
-  if (unit.x < 0) return;                                     // whole: written by its warp
-  // Pieces: the first slot, then the joined ones of the CTAs behind it, then the last warp's own where that went on with another unit.
-  const int cta0 = unit.x / 8, last = unit.y >> 1, cta1 = last / 4, own = unit.y & 1;
-  const int pieces = 1 + cta1 - cta0 - (own && cta1 > cta0 && last == 4 * cta1 ? 1 : 0) + own;
-  const int in_tile = r - rt * row_tile;
-  auto row_of = [&](int i) {
-    const int at = i == 0 ? unit.x : own && i == pieces - 1 ? 2 * last : 8 * (cta0 + i);
-    return static_cast<int64_t>(at) * row_tile + in_tile;
-  };
+  const JoinSlots slots = join_slots_of_warps(unit, p.grid);
+  if (slots.none()) return;                                   // whole: written by its warp (or given up)
+  const int pieces = slots.count, in_tile = r - rt * row_tile;
+  auto row_of = [&](int i) { return static_cast<int64_t>(slots.slot(i)) * row_tile + in_tile; };
   float top = -CUDART_INF_F;
   for (int i = tid; i < pieces; i += 128) top = fmaxf(top, p.part_ml[row_of(i)].x);
 #pragma unroll

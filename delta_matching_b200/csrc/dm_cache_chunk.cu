@@ -879,13 +879,14 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
     if (lane == 0) *lse = -CUDART_INF_F;
     return;
   }
-  if (unit.x < 0) return;                                 // whole: written by its CTA
+  const JoinSlots slots = join_slots_of_ctas(unit, p.grid);
+  if (slots.none()) return;                               // whole: written by its CTA (or given up)
   float top = -CUDART_INF_F, sum = 0.f;
   float4 acc[kVecs] = {};
-  const int first = unit.x / 2, n = unit.y + 1;               // the CTAs that have a piece of it
+  const int n = slots.count;
   // 32 results at a time, a lane each: their maxima and sums together, then the values of those that count
-  for (int i0 = first; i0 < n; i0 += 32) {
-    const int i = i0 + lane, at = (i == first ? unit.x : 2 * i) * kRows + (r & (kRows - 1));
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane, at = slots.slot(i) * kRows + (r & (kRows - 1));
     const float2 ml = i < n ? p.part_ml[at] : make_float2(-CUDART_INF_F, 0.f);         // -inf: a piece of which the row sees nothing
     float top_new = ml.x;
 #pragma unroll

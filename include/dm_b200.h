@@ -274,6 +274,11 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
                   void* o, float* lse, float* weights, int64_t w_sb, int64_t w_sh, int W, int accumulate,
                   void* workspace, int64_t workspace_bytes, int* status, void* stream);
 
+/* Test hook, host only: which slots of its workspace the joining kernel of dm_cache_attn (many_rows = 1: that of many rows) reads for a unit whose
+ * entry of the table of pieces is (x, y), with a main kernel of `grid` CTAs: the number of pieces for i < 0, otherwise the slot of piece i.  A
+ * main kernel that gave up leaves entries of any value; 0 pieces where they stand for no slots (warps: 8 grid of them, many rows: 2 grid). */
+int dm_dbg_cache_join_slots(int many_rows, int x, int y, int grid, int i);
+
 /* At most `budget` tokens a (sequence, head) into the pages of new_table, which must not be pages that hold the tokens: all where lengths[b]
  * <= budget, else the last `recent` and the budget - recent others of greatest weight (weights (B, heads, >= T * page_size) by strides; equal ones:
  * the lowest positions; NaN is least), in their order, requantised to the scales of their new blocks (slots of the last block beyond the kept
