@@ -15,8 +15,8 @@ int32 is what each sequence holds.  Both are device tensors and are never copied
 replayed with other lengths.  An entry or length out of range is therefore reported like a kernel that gave up (RuntimeError from the next
 call, or from ops.check_status), and nothing outside the buffers is touched.
 
-Input errors raise ValueError / TypeError.  These are serving operators: no autograd graph is recorded.  Under torch.compile they are
-registered ops without a graph break.  examples/decode_with_cache.py runs the three together.  The reference package has no counterpart.
+Input errors raise ValueError / TypeError.  These are serving operators: no autograd graph is recorded, a forward-mode tangent raises
+NotImplementedError.  Under torch.compile, torch.jit.trace and dispatch modes they are registered ops without a graph break.  examples/decode_with_cache.py runs the three together.  The reference package has no counterpart.
 """
 from __future__ import annotations
 
@@ -30,6 +30,18 @@ from . import torch_ops as _torch_ops  # noqa: F401  (registers torch.ops.delta_
 
 E4M3 = torch.float8_e4m3fn
 _OPS = torch.ops.delta_matching_b200
+
+
+def _recorded():
+    """Whether something outside records this call or takes its place: a compiler, torch.jit.trace, a dispatch mode (make_fx, fake tensors).  It sees
+    the registered ops and not what the functions below do through ctypes."""
+    return torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() > 0
+
+
+def _refuse_tangents(**tensors):
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and t.is_floating_point() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"delta_matching: {name} carries a forward-mode tangent; the cache functions have no derivatives")
 
 
 class _CCache(ctypes.Structure):
@@ -151,12 +163,18 @@ def dm_cache_append(cache, k, v, block_table, lengths, counts=None):
 
     Each block of 32 slots and head gets the smallest power-of-two scale that holds its new values; a block that already holds tokens keeps
     the larger of the two scales, and its codes are rounded anew when that grows."""
-    if torch.compiler.is_compiling():
+    if _recorded():
         return _OPS.cache_append(*cache, k, v, block_table, lengths, counts)
+    return append_now(cache, k, v, block_table, lengths, counts)
+
+
+def append_now(cache, k, v, block_table, lengths, counts):
+    """dm_cache_append at once, whatever records: the implementation of the registered op too."""
     new = _lib.native_cache().cache_append(cache, k, v, block_table, lengths, counts)
     if new is not None:
         return new
     pages, Hk, P, D = _check_cache(cache)
+    _refuse_tangents(k=k, v=v, ks=cache.ks, vs=cache.vs)
     dev = cache.k8.device
     k, v = _check_rows("k", k, Hk, D, dev), _check_rows("v", v, Hk, D, dev)
     if k.shape != v.shape:
@@ -187,14 +205,20 @@ def dm_cache_attn(q, cache, block_table, lengths, q_counts=None, causal=True, so
     tokens and over the query heads of its kv head; accumulate=True adds it to what is there.  return_lse=True also returns the LSE (B, H, N)
     fp32, natural log.  The logits and the softmax are those of the codes' exact values: q and the probabilities keep 8 and 11 bits or
     more, sums and statistics are fp32."""
-    if torch.compiler.is_compiling():
+    if _recorded():
         args = (q, *cache, block_table, lengths, q_counts, bool(causal), softmax_scale)
         o, lse = _OPS.cache_attn(*args) if weights is None else _OPS.cache_attn_weights(*args, weights, bool(accumulate))
         return (o, lse) if return_lse else o
+    return attn_now(q, cache, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, return_lse)
+
+
+def attn_now(q, cache, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, return_lse):
+    """dm_cache_attn at once, whatever records: the implementation of the registered ops too."""
     out = _lib.native_cache().cache_attn(q, cache, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, return_lse)
     if out is not None:
         return out
     pages, Hk, P, D = _check_cache(cache)
+    _refuse_tangents(q=q, ks=cache.ks, vs=cache.vs, weights=weights)
     dev = cache.k8.device
     q = _check_rows("q", q, None, D, dev)
     B, N, H = q.shape[:3]
@@ -237,12 +261,18 @@ def dm_cache_evict(cache, block_table, lengths, weights, new_block_table, budget
 
     Returns (new lengths (B) int32, kept (B, Hk, budget) int32: the old positions in order, -1 beyond, new weights (B, Hk, T2 * page_size) fp32: those of the
     kept tokens, 0 beyond).  The heads of a sequence keep different tokens but equally many."""
-    if torch.compiler.is_compiling():
+    if _recorded():
         return _OPS.cache_evict(*cache, block_table, lengths, weights, new_block_table, budget, recent)
+    return evict_now(cache, block_table, lengths, weights, new_block_table, budget, recent)
+
+
+def evict_now(cache, block_table, lengths, weights, new_block_table, budget, recent):
+    """dm_cache_evict at once, whatever records: the implementation of the registered op too."""
     out = _lib.native_cache().cache_evict(cache, block_table, lengths, weights, new_block_table, budget, recent)
     if out is not None:
         return out
     pages, Hk, P, D = _check_cache(cache)
+    _refuse_tangents(ks=cache.ks, vs=cache.vs, weights=weights)
     dev = cache.k8.device
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1 or lengths.numel() == 0:
         raise ValueError("delta_matching: lengths must be a 1-D tensor, one entry per sequence")

@@ -18,7 +18,7 @@ under torch.compile without a graph break (tests/test_api.py:304-317).  The impl
 delta_matching_b200.ops (CUDA only; there is no CPU implementation to fall back to); the fake implementations only
 state shapes, dtypes and devices.  Tensors are in the op layer's layout: inputs (B, H, N, D) views, codes (B, H, N, D)
 e4m3, scales (B, H, N // 32) fp32, O / dQ (B, N, H, D), dK / dV (B, N, Hk, D) bf16.  The cache's ops take its four pools one by one (those
-marked ! are written in place) and are what the functions of cache.py call while a compiler is tracing.
+marked ! are written in place) and are what the functions of cache.py call while something records: a compiler, torch.jit.trace, a dispatch mode.
 """
 from __future__ import annotations
 
@@ -114,7 +114,7 @@ def _(q8, k8, v8, do8, qs, ks, vs, dos, lse, delta, causal, ds32):
 def _cache_append(k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, k: Tensor, v: Tensor, block_table: Tensor, lengths: Tensor,
                   counts: Optional[Tensor]) -> Tensor:
     from . import cache
-    return cache.dm_cache_append(cache.KVCache8(k8, v8, ks, vs), k, v, block_table, lengths, counts)
+    return cache.append_now(cache.KVCache8(k8, v8, ks, vs), k, v, block_table, lengths, counts)
 
 
 cache_append = torch.library.custom_op(f"{NS}::cache_append", _cache_append, mutates_args=("k8", "v8", "ks", "vs"), device_types="cuda")
@@ -128,7 +128,7 @@ def _(k8, v8, ks, vs, k, v, block_table, lengths, counts):
 def _cache_attn(q: Tensor, k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, q_counts: Optional[Tensor],
                 causal: bool, softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor]:
     from . import cache
-    return cache.dm_cache_attn(q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, return_lse=True)
+    return cache.attn_now(q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, None, False, True)
 
 
 cache_attn = torch.library.custom_op(f"{NS}::cache_attn", _cache_attn, mutates_args=(), device_types="cuda")
@@ -143,7 +143,7 @@ def _(q, k8, v8, ks, vs, block_table, lengths, q_counts, causal, softmax_scale):
 def _cache_attn_weights(q: Tensor, k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, q_counts: Optional[Tensor],
                         causal: bool, softmax_scale: Optional[float], weights: Tensor, accumulate: bool) -> Tuple[Tensor, Tensor]:
     from . import cache
-    return cache.dm_cache_attn(q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, True)
+    return cache.attn_now(q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, True)
 
 
 cache_attn_weights = torch.library.custom_op(f"{NS}::cache_attn_weights", _cache_attn_weights, mutates_args=("weights",), device_types="cuda")
@@ -158,7 +158,7 @@ def _(q, k8, v8, ks, vs, block_table, lengths, q_counts, causal, softmax_scale, 
 def _cache_evict(k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, weights: Tensor, new_block_table: Tensor,
                  budget: int, recent: int) -> Tuple[Tensor, Tensor, Tensor]:
     from . import cache
-    return cache.dm_cache_evict(cache.KVCache8(k8, v8, ks, vs), block_table, lengths, weights, new_block_table, budget, recent)
+    return cache.evict_now(cache.KVCache8(k8, v8, ks, vs), block_table, lengths, weights, new_block_table, budget, recent)
 
 
 cache_evict = torch.library.custom_op(f"{NS}::cache_evict", _cache_evict, mutates_args=("k8", "v8", "ks", "vs"), device_types="cuda")
