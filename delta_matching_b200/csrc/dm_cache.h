@@ -47,8 +47,8 @@ struct CacheAttnParams {
   float scale;                      // softmax scale
   __nv_bfloat16* o;                 // (B, Nq, H, D) contiguous
   float* lse;                       // (B, H, Nq)
-  float* part_o;                    // partial results: 2 slots a warp of (row tile, D) fp32, and their (maximum, sum) pairs
-  float2* part_ml;
+  float* part_o;                    // partial results: 2 slots a warp of (row tile, D) fp32, and of their rows (m, l, u, -): the logits' sum is l 2^m, the
+  float4* part_ml;                  // values count in 2^u (a constant of the form aside)
   __half* q16;                      // many rows: the queries in f16 and the order of the row tiles, and the factors of their logits
   float* factors;
   void* starts;                     // and what each CTA begins with

@@ -148,7 +148,7 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   p.logits = x.logit_bytes > 0 ? reinterpret_cast<float*>(take(x.logit_bytes)) : nullptr;
   p.logit_rows = x.logit_rows;
   p.q16 = reinterpret_cast<__half*>(take(x.q16_bytes));
-  p.part_ml = reinterpret_cast<float2*>(take(x.part_ml_bytes));
+  p.part_ml = reinterpret_cast<float4*>(take(x.part_ml_bytes));
   p.factors = reinterpret_cast<float*>(take(x.factor_bytes));
   p.row_ml = weights != nullptr ? reinterpret_cast<float2*>(take(x.row_ml_bytes)) : nullptr;
   p.starts = take(x.start_bytes);

@@ -6,8 +6,9 @@
 // made with the keys as M (16) and the rows as N (8 a tile) of mma.m16n8k16, so that a group of up to 8 rows wastes nothing and the
 // transposed product V^T P needs P in the layout that it comes in, up to one movmatrix.  The codes are exact in f16; q is brought to f16 with
 // a power of two per row (bf16's 8 bits fit f16's 11), p = exp2(x) is rounded to f16's 11 bits; sums, maxima and accumulators are fp32.  The
-// power-of-two scale of V's block goes into the exponent of p, relative to the largest the warp has met, and the scale of K's block into
-// the factor of the logits, so no code is ever multiplied by a scale.
+// power-of-two scale of V's block goes into the exponent of p, relative to the largest product of a probability and a scale that the row has met
+// (blocks that it does not see, or gives no weight, cost it no bits), and the scale of K's block into the factor of the logits, so no code is
+// ever multiplied by a scale.
 //
 // Every warp works for itself: it takes an even share of the blocks of 32 tokens of the whole call (dm_cache_sched.cuh), one after the other, with
 // its own maximum, sum and accumulator, and fills its own ring of TMA boxes (32 rows x 128 bytes, 128-byte swizzle, straight from the pages),
@@ -29,6 +30,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxCluster = 8;
+constexpr float kNone = -3e38f;              // below all logits: a reference before the first one (infinities would not cancel)
 
 template <int D, int NT>
 struct AttnCfg {
@@ -38,7 +40,7 @@ struct AttnCfg {
   static constexpr int kCtasPerSm = D == 128 && NT == 1 ? 3 : 2;
   static constexpr int kSlots = D == 128 ? (NT == 2 ? 6 : 4) : 3;
   static constexpr int kRing = kWarps * kSlots * kSlotBytes;
-  static constexpr int kStats = kWarps * kRows * 8;           // maximum and sum of a warp's rows, for the CTA's own join
+  static constexpr int kStats = kWarps * kRows * 16;          // m, l and u of a warp's rows, for the CTA's own join
   static constexpr int kSmem = 1024 + kRing + kStats + kWarps * kSlots * 8 + 136 * 4 + 64;
   static_assert(NT * D * 32 <= kSlots * kSlotBytes, "a warp leaves its accumulator in its ring");
 };
@@ -154,7 +156,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
-  float2* stats = reinterpret_cast<float2*>(smem + C::kRing);
+  float4* stats = reinterpret_cast<float4*>(smem + C::kRing);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kStats);
   int* cum = reinterpret_cast<int*>(bars + C::kWarps * C::kSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(cum + 134);
@@ -260,23 +262,20 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (ok) issue();
   };
   float m[NT][2], l[NT][2], acc[NT][D / 16][4];
-  int vexp = -1000, slot = 2 * worker;
-  // Of a finished piece: the accumulator in its true scale and the rows' sums, complete in every lane.
+  // of a row, whole numbers: m, at most 1 below the largest logit, which l is the sum beside; u, at most 0.99 below the largest logit + log2 of its V
+  // scale: the accumulator counts in 2^(u - 15), so that it is left alone while u stays
+  float u[NT][2];
+  int slot = 2 * worker;
+  // Of a finished piece: the rows' sums, complete in every lane.
   auto settle = [&]() {
-    const float unit_exp = exp2f(static_cast<float>(max(vexp, -200) - 15));
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], o);
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][c][i] *= unit_exp;
-    }
   };
-  // The settled results of a warp: to where they belong, or to a slot for the join.  `one`: only this sixteenth of head_dim, held in the first.
+  // The results of a warp: to where they belong, or to a slot for the join.  `one`: only this sixteenth of head_dim, held in the first.
   auto write_out = [&](bool whole, int to_slot, int one) {
     const int hk = seg.unit / row_tiles, rt = seg.unit - hk * row_tiles, count = checked_count(p.c.status, p.counts, seg.b, p.Nq);
 #pragma unroll
@@ -288,7 +287,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (whole) {
           const RowInfo ri = row_info(p, r, hk, seg.n, count);
           const bool any = ri.limit > 0;
-          const float inv = any ? 1.f / l[j][e] : 0.f;
+          const float inv_l = any ? 1.f / l[j][e] : 0.f, inv = inv_l * unit_of(u[j][e], m[j][e], 15);
           __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(seg.b) * p.Nq + ri.i) * p.H + ri.head) * D + 2 * g);
           if (kCluster) {
             o[8 * one] = any ? __floats2bfloat162_rn(acc[j][0][e] * inv, acc[j][0][2 + e] * inv) : __floats2bfloat162_rn(0.f, 0.f);
@@ -300,14 +299,14 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           if (g == 0 && one == 0) {
             p.lse[(static_cast<int64_t>(seg.b) * p.H + ri.head) * p.Nq + ri.i] = any ? (m[j][e] + log2f(l[j][e])) * kLn2 : -CUDART_INF_F;
             if (p.row_ml != nullptr)
-              p.row_ml[(static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.Nq * p.rep + r] = make_float2(any ? m[j][e] : 0.f, inv);
+              p.row_ml[(static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.Nq * p.rep + r] = make_float2(any ? m[j][e] : 0.f, inv_l);
           }
         } else {
           const int64_t row = static_cast<int64_t>(to_slot) * C::kRows + in_tile;
           float2* o = reinterpret_cast<float2*>(p.part_o + row * D + 2 * g);
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) o[8 * c] = make_float2(acc[j][c][e], acc[j][c][2 + e]);
-          if (g == 0) p.part_ml[row] = make_float2(m[j][e], l[j][e]);
+          if (g == 0) p.part_ml[row] = make_float4(m[j][e], l[j][e], u[j][e], 0.f);
         }
       }
   };
@@ -330,10 +329,9 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
       for (int e = 0; e < 2; ++e) lim[j][e] = row_info(p, rt * C::kRows + 8 * j + 2 * t + e, hk, seg.n, count).limit;
     if (p.causal) lim_min = seg.n - count + 1;                // of the rows that are any
-    vexp = -1000;                                             // largest exponent of a V scale so far: the accumulator counts in 2^(vexp - 15)
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      m[j][0] = m[j][1] = -CUDART_INF_F;
+      m[j][0] = m[j][1] = u[j][0] = u[j][1] = kNone;
       l[j][0] = l[j][1] = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) acc[j][c][0] = acc[j][c][1] = acc[j][c][2] = acc[j][c][3] = 0.f;
@@ -348,15 +346,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       keys_times_queries<D, NT>(ring + get * C::kSlotBytes, qf, s);
       const int key0 = (kCluster ? blk_first + kb * blk_step : kb) * 32;
       const bool cut = key0 + 32 > lim_min;                   // some row does not see all keys of the block
-      const int e_blk = static_cast<int>((__float_as_uint(vs) >> 23) & 0xFF) - 127, e_new = max(vexp, e_blk);
-      // p comes out as 2^off exp(s - m); where V's scale is 2^-60 of another's the product vanishes anyway, but the sum must not
-      const int off = max(15 + e_blk - e_new, -45);
-      const float back = __uint_as_float((127 - off) << 23);
-      const int shrink = vexp - e_new;
-      bool moved = shrink != 0;
-      vexp = e_new;
+      const float e_blk = static_cast<float>(static_cast<int>(scale_to_sb(vs)) - 127);
       uint32_t pb[NT][2][2];
-      float2 alpha[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const float2 fs = make_float2(f[j].x * ks, f[j].y * ks);
@@ -383,44 +374,48 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o));
           mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o));
         }
-        mx.x = fmaxf(mx.x, m[j][0]);
-        mx.y = fmaxf(mx.y, m[j][1]);
-        moved |= mx.x != m[j][0] || mx.y != m[j][1];
-        const float2 mu = make_float2(mx.x == -CUDART_INF_F ? 0.f : mx.x, mx.y == -CUDART_INF_F ? 0.f : mx.y);
-        alpha[j] = make_float2(ex2_approx(m[j][0] - mu.x), ex2_approx(m[j][1] - mu.y));
-        m[j][0] = mx.x;
-        m[j][1] = mx.y;
-        const float2 sub = make_float2(off - mu.x, off - mu.y);
+        const float2 pv = make_float2(mx.x + e_blk, mx.y + e_blk);
+        if (__any_sync(0xffffffffu, mx.x > m[j][0] + 1.f || mx.y > m[j][1] + 1.f || pv.x > u[j][0] + 0.99f || pv.y > u[j][1] + 0.99f)) {
+          float keep[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float m_old = m[j][e], u_old = u[j][e], mx_e = e ? mx.y : mx.x, pv_e = e ? pv.y : pv.x;
+            if (mx_e > m_old + 1.f) m[j][e] = nearest(mx_e);
+            if (pv_e > u_old + 0.99f) u[j][e] = nearest(pv_e);
+            l[j][e] *= ex2_approx(m_old - m[j][e]);
+            keep[e] = ex2_approx(u_old - u[j][e]);
+          }
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            acc[j][c][0] *= keep[0];
+            acc[j][c][1] *= keep[1];
+            acc[j][c][2] *= keep[0];
+            acc[j][c][3] *= keep[1];
+          }
+        }
+        float sub[2], back[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // p comes out as 2^(sub + s), below 2^16; where the products are 2^-60 of the largest they vanish anyway, but the sum must not
+          sub[e] = fmaxf(15.f + e_blk - u[j][e], -45.f - m[j][e]);
+          back[e] = ex2_approx(-sub[e] - m[j][e]);            // zero where p is below 2^-111 of the largest
+        }
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           float e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            e[i] = ex2_approx(s[j][mt][i] + ((i & 1) ? sub.y : sub.x));
+            e[i] = ex2_approx(s[j][mt][i] + sub[i & 1]);
             if (i & 1) sum.y += e[i]; else sum.x += e[i];
           }
           pb[j][mt][0] = movmatrix_trans(pack_f16x2(e[0], e[1]));
           pb[j][mt][1] = movmatrix_trans(pack_f16x2(e[2], e[3]));
         }
-        l[j][0] = fmaf(l[j][0], alpha[j].x, sum.x * back);
-        l[j][1] = fmaf(l[j][1], alpha[j].y, sum.y * back);
+        l[j][0] = fmaf(sum.x, back[0], l[j][0]);
+        l[j][1] = fmaf(sum.y, back[1], l[j][1]);
       }
       release();
-      if (__any_sync(0xffffffffu, moved)) {
-        const float by = shrink == 0 ? 1.f : exp2f(static_cast<float>(shrink));
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float ax = alpha[j].x * by, ay = alpha[j].y * by;
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            acc[j][c][0] *= ax;
-            acc[j][c][1] *= ay;
-            acc[j][c][2] *= ax;
-            acc[j][c][3] *= ay;
-          }
-        }
-      }
       arrived();
       if (!ok) break;
       const uint32_t vbase = ring + get * C::kSlotBytes;
@@ -483,7 +478,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   if (kCluster && !pending) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      m[j][0] = m[j][1] = -CUDART_INF_F;
+      m[j][0] = m[j][1] = u[j][0] = u[j][1] = kNone;
       l[j][0] = l[j][1] = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) acc[j][c][0] = acc[j][c][1] = acc[j][c][2] = acc[j][c][3] = 0.f;
@@ -499,27 +494,27 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       if (g == 0) {
-        stats[warp * C::kRows + 8 * j + 2 * t] = make_float2(m[j][0], l[j][0]);
-        stats[warp * C::kRows + 8 * j + 2 * t + 1] = make_float2(m[j][1], l[j][1]);
+        stats[warp * C::kRows + 8 * j + 2 * t] = make_float4(m[j][0], l[j][0], u[j][0], 0.f);
+        stats[warp * C::kRows + 8 * j + 2 * t + 1] = make_float4(m[j][1], l[j][1], u[j][1], 0.f);
       }
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) parked[(j * (D / 16) + c) * 32 + lane] = make_float4(acc[j][c][0], acc[j][c][1], acc[j][c][2], acc[j][c][3]);
     }
   };
   // Parked results, by their base and statistics, into this warp's.
-  auto take_over = [&](const float4* from, const float2* st) {
+  auto take_over = [&](const float4* from, const float4* st) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float2 mine, theirs;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float2 x = st[8 * j + 2 * t + e];
-        const float top = fmaxf(m[j][e], x.x), mu = top == -CUDART_INF_F ? 0.f : top;
-        const float a = ex2_approx(m[j][e] - mu), b = ex2_approx(x.x - mu);
-        l[j][e] = l[j][e] * a + x.y * b;
+        const float4 x = st[8 * j + 2 * t + e];
+        const float top = fmaxf(m[j][e], x.x), top_u = fmaxf(u[j][e], x.z);
+        l[j][e] = l[j][e] * ex2_approx(m[j][e] - top) + x.y * ex2_approx(x.x - top);
+        (e ? mine.y : mine.x) = ex2_approx(u[j][e] - top_u);
+        (e ? theirs.y : theirs.x) = ex2_approx(x.z - top_u);
         m[j][e] = top;
-        (e ? mine.y : mine.x) = a;
-        (e ? theirs.y : theirs.x) = b;
+        u[j][e] = top_u;
       }
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
@@ -543,36 +538,42 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     // CTA r of the cluster joins and writes its share of the sixteenths of head_dim, a warp a sixteenth, over the CTAs in order
     const int cl = p.cluster, rank = blockIdx.x % cl, c1 = (rank + 1) * (D / 16) / cl;
     for (int c = rank * (D / 16) / cl + warp; c < c1; c += C::kWarps) {
+      // Lane (g, t) looks at CTA g's statistics of its rows; these and the values are all on their way together.
+      float4 st[NT][2], x[NT][kMaxCluster];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        float2 st[kMaxCluster][2];
-        float4 x[kMaxCluster];                                // all on their way together
 #pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-          if (r >= cl) continue;
-          const float2* from = cluster.map_shared_rank(stats, r) + 8 * j + 2 * t;
-          st[r][0] = from[0];
-          st[r][1] = from[1];
-          x[r] = cluster.map_shared_rank(reinterpret_cast<float4*>(smem), r)[(j * (D / 16) + c) * 32 + lane];
-        }
+        for (int e = 0; e < 2; ++e)
+          st[j][e] = g < cl ? cluster.map_shared_rank(stats, g)[8 * j + 2 * t + e] : make_float4(kNone, 0.f, kNone, 0.f);
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < cl) x[j][r] = cluster.map_shared_rank(reinterpret_cast<float4*>(smem), r)[(j * (D / 16) + c) * 32 + lane];
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
         float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = -CUDART_INF_F, sum = 0.f;
+          float top = st[j][e].x, top_u = st[j][e].z;
 #pragma unroll
-          for (int r = 0; r < kMaxCluster; ++r)
-            if (r < cl) top = fmaxf(top, st[r][e].x);
-          const float mu = top == -CUDART_INF_F ? 0.f : top;
+          for (int i = 4; i < 32; i <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+            top_u = fmaxf(top_u, __shfl_xor_sync(0xffffffffu, top_u, i));
+          }
+          float sum = st[j][e].y * ex2_approx(st[j][e].x - top);
+          const float w = ex2_approx(st[j][e].z - top_u);
+#pragma unroll
+          for (int i = 4; i < 32; i <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
 #pragma unroll
           for (int r = 0; r < kMaxCluster; ++r) {
             if (r >= cl) continue;
-            const float w = ex2_approx(st[r][e].x - mu);
-            sum = fmaf(st[r][e].y, w, sum);
-            o[e] = fmaf(e ? x[r].y : x[r].x, w, o[e]);
-            o[2 + e] = fmaf(e ? x[r].w : x[r].z, w, o[2 + e]);
+            const float w_r = __shfl_sync(0xffffffffu, w, 4 * r + t);
+            o[e] = fmaf(e ? x[j][r].y : x[j][r].x, w_r, o[e]);
+            o[2 + e] = fmaf(e ? x[j][r].w : x[j][r].z, w_r, o[2 + e]);
           }
           m[j][e] = top;
           l[j][e] = sum;
+          u[j][e] = top_u;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][0][i] = o[i];
@@ -605,7 +606,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 template <int D>
 __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p, const int row_tiles, const int row_tile) {
   __shared__ float part[4][D];
-  __shared__ float factors[128], red[4];
+  __shared__ float factors[128], red[8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dep_wait();
   const int R = p.Nq * p.rep;
@@ -629,22 +630,33 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
   if (slots.none()) return;                                   // whole: written by its warp (or given up)
   const int pieces = slots.count, in_tile = r - rt * row_tile;
   auto row_of = [&](int i) { return static_cast<int64_t>(slots.slot(i)) * row_tile + in_tile; };
-  float top = -CUDART_INF_F;
-  for (int i = tid; i < pieces; i += 128) top = fmaxf(top, p.part_ml[row_of(i)].x);
+  float top = -CUDART_INF_F, top_u = -CUDART_INF_F;
+  for (int i = tid; i < pieces; i += 128) {
+    const float4 x = p.part_ml[row_of(i)];
+    top = fmaxf(top, x.x);
+    top_u = fmaxf(top_u, x.z);
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) red[warp] = top;
+  for (int o = 16; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top_u = fmaxf(top_u, __shfl_xor_sync(0xffffffffu, top_u, o));
+  }
+  if (lane == 0) {
+    red[warp] = top;
+    red[4 + warp] = top_u;
+  }
   __syncthreads();
   top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  top_u = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
   float sum = 0.f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
   for (int i0 = 0; i0 < pieces; i0 += 128) {                  // 128 pieces at a time: their factors, then their rows
     float f = 0.f;
     if (i0 + tid < pieces) {
-      const float2 ml = p.part_ml[row_of(i0 + tid)];
-      f = ml.x == -CUDART_INF_F ? 0.f : exp2f(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
+      const float4 x = p.part_ml[row_of(i0 + tid)];
+      f = ex2_approx(x.z - finite_or_zero(top_u));
+      sum = fmaf(x.y, ex2_approx(x.x - finite_or_zero(top)), sum);
     }
     if (i0 > 0) __syncthreads();
     factors[tid] = f;
@@ -672,11 +684,11 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
   if (lane == 0) red[warp] = sum;
   __syncthreads();
   sum = (red[0] + red[1]) + (red[2] + red[3]);
-  const float inv = 1.f / sum;
+  const float inv_l = 1.f / sum, inv = inv_l * unit_of(top_u, top, 15);
   for (int d = tid; d < D; d += 128) o[d] = __float2bfloat16(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
   if (tid == 0) {
     *lse = (top + log2f(sum)) * kLn2;
-    if (p.row_ml != nullptr) p.row_ml[item] = make_float2(top, inv);
+    if (p.row_ml != nullptr) p.row_ml[item] = make_float2(top, inv_l);
   }
 }
 
@@ -927,7 +939,7 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   x.grid = x.cluster > 0 ? static_cast<int>(units) * x.cluster : static_cast<int>(most < wave ? most : wave);
   const int64_t slots = x.cluster > 0 ? 0 : 2ll * x.grid * (x.chunk ? 1 : 4);
   x.part_o_bytes = slots * x.row_tile * D * 4;
-  x.part_ml_bytes = slots * x.row_tile * 8;
+  x.part_ml_bytes = slots * x.row_tile * 16;
   const int64_t q_rows = x.chunk ? cache_chunk_query_rows(B, Hk, R) : 0;
   x.q16_bytes = q_rows * D * 2;
   x.factor_bytes = q_rows * 4;

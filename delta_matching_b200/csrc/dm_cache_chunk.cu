@@ -1,8 +1,8 @@
 // Attention of many new queries over the 8-bit cache (chunks of a prompt): the same result as dm_cache_attn.cu, on tcgen05.
 //
 //   S = Q K^T and O += P V as f16 tcgen05 chains with fp32 accumulators in TMEM.  The codes are exact in f16, q is brought to f16 with a power
-//   of two per row, P is f16 with the row's reference maximum at 2^12 (11 bits, never closer than 2^-37 of it); K's block scales go into
-//   the factors of the logits, V's into the exponent of P relative to the largest the row tile has met.
+//   of two per row; K's block scales go into the factors of the logits, V's into the exponent of P.  P is f16 with the row's largest product of a
+//   probability and a V scale at 2^12 (11 bits, never closer than 2^-36 of it): blocks that a row does not see, or gives no weight, cost it no bits.
 //
 // A unit is (sequence, kv head, 256 rows); rows are (new token, head of the group).  The key tiles of 128 tokens of all units are one flat
 // range, divided evenly over one CTA per SM (as the warps' blocks are in dm_cache_sched.cuh); pieces of cut units are joined by a second kernel.
@@ -12,8 +12,9 @@
 // tensor cores work for the other.
 //
 // TMEM: S0 0-127, S1 128-255 (P of a tile over the first 64 columns of its S), O0 256-383, O1 384-511.
-// The reference moves only when a row exceeds it by more than 2^3.9 (P then still fits f16's range), so O is seldom rescaled: a move costs its
-// row tile about 3000 cycles, and with a reference that follows within a factor of two some warp moved it in most tiles (6800 cycles a tile).
+// The references (of the sum, and of the products) move only when a row exceeds them by more than 2^3.9 (P then still fits f16's range), so O is seldom
+// rescaled: a move costs its row tile about 3000 cycles, and with a reference that follows within a factor of two some warp moved it in most
+// tiles (6800 cycles a tile).
 //
 // Head_dim 256: a unit is 128 rows, the two softmax groups take half of a tile's keys each and half of O, S has two buffers (0-127, 128-255) and
 // O the columns 256-511.
@@ -33,7 +34,7 @@ namespace {
 // Key tiles that a unit's queries and output are worth.  us with 1, 3 and 6 at H=32 Hk=8: 512 new tokens, B=2 with 4096 - 8192 126, 123.8 and 130.6; 128
 // new ones, B=4 with 512 35.2, 32.6 and 33.0.
 constexpr int kChunkCost = 3;
-constexpr int kPBase = 12;                  // log2 of P at the reference maximum,
+constexpr int kPBase = 12;                  // log2 of P at the reference,
 constexpr float kHeadroom = 3.9f;           // and what a row may exceed it by: P stays below 2^16
 
 // D = 256: as D = 128, but one row tile, whose two softmax groups take half of the keys each, and O of 256 columns.
@@ -58,7 +59,7 @@ struct ChunkCfg {
   static constexpr int kSmemBars = kSmemCode + (kWide ? 2 : 4) * kTile;
   static constexpr int kSmemScales = kSmemBars + 416;         // 8 tiles x (4 K scales, 4 V scales)
   static constexpr int kSmemRows = kSmemScales + 8 * 32;      // what the two groups tell each other of their rows
-  static constexpr int kSmem = kSmemRows + (kWide ? 1024 : 0) + 1024;
+  static constexpr int kSmem = kSmemRows + (kWide ? 1024 + 256 : 0) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -385,7 +386,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         ask_scales(next);
         if (lane < 4) {
           scales[(g & 7) * 8 + lane] = now.ks;                // zero where there is no block
-          scales[(g & 7) * 8 + 4 + lane] = now.vs;
+          scales[(g & 7) * 8 + 4 + lane] = static_cast<float>(static_cast<int>(scale_to_sb(now.vs)) - 127);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
@@ -604,6 +605,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const int r = warp >> 2, in_tile = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t t_o = tmem + lanes + 256 + 128 * r;      // of 256 columns, the half that this group rescales and writes
+      volatile int8_t* told_d = reinterpret_cast<volatile int8_t*>(smem + C::kSmemRows + 1024) + in_tile;        // the same, a second value
       volatile float* told = reinterpret_cast<volatile float*>(smem + C::kSmemRows) + in_tile;        // by group 0 of this row; by group 1 128 values on
       const uint32_t stage = sbase + C::kSmemOut + warp * 4096;
       int g = 0, mine = 0, asked = 0, tells = 0;              // running tile; tiles of this row tile; votes and values that the pair has exchanged
@@ -624,8 +626,9 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         // of the row's logits, K's scale aside
         const int64_t padded_row = (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + 127) / 128 * 128) + row;
         const float f = __ldg(p.factors + padded_row);
-        float m = -CUDART_INF_F, l = 0.f;
-        int vexp = -1000;
+        // Of the row, whole numbers: m, the reference of the sum l; u, that of the products of a probability and its V scale: O counts in 2^(u - kPBase).
+        // The largest logit, and logit + log2 of its V scale, are at most kHeadroom above them.
+        float m = -CUDART_INF_F, u = -CUDART_INF_F, l = 0.f;
         // P V of this group's tile i is in O.  With 256 columns the softmax may be two tiles ahead of the products, so that these have two barriers.
         auto products_of = [&](int i) { return C::kWide ? wait_warp(bar(kPvDone + (i & 1)), (i >> 1) & 1, abort_flag) : wait_warp(bar(kPvDone + r), i & 1, abort_flag); };
         // What the two warps of a row's two groups know of it (256 columns): the other's value.
@@ -644,10 +647,8 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           const float4 ks = lds_f4(sbase + C::kSmemScales + entry * 32), vs = lds_f4(sbase + C::kSmemScales + entry * 32 + 16);
           const uint32_t t_s = tmem + lanes + (C::kWide ? 128 * (mine & 1) + 64 * r : 128 * r);
           const float fc[4] = {f * (C::kWide && r ? ks.z : ks.x), f * (C::kWide && r ? ks.w : ks.y), f * ks.z, f * ks.w};
-          const int ev[4] = {static_cast<int>(scale_to_sb(vs.x)) - 127, static_cast<int>(scale_to_sb(vs.y)) - 127, static_cast<int>(scale_to_sb(vs.z)) - 127,
-                             static_cast<int>(scale_to_sb(vs.w)) - 127};
+          const float ev[4] = {C::kWide && r ? vs.z : vs.x, C::kWide && r ? vs.w : vs.y, vs.z, vs.w};
           const int seen = sees - 128 * t - (C::kWide ? 64 * r : 0);         // keys of the tile, from this group's first on, that the row sees
-          const int v_new = max(max(vexp, max(ev[0], ev[1])), max(ev[2], ev[3]));
           // 32 columns at a time, the next ones in flight; what a row does not see is -inf
           uint32_t s_buf[2][32];
           auto columns = [&](int c) {
@@ -660,7 +661,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             }
           };
           auto pair = [&](int c, int e) { return make_float2(__uint_as_float(s_buf[c & 1][2 * e]), __uint_as_float(s_buf[c & 1][2 * e + 1])); };
-          float top = -CUDART_INF_F;
+          float top = -CUDART_INF_F, top2 = -CUDART_INF_F;    // of the tile: logit, and logit + log2 of V's scale
           tmem_ld32(t_s, s_buf[0]);
 #pragma unroll
           for (int c = 0; c < C::kCols / 32; ++c) {
@@ -668,12 +669,13 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             float2 s2[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) s2[e] = pair(c, e);
-            const float top_c = max32(s2);
-            top = fmaxf(top, kCut && top_c == -CUDART_INF_F ? top_c : top_c * fc[c]);     // the factor may be zero
+            const float top_s = max32(s2), top_c = kCut && top_s == -CUDART_INF_F ? top_s : top_s * fc[c];        // the factor may be zero
+            top = fmaxf(top, top_c);
+            top2 = fmaxf(top2, top_c + ev[c]);
           }
           if (C::kWide) {
             // a common reference: seldom does a row move, so that the pair first tell each other whether any does
-            const bool moves = __any_sync(0xffffffffu, top > m + kHeadroom);
+            const bool moves = __any_sync(0xffffffffu, top > m + kHeadroom || top2 > u + kHeadroom);
             volatile uint8_t* votes = smem + C::kSmemBars + 8 * (kBars + 2 + (asked & 1));      // behind the TMEM slot and the abort flag
             const int vote = kVote + 2 * (warp & 3) + (asked & 1);
             if (lane == 0) {
@@ -683,19 +685,24 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             if (!wait_warp(bar(vote), (asked++ >> 1) & 1, abort_flag)) return false;
             if (moves || votes[warp ^ 4]) {
               float other;
+              // the second value as its distance from the first, rounded up: the same in both groups
+              const float d = fminf(fmaxf(ceilf(top2 - top), -128.f), 127.f);
+              told_d[128 * r] = static_cast<int8_t>(d);
               if (!tell(top, other)) return false;
+              top2 = fmaxf(top + d, other + static_cast<float>(told_d[128 * (r ^ 1)]));
               top = fmaxf(top, other);
             }
           }
-          const float m_new = top > m + kHeadroom ? top : m;
-          const float mu = m_new == -CUDART_INF_F ? 0.f : m_new;
           tmem_ld32(t_s, s_buf[0]);
-          if (__any_sync(0xffffffffu, m_new != m || v_new != vexp)) {
-            const float keep = ex2_approx(m - mu);
+          if (__any_sync(0xffffffffu, top > m + kHeadroom || top2 > u + kHeadroom)) {
+            const float m_old = m, u_old = u;
+            if (top > m + kHeadroom) m = ceilf(top);
+            if (top2 > u + kHeadroom) u = ceilf(top2);
+            l *= ex2_approx(m_old - finite_or_zero(m));
             if (t > x.t0) {
               if (!products_of(mine - 1)) return false;
               tc_fence_after();
-              const float a = keep * exp2f(static_cast<float>(vexp - v_new));
+              const float a = ex2_approx(u_old - finite_or_zero(u));
 #pragma unroll 1
               for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
@@ -706,15 +713,13 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 tmem_st32(t_o + 32 * c, o);
               }
             }
-            l *= keep;
-            m = m_new;
-            vexp = v_new;
           }
+          const float mu = finite_or_zero(m), uu = finite_or_zero(u);
 #pragma unroll
           for (int c = 0; c < C::kCols / 32; ++c) {
-            // P comes out as 2^off exp(s - m); where V's scale is 2^-57 of another's the product vanishes anyway, but the sum must not
-            const int off = max(kPBase + (C::kWide && r ? ev[(c + 2) & 3] : ev[c]) - vexp, -45);
-            const float2 f2 = splat2(fc[c]), sub = splat2(static_cast<float>(off) - mu);
+            // P comes out as 2^(off + s), below 2^16; where the products are 2^-57 of the largest they vanish anyway, but the sum must not
+            const float off = fmaxf(kPBase + ev[c] - uu, -45.f - mu);
+            const float2 f2 = splat2(fc[c]), sub = splat2(off);
             columns(c);
             float2 sum = make_float2(0.f, 0.f);
             uint32_t h[16];
@@ -729,7 +734,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
               sum = add2(sum, y);
               h[e] = pack_f16x2(y.x, y.y);
             }
-            l = fmaf(sum.x + sum.y, __uint_as_float(static_cast<uint32_t>(127 - off) << 23), l);
+            l = fmaf(sum.x + sum.y, ex2_approx(-off - mu), l);        // a power of two; zero where p is below 2^-111 of the largest
             tmem_st16(t_s + 16 * c, h);                       // over columns that have been read: 16 c + 15 < 32 c + 32
             if (!C::kWide && c == 1) {                        // the first half of the keys: the tensor cores may begin
               tmem_wait_st();
@@ -771,8 +776,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         const bool whole = x.t0 == 0 && x.t1 == x.tiles;
-        const float unit_exp = exp2f(static_cast<float>(vexp - kPBase));
-        const float scale = whole ? unit_exp / l : unit_exp;
+        const float scale = whole ? unit_of(u, m, kPBase) / l : 1.f;
         // where a row that sees something goes
         const int64_t out_row = limit == 0 ? -1 : ((static_cast<int64_t>(x.b) * p.Nq + i_tok) * p.H + head) * D;
         // Through shared memory, so that the lanes of a store write whole rows (a row a thread, 16 bytes at a time, took 11000 cycles a piece):
@@ -834,7 +838,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.Nq + i_tok] = (m + log2f(l)) * kLn2;
             if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(f, m + log2f(l));
           } else {
-            p.part_ml[part0 + lane] = make_float2(m, l);
+            p.part_ml[part0 + lane] = make_float4(m, l, u, 0.f);
           }
         }
         tc_fence_before();
@@ -881,24 +885,29 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
   }
   const JoinSlots slots = join_slots_of_ctas(unit, p.grid);
   if (slots.none()) return;                               // whole: written by its CTA (or given up)
-  float top = -CUDART_INF_F, sum = 0.f;
+  float top = -CUDART_INF_F, top_u = -CUDART_INF_F, sum = 0.f;
   float4 acc[kVecs] = {};
   const int n = slots.count;
   // 32 results at a time, a lane each: their maxima and sums together, then the values of those that count
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int i = i0 + lane, at = slots.slot(i) * kRows + (r & (kRows - 1));
-    const float2 ml = i < n ? p.part_ml[at] : make_float2(-CUDART_INF_F, 0.f);         // -inf: a piece of which the row sees nothing
-    float top_new = ml.x;
+    const float4 ml = i < n ? p.part_ml[at] : make_float4(-CUDART_INF_F, 0.f, -CUDART_INF_F, 0.f);     // -inf: a piece of which the row sees nothing
+    float top_new = ml.x, u_new = ml.z;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, o));
+    for (int o = 16; o > 0; o >>= 1) {
+      top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, o));
+      u_new = fmaxf(u_new, __shfl_xor_sync(0xffffffffu, u_new, o));
+    }
     top_new = fmaxf(top, top_new);
+    u_new = fmaxf(top_u, u_new);
     if (top_new == -CUDART_INF_F) continue;
-    const float a = exp2f(top - top_new), w = exp2f(ml.x - top_new);
-    float l = ml.y * w;
+    const float a = ex2_approx(top_u - u_new), w = ex2_approx(ml.z - u_new);
+    float l = ml.y * ex2_approx(ml.x - top_new);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    sum = sum * a + l;
+    sum = sum * ex2_approx(top - top_new) + l;
     top = top_new;
+    top_u = u_new;
 #pragma unroll
     for (int x = 0; x < kVecs; ++x) acc[x] = make_float4(acc[x].x * a, acc[x].y * a, acc[x].z * a, acc[x].w * a);
     const uint32_t counts = __ballot_sync(0xffffffffu, ml.x > -CUDART_INF_F);
@@ -914,7 +923,7 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
       }
     }
   }
-  const float inv = 1.f / sum;
+  const float inv = unit_of(top_u, top, kPBase) / sum;
 #pragma unroll
   for (int x = 0; x < kVecs; ++x) {
     o[64 * x] = __floats2bfloat162_rn(acc[x].x * inv, acc[x].y * inv);
