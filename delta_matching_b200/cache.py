@@ -203,8 +203,9 @@ def dm_cache_attn(q, cache, block_table, lengths, q_counts=None, causal=True, so
 
     weights: an fp32 (B, Hk, W) tensor, W >= T * page_size, that receives for every held token the softmax weight it got, summed over the new
     tokens and over the query heads of its kv head; accumulate=True adds it to what is there.  return_lse=True also returns the LSE (B, H, N)
-    fp32, natural log.  The logits and the softmax are those of the codes' exact values: q and the probabilities keep 8 and 11 bits or
-    more, sums and statistics are fp32."""
+    fp32, natural log.  The logits and the softmax are those of the codes' exact values: q keeps its 8 bits (elements below 2^-28 of the row's
+    largest lose some), sums and statistics are fp32.  In the second product a probability times the scale of its V block keeps 11 bits down to
+    2^-25 of the largest such product that the row sees; smaller ones are off by up to 2^-36 of that."""
     if _recorded():
         args = (q, *cache, block_table, lengths, q_counts, bool(causal), softmax_scale)
         o, lse = _OPS.cache_attn(*args) if weights is None else _OPS.cache_attn_weights(*args, weights, bool(accumulate))
