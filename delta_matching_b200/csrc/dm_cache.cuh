@@ -64,11 +64,8 @@ __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
   return cvt_e4m3x4(a.x * ratio, a.y * ratio, b.x * ratio, b.y * ratio);
 }
 
-__device__ __forceinline__ float finite_or_zero(float x) { return x == -CUDART_INF_F ? 0.f : x; }
-// The nearest whole number, on the FMA pipe; for sizes up to 2^22 (beyond it a number no further away than its neighbours).
-__device__ __forceinline__ float nearest(float x) { return (x + 12582912.f) - 12582912.f; }
-// What an accumulator that counts in 2^(u - base) is worth beside a sum that counts in 2^m.
-__device__ __forceinline__ float unit_of(float u, float m, int base) { return exp2f(finite_or_zero(u) - static_cast<float>(base) - finite_or_zero(m)); }
+// Below all logits: a row's reference before the first one (infinities would not cancel).
+constexpr float kNone = -3e38f;
 
 // Four 8 x 16-byte matrices; lane l gives the address of row l % 8 of matrix l / 8.  Thread (g = lane / 4, t = lane % 4) receives bytes
 // 4 t ... 4 t + 3 of row g of each.

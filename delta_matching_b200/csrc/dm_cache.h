@@ -47,10 +47,11 @@ struct CacheAttnParams {
   float scale;                      // softmax scale
   __nv_bfloat16* o;                 // (B, Nq, H, D) contiguous
   float* lse;                       // (B, H, Nq)
-  float* part_o;                    // partial results: 2 slots a warp of (row tile, D) fp32, and of their rows (m, l, u, -): the logits' sum is l 2^m, the
-  float4* part_ml;                  // values count in 2^u (a constant of the form aside)
+  float* part_o;                    // partial results: 2 slots a warp of (row tile, D) fp32, and of their rows (m, l, v, -): the sum is l 2^m, the values
+  float4* part_ml;                  // count in 2^(m + v) (and a constant of the form)
   __half* q16;                      // many rows: the queries in f16 and the order of the row tiles, and the factors of their logits
-  float* factors;
+  float* factors;                   // (negative: a row marked for the join to make by itself)
+  int* marked;                      // whether any is
   void* starts;                     // and what each CTA begins with
   int2* unit_slots;                 // per unit (B, Hk, row tiles), where its pieces are: slot of the first (-1: whole); the last worker (for the
                                     // small form twice that, plus one where its piece lies in a slot of its own)
@@ -118,8 +119,8 @@ struct CacheAttnPlan {
   int grid;
   int cluster;                      // CTAs a unit, or 0: the even division
   int logit_rows;
-  int64_t part_o_bytes, part_ml_bytes, q16_bytes, factor_bytes, start_bytes, unit_bytes, row_ml_bytes, logit_bytes;
-  int64_t bytes() const { return part_o_bytes + part_ml_bytes + q16_bytes + factor_bytes + start_bytes + unit_bytes + row_ml_bytes + logit_bytes; }
+  int64_t part_o_bytes, part_ml_bytes, q16_bytes, mark_bytes, factor_bytes, start_bytes, unit_bytes, row_ml_bytes, logit_bytes;
+  int64_t bytes() const { return part_o_bytes + part_ml_bytes + q16_bytes + mark_bytes + factor_bytes + start_bytes + unit_bytes + row_ml_bytes + logit_bytes; }
 };
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights);
 

@@ -149,6 +149,7 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   p.logit_rows = x.logit_rows;
   p.q16 = reinterpret_cast<__half*>(take(x.q16_bytes));
   p.part_ml = reinterpret_cast<float4*>(take(x.part_ml_bytes));
+  p.marked = reinterpret_cast<int*>(take(x.mark_bytes));
   p.factors = reinterpret_cast<float*>(take(x.factor_bytes));
   p.row_ml = weights != nullptr ? reinterpret_cast<float2*>(take(x.row_ml_bytes)) : nullptr;
   p.starts = take(x.start_bytes);

@@ -30,7 +30,6 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxCluster = 8;
-constexpr float kNone = -3e38f;              // below all logits: a reference before the first one (infinities would not cancel)
 
 template <int D, int NT>
 struct AttnCfg {
@@ -40,7 +39,7 @@ struct AttnCfg {
   static constexpr int kCtasPerSm = D == 128 && NT == 1 ? 3 : 2;
   static constexpr int kSlots = D == 128 ? (NT == 2 ? 6 : 4) : 3;
   static constexpr int kRing = kWarps * kSlots * kSlotBytes;
-  static constexpr int kStats = kWarps * kRows * 16;          // m, l and u of a warp's rows, for the CTA's own join
+  static constexpr int kStats = kWarps * kRows * 16;          // m, l and v of a warp's rows, for the CTA's own join
   static constexpr int kSmem = 1024 + kRing + kStats + kWarps * kSlots * 8 + 136 * 4 + 64;
   static_assert(NT * D * 32 <= kSlots * kSlotBytes, "a warp leaves its accumulator in its ring");
 };
@@ -262,9 +261,9 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (ok) issue();
   };
   float m[NT][2], l[NT][2], acc[NT][D / 16][4];
-  // of a row, whole numbers: m, at most 1 below the largest logit, which l is the sum beside; u, at most 0.99 below the largest logit + log2 of its V
-  // scale: the accumulator counts in 2^(u - 15), so that it is left alone while u stays
-  float u[NT][2];
+  // of a row, whole numbers: m, at most 1 below the largest logit, which l is the sum beside; v, such that m + v is at most 0.99 below the largest logit
+  // + log2 of its V scale: the accumulator counts in 2^(m + v - 15).  All is reckoned by differences of logits, so that it holds for large ones too.
+  float v[NT][2];
   int slot = 2 * worker;
   // Of a finished piece: the rows' sums, complete in every lane.
   auto settle = [&]() {
@@ -287,7 +286,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (whole) {
           const RowInfo ri = row_info(p, r, hk, seg.n, count);
           const bool any = ri.limit > 0;
-          const float inv_l = any ? 1.f / l[j][e] : 0.f, inv = inv_l * unit_of(u[j][e], m[j][e], 15);
+          const float inv_l = any ? 1.f / l[j][e] : 0.f, inv = inv_l * exp2f(v[j][e] - 15.f);
           __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(seg.b) * p.Nq + ri.i) * p.H + ri.head) * D + 2 * g);
           if (kCluster) {
             o[8 * one] = any ? __floats2bfloat162_rn(acc[j][0][e] * inv, acc[j][0][2 + e] * inv) : __floats2bfloat162_rn(0.f, 0.f);
@@ -306,7 +305,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           float2* o = reinterpret_cast<float2*>(p.part_o + row * D + 2 * g);
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) o[8 * c] = make_float2(acc[j][c][e], acc[j][c][2 + e]);
-          if (g == 0) p.part_ml[row] = make_float4(m[j][e], l[j][e], u[j][e], 0.f);
+          if (g == 0) p.part_ml[row] = make_float4(m[j][e], l[j][e], v[j][e], 0.f);
         }
       }
   };
@@ -331,7 +330,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (p.causal) lim_min = seg.n - count + 1;                // of the rows that are any
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      m[j][0] = m[j][1] = u[j][0] = u[j][1] = kNone;
+      m[j][0] = m[j][1] = kNone;
+      v[j][0] = v[j][1] = 0.f;
       l[j][0] = l[j][1] = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) acc[j][c][0] = acc[j][c][1] = acc[j][c][2] = acc[j][c][3] = 0.f;
@@ -355,7 +355,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[j][mt][i] *= (i & 1) ? fs.y : fs.x;
+            s[j][mt][i] = __fmul_rn(s[j][mt][i], (i & 1) ? fs.y : fs.x);       // one value for the maximum and for p, however large
             if (cut && key0 + 16 * mt + g + 8 * (i >> 1) >= lim[j][i & 1]) s[j][mt][i] = -CUDART_INF_F;
           }
         const int logit_rows = NT == 1 ? p.logit_rows : C::kRows;
@@ -374,16 +374,17 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o));
           mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o));
         }
-        const float2 pv = make_float2(mx.x + e_blk, mx.y + e_blk);
-        if (__any_sync(0xffffffffu, mx.x > m[j][0] + 1.f || mx.y > m[j][1] + 1.f || pv.x > u[j][0] + 0.99f || pv.y > u[j][1] + 0.99f)) {
+        const float2 over = make_float2(mx.x - m[j][0], mx.y - m[j][1]);
+        if (__any_sync(0xffffffffu, over.x > 1.f || over.y > 1.f || over.x + e_blk > v[j][0] + 0.99f || over.y + e_blk > v[j][1] + 0.99f)) {
           float keep[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float m_old = m[j][e], u_old = u[j][e], mx_e = e ? mx.y : mx.x, pv_e = e ? pv.y : pv.x;
-            if (mx_e > m_old + 1.f) m[j][e] = nearest(mx_e);
-            if (pv_e > u_old + 0.99f) u[j][e] = nearest(pv_e);
-            l[j][e] *= ex2_approx(m_old - m[j][e]);
-            keep[e] = ex2_approx(u_old - u[j][e]);
+            const float mx_e = e ? mx.y : mx.x, m_new = (e ? over.y : over.x) > 1.f ? ceilf(mx_e) : m[j][e];
+            const float fall = m[j][e] - m_new, v_old = v[j][e] + fall, pv = mx_e - m_new + e_blk;
+            m[j][e] = m_new;
+            v[j][e] = pv > v_old + 0.99f ? ceilf(pv) : v_old;
+            l[j][e] *= ex2_approx(fall);
+            keep[e] = ex2_approx(v_old - v[j][e]);
           }
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
@@ -393,12 +394,12 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             acc[j][c][3] *= keep[1];
           }
         }
-        float sub[2], back[2];
+        float off[2], back[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          // p comes out as 2^(sub + s), below 2^16; where the products are 2^-60 of the largest they vanish anyway, but the sum must not
-          sub[e] = fmaxf(15.f + e_blk - u[j][e], -45.f - m[j][e]);
-          back[e] = ex2_approx(-sub[e] - m[j][e]);            // zero where p is below 2^-111 of the largest
+          // p comes out as 2^(s - m + off), below 2^16; where the products are 2^-60 of the largest they vanish anyway, but the sum must not
+          off[e] = fmaxf(15.f + e_blk - v[j][e], -45.f);
+          back[e] = ex2_approx(-off[e]);                      // zero where p is below 2^-111 of the largest
         }
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -406,7 +407,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           float e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            e[i] = ex2_approx(s[j][mt][i] + sub[i & 1]);
+            e[i] = ex2_approx(s[j][mt][i] - m[j][i & 1] + off[i & 1]);
             if (i & 1) sum.y += e[i]; else sum.x += e[i];
           }
           pb[j][mt][0] = movmatrix_trans(pack_f16x2(e[0], e[1]));
@@ -478,7 +479,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   if (kCluster && !pending) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      m[j][0] = m[j][1] = u[j][0] = u[j][1] = kNone;
+      m[j][0] = m[j][1] = kNone;
+      v[j][0] = v[j][1] = 0.f;
       l[j][0] = l[j][1] = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) acc[j][c][0] = acc[j][c][1] = acc[j][c][2] = acc[j][c][3] = 0.f;
@@ -494,8 +496,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       if (g == 0) {
-        stats[warp * C::kRows + 8 * j + 2 * t] = make_float4(m[j][0], l[j][0], u[j][0], 0.f);
-        stats[warp * C::kRows + 8 * j + 2 * t + 1] = make_float4(m[j][1], l[j][1], u[j][1], 0.f);
+        stats[warp * C::kRows + 8 * j + 2 * t] = make_float4(m[j][0], l[j][0], v[j][0], 0.f);
+        stats[warp * C::kRows + 8 * j + 2 * t + 1] = make_float4(m[j][1], l[j][1], v[j][1], 0.f);
       }
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) parked[(j * (D / 16) + c) * 32 + lane] = make_float4(acc[j][c][0], acc[j][c][1], acc[j][c][2], acc[j][c][3]);
@@ -509,12 +511,12 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float4 x = st[8 * j + 2 * t + e];
-        const float top = fmaxf(m[j][e], x.x), top_u = fmaxf(u[j][e], x.z);
-        l[j][e] = l[j][e] * ex2_approx(m[j][e] - top) + x.y * ex2_approx(x.x - top);
-        (e ? mine.y : mine.x) = ex2_approx(u[j][e] - top_u);
-        (e ? theirs.y : theirs.x) = ex2_approx(x.z - top_u);
+        const float top = fmaxf(m[j][e], x.x), fall = m[j][e] - top, their_fall = x.x - top, v_new = fmaxf(v[j][e] + fall, x.z + their_fall);
+        l[j][e] = l[j][e] * ex2_approx(fall) + x.y * ex2_approx(their_fall);
+        (e ? mine.y : mine.x) = ex2_approx(v[j][e] + fall - v_new);
+        (e ? theirs.y : theirs.x) = ex2_approx(x.z + their_fall - v_new);
         m[j][e] = top;
-        u[j][e] = top_u;
+        v[j][e] = v_new;
       }
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
@@ -544,7 +546,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       for (int j = 0; j < NT; ++j) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          st[j][e] = g < cl ? cluster.map_shared_rank(stats, g)[8 * j + 2 * t + e] : make_float4(kNone, 0.f, kNone, 0.f);
+          st[j][e] = g < cl ? cluster.map_shared_rank(stats, g)[8 * j + 2 * t + e] : make_float4(kNone, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int r = 0; r < kMaxCluster; ++r)
           if (r < cl) x[j][r] = cluster.map_shared_rank(reinterpret_cast<float4*>(smem), r)[(j * (D / 16) + c) * 32 + lane];
@@ -554,14 +556,14 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = st[j][e].x, top_u = st[j][e].z;
+          float top = st[j][e].x;
 #pragma unroll
-          for (int i = 4; i < 32; i <<= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-            top_u = fmaxf(top_u, __shfl_xor_sync(0xffffffffu, top_u, i));
-          }
-          float sum = st[j][e].y * ex2_approx(st[j][e].x - top);
-          const float w = ex2_approx(st[j][e].z - top_u);
+          for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+          const float fall = st[j][e].x - top, mine = st[j][e].z + fall;
+          float v_top = mine, sum = st[j][e].y * ex2_approx(fall);
+#pragma unroll
+          for (int i = 4; i < 32; i <<= 1) v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, i));
+          const float w = ex2_approx(mine - v_top);
 #pragma unroll
           for (int i = 4; i < 32; i <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
 #pragma unroll
@@ -573,7 +575,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           }
           m[j][e] = top;
           l[j][e] = sum;
-          u[j][e] = top_u;
+          v[j][e] = v_top;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][0][i] = o[i];
@@ -606,7 +608,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 template <int D>
 __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p, const int row_tiles, const int row_tile) {
   __shared__ float part[4][D];
-  __shared__ float factors[128], red[8];
+  __shared__ float factors[128], red[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dep_wait();
   const int R = p.Nq * p.rep;
@@ -630,24 +632,23 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
   if (slots.none()) return;                                   // whole: written by its warp (or given up)
   const int pieces = slots.count, in_tile = r - rt * row_tile;
   auto row_of = [&](int i) { return static_cast<int64_t>(slots.slot(i)) * row_tile + in_tile; };
-  float top = -CUDART_INF_F, top_u = -CUDART_INF_F;
+  // over the CTA's threads
+  auto block_max = [&](float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    __syncthreads();
+    if (lane == 0) red[warp] = x;
+    __syncthreads();
+    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  };
+  float top = kNone, v_top = kNone;
+  for (int i = tid; i < pieces; i += 128) top = fmaxf(top, p.part_ml[row_of(i)].x);
+  top = block_max(top);
   for (int i = tid; i < pieces; i += 128) {
     const float4 x = p.part_ml[row_of(i)];
-    top = fmaxf(top, x.x);
-    top_u = fmaxf(top_u, x.z);
+    v_top = fmaxf(v_top, x.x - top + x.z);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    top_u = fmaxf(top_u, __shfl_xor_sync(0xffffffffu, top_u, o));
-  }
-  if (lane == 0) {
-    red[warp] = top;
-    red[4 + warp] = top_u;
-  }
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  top_u = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+  v_top = block_max(v_top);
   float sum = 0.f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
@@ -655,8 +656,8 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
     float f = 0.f;
     if (i0 + tid < pieces) {
       const float4 x = p.part_ml[row_of(i0 + tid)];
-      f = ex2_approx(x.z - finite_or_zero(top_u));
-      sum = fmaf(x.y, ex2_approx(x.x - finite_or_zero(top)), sum);
+      f = ex2_approx(x.x - top + x.z - v_top);
+      sum = fmaf(x.y, ex2_approx(x.x - top), sum);
     }
     if (i0 > 0) __syncthreads();
     factors[tid] = f;
@@ -684,7 +685,7 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
   if (lane == 0) red[warp] = sum;
   __syncthreads();
   sum = (red[0] + red[1]) + (red[2] + red[3]);
-  const float inv_l = 1.f / sum, inv = inv_l * unit_of(top_u, top, 15);
+  const float inv_l = 1.f / sum, inv = inv_l * exp2f(v_top - 15.f);
   for (int d = tid; d < D; d += 128) o[d] = __float2bfloat16(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
   if (tid == 0) {
     *lse = (top + log2f(sum)) * kLn2;
@@ -812,7 +813,7 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
               const float fs = (e ? f[j].y : f[j].x) * ks;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float x = fmaf(s[j][i >> 1][(i & 1) * 2 + e], fs, -ml.x);
+                const float x = __fmul_rn(s[j][i >> 1][(i & 1) * 2 + e], fs) - ml.x;       // as in the main kernel
                 w[i] += key0 + g + 8 * i < limit ? ex2_approx(x) * ml.y : 0.f;
               }
             }
@@ -942,6 +943,7 @@ CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int pa
   x.part_ml_bytes = slots * x.row_tile * 16;
   const int64_t q_rows = x.chunk ? cache_chunk_query_rows(B, Hk, R) : 0;
   x.q16_bytes = q_rows * D * 2;
+  x.mark_bytes = x.chunk ? 16 : 0;
   x.factor_bytes = q_rows * 4;
   x.start_bytes = x.chunk ? x.grid * cache_chunk_start_bytes() : 0;
   x.unit_bytes = static_cast<int64_t>(B) * Hk * x.row_tiles * 8;

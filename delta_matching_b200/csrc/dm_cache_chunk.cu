@@ -36,6 +36,7 @@ namespace {
 constexpr int kChunkCost = 3;
 constexpr int kPBase = 12;                  // log2 of P at the reference,
 constexpr float kHeadroom = 3.9f;           // and what a row may exceed it by: P stays below 2^16
+constexpr float kExact = 4194304.f;         // references up to this size plus a whole number are exact sums
 
 // D = 256: as D = 128, but one row tile, whose two softmax groups take half of the keys each, and O of 256 columns.
 template <int kD>
@@ -238,6 +239,7 @@ __global__ void __launch_bounds__(256) cache_chunk_queries_kernel(const CacheAtt
   __shared__ int cum[136];
   grid_dep_wait();
   if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *p.marked = 0;
     chunk_starts(p, cum);
     return;
   }
@@ -625,10 +627,10 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const bool idle = !__any_sync(0xffffffffu, limit > 0);
         // of the row's logits, K's scale aside
         const int64_t padded_row = (static_cast<int64_t>(x.b) * p.c.Hk + x.hk) * ((p.Nq * p.rep + 127) / 128 * 128) + row;
-        const float f = __ldg(p.factors + padded_row);
-        // Of the row, whole numbers: m, the reference of the sum l; u, that of the products of a probability and its V scale: O counts in 2^(u - kPBase).
-        // The largest logit, and logit + log2 of its V scale, are at most kHeadroom above them.
-        float m = -CUDART_INF_F, u = -CUDART_INF_F, l = 0.f;
+        const float f = fabsf(__ldg(p.factors + padded_row));
+        // Of the row, whole numbers: m, the reference of the sum l; m + v, that of the products of a probability and its V scale: O counts in
+        // 2^(m + v - kPBase).  The largest logit, and logit + log2 of its V scale, are at most kHeadroom above them.
+        float m = kNone, v = 0.f, l = 0.f;
         // P V of this group's tile i is in O.  With 256 columns the softmax may be two tiles ahead of the products, so that these have two barriers.
         auto products_of = [&](int i) { return C::kWide ? wait_warp(bar(kPvDone + (i & 1)), (i >> 1) & 1, abort_flag) : wait_warp(bar(kPvDone + r), i & 1, abort_flag); };
         // What the two warps of a row's two groups know of it (256 columns): the other's value.
@@ -662,6 +664,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           };
           auto pair = [&](int c, int e) { return make_float2(__uint_as_float(s_buf[c & 1][2 * e]), __uint_as_float(s_buf[c & 1][2 * e + 1])); };
           float top = -CUDART_INF_F, top2 = -CUDART_INF_F;    // of the tile: logit, and logit + log2 of V's scale
+          auto moves_row = [&]() { return top > m + kHeadroom || top2 > m + v + kHeadroom; };
           tmem_ld32(t_s, s_buf[0]);
 #pragma unroll
           for (int c = 0; c < C::kCols / 32; ++c) {
@@ -669,13 +672,14 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             float2 s2[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) s2[e] = pair(c, e);
-            const float top_s = max32(s2), top_c = kCut && top_s == -CUDART_INF_F ? top_s : top_s * fc[c];        // the factor may be zero
+            const float top_s = max32(s2);
+            const float top_c = kCut && top_s == -CUDART_INF_F ? top_s : top_s * fc[c];        // the factor may be zero
             top = fmaxf(top, top_c);
             top2 = fmaxf(top2, top_c + ev[c]);
           }
           if (C::kWide) {
             // a common reference: seldom does a row move, so that the pair first tell each other whether any does
-            const bool moves = __any_sync(0xffffffffu, top > m + kHeadroom || top2 > u + kHeadroom);
+            const bool moves = __any_sync(0xffffffffu, moves_row());
             volatile uint8_t* votes = smem + C::kSmemBars + 8 * (kBars + 2 + (asked & 1));      // behind the TMEM slot and the abort flag
             const int vote = kVote + 2 * (warp & 3) + (asked & 1);
             if (lane == 0) {
@@ -694,32 +698,39 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             }
           }
           tmem_ld32(t_s, s_buf[0]);
-          if (__any_sync(0xffffffffu, top > m + kHeadroom || top2 > u + kHeadroom)) {
-            const float m_old = m, u_old = u;
-            if (top > m + kHeadroom) m = ceilf(top);
-            if (top2 > u + kHeadroom) u = ceilf(top2);
-            l *= ex2_approx(m_old - finite_or_zero(m));
+          if (__any_sync(0xffffffffu, moves_row())) {
+            float keep = 1.f;
+            if (moves_row()) {
+              // a row of larger logits than fp32 can add whole numbers to: marked, for the join to make it by itself
+              if (fabsf(top) > kExact) {
+                p.factors[padded_row] = -f;
+                *p.marked = 1;
+              }
+              const float m_old = m, u_old = m + v, u = top2 > u_old + kHeadroom ? ceilf(top2) : u_old;
+              if (top > m + kHeadroom) m = ceilf(top);
+              v = u - m;
+              l *= ex2_approx(m_old - m);
+              keep = ex2_approx(u_old - u);
+            }
             if (t > x.t0) {
               if (!products_of(mine - 1)) return false;
               tc_fence_after();
-              const float a = ex2_approx(u_old - finite_or_zero(u));
 #pragma unroll 1
               for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
                 tmem_ld32(t_o + 32 * c, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
                 tmem_st32(t_o + 32 * c, o);
               }
             }
           }
-          const float mu = finite_or_zero(m), uu = finite_or_zero(u);
 #pragma unroll
           for (int c = 0; c < C::kCols / 32; ++c) {
-            // P comes out as 2^(off + s), below 2^16; where the products are 2^-57 of the largest they vanish anyway, but the sum must not
-            const float off = fmaxf(kPBase + ev[c] - uu, -45.f - mu);
-            const float2 f2 = splat2(fc[c]), sub = splat2(off);
+            // P comes out as 2^(s - m + off), below 2^16; where the products are 2^-57 of the largest they vanish anyway, but the sum must not
+            const float off = fmaxf(kPBase + ev[c] - v, -45.f);
+            const float2 f2 = splat2(fc[c]), sub = splat2(off - m);
             columns(c);
             float2 sum = make_float2(0.f, 0.f);
             uint32_t h[16];
@@ -734,7 +745,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
               sum = add2(sum, y);
               h[e] = pack_f16x2(y.x, y.y);
             }
-            l = fmaf(sum.x + sum.y, ex2_approx(-off - mu), l);        // a power of two; zero where p is below 2^-111 of the largest
+            l = fmaf(sum.x + sum.y, ex2_approx(-off), l);        // a power of two; zero where p is below 2^-111 of the largest
             tmem_st16(t_s + 16 * c, h);                       // over columns that have been read: 16 c + 15 < 32 c + 32
             if (!C::kWide && c == 1) {                        // the first half of the keys: the tensor cores may begin
               tmem_wait_st();
@@ -776,7 +787,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         const bool whole = x.t0 == 0 && x.t1 == x.tiles;
-        const float scale = whole ? unit_of(u, m, kPBase) / l : 1.f;
+        const float scale = whole ? exp2f(v - kPBase) / l : 1.f;
         // where a row that sees something goes
         const int64_t out_row = limit == 0 ? -1 : ((static_cast<int64_t>(x.b) * p.Nq + i_tok) * p.H + head) * D;
         // Through shared memory, so that the lanes of a store write whole rows (a row a thread, 16 bytes at a time, took 11000 cycles a piece):
@@ -838,7 +849,7 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.Nq + i_tok] = (m + log2f(l)) * kLn2;
             if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(f, m + log2f(l));
           } else {
-            p.part_ml[part0 + lane] = make_float4(m, l, u, 0.f);
+            p.part_ml[part0 + lane] = make_float4(m, l, v, 0.f);
           }
         }
         tc_fence_before();
@@ -862,9 +873,55 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// Rows of units that were cut, and rows that see nothing: a warp a row, four of a (sequence, head) a CTA.
+// A row that the main kernel marked, by one warp and from the definition: a key after the other, all in fp32, the logits' differences exact whatever their
+// size.  `factor`: of the logits, of the query as the main kernel has it.  Writes o (this lane's four channels of each 128); -> maximum (log2 domain), sum.
 template <int D>
-__global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnParams p) {
+__device__ __forceinline__ float2 one_row(const CacheAttnParams& p, int b, int hk, int head, int i_tok, int limit, float factor, __nv_bfloat162* o) {
+  constexpr int kVecs = D / 128;
+  const int lane = threadIdx.x & 31, bpp = p.c.page / 32;
+  const __half2* q = reinterpret_cast<const __half2*>(p.q16 + ((static_cast<int64_t>(b) * p.c.Hk + hk) * ((p.Nq * p.rep + 127) / 128 * 128) +
+                                                               static_cast<int64_t>(i_tok) * p.rep + head - hk * p.rep) * D) + 2 * lane;
+  float4 qv[kVecs], acc[kVecs] = {};
+#pragma unroll
+  for (int x = 0; x < kVecs; ++x) {
+    const float2 a = __half22float2(q[64 * x]), c = __half22float2(q[64 * x + 1]);
+    qv[x] = make_float4(a.x, a.y, c.x, c.y);
+  }
+  float m = kNone, l = 0.f;
+  for (int j = 0; j < limit; ++j) {
+    const int blk = j / 32, page = max(0, checked_page(p.c, __ldg(p.c.table + b * p.c.t_row + blk / bpp))), sub = blk % bpp;
+    const int64_t code = page * p.c.c_page + hk * p.c.c_head + (sub * 32 + j % 32) * p.c.c_slot + 4 * lane, scale = page * p.c.s_page + hk * p.c.s_head + sub;
+    float s = 0.f;
+    float4 v[kVecs];
+    const float vs = __ldg(p.c.vs + scale);
+#pragma unroll
+    for (int x = 0; x < kVecs; ++x) {
+      const uint32_t k4 = __ldg(reinterpret_cast<const uint32_t*>(p.c.k8 + code + 128 * x)), v4 = __ldg(reinterpret_cast<const uint32_t*>(p.c.v8 + code + 128 * x));
+      const float2 k0 = f16x2_to_float2(e4m3_lo_f16x2(k4)), k1 = f16x2_to_float2(e4m3_hi_f16x2(k4)), v0 = f16x2_to_float2(e4m3_lo_f16x2(v4)), v1 = f16x2_to_float2(e4m3_hi_f16x2(v4));
+      s = fmaf(qv[x].x, k0.x, fmaf(qv[x].y, k0.y, fmaf(qv[x].z, k1.x, fmaf(qv[x].w, k1.y, s))));
+      v[x] = make_float4(v0.x * vs, v0.y * vs, v1.x * vs, v1.y * vs);
+    }
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
+    s = __fmul_rn(s, __fmul_rn(factor, __ldg(p.c.ks + scale)));
+    const float m_new = fmaxf(m, s), keep = exp2f(m - m_new), w = exp2f(s - m_new);
+    m = m_new;
+    l = fmaf(l, keep, w);
+#pragma unroll
+    for (int x = 0; x < kVecs; ++x)
+      acc[x] = make_float4(fmaf(acc[x].x, keep, w * v[x].x), fmaf(acc[x].y, keep, w * v[x].y), fmaf(acc[x].z, keep, w * v[x].z), fmaf(acc[x].w, keep, w * v[x].w));
+  }
+#pragma unroll
+  for (int x = 0; x < kVecs; ++x) {
+    o[64 * x] = __floats2bfloat162_rn(acc[x].x / l, acc[x].y / l);
+    o[64 * x + 1] = __floats2bfloat162_rn(acc[x].z / l, acc[x].w / l);
+  }
+  return make_float2(m, l);
+}
+
+// Rows of units that were cut, rows that see nothing, marked rows: a warp a row, four of a (sequence, head) a CTA.
+template <int D>
+__global__ void __launch_bounds__(128, D == 128 ? 12 : 10) cache_chunk_join_kernel(const CacheAttnParams p) {
   constexpr int kRows = ChunkCfg<D>::kRows, kVecs = D / 128;
   grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -872,6 +929,7 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
   const int r = static_cast<int>(blockIdx.x % groups) * 4 + warp, bh = static_cast<int>(blockIdx.x / groups), hk = bh % p.c.Hk, b = bh / p.c.Hk;
   if (r >= R) return;
   const int2 unit = p.unit_slots[static_cast<int64_t>(bh) * unit_tiles_max + r / kRows];
+  const int marked = *p.marked;                           // any row of the call
   const ChunkSeq s = chunk_seq(p, b);
   const int i_tok = r / p.rep, head = hk * p.rep + r - i_tok * p.rep;
   __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(b) * p.Nq + i_tok) * p.H + head) * D) + 2 * lane;
@@ -883,34 +941,43 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
     if (lane == 0) *lse = -CUDART_INF_F;
     return;
   }
+  if (marked != 0 && p.factors[padded_row] < 0.f) {
+    const float factor = p.factors[padded_row];
+    const float2 ml = one_row<D>(p, b, hk, head, i_tok, row_limit(p, s, r), -factor, o);
+    if (lane == 0) {
+      *lse = (ml.x + log2f(ml.y)) * kLn2;
+      if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(-factor, ml.x + log2f(ml.y));
+    }
+    return;
+  }
   const JoinSlots slots = join_slots_of_ctas(unit, p.grid);
   if (slots.none()) return;                               // whole: written by its CTA (or given up)
-  float top = -CUDART_INF_F, top_u = -CUDART_INF_F, sum = 0.f;
+  float top = kNone, v_top = 0.f, sum = 0.f;
   float4 acc[kVecs] = {};
   const int n = slots.count;
   // 32 results at a time, a lane each: their maxima and sums together, then the values of those that count
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int i = i0 + lane, at = slots.slot(i) * kRows + (r & (kRows - 1));
-    const float4 ml = i < n ? p.part_ml[at] : make_float4(-CUDART_INF_F, 0.f, -CUDART_INF_F, 0.f);     // -inf: a piece of which the row sees nothing
-    float top_new = ml.x, u_new = ml.z;
+    const float4 ml = i < n ? p.part_ml[at] : make_float4(kNone, 0.f, 0.f, 0.f);       // kNone: a piece of which the row sees nothing
+    float top_new = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, o));
+    top_new = fmaxf(top, top_new);
+    const float fall = ml.x - top_new, old = v_top + (top - top_new);
+    float l = ml.y * ex2_approx(fall);
+    v_top = ml.z + fall;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, o));
-      u_new = fmaxf(u_new, __shfl_xor_sync(0xffffffffu, u_new, o));
+      l += __shfl_xor_sync(0xffffffffu, l, o);
+      v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, o));
     }
-    top_new = fmaxf(top, top_new);
-    u_new = fmaxf(top_u, u_new);
-    if (top_new == -CUDART_INF_F) continue;
-    const float a = ex2_approx(top_u - u_new), w = ex2_approx(ml.z - u_new);
-    float l = ml.y * ex2_approx(ml.x - top_new);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    v_top = fmaxf(v_top, old);
+    const float a = ex2_approx(old - v_top), w = ex2_approx(ml.z + fall - v_top);
     sum = sum * ex2_approx(top - top_new) + l;
     top = top_new;
-    top_u = u_new;
 #pragma unroll
     for (int x = 0; x < kVecs; ++x) acc[x] = make_float4(acc[x].x * a, acc[x].y * a, acc[x].z * a, acc[x].w * a);
-    const uint32_t counts = __ballot_sync(0xffffffffu, ml.x > -CUDART_INF_F);
+    const uint32_t counts = __ballot_sync(0xffffffffu, ml.x > kNone);
 #pragma unroll 8
     for (int k = 0; k < min(32, n - i0); ++k) {
       const float w_k = __shfl_sync(0xffffffffu, w, k);
@@ -923,7 +990,7 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
       }
     }
   }
-  const float inv = unit_of(top_u, top, kPBase) / sum;
+  const float inv = exp2f(v_top - kPBase) / sum;
 #pragma unroll
   for (int x = 0; x < kVecs; ++x) {
     o[64 * x] = __floats2bfloat162_rn(acc[x].x * inv, acc[x].y * inv);
@@ -931,7 +998,7 @@ __global__ void __launch_bounds__(128) cache_chunk_join_kernel(const CacheAttnPa
   }
   if (lane == 0) {
     *lse = (top + log2f(sum)) * kLn2;
-    if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(p.factors[padded_row], top + log2f(sum));
+    if (p.row_ml != nullptr) p.row_ml[padded_row] = make_float2(fabsf(p.factors[padded_row]), top + log2f(sum));
   }
 }
 
@@ -1237,7 +1304,9 @@ cache_chunk_weights_kernel(const __grid_constant__ CUtensorMap tk, const __grid_
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = add2(sum, z[e]);
           }
-          total += sum.x + sum.y;
+          // (no sum of probabilities is above their number; logits so large that their last bit counts powers of two would make it one)
+          const float both = sum.x + sum.y;
+          total += both > 32.f ? 32.f : both;
         };
         auto parts_from = [&](int c, int step, auto cut_tag) {
           if (c < parts) tmem_ld32(from + 32 * c, s_buf[0]);
