@@ -67,6 +67,9 @@ __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
 // Below all logits: a row's reference before the first one (infinities would not cancel).
 constexpr float kNone = -3e38f;
 
+// 0xFF in the bytes of four e4m3 codes that are NaN.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
+
 // Four 8 x 16-byte matrices; lane l gives the address of row l % 8 of matrix l / 8.  Thread (g = lane / 4, t = lane % 4) receives bytes
 // 4 t ... 4 t + 3 of row g of each.
 __device__ __forceinline__ void ldmatrix4(uint32_t saddr, uint32_t (&r)[4]) {

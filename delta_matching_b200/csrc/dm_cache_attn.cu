@@ -429,6 +429,57 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           sel[i] = k + 1 < seg.n ? 0x3120u : k < seg.n ? 0x4140u : 0x4444u;
         }
       }
+      // A NaN code belongs to the rows that see its token; the others would multiply it by zero.  Where some row does not see all that is held: which rows see
+      // one, by products of ones (token seen) and ones (code NaN), and zeros in its place.
+      if (key0 + 32 > lim_min && lim_min < seg.n) {
+        const uint32_t slot = vbase + lane * 128;             // a lane a token
+        uint32_t found = 0;
+#pragma unroll 1
+        for (int x = 0; x < D / 16; ++x) {
+          const float4 w = lds_f4(slot + (x >> 3) * 4096 + (x & 7) * 16);
+          found |= nan_codes(__float_as_uint(w.x)) | nan_codes(__float_as_uint(w.y)) | nan_codes(__float_as_uint(w.z)) | nan_codes(__float_as_uint(w.w));
+        }
+        if (__any_sync(0xffffffffu, found != 0 && key0 + lane < seg.n)) {
+          uint32_t sees[NT][2][2];
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = key0 + 8 * i + g;
+              sees[j][i >> 1][i & 1] = movmatrix_trans(pack_f16x2(k < lim[j][0] ? 1.f : 0.f, k < lim[j][1] ? 1.f : 0.f));
+            }
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t r[4], lo[4], hi[4];
+            ldmatrix4_trans(vbase + (c >> 3) * 4096 + lane * 128 + (((c & 7) ^ (lane & 7)) << 4), r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              r[i] = nan_codes(prmt(r[i], 0u, sel[i])) & 0x38383838u;         // one
+              lo[i] = e4m3_lo_f16x2(r[i]);
+              hi[i] = e4m3_hi_f16x2(r[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              float seen[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_f16(seen, lo[0], hi[0], lo[1], hi[1], sees[j][0][0], sees[j][0][1]);
+              mma_f16(seen, lo[2], hi[2], lo[3], hi[3], sees[j][1][0], sees[j][1][1]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (seen[i] > 0.f) acc[j][c][i] = CUDART_NAN_F;
+            }
+          }
+          __syncwarp();
+#pragma unroll 1
+          for (int x = 0; x < D / 16; ++x) {
+            const uint32_t at = slot + (x >> 3) * 4096 + (x & 7) * 16;
+            const float4 f4 = lds_f4(at);
+            const uint32_t w[4] = {__float_as_uint(f4.x), __float_as_uint(f4.y), __float_as_uint(f4.z), __float_as_uint(f4.w)};
+            sts_u4(at, w[0] & ~nan_codes(w[0]), w[1] & ~nan_codes(w[1]), w[2] & ~nan_codes(w[2]), w[3] & ~nan_codes(w[3]));
+          }
+          fence_async_smem();                                 // before the next box comes here
+          __syncwarp();
+        }
+      }
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
         uint32_t r[4], lo[4], hi[4];

@@ -794,11 +794,14 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         // 32 rows x 128 bytes at a time, 16-byte pieces XORed with the row.
         const int64_t part0 = static_cast<int64_t>(slot) * C::kRows + (C::kWide ? 0 : r * 128) + (warp & 3) * 32;
         const int col0 = C::kWide ? 128 * r : 0;
+        float any_nan = 0.f;                                  // NaN where a value is
 #pragma unroll 1
         for (int c = idle ? 4 : 0; c < 4; ++c) {
           uint32_t o[32];
           tmem_ld32(t_o + 32 * c, o);
           tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) any_nan += __uint_as_float(o[e]);
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -837,6 +840,11 @@ cache_chunk_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             for (int i = 0; i < 8; ++i) to[4 * i * (D / 4)] = v[i];
           }
           __syncwarp();
+        }
+        // A NaN may be that of a value whose token this row does not see, times zero: the row is marked too.
+        if (p.causal && limit > 0 && any_nan != any_nan) {
+          p.factors[padded_row] = -f;
+          *p.marked = 1;
         }
         // where the join finds the unit: the slot of its first piece, and the last CTA that has one (the pieces between are first ones)
         if (r == 0 && in_tile == 0) {
