@@ -771,10 +771,12 @@ __global__ void __launch_bounds__(256) cache_weights_of_logits_kernel(const Cach
   for (int r = 0; r < 16; r += 4) {
     if (r >= R) break;
     const float4 y = r == 0 ? first : x[r / 4];
-    w += ex2_approx(y.x - ml[r].x) * ml[r].y;
-    if (r + 1 < R) w += ex2_approx(y.y - ml[r + 1].x) * ml[r + 1].y;
-    if (r + 2 < R) w += ex2_approx(y.z - ml[r + 2].x) * ml[r + 2].y;
-    if (r + 3 < R) w += ex2_approx(y.w - ml[r + 3].x) * ml[r + 3].y;
+    // of a row that sees anything (1 / sum is not zero): those of others are logits of zeros, NaN where K is
+    const auto p_of = [&](float s, float2 row) { return row.y != 0.f ? ex2_approx(s - row.x) * row.y : 0.f; };
+    w += p_of(y.x, ml[r]);
+    if (r + 1 < R) w += p_of(y.y, ml[r + 1]);
+    if (r + 2 < R) w += p_of(y.z, ml[r + 2]);
+    if (r + 3 < R) w += p_of(y.w, ml[r + 3]);
   }
   *at = p.accumulate ? *at + w : w;
 }
