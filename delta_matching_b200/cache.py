@@ -230,8 +230,8 @@ def attn_now(q, cache, block_table, lengths, q_counts, causal, softmax_scale, we
     lengths = _check_lengths("lengths", lengths, B, dev)
     q_counts = None if q_counts is None else _check_lengths("q_counts", q_counts, B, dev)
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"delta_matching: softmax_scale must be positive (got {softmax_scale!r})")
+    if not 0.0 < ctypes.c_float(scale).value < float("inf"):
+        raise ValueError(f"delta_matching: softmax_scale must be positive and finite in 32 bits (got {softmax_scale!r})")
     if weights is not None:
         _check_weights(weights, B, Hk, T * P, dev)
     elif accumulate:
@@ -252,6 +252,8 @@ def attn_now(q, cache, block_table, lengths, q_counts, causal, softmax_scale, we
             *w, int(bool(accumulate)), ws.data_ptr(), bytes_, ops.status_word(dev).data_ptr(), ops._stream(q)))
         ops._after(dev)
     return (o, lse) if return_lse else o
+        if _overlaps(weights):
+            raise ValueError("delta_matching: weights share memory (an expanded tensor?): they cannot be written")
 
 
 def dm_cache_evict(cache, block_table, lengths, weights, new_block_table, budget, recent=0):

@@ -1,4 +1,6 @@
 // C-ABI layer of the 8-bit key / value cache: argument validation, tensor maps of the pools, launches (see dm_abi.cu for the conventions).
+#include <cfloat>
+
 #include "dm_abi_util.h"
 #include "dm_cache.h"
 
@@ -120,7 +122,7 @@ int dm_cache_attn(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t
   DM_TRY(check_attn_shape(B, Nq, H, cache->heads, cache->head_dim, T, cache->page_size));
   DM_TRY(check_rows("q", q, q_sb, q_sn, q_sh));
   DM_TRY(check_addresses({{o, "o"}, {lse, "lse"}, {workspace, "workspace"}}));
-  if (!(softmax_scale > 0.f)) return fail(DM_ERR_ARG, "delta_matching: softmax_scale must be positive (got %g)", softmax_scale);
+  if (!(softmax_scale > 0.f && softmax_scale <= FLT_MAX)) return fail(DM_ERR_ARG, "delta_matching: softmax_scale must be positive and finite in 32 bits (got %g)", softmax_scale);
   if (weights != nullptr && W < T * cache->page_size)
     return fail(DM_ERR_ARG, "delta_matching: weights must have room for the %d tokens of a row of the block table (got %d)", T * cache->page_size, W);
   const dm::CacheAttnPlan x = dm::plan_cache_attn(B, Nq, H, cache->heads, cache->head_dim, T, cache->page_size, weights != nullptr);

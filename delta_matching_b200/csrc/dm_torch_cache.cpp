@@ -169,7 +169,7 @@ PyObject* cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (args[6] != Py_None) {
     scale = PyFloat_AsDouble(args[6]);
     if (scale == -1.0 && PyErr_Occurred()) PyErr_Clear();
-    if (!(scale > 0.0 && std::isfinite(scale))) Py_RETURN_NONE;
+    if (!(static_cast<float>(scale) > 0.f && std::isfinite(static_cast<float>(scale)))) Py_RETURN_NONE;
   }
   const Tensor* w = nullptr;
   if (args[7] == Py_None ? accumulate != 0 : !read_weights(args[7], cache, B, table.room(cache), w)) Py_RETURN_NONE;

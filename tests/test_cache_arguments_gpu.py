@@ -1,0 +1,32 @@
+"""Arguments of the cache functions at the edges: what cannot be served raises, on either route; shared block tables are served."""
+import pytest
+import torch
+
+import delta_matching_b200 as dm
+from delta_matching_b200 import _lib, ops
+
+from .test_cache_gpu import _filled, _ints
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.fixture(params=["native", "python"])
+def route(request, monkeypatch):
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "native_cache", lambda: _lib._NoCacheRoute)
+
+
+def _call(B=2, lengths=(40, 33)):
+    cache, _, table = _filled(list(lengths), 32, 2, 128, T=4)
+    q, k = torch.randn(B, 1, 4, 128, device="cuda", dtype=BF), torch.randn(B, 1, 2, 128, device="cuda", dtype=BF)
+    return cache, table.cuda(), _ints(list(lengths)).cuda(), q, k
+
+
+@pytest.mark.parametrize("scale", [1e39, 1e-50, float("inf"), float("nan"), 0.0, -0.1])
+def test_softmax_scale_in_32_bits(route, scale):
+    cache, t, n, q, _ = _call()
+    with pytest.raises(ValueError, match="softmax_scale"):
+        dm.dm_cache_attn(q, cache, t, n, softmax_scale=scale)
+    dm.dm_cache_attn(q, cache, t, n, softmax_scale=1e-30)
+    ops.check_status("cuda")
