@@ -72,6 +72,22 @@ class KVCache8(NamedTuple):
 
 
 def _check_cache(cache):
+def _overlaps(t):
+    """Whether two elements of t may share an address: a dimension's stride is below what the dimensions of smaller strides span."""
+    reach = 1
+    for stride, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1:
+            if stride < reach:
+                return True
+            reach += (n - 1) * stride
+    return False
+
+
+def _check_written(cache):
+    if _overlaps(cache.k8) or _overlaps(cache.ks):
+        raise ValueError("delta_matching: slots or scales of the cache share memory (an expanded tensor?): they cannot be written")
+
+
     if not isinstance(cache, KVCache8) or not all(isinstance(t, torch.Tensor) for t in cache):
         raise TypeError("delta_matching: cache must be a KVCache8 of torch tensors")
     k8, v8, ks, vs = cache
@@ -175,6 +191,7 @@ def append_now(cache, k, v, block_table, lengths, counts):
         return new
     pages, Hk, P, D = _check_cache(cache)
     _refuse_tangents(k=k, v=v, ks=cache.ks, vs=cache.vs)
+    _check_written(cache)
     dev = cache.k8.device
     k, v = _check_rows("k", k, Hk, D, dev), _check_rows("v", v, Hk, D, dev)
     if k.shape != v.shape:
@@ -276,6 +293,7 @@ def evict_now(cache, block_table, lengths, weights, new_block_table, budget, rec
         return out
     pages, Hk, P, D = _check_cache(cache)
     _refuse_tangents(ks=cache.ks, vs=cache.vs, weights=weights)
+    _check_written(cache)
     dev = cache.k8.device
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1 or lengths.numel() == 0:
         raise ValueError("delta_matching: lengths must be a 1-D tensor, one entry per sequence")

@@ -29,6 +29,22 @@ struct Lib {
 
 constexpr int64_t kBlk = 32;
 
+// Whether two elements of `t` may share an address: a dimension's stride is below what the dimensions of smaller strides span.
+bool overlaps(const Tensor& t) {
+  int64_t reach = 1;                                          // elements that the dimensions looked at so far span
+  bool done[4] = {};
+  for (int64_t k = 0; k < t.dim(); ++k) {
+    int64_t least = -1;
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (!done[d] && (least < 0 || t.stride(d) < t.stride(least))) least = d;
+    done[least] = true;
+    if (t.size(least) == 1) continue;
+    if (t.stride(least) < reach) return true;
+    reach += (t.size(least) - 1) * t.stride(least);
+  }
+  return false;
+}
+
 bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
 
 // The pools of a KVCache8 (a tuple of four), as cache.py's _check_cache takes them.
@@ -36,6 +52,7 @@ struct Cache {
   const Tensor *k8, *v8, *ks, *vs;
   dm_kv_cache c;
   at::Device dev{at::kCUDA};
+  bool written_apart() const { return !overlaps(*k8) && !overlaps(*ks); }        // V's strides are K's
   bool read(PyObject* o) {
     if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
     const Tensor** t[4] = {&k8, &v8, &ks, &vs};
@@ -130,7 +147,7 @@ PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Cache cache;
   const Tensor *kp, *vp;
-  if (n != 6 || elsewhere() || !cache.read(args[0]) || !read_rows(args[1], cache, cache.c.heads, kp) || !read_rows(args[2], cache, cache.c.heads, vp) ||
+  if (n != 6 || elsewhere() || !cache.read(args[0]) || !cache.written_apart() || !read_rows(args[1], cache, cache.c.heads, kp) || !read_rows(args[2], cache, cache.c.heads, vp) ||
       kp->sizes() != vp->sizes() || !sm100(cache.dev))
     Py_RETURN_NONE;
   const int64_t B = kp->size(0), N = kp->size(1);
@@ -172,7 +189,7 @@ PyObject* cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!(static_cast<float>(scale) > 0.f && std::isfinite(static_cast<float>(scale)))) Py_RETURN_NONE;
   }
   const Tensor* w = nullptr;
-  if (args[7] == Py_None ? accumulate != 0 : !read_weights(args[7], cache, B, table.room(cache), w)) Py_RETURN_NONE;
+  if (args[7] == Py_None ? accumulate != 0 : !(read_weights(args[7], cache, B, table.room(cache), w) && !overlaps(*w))) Py_RETURN_NONE;
   const int64_t ws_bytes = g_lib.attn_workspace_bytes(static_cast<int>(B), static_cast<int>(N), static_cast<int>(H), cache.c.heads, cache.c.head_dim, table.T,
                                                       cache.c.page_size, w != nullptr);
   if (ws_bytes <= 0) Py_RETURN_NONE;
@@ -208,7 +225,7 @@ PyObject* cache_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Cache cache;
   const Tensor* len;
-  if (n != 7 || elsewhere() || !cache.read(args[0]) || !sm100(cache.dev) || !plain_cuda(args[2], len) || len->dim() != 1 || len->size(0) <= 0) Py_RETURN_NONE;
+  if (n != 7 || elsewhere() || !cache.read(args[0]) || !cache.written_apart() || !sm100(cache.dev) || !plain_cuda(args[2], len) || len->dim() != 1 || len->size(0) <= 0) Py_RETURN_NONE;
   const int64_t B = len->size(0);
   Table table, to;
   const int* lengths;

@@ -30,3 +30,22 @@ def test_softmax_scale_in_32_bits(route, scale):
         dm.dm_cache_attn(q, cache, t, n, softmax_scale=scale)
     dm.dm_cache_attn(q, cache, t, n, softmax_scale=1e-30)
     ops.check_status("cuda")
+
+
+def test_outputs_that_share_memory_are_refused(route):
+    cache, t, n, q, k = _call()
+    for w in (torch.zeros(1, 2, 128, device="cuda").expand(2, -1, -1), torch.zeros(2, 1, 128, device="cuda").expand(-1, 2, -1),
+              torch.as_strided(torch.zeros(1000, device="cuda"), (2, 2, 128), (200, 100, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            dm.dm_cache_attn(q, cache, t, n, weights=w)
+    # heads outside sequences, and gaps, are no sharing
+    w = torch.zeros(2, 2, 130, device="cuda").transpose(0, 1)[:, :, :128]
+    dm.dm_cache_attn(q, cache, t, n, weights=w)
+    one = torch.ones(cache.ks.shape[0], 1, 1, device="cuda").expand(-1, 2, -1)
+    shared = dm.KVCache8(cache.k8, cache.v8, one, one)
+    dm.dm_cache_attn(q, shared, t, n)                            # to be read, scales may be shared
+    with pytest.raises(ValueError, match="share memory"):
+        dm.dm_cache_append(shared, k, k, t, n)
+    with pytest.raises(ValueError, match="share memory"):
+        dm.dm_cache_evict(shared, t, n, torch.zeros(2, 2, 128, device="cuda"), t, 32)
+    ops.check_status("cuda")
