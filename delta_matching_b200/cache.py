@@ -21,6 +21,7 @@ NotImplementedError.  Under torch.compile, torch.jit.trace and dispatch modes th
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import NamedTuple
 
 import torch
@@ -303,7 +304,7 @@ def evict_now(cache, block_table, lengths, weights, new_block_table, budget, rec
     new_table, new_row = _check_table("new_block_table", new_block_table, B, dev)
     T, T2 = table.shape[1], new_table.shape[1]
     _check_weights(weights, B, Hk, T * P, dev)
-    budget, recent = int(budget), int(recent)
+    budget, recent = operator.index(budget), operator.index(recent)
     if not 0 < budget <= T2 * P:
         raise ValueError(f"delta_matching: budget must be between 1 and the {T2 * P} tokens of a row of new_block_table (got {budget})")
     if not 0 <= recent <= budget:

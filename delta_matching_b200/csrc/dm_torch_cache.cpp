@@ -54,7 +54,7 @@ struct Cache {
   at::Device dev{at::kCUDA};
   bool written_apart() const { return !overlaps(*k8) && !overlaps(*ks); }        // V's strides are K's
   bool read(PyObject* o) {
-    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+    if (!PyTuple_Check(o) || PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 4) return false;     // a KVCache8, no plain tuple
     const Tensor** t[4] = {&k8, &v8, &ks, &vs};
     for (int i = 0; i < 4; ++i)
       if (!plain_cuda(PyTuple_GET_ITEM(o, i), *t[i])) return false;

@@ -49,3 +49,15 @@ def test_outputs_that_share_memory_are_refused(route):
     with pytest.raises(ValueError, match="share memory"):
         dm.dm_cache_evict(shared, t, n, torch.zeros(2, 2, 128, device="cuda"), t, 32)
     ops.check_status("cuda")
+
+
+def test_types(route):
+    cache, t, n, q, k = _call()
+    w = torch.zeros(2, 2, 128, device="cuda")
+    for bad in (dict(budget=32.0), dict(budget=32.7), dict(budget=32, recent=1.5), dict(budget="32")):
+        with pytest.raises(TypeError):
+            dm.dm_cache_evict(cache, t[:, :2], n, w, t[:, 2:], **bad)
+    for call in (lambda c: dm.dm_cache_append(c, k, k, t, n), lambda c: dm.dm_cache_attn(q, c, t, n), lambda c: dm.dm_cache_evict(c, t[:, :2], n, w, t[:, 2:], 8)):
+        with pytest.raises(TypeError, match="KVCache8"):
+            call(tuple(cache))
+    ops.check_status("cuda")
