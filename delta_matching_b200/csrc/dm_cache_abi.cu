@@ -25,7 +25,7 @@ int check_table(const dm_kv_cache* c, const int* table, int64_t row, int T, cons
   if (table == nullptr) return fail(DM_ERR_ARG, "delta_matching: %s is NULL (every tensor must be a CUDA buffer)", name);
   if (lengths == nullptr) return fail(DM_ERR_ARG, "delta_matching: lengths is NULL (every tensor must be a CUDA buffer)");
   if (B <= 0 || T <= 0) return fail(DM_ERR_ARG, "delta_matching: empty %s (%d sequences, %d pages each)", name, B, T);
-  if (row < T) return fail(DM_ERR_ARG, "delta_matching: rows of %s overlap (%lld apart, %d long)", name, static_cast<long long>(row), T);
+  if (row < 0) return fail(DM_ERR_ARG, "delta_matching: rows of %s are %lld apart", name, static_cast<long long>(row));
   if (static_cast<int64_t>(B) * c->heads > 65535) return fail(DM_ERR_ARG, "delta_matching: batch * nheads_k must be at most 65535");
   if (static_cast<int64_t>(T) * c->page_size > (1ll << 30))
     return fail(DM_ERR_ARG, "delta_matching: a sequence has room for at most 2^30 tokens (got %d pages of %d)", T, c->page_size);

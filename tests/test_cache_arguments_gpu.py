@@ -61,3 +61,14 @@ def test_types(route):
         with pytest.raises(TypeError, match="KVCache8"):
             call(tuple(cache))
     ops.check_status("cuda")
+
+
+@pytest.mark.parametrize("N", [1, 12])
+def test_sequences_that_share_a_row_of_the_table(route, N):
+    """Several sequences read one prefix, before any of them goes on: an expanded block table."""
+    cache, t, n, _, _ = _call()
+    q = torch.randn(3, N, 8, 128, device="cuda", dtype=BF)
+    one, n3 = t[:1].expand(3, -1), n[:1].expand(3)
+    o = dm.dm_cache_attn(q, cache, one, n3)
+    ops.check_status("cuda")
+    assert torch.equal(o, dm.dm_cache_attn(q, cache, one.contiguous(), n3.contiguous()))
