@@ -76,7 +76,7 @@ int dm_cache_append(const dm_kv_cache* cache, const void* k, int64_t k_sb, int64
   DM_TRY(check_rows("k", k, k_sb, k_sn, k_sh));
   DM_TRY(check_rows("v", v, v_sb, v_sn, v_sh));
   if (new_lengths == nullptr) return fail(DM_ERR_ARG, "delta_matching: new lengths is NULL (every tensor must be a CUDA buffer)");
-  if ((static_cast<int64_t>(N) + 30) / 32 + 1 > (1ll << 33) / (static_cast<int64_t>(B) * cache->heads * 2))
+  if ((static_cast<int64_t>(N) + 30) / 32 + 1 > (1ll << 32) / (static_cast<int64_t>(B) * cache->heads * 2))
     return fail(DM_ERR_ARG, "delta_matching: too many tokens in one call (%d x %d)", B, N);
   DM_TRY(check_sm100());
   dm::CacheAppendParams p{};

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(128) cache_append_kernel(const CacheAppendPara
 
 cudaError_t launch_cache_append(int D, const CacheAppendParams& p, cudaStream_t stream) {
   // blocks that N tokens can touch behind any start
-  const int blocks = (p.N + 30) / 32 + 1;
+  const int blocks = static_cast<int>((static_cast<int64_t>(p.N) + 30) / 32 + 1);
   const int64_t items = static_cast<int64_t>(p.c.B) * blocks * p.c.Hk * 2;
   const dim3 grid(static_cast<unsigned>((items + 3) / 4));
   count_launch();

@@ -10,3 +10,9 @@ from .test_cache_cpu import _append, _attn, _c
 def test_softmax_scale_is_finite(scale):
     assert _attn(_c(), scale=scale) == -1
     assert "softmax_scale" in _lib.last_error()
+
+
+def test_append_refuses_what_no_grid_holds():
+    # 2^31 - 1 tokens are 2^26 + 1 blocks, of 16 sequences, 2 heads, K and V: above 2^32 items in CTAs of four
+    assert _append(_c(), N=(1 << 31) - 1, B=16) == -1
+    assert "too many tokens" in _lib.last_error()
