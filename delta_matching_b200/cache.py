@@ -72,7 +72,6 @@ class KVCache8(NamedTuple):
         return cls(code(), code(), scale(), scale())
 
 
-def _check_cache(cache):
 def _overlaps(t):
     """Whether two elements of t may share an address: a dimension's stride is below what the dimensions of smaller strides span."""
     reach = 1
@@ -89,6 +88,7 @@ def _check_written(cache):
         raise ValueError("delta_matching: slots or scales of the cache share memory (an expanded tensor?): they cannot be written")
 
 
+def _check_cache(cache):
     if not isinstance(cache, KVCache8) or not all(isinstance(t, torch.Tensor) for t in cache):
         raise TypeError("delta_matching: cache must be a KVCache8 of torch tensors")
     k8, v8, ks, vs = cache
@@ -191,8 +191,8 @@ def append_now(cache, k, v, block_table, lengths, counts):
     if new is not None:
         return new
     pages, Hk, P, D = _check_cache(cache)
-    _refuse_tangents(k=k, v=v, ks=cache.ks, vs=cache.vs)
     _check_written(cache)
+    _refuse_tangents(k=k, v=v, ks=cache.ks, vs=cache.vs)
     dev = cache.k8.device
     k, v = _check_rows("k", k, Hk, D, dev), _check_rows("v", v, Hk, D, dev)
     if k.shape != v.shape:
@@ -252,6 +252,8 @@ def attn_now(q, cache, block_table, lengths, q_counts, causal, softmax_scale, we
         raise ValueError(f"delta_matching: softmax_scale must be positive and finite in 32 bits (got {softmax_scale!r})")
     if weights is not None:
         _check_weights(weights, B, Hk, T * P, dev)
+        if _overlaps(weights):
+            raise ValueError("delta_matching: weights share memory (an expanded tensor?): they cannot be written")
     elif accumulate:
         raise ValueError("delta_matching: accumulate=True needs weights")
     ops._enter(dev)
@@ -270,8 +272,6 @@ def attn_now(q, cache, block_table, lengths, q_counts, causal, softmax_scale, we
             *w, int(bool(accumulate)), ws.data_ptr(), bytes_, ops.status_word(dev).data_ptr(), ops._stream(q)))
         ops._after(dev)
     return (o, lse) if return_lse else o
-        if _overlaps(weights):
-            raise ValueError("delta_matching: weights share memory (an expanded tensor?): they cannot be written")
 
 
 def dm_cache_evict(cache, block_table, lengths, weights, new_block_table, budget, recent=0):
@@ -293,8 +293,8 @@ def evict_now(cache, block_table, lengths, weights, new_block_table, budget, rec
     if out is not None:
         return out
     pages, Hk, P, D = _check_cache(cache)
-    _refuse_tangents(ks=cache.ks, vs=cache.vs, weights=weights)
     _check_written(cache)
+    _refuse_tangents(ks=cache.ks, vs=cache.vs, weights=weights)
     dev = cache.k8.device
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1 or lengths.numel() == 0:
         raise ValueError("delta_matching: lengths must be a 1-D tensor, one entry per sequence")
