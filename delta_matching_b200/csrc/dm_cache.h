@@ -122,6 +122,7 @@ struct CacheAttnPlan {
   int64_t part_o_bytes, part_ml_bytes, q16_bytes, mark_bytes, factor_bytes, start_bytes, unit_bytes, row_ml_bytes, logit_bytes;
   int64_t bytes() const { return part_o_bytes + part_ml_bytes + q16_bytes + mark_bytes + factor_bytes + start_bytes + unit_bytes + row_ml_bytes + logit_bytes; }
 };
+int cache_chunk_from(int D);         // rows of a head from which the form for many rows is taken
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights);
 
 cudaError_t launch_cache_append(int D, const CacheAppendParams& p, cudaStream_t stream);

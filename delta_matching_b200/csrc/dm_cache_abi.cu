@@ -100,8 +100,9 @@ static int check_attn_shape(int B, int Nq, int H, int Hk, int D, int T, int page
   if (static_cast<int64_t>(B) * H > 65535) return fail(DM_ERR_ARG, "delta_matching: batch * nheads must be at most 65535");
   if (Nq > (1 << 20) || static_cast<int64_t>(B) * H * Nq > (1ll << 30))
     return fail(DM_ERR_ARG, "delta_matching: too many query rows (%d sequences, %d heads, %d tokens)", B, H, Nq);
-  const int64_t row_tiles = (static_cast<int64_t>(Nq) * (H / Hk) + 7) / 8;
-  if (static_cast<int64_t>(T) * page / 32 + 4 > (1ll << 30) / (static_cast<int64_t>(B) * Hk * row_tiles))
+  // Steps of the division of the work are ints: of 8 rows x 32 tokens at least, for many rows of 128 x 128.
+  const int64_t rows = static_cast<int64_t>(Nq) * (H / Hk), row_tiles = (rows + 7) / 8, most = rows >= dm::cache_chunk_from(D) ? 1ll << 34 : 1ll << 30;
+  if (static_cast<int64_t>(T) * page / 32 + 4 > most / (static_cast<int64_t>(B) * Hk * row_tiles))
     return fail(DM_ERR_ARG, "delta_matching: too much work for one call (%d sequences with room for %lld tokens, %lld rows)", B,
                 static_cast<long long>(T) * page, static_cast<long long>(Nq) * H);
   return 0;

@@ -957,10 +957,6 @@ cudaError_t launch_weights(const CUtensorMap& tk, const CacheAttnParams& p, cuda
                         (p.Nq * p.rep + 8 * NT - 1) / (8 * NT));
 }
 
-// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.  us of this form and of that: at head_dim 128, H=32 Hk=8, 4096 - 8192
-// tokens, 36 rows B=1 35 and 32, B=8 91 and 65, 32 rows B=8 55 and 64; at head_dim 256, where this form takes two passes over 17 rows, H=16 Hk=4,
-// 24 rows B=1 with 8192 tokens 32 and 35 (with weights 56 and 47), B=8 77 and 65 (148 and 115), B=64 with 17 - 8191 256 and 213 (581 and 466).
-int chunk_from(int D) { return D == 128 ? 33 : 17; }
 // Blocks of a warp up to which a cluster takes a unit, joining its warps' results itself, instead of the even division with a kernel that joins.  us with and
 // without, H=32 Hk=8, one new token: B=1 with 4096 tokens 11.7 and 15.4, B=4 with 3601 - 4096 14.8 and 17.3, B=8 with 2048 14.5 and 18.0; with
 // 16 instead of 8, B=1 with 16384 tokens 25.0 against 19.4.
@@ -972,10 +968,15 @@ int small_row_tile(int R) { return R <= 8 ? 8 : 16; }
 
 }  // namespace
 
+// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.  us of this form and of that: at head_dim 128, H=32 Hk=8, 4096 - 8192
+// tokens, 36 rows B=1 35 and 32, B=8 91 and 65, 32 rows B=8 55 and 64; at head_dim 256, where this form takes two passes over 17 rows, H=16 Hk=4,
+// 24 rows B=1 with 8192 tokens 32 and 35 (with weights 56 and 47), B=8 77 and 65 (148 and 115), B=64 with 17 - 8191 256 and 213 (581 and 466).
+int cache_chunk_from(int D) { return D == 128 ? 33 : 17; }
+
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights) {
   CacheAttnPlan x;
   const int R = Nq * (H / Hk);
-  x.chunk = R >= chunk_from(D);
+  x.chunk = R >= cache_chunk_from(D);
   x.row_tile = x.chunk ? cache_chunk_rows(D) : small_row_tile(R);
   x.row_tiles = (R + x.row_tile - 1) / x.row_tile;
   const int64_t blocks = static_cast<int64_t>(T) * (page / 32), units = static_cast<int64_t>(B) * Hk * x.row_tiles;       // of a sequence; in all
