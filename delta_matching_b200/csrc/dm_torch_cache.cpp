@@ -190,13 +190,13 @@ PyObject* cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   const Tensor* w = nullptr;
   if (args[7] == Py_None ? accumulate != 0 : !(read_weights(args[7], cache, B, table.room(cache), w) && !overlaps(*w))) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(cache.dev);                // the plan is the cache's device's
   const int64_t ws_bytes = g_lib.attn_workspace_bytes(static_cast<int>(B), static_cast<int>(N), static_cast<int>(H), cache.c.heads, cache.c.head_dim, table.T,
                                                       cache.c.page_size, w != nullptr);
   if (ws_bytes <= 0) Py_RETURN_NONE;
   Tensor o, lse;
   {
     pybind11::gil_scoped_release no_gil;
-    const c10::cuda::CUDAGuard guard(cache.dev);
     int* status = status_of(cache.dev.index());
     const Tensor q = rows(*qp);
     o = empty({B, N, H, D}, at::kBFloat16, cache.dev);
