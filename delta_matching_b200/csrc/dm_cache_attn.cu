@@ -101,12 +101,6 @@ __device__ __forceinline__ void scale_queries(const CacheAttnParams& p, uint32_t
     f[j] = make_float2(__shfl_sync(0xffffffffu, back, 8 * t), __shfl_sync(0xffffffffu, back, 8 * t + 4));
   }
 }
-template <int D, int NT>
-__device__ __forceinline__ void load_queries(const CacheAttnParams& p, int b, int hk, int rt, int count, uint32_t (&qf)[NT][D / 16][2], float2 (&f)[NT]) {
-  ask_queries<D, NT>(p, b, hk, rt, count, qf);
-  scale_queries<D, NT>(p, qf, f);
-}
-
 // S^T of a block: acc[j][mt] rows: keys 16 mt + g (elements 0, 1) and + 8 (2, 3); columns: query rows 8 j + 2 t, + 1.
 template <int D, int NT>
 __device__ __forceinline__ void keys_times_queries(uint32_t kbase, const uint32_t (&qf)[NT][D / 16][2], float (&s)[NT][2][4]) {
@@ -745,11 +739,12 @@ __global__ void __launch_bounds__(128) cache_join_kernel(const CacheAttnParams p
 }
 
 // ------------------------------------------------------------------------------------------------ weights
-// weights[b, hk, j] (+)= sum over the group's rows of exp(s_rj - m_r) / l_r, with the rows' m and l from the kernels before: K is read once
-// more, a block of 32 tokens a warp, all row tiles on it; no result is shared between warps, and the sum's order is that of the rows.
-// This is the form for 17 to 32 rows of head_dim 128.  Up to 16 the main kernel leaves its logits (16 - 64 bytes a token instead of K's 128 or 256, and no
-// products), and cache_weights_of_logits_kernel adds their exponentials, one thread a token: a call with weights at H=32 Hk=8, B=16 with 2049 - 4096
-// tokens takes 33 us with one new token (59 with K read again) and 46 with four (66).
+// weights[b, hk, j] (+)= sum over the group's rows of exp(s_rj - m_r) / l_r, with the rows' m and l from the kernels before.  No result is shared between
+// warps or threads, and the sum's order is that of the rows.
+// Up to 16 rows the main kernel leaves its logits (16 - 64 bytes a token instead of K's 128 or 256, and no products), and
+// cache_weights_of_logits_kernel adds their exponentials, one thread a token: a call with weights at H=32 Hk=8, B=16 with 2049 - 4096 tokens takes 35 us
+// with one new token (59 with K read again) and 46 with four (66).  For 17 to 32 rows of head_dim 128 cache_weights_kernel reads K once more, a
+// block of 32 tokens a warp, all rows on it.
 __global__ void __launch_bounds__(256) cache_weights_of_logits_kernel(const CacheAttnParams p, const int pieces) {
   __shared__ float2 ml[16];
   grid_dep_wait();
@@ -781,9 +776,8 @@ __global__ void __launch_bounds__(256) cache_weights_of_logits_kernel(const Cach
   *at = p.accumulate ? *at + w : w;
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constant__ CUtensorMap tk, const CacheAttnParams p, const int row_tiles) {
-  constexpr int kStages = 4, kStageBytes = 32 * D, kRows = 8 * NT;
+__global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constant__ CUtensorMap tk, const CacheAttnParams p) {
+  constexpr int D = 128, NT = 4, kStages = 4, kStageBytes = 32 * D;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
@@ -822,8 +816,7 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
     if (lane == 0) {
       const uint32_t bar = my_bars + 8 * st, dst = ring + st * kStageBytes;
       asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kStageBytes) : "memory");
-#pragma unroll
-      for (int x = 0; x < D; x += 128) tma_load_4d(dst + x * 32, &tk, bar, x, sub * 32, hk, page);
+      tma_load_4d(dst, &tk, bar, 0, sub * 32, hk, page);
     }
     if (lane == st) ks_reg = __ldg(p.c.ks + page * p.c.s_page + hk * p.c.s_head + sub);
   };
@@ -842,7 +835,8 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
     const float2* row_ml = p.row_ml + (static_cast<int64_t>(seg.b) * p.c.Hk + hk) * R;
     uint32_t qf[NT][D / 16][2];
     float2 f[NT];
-    if (row_tiles == 1) load_queries<D, NT>(p, seg.b, hk, 0, count, qf, f);
+    ask_queries<D, NT>(p, seg.b, hk, 0, count, qf);
+    scale_queries<D, NT>(p, qf, f);
     for (int kb = seg.blk0; kb < seg.blk1; ++kb) {
       if (ok && !wait_warp(my_bars + 8 * st, parity, abort_flag)) {
         ok = false;
@@ -852,25 +846,22 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const __grid_constan
         const float ks = __shfl_sync(0xffffffffu, ks_reg, st);
         const int key0 = kb * 32;
         float w[4] = {0.f, 0.f, 0.f, 0.f};                    // of keys key0 + g + 8 i
-        for (int rt = 0; rt < row_tiles; ++rt) {
-          if (row_tiles > 1) load_queries<D, NT>(p, seg.b, hk, rt, count, qf, f);
-          float s[NT][2][4];
-          keys_times_queries<D, NT>(ring + st * kStageBytes, qf, s);
+        float s[NT][2][4];
+        keys_times_queries<D, NT>(ring + st * kStageBytes, qf, s);
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = rt * kRows + 8 * j + 2 * t + e;
-              const float2 ml = r < R ? row_ml[r] : make_float2(0.f, 0.f);
-              const int limit = row_info(p, r, hk, seg.n, count).limit;
-              const float fs = (e ? f[j].y : f[j].x) * ks;
+          for (int e = 0; e < 2; ++e) {
+            const int r = 8 * j + 2 * t + e;
+            const float2 ml = r < R ? row_ml[r] : make_float2(0.f, 0.f);
+            const int limit = row_info(p, r, hk, seg.n, count).limit;
+            const float fs = (e ? f[j].y : f[j].x) * ks;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float x = __fmul_rn(s[j][i >> 1][(i & 1) * 2 + e], fs) - ml.x;       // as in the main kernel
-                w[i] += key0 + g + 8 * i < limit ? ex2_approx(x) * ml.y : 0.f;
-              }
+            for (int i = 0; i < 4; ++i) {
+              const float x = __fmul_rn(s[j][i >> 1][(i & 1) * 2 + e], fs) - ml.x;         // as in the main kernel
+              w[i] += key0 + g + 8 * i < limit ? ex2_approx(x) * ml.y : 0.f;
             }
-        }
+          }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
@@ -945,16 +936,14 @@ cudaError_t launch_main(const CUtensorMap& tk, const CUtensorMap& tv, const Cach
   return launch_chained(cache_join_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(p.c.B) * p.H * p.Nq)), 128, 0, stream, p, row_tiles, C::kRows);
 }
 
-template <int D, int NT>
 cudaError_t launch_weights(const CUtensorMap& tk, const CacheAttnParams& p, cudaStream_t stream) {
-  constexpr int smem = 1024 + 4 * 4 * 32 * D + 4 * 4 * 8 + 136 * 4 + 64;
-  const cudaError_t e = allow_smem<cache_weights_kernel<D, NT>>(smem);
+  constexpr int smem = 1024 + 4 * 4 * 32 * 128 + 4 * 4 * 8 + 136 * 4 + 64;
+  const cudaError_t e = allow_smem<cache_weights_kernel>(smem);
   if (e != cudaSuccess) return e;
   // a wave, and no more warps than there can be blocks
   const int64_t most = (static_cast<int64_t>(p.c.B) * p.c.Hk * p.c.T * (p.c.page / 32) + 3) / 4, wave = sm_count() * 2ll;
   count_launch();
-  return launch_chained(cache_weights_kernel<D, NT>, dim3(static_cast<unsigned>(most < wave ? most : wave)), 128, smem, stream, tk, p,
-                        (p.Nq * p.rep + 8 * NT - 1) / (8 * NT));
+  return launch_chained(cache_weights_kernel, dim3(static_cast<unsigned>(most < wave ? most : wave)), 128, smem, stream, tk, p);
 }
 
 // Blocks of a warp up to which a cluster takes a unit, joining its warps' results itself, instead of the even division with a kernel that joins.  us with and
@@ -1023,7 +1012,7 @@ cudaError_t launch_cache_attn(int D, const CUtensorMap& tk, const CUtensorMap& t
     count_launch();
     return launch_chained(cache_weights_of_logits_kernel, dim3(static_cast<unsigned>(p.c.B) * p.c.Hk * pieces), 256, 0, stream, p, pieces);
   }
-  return launch_weights<128, 4>(tk, p, stream);              // head_dim 256 has its logits or the form for many rows
+  return launch_weights(tk, p, stream);                      // head_dim 256 has its logits or the form for many rows
 }
 
 }  // namespace dm
