@@ -180,16 +180,17 @@ def dm_cache_append(cache, k, v, block_table, lengths, counts=None):
 
     Each block of 32 slots and head gets the smallest power-of-two scale that holds its new values; a block that already holds tokens keeps
     the larger of the two scales, and its codes are rounded anew when that grows."""
+    if not torch.compiler.is_compiling():
+        new = _lib.native_cache().cache_append(cache, k, v, block_table, lengths, counts)
+        if new is not None:
+            return new
     if _recorded():
         return _OPS.cache_append(*cache, k, v, block_table, lengths, counts)
     return append_now(cache, k, v, block_table, lengths, counts)
 
 
 def append_now(cache, k, v, block_table, lengths, counts):
-    """dm_cache_append at once, whatever records: the implementation of the registered op too."""
-    new = _lib.native_cache().cache_append(cache, k, v, block_table, lengths, counts)
-    if new is not None:
-        return new
+    """dm_cache_append by the Python route, whatever records: what the registered op comes to where the native route does not take it."""
     pages, Hk, P, D = _check_cache(cache)
     _check_written(cache)
     _refuse_tangents(k=k, v=v, ks=cache.ks, vs=cache.vs)
@@ -224,6 +225,10 @@ def dm_cache_attn(q, cache, block_table, lengths, q_counts=None, causal=True, so
     fp32, natural log.  The logits and the softmax are those of the codes' exact values: q keeps its 8 bits (elements below 2^-28 of the row's
     largest lose some), sums and statistics are fp32.  In the second product a probability times the scale of its V block keeps 11 bits down to
     2^-25 of the largest such product that the row sees; smaller ones are off by up to 2^-36 of that."""
+    if not torch.compiler.is_compiling():
+        out = _lib.native_cache().cache_attn(q, cache, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, return_lse)
+        if out is not None:
+            return out
     if _recorded():
         args = (q, *cache, block_table, lengths, q_counts, bool(causal), softmax_scale)
         o, lse = _OPS.cache_attn(*args) if weights is None else _OPS.cache_attn_weights(*args, weights, bool(accumulate))
@@ -232,10 +237,7 @@ def dm_cache_attn(q, cache, block_table, lengths, q_counts=None, causal=True, so
 
 
 def attn_now(q, cache, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, return_lse):
-    """dm_cache_attn at once, whatever records: the implementation of the registered ops too."""
-    out = _lib.native_cache().cache_attn(q, cache, block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, return_lse)
-    if out is not None:
-        return out
+    """dm_cache_attn by the Python route, whatever records: what the registered ops come to where the native route does not take them."""
     pages, Hk, P, D = _check_cache(cache)
     _refuse_tangents(q=q, ks=cache.ks, vs=cache.vs, weights=weights)
     dev = cache.k8.device
@@ -282,16 +284,17 @@ def dm_cache_evict(cache, block_table, lengths, weights, new_block_table, budget
 
     Returns (new lengths (B) int32, kept (B, Hk, budget) int32: the old positions in order, -1 beyond, new weights (B, Hk, T2 * page_size) fp32: those of the
     kept tokens, 0 beyond).  The heads of a sequence keep different tokens but equally many."""
+    if not torch.compiler.is_compiling():
+        out = _lib.native_cache().cache_evict(cache, block_table, lengths, weights, new_block_table, budget, recent)
+        if out is not None:
+            return out
     if _recorded():
         return _OPS.cache_evict(*cache, block_table, lengths, weights, new_block_table, budget, recent)
     return evict_now(cache, block_table, lengths, weights, new_block_table, budget, recent)
 
 
 def evict_now(cache, block_table, lengths, weights, new_block_table, budget, recent):
-    """dm_cache_evict at once, whatever records: the implementation of the registered op too."""
-    out = _lib.native_cache().cache_evict(cache, block_table, lengths, weights, new_block_table, budget, recent)
-    if out is not None:
-        return out
+    """dm_cache_evict by the Python route, whatever records: what the registered op comes to where the native route does not take it."""
     pages, Hk, P, D = _check_cache(cache)
     _check_written(cache)
     _refuse_tangents(ks=cache.ks, vs=cache.vs, weights=weights)

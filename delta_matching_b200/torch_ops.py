@@ -111,10 +111,17 @@ def _(q8, k8, v8, do8, qs, ks, vs, dos, lse, delta, causal, ds32):
             q8.new_empty((B, N, Hk, D), dtype=BF16))
 
 
+def _cache_call(native, python, *args):
+    """What the functions of cache.py do at once: the native route, or the Python one where that takes the call."""
+    from . import _lib, cache
+    out = getattr(_lib.native_cache(), native)(*args)
+    return getattr(cache, python)(*args) if out is None else out
+
+
 def _cache_append(k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, k: Tensor, v: Tensor, block_table: Tensor, lengths: Tensor,
                   counts: Optional[Tensor]) -> Tensor:
     from . import cache
-    return cache.append_now(cache.KVCache8(k8, v8, ks, vs), k, v, block_table, lengths, counts)
+    return _cache_call("cache_append", "append_now", cache.KVCache8(k8, v8, ks, vs), k, v, block_table, lengths, counts)
 
 
 cache_append = torch.library.custom_op(f"{NS}::cache_append", _cache_append, mutates_args=("k8", "v8", "ks", "vs"), device_types="cuda")
@@ -128,7 +135,7 @@ def _(k8, v8, ks, vs, k, v, block_table, lengths, counts):
 def _cache_attn(q: Tensor, k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, q_counts: Optional[Tensor],
                 causal: bool, softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor]:
     from . import cache
-    return cache.attn_now(q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, None, False, True)
+    return _cache_call("cache_attn", "attn_now", q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, None, False, True)
 
 
 cache_attn = torch.library.custom_op(f"{NS}::cache_attn", _cache_attn, mutates_args=(), device_types="cuda")
@@ -143,7 +150,7 @@ def _(q, k8, v8, ks, vs, block_table, lengths, q_counts, causal, softmax_scale):
 def _cache_attn_weights(q: Tensor, k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, q_counts: Optional[Tensor],
                         causal: bool, softmax_scale: Optional[float], weights: Tensor, accumulate: bool) -> Tuple[Tensor, Tensor]:
     from . import cache
-    return cache.attn_now(q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, True)
+    return _cache_call("cache_attn", "attn_now", q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, q_counts, causal, softmax_scale, weights, accumulate, True)
 
 
 cache_attn_weights = torch.library.custom_op(f"{NS}::cache_attn_weights", _cache_attn_weights, mutates_args=("weights",), device_types="cuda")
@@ -158,7 +165,7 @@ def _(q, k8, v8, ks, vs, block_table, lengths, q_counts, causal, softmax_scale, 
 def _cache_evict(k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, weights: Tensor, new_block_table: Tensor,
                  budget: int, recent: int) -> Tuple[Tensor, Tensor, Tensor]:
     from . import cache
-    return cache.evict_now(cache.KVCache8(k8, v8, ks, vs), block_table, lengths, weights, new_block_table, budget, recent)
+    return _cache_call("cache_evict", "evict_now", cache.KVCache8(k8, v8, ks, vs), block_table, lengths, weights, new_block_table, budget, recent)
 
 
 cache_evict = torch.library.custom_op(f"{NS}::cache_evict", _cache_evict, mutates_args=("k8", "v8", "ks", "vs"), device_types="cuda")
