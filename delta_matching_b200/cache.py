@@ -179,7 +179,8 @@ def dm_cache_append(cache, k, v, block_table, lengths, counts=None):
     same call again leaves the same cache.
 
     Each block of 32 slots and head gets the smallest power-of-two scale that holds its new values; a block that already holds tokens keeps
-    the larger of the two scales, and its codes are rounded anew when that grows."""
+    the larger of the two scales, and its codes are rounded anew when that grows.  A page that is written belongs to one sequence: shared
+    prefixes end at a page's edge."""
     if not torch.compiler.is_compiling():
         new = _lib.native_cache().cache_append(cache, k, v, block_table, lengths, counts)
         if new is not None:

@@ -8,8 +8,8 @@
 //
 // One warp per (sequence, touched block, head, K or V): the block's rows stay in its registers between the maximum and the codes, no
 // exchange between warps.  Bound by its bytes (2 read, 1 written per element) for prompts: 10242 tokens of four sequences, 8 heads of 128, 50 MB in
-// 11.8 us = 4.3 TB/s (of 6.5; a launch and one round of loads, half the warps of the grid at a time, are 4 us of it).  By the launch for single
-// tokens: 5.7 us for 64 sequences.
+// 12.3 us = 4.1 TB/s (of 6.5; a launch and one round of loads, half the warps of the grid at a time, are 4 us of it).  By the launch for single
+// tokens: 5.4 us for 64 sequences.
 #include "dm_cache.cuh"
 #include "dm_kernels.h"
 #include "dm_quant_block.cuh"

@@ -15,10 +15,10 @@
 // K and V of a block in turn, each refilled as soon as it has been read.  Units that one warp holds whole are written at once; the pieces
 // of the others are joined by a second kernel.
 //
-// Bound by its bytes where there are many blocks a warp: one new token, H=32 Hk=8, B=64 with 17 - 8191 tokens 102 us = 5.3 TB/s of codes and
-// scales (the card copies at 6.5); H=64 Hk=8, one sequence of 131071 tokens 58 us = 4.7 TB/s; head_dim 256, H=16 Hk=16, B=8 with 4001 - 8192 73 us
-// = 5.4 TB/s.  Small calls are bound by the chain from the lengths through the block table to the first codes (about 6700 cycles), 2300 cycles a
-// block and the join (3000 - 6000): B=4 with 3601 - 4096 15 us, one sequence of 255 tokens 7.0 us.
+// Bound by its bytes where there are many blocks a warp: one new token, H=32 Hk=8, B=64 with 17 - 8191 tokens 101 us = 5.4 TB/s of codes and
+// scales (the card copies at 6.5); H=64 Hk=8, one sequence of 131071 tokens 57 us = 4.7 TB/s; head_dim 256, H=16 Hk=16, B=8 with 4001 - 8192 73 us
+// = 5.5 TB/s.  Small calls are bound by the chain from the lengths through the block table to the first codes (about 6700 cycles), 2300 cycles a
+// block and the join (3000 - 6000): B=4 with 3601 - 4096 15.4 us, one sequence of 255 tokens 7.1 us.
 #include <cooperative_groups.h>
 #include "dm_cache_sched.cuh"
 #include "dm_kernels.h"
@@ -947,8 +947,8 @@ cudaError_t launch_weights(const CUtensorMap& tk, const CacheAttnParams& p, cuda
 }
 
 // Blocks of a warp up to which a cluster takes a unit, joining its warps' results itself, instead of the even division with a kernel that joins.  us with and
-// without, H=32 Hk=8, one new token: B=1 with 4096 tokens 11.7 and 15.4, B=4 with 3601 - 4096 14.8 and 17.3, B=8 with 2048 14.5 and 18.0; with
-// 16 instead of 8, B=1 with 16384 tokens 25.0 against 19.4.
+// without, H=32 Hk=8, one new token: B=1 with 4096 tokens 12.7 and 14.8, B=4 with 3601 - 4096 15.5 and 18.5, B=8 with 2048 15.5 and 18.8; with
+// 16 instead of 8, B=1 with 16384 tokens took 25.0 against 19.4.
 constexpr int kClusterBlocks = 8;
 // A tile of 32 rows reads the codes once where two of 16 read them twice (the second time from L2), but its accumulators leave fewer warps in flight:
 // us with 32 and 16 at H=32 Hk=8, 8 new tokens: B=64 with 17 - 8191 tokens 232 and 243, B=8 with 4096 - 8192 56.4 and 54.7, B=1 with 1000
@@ -957,9 +957,9 @@ int small_row_tile(int R) { return R <= 8 ? 8 : 16; }
 
 }  // namespace
 
-// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.  us of this form and of that: at head_dim 128, H=32 Hk=8, 4096 - 8192
-// tokens, 36 rows B=1 35 and 32, B=8 91 and 65, 32 rows B=8 55 and 64; at head_dim 256, where this form takes two passes over 17 rows, H=16 Hk=4,
-// 24 rows B=1 with 8192 tokens 32 and 35 (with weights 56 and 47), B=8 77 and 65 (148 and 115), B=64 with 17 - 8191 256 and 213 (581 and 466).
+// Rows (new tokens x heads of a group) from which the tcgen05 form is taken.  us of this form and of that: at head_dim 128, H=32 Hk=8, 32 rows B=8 with
+// 4096 - 8192 tokens 59.4 and 65.6, B=1 with 8192 26.5 and 31.6, 36 rows 78.2 and 65.9, 27.0 and 31.6; at head_dim 256, where this form takes two
+// passes over 17 rows, H=16 Hk=4, 16 rows B=8 46.2 and 57.0, 24 rows 69.4 and 57.2, B=1 36.4 and 37.5, B=64 with 17 - 8191 296 and 217.
 int cache_chunk_from(int D) { return D == 128 ? 33 : 17; }
 
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights) {

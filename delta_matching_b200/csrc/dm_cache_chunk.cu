@@ -20,9 +20,9 @@
 // O the columns 256-511.
 //
 // Bound by the chain of a tile at head_dim 128: softmax 2000 - 2500 cycles, P V and the next S 1300 - 1700 until seen, beside which the other row tile
-// works; its exponentials alone are 2048 cycles for both row tiles.  512 new tokens, H=32 Hk=8, B=2 with 4096 - 8192 tokens: 122 - 130 us =
-// 760 - 810 TFLOP/s (cuBLAS in bf16: 1635).  At head_dim 256 by the conversion of the codes, 4400 cycles a tile, and their loads, for which 32 KB are left:
-// H=16 Hk=4 145 us = 680 TFLOP/s.
+// works; its exponentials alone are 2048 cycles for both row tiles.  512 new tokens, H=32 Hk=8, B=2 with 4096 - 8192 tokens: 128 - 132 us =
+// 750 - 770 TFLOP/s (cuBLAS in bf16: 1635).  At head_dim 256 by the conversion of the codes, 4400 cycles a tile, and their loads, for which 32 KB are left:
+// H=16 Hk=4 147 us = 670 TFLOP/s.
 #include <type_traits>
 #include "dm_cache.cuh"
 #include "dm_kernels.h"
@@ -31,8 +31,8 @@ namespace dm {
 
 namespace {
 
-// Key tiles that a unit's queries and output are worth.  us with 1, 3 and 6 at H=32 Hk=8: 512 new tokens, B=2 with 4096 - 8192 126, 123.8 and 130.6; 128
-// new ones, B=4 with 512 35.2, 32.6 and 33.0.
+// Key tiles that a unit's queries and output are worth.  us with 1, 3 and 6 at H=32 Hk=8: 512 new tokens, B=2 with 4096 - 8192 133.1, 129.8 and 133.0; 128
+// new ones, B=4 with 512 37.0, 34.3 and 34.2.
 constexpr int kChunkCost = 3;
 constexpr int kPBase = 12;                  // log2 of P at the reference,
 constexpr float kHeadroom = 3.9f;           // and what a row may exceed it by: P stays below 2^16

@@ -399,9 +399,9 @@ cudaError_t launch_cache_evict(int D, const CacheEvictParams& p, cudaStream_t st
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  // A CTA of the cluster takes 4096 tokens or more.  us of a call with 2048, 4096 and 8192: 32 rows of 3001 - 4096 tokens 17.7, 14.5 and 14.5, 128 rows of
-  // 2500 - 4096 51, 38 and 38, 16 rows of 16384 34, 24 and 26, 8 rows of 32768 18.8, 18.8 and 20.8 (before the tokens of a slice were taken at once).  (Clusters of 16: few are resident at
-  // a time; eight rows of 131072 tokens took 75 against 33.)
+  // A CTA of the cluster takes 4096 tokens or more.  us of a call with 2048, 4096 and 8192: 32 rows of 3001 - 4096 tokens 16.2, 13.6 and 13.6, 128 rows of
+  // 2500 - 4096 47.0, 37.5 and 37.5, 16 rows of 16384 23.2, 15.9 and 17.8, 8 rows of 32768 17.6, 17.6 and 19.5.  (Clusters of 16: few are resident
+  // at a time; eight rows of 131072 tokens took 75 against 33.)
   const int64_t most = static_cast<int64_t>(p.c.T) * p.c.page;
   int C = 1;
   while (C < kMaxCluster && most > 4096ll * C) C *= 2;

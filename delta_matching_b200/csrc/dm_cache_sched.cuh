@@ -10,8 +10,8 @@
 
 namespace dm {
 
-// us of a call with 1, 3 and 6: head_dim 256, H=16 Hk=16, B=8 with 4001 - 8192 tokens 74.9, 72.9 and 75.8; H=32 Hk=8, B=16 with 1000 - 4096, four new
-// tokens 31.1, 30.0 and 31.6.
+// us of a call with 1, 3 and 6: H=32 Hk=8, B=16 with 1000 - 4096 tokens, four new ones 36.0, 33.5 and 34.9; head_dim 256, H=16 Hk=16, B=8 with 4001 - 8192
+// 76.8, 76.8 and 76.6.
 constexpr int kUnitCost = 3;
 
 struct FlatRange {

@@ -37,7 +37,7 @@ extern "C" {
 #define DM_STATUS_TIMEOUT_PROBE 4
 #define DM_STATUS_BAD_PAGE 5      /* cache: an entry of the block table that names no page (no access was made) */
 #define DM_STATUS_BAD_LENGTH 6    /* cache: a length or count beyond what the block table has room for (it was cut) */
-/* the low four bits; the bits above name the kernel: 1 forward, 2 matched delta, 3 dK/dV, 4 dQ, 5 streaming pass, 6 tile pass */
+/* the low four bits; the bits above name the kernel: 1 forward, 2 matched delta, 3 dK/dV, 4 dQ, 5 streaming pass, 6 tile pass, 7 cache */
 
 /* Library identity.  Replaces the build-sanity ops build_gt() / build_hd128() / build_bf16dp() of
  * csrc/delta_matching_api.cpp:683-715: dm_version() is MAJOR * 10000 + MINOR * 100 + PATCH; dm_numerics() names the
@@ -240,7 +240,8 @@ int dm_copy_2d_async(void* dst, int64_t dpitch, const void* src, int64_t spitch,
  * of two, one for each block of 32 slots and head (value = code * scale).  Pages, heads and slots lie the given strides apart (codes: bytes,
  * multiples of 16; scales: elements, the blocks of a head adjacent); a slot's head_dim codes are contiguous.  K and V have equal strides.
  * A block table (B, T) int32, rows table_row entries apart, names each sequence's pages: token j is slot j % page_size of page
- * table[b, j / page_size].  lengths (B) int32 = tokens held; entries of the table beyond them are not read.
+ * table[b, j / page_size].  lengths (B) int32 = tokens held; entries of the table beyond them are not used.
+ * Rows of the table may be one and the same (table_row 0) where sequences are only read; a page that is written belongs to one sequence.
  * Table entries, lengths and counts are device data that the host does not see: a kernel that meets one out of range reports it through
  * `status` (DM_STATUS_BAD_PAGE, DM_STATUS_BAD_LENGTH), stays inside the buffers, and its outputs are invalid.
  * All pointers are the caller's word to be memory of the current device, as in dm_attn_fwd. */
