@@ -316,11 +316,9 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (!asked) ask_queries<D, NT>(p, seg.b, hk, rt, count, qf);
     asked = false;
     scale_queries<D, NT>(p, qf, f);
-    int lim[NT][2], lim_min = seg.n;
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) lim[j][e] = row_info(p, rt * C::kRows + 8 * j + 2 * t + e, hk, seg.n, count).limit;
+    // keys that this thread's row 8 j + 2 t + e sees: made where a block is cut (registers are what a block has least of)
+    auto lim = [&](int j, int e) { return row_info(p, rt * C::kRows + 8 * j + 2 * t + e, hk, seg.n, count).limit; };
+    int lim_min = seg.n;
     if (p.causal) lim_min = seg.n - count + 1;                // of the rows that are any
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -348,10 +346,15 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[j][mt][i] = __fmul_rn(s[j][mt][i], (i & 1) ? fs.y : fs.x);       // one value for the maximum and for p, however large
-            if (cut && key0 + 16 * mt + g + 8 * (i >> 1) >= lim[j][i & 1]) s[j][mt][i] = -CUDART_INF_F;
-          }
+          for (int i = 0; i < 4; ++i) s[j][mt][i] = __fmul_rn(s[j][mt][i], (i & 1) ? fs.y : fs.x);       // one value for the maximum and for p, however large
+        if (cut) {
+          const int seen[2] = {lim(j, 0) - key0 - g, lim(j, 1) - key0 - g};
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (16 * mt + 8 * (i >> 1) >= seen[i & 1]) s[j][mt][i] = -CUDART_INF_F;
+        }
         const int logit_rows = NT == 1 ? p.logit_rows : C::kRows;
         if (p.logits != nullptr && 8 * j + 2 * t < logit_rows) {        // for the weights: (b, kv head, token, row of the tile)
           float* to = p.logits + ((static_cast<int64_t>(seg.b) * p.c.Hk + hk) * p.c.T * p.c.page + key0 + g) * logit_rows + 8 * j + 2 * t;
@@ -426,11 +429,11 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       // A NaN code belongs to the rows that see its token; the others would multiply it by zero.  Where some row does not see all that is held: which rows see
       // one, by products of ones (token seen) and ones (code NaN), and zeros in its place.
       if (key0 + 32 > lim_min && lim_min < seg.n) {
-        const uint32_t slot = vbase + lane * 128;             // a lane a token
+        const uint32_t slot = vbase + lane * 128;             // a lane a token (its pieces in an order of its own: different banks)
         uint32_t found = 0;
 #pragma unroll 1
         for (int x = 0; x < D / 16; ++x) {
-          const float4 w = lds_f4(slot + (x >> 3) * 4096 + (x & 7) * 16);
+          const float4 w = lds_f4(slot + (x >> 3) * 4096 + (((x ^ lane) & 7) << 4));
           found |= nan_codes(__float_as_uint(w.x)) | nan_codes(__float_as_uint(w.y)) | nan_codes(__float_as_uint(w.z)) | nan_codes(__float_as_uint(w.w));
         }
         if (__any_sync(0xffffffffu, found != 0 && key0 + lane < seg.n)) {
@@ -440,7 +443,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int k = key0 + 8 * i + g;
-              sees[j][i >> 1][i & 1] = movmatrix_trans(pack_f16x2(k < lim[j][0] ? 1.f : 0.f, k < lim[j][1] ? 1.f : 0.f));
+              sees[j][i >> 1][i & 1] = movmatrix_trans(pack_f16x2(k < lim(j, 0) ? 1.f : 0.f, k < lim(j, 1) ? 1.f : 0.f));
             }
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
@@ -465,7 +468,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           __syncwarp();
 #pragma unroll 1
           for (int x = 0; x < D / 16; ++x) {
-            const uint32_t at = slot + (x >> 3) * 4096 + (x & 7) * 16;
+            const uint32_t at = slot + (x >> 3) * 4096 + (((x ^ lane) & 7) << 4);
             const float4 f4 = lds_f4(at);
             const uint32_t w[4] = {__float_as_uint(f4.x), __float_as_uint(f4.y), __float_as_uint(f4.z), __float_as_uint(f4.w)};
             sts_u4(at, w[0] & ~nan_codes(w[0]), w[1] & ~nan_codes(w[1]), w[2] & ~nan_codes(w[2]), w[3] & ~nan_codes(w[3]));
