@@ -962,7 +962,7 @@ int small_row_tile(int R) { return R <= 8 ? 8 : 16; }
 
 // Rows (new tokens x heads of a group) from which the tcgen05 form is taken.  us of this form and of that: at head_dim 128, H=32 Hk=8, 32 rows B=8 with
 // 4096 - 8192 tokens 59.4 and 65.6, B=1 with 8192 26.5 and 31.6, 36 rows 78.2 and 65.9, 27.0 and 31.6; at head_dim 256, where this form takes two
-// passes over 17 rows, H=16 Hk=4, 16 rows B=8 46.2 and 57.0, 24 rows 69.4 and 57.2, B=1 36.4 and 37.5, B=64 with 17 - 8191 296 and 217.
+// passes over 17 rows, H=16 Hk=4, 16 rows B=8 44.5 and 57.0, 24 rows 69.4 and 57.2, B=1 36.4 and 37.5, B=64 with 17 - 8191 296 and 217.
 int cache_chunk_from(int D) { return D == 128 ? 33 : 17; }
 
 CacheAttnPlan plan_cache_attn(int B, int Nq, int H, int Hk, int D, int T, int page, bool weights) {
