@@ -58,6 +58,11 @@ SIGNATURES = {
     "dm_cache_attn": (_I, [_P, _P, _L, _L, _L, _I, _I, _I, _P, _L, _I, _P, _P, _I, _F, _P, _P, _P, _L, _L, _I, _I, _P, _L, _P, _P]),
     "dm_dbg_cache_join_slots": (_I, [_I, _I, _I, _I, _I]),
     "dm_cache_evict": (_I, [_P, _I, _P, _L, _I, _P, _P, _L, _L, _P, _L, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "dm_draft_tree": (_I, [_P, _L, _P, _I, _I, _P, _P, _P, _P]),
+    "dm_cache_append_rotary": (_I, [_P, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _P, _I, _I, _P, _L, _I, _P, _P, _L, _P, _P, _P, _P, _P]),
+    "dm_cache_attn_tree_workspace_bytes": (_L, [_I, _I, _I, _I, _I, _I, _I]),
+    "dm_cache_attn_tree": (_I, [_P, _P, _L, _L, _L, _I, _I, _I, _P, _L, _I, _P, _P, _P, _L, _L, _F, _P, _P, _P, _L, _P, _P]),
+    "dm_cache_keep": (_I, [_P, _I, _P, _L, _I, _P, _P, _P, _L, _I, _P, _P, _P, _P]),
     "dm_kmean_static": (_I, [_P, _L, _L, _L, _I, _I, _I, _I, _P, _P, ctypes.c_char_p, _I]),
 }
 
@@ -141,21 +146,22 @@ def native_attn():
                                 lambda idx: ops.status_word(torch.device("cuda", idx)).data_ptr(), ops._raise_if_set,
                                 lambda *a: ops.bwd_fp8(*a[:11], ds32=a[11]), ops._SMALL_WS, ops._MAX_WS_TILES)
                 _dm_native.bind_cache(*(addr("dm_cache_" + n) for n in ("append", "attn", "attn_workspace_bytes", "evict")))
+                _dm_native.bind_drafts(*map(addr, ("dm_draft_tree", "dm_cache_append_rotary", "dm_cache_attn_tree", "dm_cache_attn_tree_workspace_bytes", "dm_cache_keep")))
                 _NATIVE = _dm_native.attn
     return _NATIVE
 
 
 class _NoCacheRoute:
     """In the place of the native module where the Python route has to take every call."""
-    cache_append = cache_attn = cache_evict = staticmethod(lambda *_: None)
+    cache_append = cache_attn = cache_evict = draft_tree = cache_append_rotary = cache_attn_tree = cache_keep = staticmethod(lambda *_: None)
 
 
 _CACHE_ROUTE = None
 
 
 def native_cache():
-    """The native eager route of the cache functions (csrc/dm_torch_cache.cpp): cache_append, cache_attn and cache_evict of the bound
-    module, each of which returns None when the Python route has to take the call."""
+    """The native eager route of the cache functions (csrc/dm_torch_cache.cpp, dm_torch_drafts.cpp): cache_append, cache_attn, cache_evict, draft_tree,
+    cache_append_rotary, cache_attn_tree and cache_keep of the bound module, each of which returns None when the Python route has to take the call."""
     global _CACHE_ROUTE
     if _CACHE_ROUTE is None:
         if native_attn() is _decline:

@@ -15,6 +15,7 @@ enum : int {
   kStatusTimeoutProbe = 4,
   kStatusBadPage = 5,           // a block table entry that names no page
   kStatusBadLength = 6,         // a length or count outside what the block table has room for
+  kStatusBadTree = 7,           // a parent that is no earlier node, a path that is not strictly increasing
   // which kernel it was, added to the code
   kInForward = 1 << 4,
   kInDelta = 2 << 4,

@@ -1,0 +1,177 @@
+// Trees of drafted tokens: what each node sees, and the tokens of one path moved together in the cache.
+#include "dm_cache.cuh"
+#include "dm_drafts.h"
+#include "dm_kernels.h"
+
+namespace dm {
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------ depths and ancestors
+// seen_i = {i} united with seen of i's parent; depth_i = |seen_i| - 1.  By doubling: after round r a node's set holds its first 2^r ancestors and itself
+// and jump names the ancestor behind them, so a tree of depth d takes log2(d) + 1 rounds.  One CTA a sequence, one thread a node, the sets in shared
+// memory word by word, so that the threads of a warp write adjacent words.
+__global__ void __launch_bounds__(1024) draft_tree_kernel(const DraftTreeParams p, const int words) {
+  extern __shared__ uint32_t sets[];                          // (words, N)
+  __shared__ int jumps[kMaxNodes];
+  grid_dep_wait();
+  const int b = blockIdx.x, i = threadIdx.x, N = p.N, count = checked_count(p.status, p.counts, b, N);
+  int jump = -1;
+  if (i < count) {
+    jump = __ldg(p.parents + b * p.row + i);
+    if (jump < -1 || jump >= i) {                             // no earlier node
+      report(p.status, kStatusBadTree + kInCache);
+      jump = -1;
+    }
+  }
+  if (i < N) {
+    for (int w = 0; w < words; ++w) sets[w * N + i] = i < count && w == i >> 5 ? 1u << (i & 31) : 0u;
+    jumps[i] = jump;
+  }
+  while (__syncthreads_or(jump >= 0)) {
+    int next = -1;
+    if (jump >= 0) next = jumps[jump];
+    const int last = jump >= 0 ? jump >> 5 : -1;              // ancestors come before: the words up to the jump's own
+    for (int w0 = 0; w0 < words; w0 += 8) {                   // eight words at a time: read by all before any is written
+      uint32_t x[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) x[w] = w0 + w <= last ? sets[(w0 + w) * N + jump] : 0u;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < 8; ++w)
+        if (w0 + w <= last) sets[(w0 + w) * N + i] |= x[w];
+    }
+    if (i < N) jumps[i] = next;
+    jump = next;
+  }
+  if (i < N) {
+    int bits = 0;
+    for (int w = 0; w < words; ++w) bits += __popc(sets[w * N + i]);
+    p.depth[static_cast<int64_t>(b) * N + i] = max(0, bits - 1);
+  }
+  uint32_t* out = p.seen + static_cast<int64_t>(b) * N * words;
+  for (int x = i; x < N * words; x += blockDim.x) out[x] = sets[(x % words) * N + x / words];
+}
+
+// ------------------------------------------------------------------------------------------------ keeping a path
+// Token path[i] behind `before` becomes token i behind it.  A CTA is a (sequence, kv head, K or V), a warp a block of 32 tokens that is written: it reads
+// the block's older tokens and its tokens of the path, takes the smallest power-of-two scale that holds them (as the eviction does), and rounds the codes
+// to it.  A path is strictly increasing, so a token never moves up: what a block takes lies in it or behind it, and the warps of a CTA read all that
+// they need before any of them writes; blocks of a later round are behind those.
+constexpr int kKeepWarps = 8;
+
+template <int D>
+__global__ void __launch_bounds__(kKeepWarps * 32) cache_keep_kernel(const CacheKeepParams p) {
+  constexpr int kTpr = D / 16, kRpp = 32 / kTpr, kPass = 32 / kRpp;      // lanes a row, rows a pass, passes
+  grid_dep_wait();
+  const CacheView& c = p.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int rest = blockIdx.x;
+  const bool is_v = (rest & 1) != 0;
+  rest >>= 1;
+  const int hk = rest % c.Hk, b = rest / c.Hk;
+  const int n = cache_length(c, b);
+  int start = __ldg(p.before + b), count = checked_count(c.status, p.counts, b, p.M);
+  if (start < 0 || start > n) {
+    report(c.status, kStatusBadLength + kInCache);
+    start = min(max(start, 0), n);
+  }
+  const int* path = p.path + b * p.p_row;
+  bool bad = false;
+  for (int i = threadIdx.x; i < count; i += blockDim.x) {
+    const int at = __ldg(path + i);
+    bad |= at < 0 || at >= n - start || (i > 0 && __ldg(path + i - 1) >= at);
+  }
+  if (__syncthreads_or(bad)) {                                // not a path: nothing of the sequence is changed
+    if (threadIdx.x == 0) report(c.status, kStatusBadTree + kInCache);
+    count = 0;
+  }
+  if (hk == 0 && !is_v && threadIdx.x == 0) p.new_lengths[b] = start + count;
+  if (count == 0) return;
+  uint8_t* codes = (is_v ? c.v8 : c.k8) + hk * c.c_head;
+  float* scales = (is_v ? c.vs : c.ks) + hk * c.s_head;
+  const int bpp = c.page / 32, first = start / 32, blocks = (start + count - 1) / 32 - first + 1;
+  const int c16 = (lane % kTpr) * 16, r0 = lane / kTpr;
+  for (int j0 = 0; j0 < blocks; j0 += blockDim.x / 32) {
+    const int blk = first + j0 + warp, row = blk * 32 + lane; // this lane's row of the block, of 32
+    const bool live = j0 + warp < blocks, held = live && row < start + count;
+    int page = 0, slot = 0;
+    bool good = held;
+    if (held) {
+      const int from = row < start ? row : start + __ldg(path + row - start), entry = from / c.page;
+      slot = from - entry * c.page;
+      page = checked_page(c, __ldg(c.table + b * c.t_row + entry));
+      good = page >= 0;
+    }
+    const float s_row = good ? scales[page * c.s_page + slot / 32] : 0.f;
+    uint4 y[kPass];
+    float top = 0.f;                                          // of this lane's rows' codes, times their scales
+    float s_of[kPass];
+#pragma unroll
+    for (int ps = 0; ps < kPass; ++ps) {
+      const int r = r0 + ps * kRpp;
+      const int page_r = __shfl_sync(0xffffffffu, page, r), slot_r = __shfl_sync(0xffffffffu, slot, r);
+      const bool good_r = __shfl_sync(0xffffffffu, good ? 1 : 0, r) != 0;
+      s_of[ps] = __shfl_sync(0xffffffffu, s_row, r);
+      y[ps] = make_uint4(0, 0, 0, 0);
+      if (good_r) y[ps] = *reinterpret_cast<const uint4*>(codes + page_r * c.c_page + slot_r * c.c_slot + c16);
+    }
+#pragma unroll
+    for (int ps = 0; ps < kPass; ++ps) {
+      const uint32_t w[4] = {y[ps].x, y[ps].y, y[ps].z, y[ps].w};
+      uint32_t m = 0;                                         // sizes of codes are in the order of their bytes; NaN is left out
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __vmaxu4(m, w[i] & 0x7F7F7F7Fu & ~nan_codes(w[i]));
+      m = max(max(m & 0xFFu, (m >> 8) & 0xFFu), max((m >> 16) & 0xFFu, m >> 24));
+      top = fmaxf(top, f16x2_to_float2(e4m3_lo_f16x2(m)).x * s_of[ps]);
+    }
+    const uint32_t sb = pow2_sb(warp_max(top), 1u);
+    const float s = sb_to_scale(sb);
+    // the block's own place
+    const int entry = live ? blk / bpp : 0;
+    const int to = live ? checked_page(c, __ldg(c.table + b * c.t_row + entry)) : -1;
+    __syncthreads();
+    if (to >= 0) {
+      uint8_t* out = codes + to * c.c_page + static_cast<int64_t>(blk - entry * bpp) * 32 * c.c_slot + c16;
+#pragma unroll
+      for (int ps = 0; ps < kPass; ++ps) {
+        const int r = r0 + ps * kRpp;
+        if (blk * 32 + r >= start + count) continue;
+        // a code that is not zero needs no more than 2^18; zero stays zero
+        const int e = static_cast<int>(scale_to_sb(s_of[ps])) - static_cast<int>(sb);
+        const float ratio = sb_to_scale(static_cast<uint32_t>(min(18, max(e, -100)) + 127));
+        uint4 w = y[ps];
+        if (e != 0) w = make_uint4(requant4(w.x, ratio), requant4(w.y, ratio), requant4(w.z, ratio), requant4(w.w, ratio));
+        *reinterpret_cast<uint4*>(out + r * c.c_slot) = w;
+      }
+      if (lane == 0) scales[to * c.s_page + blk - entry * bpp] = s;
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_draft_tree(const DraftTreeParams& p, cudaStream_t stream) {
+  const int words = (p.N + 31) / 32, threads = words * 32, smem = words * p.N * 4;
+  if (smem > 40 * 1024) {                                     // beyond what a kernel has unasked, its static arrays aside
+    static bool allowed[64] = {};                             // once per device: the driver call takes longer than a launch
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !allowed[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(draft_tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxNodes / 32 * kMaxNodes * 4);
+      if (e != cudaSuccess) return e;
+      if (dev >= 0 && dev < 64) allowed[dev] = true;
+    }
+  }
+  count_launch();
+  return launch_chained(draft_tree_kernel, dim3(p.B), threads, smem, stream, p, words);
+}
+
+cudaError_t launch_cache_keep(int D, const CacheKeepParams& p, cudaStream_t stream) {
+  const int blocks = (p.M + 30) / 32 + 1, warps = blocks < kKeepWarps ? blocks : kKeepWarps;       // blocks that a path can touch
+  const dim3 grid(static_cast<unsigned>(p.c.B) * p.c.Hk * 2);
+  count_launch();
+  return D == 128 ? launch_chained(cache_keep_kernel<128>, grid, warps * 32, 0, stream, p) : launch_chained(cache_keep_kernel<256>, grid, warps * 32, 0, stream, p);
+}
+
+}  // namespace dm

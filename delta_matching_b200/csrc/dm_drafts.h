@@ -1,0 +1,65 @@
+// Internal launch interface of the functions for drafted tokens (trees, rotation with append, attention of a tree, keeping a path) between their
+// C-ABI layer (dm_drafts_abi.cu) and the kernel translation units.
+#pragma once
+#include "dm_cache.h"
+
+namespace dm {
+
+constexpr int kMaxNodes = 1024;     // of a tree
+
+struct DraftTreeParams {
+  const int* parents;               // (B, N), rows `row` entries apart
+  int64_t row;
+  const int* counts;                // (B) or null: N each
+  int B, N;
+  int* depth;                       // (B, N)
+  uint32_t* seen;                   // (B, N, words)
+  int* status;
+};
+
+struct CacheRotaryParams {
+  CacheView c;
+  const __nv_bfloat16* q;           // (B, N, H, D), k, v (B, N, Hk, D) by element strides, rows 16-byte aligned
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  int64_t q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh;
+  const float* freqs;               // (half)
+  int half;                         // pairs of channels that are rotated, a multiple of 8
+  int interleaved;                  // pairs (2 j, 2 j + 1), else (j, j + half)
+  const int* offsets;               // (B, N) or null: positions behind lengths[b]; rows o_row entries apart
+  int64_t o_row;
+  const int* counts;                // (B) or null: N each
+  __nv_bfloat16* q_out;             // (B, N, H, D) contiguous
+  int* new_lengths;                 // (B)
+  int N, H;
+};
+
+struct CacheTreeParams {
+  CacheView c;
+  const __nv_bfloat16* q;           // (B, N, H, D) by element strides, rows 16-byte aligned
+  int64_t q_sb, q_sn, q_sh;
+  const int* counts;                // (B) or null: N each
+  const uint32_t* seen;             // (B, N, words): bit j % 32 of word j / 32 of node i: node i sees node j; by element strides, words adjacent
+  int64_t s_sb, s_sn;
+  int N, H, rep, words;
+  float scale;                      // softmax scale
+  __nv_bfloat16* o;                 // (B, N, H, D) contiguous
+  float* lse;                       // (B, H, N)
+};
+
+struct CacheKeepParams {
+  CacheView c;                      // lengths: with the drafted tokens
+  const int* before;                // (B): without them
+  const int* path;                  // (B, M), rows p_row entries apart
+  int64_t p_row;
+  int M;
+  const int* counts;                // (B): entries of the path
+  int* new_lengths;                 // (B)
+};
+
+cudaError_t launch_draft_tree(const DraftTreeParams& p, cudaStream_t stream);
+cudaError_t launch_cache_rotary(int D, const CacheRotaryParams& p, cudaStream_t stream);
+cudaError_t launch_cache_tree(int D, const CacheTreeParams& p, cudaStream_t stream);
+cudaError_t launch_cache_keep(int D, const CacheKeepParams& p, cudaStream_t stream);
+
+}  // namespace dm

@@ -421,6 +421,11 @@ PyMethodDef kMethods[] = {
     {"cache_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::cache_attn)), METH_FASTCALL, "cache attention on CUDA tensors, or None"},
     {"cache_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::cache_evict)), METH_FASTCALL, "cache eviction on CUDA tensors, or None"},
     {"bind_cache", dm_native::bind_cache, METH_VARARGS, "addresses of the kernel library's cache entry points"},
+    {"draft_tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::draft_tree)), METH_FASTCALL, "what the nodes of a draft see on CUDA tensors, or None"},
+    {"cache_append_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::cache_append_rotary)), METH_FASTCALL, "cache append with rotation on CUDA tensors, or None"},
+    {"cache_attn_tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::cache_attn_tree)), METH_FASTCALL, "cache attention of a tree on CUDA tensors, or None"},
+    {"cache_keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dm_native::cache_keep)), METH_FASTCALL, "a path of the drafted tokens kept on CUDA tensors, or None"},
+    {"bind_drafts", dm_native::bind_drafts, METH_VARARGS, "addresses of the kernel library's entry points for drafted tokens"},
     {"bind", bind, METH_VARARGS, "addresses of the kernel library's entry points and the op layer's callbacks"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_dm_native", "native eager route", -1, kMethods};

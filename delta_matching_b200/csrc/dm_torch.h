@@ -29,5 +29,11 @@ PyObject* cache_append(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* cache_evict(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* bind_cache(PyObject*, PyObject* args);
+// The methods of dm_torch_drafts.cpp.
+PyObject* draft_tree(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* cache_append_rotary(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* cache_attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* cache_keep(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* bind_drafts(PyObject*, PyObject* args);
 
 }  // namespace dm_native

@@ -35,7 +35,8 @@ _DEBUG = os.environ.get("DM_DEBUG", "0") not in ("", "0")
 
 STATUS_TEXT = {1: "TMA producer gave up waiting for a free stage", 2: "MMA issuer gave up waiting",
                3: "compute warps gave up waiting for an accumulator", 4: "probe kernel gave up waiting",
-               5: "a block table entry names no page", 6: "a length or count exceeds what the block table has room for"}
+               5: "a block table entry names no page", 6: "a length or count exceeds what the block table has room for",
+               7: "a drafted token's parent is no earlier one, or a path's entries do not increase or name no drafted token"}
 STATUS_KERNEL = {1: "forward", 2: "matched delta", 3: "dK/dV", 4: "dQ", 5: "streaming pass",
                  6: "tile pass", 7: "cache"}     # v >> 4
 

@@ -11,6 +11,11 @@ instead of ctypes calls it cannot look into.
     torch.ops.delta_matching_b200.cache_attn_weights(..., weights!, accumulate) -> O, LSE
     torch.ops.delta_matching_b200.cache_evict(k8!, v8!, ks!, vs!, block_table, lengths, weights, new_block_table, budget, recent)
         -> new lengths, kept, new weights
+    torch.ops.delta_matching_b200.draft_tree(parents, counts) -> depth, seen
+    torch.ops.delta_matching_b200.cache_append_rotary(k8!, v8!, ks!, vs!, q, k, v, block_table, lengths, freqs, offsets, counts, interleaved)
+        -> rotated q, new lengths
+    torch.ops.delta_matching_b200.cache_attn_tree(q, k8, v8, ks, vs, block_table, lengths, seen, counts, softmax_scale) -> O, LSE
+    torch.ops.delta_matching_b200.cache_keep(k8!, v8!, ks!, vs!, block_table, before, lengths, path, counts) -> new lengths
 
 The reference registers the same roles as real ops (csrc/delta_matching_api.cpp:683-715: fwd_fp8, delta_fp8, bwd_fp8_t)
 and its autograd function calls them through torch.ops (delta_matching/attn.py:37-118), which is what lets its API run
@@ -175,6 +180,70 @@ cache_evict = torch.library.custom_op(f"{NS}::cache_evict", _cache_evict, mutate
 def _(k8, v8, ks, vs, block_table, lengths, weights, new_block_table, budget, recent):
     B, Hk = weights.shape[:2]
     return (lengths.new_empty((B,)), lengths.new_empty((B, Hk, budget)), weights.new_empty((B, Hk, new_block_table.shape[1] * k8.shape[2])))
+
+
+def _drafts_call(native, python, *args):
+    """_cache_call for the functions of drafts.py."""
+    from . import _lib, drafts
+    out = getattr(_lib.native_cache(), native)(*args)
+    return getattr(drafts, python)(*args) if out is None else out
+
+
+def _draft_tree(parents: Tensor, counts: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    return _drafts_call("draft_tree", "tree_now", parents, counts)
+
+
+draft_tree = torch.library.custom_op(f"{NS}::draft_tree", _draft_tree, mutates_args=(), device_types="cuda")
+
+
+@draft_tree.register_fake
+def _(parents, counts):
+    B, N = parents.shape
+    return parents.new_empty((B, N)), parents.new_empty((B, N, (N + 31) // 32))
+
+
+def _cache_append_rotary(k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, q: Tensor, k: Tensor, v: Tensor, block_table: Tensor, lengths: Tensor, freqs: Tensor,
+                         offsets: Optional[Tensor], counts: Optional[Tensor], interleaved: bool) -> Tuple[Tensor, Tensor]:
+    from . import cache
+    return _drafts_call("cache_append_rotary", "append_rotary_now", cache.KVCache8(k8, v8, ks, vs), q, k, v, block_table, lengths, freqs, offsets, counts, interleaved)
+
+
+cache_append_rotary = torch.library.custom_op(f"{NS}::cache_append_rotary", _cache_append_rotary, mutates_args=("k8", "v8", "ks", "vs"), device_types="cuda")
+
+
+@cache_append_rotary.register_fake
+def _(k8, v8, ks, vs, q, k, v, block_table, lengths, freqs, offsets, counts, interleaved):
+    B, N, H, D = q.shape
+    return q.new_empty((B, N, H, D)), lengths.new_empty(lengths.shape)
+
+
+def _cache_attn_tree(q: Tensor, k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, lengths: Tensor, seen: Tensor,
+                     counts: Optional[Tensor], softmax_scale: Optional[float]) -> Tuple[Tensor, Tensor]:
+    from . import cache, drafts
+    tree = drafts.DraftTree(seen, seen, counts)              # depths are not looked at
+    return _drafts_call("cache_attn_tree", "attn_tree_now", q, cache.KVCache8(k8, v8, ks, vs), block_table, lengths, tree, softmax_scale, True)
+
+
+cache_attn_tree = torch.library.custom_op(f"{NS}::cache_attn_tree", _cache_attn_tree, mutates_args=(), device_types="cuda")
+
+
+@cache_attn_tree.register_fake
+def _(q, k8, v8, ks, vs, block_table, lengths, seen, counts, softmax_scale):
+    B, N, H, D = q.shape
+    return q.new_empty((B, N, H, D)), q.new_empty((B, H, N), dtype=F32)
+
+
+def _cache_keep(k8: Tensor, v8: Tensor, ks: Tensor, vs: Tensor, block_table: Tensor, before: Tensor, lengths: Tensor, path: Tensor, counts: Tensor) -> Tensor:
+    from . import cache
+    return _drafts_call("cache_keep", "keep_now", cache.KVCache8(k8, v8, ks, vs), block_table, before, lengths, path, counts)
+
+
+cache_keep = torch.library.custom_op(f"{NS}::cache_keep", _cache_keep, mutates_args=("k8", "v8", "ks", "vs"), device_types="cuda")
+
+
+@cache_keep.register_fake
+def _(k8, v8, ks, vs, block_table, before, lengths, path, counts):
+    return lengths.new_empty(lengths.shape)
 
 
 class _Direct:

@@ -37,6 +37,7 @@ extern "C" {
 #define DM_STATUS_TIMEOUT_PROBE 4
 #define DM_STATUS_BAD_PAGE 5      /* cache: an entry of the block table that names no page (no access was made) */
 #define DM_STATUS_BAD_LENGTH 6    /* cache: a length or count beyond what the block table has room for (it was cut) */
+#define DM_STATUS_BAD_TREE 7      /* cache: a drafted token's parent that is no earlier one, a path whose entries do not increase or name no drafted token */
 /* the low four bits; the bits above name the kernel: 1 forward, 2 matched delta, 3 dK/dV, 4 dQ, 5 streaming pass, 6 tile pass, 7 cache */
 
 /* Library identity.  Replaces the build-sanity ops build_gt() / build_hd128() / build_bf16dp() of
@@ -288,6 +289,40 @@ int dm_dbg_cache_join_slots(int many_rows, int x, int y, int grid, int i);
 int dm_cache_evict(const dm_kv_cache* cache, int B, const int* table, int64_t table_row, int T, const int* lengths,
                    const float* weights, int64_t w_sb, int64_t w_sh, const int* new_table, int64_t new_table_row, int new_T,
                    int budget, int recent, int* new_lengths, int* kept, float* new_weights, int* status, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ drafted tokens
+ * A tree of N <= 1024 drafted tokens a sequence behind what the cache holds; no counterpart in the reference.  A node's parent is an earlier node, or -1:
+ * the sequence's last token.  With counts (B), sequence b has the first counts[b] nodes; NULL: N each.
+ *
+ * dm_draft_tree: parents (B, N) int32, rows parents_row entries apart -> depth (B, N): ancestors of a node; seen (B, N, (N + 31) / 32): bit j % 32 of word
+ * j / 32 of node i is set where j is i or an ancestor of it.  Nodes beyond counts: zeros.  A parent that is no earlier node: DM_STATUS_BAD_TREE. */
+int dm_draft_tree(const int* parents, int64_t parents_row, const int* counts, int B, int N, int* depth, int* seen, int* status, void* stream);
+
+/* dm_cache_append with the rotation by position, of k and of q (bf16 by element strides for (batch, token, head)): new token i of sequence b stands at
+ * position t = lengths[b] + offsets[b, i] (i itself where offsets is NULL; rows offsets_row entries apart), and channels (j, j + n_freqs), or (2 j, 2 j + 1)
+ * where interleaved, j < n_freqs, become (x cos - y sin, y cos + x sin) of the angle t freqs[j]; other channels stay as they are.  n_freqs: a multiple of 8,
+ * at most head_dim / 2.  k is quantised from the fp32 products; q_out (B, N, H, head_dim) bf16 contiguous, 0 for tokens beyond counts. */
+int dm_cache_append_rotary(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
+                           const void* k, int64_t k_sb, int64_t k_sn, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+                           int B, int N, int H, const float* freqs, int n_freqs, int interleaved,
+                           const int* table, int64_t table_row, int T, const int* lengths, const int* offsets, int64_t offsets_row, const int* counts,
+                           void* q_out, int* new_lengths, int* status, void* stream);
+
+/* Attention of the N drafted tokens a sequence, the last counts[b] of the lengths[b] tokens that the cache holds: node i sees all tokens before the drafted
+ * ones, the earlier nodes whose bits are set in seen[b, i] (as dm_draft_tree writes them; by element strides, words adjacent) and itself; other bits are
+ * not looked at.  o (B, N, H, head_dim) bf16 contiguous, lse (B, H, N) fp32 natural log; nodes beyond counts: 0 and -inf.
+ * workspace: dm_cache_attn_tree_workspace_bytes, 16-byte aligned, contents ignored (0: a shape that is refused). */
+int64_t dm_cache_attn_tree_workspace_bytes(int B, int N, int H, int Hk, int D, int T, int page_size);
+int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, int B, int N, int H,
+                       const int* table, int64_t table_row, int T, const int* lengths, const int* counts, const int* seen, int64_t seen_sb, int64_t seen_sn,
+                       float softmax_scale, void* o, float* lse, void* workspace, int64_t workspace_bytes, int* status, void* stream);
+
+/* Of the drafted tokens before[b] ... lengths[b] - 1 those of a path are kept: path[b, 0 ... counts[b] - 1], strictly increasing indexes behind before[b]
+ * (rows path_row entries apart, M <= 1024 entries), become the tokens before[b], before[b] + 1, ...  Each block of 32 slots that is written gets the
+ * smallest power-of-two scale that holds its tokens, older ones too; slots behind the last token stay as they are.  new_lengths (B) = before + counts.  A
+ * path that does not increase or leaves the drafted tokens: DM_STATUS_BAD_TREE, and nothing of the sequence is changed. */
+int dm_cache_keep(const dm_kv_cache* cache, int B, const int* table, int64_t table_row, int T, const int* before, const int* lengths,
+                  const int* path, int64_t path_row, int M, const int* counts, int* new_lengths, int* status, void* stream);
 
 #ifdef __cplusplus
 }
