@@ -45,7 +45,19 @@ struct CacheTreeParams {
   float scale;                      // softmax scale
   __nv_bfloat16* o;                 // (B, N, H, D) contiguous
   float* lse;                       // (B, H, N)
+  float* part_o;                    // partial results: 2 slots a CTA, of row_tile rows of D fp32 each, and of their rows (m, l, u, marked): the sum is
+  float4* part_ml;                  // l 2^m, the values count in 2^u
+  int grid;                         // CTAs of the main kernel
+  int row_tile;                     // rows (drafted tokens x heads of a group) of a unit
 };
+
+// How a call of dm_cache_attn_tree is laid out, and its workspace.
+struct CacheTreePlan {
+  int row_tile, grid;
+  int64_t part_o_bytes, part_ml_bytes;
+  int64_t bytes() const { return part_o_bytes + part_ml_bytes; }
+};
+CacheTreePlan plan_cache_tree(int B, int N, int H, int Hk, int D, int T, int page);
 
 struct CacheKeepParams {
   CacheView c;                      // lengths: with the drafted tokens
@@ -59,7 +71,7 @@ struct CacheKeepParams {
 
 cudaError_t launch_draft_tree(const DraftTreeParams& p, cudaStream_t stream);
 cudaError_t launch_cache_rotary(int D, const CacheRotaryParams& p, cudaStream_t stream);
-cudaError_t launch_cache_tree(int D, const CacheTreeParams& p, cudaStream_t stream);
+cudaError_t launch_cache_tree(int D, const CUtensorMap& tk, const CUtensorMap& tv, const CacheTreeParams& p, cudaStream_t stream);
 cudaError_t launch_cache_keep(int D, const CacheKeepParams& p, cudaStream_t stream);
 
 }  // namespace dm

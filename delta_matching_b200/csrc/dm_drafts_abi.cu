@@ -25,6 +25,11 @@ int check_tree_shape(int B, int N, int H, int Hk, int D, int T, int page) {
   if (page <= 0 || page % 32) return fail(DM_ERR_ARG, "delta_matching: page size must be a positive multiple of 32 (got %d)", page);
   if (H % Hk) return fail(DM_ERR_ARG, "delta_matching: nheads (%d) must be a multiple of nheads_k (%d)", H, Hk);
   if (static_cast<int64_t>(B) * H > 65535) return fail(DM_ERR_ARG, "delta_matching: batch * nheads must be at most 65535");
+  // steps of the division of the work are ints: of 128 rows x 128 tokens, and a few a unit
+  const int64_t row_tiles = (static_cast<int64_t>(N) * (H / Hk) + 127) / 128;
+  if (static_cast<int64_t>(T) * page / 128 + 8 > (1ll << 30) / (static_cast<int64_t>(B) * Hk * row_tiles))
+    return fail(DM_ERR_ARG, "delta_matching: too much work for one call (%d sequences with room for %lld tokens, %lld rows)", B,
+                static_cast<long long>(T) * page, static_cast<long long>(N) * H);
   return 0;
 }
 
@@ -90,7 +95,7 @@ int dm_cache_append_rotary(const dm_kv_cache* cache, const void* q, int64_t q_sb
 
 int64_t dm_cache_attn_tree_workspace_bytes(int B, int N, int H, int Hk, int D, int T, int page_size) {
   if (check_tree_shape(B, N, H, Hk, D, T, page_size) != 0) return 0;
-  return 16;
+  return dm::plan_cache_tree(B, N, H, Hk, D, T, page_size).bytes();
 }
 
 int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, int B, int N, int H,
@@ -104,7 +109,8 @@ int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, in
   DM_TRY(check_pointer(seen, "seen"));
   if (seen_sb < 0 || seen_sn < 0) return fail(DM_ERR_ARG, "delta_matching: strides of seen must not be negative");
   if (!(softmax_scale > 0.f && softmax_scale <= FLT_MAX)) return fail(DM_ERR_ARG, "delta_matching: softmax_scale must be positive and finite in 32 bits (got %g)", softmax_scale);
-  const int64_t need = dm_cache_attn_tree_workspace_bytes(B, N, H, cache->heads, cache->head_dim, T, cache->page_size);
+  const dm::CacheTreePlan x = dm::plan_cache_tree(B, N, H, cache->heads, cache->head_dim, T, cache->page_size);
+  const int64_t need = x.bytes();
   if (workspace_bytes < need)
     return fail(DM_ERR_ARG, "delta_matching: workspace of %lld bytes given, %lld needed", static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   DM_TRY(check_sm100());
@@ -119,7 +125,14 @@ int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, in
   p.scale = softmax_scale;
   p.o = static_cast<__nv_bfloat16*>(o);
   p.lse = lse;
-  const cudaError_t e = dm::launch_cache_tree(cache->head_dim, p, static_cast<cudaStream_t>(stream));
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + x.part_o_bytes);
+  p.grid = x.grid;
+  p.row_tile = x.row_tile;
+  CUtensorMap tk, tv;
+  DM_TRY(pool_map(&tk, cache, cache->k8));
+  DM_TRY(pool_map(&tv, cache, cache->v8));
+  const cudaError_t e = dm::launch_cache_tree(cache->head_dim, tk, tv, p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : cuda_fail(e, "cache tree attention launch");
 }
 

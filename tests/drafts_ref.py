@@ -95,11 +95,13 @@ def keep(pools, table, before, path, counts):
 def attention(q, cache, table, lengths, counts, see, scale):
     """-> (o, lse) in fp64 and bounds of their errors, on the GPU.
 
-    Bounds.  A logit is an fp32 sum of D products in any order: 2^-19 of the sum of their sizes, as in cache_ref.py.  q may be held as two codes per element
-    relative to its row, 4 and 3 bits behind each other, which is exact down to 2^-14 of the row's largest element and 2^-21 of that off below: 2^-21 |q|max
-    times the sum of the sizes of the key's channels.  Both move a probability by twice as much relatively; exp2 and the fp32 sums by 2^-19.  A probability in the output
-    product may be held as two codes of 4 bits behind each other relative to the largest of its block of 32 keys: off by 2^-8 of itself, and never closer than 2^-21 of that
-    largest one.  o is rounded to bf16 (2^-8)."""
+    Bounds.  A logit is an fp32 sum of D products in any order: 2^-19 of the sum of their sizes, as in cache_ref.py.  q is held as two codes per element,
+    its row's largest brought to 2^7 ... 2^8: e4m3 (4 bits; a step of 2^-9 below 2^-6) and what that leaves in e5m2 (3 bits).  What is left of an element of at least 2^-6 is at
+    most 8 times its eighth bit, which 3 bits hold; below, at most 2^-10 is left, on steps of 2^-13: off by 2^-14, 2^-21 of the largest element.  That times the sum of the
+    sizes of the key's channels.  Both move a probability by twice as much relatively; exp2 and the fp32 sums by 2^-19.  A probability is held in the output product
+    with the largest of its block of 32 keys brought to 2^7 ... 2^8, in f16 (off by 2^-11 of itself), of that an e4m3 code (off by half a step, 2^(e-4) for 2^e ...
+    2^(e+1)) and an e4m3 code of the rest, 2^(e-4) at most: off by 2^(e-9).  Together less than 2^-8 of itself; where the second code is below 2^-6, by 2^-10, which is
+    2^-17 of the block's largest.  o is rounded to bf16 (2^-8)."""
     B, N, H, D = q.shape
     Hk, P = cache.k8.shape[1:3]
     dev = "cuda"
@@ -132,6 +134,6 @@ def attention(q, cache, table, lengths, counts, see, scale):
                     rows = [[x[i, sees[i]] @ y[sees[i]] for x, y in ((p, v), (p, v.abs()), (top, v.abs()))] for i in range(count)]
                     pv, pav, tav = (torch.stack(x) for x in zip(*rows))
                 o[b, :count, hh] = pv
-                do[b, :count, hh] = 2.0 ** -8 * pv.abs() + (2.0 ** -8 + 2 * eps + 2.0 ** -19)[:, None] * pav + 2.0 ** -21 * tav + 1e-37
+                do[b, :count, hh] = 2.0 ** -8 * pv.abs() + (2.0 ** -8 + 2 * eps + 2.0 ** -19)[:, None] * pav + 2.0 ** -17 * tav + 1e-37
                 dlse[b, hh, :count] = eps + 2.0 ** -19 + 2.0 ** -22 * lse[b, hh, :count].abs()
     return (o, lse), (do, dlse)
