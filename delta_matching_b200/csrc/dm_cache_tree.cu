@@ -10,8 +10,9 @@
 // small).  The power-of-two scale of V's block goes into P's scale byte and that of K's block into the factor of the logits.
 //
 // The key tiles of 128 tokens of all units are one flat range, divided evenly over the CTAs of one wave; pieces of cut units are joined by a second kernel.
-// Warps 0-3: queries, softmax and output (thread = TMEM lane).  Warp 4: TMA of the code tiles from the pages.  Warp 5: MMA.  At head_dim 128 two CTAs
-// share an SM (TMEM: S 0-127, O 128-255 each), at head_dim 256 one CTA has two S buffers (0-127, 128-255) and O at 256-511.
+// One CTA an SM.  Three teams of four softmax warps (thread = TMEM lane; two teams at head_dim 256) take the tiles of a unit in turn, each with an S buffer in TMEM;
+// P's codes and scale bytes lie over the S that they come from.  Of the last four warps one loads the code tiles from the pages by TMA and two issue the MMAs.  What the teams share of a row is the power of two that O counts in: it goes from team to team with the tiles, and moves so seldom
+// (fp32 takes 40 powers of two above it) that O is hardly ever rescaled.
 //
 // kCopies: where a unit has at most 64 or 32 rows, they stand twice or four times in the 128 lanes, and copy c looks after its share of a tile's blocks of 32
 // keys (P is zero in the others), with a reference, a sum and an accumulator of its own, which the CTA adds up at the end: the softmax of a tile is as much
@@ -34,21 +35,24 @@ template <int kD>
 struct TreeCfg {
   static constexpr int D = kD;
   static constexpr int kPanels = D / 128;                     // of 128 bytes, of a row of codes
-  static constexpr int kSBufs = D == 128 ? 1 : 2;
-  static constexpr int kCtasPerSm = D == 128 ? 2 : 1;
-  static constexpr int kThreads = 192;
+  static constexpr int kTeams = D == 128 ? 3 : 2;             // of four softmax warps, each with an S buffer: a tile goes to the next team
+  static constexpr int kThreads = 128 * (kTeams + 1);
+  static constexpr int kRegsSoftmax = 144, kRegsOther = 80;   // of 128 at launch (head_dim 128)
+  static_assert(D != 128 || kTeams * kRegsSoftmax + kRegsOther <= (kTeams + 1) * 128, "a split above the launch's own registers would wait for ever");
   static constexpr int kTile = 128 * D;                       // codes of K or V
-  static constexpr int kStages = 4;                           // of a tile of K or V: K and V in turn
-  static constexpr int kColO = 128 * kSBufs, kTmemCols = 256 * kPanels;
-  static constexpr int kSmemQ = 0;                            // first codes, second codes; staging of the output
+  static constexpr int kStages = D == 128 ? 10 : 4;           // of a tile of K or V: K and V in turn
+  static constexpr int kColO = 128 * kTeams;                  // TMEM: S buffers, then O
+  static constexpr int kSmemQ = 0;                            // first codes, second codes
   static constexpr int kSmemRing = 2 * kTile;
-  static constexpr int kSmemScales = kSmemRing + kStages * kTile;     // 8 tiles x (4 K scales, 4 exponents of V's)
-  static constexpr int kSmemStats = kSmemScales + 8 * 32;     // of a lane: m, l, u
-  static constexpr int kSmemRows = kSmemStats + 128 * 16;     // of a row: factor of its logits; where its output goes; by parity of the unit, whether it is marked; NaN tokens of two tiles
-  static constexpr int kSmemBars = kSmemRows + 128 * 16 + 32;
-  static constexpr int kSmemCum = kSmemBars + 256;            // 136 ints
-  static constexpr int kSmem = kSmemCum + 136 * 4 + 1024;
-  static_assert(kSmem + 1024 <= (228 * 1024) / kCtasPerSm, "shared memory of an SM");
+  static constexpr int kSmemOut = kSmemRing + kStages * kTile;        // staging of the output, 128 lanes x 64 bytes a team
+  static constexpr int kSmemStats = kSmemOut + kTeams * 8192; // by team and lane: m, l
+  static constexpr int kSmemU = kSmemStats + kTeams * 1024;   // by parity of the unit and lane: u
+  static constexpr int kSmemRows = kSmemU + 1024;              // by parity of the unit and row: factor of its logits; where its output goes; whether it is marked
+  static constexpr int kSmemScales = kSmemRows + 2 * 128 * 12;        // 8 tiles x (4 K scales, 4 exponents of V's)
+  static constexpr int kSmemNan = kSmemScales + 8 * 32;       // by S buffer: which tokens of a tile are NaN
+  static constexpr int kSmemBars = kSmemNan + 64;
+  static constexpr int kSmem = kSmemBars + 512 + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 // ------------------------------------------------------------------------------------------------ schedule
@@ -57,7 +61,7 @@ struct TreeSeq {
   int n, count;
   __device__ __forceinline__ int base() const { return n - count; }
   __device__ __forceinline__ int tiles() const { return (n + 127) / 128; }
-  __device__ __forceinline__ int row_tiles(const CacheTreeParams& p) const { return (count * p.rep + p.row_tile - 1) / p.row_tile; }
+  __device__ __forceinline__ int row_tiles(const CacheTreeParams& p) const { return (count * p.rep + p.row_tile - 1) >> p.row_shift; }
 };
 __device__ __forceinline__ TreeSeq tree_seq(const CacheTreeParams& p, int b) {
   TreeSeq s;
@@ -72,34 +76,38 @@ __device__ __forceinline__ TreeSeq tree_seq(const CacheTreeParams& p, int b) {
 __device__ __forceinline__ int tree_steps(const CacheTreeParams& p, const TreeSeq& s) {
   return s.count > 0 ? (s.tiles() + kTreeCost) * s.row_tiles(p) * p.c.Hk : 0;
 }
-// Steps before each group of sequences (128 groups, as in dm_cache_sched.cuh), and the workers that share them.  Executed by the whole CTA (at least 128
-// threads); `cum`: 129 ints + 4 of scratch.
+// Rows -> drafted token: r / rep.
+__device__ __forceinline__ int node_of(const CacheTreeParams& p, int r) { return p.rep == 1 ? r : p.rep_magic != 0 ? static_cast<int>(__umulhi(r, p.rep_magic)) : r / p.rep; }
+
+// The steps of all sequences, which the workers share evenly.  Each warp reckons for itself, a lane a group of sequences.
 struct TreeRange {
-  int total, workers, chunk;
+  int total, workers, quot, rest;
+  __device__ __forceinline__ int share(int w) const { return w * quot + static_cast<int>(static_cast<unsigned>(w) * static_cast<unsigned>(rest) / static_cast<unsigned>(workers)); }
 };
-__device__ __forceinline__ TreeRange tree_range(const CacheTreeParams& p, int* cum) {
-  const int tid = threadIdx.x, lane = tid & 31, chunk = (p.c.B + 127) / 128;
-  int incl = 0;
-  if (tid < 128) {
-    for (int i = tid * chunk; i < min(p.c.B, (tid + 1) * chunk); ++i) incl += tree_steps(p, tree_seq(p, i));
+__device__ __forceinline__ int warp_scan(int x) {
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += o;
-    }
-    if (lane == 31) cum[129 + (tid >> 5)] = incl;
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, x, off);
+    if ((threadIdx.x & 31) >= off) x += o;
   }
-  __syncthreads();
-  if (tid < 128) {
-    for (int w = 0; w < (tid >> 5); ++w) incl += cum[129 + w];
-    cum[tid + 1] = incl;
-    if (tid == 0) cum[0] = 0;
-  }
-  __syncthreads();
-  const int total = cum[128];
-  return TreeRange{total, min(p.grid, total), chunk};         // each has a step at least
+  return x;
 }
-__device__ __forceinline__ int tree_share(const TreeRange& r, int w) { return static_cast<int>(static_cast<int64_t>(w) * r.total / r.workers); }
+// Steps before and in sequences a ... of lane's group, for groups of `size` sequences from `from`, none behind `to`: the inclusive sums.
+__device__ __forceinline__ int tree_sums(const CacheTreeParams& p, int from, int to, int size) {
+  int x = 0;
+  const int first = from + (threadIdx.x & 31) * size, last = min(to, first + size);
+  for (int b = first; b < last; ++b) x += tree_steps(p, tree_seq(p, b));
+  return warp_scan(x);
+}
+__device__ __forceinline__ TreeRange tree_range(const CacheTreeParams& p, int& sums) {
+  sums = tree_sums(p, 0, p.c.B, (p.c.B + 31) / 32);
+  TreeRange r;
+  r.total = __shfl_sync(0xffffffffu, sums, 31);
+  r.workers = max(1, min(p.grid, r.total));                   // each has a step at least (where there are any)
+  r.quot = r.total / r.workers;
+  r.rest = r.total - r.quot * r.workers;
+  return r;
+}
 
 // A CTA's piece of a unit: key tiles t0 ... t1 - 1 (none where only steps of the unit's own cost fall to the CTA).
 struct TreePiece {
@@ -116,21 +124,21 @@ __device__ __forceinline__ void tree_cut(TreePiece& x, int f, int f_end) {
   x.t0 = max(0, f - x.begin - kTreeCost);
   x.t1 = max(0, x.f1 - x.begin - kTreeCost);
 }
-// The piece that begins at step f < f_end.
-__device__ __forceinline__ TreePiece tree_first(const CacheTreeParams& p, const TreeRange& r, const int* cum, int f, int f_end) {
-  int lo = 0, hi = 128;                                       // cum[lo] <= f < cum[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (cum[mid] <= f) lo = mid; else hi = mid;
-  }
+// The piece that begins at step f < f_end.  `sums`: of tree_range.
+__device__ __forceinline__ TreePiece tree_first(const CacheTreeParams& p, int sums, int f, int f_end) {
   TreePiece x;
-  int off = f - cum[lo];
-  for (x.b = lo * r.chunk;; ++x.b) {
-    x.s = tree_seq(p, x.b);
-    const int steps = tree_steps(p, x.s);
-    if (off < steps) break;
-    off -= steps;
+  int off = f, size = (p.c.B + 31) / 32, from = 0, to = p.c.B;
+  for (;;) {
+    const int lane = __ffs(__ballot_sync(0xffffffffu, sums > off)) - 1, before = __shfl_sync(0xffffffffu, sums, max(0, lane - 1));
+    if (lane > 0) off -= before;
+    from += lane * size;
+    to = min(to, from + size);
+    if (size == 1) break;
+    size = (size + 31) / 32;
+    sums = tree_sums(p, from, to, size);
   }
+  x.b = from;
+  x.s = tree_seq(p, x.b);
   const int unit_steps = x.s.tiles() + kTreeCost, unit = off / unit_steps, row_tiles = x.s.row_tiles(p);
   x.hk = unit / row_tiles;
   x.rt = unit - x.hk * row_tiles;
@@ -251,6 +259,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+}
 // Whether `x` holds for all threads of a named barrier, which they meet at.
 __device__ __forceinline__ bool all_of(int id, int nthreads, bool x) {
   uint32_t r;
@@ -260,19 +275,49 @@ __device__ __forceinline__ bool all_of(int id, int nthreads, bool x) {
 }
 
 enum TreeBar : int {
-  kFull = 0, kEmpty = 4,                    // of the ring
-  kQ = 8,                                   // queries of the unit written
-  kS = 9, kP = 11, kPv = 13,                // by S buffer: S computed, P written, P V done
-  kScales = 15,                             // of running tile g: entry g % 8
-  kTreeBars = 23,                           // behind them the TMEM slot and the abort flag
+  kFull = 0, kEmpty = 10,                   // of the ring
+  kQ = 20, kOut = 22,                       // by parity of the unit: queries written; output read from TMEM
+  kS = 24, kP = 27, kPv = 30,               // by S buffer: S computed, P written, P V done
+  kU = 33,                                  // by team and quarter of the lanes: the tile's references stand
+  kScales = 45,                             // of running tile g: entry g % 8
+  kCut = 53,                                // by team: a cut tile's values have been looked at
+  kTreeBars = 56,                           // behind them the TMEM slot, the abort flag and whether a row of the unit is marked (by parity)
 };
+
+// What the join needs of a cut unit, left by the worker that goes on with it first: its rows, and the workers that have tiles of it.
+struct TreeCut {
+  int b, hk, rt, count;                     // count 0: nothing to join
+  int first, last, slot, pad;               // slot of the first piece; worker w's behind it: 2 w
+};
+// Of worker j, whose share begins at step f with piece x.
+__device__ __forceinline__ TreeCut tree_cut_at(const TreeRange& range, const TreePiece& x, int j, int f) {
+  TreeCut y{};
+  if (j == 0 || x.begin >= f || range.share(j - 1) > x.begin) return y;      // no cut, or not the unit's first
+  auto worker_at = [&](int step) {                            // whose share it is: share(lo) <= step < share(hi)
+    int lo = j - 1, hi = range.workers;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (range.share(mid) <= step) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+  // of the tiles; workers before them have steps of the unit's own cost alone and no piece
+  y.first = worker_at(x.begin + kTreeCost);
+  y.last = worker_at(x.end() - 1);
+  y.slot = 2 * y.first + (y.first == j - 1 && range.share(j - 1) < x.begin ? 1 : 0);
+  y.b = x.b;
+  y.hk = x.hk;
+  y.rt = x.rt;
+  y.count = y.first == y.last ? 0 : x.s.count;                // whole: written by that worker
+  return y;
+}
 
 // ------------------------------------------------------------------------------------------------ main kernel
 template <int kD, int kCopies>
-__global__ void __launch_bounds__(TreeCfg<kD>::kThreads, TreeCfg<kD>::kCtasPerSm)
+__global__ void __launch_bounds__(TreeCfg<kD>::kThreads, 1)
 cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CacheTreeParams p) {
   using C = TreeCfg<kD>;
-  constexpr int D = C::D, kRows = 128 / kCopies;              // rows of a unit
+  constexpr int D = C::D, kTeams = C::kTeams, kRows = 128 / kCopies;      // rows of a unit
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023) & ~1023u) - raw);
@@ -280,19 +325,27 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kSmemBars);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kTreeBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kTreeBars + 1);
-  int* cum = reinterpret_cast<int*>(smem + C::kSmemCum);
+  volatile int* any_marked = abort_flag + 1;
   float* scales = reinterpret_cast<float*>(smem + C::kSmemScales);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float* factors = reinterpret_cast<float*>(smem + C::kSmemRows);
+  int* out_rows = reinterpret_cast<int*>(smem + C::kSmemRows) + 256;
+  volatile int* marks = reinterpret_cast<volatile int*>(smem + C::kSmemRows) + 512;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, role = warp - 4 * kTeams;       // of the last four warps
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(bars + kFull + i, 1);
       mbar_init(bars + kEmpty + i, 1);
     }
-    mbar_init(bars + kQ, 4);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(bars + kQ + i, 4 * kTeams);
+      mbar_init(bars + kOut + i, 4 * kTeams);
+    }
+    for (int i = 0; i < kTeams; ++i) {
       mbar_init(bars + kS + i, 1);
       mbar_init(bars + kP + i, 4);
       mbar_init(bars + kPv + i, 1);
+      for (int q = 0; q < 4; ++q) mbar_init(bars + kU + 4 * i + q, 1);
+      mbar_init(bars + kCut + i, 4);
     }
     for (int i = 0; i < 8; ++i) mbar_init(bars + kScales + i, 1);
     *abort_flag = 0;
@@ -300,30 +353,34 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
-  if (warp == 5) {
-    tmem_alloc(tmem_slot, C::kTmemCols);
+  if (role == 1) {
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
     tc_fence_before();
   }
   grid_dep_wait();
-  const TreeRange range = tree_range(p, cum);                 // its barriers publish the mbarriers and the TMEM slot too
+  int sums;
+  const TreeRange range = tree_range(p, sums);
+  __syncthreads();                                            // the mbarriers and the TMEM slot are there
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int worker = blockIdx.x;
   auto bar = [&](int i) { return smem_u32(bars + i); };
-  // of running tile g: its S buffer, and the parity of that buffer's barriers
-  auto buf_of = [&](int g) { return C::kSBufs == 2 ? g & 1 : 0; };
-  auto parity_of = [&](int g) { return static_cast<uint32_t>(C::kSBufs == 2 ? g >> 1 : g) & 1u; };
+  // running tile g goes to team and S buffer g % kTeams, whose barriers' phase it is
+  auto phase_of = [&](int g) { return static_cast<uint32_t>(g / kTeams) & 1u; };
   bool ok = true;
 
-  if (worker < range.workers) {
-    const int f_begin = tree_share(range, worker), f_end = tree_share(range, worker + 1);
-    TreePiece x = tree_first(p, range, cum, f_begin, f_end);
-    if (warp == 4) {
+  if (worker < range.workers && range.total > 0) {
+    const int f_begin = range.share(worker), f_end = range.share(worker + 1);
+    TreePiece x = tree_first(p, sums, f_begin, f_end);
+    if (role >= 0 && D == 128) reg_dec<C::kRegsOther>();
+    if (role == 0) {
       // ---------------------------------------------------------------------------------------- TMA: code tiles and their scales
-      // Lane i < 4 looks after block i of a tile.  A tile's pages are asked for two tiles ahead of its loads and its scales one tile ahead.
-      struct Ahead {
-        bool live, held;
+      // Eight tiles at a time, a lane a block: a batch's pages are asked for two batches ahead of its loads and its scales one ahead (a tile takes less than the
+      // two loads, one behind the other, that lead to its codes).
+      struct Batch {
+        int tiles;
+        bool held;
         int hk, page, sub;
         float ks, vs;
       };
@@ -331,53 +388,68 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       int t = x.t0;
       bool more = true;                                       // (x, t) is the next tile to be looked up
       auto look_up = [&]() {
-        Ahead a{};
-        while (more && t >= x.t1) {
-          more = tree_next(p, x, f_end);
-          t = x.t0;
+        Batch a{};
+        int b = 0, blk = 0;
+#pragma unroll 1
+        for (; a.tiles < 8; ++a.tiles) {
+          while (more && t >= x.t1) {
+            more = tree_next(p, x, f_end);
+            t = x.t0;
+          }
+          if (!more) break;
+          if (lane >> 2 == a.tiles) {
+            blk = 4 * t + (lane & 3);
+            a.held = blk * 32 < x.s.n;
+            a.hk = x.hk;
+            b = x.b;
+          }
+          ++t;
         }
-        a.live = more;
-        if (!more) return a;
-        const int blk = 4 * t++ + lane;
-        a.held = lane < 4 && blk * 32 < x.s.n;
-        a.hk = x.hk;
         if (a.held) {
           const int entry = blk / bpp;
           a.sub = blk - entry * bpp;
-          a.page = __ldg(p.c.table + x.b * p.c.t_row + entry);
+          a.page = __ldg(p.c.table + b * p.c.t_row + entry);
         }
         return a;
       };
-      auto ask_scales = [&](Ahead& a) {
+      auto ask_scales = [&](Batch& a) {
         if (!a.held) return;
         a.page = max(0, checked_page(p.c, a.page));
         const int64_t at = a.page * p.c.s_page + a.hk * p.c.s_head + a.sub;
         a.ks = __ldg(p.c.ks + at);
         a.vs = __ldg(p.c.vs + at);
       };
-      int j = 0;                                              // running stage
-      Ahead now = look_up(), next = look_up();
+      int g = 0, j = 0;                                       // running tile, running stage
+      Batch now = look_up();
       ask_scales(now);
-      for (int g = 0; now.live && ok; ++g) {
-        const Ahead after = look_up();
+      Batch next = look_up();
+      while (now.tiles > 0 && ok) {
         ask_scales(next);
-        if (lane < 4) {
-          scales[(g & 7) * 8 + lane] = now.ks;                // zero where there is no block
-          scales[(g & 7) * 8 + 4 + lane] = static_cast<float>(static_cast<int>(scale_to_sb(now.vs)) - 127);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
-        const int boxes = __popc(__ballot_sync(0xffffffffu, now.held)) * C::kPanels;
+        const Batch after = look_up();
+        const uint32_t held = __ballot_sync(0xffffffffu, now.held);
 #pragma unroll 1
-        for (int kv = 0; kv < 2 && ok; ++kv, ++j) {
-          const int st = j % C::kStages;
-          if (j >= C::kStages && !(ok = wait_warp(bar(kEmpty + st), (j / C::kStages - 1) & 1, abort_flag))) break;
-          if (lane == 0) mbar_expect_tx(bars + kFull + st, boxes * 4096);
-          __syncwarp();
-          if (now.held) {
+        for (int i = 0; i < now.tiles && ok; ++i, ++g) {
+          const int boxes = __popc(held >> (4 * i) & 15u) * C::kPanels;
+          const bool mine = lane >> 2 == i;
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv, ++j) {
+            const int st = j % C::kStages;
+            if (j >= C::kStages && !(ok = wait_warp(bar(kEmpty + st), (j / C::kStages - 1) & 1, abort_flag))) break;
+            if (lane == 0) mbar_expect_tx(bars + kFull + st, boxes * 4096);
+            __syncwarp();
+            if (mine && now.held) {
 #pragma unroll
-            for (int c = 0; c < C::kPanels; ++c)
-              tma_load_4d(sbase + C::kSmemRing + st * C::kTile + c * 16384 + lane * 4096, kv ? &tv : &tk, bar(kFull + st), 128 * c, now.sub * 32, now.hk, now.page);
+              for (int c = 0; c < C::kPanels; ++c)
+                tma_load_4d(sbase + C::kSmemRing + st * C::kTile + c * 16384 + (lane & 3) * 4096, kv ? &tv : &tk, bar(kFull + st), 128 * c, now.sub * 32, now.hk, now.page);
+            }
+            if (kv == 0) {
+              if (mine) {
+                scales[(g & 7) * 8 + (lane & 3)] = now.ks;    // zero where there is no block
+                scales[(g & 7) * 8 + 4 + (lane & 3)] = static_cast<float>(static_cast<int>(scale_to_sb(now.vs)) - 127);
+              }
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
+            }
           }
         }
         now = next;
@@ -389,160 +461,182 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         for (int k = 1; k <= C::kStages; ++k)
           if (j >= k) wait_or_abort(bar(kFull + (j - k) % C::kStages), ((j - k) / C::kStages) & 1, abort_flag);
       }
-    } else if (warp == 5) {
-      // ---------------------------------------------------------------------------------------- MMA
+    } else if (role == 1) {
+      // ---------------------------------------------------------------------------------------- MMA: S
+      // (an issuing warp for each product: a chain of eight holds its warp until it is nearly done)
       if (elect_one()) {
         constexpr uint32_t kIdescFirst = idesc_f8(128, 128, false, false), kIdescSecond = kIdescFirst | (1u << 7);     // A: e4m3; e5m2
         const uint32_t q_lo = desc_lo(sbase + C::kSmemQ), ring_lo = desc_lo(sbase + C::kSmemRing);
-        int g = 0, units = 0;                                 // running tile
-        // S of running tile h, behind all that read its buffer
-        auto issue_s = [&](int h) -> bool {
-          const int st = 2 * h % C::kStages;
-          if (!wait_or_abort(bar(kFull + st), (2 * h / C::kStages) & 1, abort_flag)) return false;
-          if (h >= C::kSBufs && !wait_or_abort(bar(kPv + buf_of(h)), parity_of(h - C::kSBufs), abort_flag)) return false;
-          tc_fence_after();
-          const uint32_t k_lo = ring_lo + st * (C::kTile >> 4), d = tmem + 128 * buf_of(h);
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
-            mma_f8_ss(d, q_lo + off, k_lo + off, kIdescFirst, k > 0);
-            mma_f8_ss(d, q_lo + (C::kTile >> 4) + off, k_lo + off, kIdescSecond, true);
-          }
-          tc_commit(bars + kS + buf_of(h));
-          tc_commit(bars + kEmpty + st);
-          return true;
-        };
+        int g = 0, units = 0;                                 // running tile, running unit
         do {
           if (x.t0 >= x.t1) continue;
-          const int n = x.t1 - x.t0;
-          if (!(ok = wait_or_abort(bar(kQ), units++ & 1, abort_flag))) break;
-          if (!(ok = issue_s(g))) break;
-          for (int i = 0; i < n && ok; ++i, ++g) {
-            if (C::kSBufs == 2 && i + 1 < n && !(ok = issue_s(g + 1))) break;       // the next S, while the softmax is at this one
-            const int st = (2 * g + 1) % C::kStages, held = min(4, (x.s.n - 128 * (x.t0 + i) + 31) / 32);        // blocks of the tile
-            if (!(ok = wait_or_abort(bar(kP + buf_of(g)), parity_of(g), abort_flag) && wait_or_abort(bar(kFull + st), ((2 * g + 1) / C::kStages) & 1, abort_flag))) break;
+          ok = wait_or_abort(bar(kQ + (units & 1)), (units >> 1) & 1, abort_flag);
+          for (int t = x.t0; t < x.t1 && ok; ++t, ++g) {
+            const int st = 2 * g % C::kStages, buf = g % kTeams;
+            // K, and the buffer: behind the products that read P and its scale bytes from it
+            if (g >= kTeams && !(ok = wait_or_abort(bar(kPv + buf), phase_of(g - kTeams), abort_flag))) break;
+            if (!(ok = wait_or_abort(bar(kFull + st), (2 * g / C::kStages) & 1, abort_flag))) break;
             tc_fence_after();
-            const uint32_t v_lo = ring_lo + st * (C::kTile >> 4), s = tmem + 128 * buf_of(g);
+            const uint32_t k_lo = ring_lo + st * (C::kTile >> 4), d = tmem + 128 * buf;
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+              const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+              mma_f8_ss(d, q_lo + off, k_lo + off, kIdescFirst, k > 0);
+              mma_f8_ss(d, q_lo + (C::kTile >> 4) + off, k_lo + off, kIdescSecond, true);
+            }
+            tc_commit(bars + kS + buf);
+            tc_commit(bars + kEmpty + st);
+          }
+          ++units;
+        } while (ok && tree_next(p, x, f_end));
+        if (!ok) raise_abort(abort_flag, p.c.status, kStatusTimeoutMma + kInCache);
+      }
+    } else if (role == 2) {
+      // ---------------------------------------------------------------------------------------- MMA: P V
+      if (elect_one()) {
+        const uint32_t ring_lo = desc_lo(sbase + C::kSmemRing);
+        int g = 0, units = 0;
+        do {
+          if (x.t0 >= x.t1) continue;
+          if (units > 0) ok = wait_or_abort(bar(kOut + ((units - 1) & 1)), ((units - 1) >> 1) & 1, abort_flag);      // O has been read
+          for (int t = x.t0; t < x.t1 && ok; ++t, ++g) {
+            const int st = (2 * g + 1) % C::kStages, buf = g % kTeams, held = min(4, (x.s.n - 128 * t + 31) / 32);     // blocks of the tile
+            if (!(ok = wait_or_abort(bar(kP + buf), phase_of(g), abort_flag) && wait_or_abort(bar(kFull + st), ((2 * g + 1) / C::kStages) & 1, abort_flag))) break;
+            tc_fence_after();
+            const uint32_t v_lo = ring_lo + st * (C::kTile >> 4), s = tmem + 128 * buf;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               if (k >= held) break;                           // P is zero there and V is not loaded
 #pragma unroll
               for (int c = 0; c < C::kPanels; ++c) {
                 mma_mxf8_ts(tmem + C::kColO + 128 * c, s + 32 * k, v_lo + c * (16384 >> 4) + k * (4096 >> 4), idesc_mxf8(128, 128, false, true, k, k), s + 16, s + 20,
-                            i > 0 || k > 0);
+                            t > x.t0 || k > 0);
                 mma_mxf8_ts(tmem + C::kColO + 128 * c, s + 32 * k + 8, v_lo + c * (16384 >> 4) + k * (4096 >> 4), idesc_mxf8(128, 128, false, true, k, k), s + 16, s + 20,
                             true);
               }
             }
             tc_commit(bars + kEmpty + st);
-            tc_commit(bars + kPv + buf_of(g));
-            if (C::kSBufs == 1 && i + 1 < n && !(ok = issue_s(g + 1))) break;
+            tc_commit(bars + kPv + buf);
           }
+          ++units;
         } while (ok && tree_next(p, x, f_end));
         if (!ok) raise_abort(abort_flag, p.c.status, kStatusTimeoutMma + kInCache);
       }
+    } else if (role == 3) {
+      const TreeCut y = tree_cut_at(range, x, worker, f_begin);
+      if (lane == 0) reinterpret_cast<TreeCut*>(p.cuts)[worker] = y;
     } else {
-      // ---------------------------------------------------------------------------------------- queries, softmax, output
-      const int row = tid & (kRows - 1);                      // of the unit
-      const int copy = tid / kRows;                           // looks after blocks copy * 4 / kCopies ... of a tile
+      if (D == 128) reg_inc<C::kRegsSoftmax>();
+      // ---------------------------------------------------------------------------------------- softmax, output
+      const int team = warp >> 2, quarter = warp & 3, in_tile = tid & 127;
+      const int row = in_tile & (kRows - 1);                  // of the unit
+      const int copy = in_tile / kRows;                       // looks after blocks copy * 4 / kCopies ... of a tile
       constexpr int kBlocks = 4 / kCopies;
-      const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-      float4* stats = reinterpret_cast<float4*>(smem + C::kSmemStats);
-      float* factors = reinterpret_cast<float*>(smem + C::kSmemRows);
-      int* out_rows = reinterpret_cast<int*>(smem + C::kSmemRows) + 128;
-      volatile uint32_t* nan_tokens = reinterpret_cast<volatile uint32_t*>(smem + C::kSmemRows) + 512;      // of a tile, by its parity
-      int g = 0, units = 0;                                   // running tile, running unit
-      do {
-        if (x.t0 >= x.t1) continue;
-        // (by parity: a warp may be at the next unit's queries while another looks at this one's marks)
-        volatile int* marks = reinterpret_cast<volatile int*>(smem + C::kSmemRows) + 256 + 128 * (units++ & 1);
-        // Queries, two codes an element, in the layout of the 128-byte swizzle.  A row's lanes take eight elements each.
-        {
-          constexpr int kLanes = D / 8, kPer = 32 / kLanes, kOwn = kRows / 4, kBatch = kOwn / kPer < 4 ? kOwn / kPer : 4;
-          const int l = lane % kLanes;
-#pragma unroll 1
-          for (int r0 = 0; r0 < kOwn; r0 += kBatch * kPer) {
-            uint4 w[kBatch];
-            int at_row[kBatch];
+      const int c0 = kCopies == 1 ? 0 : copy * kBlocks;
+      const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16, t_s = tmem + lanes + 128 * team, t_o = tmem + lanes + C::kColO;
+      float2* stats = reinterpret_cast<float2*>(smem + C::kSmemStats);
+      volatile uint32_t* nan_tokens = reinterpret_cast<volatile uint32_t*>(smem + C::kSmemNan) + 4 * team;
+      // Queries: two codes an element, in the layout of the 128-byte swizzle.  A row's lanes take eight elements each, the warps of all teams the rows in turn; asked
+      // for ahead.
+      constexpr int kLanes = D / 8, kPer = 32 / kLanes, kPasses = (kRows / kPer + 4 * kTeams - 1) / (4 * kTeams);
+      const int ql = lane % kLanes;
+      uint4 asked[kPasses];
+      auto ask_queries = [&](const TreePiece& y) {
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const int r = warp * kOwn + r0 + k * kPer + lane / kLanes, unit_row = x.rt * kRows + r, i = unit_row / p.rep, head = x.hk * p.rep + unit_row - i * p.rep;
-              w[k] = make_uint4(0, 0, 0, 0);
-              at_row[k] = -1;
-              if (i < x.s.count) {
-                w[k] = __ldg(reinterpret_cast<const uint4*>(p.q + x.b * p.q_sb + i * p.q_sn + head * p.q_sh) + l);
-                at_row[k] = (x.b * p.N + i) * p.H + head;
-              }
+        for (int k = 0; k < kPasses; ++k) {
+          const int r = (warp + 4 * kTeams * k) * kPer + lane / kLanes, unit_row = y.rt * kRows + r, i = node_of(p, unit_row), head = y.hk * p.rep + unit_row - i * p.rep;
+          asked[k] = make_uint4(0, 0, 0, 0);
+          if (r < kRows && i < y.s.count) asked[k] = __ldg(reinterpret_cast<const uint4*>(p.q + y.b * p.q_sb + i * p.q_sn + head * p.q_sh) + ql);
+        }
+      };
+      auto put_queries = [&](const TreePiece& y, int parity) {
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          const int r = (warp + 4 * kTeams * k) * kPer + lane / kLanes;
+          const uint32_t v[4] = {asked[k].x, asked[k].y, asked[k].z, asked[k].w};
+          // the largest size, as bits: NaN and infinities are above all others
+          uint32_t top = __vmaxu2(__vmaxu2(v[0] & 0x7FFF7FFFu, v[1] & 0x7FFF7FFFu), __vmaxu2(v[2] & 0x7FFF7FFFu, v[3] & 0x7FFF7FFFu));
+          top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const uint32_t eb = min(254u, max(14u, top >> 7));
+          const float up = sb_to_scale(261u - eb);            // largest element to [2^7, 2^8)
+          uint32_t first[2], second[2];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = __uint_as_float(v[e] << 16) * up, b = __uint_as_float(v[e] & 0xFFFF0000u) * up;
+            const uint32_t code = cvt_e4m3x2(a, b);
+            const float2 back = f16x2_to_float2(e4m3_lo_f16x2(code));
+            const uint32_t rest = cvt_e5m2x2(a - back.x, b - back.y);
+            first[e >> 1] = (e & 1) ? first[e >> 1] | code << 16 : code;
+            second[e >> 1] = (e & 1) ? second[e >> 1] | rest << 16 : rest;
+          }
+          if (r < kRows) {
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) {
+              const uint32_t at = sbase + C::kSmemQ + (ql >> 4) * 16384 + (r + c * kRows) * 128 + ((((ql & 15) >> 1) ^ (r & 7)) << 4) + (ql & 1) * 8;
+              sts_f2(at, __uint_as_float(first[0]), __uint_as_float(first[1]));
+              sts_f2(at + C::kTile, __uint_as_float(second[0]), __uint_as_float(second[1]));
             }
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const int r = warp * kOwn + r0 + k * kPer + lane / kLanes;
-              const uint32_t v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-              // the largest size, as bits: NaN and infinities are above all others
-              uint32_t top = __vmaxu2(__vmaxu2(v[0] & 0x7FFF7FFFu, v[1] & 0x7FFF7FFFu), __vmaxu2(v[2] & 0x7FFF7FFFu, v[3] & 0x7FFF7FFFu));
-              top = max(top & 0xFFFFu, top >> 16);
-#pragma unroll
-              for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-              const uint32_t eb = min(254u, max(14u, top >> 7));
-              const float up = sb_to_scale(261u - eb);        // largest element to [2^7, 2^8)
-              uint32_t first[2], second[2];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float a = __uint_as_float(v[e] << 16) * up, b = __uint_as_float(v[e] & 0xFFFF0000u) * up;
-                const uint32_t code = cvt_e4m3x2(a, b);
-                const float2 back = f16x2_to_float2(e4m3_lo_f16x2(code));
-                const uint32_t rest = cvt_e5m2x2(a - back.x, b - back.y);
-                first[e >> 1] = (e & 1) ? first[e >> 1] | code << 16 : code;
-                second[e >> 1] = (e & 1) ? second[e >> 1] | rest << 16 : rest;
-              }
-#pragma unroll
-              for (int c = 0; c < kCopies; ++c) {
-                const uint32_t at = sbase + C::kSmemQ + (l >> 4) * 16384 + (r + c * kRows) * 128 + ((((l & 15) >> 1) ^ (r & 7)) << 4) + (l & 1) * 8;
-                sts_f2(at, __uint_as_float(first[0]), __uint_as_float(first[1]));
-                sts_f2(at + C::kTile, __uint_as_float(second[0]), __uint_as_float(second[1]));
-              }
-              if (l == 0) {                                   // of a row of NaN or infinities the factor is NaN
-                factors[r] = top >= 0x7F80u ? CUDART_NAN_F : sb_to_scale(eb - 7u) * p.scale * kLog2e;
-                out_rows[r] = at_row[k];
-                marks[r] = 0;
-              }
+            if (ql == 0) {                                    // of a row of NaN or infinities the factor is NaN
+              const int unit_row = y.rt * kRows + r, i = node_of(p, unit_row);
+              factors[128 * parity + r] = top >= 0x7F80u ? CUDART_NAN_F : sb_to_scale(eb - 7u) * p.scale * kLog2e;
+              out_rows[128 * parity + r] = i < y.s.count ? (y.b * p.N + i) * p.H + y.hk * p.rep + unit_row - i * p.rep : -1;
+              marks[128 * parity + r] = 0;
             }
           }
-          fence_async_smem();
-          bar_sync(1, 128);
-          if (lane == 0) mbar_arrive(bars + kQ);
         }
-        const int unit_row = x.rt * kRows + row, node = unit_row / p.rep;
+        if (tid == 0) any_marked[parity] = 0;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kQ + parity);
+      };
+      auto to_tiles = [&](TreePiece& y) {                     // on to a piece that has some
+        while (y.t0 >= y.t1)
+          if (!tree_next(p, y, f_end)) return false;
+        return true;
+      };
+      bool live = to_tiles(x);
+      if (live) {
+        ask_queries(x);
+        put_queries(x, 0);
+      }
+      int g0 = 0, units = 0, cuts = 0;                        // running tile that the unit begins with, running unit; cut tiles of the team
+      while (live) {
+        const int parity = units & 1, n_tiles = x.t1 - x.t0;
+        volatile float* u_at = reinterpret_cast<volatile float*>(smem + C::kSmemU) + 128 * parity + in_tile;
+        ok = wait_warp(bar(kQ + parity), (units >> 1) & 1, abort_flag);
+        const int unit_row = x.rt * kRows + row, node = node_of(p, unit_row);
         const bool real = node < x.s.count;
         const bool idle = !__any_sync(0xffffffffu, real);     // a warp of rows that are none
         const uint32_t* seen = p.seen + x.b * p.s_sb + static_cast<int64_t>(min(node, x.s.count - 1)) * p.s_sn;
-        const float f = factors[row];
-        // Of the row, whole numbers: m, the reference of the sum l; u, that of the products of a probability and its V scale, in which O counts.  They
-        // move only when a row's logits exceed them by more than 2^kReach.
-        float m = kNone, u = kNone, l = 0.f;
+        const float f = factors[128 * parity + row];
+        // Of the row, whole numbers: m, the reference of this team's sum l; u, that of the products of a probability and its V scale, in which O counts and
+        // which goes from team to team with the tiles.  They move only when a row's logits exceed them by more than 2^kReach.
+        float m = kNone, l = 0.f;
         bool marked = false;
         // One key tile.  kCut: some row does not see all its keys (a compile-time variant: no select per element elsewhere).
-        auto tile = [&](int t, auto cut_tag) -> bool {
+        auto tile = [&](int g, int t, auto cut_tag) -> bool {
           constexpr bool kCut = decltype(cut_tag)::value;
-          const uint32_t entry = sbase + C::kSmemScales + (g & 7) * 32, t_s = tmem + lanes + 128 * buf_of(g);
-          const int c0 = kCopies == 1 ? 0 : copy * kBlocks;
-          uint32_t s_buf[2][32];
-          tmem_ld32(t_s + 32 * c0, s_buf[0]);
+          const uint32_t entry = sbase + C::kSmemScales + (g & 7) * 32;
           float kb[kBlocks], ev[kBlocks], sums[kBlocks];
-#pragma unroll
+          constexpr int kUnroll = kCut ? 1 : kBlocks;
+#pragma unroll kUnroll
           for (int c = 0; c < kBlocks; ++c) {
+            uint32_t s[32];
+            tmem_ld32(t_s + 32 * (c0 + c), s);
             const float fc = f * lds_f(entry + 4 * (c0 + c));
             ev[c] = lds_f(entry + 16 + 4 * (c0 + c));
-            tmem_wait_ld();
-            if (c < kBlocks - 1) tmem_ld32(t_s + 32 * (c0 + c + 1), s_buf[(c + 1) & 1]);
-            uint32_t (&s)[32] = s_buf[c & 1];
             uint32_t sees = 0xffffffffu;
             if (kCut) {
               sees = real ? seen_keys(seen, node, 128 * t + 32 * (c0 + c) - x.s.base()) : 0u;
+              marked |= (sees & nan_tokens[c0 + c]) != 0u;
+            }
+            tmem_wait_ld();
+            if (kCut) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (!((sees >> e) & 1u)) s[e] = 0xff800000u;
-              marked |= (sees & nan_tokens[4 * (g & 1) + c0 + c]) != 0u;
             }
             float2 s2[16];
 #pragma unroll
@@ -583,31 +677,36 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             top_u = fmaxf(top_u, kb[c] + ev[c]);
           }
           marked |= fabsf(top) > kExact && top > kNone;
-          const bool moves = top > m + kReach || top_u > u + kReach;
-          if (__any_sync(0xffffffffu, moves)) {
-            float keep = 1.f;
-            if (moves) {
-              l *= ex2_approx(m - top);
-              keep = ex2_approx(u - top_u);
-              m = top;
-              u = top_u;
-            }
-            if (t > x.t0) {
-              if (C::kSBufs == 2) {                           // (with one buffer this S came behind those products)
-                if (!wait_warp(bar(kPv + buf_of(g - 1)), parity_of(g - 1), abort_flag)) return false;
-                tc_fence_after();
-              }
+          if (top > m + kReach) {
+            l *= ex2_approx(m - top);
+            m = top;
+          }
+          // the tile before this one, another team's, has its u
+          if (g > 0 && !wait_warp(bar(kU + 4 * ((g - 1) % kTeams) + quarter), phase_of(g - 1), abort_flag)) return false;
+          float u_old = kNone;
+          if (g > g0) u_old = *u_at;
+          float u = u_old;
+          if (__any_sync(0xffffffffu, top_u > u_old + kReach)) {
+            if (top_u > u_old + kReach) u = top_u;
+            if (g > g0) {
+              const float keep = ex2_approx(u_old - u);
+              // O stands still between the products of the last tile and those of this one
+              if (!wait_warp(bar(kPv + (g - 1) % kTeams), phase_of(g - 1), abort_flag)) return false;
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
-                tmem_ld32(tmem + lanes + C::kColO + 32 * c, o);
+                tmem_ld32(t_o + 32 * c, o);
                 tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                tmem_st32(tmem + lanes + C::kColO + 32 * c, o);
+                tmem_st32(t_o + 32 * c, o);
               }
             }
           }
+          if (u != u_old || g == g0) *u_at = u;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + kU + 4 * team + quarter);
           uint32_t word = 0x7F7F7F7Fu;                        // scale bytes of P's codes, 2^(kb + ev - u - 8)
 #pragma unroll
           for (int c = 0; c < kBlocks; ++c) {
@@ -620,19 +719,18 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           tmem_st8(t_s + 16, words);
           return true;
         };
-        for (int t = x.t0; t < x.t1; ++t, ++g) {
-          ok = wait_warp(bar(kScales + (g & 7)), (g >> 3) & 1, abort_flag) && wait_warp(bar(kS + buf_of(g)), parity_of(g), abort_flag);
-          if (!ok) break;
-          tc_fence_after();
+        for (int g = g0 + (team + kTeams - g0 % kTeams) % kTeams; ok && g < g0 + n_tiles; g += kTeams) {
+          const int t = x.t0 + g - g0;
+          ok = wait_warp(bar(kScales + (g & 7)), (g >> 3) & 1, abort_flag) && wait_warp(bar(kS + team), phase_of(g), abort_flag);
           const bool cut = 128 * (t + 1) > x.s.base();
           if (cut) {
             // V's slots behind the length hold anything, and a drafted token may be NaN, which only the rows that see it are to meet: zeros in the place of both, or
             // they would come through the products with P's zeros.  Which tokens were NaN is left to the rows.  A thread a token.
-            const int st = (2 * g + 1) % C::kStages, j = 128 * t + tid;
-            ok = wait_warp(bar(kFull + st), ((2 * g + 1) / C::kStages) & 1, abort_flag);
+            const int st = (2 * g + 1) % C::kStages, j = 128 * t + in_tile;
+            if (ok) ok = wait_warp(bar(kFull + st), ((2 * g + 1) / C::kStages) & 1, abort_flag);
             bool nan = false;
-            if (ok && j >= x.s.base() && 128 * t + warp * 32 < x.s.n) {         // in a block that is there
-              const uint32_t at = sbase + C::kSmemRing + st * C::kTile + tid * 128;
+            if (ok && j >= x.s.base() && 128 * t + quarter * 32 < x.s.n) {      // in a block that is there
+              const uint32_t at = sbase + C::kSmemRing + st * C::kTile + in_tile * 128;
               auto piece = [&](int y) { return at + (y >> 3) * 16384 + (((y ^ lane) & 7) << 4); };      // lanes on different banks
               uint32_t found = 0;
 #pragma unroll
@@ -648,198 +746,202 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
               nan = found != 0 && j < x.s.n;
             }
             const uint32_t nans = __ballot_sync(0xffffffffu, nan);
-            if (lane == 0) nan_tokens[4 * (g & 1) + warp] = nans;
-            if (!(ok = all_of(1, 128, ok))) break;
+            if (lane == 0) {
+              nan_tokens[quarter] = nans;                     // (the team's last cut tile is done with: its P has arrived)
+              mbar_arrive(bars + kCut + team);
+            }
+            if (ok) ok = wait_warp(bar(kCut + team), cuts & 1, abort_flag);
+            ++cuts;
           }
-          if (!idle && !(ok = cut ? tile(t, std::true_type{}) : tile(t, std::false_type{}))) break;
+          if (!ok) break;
+          tc_fence_after();
+          if (idle) {
+            if (lane == 0) mbar_arrive(bars + kU + 4 * team + quarter);
+          } else if (!(ok = cut ? tile(g, t, std::true_type{}) : tile(g, t, std::false_type{}))) {
+            break;
+          }
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bars + kP + buf_of(g));
+          if (lane == 0) mbar_arrive(bars + kP + team);
         }
-        // (the four warps give up together: barriers follow)
-        if (ok) ok = wait_warp(bar(kPv + buf_of(g - 1)), parity_of(g - 1), abort_flag);
-        if (!(ok = all_of(1, 128, ok))) break;
+        g0 += n_tiles;
+        TreePiece next = x;
+        bool more = tree_next(p, next, f_end);
+        if (more) more = to_tiles(next);
+        if (more) ask_queries(next);
+        // Output, by all teams: over the teams and copies of a row, the largest references and the sum; each lane's values count w of it.
+        if (ok) ok = wait_warp(bar(kPv + (g0 - 1) % kTeams), phase_of(g0 - 1), abort_flag);
+        stats[128 * team + in_tile] = make_float2(m, l);
+        if (real && marked) {
+          marks[128 * parity + row] = 1;
+          any_marked[parity] = 1;
+        }
+        if (!(ok = all_of(4, 128 * kTeams, ok))) break;
         tc_fence_after();
-        // Output.  Over the copies of a row: the largest references, the sum; each lane's values count w of it.
+        if (more) put_queries(next, parity ^ 1);              // all S of this unit have been computed; those of the next run under the output
         const bool whole = x.whole();
-        stats[tid] = make_float4(m, l, u, 0.f);
-        if (kCopies > 1) bar_sync(1, 128);
-        float m_all = m, u_all = u, l_all = l, w = 1.f;
-        if (kCopies > 1) {
-          float4 st[kCopies];
+        float m_all = kNone, u_all = kNone, l_all = 0.f;
 #pragma unroll
-          for (int c = 0; c < kCopies; ++c) {
-            st[c] = stats[row + c * kRows];
-            m_all = fmaxf(m_all, st[c].x);
-            u_all = fmaxf(u_all, st[c].z);
-          }
-          l_all = 0.f;
+        for (int c = 0; c < kCopies; ++c) {
+          u_all = fmaxf(u_all, *(u_at - in_tile + row + c * kRows));
 #pragma unroll
-          for (int c = 0; c < kCopies; ++c) l_all = fmaf(st[c].y, ex2_approx(st[c].x - m_all), l_all);
-          w = ex2_approx(u - u_all);
+          for (int y = 0; y < kTeams; ++y) m_all = fmaxf(m_all, stats[128 * y + row + c * kRows].x);
         }
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c)
+#pragma unroll
+          for (int y = 0; y < kTeams; ++y) {
+            const float2 st = stats[128 * y + row + c * kRows];
+            l_all = fmaf(st.y, ex2_approx(st.x - m_all), l_all);
+          }
+        const float w = ex2_approx(*u_at - u_all);
         // (in two factors: what V's scales leave may be beyond either's range)
         const float d_all = u_all - m_all, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
         const float w1 = whole ? w * exp2f(d1) : w, w2 = whole ? exp2f(d_all - d1) / l_all : 1.f;
         const int slot = 2 * worker + (x.f0 == f_begin ? 0 : 1);
+        // 16 columns at a time, through shared memory: four lanes a row, eight rows a warp at a time; 16-byte pieces XORed with the lane
+        const uint32_t stage = sbase + C::kSmemOut + team * 8192;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          const uint32_t stage = sbase + C::kSmemQ + (c & 1) * 16384;         // 128 lanes x 128 bytes, 16-byte pieces XORed with the lane
-          uint32_t o[32];
-          tmem_ld32(tmem + lanes + C::kColO + 32 * c, o);
+        for (int c = team; c < D / 16; c += kTeams) {
+          uint32_t o[16];
+          tmem_ld16(t_o + 16 * c, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float4 y = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-            y = make_float4(y.x * w1 * w2, y.y * w1 * w2, y.z * w1 * w2, y.w * w1 * w2);
-            sts_u4(stage + tid * 128 + ((e ^ (lane & 7)) << 4), __float_as_uint(y.x), __float_as_uint(y.y), __float_as_uint(y.z), __float_as_uint(y.w));
-          }
-          if (kCopies > 1) bar_sync(1, 128);
-          else __syncwarp();
-          // eight lanes a row, four rows a warp at a time
+          for (int e = 0; e < 4; ++e) {
+            float y[4];
 #pragma unroll
-          for (int k = 0; k < 8 / kCopies; ++k) {
-            const int r = (kCopies == 1 ? warp * 32 : warp * (kRows / 4)) + 4 * k + (lane >> 3), piece = lane & 7;
-            float4 y = lds_f4(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+            for (int k = 0; k < 4; ++k) y[k] = __uint_as_float(o[4 * e + k]) * w1 * w2;
+            sts_u4(stage + in_tile * 64 + ((e ^ ((lane >> 1) & 3)) << 4), __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+          }
+          if (kCopies > 1) bar_sync(1 + team, 128);
+          else __syncwarp();
+          const int piece = lane & 3;
+#pragma unroll
+          for (int k = 0; k < 4 / kCopies; ++k) {
+            const int r = quarter * (kRows / 4) + 8 * k + (lane >> 2);
+            float4 y = lds_f4(stage + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
 #pragma unroll
             for (int cc = 1; cc < kCopies; ++cc) {
-              const float4 z = lds_f4(stage + (r + cc * kRows) * 128 + ((piece ^ (r & 7)) << 4));
+              const float4 z = lds_f4(stage + (r + cc * kRows) * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
               y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
             }
-            const int at = out_rows[r];
+            const int at = out_rows[128 * parity + r];
             if (at < 0) continue;
             if (whole) {
               const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
-              *reinterpret_cast<uint2*>(p.o + static_cast<int64_t>(at) * D + 32 * c + 4 * piece) =
+              *reinterpret_cast<uint2*>(p.o + static_cast<int64_t>(at) * D + 16 * c + 4 * piece) =
                   make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
             } else {
-              *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * kRows + r) * D + 32 * c + 4 * piece) = y;
+              *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * kRows + r) * D + 16 * c + 4 * piece) = y;
             }
           }
+          if (kCopies > 1) bar_sync(1 + team, 128);
+          else __syncwarp();
         }
-        if (real && marked) marks[row] = 1;
-        bar_sync(1, 128);                                     // marks are seen; and the staging has been read: the next queries may come
-        const bool mine = copy == 0 && real;
-        const bool again = mine && marks[row] != 0;
-        if (whole) {
-          const int head = x.hk * p.rep + unit_row - node * p.rep;
-          if (mine) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = (m_all + log2f(l_all)) * kLn2;
+        const bool mine = team == 0 && copy == 0 && real;
+        const int head = x.hk * p.rep + unit_row - node * p.rep;
+        const bool again = mine && marks[128 * parity + row] != 0;
+        if (mine && whole) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = (m_all + log2f(l_all)) * kLn2;
+        if (mine && !whole) p.part_ml[static_cast<int64_t>(slot) * kRows + row] = make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
+        if (whole && any_marked[parity] != 0) {
+          bar_sync(4, 128 * kTeams);                          // the rows' output stands
           for (uint32_t left = __ballot_sync(0xffffffffu, again); left != 0; left &= left - 1) {
             const int from = __ffs(left) - 1;
-            __syncwarp();
             tree_row<D>(p, x.b, __shfl_sync(0xffffffffu, node, from), __shfl_sync(0xffffffffu, head, from));
           }
-        } else if (mine) {
-          p.part_ml[static_cast<int64_t>(slot) * kRows + row] = make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
         }
         tc_fence_before();
-      } while (tree_next(p, x, f_end));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kOut + parity);
+        ++units;
+        x = next;
+        live = more;
+      }
       if (!ok && lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
     }
+  } else if (tid == 0) {
+    reinterpret_cast<TreeCut*>(p.cuts)[worker] = TreeCut{};
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (role == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::kTmemCols);
+    tmem_dealloc(tmem, 512);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ join
-// The pieces of cut units: where worker j of the main kernel goes on with a unit that worker j - 1 began, the CTAs (j, ...) join it, a warp a row; and the
-// rows behind the counts.
-constexpr int kJoinParts = 8;
-
+// The pieces of cut units, a warp a row, four rows a CTA; and the rows behind the counts.
 template <int D>
 __global__ void __launch_bounds__(128) cache_tree_join_kernel(const __grid_constant__ CacheTreeParams p) {
   constexpr int kVecs = D / 128;
-  __shared__ int cum[136];
   grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TreeCut x = reinterpret_cast<const TreeCut*>(p.cuts)[blockIdx.x];
   // rows behind the counts: zeros
   for (int b = blockIdx.x; b < p.c.B; b += gridDim.x)
-    for (int i = tree_seq(p, b).count + blockIdx.y; i < p.N; i += kJoinParts) {
+    for (int i = tree_seq(p, b).count + blockIdx.y; i < p.N; i += gridDim.y) {
       uint4* o = reinterpret_cast<uint4*>(p.o + (static_cast<int64_t>(b) * p.N + i) * p.H * D);
       for (int z = threadIdx.x; z < p.H * D / 8; z += 128) o[z] = make_uint4(0, 0, 0, 0);
       for (int z = threadIdx.x; z < p.H; z += 128) p.lse[(static_cast<int64_t>(b) * p.H + z) * p.N + i] = -CUDART_INF_F;
     }
-  const TreeRange range = tree_range(p, cum);
-  const int j = blockIdx.x;
-  if (j == 0 || j >= range.workers) return;
-  const int f = tree_share(range, j);
-  const TreePiece x = tree_first(p, range, cum, f, f + 1);
-  if (x.begin >= f || tree_share(range, j - 1) > x.begin) return;        // no cut, or not the unit's first
-  auto worker_at = [&](int step) {                            // whose share it is: share(lo) <= step < share(hi)
-    int lo = j - 1, hi = range.workers;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (tree_share(range, mid) <= step) lo = mid; else hi = mid;
+  const int r = blockIdx.y * 4 + warp, unit_row = x.rt * p.row_tile + r, node = node_of(p, unit_row), head = x.hk * p.rep + unit_row - node * p.rep;
+  if (node >= x.count) return;
+  float top = kNone, u_top = kNone, sum = 0.f;
+  float4 acc[kVecs] = {};
+  bool marked = false;
+  // 32 results at a time, a lane each: their maxima and sums together, then the values of those that count
+  for (int w0 = x.first; w0 <= x.last; w0 += 32) {
+    const int w = w0 + lane;
+    const bool there = w <= x.last;                           // each has a tile at least
+    const int64_t at = there ? static_cast<int64_t>(w == x.first ? x.slot : 2 * w) * p.row_tile + r : 0;
+    const float4 ml = there ? p.part_ml[at] : make_float4(kNone, 0.f, kNone, 0.f);
+    marked |= __any_sync(0xffffffffu, ml.w != 0.f);
+    float top_new = ml.x, u_new = ml.z;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, o));
+      u_new = fmaxf(u_new, __shfl_xor_sync(0xffffffffu, u_new, o));
     }
-    return lo;
-  };
-  // of the tiles; workers before them have steps of the unit's own cost alone and no piece
-  const int first = worker_at(x.begin + kTreeCost), last = worker_at(x.end() - 1);
-  if (first == last) return;                                  // whole: written by that worker
-  auto slot_of = [&](int w) { return 2 * w + (w == j - 1 && tree_share(range, w) < x.begin ? 1 : 0); };
-  for (int r = blockIdx.y * 4 + warp; r < p.row_tile; r += 4 * kJoinParts) {
-    const int unit_row = x.rt * p.row_tile + r, node = unit_row / p.rep, head = x.hk * p.rep + unit_row - node * p.rep;
-    if (node >= x.s.count) break;
-    float top = kNone, u_top = kNone, sum = 0.f;
-    float4 acc[kVecs] = {};
-    bool marked = false;
-    // 32 results at a time, a lane each: their maxima and sums together, then the values of those that count
-    for (int w0 = first; w0 <= last; w0 += 32) {
-      const int w = w0 + lane;
-      const bool there = w <= last;                           // each has a tile at least
-      const int64_t at = there ? static_cast<int64_t>(slot_of(w)) * p.row_tile + r : 0;
-      const float4 ml = there ? p.part_ml[at] : make_float4(kNone, 0.f, kNone, 0.f);
-      marked |= __any_sync(0xffffffffu, ml.w != 0.f);
-      float top_new = ml.x, u_new = ml.z;
+    top_new = fmaxf(top, top_new);
+    u_new = fmaxf(u_top, u_new);
+    float l = ml.y * ex2_approx(ml.x - top_new);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, o));
-        u_new = fmaxf(u_new, __shfl_xor_sync(0xffffffffu, u_new, o));
-      }
-      top_new = fmaxf(top, top_new);
-      u_new = fmaxf(u_top, u_new);
-      float l = ml.y * ex2_approx(ml.x - top_new);
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    sum = sum * ex2_approx(top - top_new) + l;
+    const float a = ex2_approx(u_top - u_new), wgt = ex2_approx(ml.z - u_new);
+    top = top_new;
+    u_top = u_new;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      sum = sum * ex2_approx(top - top_new) + l;
-      const float a = ex2_approx(u_top - u_new), wgt = ex2_approx(ml.z - u_new);
-      top = top_new;
-      u_top = u_new;
+    for (int v = 0; v < kVecs; ++v) acc[v] = make_float4(acc[v].x * a, acc[v].y * a, acc[v].z * a, acc[v].w * a);
+    const uint32_t counts = __ballot_sync(0xffffffffu, there && ml.x > kNone);          // kNone: the row sees nothing of the piece
+#pragma unroll 8
+    for (int k = 0; k < min(32, x.last - w0 + 1); ++k) {
+      const float w_k = __shfl_sync(0xffffffffu, wgt, k);
+      const int64_t at_k = __shfl_sync(0xffffffffu, at, k);
+      if (!((counts >> k) & 1)) continue;
 #pragma unroll
-      for (int v = 0; v < kVecs; ++v) acc[v] = make_float4(acc[v].x * a, acc[v].y * a, acc[v].z * a, acc[v].w * a);
-      const uint32_t counts = __ballot_sync(0xffffffffu, there && ml.x > kNone);          // kNone: the row sees nothing of the piece
-#pragma unroll 4
-      for (int k = 0; k < min(32, last - w0 + 1); ++k) {
-        const float w_k = __shfl_sync(0xffffffffu, wgt, k);
-        const int64_t at_k = __shfl_sync(0xffffffffu, at, k);
-        if (!((counts >> k) & 1)) continue;
-#pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-          const float4 y = reinterpret_cast<const float4*>(p.part_o + at_k * D)[32 * v + lane];
-          acc[v] = make_float4(fmaf(y.x, w_k, acc[v].x), fmaf(y.y, w_k, acc[v].y), fmaf(y.z, w_k, acc[v].z), fmaf(y.w, w_k, acc[v].w));
-        }
+      for (int v = 0; v < kVecs; ++v) {
+        const float4 y = reinterpret_cast<const float4*>(p.part_o + at_k * D)[32 * v + lane];
+        acc[v] = make_float4(fmaf(y.x, w_k, acc[v].x), fmaf(y.y, w_k, acc[v].y), fmaf(y.z, w_k, acc[v].z), fmaf(y.w, w_k, acc[v].w));
       }
     }
-    if (marked) {
-      tree_row<D>(p, x.b, node, head);
-      continue;
-    }
-    const float d_all = u_top - top, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
-    const float w1 = exp2f(d1), w2 = exp2f(d_all - d1) / sum;
-    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(x.b) * p.N + node) * p.H + head) * D) + 2 * lane;
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v) {
-      o[64 * v] = __floats2bfloat162_rn(acc[v].x * w1 * w2, acc[v].y * w1 * w2);
-      o[64 * v + 1] = __floats2bfloat162_rn(acc[v].z * w1 * w2, acc[v].w * w1 * w2);
-    }
-    if (lane == 0) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = (top + log2f(sum)) * kLn2;
   }
+  if (marked) {
+    tree_row<D>(p, x.b, node, head);
+    return;
+  }
+  const float d_all = u_top - top, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
+  const float w1 = exp2f(d1), w2 = exp2f(d_all - d1) / sum;
+  __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(x.b) * p.N + node) * p.H + head) * D) + 2 * lane;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    o[64 * v] = __floats2bfloat162_rn(acc[v].x * w1 * w2, acc[v].y * w1 * w2);
+    o[64 * v + 1] = __floats2bfloat162_rn(acc[v].z * w1 * w2, acc[v].w * w1 * w2);
+  }
+  if (lane == 0) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = (top + log2f(sum)) * kLn2;
 }
 
 // Once per kernel and device: the driver call takes longer than a launch.
@@ -863,20 +965,20 @@ cudaError_t launch_tree(const CUtensorMap& tk, const CUtensorMap& tv, const Cach
   e = launch_chained(cache_tree_kernel<D, kCopies>, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, p);
   if (e != cudaSuccess) return e;
   count_launch();
-  return launch_chained(cache_tree_join_kernel<D>, dim3(p.grid, kJoinParts), 128, 0, stream, p);
+  return launch_chained(cache_tree_join_kernel<D>, dim3(p.grid, p.row_tile / 4), 128, 0, stream, p);
 }
 
 }  // namespace
 
 CacheTreePlan plan_cache_tree(int B, int N, int H, int Hk, int D, int T, int page) {
   CacheTreePlan x;
-  const int64_t R = static_cast<int64_t>(N) * (H / Hk);
+  const int64_t R = static_cast<int64_t>(N) * (H / Hk), wave = sm_count();
   x.row_tile = R <= 32 ? 32 : R <= 64 ? 64 : 128;
-  const int64_t wave = static_cast<int64_t>(sm_count()) * (D == 128 ? TreeCfg<128>::kCtasPerSm : TreeCfg<256>::kCtasPerSm);
   const int64_t tiles = static_cast<int64_t>(B) * Hk * ((R + x.row_tile - 1) / x.row_tile) * ((static_cast<int64_t>(T) * page + 127) / 128);
   x.grid = static_cast<int>(tiles < wave ? tiles : wave);      // one wave, and no more workers than there can be tiles
   x.part_o_bytes = 2ll * x.grid * x.row_tile * D * 4;
   x.part_ml_bytes = 2ll * x.grid * x.row_tile * 16;
+  x.cut_bytes = x.grid * static_cast<int64_t>(sizeof(TreeCut));
   return x;
 }
 

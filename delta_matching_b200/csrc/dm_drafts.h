@@ -47,15 +47,17 @@ struct CacheTreeParams {
   float* lse;                       // (B, H, N)
   float* part_o;                    // partial results: 2 slots a CTA, of row_tile rows of D fp32 each, and of their rows (m, l, u, marked): the sum is
   float4* part_ml;                  // l 2^m, the values count in 2^u
+  void* cuts;                       // and what the join needs of each cut unit
   int grid;                         // CTAs of the main kernel
-  int row_tile;                     // rows (drafted tokens x heads of a group) of a unit
+  int row_tile, row_shift;          // rows (drafted tokens x heads of a group) of a unit, a power of two
+  uint32_t rep_magic;               // r / rep is the upper half of r times it (0: divide)
 };
 
 // How a call of dm_cache_attn_tree is laid out, and its workspace.
 struct CacheTreePlan {
   int row_tile, grid;
-  int64_t part_o_bytes, part_ml_bytes;
-  int64_t bytes() const { return part_o_bytes + part_ml_bytes; }
+  int64_t part_o_bytes, part_ml_bytes, cut_bytes;
+  int64_t bytes() const { return part_o_bytes + part_ml_bytes + cut_bytes; }
 };
 CacheTreePlan plan_cache_tree(int B, int N, int H, int Hk, int D, int T, int page);
 

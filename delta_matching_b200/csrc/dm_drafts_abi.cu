@@ -127,8 +127,12 @@ int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, in
   p.lse = lse;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + x.part_o_bytes);
+  p.cuts = static_cast<uint8_t*>(workspace) + x.part_o_bytes + x.part_ml_bytes;
   p.grid = x.grid;
   p.row_tile = x.row_tile;
+  for (p.row_shift = 0; 1 << p.row_shift < x.row_tile;) ++p.row_shift;
+  // exact up to r < 2^32 / rep
+  if (p.rep > 1 && (static_cast<int64_t>(N) * p.rep + x.row_tile) * p.rep < (1ll << 32)) p.rep_magic = static_cast<uint32_t>(((1ll << 32) + p.rep - 1) / p.rep);
   CUtensorMap tk, tv;
   DM_TRY(pool_map(&tk, cache, cache->k8));
   DM_TRY(pool_map(&tv, cache, cache->v8));
