@@ -17,6 +17,7 @@
 // kCopies: where a unit has at most 64 or 32 rows, they stand twice or four times in the 128 lanes, and copy c looks after its share of a tile's blocks of 32
 // keys (P is zero in the others), with a reference, a sum and an accumulator of its own, which the CTA adds up at the end: the softmax of a tile is as much
 // shorter, and the tensor cores, which take 128 rows whatever is in them, have no more to do.
+#include <cooperative_groups.h>
 #include <type_traits>
 #include "dm_cache.cuh"
 #include "dm_drafts.h"
@@ -25,6 +26,10 @@
 namespace dm {
 
 namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kMaxCluster = 8;
 
 // Key tiles that a unit's queries and output are worth.
 constexpr int kTreeCost = 2;
@@ -50,7 +55,8 @@ struct TreeCfg {
   static constexpr int kSmemRows = kSmemU + 1024;              // by parity of the unit and row: factor of its logits; where its output goes; whether it is marked
   static constexpr int kSmemScales = kSmemRows + 2 * 128 * 12;        // 8 tiles x (4 K scales, 4 exponents of V's)
   static constexpr int kSmemNan = kSmemScales + 8 * 32;       // by S buffer: which tokens of a tile are NaN
-  static constexpr int kSmemBars = kSmemNan + 64;
+  static constexpr int kSmemSums = kSmemNan + 64;             // of a row, for the cluster: m, l, u, marked
+  static constexpr int kSmemBars = kSmemSums + 2048;
   static constexpr int kSmem = kSmemBars + 512 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
@@ -312,8 +318,65 @@ __device__ __forceinline__ TreeCut tree_cut_at(const TreeRange& range, const Tre
   return y;
 }
 
+// CTA `rank` of a cluster writes its share of a unit's rows: the CTAs have left it their sums of them (m, l, u, marked) and their values, a CTA's behind the other's, in
+// shared memory (its own: reading others' took 4000 cycles a row).  A warp a row, over the CTAs in order; rows behind the sequence's count are zeros.
+template <int D, int kRows, int kWarps>
+__device__ __forceinline__ void join_cluster(const CacheTreeParams& p, const TreePiece& x, int rank, const uint8_t* values, const float4* sums) {
+  constexpr int kVecs = D / 128;
+  const int cl = p.cluster, rows = kRows / cl, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = warp; i < rows; i += kWarps) {
+    const int unit_row = x.rt * kRows + rank * rows + i, node = node_of(p, unit_row), head = x.hk * p.rep + unit_row - node * p.rep;
+    if (node >= p.N) break;
+    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(x.b) * p.N + node) * p.H + head) * D) + 2 * lane;
+    float* lse = p.lse + (static_cast<int64_t>(x.b) * p.H + head) * p.N + node;
+    if (node >= x.s.count) {
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) o[64 * v] = o[64 * v + 1] = __floats2bfloat162_rn(0.f, 0.f);
+      if (lane == 0) *lse = -CUDART_INF_F;
+      continue;
+    }
+    float top = kNone, u_top = kNone, marked = 0.f;
+    for (int c = 0; c < cl; ++c) {
+      const float4 st = sums[c * rows + i];
+      top = fmaxf(top, st.x);
+      u_top = fmaxf(u_top, st.z);
+      marked += st.w;
+    }
+    if (marked != 0.f) {
+      tree_row<D>(p, x.b, node, head);
+      continue;
+    }
+    float sum = 0.f;
+    float4 acc[kVecs] = {};
+    for (int c = 0; c < cl; ++c) {
+      const float4 st = sums[c * rows + i];
+      if (!(st.x > kNone)) {                                  // the row sees nothing of the CTA's tiles (or it had none); NaN may have been added to its sum
+        sum += st.y;
+        continue;
+      }
+      sum = fmaf(st.y, ex2_approx(st.x - top), sum);
+      const float w = ex2_approx(st.z - u_top);
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const float4 y = reinterpret_cast<const float4*>(values)[(c * rows + i) * (D / 4) + 32 * v + lane];
+        acc[v] = make_float4(fmaf(y.x, w, acc[v].x), fmaf(y.y, w, acc[v].y), fmaf(y.z, w, acc[v].z), fmaf(y.w, w, acc[v].w));
+      }
+    }
+    const float d_all = u_top - top, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
+    const float w1 = exp2f(d1), w2 = exp2f(d_all - d1) / sum;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      o[64 * v] = __floats2bfloat162_rn(acc[v].x * w1 * w2, acc[v].y * w1 * w2);
+      o[64 * v + 1] = __floats2bfloat162_rn(acc[v].z * w1 * w2, acc[v].w * w1 * w2);
+    }
+    if (lane == 0) *lse = (top + log2f(sum)) * kLn2;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ main kernel
-template <int kD, int kCopies>
+// kCluster: a cluster of CTAs a unit instead of the even division, each an even share of its tiles, joined through distributed shared memory: nothing is left to a
+// second kernel.
+template <int kD, int kCopies, bool kCluster>
 __global__ void __launch_bounds__(TreeCfg<kD>::kThreads, 1)
 cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CacheTreeParams p) {
   using C = TreeCfg<kD>;
@@ -359,20 +422,42 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     tc_fence_before();
   }
   grid_dep_wait();
-  int sums;
-  const TreeRange range = tree_range(p, sums);
+  // the worker's share of the steps, and its first piece
+  const int worker = blockIdx.x;
+  int f_begin = 0, f_end = 0;
+  TreePiece x{};
+  TreeRange range{};
+  const int rank = kCluster ? worker % p.cluster : 0, rows_each = kCluster ? kRows / p.cluster : kRows;      // of the cluster; rows that each CTA of it writes
+  bool met = false;                                           // the cluster's CTAs are done with their tiles
+  if constexpr (kCluster) {
+    const int unit = worker / p.cluster, row_tiles = (p.N * p.rep + kRows - 1) / kRows;
+    x.b = unit / (p.c.Hk * row_tiles);
+    const int in_sequence = unit - x.b * p.c.Hk * row_tiles;
+    x.hk = in_sequence / row_tiles;
+    x.rt = in_sequence - x.hk * row_tiles;
+    x.s = tree_seq(p, x.b);
+    if (x.rt < x.s.row_tiles(p)) {
+      x.t0 = x.s.tiles() * rank / p.cluster;
+      x.t1 = x.s.tiles() * (rank + 1) / p.cluster;
+    }
+  } else {
+    int sums;
+    range = tree_range(p, sums);
+    if (worker < range.workers && range.total > 0) {
+      f_begin = range.share(worker);
+      f_end = range.share(worker + 1);
+      x = tree_first(p, sums, f_begin, f_end);
+    }
+  }
   __syncthreads();                                            // the mbarriers and the TMEM slot are there
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int worker = blockIdx.x;
   auto bar = [&](int i) { return smem_u32(bars + i); };
   // running tile g goes to team and S buffer g % kTeams, whose barriers' phase it is
   auto phase_of = [&](int g) { return static_cast<uint32_t>(g / kTeams) & 1u; };
   bool ok = true;
 
-  if (worker < range.workers && range.total > 0) {
-    const int f_begin = range.share(worker), f_end = range.share(worker + 1);
-    TreePiece x = tree_first(p, sums, f_begin, f_end);
+  if (kCluster || f_begin < f_end) {
     if (role >= 0 && D == 128) reg_dec<C::kRegsOther>();
     if (role == 0) {
       // ---------------------------------------------------------------------------------------- TMA: code tiles and their scales
@@ -523,8 +608,10 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (!ok) raise_abort(abort_flag, p.c.status, kStatusTimeoutMma + kInCache);
       }
     } else if (role == 3) {
-      const TreeCut y = tree_cut_at(range, x, worker, f_begin);
-      if (lane == 0) reinterpret_cast<TreeCut*>(p.cuts)[worker] = y;
+      if (!kCluster) {
+        const TreeCut y = tree_cut_at(range, x, worker, f_begin);
+        if (lane == 0) reinterpret_cast<TreeCut*>(p.cuts)[worker] = y;
+      }
     } else {
       if (D == 128) reg_inc<C::kRegsSoftmax>();
       // ---------------------------------------------------------------------------------------- softmax, output
@@ -780,7 +867,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (!(ok = all_of(4, 128 * kTeams, ok))) break;
         tc_fence_after();
         if (more) put_queries(next, parity ^ 1);              // all S of this unit have been computed; those of the next run under the output
-        const bool whole = x.whole();
+        const bool whole = !kCluster && x.whole();
         float m_all = kNone, u_all = kNone, l_all = 0.f;
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) {
@@ -800,6 +887,10 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         const float d_all = u_all - m_all, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
         const float w1 = whole ? w * exp2f(d1) : w, w2 = whole ? exp2f(d_all - d1) / l_all : 1.f;
         const int slot = 2 * worker + (x.f0 == f_begin ? 0 : 1);
+        if constexpr (kCluster) {                             // the values go to the CTAs that write their rows, where the ring must be free: all CTAs' tiles are done with
+          cg::this_cluster().sync();
+          met = true;
+        }
         // 16 columns at a time, through shared memory: four lanes a row, eight rows a warp at a time; 16-byte pieces XORed with the lane
         const uint32_t stage = sbase + C::kSmemOut + team * 8192;
 #pragma unroll 1
@@ -828,7 +919,10 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             }
             const int at = out_rows[128 * parity + r];
             if (at < 0) continue;
-            if (whole) {
+            if constexpr (kCluster) {
+              const int to = r / rows_each;
+              *reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemRing + ((rank * rows_each + r - to * rows_each) * D + 16 * c + 4 * piece) * 4) = y;
+            } else if (whole) {
               const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
               *reinterpret_cast<uint2*>(p.o + static_cast<int64_t>(at) * D + 16 * c + 4 * piece) =
                   make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
@@ -843,7 +937,12 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         const int head = x.hk * p.rep + unit_row - node * p.rep;
         const bool again = mine && marks[128 * parity + row] != 0;
         if (mine && whole) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = (m_all + log2f(l_all)) * kLn2;
-        if (mine && !whole) p.part_ml[static_cast<int64_t>(slot) * kRows + row] = make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
+        if constexpr (kCluster) {
+          const int to = row / rows_each;
+          if (mine)
+            reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemSums)[rank * rows_each + row - to * rows_each] =
+                make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
+        } else if (mine && !whole) p.part_ml[static_cast<int64_t>(slot) * kRows + row] = make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
         if (whole && any_marked[parity] != 0) {
           bar_sync(4, 128 * kTeams);                          // the rows' output stands
           for (uint32_t left = __ballot_sync(0xffffffffu, again); left != 0; left &= left - 1) {
@@ -860,8 +959,22 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       }
       if (!ok && lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutCompute + kInCache);
     }
-  } else if (tid == 0) {
+  } else if (!kCluster && tid == 0) {
     reinterpret_cast<TreeCut*>(p.cuts)[worker] = TreeCut{};
+  }
+  if constexpr (kCluster) {
+    __syncwarp();
+    if (!met) {
+      cg::this_cluster().sync();
+      if (role < 0) {                                         // no tiles (or given up): nothing for the other CTAs' rows
+        for (int r = tid; r < kRows; r += 128 * kTeams) {
+          const int to = r / rows_each;
+          reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemSums)[rank * rows_each + r - to * rows_each] = make_float4(kNone, 0.f, kNone, 0.f);
+        }
+      }
+    }
+    cg::this_cluster().sync();
+    if (role < 0) join_cluster<D, kRows, 4 * kTeams>(p, x, rank, smem + C::kSmemRing, reinterpret_cast<const float4*>(smem + C::kSmemSums));
   }
   __syncwarp();
   tc_fence_before();
@@ -959,14 +1072,37 @@ cudaError_t allow_smem(int bytes) {
 template <int D, int kCopies>
 cudaError_t launch_tree(const CUtensorMap& tk, const CUtensorMap& tv, const CacheTreeParams& p, cudaStream_t stream) {
   using C = TreeCfg<D>;
-  cudaError_t e = allow_smem<cache_tree_kernel<D, kCopies>>(C::kSmem);
+  cudaError_t e;
+  if (p.cluster > 0) {
+    e = allow_smem<cache_tree_kernel<D, kCopies, true>>(C::kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.grid);
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, cache_tree_kernel<D, kCopies, true>, tk, tv, p);
+  }
+  e = allow_smem<cache_tree_kernel<D, kCopies, false>>(C::kSmem);
   if (e != cudaSuccess) return e;
   count_launch();
-  e = launch_chained(cache_tree_kernel<D, kCopies>, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, p);
+  e = launch_chained(cache_tree_kernel<D, kCopies, false>, dim3(p.grid), C::kThreads, C::kSmem, stream, tk, tv, p);
   if (e != cudaSuccess) return e;
   count_launch();
   return launch_chained(cache_tree_join_kernel<D>, dim3(p.grid, p.row_tile / 4), 128, 0, stream, p);
 }
+
+// Tiles of a CTA up to which a cluster takes a unit.
+constexpr int kClusterTiles = 12;
 
 }  // namespace
 
@@ -974,8 +1110,18 @@ CacheTreePlan plan_cache_tree(int B, int N, int H, int Hk, int D, int T, int pag
   CacheTreePlan x;
   const int64_t R = static_cast<int64_t>(N) * (H / Hk), wave = sm_count();
   x.row_tile = R <= 32 ? 32 : R <= 64 ? 64 : 128;
-  const int64_t tiles = static_cast<int64_t>(B) * Hk * ((R + x.row_tile - 1) / x.row_tile) * ((static_cast<int64_t>(T) * page + 127) / 128);
-  x.grid = static_cast<int>(tiles < wave ? tiles : wave);      // one wave, and no more workers than there can be tiles
+  const int64_t unit_tiles = (static_cast<int64_t>(T) * page + 127) / 128, units = static_cast<int64_t>(B) * Hk * ((R + x.row_tile - 1) / x.row_tile);
+  // A cluster a unit where its CTAs have few tiles each and all are resident at a time.
+  int cl = 1;
+  while (cl < kMaxCluster && units * cl * 2 <= wave && cl < unit_tiles) cl *= 2;
+  x.cluster = units * cl <= wave && unit_tiles <= static_cast<int64_t>(kClusterTiles) * cl ? cl : 0;
+  if (x.cluster > 0) {
+    x.grid = static_cast<int>(units) * cl;
+    x.part_o_bytes = x.part_ml_bytes = 0;
+    x.cut_bytes = 16;
+    return x;
+  }
+  x.grid = static_cast<int>(units * unit_tiles < wave ? units * unit_tiles : wave);      // one wave, and no more workers than there can be tiles
   x.part_o_bytes = 2ll * x.grid * x.row_tile * D * 4;
   x.part_ml_bytes = 2ll * x.grid * x.row_tile * 16;
   x.cut_bytes = x.grid * static_cast<int64_t>(sizeof(TreeCut));

@@ -49,13 +49,14 @@ struct CacheTreeParams {
   float4* part_ml;                  // l 2^m, the values count in 2^u
   void* cuts;                       // and what the join needs of each cut unit
   int grid;                         // CTAs of the main kernel
+  int cluster;                      // of a unit, or 0: the even division
   int row_tile, row_shift;          // rows (drafted tokens x heads of a group) of a unit, a power of two
   uint32_t rep_magic;               // r / rep is the upper half of r times it (0: divide)
 };
 
 // How a call of dm_cache_attn_tree is laid out, and its workspace.
 struct CacheTreePlan {
-  int row_tile, grid;
+  int row_tile, grid, cluster;
   int64_t part_o_bytes, part_ml_bytes, cut_bytes;
   int64_t bytes() const { return part_o_bytes + part_ml_bytes + cut_bytes; }
 };

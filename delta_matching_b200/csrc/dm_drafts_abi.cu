@@ -129,6 +129,7 @@ int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, in
   p.part_ml = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + x.part_o_bytes);
   p.cuts = static_cast<uint8_t*>(workspace) + x.part_o_bytes + x.part_ml_bytes;
   p.grid = x.grid;
+  p.cluster = x.cluster;
   p.row_tile = x.row_tile;
   for (p.row_shift = 0; 1 << p.row_shift < x.row_tile;) ++p.row_shift;
   // exact up to r < 2^32 / rep
