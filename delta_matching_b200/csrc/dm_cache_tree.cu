@@ -11,8 +11,8 @@
 //
 // The key tiles of 128 tokens of all units are one flat range, divided evenly over the CTAs of one wave; pieces of cut units are joined by a second kernel.
 // One CTA an SM.  Three teams of four softmax warps (thread = TMEM lane; two teams at head_dim 256) take the tiles of a unit in turn, each with an S buffer in TMEM;
-// P's codes and scale bytes lie over the S that they come from.  Of the last four warps one loads the code tiles from the pages by TMA and two issue the MMAs.  What the teams share of a row is the power of two that O counts in: it goes from team to team with the tiles, and moves so seldom
-// (fp32 takes 40 powers of two above it) that O is hardly ever rescaled.
+// P's codes and scale bytes lie over the S that they come from.  Of the last four warps one loads the code tiles from the pages by TMA and two issue the MMAs.  The power of two that a row of O counts in is fixed by the
+// unit's first blocks: fp32 has room for what may follow (rows for which it has not are marked and made by themselves), and no team waits for another's maximum.
 //
 // kCopies: where a unit has at most 64 or 32 rows, they stand twice or four times in the 128 lanes, and copy c looks after its share of a tile's blocks of 32
 // keys (P is zero in the others), with a reference, a sum and an accumulator of its own, which the CTA adds up at the end: the softmax of a tile is as much
@@ -32,9 +32,10 @@ namespace cg = cooperative_groups;
 constexpr int kMaxCluster = 8;
 
 // Key tiles that a unit's queries and output are worth.
-constexpr int kTreeCost = 2;
+constexpr int kTreeCost = 4;
 constexpr float kExact = 4194304.f;         // logits (log2) up to this size: whole numbers beside them are exact
-constexpr float kReach = 40.f;              // what a row's logits may exceed its references by, in powers of two: fp32 has room for it
+constexpr float kReach = 40.f;              // what a row's logits may exceed the reference of its sum by, in powers of two: fp32 has room for it
+constexpr int kUnitLift = 40;               // of the reference of the products, above those it was taken from
 
 template <int kD>
 struct TreeCfg {
@@ -57,7 +58,7 @@ struct TreeCfg {
   static constexpr int kSmemNan = kSmemScales + 8 * 32;       // by S buffer: which tokens of a tile are NaN
   static constexpr int kSmemSums = kSmemNan + 64;             // of a row, for the cluster: m, l, u, marked
   static constexpr int kSmemBars = kSmemSums + 2048;
-  static constexpr int kSmem = kSmemBars + 512 + 1024;
+  static constexpr int kSmem = kSmemBars + 528 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -284,10 +285,11 @@ enum TreeBar : int {
   kFull = 0, kEmpty = 10,                   // of the ring
   kQ = 20, kOut = 22,                       // by parity of the unit: queries written; output read from TMEM
   kS = 24, kP = 27, kPv = 30,               // by S buffer: S computed, P written, P V done
-  kU = 33,                                  // by team and quarter of the lanes: the tile's references stand
-  kScales = 45,                             // of running tile g: entry g % 8
-  kCut = 53,                                // by team: a cut tile's values have been looked at
-  kTreeBars = 56,                           // behind them the TMEM slot, the abort flag and whether a row of the unit is marked (by parity)
+  kU = 33,                                  // by quarter of the lanes: the unit's u stands
+  kScales = 37,                             // of running tile g: entry g % 8
+  kCut = 45,                                // by team: a cut tile's values have been looked at
+  kPHalf = 48,                              // as kP, of the first half of a tile's keys (one copy)
+  kTreeBars = 51,                           // behind them the TMEM slot, the abort flag and whether a row of the unit is marked (by parity)
 };
 
 // What the join needs of a cut unit, left by the worker that goes on with it first: its rows, and the workers that have tiles of it.
@@ -339,7 +341,7 @@ __device__ __forceinline__ void join_cluster(const CacheTreeParams& p, const Tre
     for (int c = 0; c < cl; ++c) {
       const float4 st = sums[c * rows + i];
       top = fmaxf(top, st.x);
-      u_top = fmaxf(u_top, st.z);
+      if (st.x > kNone) u_top = fmaxf(u_top, st.z);
       marked += st.w;
     }
     if (marked != 0.f) {
@@ -407,9 +409,10 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       mbar_init(bars + kS + i, 1);
       mbar_init(bars + kP + i, 4);
       mbar_init(bars + kPv + i, 1);
-      for (int q = 0; q < 4; ++q) mbar_init(bars + kU + 4 * i + q, 1);
       mbar_init(bars + kCut + i, 4);
+      mbar_init(bars + kPHalf + i, 4);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(bars + kU + i, 1);
     for (int i = 0; i < 8; ++i) mbar_init(bars + kScales + i, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -586,20 +589,27 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           if (units > 0) ok = wait_or_abort(bar(kOut + ((units - 1) & 1)), ((units - 1) >> 1) & 1, abort_flag);      // O has been read
           for (int t = x.t0; t < x.t1 && ok; ++t, ++g) {
             const int st = (2 * g + 1) % C::kStages, buf = g % kTeams, held = min(4, (x.s.n - 128 * t + 31) / 32);     // blocks of the tile
-            if (!(ok = wait_or_abort(bar(kP + buf), phase_of(g), abort_flag) && wait_or_abort(bar(kFull + st), ((2 * g + 1) / C::kStages) & 1, abort_flag))) break;
-            tc_fence_after();
             const uint32_t v_lo = ring_lo + st * (C::kTile >> 4), s = tmem + 128 * buf;
+            // one copy: by halves of the keys, each with scale bytes of its own
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              if (k >= held) break;                           // P is zero there and V is not loaded
+              if (k == 0 || (k == 2 && kCopies == 1)) {
+                if (!(ok = wait_or_abort(bar((k == 0 && kCopies == 1 ? kPHalf : kP) + buf), phase_of(g), abort_flag))) break;
+                if (k == 0 && !(ok = wait_or_abort(bar(kFull + st), ((2 * g + 1) / C::kStages) & 1, abort_flag))) break;
+                tc_fence_after();
+              }
+              if (k < held) {                                 // (beyond, P is zero and V is not loaded)
+                const uint32_t words = s + (k >= 2 && kCopies == 1 ? 80 : 16);
 #pragma unroll
-              for (int c = 0; c < C::kPanels; ++c) {
-                mma_mxf8_ts(tmem + C::kColO + 128 * c, s + 32 * k, v_lo + c * (16384 >> 4) + k * (4096 >> 4), idesc_mxf8(128, 128, false, true, k, k), s + 16, s + 20,
-                            t > x.t0 || k > 0);
-                mma_mxf8_ts(tmem + C::kColO + 128 * c, s + 32 * k + 8, v_lo + c * (16384 >> 4) + k * (4096 >> 4), idesc_mxf8(128, 128, false, true, k, k), s + 16, s + 20,
-                            true);
+                for (int c = 0; c < C::kPanels; ++c) {
+                  mma_mxf8_ts(tmem + C::kColO + 128 * c, s + 32 * k, v_lo + c * (16384 >> 4) + k * (4096 >> 4), idesc_mxf8(128, 128, false, true, k, k), words, words + 4,
+                              t > x.t0 || k > 0);
+                  mma_mxf8_ts(tmem + C::kColO + 128 * c, s + 32 * k + 8, v_lo + c * (16384 >> 4) + k * (4096 >> 4), idesc_mxf8(128, 128, false, true, k, k), words, words + 4,
+                              true);
+                }
               }
             }
+            if (!ok) break;
             tc_commit(bars + kEmpty + st);
             tc_commit(bars + kPv + buf);
           }
@@ -637,10 +647,12 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
       };
       auto put_queries = [&](const TreePiece& y, int parity) {
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < kPasses; ++k) {
           const int r = (warp + 4 * kTeams * k) * kPer + lane / kLanes;
-          const uint32_t v[4] = {asked[k].x, asked[k].y, asked[k].z, asked[k].w};
+          const uint32_t v[4] = {asked[0].x, asked[0].y, asked[0].z, asked[0].w};
+#pragma unroll
+          for (int z = 1; z < kPasses; ++z) asked[z - 1] = asked[z];
           // the largest size, as bits: NaN and infinities are above all others
           uint32_t top = __vmaxu2(__vmaxu2(v[0] & 0x7FFF7FFFu, v[1] & 0x7FFF7FFFu), __vmaxu2(v[2] & 0x7FFF7FFFu, v[3] & 0x7FFF7FFFu));
           top = max(top & 0xFFFFu, top >> 16);
@@ -691,29 +703,53 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       int g0 = 0, units = 0, cuts = 0;                        // running tile that the unit begins with, running unit; cut tiles of the team
       while (live) {
         const int parity = units & 1, n_tiles = x.t1 - x.t0;
-        volatile float* u_at = reinterpret_cast<volatile float*>(smem + C::kSmemU) + 128 * parity + in_tile;
+        volatile int* u_at = reinterpret_cast<volatile int*>(smem + C::kSmemU) + 128 * parity + in_tile;
         ok = wait_warp(bar(kQ + parity), (units >> 1) & 1, abort_flag);
         const int unit_row = x.rt * kRows + row, node = node_of(p, unit_row);
         const bool real = node < x.s.count;
         const bool idle = !__any_sync(0xffffffffu, real);     // a warp of rows that are none
         const uint32_t* seen = p.seen + x.b * p.s_sb + static_cast<int64_t>(min(node, x.s.count - 1)) * p.s_sn;
         const float f = factors[128 * parity + row];
-        // Of the row, whole numbers: m, the reference of this team's sum l; u, that of the products of a probability and its V scale, in which O counts and
-        // which goes from team to team with the tiles.  They move only when a row's logits exceed them by more than 2^kReach.
-        float m = kNone, l = 0.f;
-        bool marked = false;
+        // Of the row, whole numbers: m, the reference of this team's sum l, which moves where a block's logits exceed it by more than 2^kReach; and u, in which O counts, the same
+        // for all teams: kUnitLift above the largest product of a probability and its V scale among the first blocks of the unit, where the row sees any of these.  It does not
+        // move: fp32 has room for products 2^95 above it (hi: the largest that this team has met), and a row that has larger ones is marked.
+        float m = kNone, l = 0.f, u = 0.f, hi = kNone;
+        int u_code = 0;
+        bool knows_u = false, marked = false;
         // One key tile.  kCut: some row does not see all its keys (a compile-time variant: no select per element elsewhere).
         auto tile = [&](int g, int t, auto cut_tag) -> bool {
           constexpr bool kCut = decltype(cut_tag)::value;
           const uint32_t entry = sbase + C::kSmemScales + (g & 7) * 32;
-          float kb[kBlocks], ev[kBlocks], sums[kBlocks];
-          constexpr int kUnroll = kCut ? 1 : kBlocks;
-#pragma unroll kUnroll
+          auto scale_byte = [&](float ku) { return static_cast<uint32_t>(fminf(fmaxf(ku - u + 119.f, 0.f), 254.f)); };       // of P's codes: 2^(ku - u - 8)
+          auto put_words = [&](uint32_t at, uint32_t word) {
+            const uint32_t words[8] = {word, word, word, word, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
+            tmem_st8(at, words);
+          };
+          // The reference of the unit's products: from its first tile, or what that left.
+          auto know_u = [&](float top_u) -> bool {
+            if (g == g0) {
+              const bool none = !(top_u > kNone);
+              const int code = 2 * (none ? kUnitLift : static_cast<int>(fminf(fmaxf(top_u, -kExact), kExact)) + kUnitLift) + (none ? 1 : 0);
+              *u_at = code;
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bars + kU + quarter);
+              u_code = code;
+            } else if (!knows_u) {
+              if (!wait_warp(bar(kU + quarter), units & 1, abort_flag)) return false;
+              u_code = *u_at;
+            }
+            knows_u = true;
+            u = static_cast<float>(u_code >> 1);
+            return true;
+          };
+          float ku[2] = {kNone, kNone};                       // of two blocks, the power of two of their codes with V's scale
+          // (not unrolled, here and below: four times as much code had the warps wait for instructions a fifth of the time)
+#pragma unroll 1
           for (int c = 0; c < kBlocks; ++c) {
             uint32_t s[32];
             tmem_ld32(t_s + 32 * (c0 + c), s);
             const float fc = f * lds_f(entry + 4 * (c0 + c));
-            ev[c] = lds_f(entry + 16 + 4 * (c0 + c));
+            const float ev = lds_f(entry + 16 + 4 * (c0 + c));
             uint32_t sees = 0xffffffffu;
             if (kCut) {
               sees = real ? seen_keys(seen, node, 128 * t + 32 * (c0 + c) - x.s.base()) : 0u;
@@ -729,8 +765,8 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
             for (int e = 0; e < 16; ++e) s2[e] = make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
             const float top = max32(s2);
-            kb[c] = kCut && sees == 0u ? kNone : fmaxf(ceilf(top * fc), kNone);
-            const float2 f2 = splat2(fc), off = splat2(8.f - kb[c]);
+            const float kb = kCut && sees == 0u ? kNone : fmaxf(ceilf(top * fc), kNone);
+            const float2 f2 = splat2(fc), off = splat2(8.f - kb);
             float2 sum = make_float2(0.f, 0.f);
             uint32_t w[16];                                   // first codes, second codes
 #pragma unroll
@@ -748,62 +784,37 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
               }
               split4(y[0], y[1], w[e / 2], w[8 + e / 2]);
             }
-            sums[c] = sum.x + sum.y;
             tmem_st16(t_s + 32 * (c0 + c), w);                // over columns that have been read
-          }
-          if (kCopies > 1) {                                  // other copies' blocks
-            const uint32_t zeros[16] = {};
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (c < c0 || c >= c0 + kBlocks) tmem_st16(t_s + 32 * c, zeros);
-          }
-          float top = kb[0], top_u = kb[0] + ev[0];
-#pragma unroll
-          for (int c = 1; c < kBlocks; ++c) {
-            top = fmaxf(top, kb[c]);
-            top_u = fmaxf(top_u, kb[c] + ev[c]);
-          }
-          marked |= fabsf(top) > kExact && top > kNone;
-          if (top > m + kReach) {
-            l *= ex2_approx(m - top);
-            m = top;
-          }
-          // the tile before this one, another team's, has its u
-          if (g > 0 && !wait_warp(bar(kU + 4 * ((g - 1) % kTeams) + quarter), phase_of(g - 1), abort_flag)) return false;
-          float u_old = kNone;
-          if (g > g0) u_old = *u_at;
-          float u = u_old;
-          if (__any_sync(0xffffffffu, top_u > u_old + kReach)) {
-            if (top_u > u_old + kReach) u = top_u;
-            if (g > g0) {
-              const float keep = ex2_approx(u_old - u);
-              // O stands still between the products of the last tile and those of this one
-              if (!wait_warp(bar(kPv + (g - 1) % kTeams), phase_of(g - 1), abort_flag)) return false;
-              tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32(t_o + 32 * c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                tmem_st32(t_o + 32 * c, o);
-              }
+            marked |= fabsf(kb) > kExact && kb > kNone;
+            if (kb > m + kReach) {
+              l *= ex2_approx(m - kb);
+              m = kb;
+            }
+            l = fmaf(sum.x + sum.y, ex2_approx(kb - m - 8.f), l);
+            if (c & 1) ku[1] = kb + ev;
+            else ku[0] = kb + ev;
+            if (kCopies == 1 && c == 1) {                     // the first half of the keys: the tensor cores may begin
+              if (!know_u(fmaxf(ku[0], ku[1]))) return false;
+              hi = fmaxf(hi, fmaxf(ku[0], ku[1]));
+              put_words(t_s + 16, scale_byte(ku[0]) | scale_byte(ku[1]) << 8);
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bars + kPHalf + team);
             }
           }
-          if (u != u_old || g == g0) *u_at = u;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bars + kU + 4 * team + quarter);
-          uint32_t word = 0x7F7F7F7Fu;                        // scale bytes of P's codes, 2^(kb + ev - u - 8)
-#pragma unroll
-          for (int c = 0; c < kBlocks; ++c) {
-            l = fmaf(sums[c], ex2_approx(kb[c] - m - 8.f), l);
-            const uint32_t sb = static_cast<uint32_t>(fminf(fmaxf(kb[c] + ev[c] - u + 119.f, 0.f), 254.f));
-            if (kCopies == 1) word = c == 0 ? sb : word | sb << (8 * c);
-            else word = (word & ~(0xFFu << (8 * (c0 + c)))) | sb << (8 * (c0 + c));
+          if (kCopies > 1) {
+            const uint32_t zeros[16] = {};                    // other copies' blocks
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c)
+              if (c < c0 || c >= c0 + kBlocks) tmem_st16(t_s + 32 * c, zeros);
+            if (kBlocks == 1) ku[1] = ku[0];
+            if (!know_u(fmaxf(ku[0], ku[1]))) return false;
           }
-          const uint32_t words[8] = {word, word, word, word, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
-          tmem_st8(t_s + 16, words);
+          hi = fmaxf(hi, fmaxf(ku[0], ku[1]));
+          const uint32_t two = scale_byte(ku[0]) | scale_byte(ku[1]) << 8;
+          if (kCopies == 1) put_words(t_s + 80, two << 16);
+          else put_words(t_s + 16, kBlocks == 1 ? (two & 0xFFu) << (8 * c0) : two << (8 * c0));
           return true;
         };
         for (int g = g0 + (team + kTeams - g0 % kTeams) % kTeams; ok && g < g0 + n_tiles; g += kTeams) {
@@ -843,7 +854,10 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           if (!ok) break;
           tc_fence_after();
           if (idle) {
-            if (lane == 0) mbar_arrive(bars + kU + 4 * team + quarter);
+            if (lane == 0) {
+              if (g == g0) mbar_arrive(bars + kU + quarter);
+              if (kCopies == 1) mbar_arrive(bars + kPHalf + team);
+            }
           } else if (!(ok = cut ? tile(g, t, std::true_type{}) : tile(g, t, std::false_type{}))) {
             break;
           }
@@ -860,6 +874,8 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         // Output, by all teams: over the teams and copies of a row, the largest references and the sum; each lane's values count w of it.
         if (ok) ok = wait_warp(bar(kPv + (g0 - 1) % kTeams), phase_of(g0 - 1), abort_flag);
         stats[128 * team + in_tile] = make_float2(m, l);
+        // out of u's range: above; or below where u was not taken from the row's own products
+        marked |= hi > u + 95.f || ((u_code & 1) != 0 && hi > kNone && hi < u - 80.f);
         if (real && marked) {
           marks[128 * parity + row] = 1;
           any_marked[parity] = 1;
@@ -869,11 +885,14 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (more) put_queries(next, parity ^ 1);              // all S of this unit have been computed; those of the next run under the output
         const bool whole = !kCluster && x.whole();
         float m_all = kNone, u_all = kNone, l_all = 0.f;
+        volatile int* unit_u = u_at - in_tile + row;          // of the row's copies
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) {
-          u_all = fmaxf(u_all, *(u_at - in_tile + row + c * kRows));
+          float m_copy = kNone;
 #pragma unroll
-          for (int y = 0; y < kTeams; ++y) m_all = fmaxf(m_all, stats[128 * y + row + c * kRows].x);
+          for (int y = 0; y < kTeams; ++y) m_copy = fmaxf(m_copy, stats[128 * y + row + c * kRows].x);
+          m_all = fmaxf(m_all, m_copy);
+          if (m_copy > kNone) u_all = fmaxf(u_all, static_cast<float>(unit_u[c * kRows] >> 1));
         }
 #pragma unroll
         for (int c = 0; c < kCopies; ++c)
@@ -882,7 +901,8 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             const float2 st = stats[128 * y + row + c * kRows];
             l_all = fmaf(st.y, ex2_approx(st.x - m_all), l_all);
           }
-        const float w = ex2_approx(*u_at - u_all);
+        if (!(u_all > kNone)) u_all = static_cast<float>(kUnitLift);        // the row sees nothing here (NaN keys aside)
+        const float w = ex2_approx(static_cast<float>(*u_at >> 1) - u_all);
         // (in two factors: what V's scales leave may be beyond either's range)
         const float d_all = u_all - m_all, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
         const float w1 = whole ? w * exp2f(d1) : w, w2 = whole ? exp2f(d_all - d1) / l_all : 1.f;
@@ -891,47 +911,76 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           cg::this_cluster().sync();
           met = true;
         }
-        // 16 columns at a time, through shared memory: four lanes a row, eight rows a warp at a time; 16-byte pieces XORed with the lane
-        const uint32_t stage = sbase + C::kSmemOut + team * 8192;
+        if constexpr (kCopies == 1) {                         // 16 columns at a time, a row a lane
+          const int at = out_rows[128 * parity + row], to = row / rows_each;
+          float* part = p.part_o + (static_cast<int64_t>(slot) * kRows + row) * D;
+          if constexpr (kCluster)
+            part = reinterpret_cast<float*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemRing) + (rank * rows_each + row - to * rows_each) * D;
 #pragma unroll 1
-        for (int c = team; c < D / 16; c += kTeams) {
-          uint32_t o[16];
-          tmem_ld16(t_o + 16 * c, o);
-          tmem_wait_ld();
+          for (int c = team; c < D / 16; c += kTeams) {
+            uint32_t o[16];
+            tmem_ld16(t_o + 16 * c, o);
+            tmem_wait_ld();
+            float y[16];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = __uint_as_float(o[4 * e + k]) * w1 * w2;
-            sts_u4(stage + in_tile * 64 + ((e ^ ((lane >> 1) & 3)) << 4), __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
-          }
-          if (kCopies > 1) bar_sync(1 + team, 128);
-          else __syncwarp();
-          const int piece = lane & 3;
-#pragma unroll
-          for (int k = 0; k < 4 / kCopies; ++k) {
-            const int r = quarter * (kRows / 4) + 8 * k + (lane >> 2);
-            float4 y = lds_f4(stage + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-#pragma unroll
-            for (int cc = 1; cc < kCopies; ++cc) {
-              const float4 z = lds_f4(stage + (r + cc * kRows) * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-              y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
-            }
-            const int at = out_rows[128 * parity + r];
+            for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(o[e]) * w1 * w2;
             if (at < 0) continue;
-            if constexpr (kCluster) {
-              const int to = r / rows_each;
-              *reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemRing + ((rank * rows_each + r - to * rows_each) * D + 16 * c + 4 * piece) * 4) = y;
-            } else if (whole) {
-              const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
-              *reinterpret_cast<uint2*>(p.o + static_cast<int64_t>(at) * D + 16 * c + 4 * piece) =
-                  make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+            if (whole) {
+              uint32_t h[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]);
+                h[e] = *reinterpret_cast<const uint32_t*>(&b2);
+              }
+              uint4* to_o = reinterpret_cast<uint4*>(p.o + static_cast<int64_t>(at) * D + 16 * c);
+              to_o[0] = make_uint4(h[0], h[1], h[2], h[3]);
+              to_o[1] = make_uint4(h[4], h[5], h[6], h[7]);
             } else {
-              *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * kRows + r) * D + 16 * c + 4 * piece) = y;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) reinterpret_cast<float4*>(part + 16 * c)[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
             }
           }
-          if (kCopies > 1) bar_sync(1 + team, 128);
-          else __syncwarp();
+        } else {
+          // through shared memory: four lanes a row, eight rows a warp at a time; 16-byte pieces XORed with the lane
+          const uint32_t stage = sbase + C::kSmemOut + team * 8192;
+#pragma unroll 1
+          for (int c = team; c < D / 16; c += kTeams) {
+            uint32_t o[16];
+            tmem_ld16(t_o + 16 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float y[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) y[k] = __uint_as_float(o[4 * e + k]) * w1 * w2;
+              sts_u4(stage + in_tile * 64 + ((e ^ ((lane >> 1) & 3)) << 4), __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+            }
+            bar_sync(1 + team, 128);
+            const int piece = lane & 3;
+#pragma unroll
+            for (int k = 0; k < 4 / kCopies; ++k) {
+              const int r = quarter * (kRows / 4) + 8 * k + (lane >> 2);
+              float4 y = lds_f4(stage + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+#pragma unroll
+              for (int cc = 1; cc < kCopies; ++cc) {
+                const float4 z = lds_f4(stage + (r + cc * kRows) * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+                y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+              }
+              const int at = out_rows[128 * parity + r];
+              if (at < 0) continue;
+              if constexpr (kCluster) {
+                const int to = r / rows_each;
+                *reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemRing + ((rank * rows_each + r - to * rows_each) * D + 16 * c + 4 * piece) * 4) = y;
+              } else if (whole) {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+                *reinterpret_cast<uint2*>(p.o + static_cast<int64_t>(at) * D + 16 * c + 4 * piece) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+              } else {
+                *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * kRows + r) * D + 16 * c + 4 * piece) = y;
+              }
+            }
+            bar_sync(1 + team, 128);
+          }
         }
         const bool mine = team == 0 && copy == 0 && real;
         const int head = x.hk * p.rep + unit_row - node * p.rep;
@@ -1012,7 +1061,7 @@ __global__ void __launch_bounds__(128) cache_tree_join_kernel(const __grid_const
     const int64_t at = there ? static_cast<int64_t>(w == x.first ? x.slot : 2 * w) * p.row_tile + r : 0;
     const float4 ml = there ? p.part_ml[at] : make_float4(kNone, 0.f, kNone, 0.f);
     marked |= __any_sync(0xffffffffu, ml.w != 0.f);
-    float top_new = ml.x, u_new = ml.z;
+    float top_new = ml.x, u_new = ml.x > kNone ? ml.z : kNone;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, o));
