@@ -29,7 +29,7 @@ __device__ __forceinline__ float2 turn(double angle) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kRotaryWarps * 32) cache_rotary_kernel(const CacheRotaryParams p, const int blocks, const int group) {
+__global__ void __launch_bounds__(kRotaryWarps * 32, 3) cache_rotary_kernel(const CacheRotaryParams p, const int blocks, const int group) {
   constexpr int kTpr = D / 16, kRpp = 32 / kTpr, kPass = 32 / kRpp;      // lanes a row, rows a pass, passes
   // cos and sin of (row, pair): four float4 of two pairs each for a lane's eight pairs, lane after lane, so that the lanes of a load lie side by side
   extern __shared__ float4 turns[];
@@ -126,44 +126,36 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) cache_rotary_kernel(const C
     const float s_old = (j == 0 && r_begin > 0) ? *scale_at : 0.f;
     const __nv_bfloat16* x = is_v ? p.v + b * p.v_sb + hk * p.v_sh : p.k + b * p.k_sb + hk * p.k_sh;
     const int64_t sn = is_v ? p.v_sn : p.k_sn;
-    uint4 y[kPass][2];
-#pragma unroll
-    for (int ps = 0; ps < kPass; ++ps) {
-      const int r = r0 + ps * kRpp;
-      y[ps][0] = y[ps][1] = make_uint4(0, 0, 0, 0);
-      if (r >= r_begin && r < r_end) {
-        const uint4* src = reinterpret_cast<const uint4*>(x + (slot0 + r - start) * sn);
-        y[ps][0] = __ldg(src + va);
-        y[ps][1] = __ldg(src + vb);
-      }
-    }
-    auto values = [&](int ps, float (&f)[16]) {
+    // The rows twice, once for the maximum, once for the codes: the second time from L1 (held in registers they left room for eight warps an SM).
+    auto values = [&](int r, float (&f)[16]) {
+      const uint4* src = reinterpret_cast<const uint4*>(x + (slot0 + r - start) * sn);
+      const uint4 a = __ldg(src + va), b4 = __ldg(src + vb);
       if (is_v) {
-        bf16x8_to_float(y[ps][0], f);
-        bf16x8_to_float(y[ps][1], f + 8);
+        bf16x8_to_float(a, f);
+        bf16x8_to_float(b4, f + 8);
       } else {
-        rotate(y[ps][0], y[ps][1], r0 + ps * kRpp, f);
+        rotate(a, b4, r, f);
       }
     };
     float amax = 0.f;                                         // NaN never wins
-#pragma unroll
+#pragma unroll 4
     for (int ps = 0; ps < kPass; ++ps) {
       const int r = r0 + ps * kRpp;
       if (r < r_begin || r >= r_end) continue;
       float f[16];
-      values(ps, f);
+      values(r, f);
 #pragma unroll
       for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(f[e]));
     }
     amax = warp_max(amax);
     const float s = fmaxf(sb_to_scale(pow2_sb(amax, 1u)), s_old);
     const float inv = sb_to_inv(scale_to_sb(s));
-#pragma unroll
+#pragma unroll 4
     for (int ps = 0; ps < kPass; ++ps) {
       const int r = r0 + ps * kRpp;
       if (r < r_begin || r >= r_end) continue;
       float f[16];
-      values(ps, f);
+      values(r, f);
       uint2* to = reinterpret_cast<uint2*>(codes + r * c.c_slot);
       to[va] = make_uint2(cvt_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), cvt_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
       to[vb] = make_uint2(cvt_e4m3x4(f[8] * inv, f[9] * inv, f[10] * inv, f[11] * inv), cvt_e4m3x4(f[12] * inv, f[13] * inv, f[14] * inv, f[15] * inv));
@@ -184,8 +176,11 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) cache_rotary_kernel(const C
 
 cudaError_t launch_cache_rotary(int D, const CacheRotaryParams& p, cudaStream_t stream) {
   const int blocks = (p.N + 30) / 32 + 1, heads = 2 * p.c.Hk + p.H;      // blocks that N tokens can touch behind any start
-  const int group = heads < kRotaryWarps ? heads : kRotaryWarps;
-  const dim3 grid(static_cast<unsigned>(p.c.B) * blocks, (heads + group - 1) / group);
+  // heads to a CTA: all, which share its sines and cosines, where there are blocks enough for the SMs; otherwise fewer, a warp each at least
+  const int64_t all = static_cast<int64_t>(p.c.B) * blocks, want = 4ll * sm_count();
+  const int most = (heads + kRotaryWarps - 1) / kRotaryWarps;
+  const int groups = static_cast<int>(all >= want ? 1 : (want + all - 1) / all < most ? (want + all - 1) / all : most), group = (heads + groups - 1) / groups;
+  const dim3 grid(static_cast<unsigned>(all), groups);
   const int smem = 32 * p.half * 8;
   count_launch();
   return D == 128 ? launch_chained(cache_rotary_kernel<128>, grid, kRotaryWarps * 32, smem, stream, p, blocks, group)

@@ -8,60 +8,68 @@ namespace dm {
 namespace {
 
 // ------------------------------------------------------------------------------------------------ depths and ancestors
-// seen_i = {i} united with seen of i's parent; depth_i = |seen_i| - 1.  By doubling: after round r a node's set holds its first 2^r ancestors and itself
-// and jump names the ancestor behind them, so a tree of depth d takes log2(d) + 1 rounds.  One CTA a sequence, one thread a node, the sets in shared
-// memory word by word, so that the threads of a warp write adjacent words.
+// seen_i = {i} united with seen of i's parent; depth_i = |seen_i| - 1.  One CTA a sequence, one thread a node.  A warp's 32 nodes first find their ancestors among
+// themselves, by doubling with shuffles (five rounds), and the ancestor behind those; then each node walks from group of 32 to group of 32, at most as many steps as it has words.
 __global__ void __launch_bounds__(1024) draft_tree_kernel(const DraftTreeParams p, const int words) {
-  extern __shared__ uint32_t sets[];                          // (words, N)
-  __shared__ int jumps[kMaxNodes];
+  extern __shared__ uint32_t sets[];                          // (N, pitch)
+  __shared__ uint32_t among[kMaxNodes];                       // of a node, its ancestors in its group and itself
+  __shared__ int behind[kMaxNodes];                           // and the nearest ancestor in an earlier group, or -1
   grid_dep_wait();
-  const int b = blockIdx.x, i = threadIdx.x, N = p.N, count = checked_count(p.status, p.counts, b, N);
-  int jump = -1;
+  const int b = blockIdx.x, i = threadIdx.x, lane = i & 31, N = p.N, pitch = words | 1, count = checked_count(p.status, p.counts, b, N);
+  int parent = -1;
   if (i < count) {
-    jump = __ldg(p.parents + b * p.row + i);
-    if (jump < -1 || jump >= i) {                             // no earlier node
+    parent = __ldg(p.parents + b * p.row + i);
+    if (parent < -1 || parent >= i) {                         // no earlier node
       report(p.status, kStatusBadTree + kInCache);
-      jump = -1;
+      parent = -1;
     }
   }
-  if (i < N) {
-    for (int w = 0; w < words; ++w) sets[w * N + i] = i < count && w == i >> 5 ? 1u << (i & 31) : 0u;
-    jumps[i] = jump;
-  }
-  while (__syncthreads_or(jump >= 0)) {
-    int next = -1;
-    if (jump >= 0) next = jumps[jump];
-    const int last = jump >= 0 ? jump >> 5 : -1;              // ancestors come before: the words up to the jump's own
-    for (int w0 = 0; w0 < words; w0 += 8) {                   // eight words at a time: read by all before any is written
-      uint32_t x[8];
+  const int first = i - lane;
+  uint32_t mask = i < count ? 1u << lane : 0u;
+  int jump = parent >= first ? parent - first : -1, exit = parent >= first ? -1 : parent;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) x[w] = w0 + w <= last ? sets[(w0 + w) * N + jump] : 0u;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < 8; ++w)
-        if (w0 + w <= last) sets[(w0 + w) * N + i] |= x[w];
+  for (int r = 0; r < 5; ++r) {                               // after it, the first 2^(r + 1) ancestors of the group
+    const int from = max(jump, 0);
+    const uint32_t m = __shfl_sync(0xffffffffu, mask, from);
+    const int j = __shfl_sync(0xffffffffu, jump, from), x = __shfl_sync(0xffffffffu, exit, from);
+    if (jump >= 0) {
+      mask |= m;
+      exit = x;
+      jump = j;
     }
-    if (i < N) jumps[i] = next;
-    jump = next;
   }
+  among[i] = mask;
+  behind[i] = exit;
+  for (int x = i; x < N * pitch; x += blockDim.x) sets[x] = 0u;
+  __syncthreads();
   if (i < N) {
-    int bits = 0;
-    for (int w = 0; w < words; ++w) bits += __popc(sets[w * N + i]);
+    int bits = __popc(mask);
+    sets[i * pitch + (i >> 5)] = mask;
+    for (int at = exit; at >= 0; at = behind[at]) {           // the groups fall
+      const uint32_t m = among[at];
+      sets[i * pitch + (at >> 5)] = m;
+      bits += __popc(m);
+    }
     p.depth[static_cast<int64_t>(b) * N + i] = max(0, bits - 1);
   }
+  __syncthreads();
   uint32_t* out = p.seen + static_cast<int64_t>(b) * N * words;
-  for (int x = i; x < N * words; x += blockDim.x) out[x] = sets[(x % words) * N + x / words];
+  for (int row = i / words, w = i - row * words; row < N;) {
+    out[row * words + w] = sets[row * pitch + w];
+    const int rows = blockDim.x / words;                      // the CTA's threads are whole rows: 32 a word
+    row += rows;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ keeping a path
 // Token path[i] behind `before` becomes token i behind it.  A CTA is a (sequence, kv head, K or V), a warp a block of 32 tokens that is written: it reads
 // the block's older tokens and its tokens of the path, takes the smallest power-of-two scale that holds them (as the eviction does), and rounds the codes
 // to it.  A path is strictly increasing, so a token never moves up: what a block takes lies in it or behind it, and the warps of a CTA read all that
-// they need before any of them writes; blocks of a later round are behind those.
-constexpr int kKeepWarps = 8;
+// they need before any of them writes; blocks of a later round are behind those.  The path is looked over while the first round's codes are on their way.
+constexpr int kKeepWarps = 4;
 
 template <int D>
-__global__ void __launch_bounds__(kKeepWarps * 32) cache_keep_kernel(const CacheKeepParams p) {
+__global__ void __launch_bounds__(kKeepWarps * 32, D == 128 ? 8 : 4) cache_keep_kernel(const CacheKeepParams p) {
   constexpr int kTpr = D / 16, kRpp = 32 / kTpr, kPass = 32 / kRpp;      // lanes a row, rows a pass, passes
   grid_dep_wait();
   const CacheView& c = p.c;
@@ -82,23 +90,19 @@ __global__ void __launch_bounds__(kKeepWarps * 32) cache_keep_kernel(const Cache
     const int at = __ldg(path + i);
     bad |= at < 0 || at >= n - start || (i > 0 && __ldg(path + i - 1) >= at);
   }
-  if (__syncthreads_or(bad)) {                                // not a path: nothing of the sequence is changed
-    if (threadIdx.x == 0) report(c.status, kStatusBadTree + kInCache);
-    count = 0;
-  }
-  if (hk == 0 && !is_v && threadIdx.x == 0) p.new_lengths[b] = start + count;
-  if (count == 0) return;
+  bool first_round = true;
   uint8_t* codes = (is_v ? c.v8 : c.k8) + hk * c.c_head;
   float* scales = (is_v ? c.vs : c.ks) + hk * c.s_head;
-  const int bpp = c.page / 32, first = start / 32, blocks = (start + count - 1) / 32 - first + 1;
+  const int bpp = c.page / 32, first = start / 32, blocks = count > 0 ? (start + count - 1) / 32 - first + 1 : 1;
   const int c16 = (lane % kTpr) * 16, r0 = lane / kTpr;
   for (int j0 = 0; j0 < blocks; j0 += blockDim.x / 32) {
     const int blk = first + j0 + warp, row = blk * 32 + lane; // this lane's row of the block, of 32
-    const bool live = j0 + warp < blocks, held = live && row < start + count;
+    const bool live = j0 + warp < blocks, held = live && row < start + count && (row < start || start < n);
     int page = 0, slot = 0;
     bool good = held;
     if (held) {
-      const int from = row < start ? row : start + __ldg(path + row - start), entry = from / c.page;
+      // (not known to be a path yet: within the sequence in any case)
+      const int from = row < start ? row : start + min(max(__ldg(path + row - start), 0), max(n - start - 1, 0)), entry = from / c.page;
       slot = from - entry * c.page;
       page = checked_page(c, __ldg(c.table + b * c.t_row + entry));
       good = page >= 0;
@@ -129,8 +133,16 @@ __global__ void __launch_bounds__(kKeepWarps * 32) cache_keep_kernel(const Cache
     const float s = sb_to_scale(sb);
     // the block's own place
     const int entry = live ? blk / bpp : 0;
-    const int to = live ? checked_page(c, __ldg(c.table + b * c.t_row + entry)) : -1;
-    __syncthreads();
+    const int to = live && count > 0 && entry < c.T ? checked_page(c, __ldg(c.table + b * c.t_row + entry)) : -1;
+    if (first_round) {                                        // not a path: nothing of the sequence is changed
+      first_round = false;
+      bad = __syncthreads_or(bad) != 0;
+      if (bad && threadIdx.x == 0) report(c.status, kStatusBadTree + kInCache);
+      if (hk == 0 && !is_v && threadIdx.x == 0) p.new_lengths[b] = start + (bad ? 0 : count);
+      if (bad) return;
+    } else {
+      __syncthreads();
+    }
     if (to >= 0) {
       uint8_t* out = codes + to * c.c_page + static_cast<int64_t>(blk - entry * bpp) * 32 * c.c_slot + c16;
 #pragma unroll
@@ -152,13 +164,13 @@ __global__ void __launch_bounds__(kKeepWarps * 32) cache_keep_kernel(const Cache
 }  // namespace
 
 cudaError_t launch_draft_tree(const DraftTreeParams& p, cudaStream_t stream) {
-  const int words = (p.N + 31) / 32, threads = words * 32, smem = words * p.N * 4;
+  const int words = (p.N + 31) / 32, threads = words * 32, smem = (words | 1) * p.N * 4;
   if (smem > 40 * 1024) {                                     // beyond what a kernel has unasked, its static arrays aside
     static bool allowed[64] = {};                             // once per device: the driver call takes longer than a launch
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !allowed[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(draft_tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxNodes / 32 * kMaxNodes * 4);
+      const cudaError_t e = cudaFuncSetAttribute(draft_tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxNodes / 32 + 1) * kMaxNodes * 4);
       if (e != cudaSuccess) return e;
       if (dev >= 0 && dev < 64) allowed[dev] = true;
     }
