@@ -98,36 +98,40 @@ __global__ void __launch_bounds__(kKeepWarps * 32, D == 128 ? 8 : 4) cache_keep_
   for (int j0 = 0; j0 < blocks; j0 += blockDim.x / 32) {
     const int blk = first + j0 + warp, row = blk * 32 + lane; // this lane's row of the block, of 32
     const bool live = j0 + warp < blocks, held = live && row < start + count && (row < start || start < n);
-    int page = 0, slot = 0;
-    bool good = held;
+    int64_t at = -1;                                          // its codes
+    float s_row = 0.f;
     if (held) {
       // (not known to be a path yet: within the sequence in any case)
       const int from = row < start ? row : start + min(max(__ldg(path + row - start), 0), max(n - start - 1, 0)), entry = from / c.page;
-      slot = from - entry * c.page;
-      page = checked_page(c, __ldg(c.table + b * c.t_row + entry));
-      good = page >= 0;
+      const int slot = from - entry * c.page, page = checked_page(c, __ldg(c.table + b * c.t_row + entry));
+      if (page >= 0) {
+        at = page * c.c_page + slot * c.c_slot;
+        s_row = scales[page * c.s_page + slot / 32];
+      }
     }
-    const float s_row = good ? scales[page * c.s_page + slot / 32] : 0.f;
     uint4 y[kPass];
     float top = 0.f;                                          // of this lane's rows' codes, times their scales
     float s_of[kPass];
 #pragma unroll
     for (int ps = 0; ps < kPass; ++ps) {
       const int r = r0 + ps * kRpp;
-      const int page_r = __shfl_sync(0xffffffffu, page, r), slot_r = __shfl_sync(0xffffffffu, slot, r);
-      const bool good_r = __shfl_sync(0xffffffffu, good ? 1 : 0, r) != 0;
+      const int64_t at_r = __shfl_sync(0xffffffffu, at, r);
       s_of[ps] = __shfl_sync(0xffffffffu, s_row, r);
       y[ps] = make_uint4(0, 0, 0, 0);
-      if (good_r) y[ps] = *reinterpret_cast<const uint4*>(codes + page_r * c.c_page + slot_r * c.c_slot + c16);
+      if (at_r >= 0) y[ps] = *reinterpret_cast<const uint4*>(codes + at_r + c16);
     }
 #pragma unroll
     for (int ps = 0; ps < kPass; ++ps) {
       const uint32_t w[4] = {y[ps].x, y[ps].y, y[ps].z, y[ps].w};
-      uint32_t m = 0;                                         // sizes of codes are in the order of their bytes; NaN is left out
+      // sizes of codes are in the order of their bytes; one more, so that NaN is the least (as f16 pairs the maximum took half as long again)
+      uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m = __vmaxu4(m, w[i] & 0x7F7F7F7Fu & ~nan_codes(w[i]));
-      m = max(max(m & 0xFFu, (m >> 8) & 0xFFu), max((m >> 16) & 0xFFu, m >> 24));
-      top = fmaxf(top, f16x2_to_float2(e4m3_lo_f16x2(m)).x * s_of[ps]);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t even = ((w[i] & 0x007F007Fu) + 0x00010001u) & 0x007F007Fu, odd = ((w[i] >> 8 & 0x007F007Fu) + 0x00010001u) & 0x007F007Fu;
+        m = __vmaxu2(m, __vmaxu2(even, odd));
+      }
+      m = max(m & 0xFFFFu, m >> 16);
+      top = fmaxf(top, f16x2_to_float2(e4m3_lo_f16x2(m > 0 ? m - 1 : 0)).x * s_of[ps]);
     }
     const uint32_t sb = pow2_sb(warp_max(top), 1u);
     const float s = sb_to_scale(sb);
