@@ -6,7 +6,7 @@
 // Rows are (drafted token, head of the kv head's group); a unit is (sequence, kv head, up to 128 rows).  The codes of K and V go to the tensor cores as
 // they lie in the pages, no code is ever converted: S = Q K^T is the sum of two kind::f8f6f4 chains with q in two codes, e4m3 and what that leaves in e5m2
 // (4 and 3 significant bits, of bf16's 8 with the signs: exact down to 2^-13 of the row's largest element, 2^-21 of that off below), and O += P V the sum
-// of two block-scaled chains with P in two e4m3 codes relative to the largest of its 32 keys (off by 2^-8 of itself at most, 2^-17 of that largest one where it is
+// of two block-scaled chains with P in two e4m3 codes relative to the largest of its 32 keys (off by 2^-8 of itself at most, 2^-16 of that largest one where it is
 // small).  The power-of-two scale of V's block goes into P's scale byte and that of K's block into the factor of the logits.
 //
 // The key tiles of 128 tokens of all units are one flat range, divided evenly over the CTAs of one wave; pieces of cut units are joined by a second kernel.
@@ -247,17 +247,14 @@ __device__ __forceinline__ uint32_t cvt_e5m2x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Four values up to 448 -> four e4m3 codes, and the codes of what these leave.
+// Four values up to 448 -> four e4m3 codes of their first four significant bits, cut off, and the codes of the rest.  (Rounding to nearest would halve the error, but to know
+// what a rounded code left is to convert it back: 580 instead of 450 cycles for 32 exponentials and their codes of a warp alone, 390 instead of 340 of two warps a scheduler.)
 __device__ __forceinline__ void split4(float2 x, float2 y, uint32_t& first, uint32_t& second) {
-  asm("{\n\t.reg .b16 a, b;\n\t.reg .b32 h, g, u, v;\n\t"
-      "cvt.rn.f16x2.f32 h, %3, %2;\n\tcvt.rn.f16x2.f32 g, %5, %4;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 a, h;\n\tcvt.rn.satfinite.e4m3x2.f16x2 b, g;\n\t"
-      "mov.b32 %0, {a, b};\n\t"
-      "cvt.rn.f16x2.e4m3x2 u, a;\n\tcvt.rn.f16x2.e4m3x2 v, b;\n\t"
-      "sub.rn.f16x2 h, h, u;\n\tsub.rn.f16x2 g, g, v;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 a, h;\n\tcvt.rn.satfinite.e4m3x2.f16x2 b, g;\n\t"
-      "mov.b32 %1, {a, b};\n\t}"
-      : "=r"(first), "=r"(second) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFF00000u); };
+  const float2 a = make_float2(cut(x.x), cut(x.y)), b = make_float2(cut(y.x), cut(y.y));
+  first = cvt_e4m3x4(a.x, a.y, b.x, b.y);
+  const float2 u = add2(x, make_float2(-a.x, -a.y)), v = add2(y, make_float2(-b.x, -b.y));
+  second = cvt_e4m3x4(u.x, u.y, v.x, v.y);
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"

@@ -99,9 +99,8 @@ def attention(q, cache, table, lengths, counts, see, scale):
     its row's largest brought to 2^7 ... 2^8: e4m3 (4 bits; a step of 2^-9 below 2^-6) and what that leaves in e5m2 (3 bits).  What is left of an element of at least 2^-6 is at
     most 8 times its eighth bit, which 3 bits hold; below, at most 2^-10 is left, on steps of 2^-13: off by 2^-14, 2^-21 of the largest element.  That times the sum of the
     sizes of the key's channels.  Both move a probability by twice as much relatively; exp2 and the fp32 sums by 2^-19.  A probability is held in the output product
-    with the largest of its block of 32 keys brought to 2^7 ... 2^8, in f16 (off by 2^-11 of itself), of that an e4m3 code (off by half a step, 2^(e-4) for 2^e ...
-    2^(e+1)) and an e4m3 code of the rest, 2^(e-4) at most: off by 2^(e-9).  Together less than 2^-8 of itself; where the second code is below 2^-6, by 2^-10, which is
-    2^-17 of the block's largest.  o is rounded to bf16 (2^-8)."""
+    with the largest of its block of 32 keys brought to 2^7 ... 2^8 as an e4m3 code of its first four bits (below 2^(e-3) is left, for 2^e ... 2^(e+1)) and an e4m3 code of
+    the rest, off by 2^(e-8): 2^-8 of itself.  Where either is below 2^-6 its code is off by up to 2^-10: together 2^-9, 2^-16 of the block's largest.  o is rounded to bf16 (2^-8)."""
     B, N, H, D = q.shape
     Hk, P = cache.k8.shape[1:3]
     dev = "cuda"
@@ -134,6 +133,6 @@ def attention(q, cache, table, lengths, counts, see, scale):
                     rows = [[x[i, sees[i]] @ y[sees[i]] for x, y in ((p, v), (p, v.abs()), (top, v.abs()))] for i in range(count)]
                     pv, pav, tav = (torch.stack(x) for x in zip(*rows))
                 o[b, :count, hh] = pv
-                do[b, :count, hh] = 2.0 ** -8 * pv.abs() + (2.0 ** -8 + 2 * eps + 2.0 ** -19)[:, None] * pav + 2.0 ** -17 * tav + 1e-37
+                do[b, :count, hh] = 2.0 ** -8 * pv.abs() + (2.0 ** -8 + 2 * eps + 2.0 ** -19)[:, None] * pav + 2.0 ** -16 * tav + 1e-37
                 dlse[b, hh, :count] = eps + 2.0 ** -19 + 2.0 ** -22 * lse[b, hh, :count].abs()
     return (o, lse), (do, dlse)
