@@ -1147,27 +1147,64 @@ cudaError_t launch_tree(const CUtensorMap& tk, const CUtensorMap& tv, const Cach
   return launch_chained(cache_tree_join_kernel<D>, dim3(p.grid, p.row_tile / 4), 128, 0, stream, p);
 }
 
-// Tiles of a CTA up to which a cluster takes a unit.
+// Clusters of 2^log CTAs that the device holds at a time: fewer than its SMs would (of 148, 33 of four and 15 of eight), since a cluster lies within a part of the chip.
+int resident_clusters(int log) {
+  static int cached[64][4] = {};                              // + 1
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && cached[dev][log] > 0) return cached[dev][log] - 1;
+  using C = TreeCfg<128>;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1u << log;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(1u << log);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (allow_smem<cache_tree_kernel<128, 1, true>>(C::kSmem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, cache_tree_kernel<128, 1, true>, &cfg) != cudaSuccess) {
+    cudaGetLastError();                                       // no device: sizes are asked for all the same
+    return 0;
+  }
+  if (dev >= 0 && dev < 64) cached[dev][log] = n + 1;
+  return n;
+}
+
+// Tiles of a CTA up to which a cluster takes a unit: the lengths may be shorter than the table, which the even division makes good and a cluster does not.
 constexpr int kClusterTiles = 12;
+// Tiles that a CTA of a cluster may have above its even share: what the join by a second kernel is worth.
+constexpr int kClusterGain = 4;
+// Tiles that a CTA of the even division has at least, or the join has too many pieces.
+constexpr int kWorkerTiles = 4;
 
 }  // namespace
 
+// Measured, in us (GPU time, H 32, Hk 8; a cluster a unit against the even division): one sequence of 8000 tokens with 8 drafts 16.1 and 17.4, four of 1000 with 16 drafts 14.0
+// and 17.3, of 4000 19.6 and 22.3; three of 12000 with 8 drafts, 24 tiles a CTA against 15, 30.4 and 27.3; 16 units of 8000 tokens in clusters of 8, of which 15 are resident,
+// 30.2 and 20.1 (so clusters of 4: CacheTreePlan).  Pieces of 4 tiles against 2 in a sequence of 16000 tokens with 2 kv heads: 21.0 and 24.7; of 8, one of 12000 with 8 kv
+// heads: 21.0 and 19.4.
 CacheTreePlan plan_cache_tree(int B, int N, int H, int Hk, int D, int T, int page) {
   CacheTreePlan x;
   const int64_t R = static_cast<int64_t>(N) * (H / Hk), wave = sm_count();
-  x.row_tile = R <= 32 ? 32 : R <= 64 ? 64 : 128;
+  x.row_tile = R <= 32 ? 32 : R <= 64 ? 64 : 128;             // 8000 tokens, 8 drafts of 4 heads: 16.1 us with 32, 23.1 with 128; 4 x 4000 with 16 drafts: 19.6 with 64, 24.8
   const int64_t unit_tiles = (static_cast<int64_t>(T) * page + 127) / 128, units = static_cast<int64_t>(B) * Hk * ((R + x.row_tile - 1) / x.row_tile);
-  // A cluster a unit where its CTAs have few tiles each and all are resident at a time.
-  int cl = 1;
-  while (cl < kMaxCluster && units * cl * 2 <= wave && cl < unit_tiles) cl *= 2;
-  x.cluster = units * cl <= wave && unit_tiles <= static_cast<int64_t>(kClusterTiles) * cl ? cl : 0;
+  const int64_t pieces = units * ((unit_tiles + kWorkerTiles - 1) / kWorkerTiles);
+  const int64_t workers = pieces < wave ? pieces : wave;      // one wave
+  // A cluster a unit where its CTAs have few tiles each, not many more than their share, and all are resident at a time.
+  int log = 0;
+  while ((2 << log) <= kMaxCluster && (1 << log) < unit_tiles && units <= resident_clusters(log + 1)) ++log;
+  const int64_t tiles = (unit_tiles + (1 << log) - 1) >> log;
+  x.cluster = units <= resident_clusters(log) && tiles <= kClusterTiles && tiles <= (units * unit_tiles + workers - 1) / workers + kClusterGain ? 1 << log : 0;
   if (x.cluster > 0) {
-    x.grid = static_cast<int>(units) * cl;
+    x.grid = static_cast<int>(units) * x.cluster;
     x.part_o_bytes = x.part_ml_bytes = 0;
     x.cut_bytes = 16;
     return x;
   }
-  x.grid = static_cast<int>(units * unit_tiles < wave ? units * unit_tiles : wave);      // one wave, and no more workers than there can be tiles
+  x.grid = static_cast<int>(workers);
   x.part_o_bytes = 2ll * x.grid * x.row_tile * D * 4;
   x.part_ml_bytes = 2ll * x.grid * x.row_tile * 16;
   x.cut_bytes = x.grid * static_cast<int64_t>(sizeof(TreeCut));
