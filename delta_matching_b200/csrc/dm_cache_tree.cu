@@ -459,8 +459,11 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
   if (kCluster || f_begin < f_end) {
     if (role >= 0 && D == 128) reg_dec<C::kRegsOther>();
-    if (role == 0) {
-      // ---------------------------------------------------------------------------------------- TMA: code tiles and their scales
+    if (role == 0 || role == 3) {
+      // ---------------------------------------------------------------------------------------- TMA: K tiles and the scales of both; V tiles
+      // (a warp each: the four boxes of a tile take a warp 800 cycles, and one warp for both held up the whole CTA)
+      const int kv = role == 3;
+      const TreePiece first = x;
       // Eight tiles at a time, a lane a block: a batch's pages are asked for two batches ahead of its loads and its scales one ahead (a tile takes less than the
       // two loads, one behind the other, that lead to its codes).
       struct Batch {
@@ -475,6 +478,14 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       auto look_up = [&]() {
         Batch a{};
         int b = 0, blk = 0;
+        if (more && t + 8 <= x.t1) {                          // all of this piece
+          blk = 4 * t + lane;
+          a.held = blk * 32 < x.s.n;
+          a.hk = x.hk;
+          b = x.b;
+          a.tiles = 8;
+          t += 8;
+        }
 #pragma unroll 1
         for (; a.tiles < 8; ++a.tiles) {
           while (more && t >= x.t1) {
@@ -500,11 +511,12 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       auto ask_scales = [&](Batch& a) {
         if (!a.held) return;
         a.page = max(0, checked_page(p.c, a.page));
+        if (kv) return;
         const int64_t at = a.page * p.c.s_page + a.hk * p.c.s_head + a.sub;
         a.ks = __ldg(p.c.ks + at);
         a.vs = __ldg(p.c.vs + at);
       };
-      int g = 0, j = 0;                                       // running tile, running stage
+      int g = 0;                                              // running tile
       Batch now = look_up();
       ask_scales(now);
       Batch next = look_up();
@@ -513,39 +525,36 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         const Batch after = look_up();
         const uint32_t held = __ballot_sync(0xffffffffu, now.held);
 #pragma unroll 1
-        for (int i = 0; i < now.tiles && ok; ++i, ++g) {
-          const int boxes = __popc(held >> (4 * i) & 15u) * C::kPanels;
+        for (int i = 0; i < now.tiles; ++i, ++g) {
+          const int j = 2 * g + kv, st = j % C::kStages, boxes = __popc(held >> (4 * i) & 15u) * C::kPanels;
           const bool mine = lane >> 2 == i;
-#pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv, ++j) {
-            const int st = j % C::kStages;
-            if (j >= C::kStages && !(ok = wait_warp(bar(kEmpty + st), (j / C::kStages - 1) & 1, abort_flag))) break;
-            if (lane == 0) mbar_expect_tx(bars + kFull + st, boxes * 4096);
-            __syncwarp();
-            if (mine && now.held) {
+          if (j >= C::kStages && !(ok = wait_warp(bar(kEmpty + st), (j / C::kStages - 1) & 1, abort_flag))) break;
+          if (lane == 0) mbar_expect_tx(bars + kFull + st, boxes * 4096);
+          __syncwarp();
+          if (mine && now.held) {
 #pragma unroll
-              for (int c = 0; c < C::kPanels; ++c)
-                tma_load_4d(sbase + C::kSmemRing + st * C::kTile + c * 16384 + (lane & 3) * 4096, kv ? &tv : &tk, bar(kFull + st), 128 * c, now.sub * 32, now.hk, now.page);
+            for (int c = 0; c < C::kPanels; ++c)
+              tma_load_4d(sbase + C::kSmemRing + st * C::kTile + c * 16384 + (lane & 3) * 4096, kv ? &tv : &tk, bar(kFull + st), 128 * c, now.sub * 32, now.hk, now.page);
+          }
+          if (kv == 0) {
+            if (mine) {
+              scales[(g & 7) * 8 + (lane & 3)] = now.ks;      // zero where there is no block
+              scales[(g & 7) * 8 + 4 + (lane & 3)] = static_cast<float>(static_cast<int>(scale_to_sb(now.vs)) - 127);
             }
-            if (kv == 0) {
-              if (mine) {
-                scales[(g & 7) * 8 + (lane & 3)] = now.ks;    // zero where there is no block
-                scales[(g & 7) * 8 + 4 + (lane & 3)] = static_cast<float>(static_cast<int>(scale_to_sb(now.vs)) - 127);
-              }
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
           }
         }
         now = next;
         next = after;
       }
-      if (!ok) {
-        if (lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutProducer + kInCache);
-        // what is in flight lands before the shared memory goes
-        for (int k = 1; k <= C::kStages; ++k)
-          if (j >= k) wait_or_abort(bar(kFull + (j - k) % C::kStages), ((j - k) / C::kStages) & 1, abort_flag);
+      if (!kCluster && kv) {
+        const TreeCut y = tree_cut_at(range, first, worker, f_begin);
+        if (lane == 0) reinterpret_cast<TreeCut*>(p.cuts)[worker] = y;
       }
+      if (!ok && lane == 0) raise_abort(abort_flag, p.c.status, kStatusTimeoutProducer + kInCache);
+      // what is in flight lands before the shared memory goes, whichever role gives up
+      for (int i = max(0, g - C::kStages / 2); i < g; ++i) wait_or_abort(bar(kFull + (2 * i + kv) % C::kStages), ((2 * i + kv) / C::kStages) & 1, abort_flag);
     } else if (role == 1) {
       // ---------------------------------------------------------------------------------------- MMA: S
       // (an issuing warp for each product: a chain of eight holds its warp until it is nearly done)
@@ -613,11 +622,6 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           ++units;
         } while (ok && tree_next(p, x, f_end));
         if (!ok) raise_abort(abort_flag, p.c.status, kStatusTimeoutMma + kInCache);
-      }
-    } else if (role == 3) {
-      if (!kCluster) {
-        const TreeCut y = tree_cut_at(range, x, worker, f_begin);
-        if (lane == 0) reinterpret_cast<TreeCut*>(p.cuts)[worker] = y;
       }
     } else {
       if (D == 128) reg_inc<C::kRegsSoftmax>();
