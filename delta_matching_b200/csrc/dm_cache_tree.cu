@@ -521,8 +521,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       ask_scales(now);
       Batch next = look_up();
       while (now.tiles > 0 && ok) {
-        ask_scales(next);
-        const Batch after = look_up();
+        Batch after{};
         const uint32_t held = __ballot_sync(0xffffffffu, now.held);
 #pragma unroll 1
         for (int i = 0; i < now.tiles; ++i, ++g) {
@@ -543,6 +542,10 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + kScales + (g & 7));
+          }
+          if (i == 0) {                                       // (the first tile is on its way)
+            ask_scales(next);
+            after = look_up();
           }
         }
         now = next;
