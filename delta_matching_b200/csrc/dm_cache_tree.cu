@@ -888,7 +888,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         tc_fence_after();
         if (more) put_queries(next, parity ^ 1);              // all S of this unit have been computed; those of the next run under the output
         const bool whole = !kCluster && x.whole();
-        float m_all = kNone, u_all = kNone, l_all = 0.f;
+        float m_all = kNone, u_all = kNone, l_all = 0.f, m_own = kNone;
         volatile int* unit_u = u_at - in_tile + row;          // of the row's copies
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) {
@@ -896,6 +896,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
           for (int y = 0; y < kTeams; ++y) m_copy = fmaxf(m_copy, stats[128 * y + row + c * kRows].x);
           m_all = fmaxf(m_all, m_copy);
+          if (c == copy) m_own = m_copy;
           if (m_copy > kNone) u_all = fmaxf(u_all, static_cast<float>(unit_u[c * kRows] >> 1));
         }
 #pragma unroll
@@ -906,7 +907,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             l_all = fmaf(st.y, ex2_approx(st.x - m_all), l_all);
           }
         if (!(u_all > kNone)) u_all = static_cast<float>(kUnitLift);        // the row sees nothing here (NaN keys aside)
-        const float w = ex2_approx(static_cast<float>(*u_at >> 1) - u_all);
+        const float w = m_own > kNone ? ex2_approx(static_cast<float>(*u_at >> 1) - u_all) : 0.f;       // (a copy that has seen nothing: its u is anywhere)
         // (in two factors: what V's scales leave may be beyond either's range)
         const float d_all = u_all - m_all, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
         const float w1 = whole ? w * exp2f(d1) : w, w2 = whole ? exp2f(d_all - d1) / l_all : 1.f;

@@ -319,6 +319,20 @@ def test_attention_large_logits(N):
         assert bool(torch.isfinite(o).all())
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("scale", [1.0, 40.0, -1.0, -40.0])
+@pytest.mark.parametrize("N", [3, 25, 40])
+def test_attention_far_from_zero(N, scale, D):
+    """All logits far below or above zero, in sequences that end inside the first block, the first tile and later ones: parts of a row's keys are none."""
+    H, Hk, lengths = 2, 1, _ints([N, N + 20, N + 70, N + 300])
+    cache, _, table = _filled(lengths.tolist(), 64, Hk, D)
+    keys = cache.k8.view(torch.uint8)
+    keys.copy_(keys | 0x80)                                      # the signs of the codes: keys of negative values
+    g = torch.Generator().manual_seed(N)
+    q = (_rand(g, 4, N, H, D).abs() * (1.0 if scale > 0 else -1.0)).to(BF)
+    _attended(q, cache, table, lengths, None, dref.make_parents("any", 4, N, seed=1), scale=abs(scale))
+
+
 @pytest.mark.parametrize("layout, P", [("joint", 32), ("slots", 128), ("dense", 256)])
 def test_attention_layouts_and_strides(layout, P, route):
     """Pools in other layouts, q as a part of a packed tensor, seen as a part of a wider one, and one tree for all sequences."""
