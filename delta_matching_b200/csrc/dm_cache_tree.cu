@@ -318,57 +318,57 @@ __device__ __forceinline__ TreeCut tree_cut_at(const TreeRange& range, const Tre
 }
 
 // CTA `rank` of a cluster writes its share of a unit's rows: the CTAs have left it their sums of them (m, l, u, marked) and their values, a CTA's behind the other's, in
-// shared memory (its own: reading others' took 4000 cycles a row).  A warp a row, over the CTAs in order; rows behind the sequence's count are zeros.
+// shared memory (its own: reading others' took 4000 cycles a row; writing to others, at 16 bytes a cycle, is what bounds the exchange, so the copies are added up before),
+// 16-byte pieces XORed with the row.  Half a warp a row, over the CTAs in order; rows behind the sequence's count are zeros.
+__device__ __forceinline__ int value_at(int row, int piece) { return piece ^ (row & 31); }
 template <int D, int kRows, int kWarps>
 __device__ __forceinline__ void join_cluster(const CacheTreeParams& p, const TreePiece& x, int rank, const uint8_t* values, const float4* sums) {
-  constexpr int kVecs = D / 128;
-  const int cl = p.cluster, rows = kRows / cl, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = warp; i < rows; i += kWarps) {
-    const int unit_row = x.rt * kRows + rank * rows + i, node = node_of(p, unit_row), head = x.hk * p.rep + unit_row - node * p.rep;
-    if (node >= p.N) break;
-    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(p.o + ((static_cast<int64_t>(x.b) * p.N + node) * p.H + head) * D) + 2 * lane;
-    float* lse = p.lse + (static_cast<int64_t>(x.b) * p.H + head) * p.N + node;
-    if (node >= x.s.count) {
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v) o[64 * v] = o[64 * v + 1] = __floats2bfloat162_rn(0.f, 0.f);
-      if (lane == 0) *lse = -CUDART_INF_F;
-      continue;
-    }
-    float top = kNone, u_top = kNone, marked = 0.f;
-    for (int c = 0; c < cl; ++c) {
-      const float4 st = sums[c * rows + i];
-      top = fmaxf(top, st.x);
-      if (st.x > kNone) u_top = fmaxf(u_top, st.z);
-      marked += st.w;
-    }
-    if (marked != 0.f) {
-      tree_row<D>(p, x.b, node, head);
-      continue;
-    }
-    float sum = 0.f;
+  constexpr int kVecs = D / 64;
+  const int cl = p.cluster, rows = kRows / cl, lane = threadIdx.x & 31, l = lane & 15;
+  for (int i0 = (threadIdx.x >> 5) * 2; i0 < rows; i0 += 2 * kWarps) {
+    const int i = i0 + (lane >> 4), row = rank * rows + i, unit_row = x.rt * kRows + row, node = node_of(p, unit_row), head = x.hk * p.rep + unit_row - node * p.rep;
+    const bool mine = i < rows && node < p.N, real = mine && node < x.s.count;
     float4 acc[kVecs] = {};
-    for (int c = 0; c < cl; ++c) {
-      const float4 st = sums[c * rows + i];
-      if (!(st.x > kNone)) {                                  // the row sees nothing of the CTA's tiles (or it had none); NaN may have been added to its sum
-        sum += st.y;
-        continue;
+    float top = kNone, u_top = kNone, marked = 0.f, sum = 0.f;
+    if (real) {
+      for (int c = 0; c < cl; ++c) {
+        const float4 st = sums[c * rows + i];
+        top = fmaxf(top, st.x);
+        if (st.x > kNone) u_top = fmaxf(u_top, st.z);
+        marked += st.w;
       }
-      sum = fmaf(st.y, ex2_approx(st.x - top), sum);
-      const float w = ex2_approx(st.z - u_top);
+      for (int c = 0; c < cl; ++c) {
+        const float4 st = sums[c * rows + i];
+        if (!(st.x > kNone)) {                                // the row sees nothing of the CTA's tiles (or it had none); NaN may have been added to its sum
+          sum += st.y;
+          continue;
+        }
+        sum = fmaf(st.y, ex2_approx(st.x - top), sum);
+        const float w = ex2_approx(st.z - u_top);
+        const float4* from = reinterpret_cast<const float4*>(values) + (c * rows + i) * (D / 4);
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          const float4 y = from[value_at(row, 16 * v + l)];
+          acc[v] = make_float4(fmaf(y.x, w, acc[v].x), fmaf(y.y, w, acc[v].y), fmaf(y.z, w, acc[v].z), fmaf(y.w, w, acc[v].w));
+        }
+      }
+    }
+    if (mine && marked == 0.f) {
+      const float d_all = u_top - top, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
+      const float w1 = real ? exp2f(d1) : 0.f, w2 = real ? exp2f(d_all - d1) / sum : 0.f;
+      uint2* o = reinterpret_cast<uint2*>(p.o + ((static_cast<int64_t>(x.b) * p.N + node) * p.H + head) * D) + l;
 #pragma unroll
       for (int v = 0; v < kVecs; ++v) {
-        const float4 y = reinterpret_cast<const float4*>(values)[(c * rows + i) * (D / 4) + 32 * v + lane];
-        acc[v] = make_float4(fmaf(y.x, w, acc[v].x), fmaf(y.y, w, acc[v].y), fmaf(y.z, w, acc[v].z), fmaf(y.w, w, acc[v].w));
+        const __nv_bfloat162 a = __floats2bfloat162_rn(acc[v].x * w1 * w2, acc[v].y * w1 * w2), b = __floats2bfloat162_rn(acc[v].z * w1 * w2, acc[v].w * w1 * w2);
+        o[16 * v] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
       }
+      if (l == 0) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = real ? (top + log2f(sum)) * kLn2 : -CUDART_INF_F;
     }
-    const float d_all = u_top - top, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
-    const float w1 = exp2f(d1), w2 = exp2f(d_all - d1) / sum;
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v) {
-      o[64 * v] = __floats2bfloat162_rn(acc[v].x * w1 * w2, acc[v].y * w1 * w2);
-      o[64 * v + 1] = __floats2bfloat162_rn(acc[v].z * w1 * w2, acc[v].w * w1 * w2);
+    // rows that are made by themselves: by the whole warp
+    for (uint32_t left = __ballot_sync(0xffffffffu, real && marked != 0.f && l == 0); left != 0; left &= left - 1) {
+      const int from = __ffs(left) - 1;
+      tree_row<D>(p, x.b, __shfl_sync(0xffffffffu, node, from), __shfl_sync(0xffffffffu, head, from));
     }
-    if (lane == 0) *lse = (top + log2f(sum)) * kLn2;
   }
 }
 
@@ -886,6 +886,8 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
         if (!(ok = all_of(4, 128 * kTeams, ok))) break;
         tc_fence_after();
+        [[maybe_unused]] cg::cluster_group::arrival_token tiles_done;
+        if constexpr (kCluster) tiles_done = cg::this_cluster().barrier_arrive();
         if (more) put_queries(next, parity ^ 1);              // all S of this unit have been computed; those of the next run under the output
         const bool whole = !kCluster && x.whole();
         float m_all = kNone, u_all = kNone, l_all = 0.f, m_own = kNone;
@@ -913,14 +915,19 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         const float w1 = whole ? w * exp2f(d1) : w, w2 = whole ? exp2f(d_all - d1) / l_all : 1.f;
         const int slot = 2 * worker + (x.f0 == f_begin ? 0 : 1);
         if constexpr (kCluster) {                             // the values go to the CTAs that write their rows, where the ring must be free: all CTAs' tiles are done with
-          cg::this_cluster().sync();
+          cg::this_cluster().barrier_wait(std::move(tiles_done));
           met = true;
         }
+        // of the row's values, in the CTA that writes it
+        auto values_of = [&](int r) {
+          const int to = r / rows_each;
+          return reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemRing) + (rank * rows_each + r - to * rows_each) * (D / 4);
+        };
         if constexpr (kCopies == 1) {                         // 16 columns at a time, a row a lane
-          const int at = out_rows[128 * parity + row], to = row / rows_each;
+          const int at = out_rows[128 * parity + row];
           float* part = p.part_o + (static_cast<int64_t>(slot) * kRows + row) * D;
-          if constexpr (kCluster)
-            part = reinterpret_cast<float*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemRing) + (rank * rows_each + row - to * rows_each) * D;
+          float4* values = nullptr;
+          if constexpr (kCluster) values = values_of(row);
 #pragma unroll 1
           for (int c = team; c < D / 16; c += kTeams) {
             uint32_t o[16];
@@ -940,6 +947,9 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
               uint4* to_o = reinterpret_cast<uint4*>(p.o + static_cast<int64_t>(at) * D + 16 * c);
               to_o[0] = make_uint4(h[0], h[1], h[2], h[3]);
               to_o[1] = make_uint4(h[4], h[5], h[6], h[7]);
+            } else if constexpr (kCluster) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) values[value_at(row, 4 * c + e)] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
             } else {
 #pragma unroll
               for (int e = 0; e < 4; ++e) reinterpret_cast<float4*>(part + 16 * c)[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
@@ -974,8 +984,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
               const int at = out_rows[128 * parity + r];
               if (at < 0) continue;
               if constexpr (kCluster) {
-                const int to = r / rows_each;
-                *reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemRing + ((rank * rows_each + r - to * rows_each) * D + 16 * c + 4 * piece) * 4) = y;
+                values_of(r)[value_at(r, 4 * c + piece)] = y;
               } else if (whole) {
                 const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
                 *reinterpret_cast<uint2*>(p.o + static_cast<int64_t>(at) * D + 16 * c + 4 * piece) =
