@@ -9,14 +9,22 @@
 // of two block-scaled chains with P in two e4m3 codes relative to the largest of its 32 keys (off by 2^-8 of itself at most, 2^-16 of that largest one where it is
 // small).  The power-of-two scale of V's block goes into P's scale byte and that of K's block into the factor of the logits.
 //
-// The key tiles of 128 tokens of all units are one flat range, divided evenly over the CTAs of one wave; pieces of cut units are joined by a second kernel.
+// The key tiles of 128 tokens of all units are one flat range, divided evenly over the CTAs of one wave; pieces of cut units are joined by a second kernel.  Where units
+// have few tiles a cluster takes each, and joins it itself.
 // One CTA an SM.  Three teams of four softmax warps (thread = TMEM lane; two teams at head_dim 256) take the tiles of a unit in turn, each with an S buffer in TMEM;
-// P's codes and scale bytes lie over the S that they come from.  Of the last four warps one loads the code tiles from the pages by TMA and two issue the MMAs.  The power of two that a row of O counts in is fixed by the
-// unit's first blocks: fp32 has room for what may follow (rows for which it has not are marked and made by themselves), and no team waits for another's maximum.
+// P's codes and scale bytes lie over the S that they come from.  Of the last four warps two load the code tiles of K and of V from the pages by TMA and two issue the MMAs.
+// The power of two that a row of O counts in is fixed by the unit's first blocks: fp32 has room for what may follow (rows for which it has not are marked and made by
+// themselves), and no team waits for another's maximum.
 //
 // kCopies: where a unit has at most 64 or 32 rows, they stand twice or four times in the 128 lanes, and copy c looks after its share of a tile's blocks of 32
 // keys (P is zero in the others), with a reference, a sum and an accumulator of its own, which the CTA adds up at the end: the softmax of a tile is as much
 // shorter, and the tensor cores, which take 128 rows whatever is in them, have no more to do.
+//
+// Measured (H 32, Hk 8, head_dim 128 but for the last two): 4 sequences of 4000 tokens with 16 drafts 19.1 us; 64 of 4096 with 8 drafts 130 us, 4.1 TB/s of codes, with 25 178 us;
+// one of 65536 with 60 drafts of 64 heads 158 us; 8 of 6144 with 33 drafts of 16 heads of 256 98 us, 4.1 TB/s.  What bounds it: with few rows the chain softmax, P V, next S
+// of a buffer (2100 cycles behind a tile's 1000; the products of a tile alone take 1024) and 7000 cycles from a unit's last tile to the next one's first; with 128 rows the softmax (1350 cycles a
+// tile at saturation, of about 2200).  Above a hundred us the chip is at its power limit (1.4 - 1.7 GHz).  Small calls: 5000 cycles to the first S, 9000 from the last
+// tile to the end of the cluster's join, of 32000.
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "dm_cache.cuh"
@@ -31,7 +39,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxCluster = 8;
 
-// Key tiles that a unit's queries and output are worth.
+// Key tiles that a unit's queries and output are worth (8 instead: as fast to 2 % in calls of 4 x 8000 to 64 x 4096 tokens; 2: 5 % slower in the first).
 constexpr int kTreeCost = 4;
 constexpr float kExact = 4194304.f;         // logits (log2) up to this size: whole numbers beside them are exact
 constexpr float kReach = 40.f;              // what a row's logits may exceed the reference of its sum by, in powers of two: fp32 has room for it

@@ -9,7 +9,8 @@ namespace {
 
 // ------------------------------------------------------------------------------------------------ depths and ancestors
 // seen_i = {i} united with seen of i's parent; depth_i = |seen_i| - 1.  One CTA a sequence, one thread a node.  A warp's 32 nodes first find their ancestors among
-// themselves, by doubling with shuffles (five rounds), and the ancestor behind those; then each node walks from group of 32 to group of 32, at most as many steps as it has words.
+// themselves, by doubling with shuffles (five rounds), and the ancestor behind those; then each node walks from group of 32 to group of 32, at most as many steps as it has words.  Bound by latency: 64 trees
+// of up to 509 nodes, each within three nodes of its parent, take 3.5 us of the GPU; 10.9 where each node walked from parent to parent.
 __global__ void __launch_bounds__(1024) draft_tree_kernel(const DraftTreeParams p, const int words) {
   extern __shared__ uint32_t sets[];                          // (N, pitch)
   __shared__ uint32_t among[kMaxNodes];                       // of a node, its ancestors in its group and itself
@@ -66,6 +67,9 @@ __global__ void __launch_bounds__(1024) draft_tree_kernel(const DraftTreeParams 
 // the block's older tokens and its tokens of the path, takes the smallest power-of-two scale that holds them (as the eviction does), and rounds the codes
 // to it.  A path is strictly increasing, so a token never moves up: what a block takes lies in it or behind it, and the warps of a CTA read all that
 // they need before any of them writes; blocks of a later round are behind those.  The path is looked over while the first round's codes are on their way.
+//
+// Bound by the chain of loads (length, path, page, codes) of a round: 64 sequences of up to 250 drafts of which most are kept take 10.9 us (8 kv heads, 1.5 TB/s), 4 of 16 drafts 3.
+// Warps a CTA 4, 6, 8: 11.9, 11.4, 12.8 us there; 8.3, 10.0, 9.9 with 120 drafts; 14.7, 12.0, 13.3 with 250 drafts in each sequence.
 constexpr int kKeepWarps = 4;
 
 template <int D>
