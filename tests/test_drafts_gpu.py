@@ -1,5 +1,8 @@
 """The functions for drafted tokens against their definitions in 64 bits (tests/drafts_ref.py)."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -317,6 +320,16 @@ def test_attention_large_logits(N):
     for scale in (1.0, 1e4):
         o, lse = _attended(q, cache, table, lengths, None, dref.make_parents("any", 1, N, seed=1), scale=scale)
         assert bool(torch.isfinite(o).all())
+
+
+@pytest.mark.parametrize("B, Hk", [(5, 3), (4, 4), (11, 3), (17, 2), (37, 2), (25, 3), (37, 4), (149, 1)])
+@pytest.mark.parametrize("N, D", [(9, 128), (70, 128), (9, 256)])
+def test_attention_of_many_sequences(B, Hk, N, D):
+    """Every size of a cluster, and one unit more than the chip holds of them."""
+    lengths = [N + (37 * b) % 900 for b in range(B)]
+    cache, _, table = _filled(lengths, 64, Hk, D, seed=B)
+    g = torch.Generator().manual_seed(B)
+    _attended(_rand(g, B, N, 2 * Hk, D), cache, table, _ints(lengths), None, dref.make_parents("near", B, N, seed=1))
 
 
 @pytest.mark.parametrize("D", [128, 256])
@@ -638,3 +651,28 @@ def test_two_streams_at_once():
     for s in (0, 1):
         for got in outs[s]:
             assert all(torch.equal(_bits(x), _bits(y)) for x, y in zip(got, want[s]))
+
+
+def test_first_call_of_a_process_is_captured():
+    """What the library asks the device for once does not disturb a capture."""
+    code = """
+import torch, delta_matching_b200 as dm
+from delta_matching_b200 import ops
+ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+cache, table, parents, freqs = dm.KVCache8.empty(8, 64, 2, 128), ints(*range(8)).view(2, 4), ints([-1, 0, 0], [-1, 0, 1]), torch.ones(8, device="cuda")
+q, k, v = (torch.ones(2, 3, h, 128, device="cuda", dtype=torch.bfloat16) for h in (4, 2, 2))
+lengths, path, kept = ints(40, 90), ints([0, 2], [0, 1]), ints(2, 1)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    tree = dm.dm_draft_tree(parents)
+    turned, now = dm.dm_cache_append_rotary(cache, q, k, v, table, lengths, freqs, offsets=tree.depth)
+    o = dm.dm_cache_attn_tree(turned, cache, table, now, tree)
+    new = dm.dm_cache_keep(cache, table, lengths, now, path, kept)
+graph.replay()
+ops.check_status("cuda")
+assert new.tolist() == [42, 91] and bool(o.isfinite().all())
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
