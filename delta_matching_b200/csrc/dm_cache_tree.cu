@@ -325,6 +325,16 @@ __device__ __forceinline__ TreeCut tree_cut_at(const TreeRange& range, const Tre
   return y;
 }
 
+// 2^e, e a whole number, in two factors: values may be as far above 1 as it is below fp32's smallest.
+__device__ __forceinline__ float2 two_factors(float e) {
+  e = fminf(fmaxf(e, -250.f), 250.f);
+  const float h = truncf(0.5f * e);
+  return make_float2(ex2_approx(h), ex2_approx(e - h));
+}
+__device__ __forceinline__ float4 add_scaled(float4 acc, float4 y, float2 w) {
+  return make_float4(fmaf(y.x * w.x, w.y, acc.x), fmaf(y.y * w.x, w.y, acc.y), fmaf(y.z * w.x, w.y, acc.z), fmaf(y.w * w.x, w.y, acc.w));
+}
+
 // CTA `rank` of a cluster writes its share of a unit's rows: the CTAs have left it their sums of them (m, l, u, marked) and their values, a CTA's behind the other's, in
 // shared memory (its own: reading others' took 4000 cycles a row; writing to others, at 16 bytes a cycle, is what bounds the exchange, so the copies are added up before),
 // 16-byte pieces XORed with the row.  Half a warp a row, over the CTAs in order; rows behind the sequence's count are zeros.
@@ -352,12 +362,11 @@ __device__ __forceinline__ void join_cluster(const CacheTreeParams& p, const Tre
           continue;
         }
         sum = fmaf(st.y, ex2_approx(st.x - top), sum);
-        const float w = ex2_approx(st.z - u_top);
+        const float2 w = two_factors(st.z - u_top);
         const float4* from = reinterpret_cast<const float4*>(values) + (c * rows + i) * (D / 4);
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) {
-          const float4 y = from[value_at(row, 16 * v + l)];
-          acc[v] = make_float4(fmaf(y.x, w, acc[v].x), fmaf(y.y, w, acc[v].y), fmaf(y.z, w, acc[v].z), fmaf(y.w, w, acc[v].w));
+          acc[v] = add_scaled(acc[v], from[value_at(row, 16 * v + l)], w);
         }
       }
     }
@@ -917,10 +926,9 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             l_all = fmaf(st.y, ex2_approx(st.x - m_all), l_all);
           }
         if (!(u_all > kNone)) u_all = static_cast<float>(kUnitLift);        // the row sees nothing here (NaN keys aside)
-        const float w = m_own > kNone ? ex2_approx(static_cast<float>(*u_at >> 1) - u_all) : 0.f;       // (a copy that has seen nothing: its u is anywhere)
-        // (in two factors: what V's scales leave may be beyond either's range)
-        const float d_all = u_all - m_all, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
-        const float w1 = whole ? w * exp2f(d1) : w, w2 = whole ? exp2f(d_all - d1) / l_all : 1.f;
+        // what a value counts: 2^(u - m) / l where the row is whole here, 2^(u - the copies' largest u) else; nothing in a copy that has seen nothing, whose u is anywhere
+        const float2 w = two_factors(static_cast<float>(*u_at >> 1) - (whole ? m_all : u_all));
+        const float w1 = m_own > kNone ? w.x : 0.f, w2 = whole ? w.y / l_all : w.y;
         const int slot = 2 * worker + (x.f0 == f_begin ? 0 : 1);
         if constexpr (kCluster) {                             // the values go to the CTAs that write their rows, where the ring must be free: all CTAs' tiles are done with
           cg::this_cluster().barrier_wait(std::move(tiles_done));
@@ -1095,21 +1103,22 @@ __global__ void __launch_bounds__(128) cache_tree_join_kernel(const __grid_const
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     sum = sum * ex2_approx(top - top_new) + l;
-    const float a = ex2_approx(u_top - u_new), wgt = ex2_approx(ml.z - u_new);
+    const float2 a = two_factors(u_top - u_new);
+    const float lift = ml.z - u_new;
     top = top_new;
     u_top = u_new;
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) acc[v] = make_float4(acc[v].x * a, acc[v].y * a, acc[v].z * a, acc[v].w * a);
+    for (int v = 0; v < kVecs; ++v) acc[v] = add_scaled(make_float4(0.f, 0.f, 0.f, 0.f), acc[v], a);
     const uint32_t counts = __ballot_sync(0xffffffffu, there && ml.x > kNone);          // kNone: the row sees nothing of the piece
 #pragma unroll 8
     for (int k = 0; k < min(32, x.last - w0 + 1); ++k) {
-      const float w_k = __shfl_sync(0xffffffffu, wgt, k);
+      const float lift_k = __shfl_sync(0xffffffffu, lift, k);
       const int64_t at_k = __shfl_sync(0xffffffffu, at, k);
       if (!((counts >> k) & 1)) continue;
+      const float2 w_k = two_factors(lift_k);
 #pragma unroll
       for (int v = 0; v < kVecs; ++v) {
-        const float4 y = reinterpret_cast<const float4*>(p.part_o + at_k * D)[32 * v + lane];
-        acc[v] = make_float4(fmaf(y.x, w_k, acc[v].x), fmaf(y.y, w_k, acc[v].y), fmaf(y.z, w_k, acc[v].z), fmaf(y.w, w_k, acc[v].w));
+        acc[v] = add_scaled(acc[v], reinterpret_cast<const float4*>(p.part_o + at_k * D)[32 * v + lane], w_k);
       }
     }
   }

@@ -100,7 +100,11 @@ def attention(q, cache, table, lengths, counts, see, scale):
     most 8 times its eighth bit, which 3 bits hold; below, at most 2^-10 is left, on steps of 2^-13: off by 2^-14, 2^-21 of the largest element.  That times the sum of the
     sizes of the key's channels.  Both move a probability by twice as much relatively; exp2 and the fp32 sums by 2^-19.  A probability is held in the output product
     with the largest of its block of 32 keys brought to 2^7 ... 2^8 as an e4m3 code of its first four bits (below 2^(e-3) is left, for 2^e ... 2^(e+1)) and an e4m3 code of
-    the rest, off by 2^(e-8): 2^-8 of itself.  Where either is below 2^-6 its code is off by up to 2^-10: together 2^-9, 2^-16 of the block's largest.  o is rounded to bf16 (2^-8)."""
+    the rest, off by 2^(e-8): 2^-8 of itself.  Where either is below 2^-6 its code is off by up to 2^-10: together 2^-9, 2^-16 of the block's largest.  o is rounded to bf16 (2^-8).
+
+    The codes of a block count in powers of two from 2^-127 of 2^u on, u fixed: 40 above the largest product 2^t of a probability and a V scale in the first blocks, or 40 where the row
+    sees nothing in these (then it is made by itself if all its products are below 2^-40).  A smaller product counts as that: a key's value is off by up to 2^8 448 2^(u - 127), 2^(u - 110).  That
+    is 2^-69 of the largest product (2^(u - 41) at least), or 2^-29 where u was not taken from it: times the number of keys."""
     B, N, H, D = q.shape
     Hk, P = cache.k8.shape[1:3]
     dev = "cuda"
@@ -117,6 +121,7 @@ def attention(q, cache, table, lengths, counts, see, scale):
         sees[:, n - count:] = see[b, :count, :count].to(dev)
         for h in range(Hk):
             k, v = (c[page, h, at % P].double() * s[page, h, at % P // BLK].double()[:, None] for c, s in ((k32, cache.ks), (v32, cache.vs)))
+            vs = cache.vs[page, h, at % P // BLK].double()
             for hh in range(h * H // Hk, (h + 1) * H // Hk):
                 qi = q[b, :count, hh].to(dev).double()
                 zero = lambda x: x.masked_fill(~sees, 0.0)       # (what is not seen may be anything)
@@ -133,6 +138,6 @@ def attention(q, cache, table, lengths, counts, see, scale):
                     rows = [[x[i, sees[i]] @ y[sees[i]] for x, y in ((p, v), (p, v.abs()), (top, v.abs()))] for i in range(count)]
                     pv, pav, tav = (torch.stack(x) for x in zip(*rows))
                 o[b, :count, hh] = pv
-                do[b, :count, hh] = 2.0 ** -8 * pv.abs() + (2.0 ** -8 + 2 * eps + 2.0 ** -19)[:, None] * pav + 2.0 ** -16 * tav + 1e-37
+                do[b, :count, hh] = 2.0 ** -8 * pv.abs() + (2.0 ** -8 + 2 * eps + 2.0 ** -19)[:, None] * pav + 2.0 ** -16 * tav + (n * 2.0 ** -29 * (p * vs).amax(1))[:, None] + 1e-37
                 dlse[b, hh, :count] = eps + 2.0 ** -19 + 2.0 ** -22 * lse[b, hh, :count].abs()
     return (o, lse), (do, dlse)

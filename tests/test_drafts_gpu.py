@@ -322,6 +322,21 @@ def test_attention_large_logits(N):
         assert bool(torch.isfinite(o).all())
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("N", [2, 8, 33, 65])
+def test_attention_of_products_far_apart(N, D):
+    """V scales up to 2^120 apart and logits in the hundreds: what the first blocks, a part of the keys or another copy of the row hold may be nothing to the largest product, and the
+    other way round."""
+    for seed in range(4):
+        lengths = _ints([N, N + 190, N + 1270, N + 700])
+        cache, _, table = _filled(lengths.tolist(), 64, 3, D, seed=seed, kscale=0.05)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        cache.vs.mul_(torch.exp2(torch.randint(-60, 60, cache.vs.shape, generator=g, device="cuda").float()))
+        g = torch.Generator().manual_seed(seed)
+        q = (_rand(g, 4, N, 9, D, scale=4.0).float() * torch.exp2(torch.randint(-8, 6, (D,), generator=g).float())).to(BF)
+        _attended(q, cache, table, lengths, None, dref.make_parents("any", 4, N, seed=seed), scale=(None, 1.0, 0.01, 0.1)[seed])
+
+
 @pytest.mark.parametrize("B, Hk", [(5, 3), (4, 4), (11, 3), (17, 2), (37, 2), (25, 3), (37, 4), (149, 1)])
 @pytest.mark.parametrize("N, D", [(9, 128), (70, 128), (9, 256)])
 def test_attention_of_many_sequences(B, Hk, N, D):
