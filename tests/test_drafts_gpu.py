@@ -137,6 +137,16 @@ def test_append_rotary(N, P, layout, D, F, interleaved):
         _appended(cache, pools, table, q, k, v, lengths, _freqs(F), off, _ints([N, max(0, N - 1), N // 2, 0]) if ragged else None, interleaved)
 
 
+@pytest.mark.parametrize("D, F, interleaved", [(128, 64, False), (256, 96, True)])
+@pytest.mark.parametrize("B, N", [(1, 4099), (2, 2100)])
+def test_append_rotary_of_prompts(B, N, D, F, interleaved):
+    """From 4096 tokens on more rows are in flight; ragged, behind a start inside a block."""
+    lengths = _ints([17, 0][:B])
+    cache, pools, table = _filled(lengths.tolist(), 64, 2, D, T=-(-(17 + N) // 64))
+    g = torch.Generator().manual_seed(N)
+    _appended(cache, pools, table, _rand(g, B, N, 4, D), _rand(g, B, N, 2, D, scale=3.0), _rand(g, B, N, 2, D), lengths, _freqs(F), None, _ints([N - 5, N][:B]), interleaved)
+
+
 @pytest.mark.parametrize("start", [100003, (1 << 24) + 1])
 def test_append_rotary_far_positions(start):
     """Angles of far positions, where 32 bits would have lost them: the pages before are one and the same."""
