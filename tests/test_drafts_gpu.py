@@ -701,3 +701,44 @@ print("captured")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=200)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_pools_beyond_two_gigabytes():
+    """Pages whose codes lie more than 2^31 bytes into the pools: the bits of the same step in small ones."""
+    B, N, H, Hk, D, P = 2, 9, 8, 8, 128, 64
+    outs = []
+    for pages, first in ((8, 0), (40000, 39990)):
+        cache = dm.KVCache8(*(torch.empty(pages, Hk, P, D, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2)),
+                            *(torch.empty(pages, Hk, P // 32, device="cuda") for _ in range(2)))
+        table = (torch.arange(8, dtype=torch.int32).view(B, 4) + first).cuda()
+        g = torch.Generator().manual_seed(1)
+        lengths = torch.zeros(B, dtype=torch.int32, device="cuda")
+        for n in (100, N):
+            q, k, v = (_rand(g, B, n, h, D).cuda() for h in (H, Hk, Hk))
+            before = lengths
+            turned, lengths = dm.dm_cache_append_rotary(cache, q, k, v, table, before, _freqs(64).cuda())
+        tree = dm.dm_draft_tree(dref.make_parents("near", B, N, seed=1).cuda())
+        o, lse = dm.dm_cache_attn_tree(turned, cache, table, lengths, tree, return_lse=True)
+        new = dm.dm_cache_keep(cache, table, before, lengths, _ints([[0, 3, 8], [2, 4, 5]]).cuda(), _ints([3, 2]).cuda())
+        assert new.tolist() == [103, 102]
+        held = [c.view(torch.uint8)[first:first + 8, :, :32].flatten(1) if c.dtype != torch.float32 else c[first:first + 8, :, 0] for c in cache]
+        outs.append([turned, o, lse] + [x[[0, 4]] for x in held])
+        ops.check_status("cuda")
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+
+
+def test_thousands_of_sequences():
+    """As many as a call takes; a node alone is what the causal attention makes of one token: both are within 2^-8 of the sum of weights times values (which is less than twice the
+    largest output here) and 2^-8 of rounding, their LSE within 2^-17."""
+    B, H, Hk, D = 8191, 8, 1, 128
+    lengths = (torch.arange(B) * 7 % 64 + 1).to(torch.int32)
+    cache, _, table = _filled([64] * 4, 32, Hk, D)
+    table = table[torch.arange(B) % 4].contiguous().cuda()
+    g = torch.Generator().manual_seed(1)
+    q = _rand(g, B, 1, H, D).cuda()
+    tree = dm.dm_draft_tree(torch.full((B, 1), -1, dtype=torch.int32, device="cuda"))
+    o, lse = dm.dm_cache_attn_tree(q, cache, table, lengths.cuda(), tree, return_lse=True)
+    want, lse2 = dm.dm_cache_attn(q, cache, table, lengths.cuda(), return_lse=True)
+    ops.check_status("cuda")
+    assert bool(((lse - lse2).abs() < 1e-4).all()) and bool(((o.float() - want.float()).abs() < 0.02 * want.float().abs().amax()).all())
