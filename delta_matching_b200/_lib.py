@@ -61,6 +61,7 @@ SIGNATURES = {
     "dm_draft_tree": (_I, [_P, _L, _P, _I, _I, _P, _P, _P, _P]),
     "dm_cache_append_rotary": (_I, [_P, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _P, _I, _I, _P, _L, _I, _P, _P, _L, _P, _P, _P, _P, _P]),
     "dm_cache_attn_tree_workspace_bytes": (_L, [_I, _I, _I, _I, _I, _I, _I]),
+    "dm_dbg_cache_tree_plan": (_I, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "dm_cache_attn_tree": (_I, [_P, _P, _L, _L, _L, _I, _I, _I, _P, _L, _I, _P, _P, _P, _L, _L, _F, _P, _P, _P, _L, _P, _P]),
     "dm_cache_keep": (_I, [_P, _I, _P, _L, _I, _P, _P, _P, _L, _I, _P, _P, _P, _P]),
     "dm_kmean_static": (_I, [_P, _L, _L, _L, _I, _I, _I, _I, _P, _P, ctypes.c_char_p, _I]),

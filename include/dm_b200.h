@@ -317,6 +317,10 @@ int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, in
                        const int* table, int64_t table_row, int T, const int* lengths, const int* counts, const int* seen, int64_t seen_sb, int64_t seen_sn,
                        float softmax_scale, void* o, float* lse, void* workspace, int64_t workspace_bytes, int* status, void* stream);
 
+/* Test hook, host only: how dm_cache_attn_tree lays a call out on the current device (148 SMs without one, and no clusters).  what = 0: the CTAs of a cluster that takes a unit, 0 where the
+ * key tiles of all units are divided evenly instead; 1: CTAs; 2: rows of a unit.  Negative: a shape that is refused. */
+int dm_dbg_cache_tree_plan(int B, int N, int H, int Hk, int D, int T, int page_size, int what);
+
 /* Of the drafted tokens before[b] ... lengths[b] - 1 those of a path are kept: path[b, 0 ... counts[b] - 1], strictly increasing indexes behind before[b]
  * (rows path_row entries apart, M <= 1024 entries), become the tokens before[b], before[b] + 1, ...  Each block of 32 slots that is written gets the
  * smallest power-of-two scale that holds its tokens, older ones too; slots behind the last token stay as they are.  new_lengths (B) = before + counts.  A
