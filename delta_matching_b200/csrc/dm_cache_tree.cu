@@ -194,7 +194,7 @@ __device__ __forceinline__ uint32_t seen_keys(const uint32_t* seen, int i, int r
 
 // ------------------------------------------------------------------------------------------------ one row
 // Row (b, i, head) by one warp and from the definition: a key after the other, the logits' differences exact whatever their size.  For rows that the
-// kernel below marks.
+// kernel below marks, always when the tiles are done with: it takes about 0.6 us a key, and nothing that waits with a limit may wait for it.
 template <int D>
 __device__ __noinline__ void tree_row(const CacheTreeParams& p, int b, int i, int head) {
   constexpr int kVecs = D / 128;
@@ -297,7 +297,7 @@ enum TreeBar : int {
   kScales = 37,                             // of running tile g: entry g % 8
   kCut = 45,                                // by team: a cut tile's values have been looked at
   kPHalf = 48,                              // as kP, of the first half of a tile's keys (one copy)
-  kTreeBars = 51,                           // behind them the TMEM slot, the abort flag and whether a row of the unit is marked (by parity)
+  kTreeBars = 51,                           // behind them the TMEM slot, the abort flag and whether a row of a whole unit is marked
 };
 
 // What the join needs of a cut unit, left by the worker that goes on with it first: its rows, and the workers that have tiles of it.
@@ -432,6 +432,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     for (int i = 0; i < 4; ++i) mbar_init(bars + kU + i, 1);
     for (int i = 0; i < 8; ++i) mbar_init(bars + kScales + i, 1);
     *abort_flag = 0;
+    *any_marked = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
@@ -444,7 +445,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   grid_dep_wait();
   // the worker's share of the steps, and its first piece
   const int worker = blockIdx.x;
-  int f_begin = 0, f_end = 0;
+  int f_begin = 0, f_end = 0, sums = 0;
   TreePiece x{};
   TreeRange range{};
   const int rank = kCluster ? worker % p.cluster : 0, rows_each = kCluster ? kRows / p.cluster : kRows;      // of the cluster; rows that each CTA of it writes
@@ -461,7 +462,6 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       x.t1 = x.s.tiles() * (rank + 1) / p.cluster;
     }
   } else {
-    int sums;
     range = tree_range(p, sums);
     if (worker < range.workers && range.total > 0) {
       f_begin = range.share(worker);
@@ -709,7 +709,6 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             }
           }
         }
-        if (tid == 0) any_marked[parity] = 0;
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kQ + parity);
@@ -900,10 +899,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         stats[128 * team + in_tile] = make_float2(m, l);
         // out of u's range: above; or below where u was not taken from the row's own products
         marked |= hi > u + 95.f || ((u_code & 1) != 0 && hi > kNone && hi < u - 80.f);
-        if (real && marked) {
-          marks[128 * parity + row] = 1;
-          any_marked[parity] = 1;
-        }
+        if (real && marked) marks[128 * parity + row] = 1;
         if (!(ok = all_of(4, 128 * kTeams, ok))) break;
         tc_fence_after();
         [[maybe_unused]] cg::cluster_group::arrival_token tiles_done;
@@ -1018,20 +1014,18 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         const bool mine = team == 0 && copy == 0 && real;
         const int head = x.hk * p.rep + unit_row - node * p.rep;
         const bool again = mine && marks[128 * parity + row] != 0;
-        if (mine && whole) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = (m_all + log2f(l_all)) * kLn2;
+        if (mine && whole) {
+          const int64_t at = (static_cast<int64_t>(x.b) * p.H + head) * p.N + node;
+          p.lse[at] = (m_all + log2f(l_all)) * kLn2;
+          p.marks[at] = again;
+          if (again) *any_marked = 1;
+        }
         if constexpr (kCluster) {
           const int to = row / rows_each;
           if (mine)
             reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemSums)[rank * rows_each + row - to * rows_each] =
                 make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
         } else if (mine && !whole) p.part_ml[static_cast<int64_t>(slot) * kRows + row] = make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
-        if (whole && any_marked[parity] != 0) {
-          bar_sync(4, 128 * kTeams);                          // the rows' output stands
-          for (uint32_t left = __ballot_sync(0xffffffffu, again); left != 0; left &= left - 1) {
-            const int from = __ffs(left) - 1;
-            tree_row<D>(p, x.b, __shfl_sync(0xffffffffu, node, from), __shfl_sync(0xffffffffu, head, from));
-          }
-        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kOut + parity);
@@ -1064,6 +1058,19 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   if (role == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+  if constexpr (!kCluster) {
+    // The rows of whole units that were marked, a warp a row: here, where nothing waits for them with a limit.  By the warps of the softmax, which have the registers for it.
+    if (role < 0 && *any_marked != 0) {
+      x = tree_first(p, sums, f_begin, f_end);
+      do {
+        if (!x.whole()) continue;
+        for (int r = warp; r < kRows; r += 4 * kTeams) {
+          const int unit_row = x.rt * kRows + r, node = node_of(p, unit_row), head = x.hk * p.rep + unit_row - node * p.rep;
+          if (node < x.s.count && p.marks[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] != 0) tree_row<D>(p, x.b, node, head);
+        }
+      } while (tree_next(p, x, f_end));
+    }
   }
 }
 
@@ -1237,11 +1244,12 @@ CacheTreePlan plan_cache_tree(int B, int N, int H, int Hk, int D, int T, int pag
   x.cluster = units <= resident_clusters(log) && tiles <= kClusterTiles && tiles <= (units * unit_tiles + workers - 1) / workers + kClusterGain ? 1 << log : 0;
   if (x.cluster > 0) {
     x.grid = static_cast<int>(units) * x.cluster;
-    x.part_o_bytes = x.part_ml_bytes = 0;
+    x.part_o_bytes = x.part_ml_bytes = x.mark_bytes = 0;
     x.cut_bytes = 16;
     return x;
   }
   x.grid = static_cast<int>(workers);
+  x.mark_bytes = (static_cast<int64_t>(B) * H * N + 15) / 16 * 16;
   x.part_o_bytes = 2ll * x.grid * x.row_tile * D * 4;
   x.part_ml_bytes = 2ll * x.grid * x.row_tile * 16;
   x.cut_bytes = x.grid * static_cast<int64_t>(sizeof(TreeCut));

@@ -47,6 +47,7 @@ struct CacheTreeParams {
   float* lse;                       // (B, H, N)
   float* part_o;                    // partial results: 2 slots a CTA, of row_tile rows of D fp32 each, and of their rows (m, l, u, marked): the sum is
   float4* part_ml;                  // l 2^m, the values count in 2^u
+  uint8_t* marks;                   // (B, H, N): whether a row of a whole unit is made by itself
   void* cuts;                       // and what the join needs of each cut unit
   int grid;                         // CTAs of the main kernel
   int cluster;                      // of a unit, or 0: the even division
@@ -57,8 +58,8 @@ struct CacheTreeParams {
 // How a call of dm_cache_attn_tree is laid out, and its workspace.
 struct CacheTreePlan {
   int row_tile, grid, cluster;
-  int64_t part_o_bytes, part_ml_bytes, cut_bytes;
-  int64_t bytes() const { return part_o_bytes + part_ml_bytes + cut_bytes; }
+  int64_t part_o_bytes, part_ml_bytes, mark_bytes, cut_bytes;
+  int64_t bytes() const { return part_o_bytes + part_ml_bytes + mark_bytes + cut_bytes; }
 };
 CacheTreePlan plan_cache_tree(int B, int N, int H, int Hk, int D, int T, int page);
 

@@ -133,7 +133,8 @@ int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, in
   p.lse = lse;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + x.part_o_bytes);
-  p.cuts = static_cast<uint8_t*>(workspace) + x.part_o_bytes + x.part_ml_bytes;
+  p.marks = static_cast<uint8_t*>(workspace) + x.part_o_bytes + x.part_ml_bytes;
+  p.cuts = static_cast<uint8_t*>(workspace) + x.part_o_bytes + x.part_ml_bytes + x.mark_bytes;
   p.grid = x.grid;
   p.cluster = x.cluster;
   p.row_tile = x.row_tile;

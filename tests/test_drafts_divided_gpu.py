@@ -228,3 +228,34 @@ def test_bad_device_values_are_reported():
         dm.dm_cache_attn_tree(q, cache, bad_table.cuda(), bad_n.cuda(), tree._replace(counts=None if counts is None else counts.cuda()))
         with pytest.raises(RuntimeError, match=says):
             ops.check_status("cuda")
+
+
+def test_marked_rows_of_long_whole_units():
+    """One sequence of many has a NaN in its first draft's value, and its rows are made by themselves over 131072 tokens: its units' CTA goes on with the next unit meanwhile, and no wait
+    for it runs out.  All sequences hold the same pages, but the last one; whole units come first in each CTA's share."""
+    B, N, H, Hk, D, P, n = 300, 8, 4, 1, 128, 256, 131072
+    last = (n + N) // P
+    g = torch.Generator(device="cuda").manual_seed(0)
+    pages = last + B
+    code = lambda: (torch.randn(pages, Hk, P, D, generator=g, device="cuda") * 40).to(torch.float8_e4m3fn)
+    cache = dm.KVCache8(code(), code(), *(torch.full((pages, Hk, P // 32), 2.0 ** -5, device="cuda") for _ in range(2)))
+    table = torch.arange(last + 1, dtype=torch.int32).expand(B, -1).clone()
+    table[:, last] = last + torch.arange(B)
+    assert _divided(B, N, H, Hk, D, table, P, 32) == 148
+    lengths = _ints([n + N] * B)
+    q = torch.randn(B, N, H, D, generator=g, device="cuda").to(BF)
+    parents = dref.make_parents("chain", B, N)
+    tree = dm.dm_draft_tree(parents.cuda())
+    args = (q, cache, table.cuda(), lengths.cuda(), tree)
+    whole = dm.dm_cache_attn_tree(*args, return_lse=True)
+    v = cache.v8.view(torch.uint8)
+    v[last, 0, n % P, 9] = 0x7F
+    got = dm.dm_cache_attn_tree(*args, return_lse=True)
+    torch.cuda.synchronize()
+    ops.check_status("cuda")
+    assert all(torch.equal(a[1:], b[1:]) for a, b in zip(whole, got))
+    assert bool(got[0][0, ..., 9].isnan().all()) and int(got[0].isnan().sum()) == N * H
+    (w, wl), (d, dl) = dref.attention(q[:1].cpu(), cache, table[:1], lengths[:1], [N], dref.tree(parents[:1], [N])[1], D ** -0.5)
+    for x, want, off in ((got[0][:1], w, d), (got[1][:1], wl, dl)):
+        same = x.isnan() & want.isnan()
+        assert bool((same | ((x.double() - want).abs() <= off)).all())
