@@ -746,6 +746,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           auto scale_byte = [&](float ku) { return static_cast<uint32_t>(fminf(fmaxf(ku - u + 119.f, 0.f), 254.f)); };       // of P's codes: 2^(ku - u - 8)
           auto put_words = [&](uint32_t at, uint32_t word) {
             const uint32_t words[8] = {word, word, word, word, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
+            __syncwarp();
             tmem_st8(at, words);
           };
           // The reference of the unit's products: from its first tile, or what that left.
@@ -770,6 +771,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll 1
           for (int c = 0; c < kBlocks; ++c) {
             uint32_t s[32];
+            __syncwarp();                                     // (here and below: a TMEM access is the whole warp's, whatever branches came before)
             tmem_ld32(t_s + 32 * (c0 + c), s);
             const float fc = f * lds_f(entry + 4 * (c0 + c));
             const float ev = lds_f(entry + 16 + 4 * (c0 + c));
@@ -777,6 +779,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             if (kCut) {
               sees = real ? seen_keys(seen, node, 128 * t + 32 * (c0 + c) - x.s.base()) : 0u;
               marked |= (sees & nan_tokens[c0 + c]) != 0u;
+              __syncwarp();
             }
             tmem_wait_ld();
             if (kCut) {
@@ -828,6 +831,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           }
           if (kCopies > 1) {
             const uint32_t zeros[16] = {};                    // other copies' blocks
+            __syncwarp();
 #pragma unroll 1
             for (int c = 0; c < 4; ++c)
               if (c < c0 || c >= c0 + kBlocks) tmem_st16(t_s + 32 * c, zeros);
@@ -884,6 +888,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           } else if (!(ok = cut ? tile(g, t, std::true_type{}) : tile(g, t, std::false_type{}))) {
             break;
           }
+          __syncwarp();
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -946,13 +951,14 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll 1
           for (int c = team; c < D / 16; c += kTeams) {
             uint32_t o[16];
+            __syncwarp();
             tmem_ld16(t_o + 16 * c, o);
             tmem_wait_ld();
             float y[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(o[e]) * w1 * w2;
-            if (at < 0) continue;
-            if (whole) {
+            if (at < 0) {                                     // a row that is none
+            } else if (whole) {
               uint32_t h[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
@@ -976,6 +982,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll 1
           for (int c = team; c < D / 16; c += kTeams) {
             uint32_t o[16];
+            __syncwarp();
             tmem_ld16(t_o + 16 * c, o);
             tmem_wait_ld();
 #pragma unroll
@@ -997,8 +1004,8 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                 y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
               }
               const int at = out_rows[128 * parity + r];
-              if (at < 0) continue;
-              if constexpr (kCluster) {
+              if (at < 0) {
+              } else if (kCluster) {
                 values_of(r)[value_at(r, 4 * c + piece)] = y;
               } else if (whole) {
                 const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
@@ -1008,6 +1015,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                 *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * kRows + r) * D + 16 * c + 4 * piece) = y;
               }
             }
+            __syncwarp();
             bar_sync(1 + team, 128);
           }
         }
