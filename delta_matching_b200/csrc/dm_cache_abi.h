@@ -60,5 +60,20 @@ inline int check_rows(const char* name, const void* p, int64_t a, int64_t b, int
   return 0;
 }
 
+// Rows of int32 that a kernel reads (n entries from one row's first to the last row's last).
+struct IntRows {
+  const int* p;
+  int64_t n;
+  const char* name;
+};
+inline int64_t rows_of(int B, int64_t row, int64_t n) { return (B - 1) * row + n; }
+// The kernels' CTAs read these while one of them writes new_lengths.
+inline int check_new_lengths(const int* out, int B, std::initializer_list<IntRows> in) {
+  for (const IntRows& x : in)
+    if (x.p != nullptr && x.p < out + B && out < x.p + x.n)
+      return fail(DM_ERR_ARG, "delta_matching: new lengths must not share memory with %s (a buffer of their own)", x.name);
+  return 0;
+}
+
 }  // namespace abi
 }  // namespace dm

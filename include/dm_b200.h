@@ -245,6 +245,8 @@ int dm_copy_2d_async(void* dst, int64_t dpitch, const void* src, int64_t spitch,
  * Rows of the table may be one and the same (table_row 0) where sequences are only read; a page that is written belongs to one sequence.
  * Table entries, lengths and counts are device data that the host does not see: a kernel that meets one out of range reports it through
  * `status` (DM_STATUS_BAD_PAGE, DM_STATUS_BAD_LENGTH), stays inside the buffers, and its outputs are invalid.
+ * new_lengths of the functions below is a buffer of its own, written while other parts of the kernel still read lengths, counts and tables: one that
+ * shares memory with an int32 input is refused.  Other outputs must not share memory with inputs either, which is the caller's word.
  * All pointers are the caller's word to be memory of the current device, as in dm_attn_fwd. */
 typedef struct dm_kv_cache {
   void* k8;
