@@ -2,8 +2,8 @@
 // dm_cache_append.cu).
 //
 // A pair (a, b) of channels of frequency f at position t becomes (a cos - b sin, b cos + a sin) of the angle t f.  Angles are counted in turns and reduced in 64
-// bits (off by less than 2^-24 for t f up to 2^27; in 32 bits a position of 10^5 would leave the angle three digits), their sine and cosine are fp32 of half turns, which
-// need no reduction of their own; keys go from the fp32 products to their codes with one rounding, queries to bf16.
+// bits (in 32 bits a position of 10^5 would leave them three digits).  Sine and cosine are fp32, of half turns, which need no reduction of their own, and of what rounding these to fp32 leaves to
+// first order, so that a channel that all but vanishes keeps its digits too (64 x 20 tokens 11.1 -> 11.36 us, others as before).  Keys go from the fp32 products to their codes with one rounding, queries to bf16.
 //
 // A CTA is a (sequence, block of 32 slots, group of heads).  The block's sines and cosines are made once, in shared memory, for all its heads; then a warp
 // takes a head of k, v or q at a time.  A lane holds eight pairs of a row, so that neither needs another lane's values.
@@ -24,11 +24,13 @@ constexpr int kRotaryWarps = 8;
 // is cold), both sides equal at 2048 and 4096.
 constexpr int kManyTokens = 4096;
 
-// cos and sin of so many turns.
+// cos and sin of so many turns; `rest`: what fp32 leaves of the angle, up to 2^-25 of half a turn (its square is nothing).
 __device__ __forceinline__ float2 turn(double turns) {
+  const double half_turns = 2.0 * (turns - rint(turns));
+  const float near = static_cast<float>(half_turns), rest = static_cast<float>(half_turns - near) * 3.14159265f;
   float s, c;
-  sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-  return make_float2(c, s);
+  sincospif(near, &s, &c);
+  return make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
 }
 
 // kAhead: passes whose rows are in flight.
