@@ -44,6 +44,9 @@ constexpr int kTreeCost = 4;
 constexpr float kExact = 4194304.f;         // logits (log2) up to this size: whole numbers beside them are exact
 constexpr float kReach = 40.f;              // what a row's logits may exceed the reference of its sum by, in powers of two: fp32 has room for it
 constexpr int kUnitLift = 40;               // of the reference of the products, above those it was taken from
+// What a V scale counts for that, at least: a block of zeros (padding at a sequence's head) has 2^-126, and the products behind it may be of any size.  80 above such a block's products
+// still leaves them 2^-29 to the right.
+constexpr float kLeastScale = -86.f;
 
 template <int kD>
 struct TreeCfg {
@@ -750,8 +753,10 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             tmem_st8(at, words);
           };
           // The reference of the unit's products: from its first tile, or what that left.
-          auto know_u = [&](float top_u) -> bool {
+          auto know_u = [&](float ku0, float ku1) -> bool {
             if (g == g0) {
+              auto above = [&](int c) { return fmaxf(0.f, kLeastScale - lds_f(entry + 16 + 4 * (c0 + c))); };
+              const float top_u = fmaxf(ku0 + above(0), kBlocks > 1 ? ku1 + above(1) : kNone);
               const bool none = !(top_u > kNone);
               const int code = 2 * (none ? kUnitLift : static_cast<int>(fminf(fmaxf(top_u, -kExact), kExact)) + kUnitLift) + (none ? 1 : 0);
               *u_at = code;
@@ -820,7 +825,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             if (c & 1) ku[1] = kb + ev;
             else ku[0] = kb + ev;
             if (kCopies == 1 && c == 1) {                     // the first half of the keys: the tensor cores may begin
-              if (!know_u(fmaxf(ku[0], ku[1]))) return false;
+              if (!know_u(ku[0], ku[1])) return false;
               hi = fmaxf(hi, fmaxf(ku[0], ku[1]));
               put_words(t_s + 16, scale_byte(ku[0]) | scale_byte(ku[1]) << 8);
               tmem_wait_st();
@@ -836,7 +841,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             for (int c = 0; c < 4; ++c)
               if (c < c0 || c >= c0 + kBlocks) tmem_st16(t_s + 32 * c, zeros);
             if (kBlocks == 1) ku[1] = ku[0];
-            if (!know_u(fmaxf(ku[0], ku[1]))) return false;
+            if (!know_u(ku[0], ku[1])) return false;
           }
           hi = fmaxf(hi, fmaxf(ku[0], ku[1]));
           const uint32_t two = scale_byte(ku[0]) | scale_byte(ku[1]) << 8;

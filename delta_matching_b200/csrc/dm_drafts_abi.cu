@@ -103,7 +103,13 @@ int64_t dm_cache_attn_tree_workspace_bytes(int B, int N, int H, int Hk, int D, i
 int dm_dbg_cache_tree_plan(int B, int N, int H, int Hk, int D, int T, int page_size, int what) {
   DM_TRY(check_tree_shape(B, N, H, Hk, D, T, page_size));
   const dm::CacheTreePlan x = dm::plan_cache_tree(B, N, H, Hk, D, T, page_size);
-  return what == 0 ? x.cluster : what == 1 ? x.grid : what == 2 ? x.row_tile : fail(DM_ERR_ARG, "delta_matching: what must be 0, 1 or 2 (got %d)", what);
+  switch (what) {
+    case 0: return x.cluster;
+    case 1: return x.grid;
+    case 2: return x.row_tile;
+    case 3: return static_cast<int>(x.part_o_bytes + x.part_ml_bytes);        // (of 148 CTAs at most: 80 MB)
+  }
+  return fail(DM_ERR_ARG, "delta_matching: what must be 0 ... 3 (got %d)", what);
 }
 
 int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, int B, int N, int H,

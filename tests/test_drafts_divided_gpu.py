@@ -42,7 +42,7 @@ def _held(n, N, Hk, D, P=64, seed=0, **kw):
 
 def test_plan_refuses():
     plan = _lib.lib().dm_dbg_cache_tree_plan
-    assert plan(2, 0, 8, 2, 128, 4, 64, 0) < 0 and plan(2, 5, 8, 3, 128, 4, 64, 0) < 0 and plan(2, 5, 8, 2, 128, 4, 64, 3) < 0
+    assert plan(2, 0, 8, 2, 128, 4, 64, 0) < 0 and plan(2, 5, 8, 3, 128, 4, 64, 0) < 0 and plan(2, 5, 8, 2, 128, 4, 64, 4) < 0
     assert plan(2, 5, 8, 2, 128, 4, 64, 2) == 32 and plan(2, 9, 8, 2, 128, 4, 64, 2) == 64 and plan(2, 30, 8, 2, 128, 4, 64, 2) == 128
 
 
