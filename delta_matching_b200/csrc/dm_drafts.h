@@ -41,7 +41,7 @@ struct CacheTreeParams {
   const int* counts;                // (B) or null: N each
   const uint32_t* seen;             // (B, N, words): bit j % 32 of word j / 32 of node i: node i sees node j; by element strides, words adjacent
   int64_t s_sb, s_sn;
-  int N, H, rep, words;
+  int N, H, rep;
   float scale;                      // softmax scale
   __nv_bfloat16* o;                 // (B, N, H, D) contiguous
   float* lse;                       // (B, H, N)

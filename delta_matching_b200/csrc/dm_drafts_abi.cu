@@ -135,7 +135,7 @@ int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, in
   p.counts = counts;
   p.seen = reinterpret_cast<const uint32_t*>(seen);
   p.s_sb = seen_sb; p.s_sn = seen_sn;
-  p.N = N; p.H = H; p.rep = H / cache->heads; p.words = (N + 31) / 32;
+  p.N = N; p.H = H; p.rep = H / cache->heads;
   p.scale = softmax_scale;
   p.o = static_cast<__nv_bfloat16*>(o);
   p.lse = lse;
