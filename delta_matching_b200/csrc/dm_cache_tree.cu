@@ -41,6 +41,8 @@ constexpr int kMaxCluster = 8;
 
 // Key tiles that a unit's queries and output are worth (8 instead: as fast to 2 % in calls of 4 x 8000 to 64 x 4096 tokens; 2: 5 % slower in the first).
 constexpr int kTreeCost = 4;
+// Marks of a row: channels of it become NaN; it is made by itself.
+constexpr int kNanChannels = 1, kByItself = 2;
 constexpr float kExact = 4194304.f;         // logits (log2) up to this size: whole numbers beside them are exact
 constexpr float kReach = 40.f;              // what a row's logits may exceed the reference of its sum by, in powers of two: fp32 has room for it
 constexpr int kUnitLift = 40;               // of the reference of the products, above those it was taken from
@@ -196,10 +198,11 @@ __device__ __forceinline__ uint32_t seen_keys(const uint32_t* seen, int i, int r
 }
 
 // ------------------------------------------------------------------------------------------------ one row
-// Row (b, i, head) by one warp and from the definition: a key after the other, the logits' differences exact whatever their size.  For rows that the
-// kernel below marks, always when the tiles are done with: it takes about 0.6 us a key, and nothing that waits with a limit may wait for it.
+// Rows that the kernels below mark are seen to by one warp each, always when the tiles are done with: nothing that waits with a limit may wait for it.
+//
+// Row (b, i, head) from the definition: a key after the other, the logits' differences exact whatever their size.  About 0.6 us a key.
 template <int D>
-__device__ __noinline__ void tree_row(const CacheTreeParams& p, int b, int i, int head) {
+__device__ __forceinline__ void tree_row(const CacheTreeParams& p, int b, int i, int head) {
   constexpr int kVecs = D / 128;
   const int lane = threadIdx.x & 31, bpp = p.c.page / 32, hk = head / p.rep;
   const TreeSeq t = tree_seq(p, b);
@@ -249,6 +252,35 @@ __device__ __noinline__ void tree_row(const CacheTreeParams& p, int b, int i, in
     o[64 * x + 1] = __floats2bfloat162_rn(acc[x].z / sum, acc[x].w / sum);
   }
   if (lane == 0) p.lse[(static_cast<int64_t>(b) * p.H + head) * p.N + i] = (m + log2f(sum)) * kLn2;
+}
+
+// NaN in the channels of row (b, i, head) in which a drafted token that it sees has NaN values, where the tiles had zeros in their place.  (Keys that are NaN need nothing of the kind: their
+// logits are.)  64 sequences of 1000 tokens with 25 drafts take 0.25 ms instead of 0.09 where one of them has such a token, 19 where its rows were made by themselves instead.
+template <int D>
+__device__ __forceinline__ void nan_channels(const CacheTreeParams& p, int b, int i, int head) {
+  const int lane = threadIdx.x & 31, bpp = p.c.page / 32, hk = head / p.rep, base = tree_seq(p, b).base();
+  const uint32_t* seen = p.seen + b * p.s_sb + i * p.s_sn;
+  uint16_t* o = reinterpret_cast<uint16_t*>(p.o + ((static_cast<int64_t>(b) * p.N + i) * p.H + head) * D) + 4 * lane;
+  __syncwarp();                                               // the row stands, by whichever lanes
+#pragma unroll 1
+  for (int node = 0; node <= i; ++node) {
+    if (!((seen_word(seen, i, node >> 5) >> (node & 31)) & 1u)) continue;
+    const int j = base + node, blk = j / 32, page = max(0, checked_page(p.c, __ldg(p.c.table + b * p.c.t_row + blk / bpp)));
+    const uint8_t* code = p.c.v8 + page * p.c.c_page + hk * p.c.c_head + (blk % bpp * 32 + j % 32) * p.c.c_slot + 4 * lane;
+#pragma unroll 1
+    for (int x = 0; x < D; x += 128) {
+      const uint32_t bad = nan_codes(__ldg(reinterpret_cast<const uint32_t*>(code + x)));
+      for (int e = 0; e < 4; ++e)
+        if ((bad >> (8 * e)) & 1u) o[x + e] = 0x7FFF;
+    }
+  }
+}
+
+// A marked row, whose output stands.  (Two bits of state where the kernels mark, and one call here: as one number 19.3 us for 4 sequences of 4000 tokens became 20.4.)
+template <int D>
+__device__ __noinline__ void marked_row(const CacheTreeParams& p, int b, int i, int head, int mark) {
+  if (mark == kByItself) tree_row<D>(p, b, i, head);
+  else nan_channels<D>(p, b, i, head);
 }
 
 // ------------------------------------------------------------------------------------------------ instructions
@@ -359,7 +391,7 @@ __device__ __forceinline__ void join_cluster(const CacheTreeParams& p, const Tre
         const float4 st = sums[c * rows + i];
         top = fmaxf(top, st.x);
         if (st.x > kNone) u_top = fmaxf(u_top, st.z);
-        marked += st.w;
+        marked = fmaxf(marked, st.w);
       }
       for (int c = 0; c < cl; ++c) {
         const float4 st = sums[c * rows + i];
@@ -376,7 +408,7 @@ __device__ __forceinline__ void join_cluster(const CacheTreeParams& p, const Tre
         }
       }
     }
-    if (mine && marked == 0.f) {
+    if (mine && marked != kByItself) {
       const float d_all = u_top - top, d1 = fminf(fmaxf(d_all, -100.f), 100.f);
       const float w1 = real ? exp2f(d1) : 0.f, w2 = real ? exp2f(d_all - d1) / sum : 0.f;
       uint2* o = reinterpret_cast<uint2*>(p.o + ((static_cast<int64_t>(x.b) * p.N + node) * p.H + head) * D) + l;
@@ -387,10 +419,10 @@ __device__ __forceinline__ void join_cluster(const CacheTreeParams& p, const Tre
       }
       if (l == 0) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = real ? (top + log2f(sum)) * kLn2 : -CUDART_INF_F;
     }
-    // rows that are made by themselves: by the whole warp
+    // marked rows: by the whole warp
     for (uint32_t left = __ballot_sync(0xffffffffu, real && marked != 0.f && l == 0); left != 0; left &= left - 1) {
-      const int from = __ffs(left) - 1;
-      tree_row<D>(p, x.b, __shfl_sync(0xffffffffu, node, from), __shfl_sync(0xffffffffu, head, from));
+      const int from = __ffs(left) - 1, node_from = __shfl_sync(0xffffffffu, node, from), head_from = __shfl_sync(0xffffffffu, head, from);
+      marked_row<D>(p, x.b, node_from, head_from, static_cast<int>(__shfl_sync(0xffffffffu, marked, from)));
     }
   }
 }
@@ -741,7 +773,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         // move: fp32 has room for products 2^95 above it (hi: the largest that this team has met), and a row that has larger ones is marked.
         float m = kNone, l = 0.f, u = 0.f, hi = kNone;
         int u_code = 0;
-        bool knows_u = false, marked = false;
+        bool knows_u = false, marked = false, sees_nan = false;
         // One key tile.  kCut: some row does not see all its keys (a compile-time variant: no select per element elsewhere).
         auto tile = [&](int g, int t, auto cut_tag) -> bool {
           constexpr bool kCut = decltype(cut_tag)::value;
@@ -783,7 +815,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             uint32_t sees = 0xffffffffu;
             if (kCut) {
               sees = real ? seen_keys(seen, node, 128 * t + 32 * (c0 + c) - x.s.base()) : 0u;
-              marked |= (sees & nan_tokens[c0 + c]) != 0u;
+              sees_nan |= (sees & nan_tokens[c0 + c]) != 0u;
               __syncwarp();
             }
             tmem_wait_ld();
@@ -854,8 +886,8 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           ok = wait_warp(bar(kScales + (g & 7)), (g >> 3) & 1, abort_flag) && wait_warp(bar(kS + team), phase_of(g), abort_flag);
           const bool cut = 128 * (t + 1) > x.s.base();
           if (cut) {
-            // V's slots behind the length hold anything, and a drafted token may be NaN, which only the rows that see it are to meet: zeros in the place of both, or
-            // they would come through the products with P's zeros.  Which tokens were NaN is left to the rows.  A thread a token.
+            // V's slots behind the length hold anything, and a drafted token may have NaN values, which only the rows that see it are to meet: zeros in the place of both, or
+            // they would come through the products with P's zeros.  Which tokens had NaN is left to the rows, which get theirs when they stand.  A thread a token.
             const int st = (2 * g + 1) % C::kStages, j = 128 * t + in_tile;
             if (ok) ok = wait_warp(bar(kFull + st), ((2 * g + 1) / C::kStages) & 1, abort_flag);
             bool nan = false;
@@ -868,9 +900,17 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                 const float4 w = lds_f4(piece(y));
                 found |= nan_codes(__float_as_uint(w.x)) | nan_codes(__float_as_uint(w.y)) | nan_codes(__float_as_uint(w.z)) | nan_codes(__float_as_uint(w.w));
               }
-              if (found != 0 || j >= x.s.n) {
+              if (j >= x.s.n) {
 #pragma unroll 1
                 for (int y = 0; y < 8 * C::kPanels; ++y) sts_u4(piece(y), 0u, 0u, 0u, 0u);
+                fence_async_smem();
+              } else if (found != 0) {
+                auto clean = [](float v) { return __float_as_uint(v) & ~nan_codes(__float_as_uint(v)); };
+#pragma unroll 1
+                for (int y = 0; y < 8 * C::kPanels; ++y) {
+                  const float4 w = lds_f4(piece(y));
+                  sts_u4(piece(y), clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+                }
                 fence_async_smem();
               }
               nan = found != 0 && j < x.s.n;
@@ -909,7 +949,7 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         stats[128 * team + in_tile] = make_float2(m, l);
         // out of u's range: above; or below where u was not taken from the row's own products
         marked |= hi > u + 95.f || ((u_code & 1) != 0 && hi > kNone && hi < u - 80.f);
-        if (real && marked) marks[128 * parity + row] = 1;
+        if (real && (marked || sees_nan)) reinterpret_cast<volatile uint8_t*>(marks + 128 * parity + row)[marked ? 1 : 0] = 1;      // (teams and copies may differ)
         if (!(ok = all_of(4, 128 * kTeams, ok))) break;
         tc_fence_after();
         [[maybe_unused]] cg::cluster_group::arrival_token tiles_done;
@@ -1026,19 +1066,19 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
         const bool mine = team == 0 && copy == 0 && real;
         const int head = x.hk * p.rep + unit_row - node * p.rep;
-        const bool again = mine && marks[128 * parity + row] != 0;
+        const int said = mine ? marks[128 * parity + row] : 0, mark = said > 1 ? kByItself : said;
         if (mine && whole) {
           const int64_t at = (static_cast<int64_t>(x.b) * p.H + head) * p.N + node;
           p.lse[at] = (m_all + log2f(l_all)) * kLn2;
-          p.marks[at] = again;
-          if (again) *any_marked = 1;
+          p.marks[at] = mark;
+          if (mark != 0) *any_marked = 1;
         }
         if constexpr (kCluster) {
           const int to = row / rows_each;
           if (mine)
             reinterpret_cast<float4*>(cg::this_cluster().map_shared_rank(smem, to) + C::kSmemSums)[rank * rows_each + row - to * rows_each] =
-                make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
-        } else if (mine && !whole) p.part_ml[static_cast<int64_t>(slot) * kRows + row] = make_float4(m_all, l_all, u_all, again ? 1.f : 0.f);
+                make_float4(m_all, l_all, u_all, mark);
+        } else if (mine && !whole) p.part_ml[static_cast<int64_t>(slot) * kRows + row] = make_float4(m_all, l_all, u_all, mark);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kOut + parity);
@@ -1080,7 +1120,8 @@ cache_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (!x.whole()) continue;
         for (int r = warp; r < kRows; r += 4 * kTeams) {
           const int unit_row = x.rt * kRows + r, node = node_of(p, unit_row), head = x.hk * p.rep + unit_row - node * p.rep;
-          if (node < x.s.count && p.marks[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] != 0) tree_row<D>(p, x.b, node, head);
+          const int mark = node < x.s.count ? p.marks[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] : 0;
+          if (mark != 0) marked_row<D>(p, x.b, node, head, mark);
         }
       } while (tree_next(p, x, f_end));
     }
@@ -1106,14 +1147,14 @@ __global__ void __launch_bounds__(128) cache_tree_join_kernel(const __grid_const
   if (node >= x.count) return;
   float top = kNone, u_top = kNone, sum = 0.f;
   float4 acc[kVecs] = {};
-  bool marked = false;
+  float marked = 0.f;
   // 32 results at a time, a lane each: their maxima and sums together, then the values of those that count
   for (int w0 = x.first; w0 <= x.last; w0 += 32) {
     const int w = w0 + lane;
     const bool there = w <= x.last;                           // each has a tile at least
     const int64_t at = there ? static_cast<int64_t>(w == x.first ? x.slot : 2 * w) * p.row_tile + r : 0;
     const float4 ml = there ? p.part_ml[at] : make_float4(kNone, 0.f, kNone, 0.f);
-    marked |= __any_sync(0xffffffffu, ml.w != 0.f);
+    marked = fmaxf(marked, warp_max(ml.w));
     float top_new = ml.x, u_new = ml.x > kNone ? ml.z : kNone;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -1145,7 +1186,7 @@ __global__ void __launch_bounds__(128) cache_tree_join_kernel(const __grid_const
       }
     }
   }
-  if (marked) {
+  if (marked == kByItself) {
     tree_row<D>(p, x.b, node, head);
     return;
   }
@@ -1158,6 +1199,7 @@ __global__ void __launch_bounds__(128) cache_tree_join_kernel(const __grid_const
     o[64 * v + 1] = __floats2bfloat162_rn(acc[v].z * w1 * w2, acc[v].w * w1 * w2);
   }
   if (lane == 0) p.lse[(static_cast<int64_t>(x.b) * p.H + head) * p.N + node] = (top + log2f(sum)) * kLn2;
+  if (marked != 0.f) nan_channels<D>(p, x.b, node, head);
 }
 
 // Once per kernel and device: the driver call takes longer than a launch.

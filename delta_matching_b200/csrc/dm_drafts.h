@@ -47,7 +47,7 @@ struct CacheTreeParams {
   float* lse;                       // (B, H, N)
   float* part_o;                    // partial results: 2 slots a CTA, of row_tile rows of D fp32 each, and of their rows (m, l, u, marked): the sum is
   float4* part_ml;                  // l 2^m, the values count in 2^u
-  uint8_t* marks;                   // (B, H, N): whether a row of a whole unit is made by itself
+  uint8_t* marks;                   // (B, H, N): of a row of a whole unit, its mark
   void* cuts;                       // and what the join needs of each cut unit
   int grid;                         // CTAs of the main kernel
   int cluster;                      // of a unit, or 0: the even division

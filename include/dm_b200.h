@@ -321,7 +321,7 @@ int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, in
 
 /* Test hook, host only: how dm_cache_attn_tree lays a call out on the current device (148 SMs without one, and no clusters).  what = 0: the CTAs of a cluster that takes a unit, 0 where the
  * key tiles of all units are divided evenly instead; 1: CTAs; 2: rows of a unit; 3: where in the workspace of a divided call the marks lie, a byte for each row (B, H, N) of a unit that one CTA
- * had whole: 1 where it was made by itself.  Negative: a shape that is refused. */
+ * had whole: 1 where a drafted value that it sees is NaN, 2 where the row was made by itself.  Negative: a shape that is refused. */
 int dm_dbg_cache_tree_plan(int B, int N, int H, int Hk, int D, int T, int page_size, int what);
 
 /* Of the drafted tokens before[b] ... lengths[b] - 1 those of a path are kept: path[b, 0 ... counts[b] - 1], strictly increasing indexes behind before[b]

@@ -230,9 +230,8 @@ def test_bad_device_values_are_reported():
             ops.check_status("cuda")
 
 
-def test_marked_rows_of_long_whole_units():
-    """One sequence of many has a NaN in its first draft's value, and its rows are made by themselves over 131072 tokens: its units' CTA goes on with the next unit meanwhile, and no wait
-    for it runs out.  All sequences hold the same pages, but the last one; whole units come first in each CTA's share."""
+def _long_whole_units():
+    """Three hundred sequences of 131072 tokens, all of the same pages but the last one; whole units come first in each CTA's share."""
     B, N, H, Hk, D, P, n = 300, 8, 4, 1, 128, 256, 131072
     last = (n + N) // P
     g = torch.Generator(device="cuda").manual_seed(0)
@@ -246,16 +245,85 @@ def test_marked_rows_of_long_whole_units():
     q = torch.randn(B, N, H, D, generator=g, device="cuda").to(BF)
     parents = dref.make_parents("chain", B, N)
     tree = dm.dm_draft_tree(parents.cuda())
+    return q, cache, table, lengths, tree, parents
+
+
+@pytest.mark.parametrize("kind", ["nan", "large"])
+def test_marked_rows_of_long_whole_units(kind):
+    """One sequence of many has a NaN in its first draft's value, or logits for which its rows are made by themselves, a key after the other over 131072 tokens: its unit's CTA goes on with the
+    next unit meanwhile, and no wait runs out."""
+    q, cache, table, lengths, tree, parents = _long_whole_units()
+    N, H, D = q.shape[1:]
     args = (q, cache, table.cuda(), lengths.cuda(), tree)
     whole = dm.dm_cache_attn_tree(*args, return_lse=True)
-    v = cache.v8.view(torch.uint8)
-    v[last, 0, n % P, 9] = 0x7F
+    if kind == "nan":
+        at = int(lengths[0]) - N
+        cache.v8.view(torch.uint8)[int(table[0, at // 256]), 0, at % 256, 9] = 0x7F
+    else:
+        q[0] *= 1e6
     got = dm.dm_cache_attn_tree(*args, return_lse=True)
     torch.cuda.synchronize()
     ops.check_status("cuda")
     assert all(torch.equal(a[1:], b[1:]) for a, b in zip(whole, got))
-    assert bool(got[0][0, ..., 9].isnan().all()) and int(got[0].isnan().sum()) == N * H
+    assert int(got[0].isnan().sum()) == (N * H if kind == "nan" else 0) == int(got[0][0, ..., 9].isnan().sum())
     (w, wl), (d, dl) = dref.attention(q[:1].cpu(), cache, table[:1], lengths[:1], [N], dref.tree(parents[:1], [N])[1], D ** -0.5)
     for x, want, off in ((got[0][:1], w, d), (got[1][:1], wl, dl)):
         same = x.isnan() & want.isnan()
         assert bool((same | ((x.double() - want).abs() <= off)).all())
+
+
+@pytest.mark.parametrize("before, B", [(1000, 64), (3000, 4), (6000, 8)])
+def test_a_nan_value_costs_little(before, B):
+    """NaN in one channel of the values of a sequence's first draft, which all its rows see: nothing is summed anew, the call takes at most twenty times as long (a few hundred times if
+    those rows were made a key after the other).  Sequences whose units are whole, cut, and a cluster's."""
+    N, H, Hk, D, P = 25, 32, 8, 128, 64
+    n = [before + N] * B
+    T = -(-n[0] // P)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    code = lambda: (torch.randn(B * T, Hk, P, D, generator=g, device="cuda") * 40).to(torch.float8_e4m3fn)
+    cache = dm.KVCache8(code(), code(), *(torch.full((B * T, Hk, P // 32), 2.0 ** -5, device="cuda") for _ in range(2)))
+    table = torch.arange(B * T, dtype=torch.int32).view(B, T)
+    tree = dm.dm_draft_tree(dref.make_parents("chain", B, N).cuda())
+    q = torch.randn(B, N, H, D, generator=g, device="cuda").to(BF)
+    args = (q, cache, table.cuda(), _ints(n).cuda(), tree)
+
+    def took():
+        best = math.inf
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            out = dm.dm_cache_attn_tree(*args)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best, out
+
+    base, plain = took()
+    cache.v8.view(torch.uint8)[int(table[0, before // P]), :, before % P, 3] = 0x7F
+    with_nan, out = took()
+    ops.check_status("cuda")
+    assert bool(out[0, ..., 3].isnan().all()) and int(out.isnan().sum()) == N * H
+    keep = torch.ones(D, dtype=torch.bool, device="cuda")
+    keep[3] = False
+    assert torch.equal(out[..., keep], plain[..., keep]) and torch.equal(out[1:], plain[1:])
+    assert with_nan < 20 * base, (with_nan, base)
+
+
+@pytest.mark.parametrize("divided", [False, True])
+@pytest.mark.parametrize("N, H, Hk, D, rows", SHAPES)
+def test_nan_values_and_large_logits(N, H, Hk, D, rows, divided):
+    """Both at once, in different channels of two drafted tokens: what a row sees of them, and nothing else, is NaN; some rows have large logits, others not."""
+    n = [N + 130, N + 37, N + 700]
+    cache, _, table = _filled(n, 64, Hk, D, seed=2)
+    if divided:
+        table = _wide(table, 64)
+    assert (_plan(3, N, H, Hk, D, table, 64)[0] == 0) == divided
+    v = cache.v8.view(torch.uint8)
+    for b in range(3):
+        for node, channel in ((0, 3), (min(2, N - 1), D - 2)):
+            at = n[b] - N + node
+            v[int(table[b, at // 64]), :, at % 64, channel] = 0xFF
+    g = torch.Generator().manual_seed(3)
+    q = _rand(g, 3, N, H, D)
+    q[:, ::3] *= 1e6
+    _attended(q, cache, table, _ints(n), None, dref.make_parents("any", 3, N, seed=1), scale=10.0)
