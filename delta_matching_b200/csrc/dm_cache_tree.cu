@@ -14,16 +14,16 @@
 // One CTA an SM.  Three teams of four softmax warps (thread = TMEM lane; two teams at head_dim 256) take the tiles of a unit in turn, each with an S buffer in TMEM;
 // P's codes and scale bytes lie over the S that they come from.  Of the last four warps two load the code tiles of K and of V from the pages by TMA and two issue the MMAs.
 // The power of two that a row of O counts in is fixed by the unit's first blocks: fp32 has room for what may follow (rows for which it has not are marked and made by
-// themselves), and no team waits for another's maximum.
+// themselves when the tiles are done with), and no team waits for another's maximum.
 //
 // kCopies: where a unit has at most 64 or 32 rows, they stand twice or four times in the 128 lanes, and copy c looks after its share of a tile's blocks of 32
 // keys (P is zero in the others), with a reference, a sum and an accumulator of its own, which the CTA adds up at the end: the softmax of a tile is as much
 // shorter, and the tensor cores, which take 128 rows whatever is in them, have no more to do.
 //
-// Measured (H 32, Hk 8, head_dim 128 but for the last two): 4 sequences of 4000 tokens with 16 drafts 19.1 us; 64 of 4096 with 8 drafts 130 us, 4.1 TB/s of codes, with 25 178 us;
-// one of 65536 with 60 drafts of 64 heads 158 us; 8 of 6144 with 33 drafts of 16 heads of 256 98 us, 4.1 TB/s.  What bounds it: with few rows the chain softmax, P V, next S
+// Measured (H 32, Hk 8, head_dim 128 but for the last two): 4 sequences of 4000 tokens with 16 drafts 19.4 us; 64 of 4096 with 8 drafts 130 us, 4.1 TB/s of codes, with 25 183 us;
+// one of 65536 with 60 drafts of 64 heads 164 us; 8 of 6144 with 33 drafts of 16 heads of 256 101 us, 4.0 TB/s.  What bounds it: with few rows the chain softmax, P V, next S
 // of a buffer (2100 cycles behind a tile's 1000; the products of a tile alone take 1024) and 7000 cycles from a unit's last tile to the next one's first; with 128 rows the softmax (1350 cycles a
-// tile at saturation, of about 2200).  Above a hundred us the chip is at its power limit (1.4 - 1.7 GHz).  Small calls: 5000 cycles to the first S, 9000 from the last
+// tile at saturation, of about 2250).  Above a hundred us the chip is at its power limit (1.4 - 1.7 GHz).  Small calls: 5000 cycles to the first S, 9000 from the last
 // tile to the end of the cluster's join, of 32000.
 #include <cooperative_groups.h>
 #include <type_traits>
@@ -291,8 +291,8 @@ __device__ __forceinline__ uint32_t cvt_e5m2x2(float lo, float hi) {
   return r;
 }
 // Four values of 0 ... 256 -> four e4m3 codes of them, rounded to four significant bits, and the codes of what that leaves, of either sign and 2^(e - 4) at most for a value of
-// 2^e ... 2^(e + 1): together off by 2^(e - 9), half a step of the second code; NaN becomes that of the second code.  (Rounded as integers, ties up: to know what a rounded code left by converting it back took 580 instead of 450 cycles for
-// 32 exponentials and their codes.  Measured, 64 sequences of 4096 tokens with 25 drafts: first four bits cut off, 2^-8, 178 us; rounded 183; a third code, 2^-12, 201, and 146 instead of
+// 2^e ... 2^(e + 1): together off by 2^(e - 9), half a step of the second code; NaN becomes that of the second code.  (Rounded as integers, ties up: 32 exponentials and their codes take a warp alone 510 cycles and three warps
+// of a scheduler 335 each; 450 and 324 with the first code cut off, 580 and 341 where what a rounded one left is known by converting it back.  Measured, 64 sequences of 4096 tokens with 25 drafts: first four bits cut off, 2^-8, 178 us; rounded 183; a third code, 2^-12, 201, and 146 instead of
 // 130 with 8 drafts.  Two codes keep what bf16 weights would, and o is rounded to bf16 in any case: its error against 64 bits is 0.00083 there, of which that rounding is 0.00076;
 // with the bits cut off it was 0.00122.)
 __device__ __forceinline__ void split4(float2 x, float2 y, uint32_t& first, uint32_t& second) {

@@ -313,6 +313,9 @@ int dm_cache_append_rotary(const dm_kv_cache* cache, const void* q, int64_t q_sb
 /* Attention of the N drafted tokens a sequence, the last counts[b] of the lengths[b] tokens that the cache holds: node i sees all tokens before the drafted
  * ones, the earlier nodes whose bits are set in seen[b, i] (as dm_draft_tree writes them; by element strides, words adjacent) and itself; other bits are
  * not looked at.  o (B, N, H, head_dim) bf16 contiguous, lse (B, H, N) fp32 natural log; nodes beyond counts: 0 and -inf.
+ * q keeps its 8 bits down to 2^-13 of the row's largest element, smaller ones are off by 2^-21 of that; a probability in the second product is off by 2^-9 of itself and by
+ * 2^-16 of the largest one of its block of 32 keys; sums and statistics are fp32.  Rows with logits beyond 2^22, or whose later logits are above the first 32 to
+ * 64 keys' by 90 (by 38 where these have values of zero), are served one key after the other, about 0.6 us each.
  * workspace: dm_cache_attn_tree_workspace_bytes, 16-byte aligned, contents ignored (0: a shape that is refused). */
 int64_t dm_cache_attn_tree_workspace_bytes(int B, int N, int H, int Hk, int D, int T, int page_size);
 int dm_cache_attn_tree(const dm_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sn, int64_t q_sh, int B, int N, int H,
@@ -326,7 +329,8 @@ int dm_dbg_cache_tree_plan(int B, int N, int H, int Hk, int D, int T, int page_s
 
 /* Of the drafted tokens before[b] ... lengths[b] - 1 those of a path are kept: path[b, 0 ... counts[b] - 1], strictly increasing indexes behind before[b]
  * (rows path_row entries apart, M <= 1024 entries), become the tokens before[b], before[b] + 1, ...  Each block of 32 slots that is written gets the
- * smallest power-of-two scale that holds its tokens, older ones too; slots behind the last token stay as they are.  new_lengths (B) = before + counts.  A
+ * smallest power-of-two scale that holds its tokens, older ones too (what a rejected token's larger scale had rounded away of these does not come back); slots behind the last token stay as
+ * they are.  new_lengths (B) = before + counts.  A
  * path that does not increase or leaves the drafted tokens: DM_STATUS_BAD_TREE, and nothing of the sequence is changed. */
 int dm_cache_keep(const dm_kv_cache* cache, int B, const int* table, int64_t table_row, int T, const int* before, const int* lengths,
                   const int* path, int64_t path_row, int M, const int* counts, int* new_lengths, int* status, void* stream);
