@@ -19,7 +19,7 @@ int dm_cache_append(const dm_kv_cache* cache, const void* k, int64_t k_sb, int64
   if (new_lengths == nullptr) return fail(DM_ERR_ARG, "delta_matching: new lengths is NULL (every tensor must be a CUDA buffer)");
   if ((static_cast<int64_t>(N) + 30) / 32 + 1 > (1ll << 32) / (static_cast<int64_t>(B) * cache->heads * 2))
     return fail(DM_ERR_ARG, "delta_matching: too many tokens in one call (%d x %d)", B, N);
-  DM_TRY(check_new_lengths(new_lengths, B, {{lengths, B, "lengths"}, {counts, B, "counts"}, {table, rows_of(B, table_row, T), "block table"}}));
+  DM_TRY(check_new_lengths(new_lengths, B, {{lengths, 1, 1, "lengths"}, {counts, 1, 1, "counts"}, {table, table_row, T, "block table"}}));
   DM_TRY(check_sm100());
   dm::CacheAppendParams p{};
   p.c = view_of(cache, table, table_row, T, lengths, B, status);
@@ -136,7 +136,7 @@ int dm_cache_evict(const dm_kv_cache* cache, int B, const int* table, int64_t ta
   if (recent < 0 || recent > budget) return fail(DM_ERR_ARG, "delta_matching: recent must be between 0 and the budget (got %d)", recent);
   for (const NamedPtr& x : {NamedPtr{weights, "weights"}, {new_lengths, "new lengths"}, {kept, "kept"}, {new_weights, "new weights"}})
     if (x.p == nullptr) return fail(DM_ERR_ARG, "delta_matching: %s is NULL (every tensor must be a CUDA buffer)", x.name);
-  DM_TRY(check_new_lengths(new_lengths, B, {{lengths, B, "lengths"}, {table, rows_of(B, table_row, T), "block table"}, {new_table, rows_of(B, new_table_row, new_T), "new block table"}}));
+  DM_TRY(check_new_lengths(new_lengths, B, {{lengths, 1, 1, "lengths"}, {table, table_row, T, "block table"}, {new_table, new_table_row, new_T, "new block table"}}));
   DM_TRY(check_sm100());
   dm::CacheEvictParams p{};
   p.c = view_of(cache, table, table_row, T, lengths, B, status);

@@ -60,18 +60,20 @@ inline int check_rows(const char* name, const void* p, int64_t a, int64_t b, int
   return 0;
 }
 
-// Rows of int32 that a kernel reads (n entries from one row's first to the last row's last).
+// B rows of n int32 each that a kernel reads, `row` entries apart.
 struct IntRows {
   const int* p;
-  int64_t n;
+  int64_t row, n;
   const char* name;
 };
-inline int64_t rows_of(int B, int64_t row, int64_t n) { return (B - 1) * row + n; }
-// The kernels' CTAs read these while one of them writes new_lengths.
+// The kernels' CTAs read these while one of them writes new_lengths.  (Between two rows it may lie.)
 inline int check_new_lengths(const int* out, int B, std::initializer_list<IntRows> in) {
-  for (const IntRows& x : in)
-    if (x.p != nullptr && x.p < out + B && out < x.p + x.n)
-      return fail(DM_ERR_ARG, "delta_matching: new lengths must not share memory with %s (a buffer of their own)", x.name);
+  for (const IntRows& x : in) {
+    if (x.p == nullptr) continue;
+    const int64_t at = (static_cast<int64_t>(reinterpret_cast<uintptr_t>(out)) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(x.p))) / 4;      // behind the first row's begin
+    const int64_t b = at < x.n ? 0 : x.row > 0 ? (at - x.n) / x.row + 1 : B;          // first row that ends behind it
+    if (b < B && b * x.row < at + B) return fail(DM_ERR_ARG, "delta_matching: new lengths must not share memory with %s (a buffer of their own)", x.name);
+  }
   return 0;
 }
 

@@ -74,8 +74,7 @@ int dm_cache_append_rotary(const dm_kv_cache* cache, const void* q, int64_t q_sb
   if (offsets != nullptr && offsets_row < 0) return fail(DM_ERR_ARG, "delta_matching: rows of offsets are %lld apart", static_cast<long long>(offsets_row));
   if (N > (1 << 28) || (static_cast<int64_t>(N) + 30) / 32 + 1 > (1ll << 31) / B - 1 || static_cast<int64_t>(B) * H > 65535)
     return fail(DM_ERR_ARG, "delta_matching: too many tokens in one call (%d x %d, %d heads)", B, N, H);
-  DM_TRY(check_new_lengths(new_lengths, B, {{lengths, B, "lengths"}, {counts, B, "counts"}, {offsets, rows_of(B, offsets_row, N), "offsets"},
-                                            {table, rows_of(B, table_row, T), "block table"}}));
+  DM_TRY(check_new_lengths(new_lengths, B, {{lengths, 1, 1, "lengths"}, {counts, 1, 1, "counts"}, {offsets, offsets_row, N, "offsets"}, {table, table_row, T, "block table"}}));
   DM_TRY(check_sm100());
   dm::CacheRotaryParams p{};
   p.c = view_of(cache, table, table_row, T, lengths, B, status);
@@ -166,8 +165,7 @@ int dm_cache_keep(const dm_kv_cache* cache, int B, const int* table, int64_t tab
   DM_TRY(check_pointer(counts, "counts"));
   DM_TRY(check_pointer(new_lengths, "new lengths"));
   if (path_row < 0) return fail(DM_ERR_ARG, "delta_matching: rows of path are %lld apart", static_cast<long long>(path_row));
-  DM_TRY(check_new_lengths(new_lengths, B, {{before, B, "before"}, {lengths, B, "lengths"}, {counts, B, "counts"}, {path, rows_of(B, path_row, M), "path"},
-                                            {table, rows_of(B, table_row, T), "block table"}}));
+  DM_TRY(check_new_lengths(new_lengths, B, {{before, 1, 1, "before"}, {lengths, 1, 1, "lengths"}, {counts, 1, 1, "counts"}, {path, path_row, M, "path"}, {table, table_row, T, "block table"}}));
   DM_TRY(check_sm100());
   dm::CacheKeepParams p{};
   p.c = view_of(cache, table, table_row, T, lengths, B, status);

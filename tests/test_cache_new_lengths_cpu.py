@@ -43,3 +43,14 @@ def test_shared_buffers_are_refused(call, names):
         for new in (first - 4 * B, end):                         # beside it: what is refused is the device
             assert call(new) != 0
             assert "share memory" not in _lib.last_error(), (name, hex(new))
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="these are no real addresses")
+@pytest.mark.parametrize("call, name, row, n", [(_append, "table", 9, T), (_append_rotary, "offsets", 7, N), (_keep, "path", 8, M), (_keep, "table", 9, T), (_evict, "new_table", 9, T)])
+def test_between_rows_is_a_buffer_of_its_own(call, name, row, n):
+    """Where the gap between two rows has room for the new lengths they may lie there; one entry further on they may not."""
+    for b in range(B - 1):
+        first, last = AT[name] + 4 * (b * row + n), AT[name] + 4 * ((b + 1) * row - B)
+        for new in range(first - 4, last + 8, 4):
+            assert call(new) != 0
+            assert ("share memory" in _lib.last_error()) == (not first <= new <= last), (b, hex(new))
